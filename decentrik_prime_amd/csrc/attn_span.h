@@ -1,0 +1,233 @@
+#pragma once
+// Attention of the packed batch in which key n is seen by the queries n .. kend[n] - 1 (a sliding
+// window with sinks; answers behind a shared prompt): what the forward (span_fwd.hip) and the
+// backward (span_bwd.hip) share.
+//
+// spans [n_tokens][4] int32 holds, per token m, as query (a0, a1, kbeg) and as key kend: it sees the
+// keys [a0, a1) (a sequence's sinks or a group's prompt) and [kbeg, m] (its window or its own answer),
+// and as a key it is seen by the queries m .. kend - 1.  The two descriptions are the same set.
+#include "attn_dev.h"
+
+namespace {
+
+struct SpanArgs {
+  const f16* qkv;
+  const int32_t* spans;
+  int64_t n_tokens;
+  int nq, nkv;
+  float qk_scale, sm_scale;
+};
+
+// One query row or one key row at a time, a wave each, over exactly the keys (or queries) that it
+// sees: nothing else is read, so whatever a masked row holds cannot reach the result.
+struct RowScratch {
+  float a[kHD], b[kHD];   // the wave's row (q or k) and its partner (dO or v)
+  float p[64], ds[64];
+};
+
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) v = __fadd_rn(v, __shfl_xor(v, x));
+  return v;
+}
+
+__device__ __forceinline__ void row_to_lds(float* dst, const f16* src) {
+  const int lane = threadIdx.x & 63;
+  const f16x2 v = *reinterpret_cast<const f16x2*>(src + 2 * lane);
+  dst[2 * lane] = (float)v[0];
+  dst[2 * lane + 1] = (float)v[1];
+}
+
+// dot product of a row in LDS with this lane's row in memory
+__device__ __forceinline__ float row_dot(const float* a, const f16* row) {
+  float s = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < kHD / 8; ++i) {
+    const f16x8 x = *reinterpret_cast<const f16x8*>(row + 8 * i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = __builtin_fmaf(a[8 * i + e], (float)x[e], s);
+  }
+  return s;
+}
+
+// The keys that query m sees, as na keys from a0 and nb from b0 (kept within [0, m] whatever spans
+// holds, so every row read exists).
+struct KeyRuns {
+  int64_t a0, b0;
+  int64_t na, nb;
+  __device__ __forceinline__ int64_t row(int64_t i) const { return i < na ? a0 + i : b0 + (i - na); }
+};
+__device__ __forceinline__ KeyRuns key_runs(const SpanArgs& a, int64_t m) {
+  const int32_t* s = a.spans + 4 * m;
+  KeyRuns r;
+  r.a0 = s[0] > 0 ? s[0] : 0;
+  const int64_t a1 = s[1] < m + 1 ? s[1] : m + 1;
+  r.na = a1 > r.a0 ? a1 - r.a0 : 0;
+  r.b0 = s[2] > 0 ? s[2] : 0;
+  if (r.na > 0 && r.b0 < a1) r.b0 = a1;
+  r.nb = m + 1 > r.b0 ? m + 1 - r.b0 : 0;
+  return r;
+}
+__device__ __forceinline__ int64_t key_end(const SpanArgs& a, int64_t n) {
+  const int64_t e = a.spans[4 * n + 3];
+  return e < a.n_tokens ? e : a.n_tokens;
+}
+
+// out and lse of query m, head h
+__device__ __noinline__ void span_row_fwd(const SpanArgs& a, int64_t m, int h, f16* out, float* lse,
+                                          RowScratch& s) {
+  const int lane = threadIdx.x & 63;
+  const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD;
+  const int kvh = h / (a.nq / a.nkv);
+  const f16* kb = a.qkv + (int64_t)(a.nq + kvh) * kHD;
+  const f16* vb = kb + (int64_t)a.nkv * kHD;
+  wave_sync();
+  row_to_lds(s.a, a.qkv + m * ROW + (int64_t)h * kHD);
+  wave_sync();
+  const KeyRuns kr = key_runs(a, m);
+  const int64_t n = kr.na + kr.nb;
+  float mx = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  for (int64_t i0 = 0; i0 < n; i0 += 64) {
+    const bool on = i0 + lane < n;
+    float x = -INFINITY;
+    if (on) x = __fmul_rn(row_dot(s.a, kb + kr.row(i0 + lane) * ROW), a.qk_scale);
+    // a NaN score has to reach the sum: the maximum leaves it out, 2^(x - max) below does not
+    float t = x;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) t = fmaxf(t, __shfl_xor(t, d));
+    const float m_new = fmaxf(mx, t);
+    const float ref = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = mx == -INFINITY ? 0.0f : exp2f(__fsub_rn(mx, ref));
+    const float p = on ? exp2f(__fsub_rn(x, ref)) : 0.0f;
+    mx = m_new;
+    l = __fadd_rn(__fmul_rn(l, alpha), wave_sum(p));
+    o0 = __fmul_rn(o0, alpha);
+    o1 = __fmul_rn(o1, alpha);
+    wave_sync();
+    s.p[lane] = p;
+    wave_sync();
+    const int cnt = n - i0 < 64 ? (int)(n - i0) : 64;
+    for (int j = 0; j < cnt; ++j) {
+      const f16x2 v = *reinterpret_cast<const f16x2*>(vb + kr.row(i0 + j) * ROW + 2 * lane);
+      o0 = __builtin_fmaf(s.p[j], (float)v[0], o0);
+      o1 = __builtin_fmaf(s.p[j], (float)v[1], o1);
+    }
+  }
+  const float inv = __fdiv_rn(1.0f, l);
+  f16x2 r;
+  r[0] = (f16)__fmul_rn(o0, inv);
+  r[1] = (f16)__fmul_rn(o1, inv);
+  *reinterpret_cast<f16x2*>(out + m * (int64_t)a.nq * kHD + (int64_t)h * kHD + 2 * lane) = r;
+  if (lane == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(mx, log2f(l));
+}
+
+// dq of query m, head h
+__device__ __noinline__ void span_row_dq(const SpanArgs& a, int64_t m, int h, const f16* dout,
+                                         const float* lse, const float* delta, f16* dq,
+                                         RowScratch& s) {
+  const int lane = threadIdx.x & 63;
+  const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
+  const int kvh = h / (a.nq / a.nkv);
+  const f16* kb = a.qkv + (int64_t)(a.nq + kvh) * kHD;
+  const f16* vb = kb + (int64_t)a.nkv * kHD;
+  wave_sync();
+  row_to_lds(s.a, a.qkv + m * ROW + (int64_t)h * kHD);
+  row_to_lds(s.b, dout + m * OROW + (int64_t)h * kHD);
+  wave_sync();
+  const float lm = lse[(int64_t)h * a.n_tokens + m], dm = delta[(int64_t)h * a.n_tokens + m];
+  const KeyRuns kr = key_runs(a, m);
+  const int64_t n = kr.na + kr.nb;
+  float g0 = 0.0f, g1 = 0.0f;
+  for (int64_t i0 = 0; i0 < n; i0 += 64) {
+    float ds = 0.0f;
+    if (i0 + lane < n) {
+      const int64_t off = kr.row(i0 + lane) * ROW;
+      const float p = exp2f(__builtin_fmaf(row_dot(s.a, kb + off), a.qk_scale, -lm));
+      ds = __fmul_rn(p, __fsub_rn(row_dot(s.b, vb + off), dm));
+    }
+    wave_sync();
+    s.ds[lane] = ds;
+    wave_sync();
+    const int cnt = n - i0 < 64 ? (int)(n - i0) : 64;
+    for (int j = 0; j < cnt; ++j) {
+      const f16x2 k = *reinterpret_cast<const f16x2*>(kb + kr.row(i0 + j) * ROW + 2 * lane);
+      g0 = __builtin_fmaf(s.ds[j], (float)k[0], g0);
+      g1 = __builtin_fmaf(s.ds[j], (float)k[1], g1);
+    }
+  }
+  f16x2 r;
+  r[0] = (f16)__fmul_rn(g0, a.sm_scale);
+  r[1] = (f16)__fmul_rn(g1, a.sm_scale);
+  *reinterpret_cast<f16x2*>(dq + m * OROW + (int64_t)h * kHD + 2 * lane) = r;
+}
+
+// dk and dv of key n, KV head g, summed over the queries that see it and the heads of its group
+__device__ __noinline__ void span_key_dkdv(const SpanArgs& a, int64_t n, int g, const f16* dout,
+                                           const float* lse, const float* delta, f16* dk, f16* dv,
+                                           RowScratch& s) {
+  const int lane = threadIdx.x & 63;
+  const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
+  const int gin = a.nq / a.nkv;
+  const f16* krow = a.qkv + n * ROW + (int64_t)(a.nq + g) * kHD;
+  wave_sync();
+  row_to_lds(s.a, krow);
+  row_to_lds(s.b, krow + (int64_t)a.nkv * kHD);
+  wave_sync();
+  const int64_t end = key_end(a, n);
+  float dk0 = 0.0f, dk1 = 0.0f, dv0 = 0.0f, dv1 = 0.0f;
+  for (int hh = g * gin; hh < (g + 1) * gin; ++hh)
+    for (int64_t m0 = n; m0 < end; m0 += 64) {
+      const int64_t m = m0 + lane;
+      const f16* qb = a.qkv + (int64_t)hh * kHD;
+      const f16* ob = dout + (int64_t)hh * kHD;
+      float p = 0.0f, ds = 0.0f;
+      if (m < end) {
+        p = exp2f(__builtin_fmaf(row_dot(s.a, qb + m * ROW), a.qk_scale,
+                                 -lse[(int64_t)hh * a.n_tokens + m]));
+        ds = __fmul_rn(p, __fsub_rn(row_dot(s.b, ob + m * OROW), delta[(int64_t)hh * a.n_tokens + m]));
+      }
+      wave_sync();
+      s.p[lane] = p;
+      s.ds[lane] = ds;
+      wave_sync();
+      const int cnt = end - m0 < 64 ? (int)(end - m0) : 64;
+      for (int j = 0; j < cnt; ++j) {
+        const f16x2 q = *reinterpret_cast<const f16x2*>(qb + (m0 + j) * ROW + 2 * lane);
+        const f16x2 o = *reinterpret_cast<const f16x2*>(ob + (m0 + j) * OROW + 2 * lane);
+        dk0 = __builtin_fmaf(s.ds[j], (float)q[0], dk0);
+        dk1 = __builtin_fmaf(s.ds[j], (float)q[1], dk1);
+        dv0 = __builtin_fmaf(s.p[j], (float)o[0], dv0);
+        dv1 = __builtin_fmaf(s.p[j], (float)o[1], dv1);
+      }
+    }
+  const int64_t off = n * (int64_t)a.nkv * kHD + (int64_t)g * kHD + 2 * lane;
+  f16x2 r;
+  r[0] = (f16)__fmul_rn(dk0, a.sm_scale);
+  r[1] = (f16)__fmul_rn(dk1, a.sm_scale);
+  *reinterpret_cast<f16x2*>(dk + off) = r;
+  r[0] = (f16)dv0;
+  r[1] = (f16)dv1;
+  *reinterpret_cast<f16x2*>(dv + off) = r;
+}
+
+// the launch arguments, with the checks both entry points share
+inline int span_args(SpanArgs& a, const void* qkv, const int32_t* spans, int64_t n_tokens, int32_t nq,
+                     int32_t nkv, int32_t hd) {
+  if (hd != kHD || nq < 1 || nkv < 1 || nq % nkv || nq > 65535 || n_tokens < 0 ||
+      n_tokens > INT32_MAX / 2)
+    return DK_ERR_INVALID;
+  if (n_tokens > 0 && (!qkv || !spans)) return DK_ERR_INVALID;
+  if (!dk_aligned(qkv, 16) || !dk_aligned(spans, 16)) return DK_ERR_ALIGN;
+  const double log2e = 1.4426950408889634;
+  a = SpanArgs{(const f16*)qkv, spans, n_tokens, nq, nkv, (float)(log2e / __builtin_sqrt((double)hd)),
+               (float)(1.0 / __builtin_sqrt((double)hd))};
+  return 0;
+}
+
+}  // namespace

@@ -16,8 +16,18 @@ backward  delta = rowsum(O dO); dQ fp32 [N, nq hd]; dK, dV fp32 per query head [
 The reference's block sizes are parameters of its Triton kernels; here the blocks are fixed by
 the kernels (128 rows per workgroup, tiles of 64), and ``block_table`` must be built for
 FWD_BLOCK_M and BWD_BLOCK.
+
+``span_attention_forward`` / ``span_attention_backward`` (no counterpart in the reference) run the
+same attention over part of the keys, named by a plan built once per batch:
+``window_meta``   query i of a sequence sees its keys j <= i with i - j < window or j < sinks
+``prefix_meta``   groups of a prompt and several answers, the prompt packed once: an answer's token
+                  sees the whole prompt and its own answer up to itself
+Both are batches in which key n is seen by the queries n .. kend[n] - 1.  The gradients come back in
+fp16 (the products behind them take fp16 P and dS), dK and dV summed over each group's heads: the QKV
+epilogue backward takes them with gin = 1.
 """
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -127,6 +137,130 @@ def attention_backward(qkv, out, lse, dout, meta, nq, nkv, hd, block=BWD_BLOCK, 
                                 _lib.ptr(dkp), _lib.ptr(dvp), _lib.stream_handle(dev))
     _lib.check(rc, "dk_attn_bwd")
     return dq, dkp, dvp
+
+
+class SpanMeta:
+    """Plan of one packed batch for the attention over part of the keys (window_meta, prefix_meta).
+
+    spans [n, 4] int32 on the device: token m sees, as a query, the keys [a0, a1) and [kbeg, m]; as a
+    key it is seen by the queries m .. kend - 1.  positions [n] int32: each token's position (an
+    answer's go on from its prompt's), for the rotary embedding.  A plan serves any number of
+    calls, on any streams of its device, captured or not."""
+
+    def __init__(self, runs, spans, positions, nq, nkv, device):
+        if nq < 1 or nkv < 1 or nq % nkv:
+            raise ValueError(f"nq must be a multiple of nkv (got {nq}, {nkv})")
+        if spans.shape[0] > MAX_SPAN_TOKENS:
+            raise ValueError(f"at most {MAX_SPAN_TOKENS} tokens (got {spans.shape[0]})")
+        self.n_tokens, self.nq, self.nkv = int(spans.shape[0]), int(nq), int(nkv)
+        i32 = dict(dtype=torch.int32, device=device)
+        self.spans = torch.tensor(spans, **i32)
+        self.positions = torch.tensor(positions, **i32)
+
+
+MAX_SPAN_TOKENS = 1 << 30
+
+
+def _lengths(lens, what):
+    lens = [int(n) for n in lens]
+    if any(n < 0 for n in lens):
+        raise ValueError(f"{what} must not be negative")
+    return lens
+
+
+def window_meta(lens, window, sinks, nq, nkv, device):
+    """Plan of a packed batch with sequence lengths `lens` (zeros allowed) under a causal sliding
+    window: query i sees keys j <= i with i - j < window (window >= 1: itself at least) or
+    j < sinks (the sequence's first tokens, sinks >= 0)."""
+    lens = _lengths(lens, "lens")
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be at least 1 and sinks at least 0 (got {window}, {sinks})")
+    size = np.asarray(lens, np.int64)
+    start = np.cumsum(size) - size
+    s0, end = np.repeat(start, size), np.repeat(start + size, size)
+    m = np.arange(size.sum(), dtype=np.int64)
+    spans = np.empty((m.size, 4), np.int64)
+    spans[:, 0] = s0
+    spans[:, 1] = np.minimum(s0 + sinks, end)
+    spans[:, 2] = np.maximum(s0, m - (window - 1))
+    spans[:, 3] = np.where(m - s0 < sinks, end, np.minimum(m + window, end))
+    runs = [(int(a), int(a + n)) for a, n in zip(start, size) if n]
+    return SpanMeta(runs, spans, m - s0, nq, nkv, device)
+
+
+def prefix_meta(groups, nq, nkv, device):
+    """Plan of a packed batch of groups (prompt length, [answer lengths]), packed as the prompt's tokens
+    and then each answer's (zeros allowed).  Prompt tokens are causal; an answer's token sees the
+    group's whole prompt and its own answer up to itself, and nothing of the other answers."""
+    spans, positions, runs, g0 = [], [], [], 0
+    for prompt, answers in groups:
+        prompt, answers = _lengths([prompt], "prompt lengths")[0], _lengths(answers, "answer lengths")
+        size = np.asarray([prompt] + answers, np.int64)
+        start = g0 + np.cumsum(size) - size
+        end = g0 + int(size.sum())
+        sp = np.empty((end - g0, 4), np.int64)
+        sp[:, 0] = g0
+        sp[:prompt, 1], sp[prompt:, 1] = g0, g0 + prompt
+        sp[:, 2] = np.repeat(start, size)
+        sp[:prompt, 3], sp[prompt:, 3] = end, np.repeat(start + size, size)[prompt:]
+        pos = np.arange(g0, end) - sp[:, 2]
+        pos[prompt:] += prompt
+        spans.append(sp)
+        positions.append(pos)
+        runs += [r for r in ((g0, g0 + prompt), (g0 + prompt, end)) if r[1] > r[0]]
+        g0 = end
+    spans = np.concatenate(spans) if spans else np.empty((0, 4), np.int64)
+    positions = np.concatenate(positions) if positions else np.empty(0, np.int64)
+    return SpanMeta(runs, spans, positions, nq, nkv, device)
+
+
+def _check_span(qkv, meta, nq, nkv, hd):
+    if hd != HEAD_DIM:
+        raise ValueError(f"head size {HEAD_DIM} (got {hd})")
+    if (nq, nkv) != (meta.nq, meta.nkv):
+        raise ValueError(f"the plan is for {meta.nq} / {meta.nkv} heads (got {nq}, {nkv})")
+    _t(qkv, (torch.float16,), "qkv", (meta.n_tokens, (nq + 2 * nkv) * hd))
+    if meta.spans.device != qkv.device:
+        raise ValueError(f"the plan is on {meta.spans.device}, qkv on {qkv.device}")
+
+
+def span_attention_forward(qkv, meta, nq, nkv, hd):
+    """(out [N, nq hd] fp16, lse [nq, N] fp32) of the attention whose plan is `meta`; layouts as for
+    attention_forward."""
+    _check_span(qkv, meta, nq, nkv, hd)
+    n, dev = meta.n_tokens, qkv.device
+    out = torch.empty((n, nq * hd), dtype=torch.float16, device=dev)
+    lse = torch.empty((nq, n), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.lib().dk_attn_span_fwd(_lib.ptr(qkv), _lib.ptr(meta.spans), n, nq, nkv, hd,
+                                         _lib.ptr(out), _lib.ptr(lse), _lib.stream_handle(dev))
+    _lib.check(rc, "dk_attn_span_fwd")
+    return out, lse
+
+
+def span_attention_backward(qkv, out, lse, dout, meta, nq, nkv, hd):
+    """(dq [N, nq hd], dk [N, nkv hd], dv [N, nkv hd]) fp16 from the forward's out and lse and the
+    gradient dout of out."""
+    _check_span(qkv, meta, nq, nkv, hd)
+    n, dev = meta.n_tokens, qkv.device
+    for t, dt, what, shape in ((out, torch.float16, "out", (n, nq * hd)),
+                               (dout, torch.float16, "dout", (n, nq * hd)),
+                               (lse, torch.float32, "lse", (nq, n))):
+        _t(t, (dt,), what, shape)
+        if t.device != dev:
+            raise ValueError(f"{what} is on {t.device}, qkv on {dev}")
+    delta = torch.empty((nq, n), dtype=torch.float32, device=dev)
+    dq = torch.empty((n, nq * hd), dtype=torch.float16, device=dev)
+    dk = torch.empty((n, nkv * hd), dtype=torch.float16, device=dev)
+    dv = torch.empty((n, nkv * hd), dtype=torch.float16, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.lib().dk_attn_span_bwd(_lib.ptr(qkv), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(dout),
+                                         _lib.ptr(meta.spans), n, nq, nkv, hd, _lib.ptr(delta),
+                                         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
+                                         _lib.stream_handle(dev))
+    _lib.check(rc, "dk_attn_span_bwd")
+    return dq, dk, dv
 
 
 def warmup_specs(nq, nkv, hd):

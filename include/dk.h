@@ -162,6 +162,20 @@ int dk_attn_bwd(const void* qkv, const void* out, const float* lse, const void* 
                 float* delta, float* dq, float* dkp, float* dvp, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Causal GQA attention of the packed batch over part of the keys: a sliding window with sinks, or
+ * groups of answers behind one shared prompt.  No counterpart in the reference.  spans [n_tokens][4]
+ * int32, 16-byte aligned: token m sees, as a query, the keys [a0, a1) and [kbeg, m], and is seen, as
+ * a key, by the queries m .. kend - 1 (a0, a1, kbeg, kend in this order; the two describe the same
+ * pairs).  qkv, out and lse as for dk_attn_fwd.  The backward writes fp16 gradients, dk and dv
+ * [n_tokens, nkv hd] summed over the heads of each group; delta [nq, n_tokens] fp32 is scratch.
+ * A key that a query does not see has no influence on it, whatever it holds. */
+int dk_attn_span_fwd(const void* qkv, const int32_t* spans, int64_t n_tokens, int32_t nq,
+                     int32_t nkv, int32_t hd, void* out, float* lse, hipStream_t stream);
+int dk_attn_span_bwd(const void* qkv, const void* out, const float* lse, const void* dout,
+                     const int32_t* spans, int64_t n_tokens, int32_t nq, int32_t nkv, int32_t hd,
+                     float* delta, void* dq, void* dk, void* dv, hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * LM head over vocabulary chunks (the consumer of the final norm): the row kernels between the
  * two GEMMs of each chunk (logits_c = Y E_c^T by dk_h16_linear_fwd_lora, acc += P E_c by
  * dk_h16_linear_bwd_dx_lora with DK_OUT_F32_ACCUM).  Rows are in sorted order (rows with a target

@@ -75,3 +75,60 @@ def attention_bwd(qkv, dout, lens, nq, nkv, hd, out=None):
             dvp[sl, h] = p.T @ do[sl, h]
         s0 += L
     return dq.reshape(n, -1), dkp.reshape(n, -1), dvp.reshape(n, -1)
+
+
+def window_visible(lens, window, sinks):
+    """[N, N] bool: query i of a sequence sees its keys j <= i with i - j < window or j < sinks."""
+    n = sum(lens)
+    vis = np.zeros((n, n), bool)
+    s0 = 0
+    for L in lens:
+        i, j = np.arange(L)[:, None], np.arange(L)[None]
+        vis[s0:s0 + L, s0:s0 + L] = (j <= i) & ((i - j < window) | (j < sinks))
+        s0 += L
+    return vis
+
+
+def prefix_visible(groups):
+    """[N, N] bool: groups (prompt, answers) packed as the prompt and then each answer; an answer's
+    token sees the whole prompt and its own answer up to itself, prompt tokens are causal."""
+    n = sum(p + sum(a) for p, a in groups)
+    vis = np.zeros((n, n), bool)
+    g0 = 0
+    for p, answers in groups:
+        vis[g0:g0 + p, g0:g0 + p] = np.tril(np.ones((p, p), bool))
+        b = g0 + p
+        for a in answers:
+            vis[b:b + a, g0:g0 + p] = True
+            vis[b:b + a, b:b + a] = np.tril(np.ones((a, a), bool))
+            b += a
+        g0 = b
+    return vis
+
+
+def span_attention(qkv, visible, nq, nkv, hd, dout=None):
+    """Attention over the visible pairs [N, N] in float64: out [N, nq hd] and lse [nq, N] (exp2 domain),
+    and with dout also dq, dk, dv, the last two summed over each group's heads [N, nkv hd]."""
+    q, k, v = _split(qkv, nq, nkv, hd)
+    n, g, sm = q.shape[0], nq // nkv, 1.0 / np.sqrt(hd)
+    out, lse = np.zeros((n, nq, hd)), np.zeros((nq, n))
+    dq, dk, dv = np.zeros((n, nq, hd)), np.zeros((n, nkv, hd)), np.zeros((n, nkv, hd))
+    do = None if dout is None else np.asarray(dout, np.float64).reshape(n, nq, hd)
+    for h in range(nq):
+        kk, vv = k[:, h // g], v[:, h // g]
+        s = np.where(visible, sm * (q[:, h] @ kk.T), -np.inf)
+        mx = s.max(1, keepdims=True)
+        e = np.exp(s - mx)
+        z = e.sum(1, keepdims=True)
+        p = e / z
+        out[:, h] = p @ vv
+        lse[h] = (mx + np.log(z))[:, 0] / np.log(2.0)
+        if do is None:
+            continue
+        dp = do[:, h] @ vv.T
+        ds = sm * p * (dp - (p * dp).sum(1, keepdims=True))
+        dq[:, h] = ds @ kk
+        dk[:, h // g] += ds.T @ q[:, h]
+        dv[:, h // g] += p.T @ do[:, h]
+    result = (out.reshape(n, -1), lse)
+    return result if dout is None else result + tuple(x.reshape(n, -1) for x in (dq, dk, dv))

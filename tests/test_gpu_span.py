@@ -1,0 +1,281 @@
+"""GPU parity of the attention over part of the keys (a sliding window with sinks; answers behind a
+shared prompt), forward and backward, against the definition in 64 bits."""
+
+import math
+
+import numpy as np
+import pytest
+
+from tests.helpers import log
+
+pytestmark = pytest.mark.gpu
+HD = 128
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+    return t
+
+
+def _meta(spec, nq, nkv):
+    from decentrik_prime_amd import k_attn
+    if spec[0] == "window":
+        return k_attn.window_meta(spec[1], spec[2], spec[3], nq, nkv, "cuda")
+    return k_attn.prefix_meta(spec[1], nq, nkv, "cuda")
+
+
+def _visible(spec):
+    from oracle import attn
+    return attn.window_visible(*spec[1:]) if spec[0] == "window" else attn.prefix_visible(spec[1])
+
+
+def _inputs(torch, n, nq, nkv, seed, scale=0.8):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    qkv = (torch.randn(n, (nq + 2 * nkv) * HD, device="cuda", generator=g) * scale).half()
+    return qkv, torch.randn(n, nq * HD, device="cuda", generator=g).half()
+
+
+def _run(qkv, dout, meta, nq, nkv):
+    from decentrik_prime_amd import k_attn
+    out, lse = k_attn.span_attention_forward(qkv, meta, nq, nkv, HD)
+    return (out, lse) + k_attn.span_attention_backward(qkv, out, lse, dout, meta, nq, nkv, HD)
+
+
+def _near(got, want, lim, what):
+    over = (got.double() - want).abs() - lim
+    assert bool((over <= 0).all()), f"{what}: {int((~(over <= 0)).sum())} of {over.numel()} outside, " \
+                                    f"worst by {float(over.max()):.3g}"
+
+
+def _check(torch, spec, nq, nkv, qkv, dout, got):
+    """Every output against the formulas, with what the roundings may move it by: P and dS are rounded
+    to fp16 (half a step, 2^-11 of the value, 2^-25 below the normal range), the scores' fp32 sums move
+    P by at most HD 2^-24 of the products' magnitudes and the fp32 sums over the keys by less than
+    2^-12 (together under 2^-10 of the magnitudes summed), and the result itself is rounded to fp16
+    (2^-11; 2^-25 below the normal range)."""
+    vis = torch.from_numpy(_visible(spec)).cuda()
+    n, gin, sm = qkv.shape[0], nq // nkv, HD ** -0.5
+    x = qkv.double().view(n, nq + 2 * nkv, HD)
+    out, lse, dq, dk, dv = (t.view(n, -1, HD) if t.dtype == torch.float16 else t for t in got)
+    wk, wv, lk, lv = (torch.zeros(n, nkv, HD, dtype=torch.float64, device="cuda") for _ in range(4))
+    for h in range(nq):
+        g = h // gin
+        q, k, v = x[:, h], x[:, nq + g], x[:, nq + nkv + g]
+        o, do = out[:, h].double(), dout.view(n, nq, HD)[:, h].double()
+        sc = torch.where(vis, sm * (q @ k.t()), -float("inf"))
+        p = torch.softmax(sc, 1)
+        dl = (o * do).sum(1, keepdim=True)
+        ds = p * (do @ v.t() - dl)
+        what = f"{spec}, {nq}/{nkv} heads, head {h}: "
+        _near(out[:, h], p @ v, 2.0 ** -10 * (p @ v.abs()) + 2.0 ** -11 * (p @ v).abs() + 2.0 ** -24,
+              what + "out")
+        _near(lse[h], torch.logsumexp(sc, 1) / math.log(2.0), 2.0 ** -12, what + "lse")
+        eds = torch.where(vis, 2.0 ** -10 * ds.abs() + 2.0 ** -25 + HD * 2.0 ** -23 * p * (
+            do.abs() @ v.abs().t() + (o * do).abs().sum(1, keepdim=True)), 0.0)
+        want = sm * (ds @ k)
+        _near(dq[:, h], want, sm * (eds @ k.abs()) + 2.0 ** -11 * want.abs() + 2.0 ** -24, what + "dq")
+        wk[:, g] += sm * (ds.t() @ q)
+        lk[:, g] += sm * (eds.t() @ q.abs())
+        wv[:, g] += p.t() @ do
+        lv[:, g] += torch.where(vis, 2.0 ** -10 * p + 2.0 ** -25, 0.0).t() @ do.abs()
+    _near(dk, wk, lk + 2.0 ** -11 * wk.abs() + 2.0 ** -24, f"{spec}, {nq}/{nkv} heads: dk")
+    _near(dv, wv, lv + 2.0 ** -11 * wv.abs() + 2.0 ** -24, f"{spec}, {nq}/{nkv} heads: dv")
+
+
+CASES = [
+    # one token; an empty sequence; a window of one token with and without sinks
+    (("window", [1], 1, 0), 12, 2), (("window", [0, 3, 0, 1], 1, 0), 4, 2), (("window", [70, 200], 1, 1), 2, 1),
+    # windows that end inside, at and past a tile; sinks fewer and more than a tile, than the window,
+    # than the sequence; blocks whose window meets the sinks
+    (("window", [300, 65], 64, 4), 12, 2), (("window", [513], 63, 0), 3, 3), (("window", [700, 1, 129], 200, 70), 4, 2),
+    (("window", [400], 17, 130), 8, 1), (("window", [257, 30], 5, 600), 6, 2), (("window", [260, 128], 4096, 3), 5, 1),
+    (("window", [1300], 256, 4), 14, 2), (("window", [2100], 1000, 64), 2, 2),
+    # a prompt alone, answers alone, one-token answers, answers that share a tile, empty ones
+    (("prefix", [(130, [])]), 4, 2), (("prefix", [(0, [5, 130])]), 12, 2), (("prefix", [(1, [1])]), 4, 1),
+    (("prefix", [(200, [1] * 70)]), 12, 2), (("prefix", [(64, [64, 128, 0, 63])]), 2, 2),
+    (("prefix", [(500, [40, 3, 77, 0, 190]), (0, [33]), (17, [1, 300]), (300, [0])]), 28, 4),
+    (("prefix", [(1100, [150, 90, 301])]), 6, 1), (("prefix", [(77, [9] * 33)]), 8, 8),
+]
+
+
+@pytest.mark.parametrize("spec,nq,nkv", CASES)
+def test_against_the_definition(torch, spec, nq, nkv):
+    log(f"span attention fwd+bwd, {spec}, {nq}/{nkv} heads")
+    meta = _meta(spec, nq, nkv)
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=meta.n_tokens + nq)
+    _check(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv))
+
+
+def test_no_tokens(torch):
+    for spec in (("window", [], 4, 1), ("prefix", [(0, [0])])):
+        meta = _meta(spec, 4, 2)
+        qkv, dout = _inputs(torch, 0, 4, 2, seed=0)
+        for t in _run(qkv, dout, meta, 4, 2):
+            assert t.numel() == 0
+
+
+def test_growing_scores(torch):
+    """Scores that grow along the keys by far more than a rescaling's threshold per tile, and a window
+    that leaves the largest behind."""
+    for spec in (("window", [700], 150, 3), ("prefix", [(300, [100, 200])])):
+        log(f"span attention, growing scores, {spec}")
+        meta = _meta(spec, 2, 1)
+        qkv, dout = _inputs(torch, meta.n_tokens, 2, 1, seed=5, scale=0.3)
+        qkv[:, 2 * HD] = (0.25 * meta.positions).half()
+        qkv[:, 0] = qkv[:, HD] = 8.0
+        got = _run(qkv, dout, meta, 2, 1)
+        vis = torch.from_numpy(_visible(spec)).cuda()
+        sc = torch.where(vis, HD ** -0.5 * (qkv[:, :HD].double() @ qkv[:, 2 * HD:3 * HD].double().t()),
+                         -float("inf"))
+        p = torch.softmax(sc, 1)
+        v = qkv[:, 3 * HD:].double()
+        # scores up to 130 in sums of fp32: P off by 2^-24 HD 2^7, below 2^-10
+        _near(got[0][:, :HD], p @ v, 2.0 ** -9 * (p @ v.abs()) + 2.0 ** -24, "out")
+
+
+def test_wide_window_is_plain_causal_attention(torch):
+    from decentrik_prime_amd import k_attn
+    lens, nq, nkv = [1, 37, 64, 500], 12, 2
+    qkv, dout = _inputs(torch, sum(lens), nq, nkv, seed=3)
+    plain = k_attn.attention_forward(qkv, k_attn.meta_for(lens, "cuda"), nq, nkv, HD)
+    for spec in (("window", lens, 500, 0), ("window", lens, 1, 500), ("prefix", [(0, lens)])):
+        got = k_attn.span_attention_forward(qkv, _meta(spec, nq, nkv), nq, nkv, HD)
+        # both within 2^-10 of the same sums of |p v| (at most max |v|, 4) and one fp16 rounding
+        assert float((got[0].double() - plain[0].double()).abs().max()) < 2 * 4 * (2.0 ** -10 + 2.0 ** -11)
+        assert float((got[1] - plain[1]).abs().max()) < 2.0 ** -11
+
+
+@pytest.mark.parametrize("spec,bad,clean", [
+    # an answer's token, which nothing of the other answers or the prompt sees
+    (("prefix", [(40, [20, 30, 9]), (3, [50])]), 65, lambda m: (m < 65) | (m >= 90)),
+    # a token in the middle of a sequence: earlier queries, and those past the window
+    (("window", [20, 300, 40], 50, 4), 20 + 100, lambda m: (m < 120) | (m >= 170)),
+    # a token of the second sequence's end
+    (("window", [20, 300, 40], 50, 4), 319, lambda m: m != 319)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 65504.0])
+def test_unseen_rows_have_no_influence(torch, spec, bad, clean, value):
+    """A row full of NaN, infinities or the type's largest value changes nothing for the queries that do
+    not see it, nor for the keys that it does not see."""
+    nq, nkv = 4, 2
+    log(f"span attention with {value} in row {bad}, {spec}")
+    meta = _meta(spec, nq, nkv)
+    n = meta.n_tokens
+    qkv, dout = _inputs(torch, n, nq, nkv, seed=11)
+    want = _run(qkv, dout, meta, nq, nkv)
+    bad_qkv, bad_dout = qkv.clone(), dout.clone()
+    bad_qkv[bad], bad_dout[bad] = value, value
+    got = _run(bad_qkv, bad_dout, meta, nq, nkv)
+    vis = torch.from_numpy(_visible(spec)).cuda()
+    m = torch.arange(n, device="cuda")
+    same = ~vis[:, bad]                         # queries that do not see the row
+    assert bool((same == clean(m)).all())
+    # keys whose queries (and what those saw) are all untouched
+    keys = ~vis[~same].any(0)
+    for t, w, rows, what in ((got[0], want[0], same, "out"), (got[1].t(), want[1].t(), same, "lse"),
+                             (got[2], want[2], same, "dq"), (got[3], want[3], keys, "dk"),
+                             (got[4], want[4], keys, "dv")):
+        assert bool(torch.isfinite(t[rows].float()).all()), what
+        # the same sums, in another order at the most where a row was recomputed on its own
+        lim = 2.0 ** -9 * w[rows].double().abs() + 2.0 ** -9
+        assert bool(((t[rows].double() - w[rows].double()).abs() <= lim).all()), what
+    if value != value:
+        assert bool(torch.isnan(got[0][~same]).all())
+
+
+def test_repeats_and_streams(torch):
+    """The same bits on every call, on a stream of its own, and on two streams at once."""
+    nq, nkv = 12, 2
+    for spec in (("window", [1500, 200], 300, 4), ("prefix", [(900, [40, 60, 300])])):
+        meta = _meta(spec, nq, nkv)
+        qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=1)
+        want = _run(qkv, dout, meta, nq, nkv)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = []
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(_run(qkv, dout, meta, nq, nkv))
+        torch.cuda.synchronize()
+        for res in got:
+            for a, b in zip(res, want):
+                assert torch.equal(a, b)
+
+
+def test_captured_and_replayed(torch):
+    """A training step's two calls in one graph, replayed on new inputs with eager calls between."""
+    nq, nkv = 12, 2
+    for spec in (("window", [900, 1, 333], 200, 4), ("prefix", [(700, [1, 40, 260])])):
+        meta = _meta(spec, nq, nkv)
+        qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=2)
+        _run(qkv, dout, meta, nq, nkv)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = _run(qkv, dout, meta, nq, nkv)
+        for r in range(3):
+            a, b = _inputs(torch, meta.n_tokens, nq, nkv, seed=30 + r)
+            qkv.copy_(a)
+            dout.copy_(b)
+            want = _run(qkv, dout, meta, nq, nkv)
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(res, want):
+                assert torch.equal(x, y), f"replay {r}"
+
+
+def test_refusals(torch):
+    from decentrik_prime_amd import k_attn
+    nq, nkv = 4, 2
+    meta = k_attn.window_meta([5, 7], 4, 1, nq, nkv, "cuda")
+    qkv, dout = _inputs(torch, 12, nq, nkv, seed=0)
+    out, lse = k_attn.span_attention_forward(qkv, meta, nq, nkv, HD)
+    on_cpu = k_attn.window_meta([5, 7], 4, 1, nq, nkv, "cpu")
+    for call in (lambda: k_attn.span_attention_forward(qkv[:11], meta, nq, nkv, HD),
+                 lambda: k_attn.span_attention_forward(qkv.float(), meta, nq, nkv, HD),
+                 lambda: k_attn.span_attention_forward(qkv.t().contiguous().t(), meta, nq, nkv, HD),
+                 lambda: k_attn.span_attention_forward(qkv, meta, nq, nkv, 64),
+                 lambda: k_attn.span_attention_forward(qkv, meta, 2, 2, HD),
+                 lambda: k_attn.span_attention_forward(qkv, on_cpu, nq, nkv, HD),
+                 lambda: k_attn.span_attention_backward(qkv, out, lse.half(), dout, meta, nq, nkv, HD),
+                 lambda: k_attn.span_attention_backward(qkv, out, lse.t(), dout, meta, nq, nkv, HD),
+                 lambda: k_attn.span_attention_backward(qkv, out, lse, dout[:, :HD], meta, nq, nkv, HD),
+                 lambda: k_attn.span_attention_backward(qkv, out.cpu(), lse, dout, meta, nq, nkv, HD)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_a_layer_around_it(torch):
+    """The QKV epilogue, the attention and their backwards together, as a layer runs them: the rotary
+    positions of the plan, dk and dv already summed (gin = 1)."""
+    from decentrik_prime_amd import k_attn, k_rope
+    from decentrik_prime_amd.model import rope_tables
+    nq, nkv = 12, 2
+    spec = ("prefix", [(90, [20, 33]), (0, [40])])
+    meta = _meta(spec, nq, nkv)
+    n = meta.n_tokens
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    raw = (torch.randn(n, (nq + 2 * nkv) * HD, device="cuda", generator=g) * 0.8).half()
+    dout = torch.randn(n, nq * HD, device="cuda", generator=g).half()
+    cos, sin = rope_tables(int(meta.positions.max()) + 1)
+    zq = torch.zeros(n, nq * HD, dtype=torch.float16, device="cuda")
+    qkv = raw.clone()
+    k_rope.qkv_epilogue_forward(qkv, zq, zq[:, :nkv * HD].contiguous(), meta.positions, cos, sin, 0.0,
+                                nq, nkv, HD)
+    out, lse, dq, dk, dv = got = _run(qkv, dout, meta, nq, nkv)
+    _check(torch, spec, nq, nkv, qkv, dout, got)
+    dqkv = torch.empty_like(qkv)
+    k_rope.qkv_epilogue_backward(dq, dk, dv, meta.positions, cos, sin, dqkv, nq, nkv, HD, 1)
+    # the transposed rotation of dq and dk (fp32 products, one fp16 rounding), dv as it is
+    c, s = cos[meta.positions.long()][:, None], sin[meta.positions.long()][:, None]
+    for lo, d in ((0, dq), (nq, dk)):
+        heads = d.view(n, -1, HD).double()
+        a, b = heads[..., :HD // 2], heads[..., HD // 2:]
+        c1, s1 = c[..., :HD // 2].double(), s[..., :HD // 2].double()
+        want = torch.cat([a * c1 + b * s1, b * c1 - a * s1], 2)
+        have = dqkv.view(n, -1, HD)[:, lo:lo + heads.shape[1]]
+        _near(have, want, 2.0 ** -11 * want.abs() + 2.0 ** -22 * (heads.abs().amax(2, keepdim=True)) + 2.0 ** -24,
+              "rotated gradient")
+    assert torch.equal(dqkv[:, (nq + nkv) * HD:], dv)

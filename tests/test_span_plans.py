@@ -1,0 +1,94 @@
+"""CPU checks of the attention over part of the keys: the oracle against autograd and differences, the
+plans (k_attn.window_meta, prefix_meta) against the definition of what sees what, and refusals before
+any launch."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from decentrik_prime_amd import _lib, k_attn
+from oracle import attn
+
+NQ, NKV, HD = 4, 2, 128
+WINDOWS = [([1], 1, 0), ([5, 0, 3], 1, 0), ([40], 7, 3), ([17, 64, 1, 30], 16, 0), ([50, 9], 8, 60),
+           ([33, 70], 1000, 4), ([90], 1, 1), ([0], 4, 4)]
+GROUPS = [[(5, [1])], [(0, [1])], [(0, [7, 3])], [(12, [])], [(12, [0, 0])], [(30, [4, 0, 9, 1]), (0, [6]),
+          (1, [1, 1, 1])], [(64, [64, 64])], []]
+
+
+def _visible_from_spans(spans):
+    """The pairs a plan's spans name, once as seen by each query and once as seen from each key."""
+    s = np.asarray(spans, np.int64)
+    m, n = np.arange(len(s))[:, None], np.arange(len(s))[None]
+    as_query = ((n >= s[:, :1]) & (n < s[:, 1:2]) & (n <= m)) | ((n >= s[:, 2:3]) & (n <= m))
+    as_key = (m >= n) & (m < s[None, :, 3])
+    return as_query, as_key
+
+
+@pytest.mark.parametrize("lens,window,sinks", WINDOWS)
+def test_window_plan_names_the_visible_pairs(lens, window, sinks):
+    meta = k_attn.window_meta(lens, window, sinks, NQ, NKV, "cpu")
+    want = attn.window_visible(lens, window, sinks)
+    for got in _visible_from_spans(meta.spans):
+        np.testing.assert_array_equal(got, want)
+    np.testing.assert_array_equal(meta.positions, np.concatenate([np.arange(n) for n in lens]))
+
+
+@pytest.mark.parametrize("groups", GROUPS)
+def test_prefix_plan_names_the_visible_pairs(groups):
+    meta = k_attn.prefix_meta(groups, NQ, NKV, "cpu")
+    want = attn.prefix_visible(groups)
+    for got in _visible_from_spans(meta.spans):
+        np.testing.assert_array_equal(got, want)
+    pos = [np.concatenate([np.arange(p)] + [p + np.arange(a) for a in ans]) for p, ans in groups]
+    np.testing.assert_array_equal(meta.positions, np.concatenate(pos) if pos else [])
+
+
+def test_oracle_gradients_against_autograd_and_differences():
+    lens, window, sinks = [9, 1, 20], 5, 2
+    vis = attn.window_visible(lens, window, sinks)
+    rng = np.random.default_rng(0)
+    n = sum(lens)
+    qkv = rng.standard_normal((n, (NQ + 2 * NKV) * HD)) * 0.5
+    dout = rng.standard_normal((n, NQ * HD))
+    out, lse, dq, dk, dv = attn.span_attention(qkv, vis, NQ, NKV, HD, dout)
+    t = torch.from_numpy(qkv).requires_grad_(True)
+    x = t.view(n, NQ + 2 * NKV, HD).transpose(0, 1)
+    k, v = (x[i:i + NKV].repeat_interleave(NQ // NKV, 0) for i in (NQ, NQ + NKV))
+    ref = torch.nn.functional.scaled_dot_product_attention(x[:NQ], k, v, torch.from_numpy(vis))
+    ref = ref.transpose(0, 1).reshape(n, -1)
+    ref.backward(torch.from_numpy(dout))
+    # 64-bit sums of at most 128 x 20 terms of size 1: 2560 x 2^-53
+    np.testing.assert_allclose(out, ref.detach().numpy(), rtol=1e-11, atol=1e-12)
+    np.testing.assert_allclose(np.concatenate([dq, dk, dv], 1), t.grad.numpy(), rtol=1e-10, atol=1e-11)
+    step = rng.standard_normal(qkv.shape)
+    step /= np.linalg.norm(step)
+    h = 1e-4   # error of a central difference: h^2 / 6 of the third derivative, about 1e-8 here
+    f = [(attn.span_attention(qkv + e * step, vis, NQ, NKV, HD)[0] * dout).sum() for e in (h, -h)]
+    want = (np.concatenate([dq, dk, dv], 1) * step).sum()
+    assert abs((f[0] - f[1]) / (2 * h) - want) < 1e-6 * max(1.0, abs(want))
+    full = attn.span_attention(qkv, attn.window_visible(lens, 100, 0), NQ, NKV, HD)
+    for a, b in zip(full, attn.attention_fwd(qkv, lens, NQ, NKV, HD)):
+        np.testing.assert_allclose(a, b, rtol=1e-12, atol=1e-12)
+
+
+def test_plan_refusals():
+    for lens, window, sinks, nq, nkv in (([4], 0, 0, 4, 2), ([4], 2, -1, 4, 2), ([-1], 2, 0, 4, 2),
+                                         ([4], 2, 0, 4, 3), ([4], 2, 0, 4, 0), ([4], 2, 0, 0, 1)):
+        with pytest.raises(ValueError):
+            k_attn.window_meta(lens, window, sinks, nq, nkv, "cpu")
+    for groups in ([(-1, [2])], [(3, [2, -2])]):
+        with pytest.raises(ValueError):
+            k_attn.prefix_meta(groups, 4, 2, "cpu")
+
+
+def test_call_refusals_before_any_launch():
+    meta = k_attn.window_meta([5, 7], 4, 1, NQ, NKV, "cpu")
+    qkv = torch.zeros(12, (NQ + 2 * NKV) * HD, dtype=torch.float16)
+    for call in (lambda: k_attn.span_attention_forward(qkv, meta, NQ, NKV, HD),            # not on a GPU
+                 lambda: k_attn.span_attention_forward(qkv, meta, NQ, NKV, 64),            # head size
+                 lambda: k_attn.span_attention_forward(qkv, meta, 2, 2, HD)):              # other heads
+        with pytest.raises(ValueError):
+            call()
