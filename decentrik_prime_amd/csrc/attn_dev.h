@@ -25,6 +25,7 @@
 
 namespace {
 
+using dk::dma16;
 using dk::dma16s;
 using dk::dma4;
 using dk::lds_addr;

@@ -18,6 +18,82 @@ struct SpanArgs {
   float qk_scale, sm_scale;
 };
 
+// A block of up to kBM stacked query rows and the keys that they see (SPAN_ITEM_INTS int32, written by
+// k_attn.SpanMeta).  The rows of a run of tokens are stacked (token, query head of one KV head's
+// group): row i of the block is token t0 + (phase + i) / gin, head g gin + (phase + i) % gin, so one
+// K / V tile serves a group's heads, and a block spans few tokens, whatever their number.  Its keys are
+// numbered j = 0 .. nk - 1: na rows from a0 (sinks or prompt), then rows b0 .. up to the last token.
+// A tile is kBN keys; those of [0, f0) and [f1, f2) are seen by every row.  The item walks tiles
+// [tb, te); slot: the partial that it writes, or -1 for the outputs themselves.
+constexpr int kItemInts = DK_ATTN_SPAN_ITEM_INTS;
+struct SpanItem {
+  int t0, phase, rows, g;
+  int a0, na, b0, nk;
+  int f0, f1, f2, tb;
+  int te, slot;
+};
+__device__ __forceinline__ bool span_item(const SpanArgs& a, const int32_t* items, int i, int n_slots,
+                                          SpanItem* it) {
+  const int32_t* p = items + (int64_t)i * kItemInts;
+  auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(p[k]); };
+  *it = SpanItem{u(0), u(1), u(2), u(3), u(4), u(5), u(6), u(7), u(8), u(9), u(10), u(11), u(12), u(13)};
+  const int gin = a.nq / a.nkv;
+  // an entry that names rows outside the batch is skipped before any load
+  return it->t0 >= 0 && it->phase >= 0 && it->phase < gin && it->rows >= 1 && it->rows <= kBM &&
+         it->g >= 0 && it->g < a.nkv &&
+         (int64_t)it->t0 + (it->phase + it->rows - 1) / gin < a.n_tokens && it->a0 >= 0 &&
+         it->na >= 0 && (int64_t)it->a0 + it->na <= a.n_tokens && it->b0 >= 0 && it->nk > it->na &&
+         (int64_t)it->b0 + it->nk - it->na <= a.n_tokens &&
+         (it->na == 0 || (it->b0 >= it->a0 + it->na &&
+                          ((int64_t)it->b0 - it->a0 - it->na + kBN) * (a.nq + 2 * a.nkv) * kHD * 2 <
+                              (int64_t)DK_ATTN_SPAN_REACH_BYTES)) && it->tb >= 0 && it->tb < it->te &&
+         it->te <= (it->nk + kBN - 1) / kBN && it->slot < n_slots;
+}
+__device__ __forceinline__ bool full_tile(const SpanItem& it, int t) {
+  return t < it.f0 || (t >= it.f1 && t < it.f2);
+}
+
+// A tile of the item's keys, one operand, by LDS DMA: instruction i fills rows 4 (W i + wave) .. + 3 of
+// the tile (W waves), 16 lanes a row, from a scalar base per tile and a 32-bit offset per lane.  In the
+// tile that holds keys of both runs the second run's lie a gap further on (span_item: it fits).  Keys
+// past the last one read its row (finite, and masked).
+struct KeySource {
+  unsigned rowb, r0, off0, chunk;   // bytes per row; this lane's row, offset and chunk for instruction 0
+};
+__device__ __forceinline__ KeySource key_source(int64_t row_halves, int wave, int lane) {
+  KeySource s;
+  s.rowb = (unsigned)(row_halves * (int64_t)sizeof(f16));
+  s.r0 = (unsigned)(4 * wave + (lane >> 4));
+  s.chunk = (unsigned)(((lane & 15) ^ swz16((int)s.r0)) << 4);
+  s.off0 = s.r0 * s.rowb + s.chunk;
+  return s;
+}
+template <int W>
+__device__ __forceinline__ void key_tile_load(const SpanItem& it, const KeySource& s, int t, uint64_t base,
+                                              const f16* stage, int wave) {
+  const int j0 = t * kBN;
+  const bool second = j0 >= it.na;
+  const uint64_t tb = base + (uint64_t)(second ? it.b0 + (j0 - it.na) : it.a0 + j0) * s.rowb;
+  const unsigned thr = second ? kBN : (unsigned)(it.na - j0);   // the second run's first row here
+  const unsigned gap = (unsigned)(it.b0 - it.a0 - it.na) * s.rowb;
+  const unsigned rows = (unsigned)(it.nk - 1 - j0);
+  const unsigned last = (rows < kBN ? rows * s.rowb + (rows >= thr ? gap : 0u) : ~0u - 4096u) + s.chunk;
+#pragma unroll
+  for (int i = 0; i < kBN / 4 / W; ++i) {
+    unsigned off = s.off0 + (unsigned)(4 * W * i) * s.rowb;
+    off += s.r0 + 4 * W * i >= thr ? gap : 0u;
+    dma16s(tb, off < last ? off : last,
+           __builtin_amdgcn_readfirstlane(lds_addr(stage + (W * i + wave) * 512)));
+  }
+}
+// the keys' ends, by one wave
+__device__ __forceinline__ void key_ends_load(const SpanArgs& a, const SpanItem& it, int t, const int* dst,
+                                              int lane) {
+  const int jj = t * kBN + lane, j = jj < it.nk ? jj : it.nk - 1;
+  const int64_t row = j < it.na ? it.a0 + j : it.b0 + (j - it.na);
+  dma4(a.spans + 4 * row + 3, __builtin_amdgcn_readfirstlane(lds_addr(dst)));
+}
+
 // One query row or one key row at a time, a wave each, over exactly the keys (or queries) that it
 // sees: nothing else is read, so whatever a masked row holds cannot reach the result.
 struct RowScratch {
@@ -80,7 +156,7 @@ __device__ __forceinline__ int64_t key_end(const SpanArgs& a, int64_t n) {
 }
 
 // out and lse of query m, head h
-__device__ __noinline__ void span_row_fwd(const SpanArgs& a, int64_t m, int h, f16* out, float* lse,
+__device__ __forceinline__ void span_row_fwd(const SpanArgs& a, int64_t m, int h, f16* out, float* lse,
                                           RowScratch& s) {
   const int lane = threadIdx.x & 63;
   const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD;

@@ -1,30 +1,401 @@
-// Forward of the attention over part of the keys (attn_span.h), one wave per (query, head).
+// Forward of the attention over part of the keys (attn_span.h): an online softmax in the exp2 domain
+// over the key tiles of each block of stacked query rows.  Built with the MFMA accumulators in VGPRs
+// like attn_fwd.hip.
 #include "attn_span.h"
 
 namespace {
 
-__global__ __launch_bounds__(kAThreads) void span_fwd_rows_kernel(SpanArgs a, f16* __restrict__ out,
-                                                                  float* __restrict__ lse) {
-  __shared__ RowScratch s[kAThreads / 64];
-  const int w = threadIdx.x >> 6;
-  const int64_t pair = (int64_t)blockIdx.x * (kAThreads / 64) + w;
-  if (pair >= a.n_tokens * a.nq) return;
-  span_row_fwd(a, pair / a.nq, (int)(pair % a.nq), out, lse, s[w]);
+constexpr int kFThreads = 512;
+constexpr int kFWaves = kFThreads / 64;
+// a partial: O (lane-major, below) and the rows' m and l
+constexpr int kPartFloats = kBM * kHD + 2 * kBM;
+
+// max over the two lanes l, l ^ 32 (the two key halves of one query)
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The rows whose result is not finite, recomputed over exactly the keys that they see: a masked key's
+// probability is 0, but 0 times a NaN or infinity in its value row is not.  bad [kBM]: row flags in
+// LDS, written before a barrier; s: a scratch per wave.
+template <int W>
+__device__ __forceinline__ void redo_rows(const SpanArgs& a, int t0, int phase, int rows, int g,
+                                          const int* bad, RowScratch* s, f16* out, float* lse) {
+  const int gin = a.nq / a.nkv, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  for (int i = wave; i < rows; i += W) {
+    if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
+    span_row_fwd(a, t0 + (phase + i) / gin, g * gin + (phase + i) % gin, out, lse, s[wave]);
+  }
+}
+
+__global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const int32_t* __restrict__ items,
+                                                             int n_slots, f16* __restrict__ out,
+                                                             float* __restrict__ lse,
+                                                             float* __restrict__ parts) {
+  SpanItem it;
+  if (!span_item(a, items, (int)blockIdx.x, n_slots, &it)) return;
+  const int lane = threadIdx.x & 63, hl = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int qw = wave & 3, kg = wave >> 2;   // query group, key-tile parity
+  const int gin = a.nq / a.nkv;
+  const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD;
+  const int row = 32 * qw + c;               // this lane's stacked row
+  const bool mval = row < it.rows;
+  const int rr = it.phase + (mval ? row : 0);
+  const int m = it.t0 + rr / gin, h = it.g * gin + rr % gin;
+  const int jlim = mval ? m - it.b0 + it.na : -1;   // its last key
+  __shared__ __attribute__((aligned(1024))) f16 Ks[kFwdStages * kTileHalves];
+  __shared__ __attribute__((aligned(1024))) f16 Vs[kFwdStages * kTileHalves];
+  __shared__ __attribute__((aligned(16))) int ends[kFwdStages][kBN];
+  __shared__ int bad[kBM];
+
+  f32x16 oacc[kHD / 32];
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb) oacc[hb] = zero16();
+  float m_i = -1.0e30f, l_i = 0.0f;   // l_i: this lane's half of the keys (joined at the end)
+  const int n_tiles = it.te - it.tb, n_pairs = (n_tiles + 1) / 2;
+  const uint64_t kbase = uniform64((uint64_t)(a.qkv + (int64_t)(a.nq + it.g) * kHD));
+  const uint64_t vbase = kbase + (uint64_t)a.nkv * kHD * sizeof(f16);
+  const KeySource src = key_source(ROW, wave, lane);
+  // tile pair u (tiles 2 u, 2 u + 1 of the walk) of one operand into stages t % 4
+  auto issue = [&](uint64_t base, f16* ring, int u) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int t = 2 * u + b;
+      if (t >= n_tiles) continue;
+      key_tile_load<kFWaves>(it, src, it.tb + t, base, ring + (t % kFwdStages) * kTileHalves, wave);
+    }
+  };
+  auto issue_v = [&](int u) {
+    issue(vbase, Vs, u);
+    const int t = 2 * u + wave;
+    if (wave < 2 && t < n_tiles) key_ends_load(a, it, it.tb + t, ends[t % kFwdStages], lane);
+  };
+  issue(kbase, Ks, 0);
+  // this lane's query row as the B operand (rows past the block: zeros).  Loaded unconditionally and
+  // selected at once, so the compiler's wait for these loads stands here and not inside the loop.
+  f16x8 qf[kHD / 16];
+  {
+    const f16* qrow = a.qkv + (int64_t)m * ROW + (int64_t)h * kHD + 8 * hl;
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) qf[s] = *reinterpret_cast<const f16x8*>(qrow + 16 * s);
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) asm volatile("" : "+v"(qf[s]));
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) qf[s] = mval ? qf[s] : zero8();
+  }
+  if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
+  wait_vmem<0>();
+  issue_v(0);
+  issue(kbase, Ks, 1);
+  __syncthreads();
+  const unsigned krow = lds_addr(Ks) + row_base(lane), vcol = lds_addr(Vs) + col_base(lane);
+  // S^T = K Q^T of tile t: keys kb * 32 + (row of the result), queries on the lanes
+  auto scores = [&](f32x16 (&sc)[2], int t) {
+    const unsigned ka = fresh(krow + (unsigned)((t % kFwdStages) * kTileHalves * 2));
+    sc[0] = sc[1] = zero16();
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        sc[kb] = mfma(lds_read8(ka ^ (unsigned)(32 * s), kb * 32 * kHD * 2), qf[s], sc[kb]);
+  };
+  f32x16 sc[2], sn[2];
+  if (kg < n_tiles) scores(sc, kg);
+  else sc[0] = sc[1] = zero16();
+  wait_vmem<0>();
+  __syncthreads();
+  // tile t, whose scores are in sc: its softmax and O^T += V^T P^T, beside the scores of tile t + 2
+  // into sn when there is one.  MASK: key j of the tile counts iff j <= jlim and the key's end lies
+  // past this lane's token; the others' probabilities are set to 0 (a lane may see none of a tile's
+  // keys before its first).
+  auto tile = [&](int t, bool more, f32x16 (&sc)[2], f32x16 (&sn)[2], auto mask_c) {
+    constexpr bool MASK = decltype(mask_c)::value;
+    const unsigned va = fresh(vcol + (unsigned)((t % kFwdStages) * kTileHalves * 2));
+    const int lim = jlim - (it.tb + t) * kBN - 4 * hl;
+    unsigned on = 0;
+    if constexpr (MASK) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        const i32x4 e4 = *reinterpret_cast<const i32x4*>(&ends[t % kFwdStages][8 * q + 4 * hl]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool k = (8 * q + e <= lim) & (m < e4[e]);
+          on |= k ? 1u << (4 * q + e) : 0u;
+          sc[q >> 2][4 * (q & 3) + e] = k ? sc[q >> 2][4 * (q & 3) + e] : -1.0e30f;
+        }
+      }
+    }
+    // the row maximum of the raw scores, scaled once (the scaling is monotonic)
+    float mx = -1.0e30f;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[kb][v]);
+    mx = half_max(mx);
+    // m_i moves (and O and l are rescaled) only when some lane's maximum exceeds it by more than
+    // 2^8, so p stays below 256
+    const float mt = __fmul_rn(mx, a.qk_scale);
+    if (__builtin_amdgcn_ballot_w64(mt > m_i + 8.0f) != 0) {
+      const float m_new = fmaxf(m_i, mt);
+      const float alpha = ex2(__fsub_rn(m_i, m_new));
+      l_i = __fmul_rn(l_i, alpha);
+      m_i = m_new;
+#pragma unroll
+      for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) oacc[hb][v] = __fmul_rn(oacc[hb][v], alpha);
+    }
+    if (!MASK || more) scores(sn, t + 2);
+    else sn[0] = sn[1] = zero16();   // nothing of the last tile's buffer stays live
+    float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    f16x8 pf[kBN / 16];   // P^T as the B operand: keys 16 tt .. + 15
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        float p = ex2(__builtin_fmaf(sc[kb][v], a.qk_scale, -m_i));
+        if constexpr (MASK) p = (on >> (16 * kb + v)) & 1 ? p : 0.0f;
+        rs[v & 3] = __fadd_rn(rs[v & 3], p);
+        pf[2 * kb + (v >> 3)][v & 7] = (f16)p;
+      }
+    l_i = __fadd_rn(l_i, __fadd_rn(__fadd_rn(rs[0], rs[1]), __fadd_rn(rs[2], rs[3])));
+    // O^T += V^T P^T over the tile's 64 keys, 16 per step
+#pragma unroll
+    for (int tt = 0; tt < kBN / 16; ++tt)
+#pragma unroll
+      for (int hb = 0; hb < kHD / 32; ++hb)
+        oacc[hb] = mfma(lds_col8(va, hb, 16 * tt * kHD * 2), pf[tt], oacc[hb]);
+    // the next tile's scores spread over the exponentials, their operands read four MFMAs ahead;
+    // then O, its operands four MFMAs (eight reads) ahead
+    if constexpr (!MASK) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < 12; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+      }
+    } else {
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 200, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  };
+  using Mask = std::integral_constant<bool, true>;
+  using Full = std::integral_constant<bool, false>;
+  // V of pair u and K of pair u + 1 are in LDS; K of pair u + 2 goes where pair u's was (its
+  // scores are done), V of pair u + 1 where pair u - 1's was
+  auto fetch = [&](int u) {
+    issue_v(u + 1);
+    issue(kbase, Ks, u + 2);
+  };
+  auto next = [&]() {
+    wait_vmem<0>();
+    __syncthreads();
+  };
+  // this wave's tile of pair u: unmasked, and with a next tile whose scores it computes beside it
+  auto full = [&](int u) {
+    return 2 * u + kg + 2 < n_tiles && full_tile(it, it.tb + 2 * u + kg);
+  };
+  int u = 0;
+  while (u < n_pairs) {
+    for (; full(u) && full(u + 1); u += 2) {   // the two score buffers need no copies
+      fetch(u);
+      tile(2 * u + kg, true, sc, sn, Full{});
+      next();
+      fetch(u + 1);
+      tile(2 * u + 2 + kg, true, sn, sc, Full{});
+      next();
+    }
+    if (u < n_pairs) {
+      fetch(u);
+      const int t = 2 * u + kg;
+      if (t < n_tiles) tile(t, t + 2 < n_tiles, sc, sn, Mask{});
+      else sn[0] = sn[1] = zero16();
+      sc[0] = sn[0];
+      sc[1] = sn[1];
+      next();
+      ++u;
+    }
+  }
+  l_i = __fadd_rn(l_i, __shfl_xor(l_i, 32));
+  // merge: the odd-tile wave of each query group hands its state (O lane-major, 16 KB per wave,
+  // in the K stages; m and l in the V stages' last KB) to the even-tile wave
+  float* ohand = reinterpret_cast<float*>(Ks) + qw * (kHD / 32) * 16 * 64;
+  float* mlhand = reinterpret_cast<float*>(Vs) + (kFwdStages * kTileHalves / 2 - 256) + qw * 64;
+  static_assert(4 * (kHD / 32) * 16 * 64 * 4 <= kFwdStages * kTileHalves * 2, "O hand-over in Ks");
+  if (kg == 1) {
+#pragma unroll
+    for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) ohand[(hb * 16 + v) * 64 + lane] = oacc[hb][v];
+    if (hl == 0) {
+      mlhand[c] = m_i;
+      mlhand[32 + c] = l_i;
+    }
+  }
+  __syncthreads();
+  constexpr int kOStride = kHD + 8;   // halves per staged row
+  static_assert(4 * 32 * kOStride + 512 <= kFwdStages * kTileHalves, "O staging in Vs");
+  f16* ostage = Vs + qw * 32 * kOStride;
+  if (kg == 0) {
+    const float m1 = mlhand[c], l1 = mlhand[32 + c];
+    const float mm = fmaxf(m_i, m1);
+    const float a0 = ex2(__fsub_rn(m_i, mm)), a1 = ex2(__fsub_rn(m1, mm));
+    const float l = __fadd_rn(__fmul_rn(l_i, a0), __fmul_rn(l1, a1));
+    if (it.slot >= 0) {
+      float* part = parts + (int64_t)it.slot * kPartFloats;
+#pragma unroll
+      for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          part[((qw * (kHD / 32) + hb) * 16 + v) * 64 + lane] =
+              __fadd_rn(__fmul_rn(oacc[hb][v], a0), __fmul_rn(ohand[(hb * 16 + v) * 64 + lane], a1));
+      if (hl == 0) {
+        part[kBM * kHD + row] = mm;
+        part[kBM * kHD + kBM + row] = l;
+      }
+      return;
+    }
+    const float inv_l = __fdiv_rn(1.0f, l);   // rows past the block: not stored
+    float chk = __fmul_rn(l, 0.0f);           // NaN if anything below is not finite
+#pragma unroll
+    for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f16x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = 4 * q + e;
+          const float ov = __fadd_rn(__fmul_rn(oacc[hb][v], a0),
+                                     __fmul_rn(ohand[(hb * 16 + v) * 64 + lane], a1));
+          chk = __builtin_fmaf(ov, 0.0f, chk);
+          o[e] = (f16)__fmul_rn(ov, inv_l);
+        }
+        *reinterpret_cast<f16x4*>(ostage + c * kOStride + hb * 32 + 8 * q + 4 * hl) = o;
+      }
+    chk = __fadd_rn(chk, __shfl_xor(chk, 32));
+    if (chk != 0.0f) bad[row] = 1;
+    else if (mval && hl == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(mm, log2f(l));
+  } else if (it.slot >= 0) {
+    return;
+  }
+  __syncthreads();
+  // the two waves of a query group store 16 of its 32 rows each, four whole 256-byte rows per store
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 16 * kg + 4 * i + (lane >> 4), cc = lane & 15;
+    const int srow = 32 * qw + r, sr = it.phase + srow;
+    const f16x8 v = *reinterpret_cast<const f16x8*>(ostage + r * kOStride + 8 * cc);
+    if (srow < it.rows && !bad[srow])
+      *reinterpret_cast<f16x8*>(out + (int64_t)(it.t0 + sr / gin) * a.nq * kHD +
+                                (int64_t)(it.g * gin + sr % gin) * kHD + 8 * cc) = v;
+  }
+  static_assert(kFWaves * sizeof(RowScratch) <= kFwdStages * kTileHalves * 2, "row scratch in Ks");
+  redo_rows<kFWaves>(a, it.t0, it.phase, it.rows, it.g, bad, reinterpret_cast<RowScratch*>(Ks), out, lse);
+}
+
+// The partials of a block put together: O = sum_s O_s 2^(m_s - m) / l, m = max m_s, l likewise, in slot
+// order.  Wave w takes query group w / 2 and half w % 2 of the columns.
+__global__ __launch_bounds__(kFThreads) void span_join_kernel(SpanArgs a, const int32_t* __restrict__ joins,
+                                                              int n_slots, f16* __restrict__ out,
+                                                              float* __restrict__ lse,
+                                                              const float* __restrict__ parts) {
+  const int32_t* j = joins + (int64_t)blockIdx.x * DK_ATTN_SPAN_JOIN_INTS;
+  const int t0 = j[0], phase = j[1], rows = j[2], g = j[3], s0 = j[4], cnt = j[5];
+  const int gin = a.nq / a.nkv;
+  if (t0 < 0 || phase < 0 || phase >= gin || rows < 1 || rows > kBM || g < 0 || g >= a.nkv ||
+      (int64_t)t0 + (phase + rows - 1) / gin >= a.n_tokens || s0 < 0 || cnt < 1 || cnt > n_slots - s0)
+    return;
+  __shared__ int bad[kBM];
+  __shared__ RowScratch scratch[kFWaves];
+  if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, hl = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int qw = wave >> 1, hb0 = 2 * (wave & 1), row = 32 * qw + c;
+  const float* p0 = parts + (int64_t)s0 * kPartFloats;
+  float mm = -1.0e30f;
+  for (int s = 0; s < cnt; ++s) mm = fmaxf(mm, p0[(int64_t)s * kPartFloats + kBM * kHD + row]);
+  float l = 0.0f;
+  f32x16 o[2] = {zero16(), zero16()};
+  for (int s = 0; s < cnt; ++s) {
+    const float* p = p0 + (int64_t)s * kPartFloats;
+    const float w = ex2(__fsub_rn(p[kBM * kHD + row], mm));
+    l = __builtin_fmaf(p[kBM * kHD + kBM + row], w, l);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        o[b][v] = __builtin_fmaf(p[((qw * (kHD / 32) + hb0 + b) * 16 + v) * 64 + lane], w, o[b][v]);
+  }
+  float chk = __fmul_rn(l, 0.0f);
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) chk = __builtin_fmaf(o[b][v], 0.0f, chk);
+  if (chk != 0.0f) bad[row] = 1;
+  __syncthreads();
+  if (row < rows && !bad[row]) {
+    const int rr = phase + row, m = t0 + rr / gin, h = g * gin + rr % gin;
+    const float inv_l = __fdiv_rn(1.0f, l);
+    f16* orow = out + (int64_t)m * a.nq * kHD + (int64_t)h * kHD;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f16x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (f16)__fmul_rn(o[b][4 * q + e], inv_l);
+        *reinterpret_cast<f16x4*>(orow + (hb0 + b) * 32 + 8 * q + 4 * hl) = x;
+      }
+    if (hl == 0 && hb0 == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(mm, log2f(l));
+  }
+  redo_rows<kFWaves>(a, t0, phase, rows, g, bad, scratch, out, lse);
 }
 
 }  // namespace
 
-extern "C" int dk_attn_span_fwd(const void* qkv, const int32_t* spans, int64_t n_tokens, int32_t nq,
-                                int32_t nkv, int32_t hd, void* out, float* lse, hipStream_t stream) {
+extern "C" int64_t dk_attn_span_workspace(int64_t n_slots) {
+  return n_slots > 0 ? n_slots * (int64_t)(kPartFloats * sizeof(float)) : 0;
+}
+
+extern "C" int dk_attn_span_fwd(const void* qkv, const int32_t* spans, const int32_t* items,
+                                int32_t n_items, const int32_t* joins, int32_t n_joins,
+                                int32_t n_slots, int64_t n_tokens, int32_t nq, int32_t nkv, int32_t hd,
+                                void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                hipStream_t stream) {
   SpanArgs a;
   if (int e = span_args(a, qkv, spans, n_tokens, nq, nkv, hd)) return e;
-  if (n_tokens == 0) return 0;
-  if (!out || !lse) return DK_ERR_INVALID;
-  if (!dk_aligned(out, 16) || !dk_aligned(lse, 4)) return DK_ERR_ALIGN;
-  const int64_t wgs = (n_tokens * nq + 3) / 4;
-  if (wgs > INT32_MAX / kAThreads) return DK_ERR_INVALID;
-  hipLaunchKernelGGL(span_fwd_rows_kernel, dim3((unsigned)wgs), dim3(kAThreads), 0, stream, a,
-                     (f16*)out, lse);
+  if (n_items < 0 || n_joins < 0 || n_slots < 0) return DK_ERR_INVALID;
+  if (n_tokens == 0 || n_items == 0) return 0;
+  if (!items || !out || !lse || (n_joins > 0 && !joins)) return DK_ERR_INVALID;
+  if (!dk_aligned(out, 16) || !dk_aligned(lse, 4) || !dk_aligned(items, 4) || !dk_aligned(joins, 4) ||
+      !dk_aligned(workspace, 256))
+    return DK_ERR_ALIGN;
+  if (n_slots > 0 && (!workspace || workspace_bytes < dk_attn_span_workspace(n_slots)))
+    return DK_ERR_WORKSPACE;
+  if (n_items > INT32_MAX / kFThreads || n_joins > INT32_MAX / kFThreads) return DK_ERR_INVALID;
+  hipLaunchKernelGGL(span_fwd_kernel, dim3((unsigned)n_items), dim3(kFThreads), 0, stream, a, items,
+                     n_slots, (f16*)out, lse, (float*)workspace);
   DK_CHECK_LAUNCH();
+  if (n_joins > 0) {
+    hipLaunchKernelGGL(span_join_kernel, dim3((unsigned)n_joins), dim3(kFThreads), 0, stream, a, joins,
+                       n_slots, (f16*)out, lse, (const float*)workspace);
+    DK_CHECK_LAUNCH();
+  }
   return 0;
 }

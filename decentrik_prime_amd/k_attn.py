@@ -153,12 +153,72 @@ class SpanMeta:
         if spans.shape[0] > MAX_SPAN_TOKENS:
             raise ValueError(f"at most {MAX_SPAN_TOKENS} tokens (got {spans.shape[0]})")
         self.n_tokens, self.nq, self.nkv = int(spans.shape[0]), int(nq), int(nkv)
+        blocks = _query_blocks(runs, spans, nq // nkv, nkv)
+        items, joins, self.n_slots = _split_items(blocks, _fwd_tiles(blocks))
         i32 = dict(dtype=torch.int32, device=device)
         self.spans = torch.tensor(spans, **i32)
         self.positions = torch.tensor(positions, **i32)
+        self.items, self.joins = torch.tensor(items, **i32), torch.tensor(joins, **i32)
 
 
 MAX_SPAN_TOKENS = 1 << 30
+_KEYS = 64            # keys of a tile
+_ROWS = 128           # stacked query rows of a block
+# columns of an item (include/dk.h)
+_T0, _PHASE, _N_ROWS, _G, _A0, _NA, _B0, _NK, _F0, _F1, _F2, _TB, _TE, _SLOT = range(14)
+
+
+def _query_blocks(runs, spans, gin, nkv):
+    """The blocks of stacked query rows of every run of tokens (all with the same [a0, a1) and with kbeg
+    and kend that do not fall) and every KV head, as items [n, 16] that walk all of their tiles."""
+    parts = []
+    for r0, r1 in runs:
+        j0 = np.arange(0, (r1 - r0) * gin, _ROWS, dtype=np.int64)
+        rows = np.minimum(_ROWS, (r1 - r0) * gin - j0)
+        t0, last = r0 + j0 // gin, r0 + (j0 + rows - 1) // gin
+        a0, a1, kbeg = (spans[t0, i] for i in range(3))
+        # the window of the first row meets the sinks: one run of keys from a0
+        one = (a1 > a0) & (kbeg <= a1)
+        na = np.where(one | (a1 <= a0), 0, a1 - a0)
+        b0 = np.where(one, a0, kbeg)
+        nk = na + last + 1 - b0
+        # every row sees the first run, and of the second the keys from the last row's kbeg to t0
+        lo = np.maximum(spans[last, 2], b0) - b0 + na
+        hi = t0 - b0 + na + 1
+        x = np.zeros((j0.size, 16), np.int64)
+        x[:, _T0], x[:, _PHASE], x[:, _N_ROWS] = t0, j0 % gin, rows
+        x[:, _A0], x[:, _NA], x[:, _B0], x[:, _NK] = a0, na, b0, nk
+        x[:, _F0] = np.where(lo == na, hi, na) // _KEYS
+        x[:, _F1] = -(-lo // _KEYS)
+        x[:, _F2] = np.maximum(hi // _KEYS, x[:, _F1])
+        x[:, _TE], x[:, _SLOT] = -(-nk // _KEYS), -1
+        parts += [x + np.eye(1, 16, _G, dtype=np.int64) * g for g in range(nkv)]
+    return np.concatenate(parts) if parts else np.empty((0, 16), np.int64)
+
+
+def _fwd_tiles(blocks):
+    """Tiles per item of the forward."""
+    return 1 << 30
+
+
+def _split_items(blocks, most):
+    """(items, joins, partials): blocks of more than `most` tiles cut into walks of as many tiles each,
+    longest walks first."""
+    n = blocks[:, _TE]
+    cut = -(-n // most)
+    idx = np.repeat(np.arange(n.size), cut)
+    part = np.arange(idx.size) - np.repeat(np.cumsum(cut) - cut, cut)
+    items = blocks[idx].copy()
+    items[:, _TB] = part * n[idx] // cut[idx]
+    items[:, _TE] = (part + 1) * n[idx] // cut[idx]
+    split = cut > 1
+    first = np.cumsum(np.where(split, cut, 0)) - np.where(split, cut, 0)
+    items[:, _SLOT] = np.where(split[idx], first[idx] + part, -1)
+    joins = np.zeros((int(split.sum()), 8), np.int64)
+    joins[:, :4] = blocks[split][:, [_T0, _PHASE, _N_ROWS, _G]]
+    joins[:, 4], joins[:, 5] = first[split], cut[split]
+    order = np.argsort(items[:, _TB] - items[:, _TE], kind="stable")
+    return items[order], joins, int(cut[split].sum())
 
 
 def _lengths(lens, what):
@@ -232,9 +292,14 @@ def span_attention_forward(qkv, meta, nq, nkv, hd):
     n, dev = meta.n_tokens, qkv.device
     out = torch.empty((n, nq * hd), dtype=torch.float16, device=dev)
     lse = torch.empty((nq, n), dtype=torch.float32, device=dev)
+    nbytes = _lib.lib().dk_attn_span_workspace(meta.n_slots)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with torch.cuda.device(dev):
-        rc = _lib.lib().dk_attn_span_fwd(_lib.ptr(qkv), _lib.ptr(meta.spans), n, nq, nkv, hd,
-                                         _lib.ptr(out), _lib.ptr(lse), _lib.stream_handle(dev))
+        rc = _lib.lib().dk_attn_span_fwd(_lib.ptr(qkv), _lib.ptr(meta.spans), _lib.ptr(meta.items),
+                                         meta.items.shape[0], _lib.ptr(meta.joins),
+                                         meta.joins.shape[0], meta.n_slots, n, nq, nkv, hd,
+                                         _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws), nbytes,
+                                         _lib.stream_handle(dev))
     _lib.check(rc, "dk_attn_span_fwd")
     return out, lse
 

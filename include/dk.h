@@ -168,9 +168,27 @@ int dk_attn_bwd(const void* qkv, const void* out, const float* lse, const void* 
  * a key, by the queries m .. kend - 1 (a0, a1, kbeg, kend in this order; the two describe the same
  * pairs).  qkv, out and lse as for dk_attn_fwd.  The backward writes fp16 gradients, dk and dv
  * [n_tokens, nkv hd] summed over the heads of each group; delta [nq, n_tokens] fp32 is scratch.
- * A key that a query does not see has no influence on it, whatever it holds. */
-int dk_attn_span_fwd(const void* qkv, const int32_t* spans, int64_t n_tokens, int32_t nq,
-                     int32_t nkv, int32_t hd, void* out, float* lse, hipStream_t stream);
+ * A key that a query does not see has no influence on it, whatever it holds.
+ *
+ * items [n_items][16] int32: the forward's blocks of up to 128 stacked query rows, as
+ * k_attn.SpanMeta writes them from spans: t0, phase, rows, g, a0, na, b0, nk, f0, f1, f2, tb, te,
+ * slot, 0, 0.  Row i of a block is token t0 + (phase + i) / gin, query head g gin + (phase + i) % gin
+ * (gin = nq / nkv); its keys are the na rows from a0 and nk - na rows from b0, the last of them its last
+ * row's token, in tiles of 64, of which it walks [tb, te); every row sees all of the tiles [0, f0) and
+ * [f1, f2).  slot -1: the block's rows of out and lse; slot s >= 0: partial s of the workspace
+ * (dk_attn_span_workspace(n_slots) bytes, 256-byte aligned, n_slots the count of partials), which
+ * joins [n_joins][8] int32 put together: t0, phase, rows, g, first slot, slots, 0, 0.  An entry that
+ * names rows outside the batch or slots outside the workspace is skipped. */
+#define DK_ATTN_SPAN_ITEM_INTS 16
+/* The keys of both runs of an item lie within this many bytes of qkv rows (an item whose do not is
+ * skipped, too). */
+#define DK_ATTN_SPAN_REACH_BYTES 0xfff00000u
+#define DK_ATTN_SPAN_JOIN_INTS 8
+int64_t dk_attn_span_workspace(int64_t n_slots);
+int dk_attn_span_fwd(const void* qkv, const int32_t* spans, const int32_t* items, int32_t n_items,
+                     const int32_t* joins, int32_t n_joins, int32_t n_slots, int64_t n_tokens,
+                     int32_t nq, int32_t nkv, int32_t hd, void* out, float* lse, void* workspace,
+                     int64_t workspace_bytes, hipStream_t stream);
 int dk_attn_span_bwd(const void* qkv, const void* out, const float* lse, const void* dout,
                      const int32_t* spans, int64_t n_tokens, int32_t nq, int32_t nkv, int32_t hd,
                      float* delta, void* dq, void* dk, void* dv, hipStream_t stream);

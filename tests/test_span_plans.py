@@ -92,3 +92,49 @@ def test_call_refusals_before_any_launch():
                  lambda: k_attn.span_attention_forward(qkv, meta, 2, 2, HD)):              # other heads
         with pytest.raises(ValueError):
             call()
+
+
+def _pairs_of_items(meta, rows_seen):
+    """Walks a plan's items as the kernel does and counts, per stacked row, the keys it visits."""
+    gin, s = meta.nq // meta.nkv, np.asarray(meta.spans, np.int64)
+    count = np.zeros((meta.nkv, gin, meta.n_tokens, meta.n_tokens), np.int64)
+    for it in np.asarray(meta.items, np.int64):
+        t0, phase, rows, g, a0, na, b0, nk, f0, f1, f2, tb, te, slot = it[:14]
+        assert 1 <= rows <= 128 and 0 <= phase < gin and 0 <= tb < te <= -(-nk // 64)
+        j = np.arange(64 * tb, min(64 * te, nk))
+        key = np.where(j < na, a0 + j, b0 + j - na)
+        full = (j // 64 < f0) | ((j // 64 >= f1) & (j // 64 < f2))
+        for i in range(rows):
+            m, e = t0 + (phase + i) // gin, (phase + i) % gin
+            seen = (j <= m - b0 + na) & (m < s[key, 3])
+            assert not (full & ~seen).any(), "a tile named full holds a masked key"
+            count[g, e, m, key[seen]] += 1
+            rows_seen[g * gin + e, m] += slot < 0 or tb == 0
+    return count
+
+
+@pytest.mark.parametrize("nq,nkv", [(4, 2), (5, 1), (3, 3)])
+def test_items_visit_every_visible_pair_once(nq, nkv):
+    for make, spec in ([(attn.window_visible, w) for w in WINDOWS + [([300, 41], 100, 3), ([260], 30, 90)]] +
+                       [(attn.prefix_visible, (g,)) for g in GROUPS + [[(200, [40, 3, 70]), (9, [150])]]]):
+        build = k_attn.window_meta if make is attn.window_visible else k_attn.prefix_meta
+        meta = build(*spec, nq, nkv, "cpu")
+        rows = np.zeros((nq, meta.n_tokens), np.int64)
+        count = _pairs_of_items(meta, rows)
+        assert (rows == 1).all()
+        assert (count == make(*spec)[None, None]).all()
+
+
+def test_split_items_cover_the_walks():
+    meta = k_attn.window_meta([700, 20], 400, 4, 12, 2, "cpu")
+    blocks = k_attn._query_blocks([(0, 700), (700, 720)], np.asarray(meta.spans, np.int64), 6, 2)
+    for most in (1, 2, 3, 100):
+        items, joins, slots = k_attn._split_items(blocks, most)
+        assert (items[:, 12] - items[:, 11]).max() <= most and (items[:, 12] > items[:, 11]).all()
+        assert sorted(x for x in items[:, 13] if x >= 0) == list(range(slots))
+        for t0, phase, rows, g, first, cnt, _, _ in joins:
+            own = items[(items[:, 13] >= first) & (items[:, 13] < first + cnt)]
+            own = own[np.argsort(own[:, 13])]
+            assert len(own) == cnt > 1 and (own[:, [0, 1, 2, 3]] == [t0, phase, rows, g]).all()
+            assert own[0, 11] == 0 and (own[1:, 11] == own[:-1, 12]).all()
+            assert own[-1, 12] == -(-own[-1, 7] // 64)
