@@ -141,8 +141,9 @@ SIGNATURES = {
     "dk_attn_span_workspace": (_i64, [_i64]),
     "dk_attn_span_fwd": (_int, [_c_p, _c_p, _c_p, _int, _c_p, _int, _int, _i64, _int, _int, _int, _c_p,
                                 _c_p, _c_p, _i64, _c_p]),
-    "dk_attn_span_bwd": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _i64, _int, _int, _int, _c_p, _c_p,
-                                _c_p, _c_p, _c_p]),
+    "dk_attn_span_bwd_workspace": (_i64, [_i64]),
+    "dk_attn_span_bwd": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _int, _c_p, _int, _int, _i64, _int,
+                                _int, _int, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p]),
     "dk_head_chunk": (_int, [_c_p, _c_p, _c_p, _c_p, _i64, _i64, _i64, _i64, _f32, _i64, _c_p]),
     "dk_head_finalize": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _i64, _f32, _f32,
                                 _i64, _c_p]),

@@ -10,6 +10,8 @@
 
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
 struct SpanArgs {
   const f16* qkv;
   const int32_t* spans;
@@ -204,7 +206,7 @@ __device__ __forceinline__ void span_row_fwd(const SpanArgs& a, int64_t m, int h
 }
 
 // dq of query m, head h
-__device__ __noinline__ void span_row_dq(const SpanArgs& a, int64_t m, int h, const f16* dout,
+__device__ __forceinline__ void span_row_dq(const SpanArgs& a, int64_t m, int h, const f16* dout,
                                          const float* lse, const float* delta, f16* dq,
                                          RowScratch& s) {
   const int lane = threadIdx.x & 63;
@@ -244,7 +246,7 @@ __device__ __noinline__ void span_row_dq(const SpanArgs& a, int64_t m, int h, co
 }
 
 // dk and dv of key n, KV head g, summed over the queries that see it and the heads of its group
-__device__ __noinline__ void span_key_dkdv(const SpanArgs& a, int64_t n, int g, const f16* dout,
+__device__ __forceinline__ void span_key_dkdv(const SpanArgs& a, int64_t n, int g, const f16* dout,
                                            const float* lse, const float* delta, f16* dk, f16* dv,
                                            RowScratch& s) {
   const int lane = threadIdx.x & 63;

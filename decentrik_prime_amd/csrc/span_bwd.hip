@@ -1,44 +1,667 @@
-// Backward of the attention over part of the keys (attn_span.h): delta, then a wave per (query, head)
-// for dq and per (key, KV head) for dk and dv.
+// Backward of the attention over part of the keys (attn_span.h): delta, then dK/dV and dQ on MFMA tiles,
+// then the partials of walks that were split.  The tile steps are attn.hip's.
 #include "attn_delta.h"
 #include "attn_span.h"
 
 namespace {
 
-__global__ __launch_bounds__(kAThreads) void span_bwd_rows_kernel(
-    SpanArgs a, const f16* __restrict__ dout, const float* __restrict__ lse,
-    const float* __restrict__ delta, f16* __restrict__ dq, f16* __restrict__ dk, f16* __restrict__ dv) {
-  __shared__ RowScratch s[kAThreads / 64];
-  const int w = threadIdx.x >> 6;
-  int64_t i = (int64_t)blockIdx.x * (kAThreads / 64) + w;
-  if (i < a.n_tokens * a.nkv) {
-    span_key_dkdv(a, i / a.nkv, (int)(i % a.nkv), dout, lse, delta, dk, dv, s[w]);
+constexpr int kUnitFloats = kBM * kHD;   // a partial of dQ; dK and dV take two
+constexpr int kStride16 = kHD + 8;       // halves per staged row of a result
+
+// The tile ring of both backward kernels: a tile of two operands (kBN rows each) in one of four
+// LDS stages, filled by LDS DMA.  Wave w's instruction i fills chunks (4 i + w) 64 + lane of an
+// operand: row 16 i + 4 w + lane / 16, with a wave-uniform base per tile and a 32-bit offset per
+// lane; rows past `rows` (the rows left in the sequence, less one) read that row (finite, masked
+// to p = 0).
+constexpr int kBwdStages = 4;
+constexpr int kBwdLoads = kTileHalves / 8 / kAThreads;   // per operand per lane: 4
+constexpr unsigned kStageBytes = kTileHalves * 2;
+
+struct TileSource {
+  uint64_t base;      // first row of tile 0
+  unsigned rowb;      // bytes per row
+  unsigned off0;      // this lane's offset for instruction 0
+  unsigned chunk;     // this lane's (swizzled) chunk offset inside a row
+};
+__device__ __forceinline__ TileSource tile_source(const f16* base, int64_t row_halves, int wave,
+                                                  int lane) {
+  TileSource t;
+  t.base = uniform64((uint64_t)base);
+  t.rowb = (unsigned)(row_halves * (int64_t)sizeof(f16));
+  const int r0 = 4 * wave + (lane >> 4);
+  t.chunk = (unsigned)(((lane & 15) ^ swz16(r0)) << 4);
+  t.off0 = (unsigned)r0 * t.rowb + t.chunk;
+  return t;
+}
+__device__ __forceinline__ void tile_load(const TileSource& src, int64_t first_row, uint64_t more, int rows,
+                                          const f16* stage, int wave) {
+  const uint64_t tb = src.base + (uint64_t)first_row * src.rowb + more;
+  const unsigned last = (unsigned)(rows < kBN ? rows : kBN) * src.rowb + src.chunk;
+#pragma unroll
+  for (int i = 0; i < kBwdLoads; ++i) {
+    const unsigned off = src.off0 + (unsigned)(16 * i) * src.rowb;
+    dma16s(tb, off < last ? off : last,
+           __builtin_amdgcn_readfirstlane(lds_addr(stage + (4 * i + wave) * 512)));
+  }
+}
+
+// A barrier that orders the LDS DMA waited for before it, without a wait for the operand reads in
+// flight (they are of stages that no load in flight touches).
+__device__ __forceinline__ void tile_barrier() {
+  wait_vmem<0>();
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+constexpr int kAhead1 = 6, kAhead2 = 4;
+
+// The rows (or keys) whose result is not finite, recomputed over exactly what they see: 0 times a NaN
+// or infinity of a masked row is not 0.  bad: row flags in LDS, written before a barrier.
+template <int W>
+__device__ __forceinline__ void redo_dq(const SpanArgs& a, int t0, int phase, int rows, int g,
+                                        const int* bad, RowScratch* s, const f16* dout, const float* lse,
+                                        const float* delta, f16* dq) {
+  const int gin = a.nq / a.nkv, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  for (int i = wave; i < rows; i += W) {
+    if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
+    span_row_dq(a, t0 + (phase + i) / gin, g * gin + (phase + i) % gin, dout, lse, delta, dq, s[wave]);
+  }
+}
+template <int W>
+__device__ __forceinline__ void redo_dkdv(const SpanArgs& a, int k0, int nk, int g, const int* bad,
+                                          RowScratch* s, const f16* dout, const float* lse,
+                                          const float* delta, f16* dk, f16* dv) {
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  __syncthreads();   // the staged rows have been read
+  for (int i = wave; i < nk; i += W) {
+    if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
+    span_key_dkdv(a, (int64_t)k0 + i, g, dout, lse, delta, dk, dv, s[wave]);
+  }
+}
+
+// The wave's 32 keys of dK and dV, rounded, staged in its quarter of two LDS buffers and written back
+// 16 bytes per lane, four whole rows per store.  Result register v of block hb: key 32 w +
+// 8 (v / 4) + 4 (l / 32) + v % 4, column 32 hb + l % 32.
+__device__ __forceinline__ void store_dkdv(const SpanArgs& a, int k0, int nk, int g,
+                                           const f32x16 (&dkacc)[kHD / 32], const f32x16 (&dvacc)[kHD / 32],
+                                           f16* s0, f16* s1, int* bad, f16* dk, f16* dv) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hl = lane >> 5, c = lane & 31;
+  f16* kst = s0 + w * 32 * kStride16;
+  f16* vst = s1 + w * 32 * kStride16;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) {
+    const int r = 8 * (v >> 2) + 4 * hl + (v & 3);
+    float chk = 0.0f;   // NaN if a value is not finite
+#pragma unroll
+    for (int hb = 0; hb < kHD / 32; ++hb) {
+      chk = __builtin_fmaf(dkacc[hb][v], 0.0f, __builtin_fmaf(dvacc[hb][v], 0.0f, chk));
+      kst[r * kStride16 + hb * 32 + c] = (f16)__fmul_rn(dkacc[hb][v], a.sm_scale);
+      vst[r * kStride16 + hb * 32 + c] = (f16)dvacc[hb][v];
+    }
+    if (chk != 0.0f) bad[32 * w + r] = 1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 4), cc = lane & 15, key = 32 * w + r;
+    const f16x8 kv = *reinterpret_cast<const f16x8*>(kst + r * kStride16 + 8 * cc);
+    const f16x8 vv = *reinterpret_cast<const f16x8*>(vst + r * kStride16 + 8 * cc);
+    if (key < nk && !bad[key]) {
+      const int64_t o = ((int64_t)k0 + key) * a.nkv * kHD + (int64_t)g * kHD + 8 * cc;
+      *reinterpret_cast<f16x8*>(dk + o) = kv;
+      *reinterpret_cast<f16x8*>(dv + o) = vv;
+    }
+  }
+}
+
+// dQ of a block of stacked query rows, over the key tiles of its item
+__device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items, int idx, int n_units,
+                                        const f16* __restrict__ dout, const float* __restrict__ lse,
+                                        const float* __restrict__ delta, f16* __restrict__ dq,
+                                        float* __restrict__ parts, f16* Ks, f16* Vs, int (*ends)[kBN],
+                                        int* bad) {
+  SpanItem it;
+  if (!span_item(a, items, idx, n_units, &it)) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hl = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(w);
+  const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
+  const int gin = a.nq / a.nkv, row = 32 * w + c;
+  const bool mval = row < it.rows;
+  const int rr = it.phase + (mval ? row : 0);
+  const int m = it.t0 + rr / gin, h = it.g * gin + rr % gin;
+  const int jlim = mval ? m - it.b0 + it.na : -1;   // this lane's last key
+
+  const int n_tiles = it.te - it.tb;
+  const KeySource src = key_source(ROW, wave, lane);
+  const uint64_t kbase = uniform64((uint64_t)(a.qkv + (int64_t)(a.nq + it.g) * kHD));
+  const uint64_t vbase = kbase + (uint64_t)a.nkv * kHD * sizeof(f16);
+  auto issue = [&](int t) {
+    if (t >= n_tiles) return;
+    const int st = t % kBwdStages;
+    key_tile_load<4>(it, src, it.tb + t, kbase, Ks + st * kTileHalves, wave);
+    key_tile_load<4>(it, src, it.tb + t, vbase, Vs + st * kTileHalves, wave);
+    if (wave == 0) key_ends_load(a, it, it.tb + t, ends[st], lane);
+  };
+  issue(0);
+  issue(1);
+  issue(2);
+  // this lane's query and dO rows and statistics, loaded unconditionally and selected at once (the
+  // compiler's wait for them stands here, not in the loop)
+  f16x8 qf[kHD / 16], dof[kHD / 16];
+  float lse_m, dl_m;
+  {
+    const f16* qrow = a.qkv + (int64_t)m * ROW + (int64_t)h * kHD + 8 * hl;
+    const f16* drow = dout + (int64_t)m * OROW + (int64_t)h * kHD + 8 * hl;
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) {
+      qf[s] = *reinterpret_cast<const f16x8*>(qrow + 16 * s);
+      dof[s] = *reinterpret_cast<const f16x8*>(drow + 16 * s);
+    }
+    lse_m = lse[(int64_t)h * a.n_tokens + m];
+    dl_m = delta[(int64_t)h * a.n_tokens + m];
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) asm volatile("" : "+v"(qf[s]), "+v"(dof[s]));
+    asm volatile("" : "+v"(lse_m), "+v"(dl_m));
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) {
+      qf[s] = mval ? qf[s] : zero8();
+      dof[s] = mval ? dof[s] : zero8();
+    }
+    lse_m = mval ? lse_m : 0.0f;
+    dl_m = mval ? dl_m : 0.0f;
+  }
+  if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
+  f32x16 dqacc[kHD / 32];
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb) dqacc[hb] = zero16();
+  const unsigned krow = lds_addr(Ks) + row_base(lane), vrow = lds_addr(Vs) + row_base(lane);
+  const unsigned kcol = lds_addr(Ks) + col_base(lane);
+  // operand i of a tile's products: S^T = K Q^T and dP^T = V dO^T (keys kb * 32 + (row), queries
+  // on the lanes): sub-step i / 4, dP^T for i / 2 odd, key half i % 2
+  auto rd1 = [&](unsigned ka, unsigned va, int i) {
+    return lds_read8((((i >> 1) & 1) ? va : ka) ^ (unsigned)(32 * (i >> 2)), (i & 1) * 32 * kHD * 2);
+  };
+  auto product = [&](f32x16 (&sacc)[2], f32x16 (&dpacc)[2], const f16x8& f, int i) {
+    const int s = i >> 2, kb = i & 1;
+    if ((i >> 1) & 1) dpacc[kb] = mfma(f, dof[s], s == 0 ? zero16() : dpacc[kb]);
+    else sacc[kb] = mfma(f, qf[s], s == 0 ? zero16() : sacc[kb]);
+  };
+  f16x8 fr[kAhead1];
+  // the wait for all three tiles costs no more than the query rows' own
+  tile_barrier();
+  f32x16 s_a[2], d_a[2], s_b[2], d_b[2];
+  {
+    const unsigned ka = fresh(krow), va = fresh(vrow);
+#pragma unroll
+    for (int i = 0; i < kAhead1; ++i) fr[i] = rd1(ka, va, i);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      product(s_a, d_a, fr[i % kAhead1], i);
+      if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(ka, va, i + kAhead1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const unsigned ka1 = fresh(krow + kStageBytes), va1 = fresh(vrow + kStageBytes);
+#pragma unroll
+    for (int i = 0; i < kAhead1; ++i) fr[i] = rd1(ka1, va1, i);
+  }
+  auto step = [&](int t, f32x16 (&sc)[2], f32x16 (&dc)[2], f32x16 (&sn)[2], f32x16 (&dn)[2],
+                  auto more_c) {
+    constexpr bool MORE = decltype(more_c)::value;   // tile t + 1 exists
+    // key j of a tile that some row of the block does not see whole is kept iff j <= jlim and its end
+    // lies past this lane's token; the others' probabilities come out as 0.  Rows past the block have
+    // zero q, dO and delta, so their dS is zero whatever P is.
+    if (!full_tile(it, it.tb + t)) {
+      const int lim = jlim - (it.tb + t) * kBN - 4 * hl;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const i32x4 e4 = *reinterpret_cast<const i32x4*>(&ends[t % kBwdStages][8 * q + 4 * hl]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sc[q >> 2][4 * (q & 3) + e] =
+              (8 * q + e <= lim) & (m < e4[e]) ? sc[q >> 2][4 * (q & 3) + e] : -1.0e30f;
+      }
+    }
+    const unsigned nst = (unsigned)((t + 1) % kBwdStages) * kStageBytes;
+    const unsigned ka = fresh(krow + nst), va = fresh(vrow + nst);
+    const unsigned kc = fresh(kcol + (unsigned)(t % kBwdStages) * kStageBytes);
+    auto rd2 = [&](int i) { return lds_col8(kc, i & 3, 16 * (i >> 2) * kHD * 2); };
+    Frag8 dsf[kBN / 16];
+    f16x8 gr[kAhead2];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      if constexpr (MORE) {
+        product(sn, dn, fr[i % kAhead1], i);
+        if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(ka, va, i + kAhead1);
+      }
+      const int kb = i >> 4, v = i & 15;
+      const float p = ex2(__builtin_fmaf(sc[kb][v], a.qk_scale, -lse_m));
+      dc[kb][v] = __fmul_rn(p, __fsub_rn(dc[kb][v], dl_m));
+      if (i & 1) dsf[i >> 3].h[(i >> 1) & 3] = pinned(dc[kb][v - 1], dc[kb][v]);
+      if (i >= 32 - kAhead2) gr[i - (32 - kAhead2)] = rd2(i - (32 - kAhead2));
+      if constexpr (MORE) __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (MORE) {
+      tile_barrier();
+      issue(t + 3);
+    }
+    const unsigned nst2 = (unsigned)((t + 2) % kBwdStages) * kStageBytes;
+    const unsigned ka2 = fresh(krow + nst2), va2 = fresh(vrow + nst2);
+    // dQ^T += K^T dS^T
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      dqacc[i & 3] = mfma(gr[i % kAhead2], dsf[i >> 2].get(), dqacc[i & 3]);
+      if (i + kAhead2 < 16) gr[i % kAhead2] = rd2(i + kAhead2);
+      // (past the last tile: a stale stage, never used)
+      if (MORE && i >= 16 - kAhead1) fr[i - (16 - kAhead1)] = rd1(ka2, va2, i - (16 - kAhead1));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using More = std::integral_constant<bool, true>;
+  using Last = std::integral_constant<bool, false>;
+  int t = 0;
+  for (; t + 2 < n_tiles; t += 2) {
+    step(t, s_a, d_a, s_b, d_b, More{});
+    step(t + 1, s_b, d_b, s_a, d_a, More{});
+  }
+  if (t + 1 < n_tiles) {
+    step(t, s_a, d_a, s_b, d_b, More{});
+    ++t;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      s_a[kb] = s_b[kb];
+      d_a[kb] = d_b[kb];
+    }
+  }
+  step(t, s_a, d_a, s_b, d_b, Last{});
+  __syncthreads();
+  if (it.slot >= 0) {
+    float* part = parts + (int64_t)it.slot * kUnitFloats;
+#pragma unroll
+    for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        part[((w * (kHD / 32) + hb) * 16 + v) * 64 + lane] = dqacc[hb][v];
     return;
   }
-  i -= a.n_tokens * a.nkv;
-  if (i < a.n_tokens * a.nq) span_row_dq(a, i / a.nq, (int)(i % a.nq), dout, lse, delta, dq, s[w]);
+  // the wave's 32 x 128 block of dQ staged in the (now free) tile ring, then written back 16 bytes per
+  // lane, four whole 256-byte rows per store instruction
+  f16* stage = Ks + w * 32 * kStride16;
+  float chk = 0.0f;   // NaN if a value is not finite
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f16x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        chk = __builtin_fmaf(dqacc[hb][4 * q + e], 0.0f, chk);
+        o[e] = (f16)__fmul_rn(dqacc[hb][4 * q + e], a.sm_scale);
+      }
+      *reinterpret_cast<f16x4*>(stage + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = o;
+    }
+  if (chk != 0.0f) bad[row] = 1;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 4), cc = lane & 15;
+    const int srow = 32 * w + r, sr = it.phase + srow;
+    const f16x8 v = *reinterpret_cast<const f16x8*>(stage + r * kStride16 + 8 * cc);
+    if (srow < it.rows && !bad[srow])
+      *reinterpret_cast<f16x8*>(dq + (int64_t)(it.t0 + sr / gin) * OROW +
+                                (int64_t)(it.g * gin + sr % gin) * kHD + 8 * cc) = v;
+  }
+  redo_dq<4>(a, it.t0, it.phase, it.rows, it.g, bad, reinterpret_cast<RowScratch*>(Vs), dout, lse, delta, dq);
+}
+
+// dK and dV of a block of up to kBM keys, summed over the heads of the KV head's group: K and V stay in
+// registers while the walk goes over every head's query tiles, from the block's first key to the last
+// query that sees any of its keys.  The Q and dO tiles and the tiles' lse and delta rows (by dword DMA,
+// one lane per query, waves 0 and 1) come through the four-stage ring.
+__device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* items, int idx, int n_units,
+                                          const f16* __restrict__ dout, const float* __restrict__ lse,
+                                          const float* __restrict__ delta, f16* __restrict__ dk,
+                                          f16* __restrict__ dv, float* __restrict__ parts, f16* Qs,
+                                          f16* Ds, float (*lse_s)[kBN], float (*dl_s)[kBN], int* bad) {
+  const int32_t* p = items + (int64_t)idx * kItemInts;
+  auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(p[k]); };
+  const int k0 = u(0), nk = u(2), g = u(3), qend = u(4), tb = u(11), te = u(12), slot = u(13);
+  const int gin = a.nq / a.nkv;
+  if (k0 < 0 || nk < 1 || nk > kBM || g < 0 || g >= a.nkv || (int64_t)k0 + nk > a.n_tokens ||
+      qend <= k0 || qend > a.n_tokens || tb < 0 || tb >= te || (slot >= 0 && slot > n_units - 2))
+    return;
+  const int per_head = (qend - k0 + kBN - 1) / kBN;   // query tiles of a head's walk
+  if (te > (int64_t)gin * per_head) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, hl = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(w);
+  const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
+  const bool nval = 32 * w + c < nk;
+  const int n = k0 + (nval ? 32 * w + c : 0);   // this lane's key
+  const int end = (int)key_end(a, n);
+  // the first end among the wave's keys
+  int end_min = nval ? end : INT32_MAX;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) end_min = min(end_min, __shfl_xor(end_min, x));
+  end_min = __builtin_amdgcn_readfirstlane(end_min);
+
+  const int n_tiles = te - tb;
+  if (tid < kBN) lse_s[kBwdStages][tid] = 0.0f;
+  if (tid < kBM) bad[tid] = 0;
+  const TileSource qsrc = tile_source(a.qkv + (int64_t)k0 * ROW + (int64_t)g * gin * kHD, ROW, wave, lane);
+  const TileSource dsrc = tile_source(dout + (int64_t)k0 * OROW + (int64_t)g * gin * kHD, OROW, wave, lane);
+  // The walk: every head of the group in turn, each over the query tiles k0 + 64 i up to qend.  Tiles
+  // are issued in order: (head, tile of the head) of the next one.
+  int ihead = tb / per_head, itile = tb % per_head;
+  int walk = itile;   // and of the next step
+  auto issue = [&](int t) {
+    if (t >= n_tiles) return;
+    const int st = t % kBwdStages, m0 = k0 + itile * kBN;
+    tile_load(qsrc, (int64_t)itile * kBN, (uint64_t)ihead * kHD * 2, qend - 1 - m0, Qs + st * kTileHalves, wave);
+    tile_load(dsrc, (int64_t)itile * kBN, (uint64_t)ihead * kHD * 2, qend - 1 - m0, Ds + st * kTileHalves, wave);
+    if (wave < 2) {
+      const int qq = m0 + lane < qend ? m0 + lane : qend - 1;
+      const float* src = (wave == 0 ? lse : delta) + (int64_t)(g * gin + ihead) * a.n_tokens + qq;
+      dma4(src, __builtin_amdgcn_readfirstlane(lds_addr(wave == 0 ? lse_s[st] : dl_s[st])));
+    }
+    if (++itile == per_head) {
+      itile = 0;
+      ++ihead;
+    }
+  };
+  issue(0);
+  issue(1);
+  issue(2);
+
+  // this lane's key and value rows as B operands, loaded unconditionally and selected at once
+  // (the compiler's wait for them stands here, not in the loop)
+  f16x8 kf[kHD / 16], vf[kHD / 16];
+  {
+    const f16* krow = a.qkv + (int64_t)n * ROW + (int64_t)(a.nq + g) * kHD + 8 * hl;
+    const f16* vrow = krow + (int64_t)a.nkv * kHD;
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) {
+      kf[s] = *reinterpret_cast<const f16x8*>(krow + 16 * s);
+      vf[s] = *reinterpret_cast<const f16x8*>(vrow + 16 * s);
+    }
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) asm volatile("" : "+v"(kf[s]), "+v"(vf[s]));
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) {
+      kf[s] = nval ? kf[s] : zero8();
+      vf[s] = nval ? vf[s] : zero8();
+    }
+  }
+  f32x16 dkacc[kHD / 32], dvacc[kHD / 32];
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb) dkacc[hb] = dvacc[hb] = zero16();
+  const unsigned qrow = lds_addr(Qs) + row_base(lane), drow = lds_addr(Ds) + row_base(lane);
+  const unsigned qcol = lds_addr(Qs) + col_base(lane), dcol = lds_addr(Ds) + col_base(lane);
+  // operand i of a tile's products S = Q K^T and dP = dO V^T (queries qb * 32 + (row of the
+  // result), keys on the lanes): sub-step i / 4, dP for i / 2 odd, query half i % 2
+  auto rd1 = [&](unsigned qa, unsigned da, int i) {
+    return lds_read8((((i >> 1) & 1) ? da : qa) ^ (unsigned)(32 * (i >> 2)), (i & 1) * 32 * kHD * 2);
+  };
+  auto product = [&](f32x16 (&sacc)[2], f32x16 (&dpacc)[2], const f16x8& f, int i) {
+    const int s = i >> 2, qb = i & 1;
+    if ((i >> 1) & 1) dpacc[qb] = mfma(f, vf[s], s == 0 ? zero16() : dpacc[qb]);
+    else sacc[qb] = mfma(f, kf[s], s == 0 ? zero16() : sacc[qb]);
+  };
+  // the statistics of rows 8 g + 4 (l / 32) + 0..3 of the tile in stage st (g = 0..7)
+  auto stat = [&](const float (*tab)[kBN], int st, int g) {
+    return *reinterpret_cast<const f32x4*>(&tab[st][8 * g + 4 * hl]);
+  };
+  f16x8 fr[kAhead1];
+  f32x4 ls[2], dl[2];
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the row of zeros is written
+  tile_barrier();
+  f32x16 s_a[2], d_a[2], s_b[2], d_b[2];
+  {
+    const unsigned qa = fresh(qrow), da = fresh(drow);
+#pragma unroll
+    for (int i = 0; i < kAhead1; ++i) fr[i] = rd1(qa, da, i);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      product(s_a, d_a, fr[i % kAhead1], i);
+      if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(qa, da, i + kAhead1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const unsigned qa1 = fresh(qrow + kStageBytes), da1 = fresh(drow + kStageBytes);
+#pragma unroll
+    for (int i = 0; i < kAhead1; ++i) fr[i] = rd1(qa1, da1, i);
+    ls[0] = stat(lse_s, 0, 0);
+    dl[0] = stat(dl_s, 0, 0);
+  }
+  auto step = [&](int t, f32x16 (&sc)[2], f32x16 (&dc)[2], f32x16 (&sn)[2], f32x16 (&dn)[2],
+                  auto more_c) {
+    constexpr bool MORE = decltype(more_c)::value;   // tile t + 1 exists
+    const int st = t % kBwdStages, m0 = k0 + walk * kBN;
+    walk = walk + 1 == per_head ? 0 : walk + 1;
+    // Keys past the block only reach rows that are not stored; queries before a key or at its end and
+    // past it are masked only on the tiles that hold such a query for this wave (a wave-uniform
+    // test): query m0 + off + 4 (l / 32) is kept iff lo <= off < hi.  There the exponent is formed before
+    // the selection and the loop below is given scale 1 and a row of zeros for lse, so that the others'
+    // probabilities are 0 whatever their lse is.
+    float scale = a.qk_scale;
+    int lrow = st;
+    if (m0 < k0 + 32 * wave + 31 || m0 + kBN > end_min) {
+      const int lo = n - m0 - 4 * hl, hi = end - m0 - 4 * hl;
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const f32x4 l = g == 0 ? ls[0] : stat(lse_s, st, g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int off = 8 * g + e;
+          const float x = __builtin_fmaf(sc[g >> 2][4 * (g & 3) + e], a.qk_scale, -l[e]);
+          sc[g >> 2][4 * (g & 3) + e] = ((off >= lo) & (off < hi)) ? x : -1.0e30f;
+        }
+      }
+      scale = 1.0f;
+      lrow = kBwdStages;
+      ls[0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const unsigned nst = (unsigned)((t + 1) % kBwdStages) * kStageBytes;
+    const unsigned qa = fresh(qrow + nst), da = fresh(drow + nst);
+    const unsigned qc = fresh(qcol + (unsigned)st * kStageBytes), dc_ = fresh(dcol + (unsigned)st * kStageBytes);
+    auto rd2 = [&](int i) { return lds_col8((i & 1) ? qc : dc_, (i >> 1) & 3, 16 * (i >> 3) * kHD * 2); };
+    Frag8 pf[kBN / 16], dsf[kBN / 16];
+    f16x8 gr[kAhead2];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      if constexpr (MORE) {
+        product(sn, dn, fr[i % kAhead1], i);
+        if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(qa, da, i + kAhead1);
+      }
+      const int qb = i >> 4, v = i & 15, g = i >> 2;
+      if ((i & 3) == 0 && g + 1 < 8) {
+        ls[(g + 1) & 1] = stat(lse_s, lrow, g + 1);
+        dl[(g + 1) & 1] = stat(dl_s, st, g + 1);
+      }
+      sc[qb][v] = ex2(__builtin_fmaf(sc[qb][v], scale, -ls[g & 1][i & 3]));
+      dc[qb][v] = __fmul_rn(sc[qb][v], __fsub_rn(dc[qb][v], dl[g & 1][i & 3]));
+      if (i & 1) {
+        pf[i >> 3].h[(i >> 1) & 3] = pinned(sc[qb][v - 1], sc[qb][v]);
+        dsf[i >> 3].h[(i >> 1) & 3] = pinned(dc[qb][v - 1], dc[qb][v]);
+      }
+      if (i >= 32 - kAhead2) gr[i - (32 - kAhead2)] = rd2(i - (32 - kAhead2));
+      if constexpr (MORE) __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (MORE) {
+      tile_barrier();
+      issue(t + 3);
+    }
+    const unsigned nst2 = (unsigned)((t + 2) % kBwdStages) * kStageBytes;
+    const unsigned qa2 = fresh(qrow + nst2), da2 = fresh(drow + nst2);
+    // dV += P^T dO, dK += dS^T Q over the tile's 64 queries, 16 per step
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int hb = (i >> 1) & 3;
+      if (i & 1) dkacc[hb] = mfma(dsf[i >> 3].get(), gr[i % kAhead2], dkacc[hb]);
+      else dvacc[hb] = mfma(pf[i >> 3].get(), gr[i % kAhead2], dvacc[hb]);
+      if (i + kAhead2 < 32) gr[i % kAhead2] = rd2(i + kAhead2);
+      if constexpr (MORE) {
+        // (past the last tile: a stale stage, never used)
+        if (i >= 32 - kAhead1) fr[i - (32 - kAhead1)] = rd1(qa2, da2, i - (32 - kAhead1));
+        if (i == 28) ls[0] = stat(lse_s, (t + 1) % kBwdStages, 0);
+        if (i == 29) dl[0] = stat(dl_s, (t + 1) % kBwdStages, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using More = std::integral_constant<bool, true>;
+  using Last = std::integral_constant<bool, false>;
+  int t = 0;
+  for (; t + 2 < n_tiles; t += 2) {
+    step(t, s_a, d_a, s_b, d_b, More{});
+    step(t + 1, s_b, d_b, s_a, d_a, More{});
+  }
+  if (t + 1 < n_tiles) {
+    step(t, s_a, d_a, s_b, d_b, More{});
+    ++t;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      s_a[qb] = s_b[qb];
+      d_a[qb] = d_b[qb];
+    }
+  }
+  step(t, s_a, d_a, s_b, d_b, Last{});
+  __syncthreads();
+  if (slot >= 0) {
+    float* part = parts + (int64_t)slot * kUnitFloats;
+#pragma unroll
+    for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int o = ((w * (kHD / 32) + hb) * 16 + v) * 64 + lane;
+        part[o] = dkacc[hb][v];
+        part[kUnitFloats + o] = dvacc[hb][v];
+      }
+    return;
+  }
+  store_dkdv(a, k0, nk, g, dkacc, dvacc, Qs, Ds, bad, dk, dv);
+  redo_dkdv<4>(a, k0, nk, g, bad, reinterpret_cast<RowScratch*>(Qs), dout, lse, delta, dk, dv);
+}
+
+// Every item of the backward in one launch, longest walks first (the plan's order): dK/dV walks and
+// dQ walks share the CUs, one workgroup each.
+__global__ __launch_bounds__(kAThreads) void span_bwd_kernel(
+    SpanArgs a, const int32_t* __restrict__ items, int n_units, const f16* __restrict__ dout,
+    const float* __restrict__ lse, const float* __restrict__ delta, f16* __restrict__ dq,
+    f16* __restrict__ dk, f16* __restrict__ dv, float* __restrict__ parts) {
+  static_assert(kBwdStages == kFwdStages, "dK/dV and dQ share the tile ring");
+  __shared__ __attribute__((aligned(1024))) f16 T0[kBwdStages * kTileHalves];
+  __shared__ __attribute__((aligned(1024))) f16 T1[kBwdStages * kTileHalves];
+  __shared__ __attribute__((aligned(16))) float lse_s[kBwdStages + 1][kBN], dl_s[kBwdStages][kBN];
+  __shared__ int bad[kBM];
+  const int idx = (int)blockIdx.x;
+  if (__builtin_amdgcn_readfirstlane(items[(int64_t)idx * kItemInts + 14]))
+    dkdv_item(a, items, idx, n_units, dout, lse, delta, dk, dv, parts, T0, T1, lse_s, dl_s, bad);
+  else
+    dq_item(a, items, idx, n_units, dout, lse, delta, dq, parts, T0, T1,
+            reinterpret_cast<int (*)[kBN]>(lse_s), bad);
+}
+
+// The partials of a split walk summed in slot order.  Wave w holds rows (or keys) 32 w .. + 31 as the
+// walks left them.
+__global__ __launch_bounds__(kAThreads) void span_bwd_join_kernel(
+    SpanArgs a, const int32_t* __restrict__ joins, int n_units, const f16* __restrict__ dout,
+    const float* __restrict__ lse, const float* __restrict__ delta, f16* __restrict__ dq,
+    f16* __restrict__ dk, f16* __restrict__ dv, const float* __restrict__ parts) {
+  const int32_t* j = joins + (int64_t)blockIdx.x * DK_ATTN_SPAN_JOIN_INTS;
+  auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(j[k]); };
+  const int t0 = u(0), phase = u(1), rows = u(2), g = u(3), s0 = u(4), cnt = u(5), keys = u(6);
+  const int gin = a.nq / a.nkv, step = keys ? 2 : 1;
+  if (t0 < 0 || phase < 0 || phase >= gin || rows < 1 || rows > kBM || g < 0 || g >= a.nkv ||
+      (int64_t)t0 + (keys ? rows - 1 : (phase + rows - 1) / gin) >= a.n_tokens || s0 < 0 || cnt < 1 ||
+      (int64_t)s0 + (int64_t)cnt * step > n_units)
+    return;
+  __shared__ __attribute__((aligned(16))) f16 S0[kBM * kStride16], S1[kBM * kStride16];
+  __shared__ int bad[kBM];
+  if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hl = lane >> 5, c = lane & 31;
+  f32x16 x[kHD / 32], y[kHD / 32];
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb) x[hb] = y[hb] = zero16();
+  for (int s = 0; s < cnt; ++s) {
+    const float* p = parts + ((int64_t)s0 + (int64_t)s * step) * kUnitFloats + w * (kHD / 32) * 16 * 64 + lane;
+#pragma unroll
+    for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        x[hb][v] = __fadd_rn(x[hb][v], p[(hb * 16 + v) * 64]);
+        if (keys) y[hb][v] = __fadd_rn(y[hb][v], p[kUnitFloats + (hb * 16 + v) * 64]);
+      }
+  }
+  if (keys) {
+    store_dkdv(a, t0, rows, g, x, y, S0, S1, bad, dk, dv);
+    redo_dkdv<4>(a, t0, rows, g, bad, reinterpret_cast<RowScratch*>(S0), dout, lse, delta, dk, dv);
+    return;
+  }
+  const int row = 32 * w + c, rr = phase + row;
+  float chk = 0.0f;
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) chk = __builtin_fmaf(x[hb][v], 0.0f, chk);
+  if (chk != 0.0f) bad[row] = 1;
+  __syncthreads();
+  if (row < rows && !bad[row]) {
+    f16* o = dq + ((int64_t)t0 + rr / gin) * a.nq * kHD + (int64_t)(g * gin + rr % gin) * kHD + 4 * hl;
+#pragma unroll
+    for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f16x4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = (f16)__fmul_rn(x[hb][4 * q + e], a.sm_scale);
+        *reinterpret_cast<f16x4*>(o + hb * 32 + 8 * q) = r;
+      }
+  }
+  redo_dq<4>(a, t0, phase, rows, g, bad, reinterpret_cast<RowScratch*>(S0), dout, lse, delta, dq);
 }
 
 }  // namespace
 
+extern "C" int64_t dk_attn_span_bwd_workspace(int64_t n_units) {
+  return n_units > 0 ? n_units * (int64_t)(kUnitFloats * sizeof(float)) : 0;
+}
+
 extern "C" int dk_attn_span_bwd(const void* qkv, const void* out, const float* lse, const void* dout,
-                                const int32_t* spans, int64_t n_tokens, int32_t nq, int32_t nkv,
-                                int32_t hd, float* delta, void* dq, void* dk, void* dv,
-                                hipStream_t stream) {
+                                const int32_t* spans, const int32_t* items, int32_t n_items,
+                                const int32_t* joins, int32_t n_joins, int32_t n_units,
+                                int64_t n_tokens, int32_t nq, int32_t nkv, int32_t hd, float* delta,
+                                void* dq, void* dk, void* dv, void* workspace,
+                                int64_t workspace_bytes, hipStream_t stream) {
   SpanArgs a;
   if (int e = span_args(a, qkv, spans, n_tokens, nq, nkv, hd)) return e;
-  if (n_tokens == 0) return 0;
-  if (!out || !lse || !dout || !delta || !dq || !dk || !dv) return DK_ERR_INVALID;
+  if (n_items < 0 || n_joins < 0 || n_units < 0) return DK_ERR_INVALID;
+  if (n_tokens == 0 || n_items == 0) return 0;
+  if (!out || !lse || !dout || !items || (n_joins > 0 && !joins) || !delta || !dq || !dk || !dv)
+    return DK_ERR_INVALID;
   if (!dk_aligned(out, 16) || !dk_aligned(dout, 16) || !dk_aligned(lse, 4) || !dk_aligned(delta, 4) ||
-      !dk_aligned(dq, 16) || !dk_aligned(dk, 16) || !dk_aligned(dv, 16))
+      !dk_aligned(dq, 16) || !dk_aligned(dk, 16) || !dk_aligned(dv, 16) || !dk_aligned(items, 4) ||
+      !dk_aligned(joins, 4) || !dk_aligned(workspace, 256))
     return DK_ERR_ALIGN;
-  const int64_t pairs = n_tokens * nq, wgs = (pairs + n_tokens * nkv + 3) / 4;
-  if (wgs > INT32_MAX / kAThreads) return DK_ERR_INVALID;
-  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((pairs + 15) / 16)), dim3(kAThreads), 0,
-                     stream, (const f16*)out, (const f16*)dout, delta, n_tokens, nq);
+  if (n_units > 0 && (!workspace || workspace_bytes < dk_attn_span_bwd_workspace(n_units)))
+    return DK_ERR_WORKSPACE;
+  const int64_t pairs = n_tokens * nq, wgs = (pairs + 15) / 16;
+  if (n_items > INT32_MAX / kAThreads || n_joins > INT32_MAX / kAThreads || wgs > INT32_MAX / kAThreads)
+    return DK_ERR_INVALID;
+  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)wgs), dim3(kAThreads), 0, stream,
+                     (const f16*)out, (const f16*)dout, delta, n_tokens, nq);
   DK_CHECK_LAUNCH();
-  hipLaunchKernelGGL(span_bwd_rows_kernel, dim3((unsigned)wgs), dim3(kAThreads), 0, stream, a,
-                     (const f16*)dout, lse, delta, (f16*)dq, (f16*)dk, (f16*)dv);
+  hipLaunchKernelGGL(span_bwd_kernel, dim3((unsigned)n_items), dim3(kAThreads), 0, stream, a, items,
+                     n_units, (const f16*)dout, lse, delta, (f16*)dq, (f16*)dk, (f16*)dv,
+                     (float*)workspace);
   DK_CHECK_LAUNCH();
+  if (n_joins > 0) {
+    hipLaunchKernelGGL(span_bwd_join_kernel, dim3((unsigned)n_joins), dim3(kAThreads), 0, stream, a,
+                       joins, n_units, (const f16*)dout, lse, delta, (f16*)dq, (f16*)dk, (f16*)dv,
+                       (const float*)workspace);
+    DK_CHECK_LAUNCH();
+  }
   return 0;
 }

@@ -118,7 +118,6 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
     if constexpr (MASK) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        typedef int i32x4 __attribute__((ext_vector_type(4)));
         const i32x4 e4 = *reinterpret_cast<const i32x4*>(&ends[t % kFwdStages][8 * q + 4 * hl]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

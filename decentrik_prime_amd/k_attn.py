@@ -147,25 +147,31 @@ class SpanMeta:
     answer's go on from its prompt's), for the rotary embedding.  A plan serves any number of
     calls, on any streams of its device, captured or not."""
 
-    def __init__(self, runs, spans, positions, nq, nkv, device):
+    def __init__(self, runs, key_runs, spans, positions, nq, nkv, device):
         if nq < 1 or nkv < 1 or nq % nkv:
             raise ValueError(f"nq must be a multiple of nkv (got {nq}, {nkv})")
         if spans.shape[0] > MAX_SPAN_TOKENS:
             raise ValueError(f"at most {MAX_SPAN_TOKENS} tokens (got {spans.shape[0]})")
         self.n_tokens, self.nq, self.nkv = int(spans.shape[0]), int(nq), int(nkv)
         blocks = _query_blocks(runs, spans, nq // nkv, nkv)
-        items, joins, self.n_slots = _split_items(blocks, _fwd_tiles(blocks))
+        items, joins, self.n_slots = _split_items(blocks, blocks[:, _TE], _fwd_tiles(blocks))
+        blocks = np.concatenate([_key_blocks(key_runs, spans, nq // nkv, nkv), blocks])
+        # a tile of a dK/dV walk takes 64 MFMAs a wave, one of a dQ walk 48
+        cost = blocks[:, _TE] * (3 + blocks[:, _KIND])
+        items_b, joins_b, self.n_units = _split_items(blocks, cost, _bwd_cost(cost))
         i32 = dict(dtype=torch.int32, device=device)
         self.spans = torch.tensor(spans, **i32)
         self.positions = torch.tensor(positions, **i32)
         self.items, self.joins = torch.tensor(items, **i32), torch.tensor(joins, **i32)
+        self.items_bwd, self.joins_bwd = torch.tensor(items_b, **i32), torch.tensor(joins_b, **i32)
 
 
 MAX_SPAN_TOKENS = 1 << 30
 _KEYS = 64            # keys of a tile
 _ROWS = 128           # stacked query rows of a block
 # columns of an item (include/dk.h)
-_T0, _PHASE, _N_ROWS, _G, _A0, _NA, _B0, _NK, _F0, _F1, _F2, _TB, _TE, _SLOT = range(14)
+_T0, _PHASE, _N_ROWS, _G, _A0, _NA, _B0, _NK, _F0, _F1, _F2, _TB, _TE, _SLOT, _KIND = range(15)
+_QEND = 4             # of a block of keys
 
 
 def _query_blocks(runs, spans, gin, nkv):
@@ -196,29 +202,51 @@ def _query_blocks(runs, spans, gin, nkv):
     return np.concatenate(parts) if parts else np.empty((0, 16), np.int64)
 
 
+def _key_blocks(key_runs, spans, gin, nkv):
+    """The blocks of keys of every run (with kend that does not fall) and KV head, as items whose walk
+    over the group's heads and their queries is whole."""
+    parts = []
+    for r0, r1 in key_runs:
+        k0 = np.arange(r0, r1, _ROWS, dtype=np.int64)
+        nk = np.minimum(_ROWS, r1 - k0)
+        x = np.zeros((k0.size, 16), np.int64)
+        x[:, _T0], x[:, _N_ROWS], x[:, _KIND], x[:, _SLOT] = k0, nk, 1, -1
+        x[:, _QEND] = spans[k0 + nk - 1, 3]
+        x[:, _TE] = gin * -(-(x[:, _QEND] - k0) // _KEYS)
+        parts += [x + np.eye(1, 16, _G, dtype=np.int64) * g for g in range(nkv)]
+    return np.concatenate(parts) if parts else np.empty((0, 16), np.int64)
+
+
 def _fwd_tiles(blocks):
-    """Tiles per item of the forward."""
+    """Tiles per item of the forward at most."""
     return 1 << 30
 
 
-def _split_items(blocks, most):
-    """(items, joins, partials): blocks of more than `most` tiles cut into walks of as many tiles each,
-    longest walks first."""
+def _bwd_cost(cost):
+    """Cost per item of the backward at most."""
+    return 1 << 30
+
+
+def _split_items(blocks, cost, most):
+    """(items, joins, partials): blocks that cost more than `most` cut into walks of as many tiles each,
+    the costliest walks first."""
     n = blocks[:, _TE]
-    cut = -(-n // most)
+    cut = np.minimum(n, -(-cost // most))
     idx = np.repeat(np.arange(n.size), cut)
     part = np.arange(idx.size) - np.repeat(np.cumsum(cut) - cut, cut)
     items = blocks[idx].copy()
     items[:, _TB] = part * n[idx] // cut[idx]
     items[:, _TE] = (part + 1) * n[idx] // cut[idx]
     split = cut > 1
-    first = np.cumsum(np.where(split, cut, 0)) - np.where(split, cut, 0)
-    items[:, _SLOT] = np.where(split[idx], first[idx] + part, -1)
+    size = 1 + blocks[:, _KIND]           # units of a partial: dK and dV take two
+    units = np.where(split, cut * size, 0)
+    first = np.cumsum(units) - units
+    items[:, _SLOT] = np.where(split[idx], first[idx] + part * size[idx], -1)
     joins = np.zeros((int(split.sum()), 8), np.int64)
     joins[:, :4] = blocks[split][:, [_T0, _PHASE, _N_ROWS, _G]]
-    joins[:, 4], joins[:, 5] = first[split], cut[split]
-    order = np.argsort(items[:, _TB] - items[:, _TE], kind="stable")
-    return items[order], joins, int(cut[split].sum())
+    joins[:, 4], joins[:, 5], joins[:, 6] = first[split], cut[split], blocks[split][:, _KIND]
+    order = np.argsort(-cost[idx] // cut[idx], kind="stable")
+    return items[order], joins, int(units.sum())
 
 
 def _lengths(lens, what):
@@ -246,7 +274,8 @@ def window_meta(lens, window, sinks, nq, nkv, device):
     spans[:, 2] = np.maximum(s0, m - (window - 1))
     spans[:, 3] = np.where(m - s0 < sinks, end, np.minimum(m + window, end))
     runs = [(int(a), int(a + n)) for a, n in zip(start, size) if n]
-    return SpanMeta(runs, spans, m - s0, nq, nkv, device)
+    key_runs = [r for a, b in runs for r in ((a, min(a + sinks, b)), (a + sinks, b)) if r[1] > r[0]]
+    return SpanMeta(runs, key_runs, spans, m - s0, nq, nkv, device)
 
 
 def prefix_meta(groups, nq, nkv, device):
@@ -272,7 +301,7 @@ def prefix_meta(groups, nq, nkv, device):
         g0 = end
     spans = np.concatenate(spans) if spans else np.empty((0, 4), np.int64)
     positions = np.concatenate(positions) if positions else np.empty(0, np.int64)
-    return SpanMeta(runs, spans, positions, nq, nkv, device)
+    return SpanMeta(runs, runs, spans, positions, nq, nkv, device)
 
 
 def _check_span(qkv, meta, nq, nkv, hd):
@@ -319,11 +348,15 @@ def span_attention_backward(qkv, out, lse, dout, meta, nq, nkv, hd):
     dq = torch.empty((n, nq * hd), dtype=torch.float16, device=dev)
     dk = torch.empty((n, nkv * hd), dtype=torch.float16, device=dev)
     dv = torch.empty((n, nkv * hd), dtype=torch.float16, device=dev)
+    nbytes = _lib.lib().dk_attn_span_bwd_workspace(meta.n_units)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with torch.cuda.device(dev):
         rc = _lib.lib().dk_attn_span_bwd(_lib.ptr(qkv), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(dout),
-                                         _lib.ptr(meta.spans), n, nq, nkv, hd, _lib.ptr(delta),
-                                         _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
-                                         _lib.stream_handle(dev))
+                                         _lib.ptr(meta.spans), _lib.ptr(meta.items_bwd),
+                                         meta.items_bwd.shape[0], _lib.ptr(meta.joins_bwd),
+                                         meta.joins_bwd.shape[0], meta.n_units, n, nq, nkv, hd,
+                                         _lib.ptr(delta), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
+                                         _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
     _lib.check(rc, "dk_attn_span_bwd")
     return dq, dk, dv
 

@@ -189,9 +189,18 @@ int dk_attn_span_fwd(const void* qkv, const int32_t* spans, const int32_t* items
                      const int32_t* joins, int32_t n_joins, int32_t n_slots, int64_t n_tokens,
                      int32_t nq, int32_t nkv, int32_t hd, void* out, float* lse, void* workspace,
                      int64_t workspace_bytes, hipStream_t stream);
+/* The backward's items: a block of query rows as above whose tiles are walked for dq (slot s: partial s
+ * of the workspace, a unit), or with item[14] = 1 the keys k0 .. k0 + nk - 1 of KV head g for dk and dv:
+ * k0, 0, nk, g, qend, 0, 0, 0, 0, 0, 0, tb, te, slot, 1, 0.  Its walk goes over the group's gin heads,
+ * each over the query tiles k0 + 64 i of [k0, qend), numbered through (slot s: units s and s + 1).
+ * joins: t0 or k0, phase, rows or nk, g, first unit, partials, 1 for keys, 0.  The workspace holds
+ * n_units units (dk_attn_span_bwd_workspace bytes, 256-byte aligned). */
+int64_t dk_attn_span_bwd_workspace(int64_t n_units);
 int dk_attn_span_bwd(const void* qkv, const void* out, const float* lse, const void* dout,
-                     const int32_t* spans, int64_t n_tokens, int32_t nq, int32_t nkv, int32_t hd,
-                     float* delta, void* dq, void* dk, void* dv, hipStream_t stream);
+                     const int32_t* spans, const int32_t* items, int32_t n_items,
+                     const int32_t* joins, int32_t n_joins, int32_t n_units, int64_t n_tokens,
+                     int32_t nq, int32_t nkv, int32_t hd, float* delta, void* dq, void* dk, void* dv,
+                     void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * LM head over vocabulary chunks (the consumer of the final norm): the row kernels between the

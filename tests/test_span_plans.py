@@ -129,12 +129,44 @@ def test_split_items_cover_the_walks():
     meta = k_attn.window_meta([700, 20], 400, 4, 12, 2, "cpu")
     blocks = k_attn._query_blocks([(0, 700), (700, 720)], np.asarray(meta.spans, np.int64), 6, 2)
     for most in (1, 2, 3, 100):
-        items, joins, slots = k_attn._split_items(blocks, most)
+        items, joins, slots = k_attn._split_items(blocks, blocks[:, 12], most)
         assert (items[:, 12] - items[:, 11]).max() <= most and (items[:, 12] > items[:, 11]).all()
         assert sorted(x for x in items[:, 13] if x >= 0) == list(range(slots))
-        for t0, phase, rows, g, first, cnt, _, _ in joins:
+        for t0, phase, rows, g, first, cnt, keys, _ in joins:
+            assert keys == 0
             own = items[(items[:, 13] >= first) & (items[:, 13] < first + cnt)]
             own = own[np.argsort(own[:, 13])]
             assert len(own) == cnt > 1 and (own[:, [0, 1, 2, 3]] == [t0, phase, rows, g]).all()
             assert own[0, 11] == 0 and (own[1:, 11] == own[:-1, 12]).all()
             assert own[-1, 12] == -(-own[-1, 7] // 64)
+
+
+@pytest.mark.parametrize("nq,nkv", [(4, 2), (3, 1)])
+def test_key_items_visit_every_visible_pair_once(nq, nkv):
+    gin = nq // nkv
+    for make, spec in ([(attn.window_visible, w) for w in WINDOWS + [([300, 41], 100, 3), ([260], 30, 90)]] +
+                       [(attn.prefix_visible, (g,)) for g in GROUPS + [[(200, [40, 3, 70]), (9, [150])]]]):
+        build = k_attn.window_meta if make is attn.window_visible else k_attn.prefix_meta
+        meta = build(*spec, nq, nkv, "cpu")
+        s = np.asarray(meta.spans, np.int64)
+        count = np.zeros((nq, meta.n_tokens, meta.n_tokens), np.int64)
+        units, rows = set(), np.zeros((nq, meta.n_tokens), np.int64)
+        for it in np.asarray(meta.items_bwd, np.int64):
+            t0, phase, n, g, qend = it[:5]
+            tb, te, slot, kind = it[11:15]
+            if slot >= 0:
+                assert not units & set(range(slot, slot + 1 + kind))
+                units |= set(range(slot, slot + 1 + kind))
+            if not kind:
+                for i in range(n if tb == 0 else 0):
+                    rows[g * gin + (phase + i) % gin, t0 + (phase + i) // gin] += 1
+                continue
+            per_head = -(-(qend - t0) // 64)
+            assert 0 <= tb < te <= gin * per_head
+            for t in range(tb, te):
+                q0 = t0 + 64 * (t % per_head)
+                q = np.arange(q0, min(q0 + 64, qend))[:, None]
+                k = np.arange(t0, t0 + n)[None]
+                count[g * gin + t // per_head, q, k] += (q >= k) & (q < s[k, 3])
+        assert (rows == 1).all() and len(units) == meta.n_units
+        assert (count == make(*spec)[None]).all()
