@@ -8,6 +8,14 @@ namespace {
 constexpr int kUnitFloats = kBM * kHD;   // a partial of dQ; dK and dV take two
 constexpr int kStride16 = kHD + 8;       // halves per staged row of a result
 
+// Where quad q of result block hb of wave w's rows stands in a partial: 16 bytes per lane, lane-major.
+__device__ __forceinline__ int part_off(int w, int hb, int q, int lane) {
+  return ((w * (kHD / 32) + hb) * 4 + q) * 256 + 4 * lane;
+}
+__device__ __forceinline__ f32x4 quad(const f32x16& x, int q) {
+  return f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+}
+
 // The tile ring of both backward kernels: a tile of two operands (kBN rows each) in one of four
 // LDS stages, filled by LDS DMA.  Wave w's instruction i fills chunks (4 i + w) 64 + lane of an
 // operand: row 16 i + 4 w + lane / 16, with a wave-uniform base per tile and a 32-bit offset per
@@ -74,7 +82,6 @@ __device__ __forceinline__ void redo_dkdv(const SpanArgs& a, int k0, int nk, int
                                           RowScratch* s, const f16* dout, const float* lse,
                                           const float* delta, f16* dk, f16* dv) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  __syncthreads();   // the staged rows have been read
   for (int i = wave; i < nk; i += W) {
     if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
     span_key_dkdv(a, (int64_t)k0 + i, g, dout, lse, delta, dk, dv, s[wave]);
@@ -282,8 +289,8 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
 #pragma unroll
     for (int hb = 0; hb < kHD / 32; ++hb)
 #pragma unroll
-      for (int v = 0; v < 16; ++v)
-        part[((w * (kHD / 32) + hb) * 16 + v) * 64 + lane] = dqacc[hb][v];
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(part + part_off(w, hb, q, lane)) = quad(dqacc[hb], q);
     return;
   }
   // the wave's 32 x 128 block of dQ staged in the (now free) tile ring, then written back 16 bytes per
@@ -533,14 +540,15 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
 #pragma unroll
     for (int hb = 0; hb < kHD / 32; ++hb)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int o = ((w * (kHD / 32) + hb) * 16 + v) * 64 + lane;
-        part[o] = dkacc[hb][v];
-        part[kUnitFloats + o] = dvacc[hb][v];
+      for (int q = 0; q < 4; ++q) {
+        const int o = part_off(w, hb, q, lane);
+        *reinterpret_cast<f32x4*>(part + o) = quad(dkacc[hb], q);
+        *reinterpret_cast<f32x4*>(part + kUnitFloats + o) = quad(dvacc[hb], q);
       }
     return;
   }
   store_dkdv(a, k0, nk, g, dkacc, dvacc, Qs, Ds, bad, dk, dv);
+  __syncthreads();   // the staged rows have been read
   redo_dkdv<4>(a, k0, nk, g, bad, reinterpret_cast<RowScratch*>(Qs), dout, lse, delta, dk, dv);
 }
 
@@ -563,64 +571,107 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_kernel(
             reinterpret_cast<int (*)[kBN]>(lse_s), bad);
 }
 
-// The partials of a split walk summed in slot order.  Wave w holds rows (or keys) 32 w .. + 31 as the
-// walks left them.
+// The partials of a split walk summed in slot order: a workgroup per 32 rows (or keys) of a block, a
+// wave per 32 columns, four partials' loads in flight.
 __global__ __launch_bounds__(kAThreads) void span_bwd_join_kernel(
     SpanArgs a, const int32_t* __restrict__ joins, int n_units, const f16* __restrict__ dout,
     const float* __restrict__ lse, const float* __restrict__ delta, f16* __restrict__ dq,
     f16* __restrict__ dk, f16* __restrict__ dv, const float* __restrict__ parts) {
-  const int32_t* j = joins + (int64_t)blockIdx.x * DK_ATTN_SPAN_JOIN_INTS;
+  const int32_t* j = joins + (int64_t)(blockIdx.x >> 2) * DK_ATTN_SPAN_JOIN_INTS;
+  const int w = blockIdx.x & 3;   // the row group
   auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(j[k]); };
-  const int t0 = u(0), phase = u(1), rows = u(2), g = u(3), s0 = u(4), cnt = u(5), keys = u(6);
+  int t0 = u(0), phase = u(1), rows = u(2);
+  const int g = u(3), s0 = u(4), cnt = u(5), keys = u(6);
   const int gin = a.nq / a.nkv, step = keys ? 2 : 1;
   if (t0 < 0 || phase < 0 || phase >= gin || rows < 1 || rows > kBM || g < 0 || g >= a.nkv ||
       (int64_t)t0 + (keys ? rows - 1 : (phase + rows - 1) / gin) >= a.n_tokens || s0 < 0 || cnt < 1 ||
-      (int64_t)s0 + (int64_t)cnt * step > n_units)
+      (int64_t)s0 + (int64_t)cnt * step > n_units || rows <= 32 * w)
     return;
-  __shared__ __attribute__((aligned(16))) f16 S0[kBM * kStride16], S1[kBM * kStride16];
-  __shared__ int bad[kBM];
-  if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
-  __syncthreads();
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hl = lane >> 5, c = lane & 31;
-  f32x16 x[kHD / 32], y[kHD / 32];
-#pragma unroll
-  for (int hb = 0; hb < kHD / 32; ++hb) x[hb] = y[hb] = zero16();
-  for (int s = 0; s < cnt; ++s) {
-    const float* p = parts + ((int64_t)s0 + (int64_t)s * step) * kUnitFloats + w * (kHD / 32) * 16 * 64 + lane;
-#pragma unroll
-    for (int hb = 0; hb < kHD / 32; ++hb)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        x[hb][v] = __fadd_rn(x[hb][v], p[(hb * 16 + v) * 64]);
-        if (keys) y[hb][v] = __fadd_rn(y[hb][v], p[kUnitFloats + (hb * 16 + v) * 64]);
-      }
-  }
+  // the group's own rows
+  rows = rows - 32 * w < 32 ? rows - 32 * w : 32;
   if (keys) {
-    store_dkdv(a, t0, rows, g, x, y, S0, S1, bad, dk, dv);
-    redo_dkdv<4>(a, t0, rows, g, bad, reinterpret_cast<RowScratch*>(S0), dout, lse, delta, dk, dv);
-    return;
+    t0 += 32 * w;
+  } else {
+    t0 += (phase + 32 * w) / gin;
+    phase = (phase + 32 * w) % gin;
   }
-  const int row = 32 * w + c, rr = phase + row;
-  float chk = 0.0f;
-#pragma unroll
-  for (int hb = 0; hb < kHD / 32; ++hb)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) chk = __builtin_fmaf(x[hb][v], 0.0f, chk);
-  if (chk != 0.0f) bad[row] = 1;
+  __shared__ __attribute__((aligned(16))) f16 S0[32 * kStride16], S1[32 * kStride16];
+  __shared__ RowScratch scratch[kAThreads / 64];
+  __shared__ int bad[32];
+  if (threadIdx.x < 32) bad[threadIdx.x] = 0;
   __syncthreads();
-  if (row < rows && !bad[row]) {
-    f16* o = dq + ((int64_t)t0 + rr / gin) * a.nq * kHD + (int64_t)(g * gin + rr % gin) * kHD + 4 * hl;
+  const int lane = threadIdx.x & 63, hb = threadIdx.x >> 6, hl = lane >> 5, c = lane & 31;
+  f32x4 x[4], y[4];
 #pragma unroll
-    for (int hb = 0; hb < kHD / 32; ++hb)
+  for (int q = 0; q < 4; ++q) x[q] = y[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const float* p = parts + (int64_t)s0 * kUnitFloats + part_off(w, hb, 0, lane);
+  auto sum = [&](f32x4 (&acc)[4], const float* base) {
+    int s = 0;
+    for (; s + 4 <= cnt; s += 4) {
+      f32x4 t[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          t[i][q] = *reinterpret_cast<const f32x4*>(base + (int64_t)(s + i) * step * kUnitFloats + 256 * q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[q][e] = __fadd_rn(acc[q][e], t[i][q][e]);
+    }
+    for (; s < cnt; ++s)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        f16x4 r;
+        const f32x4 t = *reinterpret_cast<const f32x4*>(base + (int64_t)s * step * kUnitFloats + 256 * q);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = (f16)__fmul_rn(x[hb][4 * q + e], a.sm_scale);
-        *reinterpret_cast<f16x4*>(o + hb * 32 + 8 * q) = r;
+        for (int e = 0; e < 4; ++e) acc[q][e] = __fadd_rn(acc[q][e], t[e]);
       }
+  };
+  sum(x, p);
+  if (keys) sum(y, p + kUnitFloats);
+  // staged as rows of 128: dq's lane holds 16 columns of its row, dK's and dV's a column of 16 keys
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (!keys) {
+      f16x4 o;
+      float chk = 0.0f;   // NaN if a value is not finite
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        chk = __builtin_fmaf(x[q][e], 0.0f, chk);
+        o[e] = (f16)__fmul_rn(x[q][e], a.sm_scale);
+      }
+      if (chk != 0.0f) bad[c] = 1;
+      *reinterpret_cast<f16x4*>(S0 + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 8 * q + 4 * hl + e;
+        if (__builtin_fmaf(x[q][e], 0.0f, __fmul_rn(y[q][e], 0.0f)) != 0.0f) bad[r] = 1;
+        S0[r * kStride16 + hb * 32 + c] = (f16)__fmul_rn(x[q][e], a.sm_scale);
+        S1[r * kStride16 + hb * 32 + c] = (f16)y[q][e];
+      }
+    }
   }
-  redo_dq<4>(a, t0, phase, rows, g, bad, reinterpret_cast<RowScratch*>(S0), dout, lse, delta, dq);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * i + (threadIdx.x >> 4), cc = lane & 15;
+    if (r >= rows || bad[r]) continue;
+    const f16x8 v = *reinterpret_cast<const f16x8*>(S0 + r * kStride16 + 8 * cc);
+    if (keys) {
+      const int64_t o = ((int64_t)t0 + r) * a.nkv * kHD + (int64_t)g * kHD + 8 * cc;
+      *reinterpret_cast<f16x8*>(dk + o) = v;
+      *reinterpret_cast<f16x8*>(dv + o) = *reinterpret_cast<const f16x8*>(S1 + r * kStride16 + 8 * cc);
+    } else {
+      const int rr = phase + r;
+      *reinterpret_cast<f16x8*>(dq + ((int64_t)t0 + rr / gin) * a.nq * kHD +
+                                (int64_t)(g * gin + rr % gin) * kHD + 8 * cc) = v;
+    }
+  }
+  if (keys) redo_dkdv<4>(a, t0, rows, g, bad, scratch, dout, lse, delta, dk, dv);
+  else redo_dq<4>(a, t0, phase, rows, g, bad, scratch, dout, lse, delta, dq);
 }
 
 }  // namespace
@@ -648,7 +699,7 @@ extern "C" int dk_attn_span_bwd(const void* qkv, const void* out, const float* l
   if (n_units > 0 && (!workspace || workspace_bytes < dk_attn_span_bwd_workspace(n_units)))
     return DK_ERR_WORKSPACE;
   const int64_t pairs = n_tokens * nq, wgs = (pairs + 15) / 16;
-  if (n_items > INT32_MAX / kAThreads || n_joins > INT32_MAX / kAThreads || wgs > INT32_MAX / kAThreads)
+  if (n_items > INT32_MAX / kAThreads || n_joins > INT32_MAX / (4 * kAThreads) || wgs > INT32_MAX / kAThreads)
     return DK_ERR_INVALID;
   hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)wgs), dim3(kAThreads), 0, stream,
                      (const f16*)out, (const f16*)dout, delta, n_tokens, nq);
@@ -658,7 +709,7 @@ extern "C" int dk_attn_span_bwd(const void* qkv, const void* out, const float* l
                      (float*)workspace);
   DK_CHECK_LAUNCH();
   if (n_joins > 0) {
-    hipLaunchKernelGGL(span_bwd_join_kernel, dim3((unsigned)n_joins), dim3(kAThreads), 0, stream, a,
+    hipLaunchKernelGGL(span_bwd_join_kernel, dim3((unsigned)(4 * n_joins)), dim3(kAThreads), 0, stream, a,
                        joins, n_units, (const f16*)dout, lse, delta, (f16*)dq, (f16*)dk, (f16*)dv,
                        (const float*)workspace);
     DK_CHECK_LAUNCH();

@@ -223,8 +223,10 @@ def _fwd_tiles(blocks):
 
 
 def _bwd_cost(cost):
-    """Cost per item of the backward at most."""
-    return 1 << 30
+    """Cost per item of the backward at most: a little over a CU's share of the whole (256 CUs, an item
+    each at a time), so that no walk (a prompt's or a sink's keys over every later query) outlasts the
+    rest, and few partials are written."""
+    return max(32, int(1.2 * cost.sum() / 256) + 1)
 
 
 def _split_items(blocks, cost, most):

@@ -108,6 +108,20 @@ def test_against_the_definition(torch, spec, nq, nkv):
     _check(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv))
 
 
+@pytest.mark.parametrize("spec,nq,nkv", [CASES[i] for i in (0, 3, 5, 6, 7, 9, 11, 14, 15, 16)])
+@pytest.mark.parametrize("tiles", [1, 3])
+def test_walks_cut_in_parts(torch, monkeypatch, spec, nq, nkv, tiles):
+    """The same with every walk cut after a few tiles and joined again."""
+    from decentrik_prime_amd import k_attn
+    log(f"span attention fwd+bwd in walks of {tiles} tiles, {spec}, {nq}/{nkv} heads")
+    monkeypatch.setattr(k_attn, "_fwd_tiles", lambda blocks: tiles)
+    monkeypatch.setattr(k_attn, "_bwd_cost", lambda cost: 4 * tiles)
+    meta = _meta(spec, nq, nkv)
+    assert meta.n_units > 0 or meta.n_tokens < 64
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=meta.n_tokens + nq)
+    _check(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv))
+
+
 def test_no_tokens(torch):
     for spec in (("window", [], 4, 1), ("prefix", [(0, [0])])):
         meta = _meta(spec, 4, 2)
@@ -155,11 +169,16 @@ def test_wide_window_is_plain_causal_attention(torch):
     # a token of the second sequence's end
     (("window", [20, 300, 40], 50, 4), 319, lambda m: m != 319)])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), 65504.0])
-def test_unseen_rows_have_no_influence(torch, spec, bad, clean, value):
+@pytest.mark.parametrize("cut", [False, True])
+def test_unseen_rows_have_no_influence(torch, monkeypatch, spec, bad, clean, value, cut):
     """A row full of NaN, infinities or the type's largest value changes nothing for the queries that do
     not see it, nor for the keys that it does not see."""
     nq, nkv = 4, 2
     log(f"span attention with {value} in row {bad}, {spec}")
+    if cut:
+        from decentrik_prime_amd import k_attn
+        monkeypatch.setattr(k_attn, "_fwd_tiles", lambda blocks: 2)
+        monkeypatch.setattr(k_attn, "_bwd_cost", lambda cost: 8)
     meta = _meta(spec, nq, nkv)
     n = meta.n_tokens
     qkv, dout = _inputs(torch, n, nq, nkv, seed=11)
