@@ -123,6 +123,53 @@ __device__ __forceinline__ void store_dkdv(const SpanArgs& a, int k0, int nk, in
   }
 }
 
+// Up to 32 rows of dQ (or keys of dK and dV), wave hb holding columns 32 hb .. + 31 of them as quads,
+// rounded, staged and written back.  bad [32] is zero before.
+__device__ __forceinline__ void store_group(const SpanArgs& a, bool keys, int t0, int phase, int rows,
+                                            int g, int hb, const f32x4 (&x)[4], const f32x4 (&y)[4],
+                                            f16* S0, f16* S1, int* bad, f16* dq, f16* dk, f16* dv) {
+  const int lane = threadIdx.x & 63, hl = lane >> 5, c = lane & 31, gin = a.nq / a.nkv;
+  // staged as rows of 128: dq's lane holds 16 columns of its row, dK's and dV's a column of 16 keys
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (!keys) {
+      f16x4 o;
+      float chk = 0.0f;   // NaN if a value is not finite
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        chk = __builtin_fmaf(x[q][e], 0.0f, chk);
+        o[e] = (f16)__fmul_rn(x[q][e], a.sm_scale);
+      }
+      if (chk != 0.0f) bad[c] = 1;
+      *reinterpret_cast<f16x4*>(S0 + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = o;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 8 * q + 4 * hl + e;
+        if (__builtin_fmaf(x[q][e], 0.0f, __fmul_rn(y[q][e], 0.0f)) != 0.0f) bad[r] = 1;
+        S0[r * kStride16 + hb * 32 + c] = (f16)__fmul_rn(x[q][e], a.sm_scale);
+        S1[r * kStride16 + hb * 32 + c] = (f16)y[q][e];
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * i + (threadIdx.x >> 4), cc = lane & 15;
+    if (r >= rows || bad[r]) continue;
+    const f16x8 v = *reinterpret_cast<const f16x8*>(S0 + r * kStride16 + 8 * cc);
+    if (keys) {
+      const int64_t o = ((int64_t)t0 + r) * a.nkv * kHD + (int64_t)g * kHD + 8 * cc;
+      *reinterpret_cast<f16x8*>(dk + o) = v;
+      *reinterpret_cast<f16x8*>(dv + o) = *reinterpret_cast<const f16x8*>(S1 + r * kStride16 + 8 * cc);
+    } else {
+      const int rr = phase + r;
+      *reinterpret_cast<f16x8*>(dq + ((int64_t)t0 + rr / gin) * a.nq * kHD +
+                                (int64_t)(g * gin + rr % gin) * kHD + 8 * cc) = v;
+    }
+  }
+}
+
 // dQ of a block of stacked query rows, over the key tiles of its item
 __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items, int idx, int n_units,
                                         const f16* __restrict__ dout, const float* __restrict__ lse,
@@ -552,6 +599,171 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
   redo_dkdv<4>(a, k0, nk, g, bad, reinterpret_cast<RowScratch*>(Qs), dout, lse, delta, dk, dv);
 }
 
+// The same for a block of at most 32 keys (sinks, whose walk is the whole sequence): a step takes two
+// tiles, 32 queries of them to each wave, every wave against all the keys; the waves' sums are put
+// together at the end.  Per 64 queries that is a quarter of the products that four groups of 32
+// keys, three of them empty, would take.
+__device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* items, int idx, int n_units,
+                                            const f16* __restrict__ dout, const float* __restrict__ lse,
+                                            const float* __restrict__ delta, f16* __restrict__ dk,
+                                            f16* __restrict__ dv, float* __restrict__ parts, f16* Qs,
+                                            f16* Ds, float (*lse_s)[kBN], float (*dl_s)[kBN], int* bad) {
+  const int32_t* p = items + (int64_t)idx * kItemInts;
+  auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(p[k]); };
+  const int k0 = u(0), nk = u(2), g = u(3), qend = u(4), tb = u(11), te = u(12), slot = u(13);
+  const int gin = a.nq / a.nkv;
+  if (k0 < 0 || nk < 1 || nk > 32 || g < 0 || g >= a.nkv || (int64_t)k0 + nk > a.n_tokens ||
+      qend <= k0 || qend > a.n_tokens || tb < 0 || tb >= te || (slot >= 0 && slot > n_units - 2))
+    return;
+  const int per_head = (qend - k0 + kBN - 1) / kBN;
+  if (te > (int64_t)gin * per_head) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, hl = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(w);
+  const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
+  const bool nval = c < nk;
+  const int n = k0 + (nval ? c : 0);   // this lane's key
+  const int end = (int)key_end(a, n);
+  int end_min = nval ? end : INT32_MAX;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) end_min = min(end_min, __shfl_xor(end_min, x));
+  end_min = __builtin_amdgcn_readfirstlane(end_min);
+  if (tid < kBM) bad[tid] = 0;
+
+  const int n_tiles = te - tb, n_steps = (n_tiles + 1) / 2;
+  const TileSource qsrc = tile_source(a.qkv + (int64_t)k0 * ROW + (int64_t)g * gin * kHD, ROW, wave, lane);
+  const TileSource dsrc = tile_source(dout + (int64_t)k0 * OROW + (int64_t)g * gin * kHD, OROW, wave, lane);
+  int ihead = tb / per_head, itile = tb % per_head;
+  auto issue = [&](int t) {
+    if (t >= n_tiles) return;
+    const int st = t % kBwdStages, m0 = k0 + itile * kBN;
+    tile_load(qsrc, (int64_t)itile * kBN, (uint64_t)ihead * kHD * 2, qend - 1 - m0, Qs + st * kTileHalves, wave);
+    tile_load(dsrc, (int64_t)itile * kBN, (uint64_t)ihead * kHD * 2, qend - 1 - m0, Ds + st * kTileHalves, wave);
+    if (wave < 2) {
+      const int qq = m0 + lane < qend ? m0 + lane : qend - 1;
+      const float* src = (wave == 0 ? lse : delta) + (int64_t)(g * gin + ihead) * a.n_tokens + qq;
+      dma4(src, __builtin_amdgcn_readfirstlane(lds_addr(wave == 0 ? lse_s[st] : dl_s[st])));
+    }
+    if (++itile == per_head) {
+      itile = 0;
+      ++ihead;
+    }
+  };
+  issue(0);
+  issue(1);
+  f16x8 kf[kHD / 16], vf[kHD / 16];
+  {
+    const f16* krow = a.qkv + (int64_t)n * ROW + (int64_t)(a.nq + g) * kHD + 8 * hl;
+    const f16* vrow = krow + (int64_t)a.nkv * kHD;
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) {
+      kf[s] = *reinterpret_cast<const f16x8*>(krow + 16 * s);
+      vf[s] = *reinterpret_cast<const f16x8*>(vrow + 16 * s);
+    }
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) asm volatile("" : "+v"(kf[s]), "+v"(vf[s]));
+#pragma unroll
+    for (int s = 0; s < kHD / 16; ++s) {
+      kf[s] = nval ? kf[s] : zero8();
+      vf[s] = nval ? vf[s] : zero8();
+    }
+  }
+  f32x16 dkacc[kHD / 32], dvacc[kHD / 32];
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb) dkacc[hb] = dvacc[hb] = zero16();
+  const int half = wave & 1;   // this wave's 32 queries of its tile
+  const unsigned hoff = (unsigned)(half * 32 * kHD * 2);
+  const unsigned qrow = lds_addr(Qs) + row_base(lane) + hoff, drow = lds_addr(Ds) + row_base(lane) + hoff;
+  const unsigned qcol = lds_addr(Qs) + col_base(lane) + hoff, dcol = lds_addr(Ds) + col_base(lane) + hoff;
+  int walk = tb % per_head;   // the step's first tile within its head
+  for (int s = 0; s < n_steps; ++s) {
+    tile_barrier();   // the step's tiles are there, and every wave is done with those before
+    issue(2 * s + 2);
+    issue(2 * s + 3);
+    const int t = 2 * s + (wave >> 1);
+    int tile = walk + (wave >> 1);
+    tile = tile >= per_head ? tile - per_head : tile;
+    walk += 2;
+    while (walk >= per_head) walk -= per_head;
+    if (t >= n_tiles) continue;
+    const int st = t % kBwdStages, m0 = k0 + (per_head == 1 ? 0 : tile) * kBN + 32 * half;
+    const unsigned so = (unsigned)st * kStageBytes;
+    const unsigned qa = fresh(qrow + so), da = fresh(drow + so);
+    f32x16 sc = zero16(), dc = zero16();
+#pragma unroll
+    for (int i = 0; i < kHD / 16; ++i) {
+      sc = mfma(lds_read8(qa ^ (unsigned)(32 * i), 0), kf[i], sc);
+      dc = mfma(lds_read8(da ^ (unsigned)(32 * i), 0), vf[i], dc);
+    }
+    // query m0 + off + 4 (l / 32) counts iff lo <= off < hi; the others' P is 0
+    const bool masked = m0 < k0 + 31 || m0 + 32 > end_min;
+    const int lo = n - m0 - 4 * hl, hi = end - m0 - 4 * hl;
+    f16x8 pf[2], dsf[2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 l = *reinterpret_cast<const f32x4*>(&lse_s[st][32 * half + 8 * q + 4 * hl]);
+      const f32x4 d = *reinterpret_cast<const f32x4*>(&dl_s[st][32 * half + 8 * q + 4 * hl]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int v = 4 * q + e, off = 8 * q + e;
+        float x = __builtin_fmaf(sc[v], a.qk_scale, -l[e]);
+        if (masked) x = ((off >= lo) & (off < hi)) ? x : -1.0e30f;
+        const float pv = ex2(x);
+        pf[v >> 3][v & 7] = (f16)pv;
+        dsf[v >> 3][v & 7] = (f16)__fmul_rn(pv, __fsub_rn(dc[v], d[e]));
+      }
+    }
+    // dV += P^T dO, dK += dS^T Q over the wave's 32 queries, 16 per product
+    const unsigned qc = fresh(qcol + so), dc_ = fresh(dcol + so);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int hb = 0; hb < kHD / 32; ++hb) {
+        dvacc[hb] = mfma(pf[i], lds_col8(dc_, hb, 16 * i * kHD * 2), dvacc[hb]);
+        dkacc[hb] = mfma(dsf[i], lds_col8(qc, hb, 16 * i * kHD * 2), dkacc[hb]);
+      }
+  }
+  __syncthreads();
+  // the waves' sums, in wave order: 16 KB a wave of each, then wave w takes columns 32 w .. + 31
+  float* kx = reinterpret_cast<float*>(Qs);
+  float* vx = reinterpret_cast<float*>(Ds);
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      *reinterpret_cast<f32x4*>(kx + part_off(w, hb, q, lane)) = quad(dkacc[hb], q);
+      *reinterpret_cast<f32x4*>(vx + part_off(w, hb, q, lane)) = quad(dvacc[hb], q);
+    }
+  __syncthreads();
+  f32x4 x[4], y[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    x[q] = y[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+      const f32x4 kq = *reinterpret_cast<const f32x4*>(kx + part_off(o, w, q, lane));
+      const f32x4 vq = *reinterpret_cast<const f32x4*>(vx + part_off(o, w, q, lane));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[q][e] = __fadd_rn(x[q][e], kq[e]);
+        y[q][e] = __fadd_rn(y[q][e], vq[e]);
+      }
+    }
+  }
+  if (slot >= 0) {
+    float* part = parts + (int64_t)slot * kUnitFloats;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      *reinterpret_cast<f32x4*>(part + part_off(0, w, q, lane)) = x[q];
+      *reinterpret_cast<f32x4*>(part + kUnitFloats + part_off(0, w, q, lane)) = y[q];
+    }
+    return;
+  }
+  __syncthreads();   // the sums have been read
+  store_group(a, true, k0, 0, nk, g, w, x, y, Qs, Ds, bad, nullptr, dk, dv);
+  __syncthreads();   // and the staged rows
+  redo_dkdv<4>(a, k0, nk, g, bad, reinterpret_cast<RowScratch*>(Qs), dout, lse, delta, dk, dv);
+}
+
 // Every item of the backward in one launch, longest walks first (the plan's order): dK/dV walks and
 // dQ walks share the CUs, one workgroup each.
 __global__ __launch_bounds__(kAThreads) void span_bwd_kernel(
@@ -564,7 +776,10 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_kernel(
   __shared__ __attribute__((aligned(16))) float lse_s[kBwdStages + 1][kBN], dl_s[kBwdStages][kBN];
   __shared__ int bad[kBM];
   const int idx = (int)blockIdx.x;
-  if (__builtin_amdgcn_readfirstlane(items[(int64_t)idx * kItemInts + 14]))
+  const int kind = __builtin_amdgcn_readfirstlane(items[(int64_t)idx * kItemInts + 14]);
+  if (kind == 2)
+    dkdv_narrow(a, items, idx, n_units, dout, lse, delta, dk, dv, parts, T0, T1, lse_s, dl_s, bad);
+  else if (kind == 1)
     dkdv_item(a, items, idx, n_units, dout, lse, delta, dk, dv, parts, T0, T1, lse_s, dl_s, bad);
   else
     dq_item(a, items, idx, n_units, dout, lse, delta, dq, parts, T0, T1,
@@ -600,7 +815,7 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_join_kernel(
   __shared__ int bad[32];
   if (threadIdx.x < 32) bad[threadIdx.x] = 0;
   __syncthreads();
-  const int lane = threadIdx.x & 63, hb = threadIdx.x >> 6, hl = lane >> 5, c = lane & 31;
+  const int lane = threadIdx.x & 63, hb = threadIdx.x >> 6;
   f32x4 x[4], y[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) x[q] = y[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -631,45 +846,7 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_join_kernel(
   };
   sum(x, p);
   if (keys) sum(y, p + kUnitFloats);
-  // staged as rows of 128: dq's lane holds 16 columns of its row, dK's and dV's a column of 16 keys
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (!keys) {
-      f16x4 o;
-      float chk = 0.0f;   // NaN if a value is not finite
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        chk = __builtin_fmaf(x[q][e], 0.0f, chk);
-        o[e] = (f16)__fmul_rn(x[q][e], a.sm_scale);
-      }
-      if (chk != 0.0f) bad[c] = 1;
-      *reinterpret_cast<f16x4*>(S0 + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = o;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 8 * q + 4 * hl + e;
-        if (__builtin_fmaf(x[q][e], 0.0f, __fmul_rn(y[q][e], 0.0f)) != 0.0f) bad[r] = 1;
-        S0[r * kStride16 + hb * 32 + c] = (f16)__fmul_rn(x[q][e], a.sm_scale);
-        S1[r * kStride16 + hb * 32 + c] = (f16)y[q][e];
-      }
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 16 * i + (threadIdx.x >> 4), cc = lane & 15;
-    if (r >= rows || bad[r]) continue;
-    const f16x8 v = *reinterpret_cast<const f16x8*>(S0 + r * kStride16 + 8 * cc);
-    if (keys) {
-      const int64_t o = ((int64_t)t0 + r) * a.nkv * kHD + (int64_t)g * kHD + 8 * cc;
-      *reinterpret_cast<f16x8*>(dk + o) = v;
-      *reinterpret_cast<f16x8*>(dv + o) = *reinterpret_cast<const f16x8*>(S1 + r * kStride16 + 8 * cc);
-    } else {
-      const int rr = phase + r;
-      *reinterpret_cast<f16x8*>(dq + ((int64_t)t0 + rr / gin) * a.nq * kHD +
-                                (int64_t)(g * gin + rr % gin) * kHD + 8 * cc) = v;
-    }
-  }
+  store_group(a, keys, t0, phase, rows, g, hb, x, y, S0, S1, bad, dq, dk, dv);
   if (keys) redo_dkdv<4>(a, t0, rows, g, bad, scratch, dout, lse, delta, dk, dv);
   else redo_dq<4>(a, t0, phase, rows, g, bad, scratch, dout, lse, delta, dq);
 }

@@ -156,8 +156,7 @@ class SpanMeta:
         blocks = _query_blocks(runs, spans, nq // nkv, nkv)
         items, joins, self.n_slots = _split_items(blocks, blocks[:, _TE], _fwd_tiles(blocks))
         blocks = np.concatenate([_key_blocks(key_runs, spans, nq // nkv, nkv), blocks])
-        # a tile of a dK/dV walk takes 64 MFMAs a wave, one of a dQ walk 48
-        cost = blocks[:, _TE] * (3 + blocks[:, _KIND])
+        cost = blocks[:, _TE] * _TILE_COST[blocks[:, _KIND]]
         items_b, joins_b, self.n_units = _split_items(blocks, cost, _bwd_cost(cost))
         i32 = dict(dtype=torch.int32, device=device)
         self.spans = torch.tensor(spans, **i32)
@@ -172,6 +171,9 @@ _ROWS = 128           # stacked query rows of a block
 # columns of an item (include/dk.h)
 _T0, _PHASE, _N_ROWS, _G, _A0, _NA, _B0, _NK, _F0, _F1, _F2, _TB, _TE, _SLOT, _KIND = range(15)
 _QEND = 4             # of a block of keys
+# a tile of a dQ walk, of a dK/dV walk of 128 keys and of 32: 48, 64 and 16 MFMAs a wave, the last not
+# overlapped
+_TILE_COST = np.array([3, 4, 2])
 
 
 def _query_blocks(runs, spans, gin, nkv):
@@ -210,7 +212,8 @@ def _key_blocks(key_runs, spans, gin, nkv):
         k0 = np.arange(r0, r1, _ROWS, dtype=np.int64)
         nk = np.minimum(_ROWS, r1 - k0)
         x = np.zeros((k0.size, 16), np.int64)
-        x[:, _T0], x[:, _N_ROWS], x[:, _KIND], x[:, _SLOT] = k0, nk, 1, -1
+        x[:, _T0], x[:, _N_ROWS], x[:, _SLOT] = k0, nk, -1
+        x[:, _KIND] = np.where(nk <= 32, 2, 1)     # few keys (sinks): the walk of 32
         x[:, _QEND] = spans[k0 + nk - 1, 3]
         x[:, _TE] = gin * -(-(x[:, _QEND] - k0) // _KEYS)
         parts += [x + np.eye(1, 16, _G, dtype=np.int64) * g for g in range(nkv)]
@@ -223,10 +226,10 @@ def _fwd_tiles(blocks):
 
 
 def _bwd_cost(cost):
-    """Cost per item of the backward at most: a little over a CU's share of the whole (256 CUs, an item
-    each at a time), so that no walk (a prompt's or a sink's keys over every later query) outlasts the
-    rest, and few partials are written."""
-    return max(32, int(1.2 * cost.sum() / 256) + 1)
+    """Cost per item of the backward at most: a CU's share of the whole (256 CUs, an item each at a time)
+    and a little, so that no walk (a prompt's or a sink's keys over every later query) outlasts the rest,
+    and few partials are written."""
+    return int(cost.sum() / 256) + 16
 
 
 def _split_items(blocks, cost, most):
@@ -240,13 +243,13 @@ def _split_items(blocks, cost, most):
     items[:, _TB] = part * n[idx] // cut[idx]
     items[:, _TE] = (part + 1) * n[idx] // cut[idx]
     split = cut > 1
-    size = 1 + blocks[:, _KIND]           # units of a partial: dK and dV take two
+    size = np.where(blocks[:, _KIND] > 0, 2, 1)   # units of a partial: dK and dV take two
     units = np.where(split, cut * size, 0)
     first = np.cumsum(units) - units
     items[:, _SLOT] = np.where(split[idx], first[idx] + part * size[idx], -1)
     joins = np.zeros((int(split.sum()), 8), np.int64)
     joins[:, :4] = blocks[split][:, [_T0, _PHASE, _N_ROWS, _G]]
-    joins[:, 4], joins[:, 5], joins[:, 6] = first[split], cut[split], blocks[split][:, _KIND]
+    joins[:, 4], joins[:, 5], joins[:, 6] = first[split], cut[split], blocks[split][:, _KIND] > 0
     order = np.argsort(-cost[idx] // cut[idx], kind="stable")
     return items[order], joins, int(units.sum())
 

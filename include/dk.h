@@ -191,7 +191,8 @@ int dk_attn_span_fwd(const void* qkv, const int32_t* spans, const int32_t* items
                      int64_t workspace_bytes, hipStream_t stream);
 /* The backward's items: a block of query rows as above whose tiles are walked for dq (slot s: partial s
  * of the workspace, a unit), or with item[14] = 1 the keys k0 .. k0 + nk - 1 of KV head g for dk and dv:
- * k0, 0, nk, g, qend, 0, 0, 0, 0, 0, 0, tb, te, slot, 1, 0.  Its walk goes over the group's gin heads,
+ * k0, 0, nk, g, qend, 0, 0, 0, 0, 0, 0, tb, te, slot, 1, 0 (2 in place of 1, with nk <= 32: a wave's
+ * products take all of the keys).  Its walk goes over the group's gin heads,
  * each over the query tiles k0 + 64 i of [k0, qend), numbered through (slot s: units s and s + 1).
  * joins: t0 or k0, phase, rows or nk, g, first unit, partials, 1 for keys, 0.  The workspace holds
  * n_units units (dk_attn_span_bwd_workspace bytes, 256-byte aligned). */

@@ -155,12 +155,14 @@ def test_key_items_visit_every_visible_pair_once(nq, nkv):
             t0, phase, n, g, qend = it[:5]
             tb, te, slot, kind = it[11:15]
             if slot >= 0:
-                assert not units & set(range(slot, slot + 1 + kind))
-                units |= set(range(slot, slot + 1 + kind))
+                own = set(range(slot, slot + (2 if kind else 1)))
+                assert not units & own
+                units |= own
             if not kind:
                 for i in range(n if tb == 0 else 0):
                     rows[g * gin + (phase + i) % gin, t0 + (phase + i) // gin] += 1
                 continue
+            assert n <= (128 if kind == 1 else 32)
             per_head = -(-(qend - t0) // 64)
             assert 0 <= tb < te <= gin * per_head
             for t in range(tb, te):
