@@ -70,23 +70,39 @@ __device__ __forceinline__ KeySource key_source(int64_t row_halves, int wave, in
   s.off0 = s.r0 * s.rowb + s.chunk;
   return s;
 }
+// One operand's tiles in order: where key 0 would lie in each run, and the bytes of the tiles before.
+struct KeyWalk {
+  uint64_t pa, pb, adv;
+  int t;
+};
+__device__ __forceinline__ KeyWalk key_walk(const SpanItem& it, uint64_t base, unsigned rowb) {
+  return KeyWalk{base + (uint64_t)it.a0 * rowb, base + (uint64_t)((int64_t)it.b0 - it.na) * rowb,
+                 (uint64_t)it.tb * kBN * rowb, it.tb};
+}
 template <int W>
-__device__ __forceinline__ void key_tile_load(const SpanItem& it, const KeySource& s, int t, uint64_t base,
+__device__ __forceinline__ void next_key_tile(const SpanItem& it, KeyWalk& k, const KeySource& s,
                                               const f16* stage, int wave) {
-  const int j0 = t * kBN;
+  const int j0 = k.t * kBN;
   const bool second = j0 >= it.na;
-  const uint64_t tb = base + (uint64_t)(second ? it.b0 + (j0 - it.na) : it.a0 + j0) * s.rowb;
-  const unsigned thr = second ? kBN : (unsigned)(it.na - j0);   // the second run's first row here
-  const unsigned gap = (unsigned)(it.b0 - it.a0 - it.na) * s.rowb;
-  const unsigned rows = (unsigned)(it.nk - 1 - j0);
-  const unsigned last = (rows < kBN ? rows * s.rowb + (rows >= thr ? gap : 0u) : ~0u - 4096u) + s.chunk;
+  const uint64_t tb = (second ? k.pb : k.pa) + k.adv;
+  const unsigned dst = __builtin_amdgcn_readfirstlane(lds_addr(stage + wave * 512));
+  if ((second || j0 + kBN <= it.na) && j0 + kBN <= it.nk) {
 #pragma unroll
-  for (int i = 0; i < kBN / 4 / W; ++i) {
-    unsigned off = s.off0 + (unsigned)(4 * W * i) * s.rowb;
-    off += s.r0 + 4 * W * i >= thr ? gap : 0u;
-    dma16s(tb, off < last ? off : last,
-           __builtin_amdgcn_readfirstlane(lds_addr(stage + (W * i + wave) * 512)));
+    for (int i = 0; i < kBN / 4 / W; ++i) dma16s(tb, s.off0 + (unsigned)(4 * W * i) * s.rowb, dst + W * i * 1024);
+  } else {
+    const unsigned thr = second ? kBN : (unsigned)(it.na - j0);   // the second run's first row here
+    const unsigned gap = (unsigned)(it.b0 - it.a0 - it.na) * s.rowb;
+    const unsigned rows = (unsigned)(it.nk - 1 - j0);
+    const unsigned last = (rows < kBN ? rows * s.rowb + (rows >= thr ? gap : 0u) : ~0u - 4096u) + s.chunk;
+#pragma unroll
+    for (int i = 0; i < kBN / 4 / W; ++i) {
+      unsigned off = s.off0 + (unsigned)(4 * W * i) * s.rowb;
+      off += s.r0 + 4 * W * i >= thr ? gap : 0u;
+      dma16s(tb, off < last ? off : last, dst + W * i * 1024);
+    }
   }
+  k.adv += (uint64_t)kBN * s.rowb;
+  ++k.t;
 }
 // the keys' ends, by one wave
 __device__ __forceinline__ void key_ends_load(const SpanArgs& a, const SpanItem& it, int t, const int* dst,

@@ -191,11 +191,12 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
   const KeySource src = key_source(ROW, wave, lane);
   const uint64_t kbase = uniform64((uint64_t)(a.qkv + (int64_t)(a.nq + it.g) * kHD));
   const uint64_t vbase = kbase + (uint64_t)a.nkv * kHD * sizeof(f16);
+  KeyWalk kw = key_walk(it, kbase, src.rowb), vw = key_walk(it, vbase, src.rowb);
   auto issue = [&](int t) {
     if (t >= n_tiles) return;
     const int st = t % kBwdStages;
-    key_tile_load<4>(it, src, it.tb + t, kbase, Ks + st * kTileHalves, wave);
-    key_tile_load<4>(it, src, it.tb + t, vbase, Vs + st * kTileHalves, wave);
+    next_key_tile<4>(it, kw, src, Ks + st * kTileHalves, wave);
+    next_key_tile<4>(it, vw, src, Vs + st * kTileHalves, wave);
     if (wave == 0) key_ends_load(a, it, it.tb + t, ends[st], lane);
   };
   issue(0);

@@ -58,21 +58,19 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
   const uint64_t kbase = uniform64((uint64_t)(a.qkv + (int64_t)(a.nq + it.g) * kHD));
   const uint64_t vbase = kbase + (uint64_t)a.nkv * kHD * sizeof(f16);
   const KeySource src = key_source(ROW, wave, lane);
-  // tile pair u (tiles 2 u, 2 u + 1 of the walk) of one operand into stages t % 4
-  auto issue = [&](uint64_t base, f16* ring, int u) {
+  KeyWalk kw = key_walk(it, kbase, src.rowb), vw = key_walk(it, vbase, src.rowb);
+  // the next pair of tiles (tiles 2 u, 2 u + 1 of the walk) of one operand into stages t % 4
+  auto issue = [&](KeyWalk& x, f16* ring) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int t = 2 * u + b;
-      if (t >= n_tiles) continue;
-      key_tile_load<kFWaves>(it, src, it.tb + t, base, ring + (t % kFwdStages) * kTileHalves, wave);
-    }
+    for (int b = 0; b < 2; ++b)
+      if (x.t < it.te) next_key_tile<kFWaves>(it, x, src, ring + ((x.t - it.tb) % kFwdStages) * kTileHalves, wave);
   };
   auto issue_v = [&](int u) {
-    issue(vbase, Vs, u);
+    issue(vw, Vs);
     const int t = 2 * u + wave;
     if (wave < 2 && t < n_tiles) key_ends_load(a, it, it.tb + t, ends[t % kFwdStages], lane);
   };
-  issue(kbase, Ks, 0);
+  issue(kw, Ks);
   // this lane's query row as the B operand (rows past the block: zeros).  Loaded unconditionally and
   // selected at once, so the compiler's wait for these loads stands here and not inside the loop.
   f16x8 qf[kHD / 16];
@@ -88,7 +86,7 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
   if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
   wait_vmem<0>();
   issue_v(0);
-  issue(kbase, Ks, 1);
+  issue(kw, Ks);
   __syncthreads();
   const unsigned krow = lds_addr(Ks) + row_base(lane), vcol = lds_addr(Vs) + col_base(lane);
   // S^T = K Q^T of tile t: keys kb * 32 + (row of the result), queries on the lanes
@@ -199,7 +197,7 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
   // scores are done), V of pair u + 1 where pair u - 1's was
   auto fetch = [&](int u) {
     issue_v(u + 1);
-    issue(kbase, Ks, u + 2);
+    issue(kw, Ks);
   };
   auto next = [&]() {
     wait_vmem<0>();

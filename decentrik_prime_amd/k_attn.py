@@ -229,7 +229,7 @@ def _bwd_cost(cost):
     """Cost per item of the backward at most: a CU's share of the whole (256 CUs, an item each at a time)
     and a little, so that no walk (a prompt's or a sink's keys over every later query) outlasts the rest,
     and few partials are written."""
-    return int(cost.sum() / 256) + 16
+    return int(1.25 * cost.sum() / 256) + 12
 
 
 def _split_items(blocks, cost, most):
@@ -252,6 +252,7 @@ def _split_items(blocks, cost, most):
     joins[:, 4], joins[:, 5], joins[:, 6] = first[split], cut[split], blocks[split][:, _KIND] > 0
     order = np.argsort(-cost[idx] // cut[idx], kind="stable")
     return items[order], joins, int(units.sum())
+
 
 
 def _lengths(lens, what):
