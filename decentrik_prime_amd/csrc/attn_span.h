@@ -112,6 +112,16 @@ __device__ __forceinline__ void key_ends_load(const SpanArgs& a, const SpanItem&
   dma4(a.spans + 4 * row + 3, __builtin_amdgcn_readfirstlane(lds_addr(dst)));
 }
 
+constexpr int kStride16 = kHD + 8;   // halves per staged row of a result
+
+// Where quad q of result block hb of wave w's rows stands in a partial: 16 bytes per lane, lane-major.
+__device__ __forceinline__ int part_off(int w, int hb, int q, int lane) {
+  return ((w * (kHD / 32) + hb) * 4 + q) * 256 + 4 * lane;
+}
+__device__ __forceinline__ f32x4 quad(const f32x16& x, int q) {
+  return f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+}
+
 // One query row or one key row at a time, a wave each, over exactly the keys (or queries) that it
 // sees: nothing else is read, so whatever a masked row holds cannot reach the result.
 struct RowScratch {

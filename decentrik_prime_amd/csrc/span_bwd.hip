@@ -6,15 +6,6 @@
 namespace {
 
 constexpr int kUnitFloats = kBM * kHD;   // a partial of dQ; dK and dV take two
-constexpr int kStride16 = kHD + 8;       // halves per staged row of a result
-
-// Where quad q of result block hb of wave w's rows stands in a partial: 16 bytes per lane, lane-major.
-__device__ __forceinline__ int part_off(int w, int hb, int q, int lane) {
-  return ((w * (kHD / 32) + hb) * 4 + q) * 256 + 4 * lane;
-}
-__device__ __forceinline__ f32x4 quad(const f32x16& x, int q) {
-  return f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
-}
 
 // The tile ring of both backward kernels: a tile of two operands (kBN rows each) in one of four
 // LDS stages, filled by LDS DMA.  Wave w's instruction i fills chunks (4 i + w) 64 + lane of an

@@ -5,9 +5,8 @@
 
 namespace {
 
-constexpr int kFThreads = 512;
-constexpr int kFWaves = kFThreads / 64;
-// a partial: O (lane-major, below) and the rows' m and l
+constexpr int kStages = 2;   // of each operand's ring
+// a partial: O (part_off) and the rows' m and l
 constexpr int kPartFloats = kBM * kHD + 2 * kBM;
 
 // max over the two lanes l, l ^ 32 (the two key halves of one query)
@@ -29,7 +28,7 @@ __device__ __forceinline__ void redo_rows(const SpanArgs& a, int t0, int phase, 
   }
 }
 
-__global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const int32_t* __restrict__ items,
+__global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, const int32_t* __restrict__ items,
                                                              int n_slots, f16* __restrict__ out,
                                                              float* __restrict__ lse,
                                                              float* __restrict__ parts) {
@@ -37,38 +36,35 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
   if (!span_item(a, items, (int)blockIdx.x, n_slots, &it)) return;
   const int lane = threadIdx.x & 63, hl = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int qw = wave & 3, kg = wave >> 2;   // query group, key-tile parity
   const int gin = a.nq / a.nkv;
   const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD;
-  const int row = 32 * qw + c;               // this lane's stacked row
+  const int row = 32 * wave + c;             // this lane's stacked row
   const bool mval = row < it.rows;
   const int rr = it.phase + (mval ? row : 0);
   const int m = it.t0 + rr / gin, h = it.g * gin + rr % gin;
   const int jlim = mval ? m - it.b0 + it.na : -1;   // its last key
-  __shared__ __attribute__((aligned(1024))) f16 Ks[kFwdStages * kTileHalves];
-  __shared__ __attribute__((aligned(1024))) f16 Vs[kFwdStages * kTileHalves];
-  __shared__ __attribute__((aligned(16))) int ends[kFwdStages][kBN];
+  __shared__ __attribute__((aligned(1024))) f16 ring[2 * kStages * kTileHalves];
+  __shared__ __attribute__((aligned(16))) int ends[kStages][kBN];
+  f16* const Ks = ring;
+  f16* const Vs = ring + kStages * kTileHalves;
   __shared__ int bad[kBM];
 
   f32x16 oacc[kHD / 32];
 #pragma unroll
   for (int hb = 0; hb < kHD / 32; ++hb) oacc[hb] = zero16();
   float m_i = -1.0e30f, l_i = 0.0f;   // l_i: this lane's half of the keys (joined at the end)
-  const int n_tiles = it.te - it.tb, n_pairs = (n_tiles + 1) / 2;
+  const int n_tiles = it.te - it.tb;
   const uint64_t kbase = uniform64((uint64_t)(a.qkv + (int64_t)(a.nq + it.g) * kHD));
   const uint64_t vbase = kbase + (uint64_t)a.nkv * kHD * sizeof(f16);
   const KeySource src = key_source(ROW, wave, lane);
   KeyWalk kw = key_walk(it, kbase, src.rowb), vw = key_walk(it, vbase, src.rowb);
-  // the next pair of tiles (tiles 2 u, 2 u + 1 of the walk) of one operand into stages t % 4
-  auto issue = [&](KeyWalk& x, f16* ring) {
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-      if (x.t < it.te) next_key_tile<kFWaves>(it, x, src, ring + ((x.t - it.tb) % kFwdStages) * kTileHalves, wave);
+  // the next tile of one operand into stage t % 2
+  auto issue = [&](KeyWalk& x, f16* stages) {
+    if (x.t < it.te) next_key_tile<4>(it, x, src, stages + ((x.t - it.tb) % kStages) * kTileHalves, wave);
   };
-  auto issue_v = [&](int u) {
+  auto issue_v = [&](int t) {
     issue(vw, Vs);
-    const int t = 2 * u + wave;
-    if (wave < 2 && t < n_tiles) key_ends_load(a, it, it.tb + t, ends[t % kFwdStages], lane);
+    if (wave == 0 && t < n_tiles) key_ends_load(a, it, it.tb + t, ends[t % kStages], lane);
   };
   issue(kw, Ks);
   // this lane's query row as the B operand (rows past the block: zeros).  Loaded unconditionally and
@@ -91,7 +87,7 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
   const unsigned krow = lds_addr(Ks) + row_base(lane), vcol = lds_addr(Vs) + col_base(lane);
   // S^T = K Q^T of tile t: keys kb * 32 + (row of the result), queries on the lanes
   auto scores = [&](f32x16 (&sc)[2], int t) {
-    const unsigned ka = fresh(krow + (unsigned)((t % kFwdStages) * kTileHalves * 2));
+    const unsigned ka = fresh(krow + (unsigned)((t % kStages) * kTileHalves * 2));
     sc[0] = sc[1] = zero16();
 #pragma unroll
     for (int s = 0; s < kHD / 16; ++s)
@@ -100,23 +96,22 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
         sc[kb] = mfma(lds_read8(ka ^ (unsigned)(32 * s), kb * 32 * kHD * 2), qf[s], sc[kb]);
   };
   f32x16 sc[2], sn[2];
-  if (kg < n_tiles) scores(sc, kg);
-  else sc[0] = sc[1] = zero16();
+  scores(sc, 0);
   wait_vmem<0>();
   __syncthreads();
-  // tile t, whose scores are in sc: its softmax and O^T += V^T P^T, beside the scores of tile t + 2
+  // tile t, whose scores are in sc: its softmax and O^T += V^T P^T, beside the scores of tile t + 1
   // into sn when there is one.  MASK: key j of the tile counts iff j <= jlim and the key's end lies
   // past this lane's token; the others' probabilities are set to 0 (a lane may see none of a tile's
   // keys before its first).
   auto tile = [&](int t, bool more, f32x16 (&sc)[2], f32x16 (&sn)[2], auto mask_c) {
     constexpr bool MASK = decltype(mask_c)::value;
-    const unsigned va = fresh(vcol + (unsigned)((t % kFwdStages) * kTileHalves * 2));
+    const unsigned va = fresh(vcol + (unsigned)((t % kStages) * kTileHalves * 2));
     const int lim = jlim - (it.tb + t) * kBN - 4 * hl;
     unsigned on = 0;
     if constexpr (MASK) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const i32x4 e4 = *reinterpret_cast<const i32x4*>(&ends[t % kFwdStages][8 * q + 4 * hl]);
+        const i32x4 e4 = *reinterpret_cast<const i32x4*>(&ends[t % kStages][8 * q + 4 * hl]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const bool k = (8 * q + e <= lim) & (m < e4[e]);
@@ -145,7 +140,7 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
 #pragma unroll
         for (int v = 0; v < 16; ++v) oacc[hb][v] = __fmul_rn(oacc[hb][v], alpha);
     }
-    if (!MASK || more) scores(sn, t + 2);
+    if (!MASK || more) scores(sn, t + 1);
     else sn[0] = sn[1] = zero16();   // nothing of the last tile's buffer stays live
     float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     f16x8 pf[kBN / 16];   // P^T as the B operand: keys 16 tt .. + 15
@@ -193,175 +188,169 @@ __global__ __launch_bounds__(kFThreads) void span_fwd_kernel(SpanArgs a, const i
   };
   using Mask = std::integral_constant<bool, true>;
   using Full = std::integral_constant<bool, false>;
-  // V of pair u and K of pair u + 1 are in LDS; K of pair u + 2 goes where pair u's was (its
-  // scores are done), V of pair u + 1 where pair u - 1's was
-  auto fetch = [&](int u) {
-    issue_v(u + 1);
+  // V of tile t and K of tile t + 1 are in LDS; K of tile t + 2 goes where tile t's was (its scores are
+  // done), V of tile t + 1 where tile t - 1's was
+  auto fetch = [&](int t) {
+    issue_v(t + 1);
     issue(kw, Ks);
   };
   auto next = [&]() {
     wait_vmem<0>();
     __syncthreads();
   };
-  // this wave's tile of pair u: unmasked, and with a next tile whose scores it computes beside it
-  auto full = [&](int u) {
-    return 2 * u + kg + 2 < n_tiles && full_tile(it, it.tb + 2 * u + kg);
-  };
-  int u = 0;
-  while (u < n_pairs) {
-    for (; full(u) && full(u + 1); u += 2) {   // the two score buffers need no copies
-      fetch(u);
-      tile(2 * u + kg, true, sc, sn, Full{});
+  // unmasked, and with a next tile whose scores are computed beside it
+  auto full = [&](int t) { return t + 1 < n_tiles && full_tile(it, it.tb + t); };
+  int t = 0;
+  while (t < n_tiles) {
+    for (; full(t) && full(t + 1); t += 2) {   // the two score buffers need no copies
+      fetch(t);
+      tile(t, true, sc, sn, Full{});
       next();
-      fetch(u + 1);
-      tile(2 * u + 2 + kg, true, sn, sc, Full{});
+      fetch(t + 1);
+      tile(t + 1, true, sn, sc, Full{});
       next();
     }
-    if (u < n_pairs) {
-      fetch(u);
-      const int t = 2 * u + kg;
-      if (t < n_tiles) tile(t, t + 2 < n_tiles, sc, sn, Mask{});
-      else sn[0] = sn[1] = zero16();
+    if (t < n_tiles) {
+      fetch(t);
+      tile(t, t + 1 < n_tiles, sc, sn, Mask{});
       sc[0] = sn[0];
       sc[1] = sn[1];
       next();
-      ++u;
+      ++t;
     }
   }
   l_i = __fadd_rn(l_i, __shfl_xor(l_i, 32));
-  // merge: the odd-tile wave of each query group hands its state (O lane-major, 16 KB per wave,
-  // in the K stages; m and l in the V stages' last KB) to the even-tile wave
-  float* ohand = reinterpret_cast<float*>(Ks) + qw * (kHD / 32) * 16 * 64;
-  float* mlhand = reinterpret_cast<float*>(Vs) + (kFwdStages * kTileHalves / 2 - 256) + qw * 64;
-  static_assert(4 * (kHD / 32) * 16 * 64 * 4 <= kFwdStages * kTileHalves * 2, "O hand-over in Ks");
-  if (kg == 1) {
+  if (it.slot >= 0) {
+    float* part = parts + (int64_t)it.slot * kPartFloats;
 #pragma unroll
     for (int hb = 0; hb < kHD / 32; ++hb)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) ohand[(hb * 16 + v) * 64 + lane] = oacc[hb][v];
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(part + part_off(wave, hb, q, lane)) = quad(oacc[hb], q);
     if (hl == 0) {
-      mlhand[c] = m_i;
-      mlhand[32 + c] = l_i;
+      part[kBM * kHD + row] = m_i;
+      part[kBM * kHD + kBM + row] = l_i;
     }
-  }
-  __syncthreads();
-  constexpr int kOStride = kHD + 8;   // halves per staged row
-  static_assert(4 * 32 * kOStride + 512 <= kFwdStages * kTileHalves, "O staging in Vs");
-  f16* ostage = Vs + qw * 32 * kOStride;
-  if (kg == 0) {
-    const float m1 = mlhand[c], l1 = mlhand[32 + c];
-    const float mm = fmaxf(m_i, m1);
-    const float a0 = ex2(__fsub_rn(m_i, mm)), a1 = ex2(__fsub_rn(m1, mm));
-    const float l = __fadd_rn(__fmul_rn(l_i, a0), __fmul_rn(l1, a1));
-    if (it.slot >= 0) {
-      float* part = parts + (int64_t)it.slot * kPartFloats;
-#pragma unroll
-      for (int hb = 0; hb < kHD / 32; ++hb)
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          part[((qw * (kHD / 32) + hb) * 16 + v) * 64 + lane] =
-              __fadd_rn(__fmul_rn(oacc[hb][v], a0), __fmul_rn(ohand[(hb * 16 + v) * 64 + lane], a1));
-      if (hl == 0) {
-        part[kBM * kHD + row] = mm;
-        part[kBM * kHD + kBM + row] = l;
-      }
-      return;
-    }
-    const float inv_l = __fdiv_rn(1.0f, l);   // rows past the block: not stored
-    float chk = __fmul_rn(l, 0.0f);           // NaN if anything below is not finite
-#pragma unroll
-    for (int hb = 0; hb < kHD / 32; ++hb)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f16x4 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = 4 * q + e;
-          const float ov = __fadd_rn(__fmul_rn(oacc[hb][v], a0),
-                                     __fmul_rn(ohand[(hb * 16 + v) * 64 + lane], a1));
-          chk = __builtin_fmaf(ov, 0.0f, chk);
-          o[e] = (f16)__fmul_rn(ov, inv_l);
-        }
-        *reinterpret_cast<f16x4*>(ostage + c * kOStride + hb * 32 + 8 * q + 4 * hl) = o;
-      }
-    chk = __fadd_rn(chk, __shfl_xor(chk, 32));
-    if (chk != 0.0f) bad[row] = 1;
-    else if (mval && hl == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(mm, log2f(l));
-  } else if (it.slot >= 0) {
     return;
   }
-  __syncthreads();
-  // the two waves of a query group store 16 of its 32 rows each, four whole 256-byte rows per store
+  // the wave's 32 x 128 block of O staged in the (now free) ring, one correctly rounded reciprocal per
+  // row, and written back 16 bytes per lane, four whole 256-byte rows per store
+  static_assert(4 * 32 * kStride16 <= 2 * kStages * kTileHalves, "O staging in the ring");
+  f16* ostage = ring + wave * 32 * kStride16;
+  const float inv_l = __fdiv_rn(1.0f, l_i);   // rows past the block: not stored
+  float chk = __fmul_rn(l_i, 0.0f);           // NaN if anything below is not finite
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 16 * kg + 4 * i + (lane >> 4), cc = lane & 15;
-    const int srow = 32 * qw + r, sr = it.phase + srow;
-    const f16x8 v = *reinterpret_cast<const f16x8*>(ostage + r * kOStride + 8 * cc);
+  for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f16x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float ov = oacc[hb][4 * q + e];
+        chk = __builtin_fmaf(ov, 0.0f, chk);
+        o[e] = (f16)__fmul_rn(ov, inv_l);
+      }
+      *reinterpret_cast<f16x4*>(ostage + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = o;
+    }
+  chk = __fadd_rn(chk, __shfl_xor(chk, 32));
+  if (chk != 0.0f) bad[row] = 1;
+  else if (mval && hl == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(m_i, log2f(l_i));
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 4), cc = lane & 15;
+    const int srow = 32 * wave + r, sr = it.phase + srow;
+    const f16x8 v = *reinterpret_cast<const f16x8*>(ostage + r * kStride16 + 8 * cc);
     if (srow < it.rows && !bad[srow])
       *reinterpret_cast<f16x8*>(out + (int64_t)(it.t0 + sr / gin) * a.nq * kHD +
                                 (int64_t)(it.g * gin + sr % gin) * kHD + 8 * cc) = v;
   }
-  static_assert(kFWaves * sizeof(RowScratch) <= kFwdStages * kTileHalves * 2, "row scratch in Ks");
-  redo_rows<kFWaves>(a, it.t0, it.phase, it.rows, it.g, bad, reinterpret_cast<RowScratch*>(Ks), out, lse);
+  __syncthreads();   // the staged rows have been read
+  redo_rows<4>(a, it.t0, it.phase, it.rows, it.g, bad, reinterpret_cast<RowScratch*>(ring), out, lse);
 }
 
 // The partials of a block put together: O = sum_s O_s 2^(m_s - m) / l, m = max m_s, l likewise, in slot
-// order.  Wave w takes query group w / 2 and half w % 2 of the columns.
-__global__ __launch_bounds__(kFThreads) void span_join_kernel(SpanArgs a, const int32_t* __restrict__ joins,
+// order.  A workgroup per 32 rows, a wave per 32 columns, four partials' loads in flight.
+__global__ __launch_bounds__(kAThreads) void span_join_kernel(SpanArgs a, const int32_t* __restrict__ joins,
                                                               int n_slots, f16* __restrict__ out,
                                                               float* __restrict__ lse,
                                                               const float* __restrict__ parts) {
-  const int32_t* j = joins + (int64_t)blockIdx.x * DK_ATTN_SPAN_JOIN_INTS;
-  const int t0 = j[0], phase = j[1], rows = j[2], g = j[3], s0 = j[4], cnt = j[5];
+  const int32_t* j = joins + (int64_t)(blockIdx.x >> 2) * DK_ATTN_SPAN_JOIN_INTS;
+  const int qw = blockIdx.x & 3;   // the row group
+  auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(j[k]); };
+  int t0 = u(0), phase = u(1), rows = u(2);
+  const int g = u(3), s0 = u(4), cnt = u(5);
   const int gin = a.nq / a.nkv;
   if (t0 < 0 || phase < 0 || phase >= gin || rows < 1 || rows > kBM || g < 0 || g >= a.nkv ||
-      (int64_t)t0 + (phase + rows - 1) / gin >= a.n_tokens || s0 < 0 || cnt < 1 || cnt > n_slots - s0)
+      (int64_t)t0 + (phase + rows - 1) / gin >= a.n_tokens || s0 < 0 || cnt < 1 || cnt > n_slots - s0 ||
+      rows <= 32 * qw)
     return;
-  __shared__ int bad[kBM];
-  __shared__ RowScratch scratch[kFWaves];
-  if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
+  rows = rows - 32 * qw < 32 ? rows - 32 * qw : 32;   // the group's own rows
+  t0 += (phase + 32 * qw) / gin;
+  phase = (phase + 32 * qw) % gin;
+  __shared__ __attribute__((aligned(16))) f16 stage[32 * kStride16];
+  __shared__ RowScratch scratch[kAThreads / 64];
+  __shared__ int bad[32];
+  if (threadIdx.x < 32) bad[threadIdx.x] = 0;
   __syncthreads();
-  const int lane = threadIdx.x & 63, hl = lane >> 5, c = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int qw = wave >> 1, hb0 = 2 * (wave & 1), row = 32 * qw + c;
+  const int lane = threadIdx.x & 63, hb = threadIdx.x >> 6, hl = lane >> 5, c = lane & 31;
   const float* p0 = parts + (int64_t)s0 * kPartFloats;
-  float mm = -1.0e30f;
-  for (int s = 0; s < cnt; ++s) mm = fmaxf(mm, p0[(int64_t)s * kPartFloats + kBM * kHD + row]);
-  float l = 0.0f;
-  f32x16 o[2] = {zero16(), zero16()};
-  for (int s = 0; s < cnt; ++s) {
-    const float* p = p0 + (int64_t)s * kPartFloats;
-    const float w = ex2(__fsub_rn(p[kBM * kHD + row], mm));
-    l = __builtin_fmaf(p[kBM * kHD + kBM + row], w, l);
+  const float* ml = p0 + kBM * kHD + 32 * qw + c;
+  float mm = -1.0e30f, l = 0.0f;
+  for (int s = 0; s < cnt; ++s) mm = fmaxf(mm, ml[(int64_t)s * kPartFloats]);
+  f32x4 o[4];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+  for (int q = 0; q < 4; ++q) o[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const float* p = p0 + part_off(qw, hb, 0, lane);
+  for (int s = 0; s < cnt; s += 4) {
+    f32x4 t[4][4];
+    float w[4], ls[4];
 #pragma unroll
-      for (int v = 0; v < 16; ++v)
-        o[b][v] = __builtin_fmaf(p[((qw * (kHD / 32) + hb0 + b) * 16 + v) * 64 + lane], w, o[b][v]);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t x = (int64_t)(s + i < cnt ? s + i : cnt - 1) * kPartFloats;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) t[i][q] = *reinterpret_cast<const f32x4*>(p + x + 256 * q);
+      w[i] = ml[x];
+      ls[i] = ml[x + kBM];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s + i >= cnt) break;
+      w[i] = ex2(__fsub_rn(w[i], mm));
+      l = __builtin_fmaf(ls[i], w[i], l);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[q][e] = __builtin_fmaf(t[i][q][e], w[i], o[q][e]);
+    }
   }
-  float chk = __fmul_rn(l, 0.0f);
+  const float inv_l = __fdiv_rn(1.0f, l);
+  float chk = __fmul_rn(l, 0.0f);   // NaN if a value is not finite
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int q = 0; q < 4; ++q) {
+    f16x4 x;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) chk = __builtin_fmaf(o[b][v], 0.0f, chk);
-  if (chk != 0.0f) bad[row] = 1;
+    for (int e = 0; e < 4; ++e) {
+      chk = __builtin_fmaf(o[q][e], 0.0f, chk);
+      x[e] = (f16)__fmul_rn(o[q][e], inv_l);
+    }
+    *reinterpret_cast<f16x4*>(stage + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = x;
+  }
+  if (chk != 0.0f) bad[c] = 1;
   __syncthreads();
-  if (row < rows && !bad[row]) {
-    const int rr = phase + row, m = t0 + rr / gin, h = g * gin + rr % gin;
-    const float inv_l = __fdiv_rn(1.0f, l);
-    f16* orow = out + (int64_t)m * a.nq * kHD + (int64_t)h * kHD;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f16x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = (f16)__fmul_rn(o[b][4 * q + e], inv_l);
-        *reinterpret_cast<f16x4*>(orow + (hb0 + b) * 32 + 8 * q + 4 * hl) = x;
-      }
-    if (hl == 0 && hb0 == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(mm, log2f(l));
+  if (threadIdx.x < rows && !bad[threadIdx.x]) {   // wave 0, its first half: c is the row
+    const int rr = phase + c;
+    lse[(int64_t)(g * gin + rr % gin) * a.n_tokens + t0 + rr / gin] = __fadd_rn(mm, log2f(l));
   }
-  redo_rows<kFWaves>(a, t0, phase, rows, g, bad, scratch, out, lse);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * i + (threadIdx.x >> 4), cc = lane & 15, rr = phase + r;
+    const f16x8 v = *reinterpret_cast<const f16x8*>(stage + r * kStride16 + 8 * cc);
+    if (r < rows && !bad[r])
+      *reinterpret_cast<f16x8*>(out + ((int64_t)t0 + rr / gin) * a.nq * kHD +
+                                (int64_t)(g * gin + rr % gin) * kHD + 8 * cc) = v;
+  }
+  redo_rows<4>(a, t0, phase, rows, g, bad, scratch, out, lse);
 }
 
 }  // namespace
@@ -385,12 +374,12 @@ extern "C" int dk_attn_span_fwd(const void* qkv, const int32_t* spans, const int
     return DK_ERR_ALIGN;
   if (n_slots > 0 && (!workspace || workspace_bytes < dk_attn_span_workspace(n_slots)))
     return DK_ERR_WORKSPACE;
-  if (n_items > INT32_MAX / kFThreads || n_joins > INT32_MAX / kFThreads) return DK_ERR_INVALID;
-  hipLaunchKernelGGL(span_fwd_kernel, dim3((unsigned)n_items), dim3(kFThreads), 0, stream, a, items,
+  if (n_items > INT32_MAX / kAThreads || n_joins > INT32_MAX / (4 * kAThreads)) return DK_ERR_INVALID;
+  hipLaunchKernelGGL(span_fwd_kernel, dim3((unsigned)n_items), dim3(kAThreads), 0, stream, a, items,
                      n_slots, (f16*)out, lse, (float*)workspace);
   DK_CHECK_LAUNCH();
   if (n_joins > 0) {
-    hipLaunchKernelGGL(span_join_kernel, dim3((unsigned)n_joins), dim3(kFThreads), 0, stream, a, joins,
+    hipLaunchKernelGGL(span_join_kernel, dim3((unsigned)(4 * n_joins)), dim3(kAThreads), 0, stream, a, joins,
                        n_slots, (f16*)out, lse, (const float*)workspace);
     DK_CHECK_LAUNCH();
   }

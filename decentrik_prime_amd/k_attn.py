@@ -221,8 +221,9 @@ def _key_blocks(key_runs, spans, gin, nkv):
 
 
 def _fwd_tiles(blocks):
-    """Tiles per item of the forward at most."""
-    return 1 << 30
+    """Tiles per item of the forward at most: a little over the share of one of the 512 workgroups that run
+    at a time, two to a CU, and no fewer than make up for a partial."""
+    return max(6, int(0.6 * blocks[:, _TE].sum() / 256) + 1)
 
 
 def _bwd_cost(cost):
