@@ -54,7 +54,8 @@ def _check(torch, spec, nq, nkv, qkv, dout, got):
     to fp16 (half a step, 2^-11 of the value, 2^-25 below the normal range), the scores' fp32 sums move
     P by at most HD 2^-24 of the products' magnitudes and the fp32 sums over the keys by less than
     2^-12 (together under 2^-10 of the magnitudes summed), and the result itself is rounded to fp16
-    (2^-11; 2^-25 below the normal range)."""
+    (2^-11; 2^-25 below the normal range).  delta is taken from the returned out, off by what out is, and
+    moves dS by that times P."""
     vis = torch.from_numpy(_visible(spec)).cuda()
     n, gin, sm = qkv.shape[0], nq // nkv, HD ** -0.5
     x = qkv.double().view(n, nq + 2 * nkv, HD)
@@ -63,17 +64,18 @@ def _check(torch, spec, nq, nkv, qkv, dout, got):
     for h in range(nq):
         g = h // gin
         q, k, v = x[:, h], x[:, nq + g], x[:, nq + nkv + g]
-        o, do = out[:, h].double(), dout.view(n, nq, HD)[:, h].double()
+        do = dout.view(n, nq, HD)[:, h].double()
         sc = torch.where(vis, sm * (q @ k.t()), -float("inf"))
         p = torch.softmax(sc, 1)
-        dl = (o * do).sum(1, keepdim=True)
+        dl = ((p @ v) * do).sum(1, keepdim=True)
         ds = p * (do @ v.t() - dl)
+        off = ((2.0 ** -10 * (p @ v.abs()) + 2.0 ** -11 * (p @ v).abs() + 2.0 ** -24) * do.abs()).sum(1, keepdim=True)
         what = f"{spec}, {nq}/{nkv} heads, head {h}: "
         _near(out[:, h], p @ v, 2.0 ** -10 * (p @ v.abs()) + 2.0 ** -11 * (p @ v).abs() + 2.0 ** -24,
               what + "out")
         _near(lse[h], torch.logsumexp(sc, 1) / math.log(2.0), 2.0 ** -12, what + "lse")
         eds = torch.where(vis, 2.0 ** -10 * ds.abs() + 2.0 ** -25 + HD * 2.0 ** -23 * p * (
-            do.abs() @ v.abs().t() + (o * do).abs().sum(1, keepdim=True)), 0.0)
+            do.abs() @ v.abs().t() + ((p @ v) * do).abs().sum(1, keepdim=True)) + off * p, 0.0)
         want = sm * (ds @ k)
         _near(dq[:, h], want, sm * (eds @ k.abs()) + 2.0 ** -11 * want.abs() + 2.0 ** -24, what + "dq")
         wk[:, g] += sm * (ds.t() @ q)
