@@ -67,6 +67,8 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, cons
     if (wave == 0 && t < n_tiles) key_ends_load(a, it, it.tb + t, ends[t % kStages], lane);
   };
   issue(kw, Ks);
+  issue_v(0);
+  issue(kw, Ks);
   // this lane's query row as the B operand (rows past the block: zeros).  Loaded unconditionally and
   // selected at once, so the compiler's wait for these loads stands here and not inside the loop.
   f16x8 qf[kHD / 16];
@@ -81,8 +83,6 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, cons
   }
   if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
   wait_vmem<0>();
-  issue_v(0);
-  issue(kw, Ks);
   __syncthreads();
   const unsigned krow = lds_addr(Ks) + row_base(lane), vcol = lds_addr(Vs) + col_base(lane);
   // S^T = K Q^T of tile t: keys kb * 32 + (row of the result), queries on the lanes
@@ -97,13 +97,12 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, cons
   };
   f32x16 sc[2], sn[2];
   scores(sc, 0);
-  wait_vmem<0>();
-  __syncthreads();
+  __syncthreads();   // every wave is done with K of tile 0
   // tile t, whose scores are in sc: its softmax and O^T += V^T P^T, beside the scores of tile t + 1
   // into sn when there is one.  MASK: key j of the tile counts iff j <= jlim and the key's end lies
   // past this lane's token; the others' probabilities are set to 0 (a lane may see none of a tile's
   // keys before its first).
-  auto tile = [&](int t, bool more, f32x16 (&sc)[2], f32x16 (&sn)[2], auto mask_c) {
+  auto tile = [&](int t, f32x16 (&sc)[2], f32x16 (&sn)[2], auto mask_c) {
     constexpr bool MASK = decltype(mask_c)::value;
     const unsigned va = fresh(vcol + (unsigned)((t % kStages) * kTileHalves * 2));
     const int lim = jlim - (it.tb + t) * kBN - 4 * hl;
@@ -140,8 +139,7 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, cons
 #pragma unroll
         for (int v = 0; v < 16; ++v) oacc[hb][v] = __fmul_rn(oacc[hb][v], alpha);
     }
-    if (!MASK || more) scores(sn, t + 1);
-    else sn[0] = sn[1] = zero16();   // nothing of the last tile's buffer stays live
+    scores(sn, t + 1);
     float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     f16x8 pf[kBN / 16];   // P^T as the B operand: keys 16 tt .. + 15
 #pragma unroll
@@ -162,23 +160,18 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, cons
         oacc[hb] = mfma(lds_col8(va, hb, 16 * tt * kHD * 2), pf[tt], oacc[hb]);
     // the next tile's scores spread over the exponentials, their operands read four MFMAs ahead;
     // then O, its operands four MFMAs (eight reads) ahead
-    if constexpr (!MASK) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-      for (int i = 0; i < 12; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
-      }
+    for (int i = 0; i < 12; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
-      }
-    } else {
-      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 200, 0);
+    for (int i = 0; i < 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -198,21 +191,20 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, cons
     wait_vmem<0>();
     __syncthreads();
   };
-  // unmasked, and with a next tile whose scores are computed beside it
   auto full = [&](int t) { return t + 1 < n_tiles && full_tile(it, it.tb + t); };
   int t = 0;
   while (t < n_tiles) {
     for (; full(t) && full(t + 1); t += 2) {   // the two score buffers need no copies
       fetch(t);
-      tile(t, true, sc, sn, Full{});
+      tile(t, sc, sn, Full{});
       next();
       fetch(t + 1);
-      tile(t + 1, true, sn, sc, Full{});
+      tile(t + 1, sn, sc, Full{});
       next();
     }
     if (t < n_tiles) {
       fetch(t);
-      tile(t, t + 1 < n_tiles, sc, sn, Mask{});
+      tile(t, sc, sn, Mask{});
       sc[0] = sn[0];
       sc[1] = sn[1];
       next();
