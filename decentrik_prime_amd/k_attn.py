@@ -145,7 +145,7 @@ class SpanMeta:
     spans [n, 4] int32 on the device: token m sees, as a query, the keys [a0, a1) and [kbeg, m]; as a
     key it is seen by the queries m .. kend - 1.  positions [n] int32: each token's position (an
     answer's go on from its prompt's), for the rotary embedding.  A plan serves any number of
-    calls, on any streams of its device, captured or not."""
+    calls, on any streams of its device, captured or not.  n_pairs: visible (query, key) pairs of a head."""
 
     def __init__(self, runs, key_runs, spans, positions, nq, nkv, device):
         if nq < 1 or nkv < 1 or nq % nkv:
@@ -153,6 +153,7 @@ class SpanMeta:
         if spans.shape[0] > MAX_SPAN_TOKENS:
             raise ValueError(f"at most {MAX_SPAN_TOKENS} tokens (got {spans.shape[0]})")
         self.n_tokens, self.nq, self.nkv = int(spans.shape[0]), int(nq), int(nkv)
+        self.n_pairs = int((spans[:, 3] - np.arange(self.n_tokens)).sum())
         blocks = _query_blocks(runs, spans, nq // nkv, nkv)
         items, joins, self.n_slots = _split_items(blocks, blocks[:, _TE], _fwd_tiles(blocks))
         blocks = np.concatenate([_key_blocks(key_runs, spans, nq // nkv, nkv), blocks])

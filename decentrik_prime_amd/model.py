@@ -17,6 +17,9 @@ Every activation the backward needs is kept in HBM (about 120 MB per layer at 20
 reference's host arenas, recompute plans and offload options exist for a 16 GB card and are not
 built.  Weights are random (W ~ N(0, 0.02) NF4, norm weights near 1, embedding ~ N(0, 0.02));
 the tokens and targets are random ids, each sequence's targets its next token (-1 at its end).
+
+``window`` (and ``sinks``) or ``groups`` select k_attn's attention over part of the keys in place of
+causal attention: a sliding window in every layer, or answers behind shared prompts.
 """
 
 import torch
@@ -42,10 +45,21 @@ def rope_tables(positions, hd=HD, theta=1.0e6, device="cuda"):
 
 class QwenQLoRAStep(NF4LinearStack):
     """Random-init Qwen2.5-1.5B (n_layers decoder layers, the LM head over `vocab`) with rank-16
-    LoRA on q and v, one packed batch of sequences of lengths `lens`."""
+    LoRA on q and v, one packed batch of sequences of lengths `lens`.  window, sinks: causal attention
+    inside a sliding window and to a sequence's first tokens (k_attn.window_meta).  groups: the batch is
+    groups (prompt length, [answer lengths]) in place of sequences (k_attn.prefix_meta; lens is None)."""
 
     def __init__(self, lens, n_layers=28, vocab=VOCAB, seed=0, device="cuda", eps=1e-6,
-                 head_grad_scale=1024.0, head_chunk=k_head.CHUNK, ahead="layer"):
+                 head_grad_scale=1024.0, head_chunk=k_head.CHUNK, ahead="layer", window=None, sinks=0,
+                 groups=None):
+        if (lens is None) == (groups is None):
+            raise ValueError("either lens or groups")
+        if groups is not None:
+            if window is not None:
+                raise ValueError("a window over groups is not supported")
+            lens = [n for prompt, answers in groups for n in (prompt, *answers)]
+        if sinks and window is None:
+            raise ValueError("sinks need a window")
         m = int(sum(lens))
         super().__init__(n_layers, m, seed=seed, device=device, ahead=ahead)
         dev, f16, f32 = self.device, torch.float16, torch.float32
@@ -58,9 +72,20 @@ class QwenQLoRAStep(NF4LinearStack):
         self.w_in = [norm_w() for _ in range(n_layers)]
         self.w_post = [norm_w() for _ in range(n_layers)]
         self.w_final = norm_w()
-        self.cos, self.sin = rope_tables(max(lens), device=dev)
-        self.pos = torch.cat([torch.arange(n, dtype=torch.int32, device=dev) for n in lens])
-        self.meta = k_attn.meta_for(lens, dev)
+        if groups is not None:
+            self.meta = k_attn.prefix_meta(groups, NQ, NKV, dev)
+        elif window is not None:
+            self.meta = k_attn.window_meta(lens, window, sinks, NQ, NKV, dev)
+        else:
+            self.meta = k_attn.meta_for(lens, dev)
+        self.span = isinstance(self.meta, k_attn.SpanMeta)
+        if self.span:
+            self.pos = self.meta.positions
+            positions = int(self.pos.max()) + 1
+        else:
+            self.pos = torch.cat([torch.arange(n, dtype=torch.int32, device=dev) for n in lens])
+            positions = max(lens)
+        self.cos, self.sin = rope_tables(positions, device=dev)
         # embedding, tokens and next-token targets (sorted: rows with a target first)
         self.emb = (torch.randn(vocab, D, generator=gen, device=dev) * 0.02).half()
         ids = torch.randint(0, vocab, (m,), generator=gen, device=dev)
@@ -100,7 +125,7 @@ class QwenQLoRAStep(NF4LinearStack):
     def for_batch(cls, batch, **kwargs):
         """The step on the tokens of a packed batch (trainer.pack): its rows' lengths, token ids
         and next-token targets; the weights are random-init as for any instance."""
-        st = cls(batch.lens, **kwargs)
+        st = cls(None if batch.groups else batch.lens, groups=batch.groups, **kwargs)
         st.use_tokens(batch.ids, batch.tgt)
         return st
 
@@ -127,7 +152,8 @@ class QwenQLoRAStep(NF4LinearStack):
     def flops_per_step(self):
         """Algorithmic FLOPs: the linear layers, the causal attention (2 hd L(L+1) per sequence and
         head forward, 2.5 times that backward), the LM head (logits and P E, 2 M V D each)."""
-        att = sum(2 * HD * n * (n + 1) for n in self.lens) * NQ * 3.5
+        pairs = self.meta.n_pairs if self.span else sum(n * (n + 1) // 2 for n in self.lens)
+        att = 4 * HD * pairs * NQ * 3.5
         return self.n_layers * (layer_flops(self.m) + att) + 2 * 2 * self.m * self.emb.shape[0] * D
 
     def forward(self):
@@ -152,7 +178,8 @@ class QwenQLoRAStep(NF4LinearStack):
                                 self.sin, (NQ + NKV) * HD, out=self.qkv_b[i], w16=w16("qkv", i),
                                 side=side("qkv", i + 1))
             done("qkv", i + 1)
-            self.att[i], self.lse[i] = k_attn.attention_forward(self.qkv_b[i], self.meta, NQ, NKV, HD)
+            attend = k_attn.span_attention_forward if self.span else k_attn.attention_forward
+            self.att[i], self.lse[i] = attend(self.qkv_b[i], self.meta, NQ, NKV, HD)
             linear_forward(self.att[i], Lw["o"], out=self.op[i], w16=w16("o", i), side=side("o", i + 1))
             done("o", i + 1)
             k_norm.rms_forward(self.xin[i], self.w_post[i], self.y2, self.rstd2[i], self.eps,
@@ -191,11 +218,12 @@ class QwenQLoRAStep(NF4LinearStack):
             linear_backward_dx(dh16, Lw["o"], out=self.dout, out_dtype=torch.float16,
                                w16=w16("o", i), side=side("o", i - 1))
             done("o", i - 1)
-            dq, dkp, dvp = k_attn.attention_backward(self.qkv_b[i], self.att[i], self.lse[i],
-                                                     self.dout, self.meta, NQ, NKV, HD)
+            attend = k_attn.span_attention_backward if self.span else k_attn.attention_backward
+            dq, dkp, dvp = attend(self.qkv_b[i], self.att[i], self.lse[i], self.dout, self.meta, NQ,
+                                  NKV, HD)
             dqkv = self.qkv_b[i]      # the QKV epilogue backward writes d(qkv) over the forward's qkv
             k_rope.qkv_epilogue_backward(dq, dkp, dvp, self.pos, self.cos, self.sin, dqkv, NQ, NKV,
-                                         HD, NQ // NKV)
+                                         HD, 1 if self.span else NQ // NKV)
             del dq, dkp, dvp
             terms = [(dqkv[:, :D], z["q"], lo["Bq"], self.s, None, 1.0, self.xq[i]),
                      (dqkv[:, D + KV:], z["v"], lo["Bv"], self.s, None, 1.0, self.xv[i])]

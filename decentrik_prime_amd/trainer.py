@@ -33,6 +33,7 @@ class PackedBatch:
     n_real     n, the number of real (unpadded) tokens
     n_lab      tokens with a target
     B, T       batch rows and padded length
+    groups     None, or the batch's (prompt length, [answer lengths]) (pack_answers)
     """
     lens: list
     ids: torch.Tensor
@@ -45,6 +46,7 @@ class PackedBatch:
     n_lab: int
     B: int
     T: int
+    groups: list = None
 
 
 def _row_length(mask_row):
@@ -94,6 +96,44 @@ def pack(input_ids, attention_mask, labels, vocab):
     return PackedBatch(lens=lens, ids=ids, tgt=tgt, perm=perm, tgt_sorted=tgt[perm],
                        row_sorted=rows[perm], valid_sorted=has[perm], n_real=int(ids.numel()),
                        n_lab=int(has.sum()), B=B, T=T)
+
+
+def pack_answers(groups, vocab):
+    """Host-side packing of groups of answers that share a prompt, each prompt packed once (no
+    counterpart in the reference, which repeats the prompt in every row): groups of (prompt ids,
+    [answer ids]), 1-D integer tensors or lists.  The loss is over the answers' tokens, a batch row per
+    answer, each as if it stood alone behind its prompt: the prompt's last token, whose target differs
+    from answer to answer, begins each answer.  Returns None when the batch is not packable: no answers,
+    an empty prompt or answer, or an id outside the vocabulary."""
+    shape, lens, ids, tgt, rows, longest = [], [], [], [], [], 0
+
+    def piece(tokens, targets, row):
+        lens.append(tokens.numel())
+        ids.append(tokens)
+        tgt.append(targets)
+        rows.append(torch.full((tokens.numel(),), row, dtype=torch.int64))
+    B = 0
+    for prompt, answers in groups:
+        prompt = torch.as_tensor(prompt, dtype=torch.int64, device="cpu")
+        answers = [torch.as_tensor(a, dtype=torch.int64, device="cpu") for a in answers]
+        if any(t.dim() != 1 or t.numel() == 0 for t in (prompt, *answers)) or not answers:
+            return None
+        piece(prompt[:-1], torch.full((prompt.numel() - 1,), -1, dtype=torch.int64), B)
+        for a in answers:
+            piece(torch.cat([prompt[-1:], a]), torch.cat([a, a.new_full((1,), -1)]), B)
+            longest = max(longest, prompt.numel() + a.numel())
+            B += 1
+        shape.append((prompt.numel() - 1, [1 + a.numel() for a in answers]))
+    if B == 0:
+        return None
+    ids, tgt, rows = torch.cat(ids), torch.cat(tgt), torch.cat(rows)
+    if int(ids.min()) < 0 or int(ids.max()) >= vocab:
+        return None
+    has = tgt >= 0
+    perm = torch.sort((~has).to(torch.int8), stable=True).indices
+    return PackedBatch(lens=lens, ids=ids, tgt=tgt, perm=perm, tgt_sorted=tgt[perm],
+                       row_sorted=rows[perm], valid_sorted=has[perm], n_real=int(ids.numel()),
+                       n_lab=int(has.sum()), B=B, T=longest, groups=shape)
 
 
 def batch_metrics(batch, stats):

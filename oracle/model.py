@@ -19,12 +19,13 @@ import math
 import torch
 
 
-def qwen_step(p, lens, nq=12, nkv=2, hd=128):
+def qwen_step(p, lens, nq=12, nkv=2, hd=128, visible=None):
     """p: CPU tensors x0 [n, D] fp32, emb [V, D], tgt [n] (-1 = none), pos [n], cos / sin
     [positions, hd], w_final [D], eps, ks (dropout keep scale), s (LoRA scale), and layers: dicts
     of wqkv [(nq + 2 nkv) hd, D], bias, wo [D, nq hd], wgu [2 I, D] (gate rows, then up rows),
     wd [D, I], w_in, w_post [D], Aq [r, D], Bq [nq hd, r], Av [r, D], Bv [nkv hd, r], mq / mv
-    [n, D] (nonzero = keep).  Returns (loss_sum, [(dA_q, dB_q, dA_v, dB_v) per layer])."""
+    [n, D] (nonzero = keep).  visible [n, n] bool: the keys that each query sees, in place of causal
+    attention inside sequences of lengths lens.  Returns (loss_sum, [(dA_q, dB_q, dA_v, dB_v) per layer])."""
     dt = torch.float64
     eps, ks, s = float(p["eps"]), float(p["ks"]), float(p["s"])
     n = p["x0"].shape[0]
@@ -58,13 +59,14 @@ def qwen_step(p, lens, nq=12, nkv=2, hd=128):
         k = rope(k.view(n, nkv, hd))
         v = v.view(n, nkv, hd)
         outs, s0 = [], 0
-        for ln in lens:
+        for ln in ([n] if visible is not None else lens):
             sl = slice(s0, s0 + ln)
             qq = q[sl].transpose(0, 1)
             kk = k[sl].transpose(0, 1).repeat_interleave(g, 0)
             vv = v[sl].transpose(0, 1).repeat_interleave(g, 0)
             o = torch.nn.functional.scaled_dot_product_attention(
-                qq[None], kk[None], vv[None], is_causal=True, scale=1.0 / math.sqrt(hd))[0]
+                qq[None], kk[None], vv[None], visible, is_causal=visible is None,
+                scale=1.0 / math.sqrt(hd))[0]
             outs.append(o.transpose(0, 1).reshape(ln, qd))
             s0 += ln
         h = x + torch.cat(outs) @ L["wo"].to(dt).T

@@ -135,3 +135,92 @@ def test_trainer_metrics_of_a_packed_batch(torch):
     mean = float(trainer.compute_loss(loss_sum, batch))
     ref_mean = float(tok[batch.tgt.numpy() >= 0, 0].sum()) / batch.n_lab
     assert abs(mean - ref_mean) <= 2e-3 * abs(ref_mean)
+
+
+def _reference_inputs(torch, st, k_nf4):
+    layers = []
+    for i in range(st.n_layers):
+        pk = st.layers[i]["packed"]
+        buf = torch.empty(pk.numel, dtype=torch.float16, device="cuda")
+        k_nf4.dequant_layer(pk, st.code2, st.nf4, buf)
+
+        def w(kind):
+            start, n = st.views[kind]
+            W = st.layers[i][kind]
+            return buf[start:start + n].view(W.rows, W.cols).cpu()
+        lo = st.lora[i]
+        layers.append(dict(wqkv=w("qkv"), wo=w("o"), wgu=w("gu"), wd=w("d"), bias=lo["bias"].cpu(),
+                           w_in=st.w_in[i].cpu(), w_post=st.w_post[i].cpu(),
+                           **{k: lo[k].cpu() for k in ("Aq", "Bq", "Av", "Bv", "mq", "mv")}))
+    return dict(x0=st.x0.cpu(), emb=st.emb.cpu(), tgt=st.tgt.cpu(), pos=st.pos.cpu(), cos=st.cos.cpu(),
+                sin=st.sin.cpu(), w_final=st.w_final.cpu(), eps=st.eps, ks=st.keep_scale, s=st.s,
+                layers=layers)
+
+
+@pytest.mark.parametrize("kind", ["window", "groups"])
+def test_step_over_part_of_the_keys(torch, kind):
+    """The whole step under a sliding window with sinks, and over groups of answers behind shared
+    prompts, against the float64 reference with the same visible pairs; tolerances as for the causal
+    step."""
+    from decentrik_prime_amd import k_nf4, model
+    from oracle import attn
+    from oracle import model as ref
+    if kind == "window":
+        lens, window, sinks = [37, 210, 64], 50, 4
+        st = model.QwenQLoRAStep(lens, n_layers=2, vocab=4096, seed=5, head_chunk=1024, window=window,
+                                 sinks=sinks)
+        vis = attn.window_visible(lens, window, sinks)
+    else:
+        groups = [(70, [30, 1, 45]), (0, [40]), (33, [20, 20])]
+        st = model.QwenQLoRAStep(None, n_layers=2, vocab=4096, seed=5, head_chunk=1024, groups=groups)
+        vis = attn.prefix_visible(groups)
+    log(f"whole QLoRA step over part of the keys: {kind}")
+    loss = st.step()
+    loss2 = st.step()
+    torch.cuda.synchronize()
+    assert float(loss) == float(loss2), "the step is deterministic"
+    ref_loss, ref_grads = ref.qwen_step(_reference_inputs(torch, st, k_nf4), st.lens,
+                                        visible=torch.from_numpy(vis))
+    assert abs(float(loss) - ref_loss) <= 1e-4 * abs(ref_loss), (float(loss), ref_loss)
+    for i in range(2):
+        for nm, got, want in zip(("dA_q", "dB_q", "dA_v", "dB_v"), st.grads[i], ref_grads[i]):
+            g, r = host(got).astype(np.float64), want.numpy()
+            err = float(np.abs(g - r).max()) / float(np.abs(r).max())
+            assert err <= 1e-2, f"layer {i} {nm}: {err:.3g}"
+
+
+def test_shared_prompts_train_as_rows_of_their_own(torch):
+    """A batch packed by trainer.pack_answers gives the loss and the LoRA gradients of the same answers as
+    rows with a prompt each (trainer.pack), without dropout: both within the causal step's tolerance of
+    the same float64 values."""
+    from decentrik_prime_amd import model, trainer
+    rng = np.random.default_rng(3)
+    vocab = 4096
+    groups = [(rng.integers(0, vocab, p), [rng.integers(0, vocab, a) for a in ans])
+              for p, ans in ((120, (30, 7, 55)), (40, (60, 1)))]
+    log("shared prompts against rows of their own")
+    kw = dict(n_layers=2, vocab=vocab, seed=9, head_chunk=1024)
+    shared = model.QwenQLoRAStep.for_batch(trainer.pack_answers(groups, vocab), **kw)
+    whole = [(np.concatenate([p, a]), len(p)) for p, ans in groups for a in ans]
+    T = max(len(w) for w, _ in whole)
+    ids, mask, labels = (torch.zeros(len(whole), T, dtype=torch.int64) for _ in range(3))
+    labels -= 100
+    for b, (w, n) in enumerate(whole):
+        ids[b, :len(w)], mask[b, :len(w)] = torch.from_numpy(w), 1
+        labels[b, n:len(w)] = torch.from_numpy(w[n:])
+    rows = model.QwenQLoRAStep.for_batch(trainer.pack(ids, mask, labels, vocab), **kw)
+    for st in (shared, rows):
+        st.keep_scale = 1.0
+        for i in range(2):
+            st.layers[i] = shared.layers[i]
+            for k, v in shared.lora[i].items():
+                st.lora[i][k] = v if k not in ("mq", "mv") else torch.ones_like(st.lora[i][k])
+    a, b = shared.step(), rows.step()
+    torch.cuda.synchronize()
+    assert shared.n_lab == rows.n_lab and shared.m < rows.m
+    assert abs(float(a) - float(b)) <= 2e-4 * abs(float(b)), (float(a), float(b))
+    for i in range(2):
+        for nm, x, y in zip(("dA_q", "dB_q", "dA_v", "dB_v"), shared.grads[i], rows.grads[i]):
+            x, y = host(x).astype(np.float64), host(y).astype(np.float64)
+            err = float(np.abs(x - y).max()) / float(np.abs(y).max())
+            assert err <= 2e-2, f"layer {i} {nm}: {err:.3g}"

@@ -154,3 +154,47 @@ def test_padded_walk_known_answer():
     tok = [stats[(0, 0)], stats[(0, 1)], stats[(0, 2)], stats[(1, 0)], stats[(1, 1)]]
     st = torch.tensor([list(tok[i]) + [0.0] for i in b.perm.tolist()], dtype=torch.float64)
     assert trainer.batch_metrics(b, st) == want
+
+
+def test_pack_answers_against_a_token_walk():
+    """Every answer's row of targets is that of the prompt and the answer packed alone with the prompt's
+    labels ignored; the prompt stands once; what an answer's token sees are the tokens before it."""
+    from decentrik_prime_amd import k_attn
+    from oracle import attn
+    rng = np.random.default_rng(5)
+    groups = [(rng.integers(0, 40, p), [rng.integers(0, 40, a) for a in ans])
+              for p, ans in ((6, (3, 1, 4)), (1, (5,)), (9, (2, 2)))]
+    b = trainer.pack_answers(groups, vocab=40)
+    assert b.groups == [(5, [4, 2, 5]), (0, [6]), (8, [3, 3])] and b.B == 6 and b.T == 11
+    assert sum(b.lens) == b.n_real == b.ids.numel() and b.n_lab == 17
+    vis = attn.prefix_visible(b.groups)
+    meta = k_attn.prefix_meta(b.groups, 2, 1, "cpu")
+    at, row = 0, 0
+    for prompt, answers in groups:
+        first = at
+        assert b.ids[at:at + len(prompt) - 1].tolist() == prompt[:-1].tolist()
+        assert (b.tgt[at:at + len(prompt) - 1] == -1).all()
+        at += len(prompt) - 1
+        for a in answers:
+            whole = np.concatenate([prompt, a])
+            lab = np.concatenate([np.full(len(prompt), -100), a])
+            alone = trainer.pack(torch.from_numpy(whole)[None], torch.ones(1, len(whole), dtype=torch.int64),
+                                 torch.from_numpy(lab)[None], 40)
+            end = at + 1 + len(a)
+            assert b.ids[at:end].tolist() == whole[len(prompt) - 1:].tolist()
+            assert b.tgt[at:end].tolist() == alone.tgt[len(prompt) - 1:].tolist()
+            for t in range(at, end):
+                seen = np.nonzero(vis[t])[0]
+                assert b.ids[seen].tolist() == whole[:len(prompt) + t - at].tolist()
+                assert int(meta.positions[t]) == len(seen) - 1
+            of_row = b.row_sorted[(b.perm >= at) & (b.perm < end)]
+            assert (of_row == row).all()
+            at, row = end, row + 1
+        assert at > first
+    assert at == b.n_real
+
+
+def test_pack_answers_refuses():
+    for groups in ([], [([1, 2], [])], [([], [[1]])], [([1], [[]])], [([1], [[40]])], [([-1], [[3]])],
+                   [([[1, 2]], [[3]])]):
+        assert trainer.pack_answers(groups, vocab=40) is None
