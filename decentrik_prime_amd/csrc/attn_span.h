@@ -46,7 +46,7 @@ __device__ __forceinline__ bool span_item(const SpanArgs& a, const int32_t* item
          (int64_t)it->t0 + (it->phase + it->rows - 1) / gin < a.n_tokens && it->a0 >= 0 &&
          it->na >= 0 && (int64_t)it->a0 + it->na <= a.n_tokens && it->b0 >= 0 && it->nk > it->na &&
          (int64_t)it->b0 + it->nk - it->na <= a.n_tokens &&
-         (it->na == 0 || (it->b0 >= it->a0 + it->na &&
+         (it->na % kBN == 0 || (it->b0 >= it->a0 + it->na &&
                           ((int64_t)it->b0 - it->a0 - it->na + kBN) * (a.nq + 2 * a.nkv) * kHD * 2 <
                               (int64_t)DK_ATTN_SPAN_REACH_BYTES)) && it->tb >= 0 && it->tb < it->te &&
          it->te <= (it->nk + kBN - 1) / kBN && it->slot < n_slots;

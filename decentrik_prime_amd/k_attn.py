@@ -144,31 +144,44 @@ class SpanMeta:
 
     spans [n, 4] int32 on the device: token m sees, as a query, the keys [a0, a1) and [kbeg, m]; as a
     key it is seen by the queries m .. kend - 1.  positions [n] int32: each token's position (an
-    answer's go on from its prompt's), for the rotary embedding.  A plan serves any number of
-    calls, on any streams of its device, captured or not.  n_pairs: visible (query, key) pairs of a head."""
+    answer's go on from its prompt's), for the rotary embedding.  n_pairs: visible (query, key) pairs of
+    a head.  The other tables are the kernels' work, cut into items here on the host (include/dk.h).  A
+    plan serves any number of calls, on any streams of its device, captured or not."""
 
     def __init__(self, runs, key_runs, spans, positions, nq, nkv, device):
+        """runs: (first, past the last) token arrays of the runs whose tokens share [a0, a1) and whose kbeg
+        does not fall; key_runs: of the runs whose kend does not fall."""
+        n = int(spans.shape[0])
         if nq < 1 or nkv < 1 or nq % nkv:
             raise ValueError(f"nq must be a multiple of nkv (got {nq}, {nkv})")
-        if spans.shape[0] > MAX_SPAN_TOKENS:
-            raise ValueError(f"at most {MAX_SPAN_TOKENS} tokens (got {spans.shape[0]})")
-        self.n_tokens, self.nq, self.nkv = int(spans.shape[0]), int(nq), int(nkv)
-        self.n_pairs = int((spans[:, 3] - np.arange(self.n_tokens)).sum())
-        blocks = _query_blocks(runs, spans, nq // nkv, nkv)
+        if n > MAX_SPAN_TOKENS:
+            raise ValueError(f"at most {MAX_SPAN_TOKENS} tokens (got {n})")
+        self.n_tokens, self.nq, self.nkv = n, int(nq), int(nkv)
+        self.n_pairs = int((spans[:, 3] - np.arange(n)).sum())
+        blocks = _query_blocks(runs, spans, nq, nkv)
         items, joins, self.n_slots = _split_items(blocks, blocks[:, _TE], _fwd_tiles(blocks))
         blocks = np.concatenate([_key_blocks(key_runs, spans, nq // nkv, nkv), blocks])
         cost = blocks[:, _TE] * _TILE_COST[blocks[:, _KIND]]
         items_b, joins_b, self.n_units = _split_items(blocks, cost, _bwd_cost(cost))
-        i32 = dict(dtype=torch.int32, device=device)
-        self.spans = torch.tensor(spans, **i32)
-        self.positions = torch.tensor(positions, **i32)
-        self.items, self.joins = torch.tensor(items, **i32), torch.tensor(joins, **i32)
-        self.items_bwd, self.joins_bwd = torch.tensor(items_b, **i32), torch.tensor(joins_b, **i32)
+        lib = _lib.lib()
+        self.fwd_bytes = lib.dk_attn_span_workspace(self.n_slots)
+        self.bwd_bytes = lib.dk_attn_span_bwd_workspace(self.n_units)
+        # one copy to the device, every table 16-byte aligned in it
+        tables = (spans, items, joins, items_b, joins_b, positions)
+        ends = np.cumsum([t.size + -t.size % 4 for t in tables])
+        flat = np.zeros(int(ends[-1]), np.int32)
+        for t, end in zip(tables, ends):
+            end -= t.size + -t.size % 4
+            flat[end:end + t.size] = t.reshape(-1)
+        flat = torch.from_numpy(flat).to(device)
+        (self.spans, self.items, self.joins, self.items_bwd, self.joins_bwd, self.positions) = (
+            flat[end - (t.size + -t.size % 4):][:t.size].view(t.shape) for t, end in zip(tables, ends))
 
 
-MAX_SPAN_TOKENS = 1 << 30
+MAX_SPAN_TOKENS = (1 << 30) - 1
 _KEYS = 64            # keys of a tile
 _ROWS = 128           # stacked query rows of a block
+_REACH = 0xfff00000   # DK_ATTN_SPAN_REACH_BYTES
 # columns of an item (include/dk.h)
 _T0, _PHASE, _N_ROWS, _G, _A0, _NA, _B0, _NK, _F0, _F1, _F2, _TB, _TE, _SLOT, _KIND = range(15)
 _QEND = 4             # of a block of keys
@@ -177,48 +190,65 @@ _QEND = 4             # of a block of keys
 _TILE_COST = np.array([3, 4, 2])
 
 
-def _query_blocks(runs, spans, gin, nkv):
-    """The blocks of stacked query rows of every run of tokens (all with the same [a0, a1) and with kbeg
-    and kend that do not fall) and every KV head, as items [n, 16] that walk all of their tiles."""
-    parts = []
-    for r0, r1 in runs:
-        j0 = np.arange(0, (r1 - r0) * gin, _ROWS, dtype=np.int64)
-        rows = np.minimum(_ROWS, (r1 - r0) * gin - j0)
-        t0, last = r0 + j0 // gin, r0 + (j0 + rows - 1) // gin
-        a0, a1, kbeg = (spans[t0, i] for i in range(3))
-        # the window of the first row meets the sinks: one run of keys from a0
-        one = (a1 > a0) & (kbeg <= a1)
-        na = np.where(one | (a1 <= a0), 0, a1 - a0)
-        b0 = np.where(one, a0, kbeg)
-        nk = na + last + 1 - b0
-        # every row sees the first run, and of the second the keys from the last row's kbeg to t0
-        lo = np.maximum(spans[last, 2], b0) - b0 + na
-        hi = t0 - b0 + na + 1
-        x = np.zeros((j0.size, 16), np.int64)
-        x[:, _T0], x[:, _PHASE], x[:, _N_ROWS] = t0, j0 % gin, rows
-        x[:, _A0], x[:, _NA], x[:, _B0], x[:, _NK] = a0, na, b0, nk
-        x[:, _F0] = np.where(lo == na, hi, na) // _KEYS
-        x[:, _F1] = -(-lo // _KEYS)
-        x[:, _F2] = np.maximum(hi // _KEYS, x[:, _F1])
-        x[:, _TE], x[:, _SLOT] = -(-nk // _KEYS), -1
-        parts += [x + np.eye(1, 16, _G, dtype=np.int64) * g for g in range(nkv)]
-    return np.concatenate(parts) if parts else np.empty((0, 16), np.int64)
+def _blocks_of(runs, per_token, size):
+    """(run, first) of every block of `size` of each run's per_token elements per token."""
+    n = -(-(runs[1] - runs[0]) * per_token // size)
+    run = np.repeat(np.arange(n.size), n)
+    return run, (np.arange(run.size) - np.repeat(np.cumsum(n) - n, n)) * size
+
+
+def _each_head(x, nkv):
+    """The items x for every KV head."""
+    y = np.tile(x, (nkv, 1))
+    y[:, _G] = np.repeat(np.arange(nkv), len(x))
+    return y
+
+
+def _query_blocks(runs, spans, nq, nkv):
+    """The blocks of stacked query rows of every run and KV head, as items [n, 16] that walk all of their
+    tiles."""
+    gin, row_bytes = nq // nkv, 2 * HEAD_DIM * (nq + 2 * nkv)
+    run, j0 = _blocks_of(runs, gin, _ROWS)
+    r0, r1 = runs[0][run], runs[1][run]
+    rows = np.minimum(_ROWS, (r1 - r0) * gin - j0)
+    t0, last = r0 + j0 // gin, r0 + (j0 + rows - 1) // gin
+    a0, a1, kbeg = (spans[t0, i] for i in range(3))
+    # the window of the first row meets the sinks: one run of keys from a0
+    one = (a1 > a0) & (kbeg <= a1)
+    b0 = np.where(one, a0, kbeg)
+    seen = np.where(one | (a1 <= a0), 0, a1 - a0)
+    # A tile of both runs' keys needs them within the kernels' 32-bit offsets.  Beyond, the first run
+    # goes on to the end of its tile: keys that no row of the block sees.
+    far = (b0 - a0 - seen + _KEYS) * row_bytes >= _REACH
+    na = np.where(far, -(-seen // _KEYS) * _KEYS, seen)
+    if (a0 + na > b0)[far].any():
+        raise ValueError(f"rows of {row_bytes} bytes are too long for keys that far apart")
+    nk = na + last + 1 - b0
+    # every row sees the first run, and of the second the keys from the last row's kbeg to t0
+    lo = np.maximum(spans[last, 2], b0) - b0 + na
+    hi = t0 - b0 + na + 1
+    x = np.zeros((j0.size, 16), np.int64)
+    x[:, _T0], x[:, _PHASE], x[:, _N_ROWS] = t0, j0 % gin, rows
+    x[:, _A0], x[:, _NA], x[:, _B0], x[:, _NK] = a0, na, b0, nk
+    x[:, _F0] = np.where((lo == na) & (na == seen), hi, seen) // _KEYS
+    x[:, _F1] = -(-lo // _KEYS)
+    x[:, _F2] = np.maximum(hi // _KEYS, x[:, _F1])
+    x[:, _TE], x[:, _SLOT] = -(-nk // _KEYS), -1
+    return _each_head(x, nkv)
 
 
 def _key_blocks(key_runs, spans, gin, nkv):
-    """The blocks of keys of every run (with kend that does not fall) and KV head, as items whose walk
-    over the group's heads and their queries is whole."""
-    parts = []
-    for r0, r1 in key_runs:
-        k0 = np.arange(r0, r1, _ROWS, dtype=np.int64)
-        nk = np.minimum(_ROWS, r1 - k0)
-        x = np.zeros((k0.size, 16), np.int64)
-        x[:, _T0], x[:, _N_ROWS], x[:, _SLOT] = k0, nk, -1
-        x[:, _KIND] = np.where(nk <= 32, 2, 1)     # few keys (sinks): the walk of 32
-        x[:, _QEND] = spans[k0 + nk - 1, 3]
-        x[:, _TE] = gin * -(-(x[:, _QEND] - k0) // _KEYS)
-        parts += [x + np.eye(1, 16, _G, dtype=np.int64) * g for g in range(nkv)]
-    return np.concatenate(parts) if parts else np.empty((0, 16), np.int64)
+    """The blocks of keys of every run and KV head, as items whose walk over the group's heads and their
+    queries is whole."""
+    run, k0 = _blocks_of(key_runs, 1, _ROWS)
+    k0 = k0 + key_runs[0][run]
+    nk = np.minimum(_ROWS, key_runs[1][run] - k0)
+    x = np.zeros((k0.size, 16), np.int64)
+    x[:, _T0], x[:, _N_ROWS], x[:, _SLOT] = k0, nk, -1
+    x[:, _KIND] = np.where(nk <= 32, 2, 1)     # few keys (sinks): the walk of 32
+    x[:, _QEND] = spans[k0 + nk - 1, 3]
+    x[:, _TE] = gin * -(-(x[:, _QEND] - k0) // _KEYS)
+    return _each_head(x, nkv)
 
 
 def _fwd_tiles(blocks):
@@ -256,6 +286,11 @@ def _split_items(blocks, cost, most):
     return items[order], joins, int(units.sum())
 
 
+def _runs(first, last):
+    """The runs that hold tokens, of arrays of first and past-the-last tokens."""
+    some = last > first
+    return first[some], last[some]
+
 
 def _lengths(lens, what):
     lens = [int(n) for n in lens]
@@ -281,34 +316,36 @@ def window_meta(lens, window, sinks, nq, nkv, device):
     spans[:, 1] = np.minimum(s0 + sinks, end)
     spans[:, 2] = np.maximum(s0, m - (window - 1))
     spans[:, 3] = np.where(m - s0 < sinks, end, np.minimum(m + window, end))
-    runs = [(int(a), int(a + n)) for a, n in zip(start, size) if n]
-    key_runs = [r for a, b in runs for r in ((a, min(a + sinks, b)), (a + sinks, b)) if r[1] > r[0]]
-    return SpanMeta(runs, key_runs, spans, m - s0, nq, nkv, device)
+    last = start + size
+    sunk = np.minimum(start + sinks, last)
+    key_runs = _runs(np.concatenate([start, sunk]), np.concatenate([sunk, last]))
+    return SpanMeta(_runs(start, last), key_runs, spans, m - s0, nq, nkv, device)
 
 
 def prefix_meta(groups, nq, nkv, device):
     """Plan of a packed batch of groups (prompt length, [answer lengths]), packed as the prompt's tokens
     and then each answer's (zeros allowed).  Prompt tokens are causal; an answer's token sees the
     group's whole prompt and its own answer up to itself, and nothing of the other answers."""
-    spans, positions, runs, g0 = [], [], [], 0
+    size, lead = [], []        # the pieces' lengths; 1 at a prompt
     for prompt, answers in groups:
-        prompt, answers = _lengths([prompt], "prompt lengths")[0], _lengths(answers, "answer lengths")
-        size = np.asarray([prompt] + answers, np.int64)
-        start = g0 + np.cumsum(size) - size
-        end = g0 + int(size.sum())
-        sp = np.empty((end - g0, 4), np.int64)
-        sp[:, 0] = g0
-        sp[:prompt, 1], sp[prompt:, 1] = g0, g0 + prompt
-        sp[:, 2] = np.repeat(start, size)
-        sp[:prompt, 3], sp[prompt:, 3] = end, np.repeat(start + size, size)[prompt:]
-        pos = np.arange(g0, end) - sp[:, 2]
-        pos[prompt:] += prompt
-        spans.append(sp)
-        positions.append(pos)
-        runs += [r for r in ((g0, g0 + prompt), (g0 + prompt, end)) if r[1] > r[0]]
-        g0 = end
-    spans = np.concatenate(spans) if spans else np.empty((0, 4), np.int64)
-    positions = np.concatenate(positions) if positions else np.empty(0, np.int64)
+        size += _lengths([prompt], "prompt lengths") + _lengths(answers, "answer lengths")
+        lead += [1] + [0] * (len(size) - len(lead) - 1)
+    size, lead = np.asarray(size, np.int64), np.asarray(lead, np.int64)
+    start = np.cumsum(size) - size
+    group = np.cumsum(lead) - 1
+    at = np.nonzero(lead)[0]                                   # the prompts
+    g0, p1 = start[at], start[at] + size[at]                   # group and prompt ends
+    g1 = np.append(g0[1:], size.sum())[:g0.size]
+    piece = np.repeat(np.arange(size.size), size)
+    g, is_prompt = group[piece], lead[piece] == 1
+    m = np.arange(size.sum(), dtype=np.int64)
+    spans = np.empty((m.size, 4), np.int64)
+    spans[:, 0] = g0[g]
+    spans[:, 1] = np.where(is_prompt, g0[g], p1[g])
+    spans[:, 2] = start[piece]
+    spans[:, 3] = np.where(is_prompt, g1[g], (start + size)[piece])
+    positions = m - start[piece] + np.where(is_prompt, 0, size[at][g])
+    runs = _runs(np.concatenate([g0, p1]), np.concatenate([p1, g1]))
     return SpanMeta(runs, runs, spans, positions, nq, nkv, device)
 
 
@@ -322,6 +359,16 @@ def _check_span(qkv, meta, nq, nkv, hd):
         raise ValueError(f"the plan is on {meta.spans.device}, qkv on {qkv.device}")
 
 
+def _launch(dev, entry, what, *args):
+    """The C entry point on dev's current stream, with dev the current device."""
+    if torch.cuda.current_device() == dev.index:
+        rc = entry(*args, _lib.stream_handle(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, _lib.stream_handle(dev))
+    _lib.check(rc, what)
+
+
 def span_attention_forward(qkv, meta, nq, nkv, hd):
     """(out [N, nq hd] fp16, lse [nq, N] fp32) of the attention whose plan is `meta`; layouts as for
     attention_forward."""
@@ -329,15 +376,10 @@ def span_attention_forward(qkv, meta, nq, nkv, hd):
     n, dev = meta.n_tokens, qkv.device
     out = torch.empty((n, nq * hd), dtype=torch.float16, device=dev)
     lse = torch.empty((nq, n), dtype=torch.float32, device=dev)
-    nbytes = _lib.lib().dk_attn_span_workspace(meta.n_slots)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with torch.cuda.device(dev):
-        rc = _lib.lib().dk_attn_span_fwd(_lib.ptr(qkv), _lib.ptr(meta.spans), _lib.ptr(meta.items),
-                                         meta.items.shape[0], _lib.ptr(meta.joins),
-                                         meta.joins.shape[0], meta.n_slots, n, nq, nkv, hd,
-                                         _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws), nbytes,
-                                         _lib.stream_handle(dev))
-    _lib.check(rc, "dk_attn_span_fwd")
+    ws = torch.empty(meta.fwd_bytes, dtype=torch.uint8, device=dev) if meta.fwd_bytes else None
+    _launch(dev, _lib.lib().dk_attn_span_fwd, "dk_attn_span_fwd", qkv.data_ptr(), meta.spans.data_ptr(),
+            meta.items.data_ptr(), meta.items.shape[0], meta.joins.data_ptr(), meta.joins.shape[0],
+            meta.n_slots, n, nq, nkv, hd, out.data_ptr(), lse.data_ptr(), _lib.ptr(ws), meta.fwd_bytes)
     return out, lse
 
 
@@ -356,16 +398,12 @@ def span_attention_backward(qkv, out, lse, dout, meta, nq, nkv, hd):
     dq = torch.empty((n, nq * hd), dtype=torch.float16, device=dev)
     dk = torch.empty((n, nkv * hd), dtype=torch.float16, device=dev)
     dv = torch.empty((n, nkv * hd), dtype=torch.float16, device=dev)
-    nbytes = _lib.lib().dk_attn_span_bwd_workspace(meta.n_units)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with torch.cuda.device(dev):
-        rc = _lib.lib().dk_attn_span_bwd(_lib.ptr(qkv), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(dout),
-                                         _lib.ptr(meta.spans), _lib.ptr(meta.items_bwd),
-                                         meta.items_bwd.shape[0], _lib.ptr(meta.joins_bwd),
-                                         meta.joins_bwd.shape[0], meta.n_units, n, nq, nkv, hd,
-                                         _lib.ptr(delta), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
-                                         _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
-    _lib.check(rc, "dk_attn_span_bwd")
+    ws = torch.empty(meta.bwd_bytes, dtype=torch.uint8, device=dev) if meta.bwd_bytes else None
+    _launch(dev, _lib.lib().dk_attn_span_bwd, "dk_attn_span_bwd", qkv.data_ptr(), out.data_ptr(),
+            lse.data_ptr(), dout.data_ptr(), meta.spans.data_ptr(), meta.items_bwd.data_ptr(),
+            meta.items_bwd.shape[0], meta.joins_bwd.data_ptr(), meta.joins_bwd.shape[0], meta.n_units, n,
+            nq, nkv, hd, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws),
+            meta.bwd_bytes)
     return dq, dk, dv
 
 

@@ -180,8 +180,8 @@ int dk_attn_bwd(const void* qkv, const void* out, const float* lse, const void* 
  * joins [n_joins][8] int32 put together: t0, phase, rows, g, first slot, slots, 0, 0.  An entry that
  * names rows outside the batch or slots outside the workspace is skipped. */
 #define DK_ATTN_SPAN_ITEM_INTS 16
-/* The keys of both runs of an item lie within this many bytes of qkv rows (an item whose do not is
- * skipped, too). */
+/* A tile with keys of both runs has them within this many bytes of qkv rows (an item that does not is
+ * skipped, too; one whose na is a multiple of 64 has no such tile). */
 #define DK_ATTN_SPAN_REACH_BYTES 0xfff00000u
 #define DK_ATTN_SPAN_JOIN_INTS 8
 int64_t dk_attn_span_workspace(int64_t n_slots);

@@ -124,6 +124,82 @@ def test_walks_cut_in_parts(torch, monkeypatch, spec, nq, nkv, tiles):
     _check(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv))
 
 
+@pytest.mark.parametrize("spec,nq,nkv", [CASES[i] for i in (3, 5, 6, 9, 15)])
+def test_runs_of_keys_too_far_apart_for_a_tile(torch, monkeypatch, spec, nq, nkv):
+    """The plan of sinks or prompts more than 4 GiB of rows before the window or answer."""
+    from decentrik_prime_amd import k_attn
+    monkeypatch.setattr(k_attn, "_REACH", 127 * 2 * HD * (nq + 2 * nkv))
+    meta = _meta(spec, nq, nkv)
+    assert bool(((meta.items[:, 5] > 0) & (meta.items[:, 5] % 64 == 0)).any())
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=meta.n_tokens + nq)
+    _check(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv))
+
+
+def test_table_entries_that_name_no_rows_are_skipped(torch):
+    """Items and joins outside the batch, the heads or the workspace change nothing."""
+    nq, nkv = 4, 2
+    meta = _meta(("window", [300, 77], 90, 3), nq, nkv)
+    n = meta.n_tokens
+    qkv, dout = _inputs(torch, n, nq, nkv, seed=9)
+    want = _run(qkv, dout, meta, nq, nkv)
+
+    def entries(width, rows):
+        return torch.tensor([r + [0] * (width - len(r)) for r in rows], dtype=torch.int32, device="cuda")
+    query = [[n, 0, 1, 0, 0, 0, 0, 1, 0, 0, 0, 0, 1, -1], [-1, 0, 1, 0, 0, 0, 0, 1, 0, 0, 0, 0, 1, -1],
+             [n - 1, 0, 128, 0, 0, 0, 0, 5, 0, 0, 0, 0, 1, -1], [0, 0, 1, nkv, 0, 0, 0, 1, 0, 0, 0, 0, 1, -1],
+             [0, 2, 1, 0, 0, 0, 0, 1, 0, 0, 0, 0, 1, -1], [0, 0, 0, 0, 0, 0, 0, 1, 0, 0, 0, 0, 1, -1],
+             [0, 0, 1, 0, 0, 0, n, 1, 0, 0, 0, 0, 1, -1], [0, 0, 1, 0, 0, 0, 0, 1, 0, 0, 0, 0, 2, -1],
+             [0, 0, 1, 0, 0, 0, 0, 1, 0, 0, 0, 1, 1, -1], [0, 0, 1, 0, 0, 0, 0, 1, 0, 0, 0, 0, 1, 1 << 20],
+             [0, 0, 1, 0, -1, 3, 5, 4, 0, 0, 0, 0, 1, -1], [0, 0, 1, 0, 4, 3, 5, 4, 0, 0, 0, 0, 1, -1]]
+    keys = [[n, 0, 1, 0, n + 1, 0, 0, 0, 0, 0, 0, 0, 1, -1], [0, 0, 129, 0, n, 0, 0, 0, 0, 0, 0, 0, 1, -1],
+            [0, 0, 1, 0, n + 1, 0, 0, 0, 0, 0, 0, 0, 1, -1], [5, 0, 1, 0, 5, 0, 0, 0, 0, 0, 0, 0, 1, -1],
+            [0, 0, 1, 0, 64, 0, 0, 0, 0, 0, 0, 0, 3, -1], [0, 0, 1, 0, 64, 0, 0, 0, 0, 0, 0, 0, 1, 1 << 20],
+            [0, 0, 1, -1, 64, 0, 0, 0, 0, 0, 0, 0, 1, -1]]
+    joins = [[n, 0, 1, 0, 0, 1], [0, 0, 1, 0, -1, 1], [0, 0, 1, 0, 0, 1 << 20], [0, 2, 1, 0, 0, 1],
+             [0, 0, 129, 0, 0, 1], [0, 0, 1, 0, 1 << 20, 1], [0, 0, 1, 0, 0, 0]]
+    bad = entries(16, query + [k + [kind] for k in keys + [[0, 0, 33, 0, n, 0, 0, 0, 0, 0, 0, 0, 1, -1]]
+                               for kind in ((2,) if k[2] == 33 else (1, 2))])
+    meta.items = torch.cat([entries(16, query), meta.items])
+    meta.joins = torch.cat([meta.joins, entries(8, joins)])
+    meta.items_bwd = torch.cat([bad, meta.items_bwd])
+    meta.joins_bwd = torch.cat([meta.joins_bwd, entries(8, joins + [j[:6] + [1] for j in joins if j[1] == 0])])
+    for a, b in zip(_run(qkv, dout, meta, nq, nkv), want):
+        assert torch.equal(a, b)
+
+
+def test_many_short_sequences(torch):
+    """2^17 sequences of one token and 2^14 answers of one token to a prompt of one: a key or two each."""
+    from decentrik_prime_amd import k_attn
+    nq, nkv = 4, 1
+    n = 1 << 17
+    log(f"span attention, {n} one-token sequences")
+    qkv, dout = _inputs(torch, n, nq, nkv, seed=4)
+    got = _run(qkv, dout, k_attn.window_meta([1] * n, 5, 1, nq, nkv, "cuda"), nq, nkv)
+    v = qkv[:, (nq + 1) * HD:]
+    assert torch.equal(got[0].view(n, nq, HD), v[:, None].expand(-1, nq, -1))
+    # dS = P (dO V - out dO): 0 but for the two sums' rounding, HD 2^-24 of their magnitudes, twice
+    mag = (dout.view(n, nq, HD).double().abs() * v[:, None].double().abs()).sum(2)
+    lim = 2 * HD * 2.0 ** -24 * mag.amax() * 8 * HD ** -0.5 * nq
+    assert float(got[2].abs().max()) <= lim and float(got[3].abs().max()) <= lim
+    want = dout.view(n, nq, HD).double().sum(1)
+    _near(got[4], want, 2.0 ** -10 * dout.view(n, nq, HD).double().abs().sum(1) + 2.0 ** -11 * want.abs() + 2.0 ** -24, "dv")
+    answers = 1 << 14
+    meta = k_attn.prefix_meta([(1, [1] * answers)], nq, nkv, "cuda")
+    qkv, dout = qkv[:answers + 1].contiguous(), dout[:answers + 1].contiguous()
+    got = _run(qkv, dout, meta, nq, nkv)
+    x = qkv.double().view(-1, nq + 2, HD)
+    k, v = x[:, nq], x[:, nq + 1]
+    s = torch.stack([(x[1:, :nq] @ k[0]), (x[1:, :nq] * k[1:, None]).sum(2)], 2) * HD ** -0.5
+    p = torch.softmax(s, 2)
+    want = p[..., :1] * v[0] + p[..., 1:] * v[1:, None]
+    mag = p[..., :1] * v[0].abs() + p[..., 1:] * v[1:, None].abs()
+    _near(got[0].view(-1, nq, HD)[1:], want, 2.0 ** -10 * mag + 2.0 ** -11 * want.abs() + 2.0 ** -24, "out")
+    do = dout.double().view(-1, nq, HD)
+    want = do[0].sum(0) + (p[..., :1] * do[1:]).sum((0, 1))
+    mag = do[0].abs().sum(0) + (p[..., :1] * do[1:].abs()).sum((0, 1))
+    _near(got[4][0], want, 2.0 ** -10 * mag + 2.0 ** -11 * want.abs(), "dv of the prompt")
+
+
 def test_no_tokens(torch):
     for spec in (("window", [], 4, 1), ("prefix", [(0, [0])])):
         meta = _meta(spec, 4, 2)

@@ -84,6 +84,12 @@ def test_plan_refusals():
             k_attn.prefix_meta(groups, 4, 2, "cpu")
 
 
+def test_plan_refuses_keys_out_of_reach(monkeypatch):
+    monkeypatch.setattr(k_attn, "_REACH", 65 * 2 * HD * (NQ + 2 * NKV))
+    with pytest.raises(ValueError):
+        k_attn.window_meta([300], 100, 3, NQ, NKV, "cpu")
+
+
 def test_call_refusals_before_any_launch():
     meta = k_attn.window_meta([5, 7], 4, 1, NQ, NKV, "cpu")
     qkv = torch.zeros(12, (NQ + 2 * NKV) * HD, dtype=torch.float16)
@@ -107,6 +113,7 @@ def _pairs_of_items(meta, rows_seen):
         for i in range(rows):
             m, e = t0 + (phase + i) // gin, (phase + i) % gin
             seen = (j <= m - b0 + na) & (m < s[key, 3])
+            assert na % 64 == 0 or (b0 - a0 - na + 64) * 2 * HD * (meta.nq + 2 * meta.nkv) < k_attn._REACH
             assert not (full & ~seen).any(), "a tile named full holds a masked key"
             count[g, e, m, key[seen]] += 1
             rows_seen[g * gin + e, m] += slot < 0 or tb == 0
@@ -114,7 +121,11 @@ def _pairs_of_items(meta, rows_seen):
 
 
 @pytest.mark.parametrize("nq,nkv", [(4, 2), (5, 1), (3, 3)])
-def test_items_visit_every_visible_pair_once(nq, nkv):
+@pytest.mark.parametrize("near", [False, True])
+def test_items_visit_every_visible_pair_once(monkeypatch, nq, nkv, near):
+    """near: as if two runs of keys 63 rows apart were too far from each other for one tile."""
+    if near:
+        monkeypatch.setattr(k_attn, "_REACH", 127 * 2 * HD * (nq + 2 * nkv))
     for make, spec in ([(attn.window_visible, w) for w in WINDOWS + [([300, 41], 100, 3), ([260], 30, 90)]] +
                        [(attn.prefix_visible, (g,)) for g in GROUPS + [[(200, [40, 3, 70]), (9, [150])]]]):
         build = k_attn.window_meta if make is attn.window_visible else k_attn.prefix_meta
@@ -127,7 +138,7 @@ def test_items_visit_every_visible_pair_once(nq, nkv):
 
 def test_split_items_cover_the_walks():
     meta = k_attn.window_meta([700, 20], 400, 4, 12, 2, "cpu")
-    blocks = k_attn._query_blocks([(0, 700), (700, 720)], np.asarray(meta.spans, np.int64), 6, 2)
+    blocks = k_attn._query_blocks((np.array([0, 700]), np.array([700, 720])), np.asarray(meta.spans, np.int64), 12, 2)
     for most in (1, 2, 3, 100):
         items, joins, slots = k_attn._split_items(blocks, blocks[:, 12], most)
         assert (items[:, 12] - items[:, 11]).max() <= most and (items[:, 12] > items[:, 11]).all()
