@@ -25,7 +25,6 @@
 
 namespace {
 
-using dk::dma16;
 using dk::dma16s;
 using dk::dma4;
 using dk::lds_addr;

@@ -36,20 +36,6 @@ __device__ __forceinline__ void dma16s(uint64_t base, unsigned off, unsigned lds
       : "memory");
 }
 
-// 16 bytes per lane from an address per lane: for tiles whose rows a 32-bit offset may not reach.
-__device__ __forceinline__ void dma16(const void* src, unsigned lds) {
-  unsigned saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %1\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %2, off\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "s"(lds), "v"(src)
-      : "memory");
-}
-
 // 4 bytes per lane from global memory (an address per lane) into LDS at lds + 4 * lane.
 __device__ __forceinline__ void dma4(const void* src, unsigned lds) {
   unsigned saved;

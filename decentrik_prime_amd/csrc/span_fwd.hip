@@ -1,6 +1,8 @@
-// Forward of the attention over part of the keys (attn_span.h): an online softmax in the exp2 domain
-// over the key tiles of each block of stacked query rows.  Built with the MFMA accumulators in VGPRs
-// like attn_fwd.hip.
+// Forward of the attention over part of the keys (attn_span.h): with s = scale q . k over the keys that a
+// row sees (log2 units), m = max s, l = sum 2^(s - m): out = sum 2^(s - m) v / l, lse = m + log2 l, m and
+// l running over the tiles.  P is rounded to fp16 for its product (half a step, 2^-11 of each value; the
+// sum l takes it unrounded), everything else is fp32 up to the one rounding of out.  Built with the MFMA
+// accumulators in VGPRs like attn_fwd.hip.
 #include "attn_span.h"
 
 namespace {
@@ -28,10 +30,21 @@ __device__ __forceinline__ void redo_rows(const SpanArgs& a, int t0, int phase, 
   }
 }
 
-__global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, const int32_t* __restrict__ items,
-                                                             int n_slots, f16* __restrict__ out,
-                                                             float* __restrict__ lse,
-                                                             float* __restrict__ parts) {
+// A workgroup per item: 4 waves of 32 stacked rows, lane l % 32 a row, over 64-key tiles.
+//
+// Bound: per tile a wave has 32 MFMAs (1024 clocks), about as many clocks of exponentials and
+// conversions, and 48 LDS operand reads, one after the other for a wave on its own.  So the scores of
+// the next tile stand beside the exponentials of the current one (K runs a tile ahead of V), and a CU
+// holds two workgroups (two stages of K and V, 66 KB; 254 registers), whose first loads, barriers and
+// stores stand beside the other's products.  Stacking a group's heads on the rows makes a block span
+// 128 / gin tokens: fewer masked keys at a window's edges, and answers of a token fill blocks.
+// Measured on MI355X, 12 query / 2 KV heads (graph replays): 16384 tokens, window 4096, 4 sinks 427 us
+// (846 TFLOP/s); 8192 tokens, window 1024, 87; a prompt of 8192 with 64 answers of a token 257; one
+// workgroup of 8 waves to a CU, the waves of a SIMD on alternate tiles, took 500, 100 and 302.
+// Walks are cut where one would outlast the rest (k_attn._fwd_tiles): that prompt uncut 360 us.
+__global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
+    SpanArgs a, const int32_t* __restrict__ items, int n_slots, f16* __restrict__ out,
+    float* __restrict__ lse, float* __restrict__ parts) {
   SpanItem it;
   if (!span_item(a, items, (int)blockIdx.x, n_slots, &it)) return;
   const int lane = threadIdx.x & 63, hl = lane >> 5, c = lane & 31;
@@ -99,9 +112,9 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, cons
   scores(sc, 0);
   __syncthreads();   // every wave is done with K of tile 0
   // tile t, whose scores are in sc: its softmax and O^T += V^T P^T, beside the scores of tile t + 1
-  // into sn when there is one.  MASK: key j of the tile counts iff j <= jlim and the key's end lies
-  // past this lane's token; the others' probabilities are set to 0 (a lane may see none of a tile's
-  // keys before its first).
+  // into sn (after the last tile: of a stale stage, never used).  MASK: key j of the tile counts iff
+  // j <= jlim and the key's end lies past this lane's token; the others' probabilities are set to 0
+  // (a lane may see none of a tile's keys before its first).
   auto tile = [&](int t, f32x16 (&sc)[2], f32x16 (&sn)[2], auto mask_c) {
     constexpr bool MASK = decltype(mask_c)::value;
     const unsigned va = fresh(vcol + (unsigned)((t % kStages) * kTileHalves * 2));
@@ -191,6 +204,7 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(SpanArgs a, cons
     wait_vmem<0>();
     __syncthreads();
   };
+  // seen whole by every row (and not the last: without that test the compiler spilled registers)
   auto full = [&](int t) { return t + 1 < n_tiles && full_tile(it, it.tb + t); };
   int t = 0;
   while (t < n_tiles) {

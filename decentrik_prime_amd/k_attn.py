@@ -307,6 +307,7 @@ def window_meta(lens, window, sinks, nq, nkv, device):
     window, sinks = int(window), int(sinks)
     if window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 and sinks at least 0 (got {window}, {sinks})")
+    window, sinks = min(window, sum(lens) + 1), min(sinks, sum(lens))
     size = np.asarray(lens, np.int64)
     start = np.cumsum(size) - size
     s0, end = np.repeat(start, size), np.repeat(start + size, size)

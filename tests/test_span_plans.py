@@ -13,7 +13,7 @@ from oracle import attn
 
 NQ, NKV, HD = 4, 2, 128
 WINDOWS = [([1], 1, 0), ([5, 0, 3], 1, 0), ([40], 7, 3), ([17, 64, 1, 30], 16, 0), ([50, 9], 8, 60),
-           ([33, 70], 1000, 4), ([90], 1, 1), ([0], 4, 4)]
+           ([33, 70], 1 << 70, 4), ([90], 1, 1), ([0], 4, 4), ([30], 5, 1 << 70)]
 GROUPS = [[(5, [1])], [(0, [1])], [(0, [7, 3])], [(12, [])], [(12, [0, 0])], [(30, [4, 0, 9, 1]), (0, [6]),
           (1, [1, 1, 1])], [(64, [64, 64])], []]
 
@@ -183,3 +183,37 @@ def test_key_items_visit_every_visible_pair_once(nq, nkv):
                 count[g * gin + t // per_head, q, k] += (q >= k) & (q < s[k, 3])
         assert (rows == 1).all() and len(units) == meta.n_units
         assert (count == make(*spec)[None]).all()
+
+
+def test_c_entry_refusals_before_any_launch():
+    lib, p, odd = _lib.lib(), ctypes.c_void_p(256), ctypes.c_void_p(8)
+
+    def fwd(qkv=p, spans=p, items=p, n_items=1, joins=p, n_joins=0, n_slots=0, n=4, nq=4, nkv=2, hd=128,
+            out=p, lse=p, ws=None, nbytes=0):
+        return lib.dk_attn_span_fwd(qkv, spans, items, n_items, joins, n_joins, n_slots, n, nq, nkv, hd, out,
+                                    lse, ws, nbytes, None)
+
+    def bwd(qkv=p, out=p, lse=p, dout=p, spans=p, items=p, n_items=1, joins=p, n_joins=0, n_units=0, n=4, nq=4,
+            nkv=2, hd=128, delta=p, dq=p, dk=p, dv=p, ws=None, nbytes=0):
+        return lib.dk_attn_span_bwd(qkv, out, lse, dout, spans, items, n_items, joins, n_joins, n_units, n, nq,
+                                    nkv, hd, delta, dq, dk, dv, ws, nbytes, None)
+    both = [dict(hd=64), dict(nq=3), dict(nkv=0), dict(nq=0), dict(nq=65536, nkv=1), dict(n=-1),
+            dict(n=1 << 31), dict(qkv=None), dict(spans=None), dict(items=None), dict(n_items=-1),
+            dict(n_joins=-1), dict(n_joins=1, joins=None), dict(out=None), dict(lse=None),
+            dict(n_items=1 << 30), dict(n_joins=1 << 30)]
+    for call, more in ((fwd, [dict(n_slots=-1)]),
+                       (bwd, [dict(n_units=-1)] + [{k: None} for k in ("dout", "delta", "dq", "dk", "dv")])):
+        for bad in both + more:
+            assert call(**bad) == _lib.DK_ERR_INVALID, bad
+        for k in ("qkv", "spans", "out") + (("dout", "dq", "dk", "dv") if call is bwd else ()):
+            assert call(**{k: odd}) == _lib.DK_ERR_ALIGN, k
+        assert call(ws=odd) == _lib.DK_ERR_ALIGN
+        assert call(n=0, qkv=None, spans=None, items=None, out=None, lse=None) == 0
+    for slots in (1, 3):
+        need = lib.dk_attn_span_workspace(slots)
+        assert need == slots * (128 * 128 + 256) * 4
+        assert fwd(n_slots=slots) == fwd(n_slots=slots, ws=p, nbytes=need - 1) == _lib.DK_ERR_WORKSPACE
+        need = lib.dk_attn_span_bwd_workspace(slots)
+        assert need == slots * 128 * 128 * 4
+        assert bwd(n_units=slots) == bwd(n_units=slots, ws=p, nbytes=need - 1) == _lib.DK_ERR_WORKSPACE
+    assert lib.dk_attn_span_workspace(0) == lib.dk_attn_span_bwd_workspace(0) == 0
