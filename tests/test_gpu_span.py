@@ -200,6 +200,62 @@ def test_many_short_sequences(torch):
     _near(got[4][0], want, 2.0 ** -10 * mag + 2.0 ** -11 * want.abs(), "dv of the prompt")
 
 
+def test_rows_past_four_gigabytes(torch):
+    """A sequence of 4.6 GB of qkv rows: sinks further from the window than a 32-bit offset reaches.  The
+    last rows and keys against their own definition."""
+    from decentrik_prime_amd import k_attn
+    nq, nkv, window, sinks = 12, 2, 70, 5
+    n = (1 << 32) // (2 * HD * (nq + 2 * nkv)) + 70000
+    log(f"span attention, one sequence of {n} tokens")
+    meta = k_attn.window_meta([n], window, sinks, nq, nkv, "cuda")
+    far = meta.items[:, 5] == 64
+    assert bool(far.any()) and bool((meta.items[:, 5] == sinks).any())
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    qkv = torch.randn(n, (nq + 2 * nkv) * HD, device="cuda", generator=g, dtype=torch.float16)
+    dout = torch.randn(n, nq * HD, device="cuda", generator=g, dtype=torch.float16)
+    out, lse, dq, dk, dv = _run(qkv, dout, meta, nq, nkv)
+    for t in (out, lse, dq, dk, dv):
+        assert bool(torch.isfinite(t[-1000:] if t.shape[0] == n else t).all())
+    # the last 300 queries, and the last 300 - window keys, whose queries are all among them
+    rows = 300
+    m = torch.arange(n - rows, n, device="cuda")
+    cols = torch.cat([torch.arange(sinks, device="cuda"), torch.arange(n - rows - window, n, device="cuda")])
+    vis = (cols[None] <= m[:, None]) & ((m[:, None] - cols[None] < window) | (cols[None] < sinks))
+    x = qkv[cols].double().view(cols.numel(), nq + 2 * nkv, HD)
+    q_all = qkv[m].double().view(rows, nq + 2 * nkv, HD)
+    gk, gv = (torch.zeros(cols.numel(), nkv, HD, dtype=torch.float64, device="cuda") for _ in range(2))
+    lk, lv = torch.zeros_like(gk), torch.zeros_like(gk)
+    sm = HD ** -0.5
+    for h in range(nq):
+        kv = h // (nq // nkv)
+        q, k, v = q_all[:, h], x[:, nq + kv], x[:, nq + nkv + kv]
+        do = dout[m].double().view(rows, nq, HD)[:, h]
+        sc = torch.where(vis, sm * (q @ k.t()), -float("inf"))
+        p = torch.softmax(sc, 1)
+        o = p @ v
+        dl = (o * do).sum(1, keepdim=True)
+        ds = p * (do @ v.t() - dl)
+        # the tolerances of _check
+        lo = 2.0 ** -10 * (p @ v.abs()) + 2.0 ** -11 * o.abs() + 2.0 ** -24
+        eds = torch.where(vis, 2.0 ** -10 * ds.abs() + 2.0 ** -25 + HD * 2.0 ** -23 * p * (
+            do.abs() @ v.abs().t() + (o * do).abs().sum(1, keepdim=True)) +
+            (lo * do.abs()).sum(1, keepdim=True) * p, 0.0)
+        _near(out[m].view(rows, nq, HD)[:, h], o, lo, f"head {h}: out")
+        _near(lse[h, m], torch.logsumexp(sc, 1) / math.log(2.0), 2.0 ** -12, f"head {h}: lse")
+        want = sm * (ds @ k)
+        _near(dq[m].view(rows, nq, HD)[:, h], want, sm * (eds @ k.abs()) + 2.0 ** -11 * want.abs() + 2.0 ** -24,
+              f"head {h}: dq")
+        gk[:, kv] += sm * (ds.t() @ q)
+        lk[:, kv] += sm * (eds.t() @ q.abs())
+        gv[:, kv] += p.t() @ do
+        lv[:, kv] += torch.where(vis, 2.0 ** -10 * p + 2.0 ** -25, 0.0).t() @ do.abs()
+    own = slice(sinks + window + window, None)
+    for t, w, lim, what in ((dk, gk, lk, "dk"), (dv, gv, lv, "dv")):
+        t = t[cols[own]].view(-1, nkv, HD)
+        _near(t, w[own], lim[own] + 2.0 ** -11 * w[own].abs() + 2.0 ** -24, what)
+
+
 def test_no_tokens(torch):
     for spec in (("window", [], 4, 1), ("prefix", [(0, [0])])):
         meta = _meta(spec, 4, 2)
