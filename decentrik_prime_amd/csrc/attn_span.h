@@ -123,7 +123,9 @@ __device__ __forceinline__ f32x4 quad(const f32x16& x, int q) {
 }
 
 // One query row or one key row at a time, a wave each, over exactly the keys (or queries) that it
-// sees: nothing else is read, so whatever a masked row holds cannot reach the result.
+// sees: nothing else is read, so whatever a masked row holds cannot reach the result.  Where a token's
+// term with itself, which it always sees, is NaN already, so is the whole row, and the walk is spared: a
+// batch of nothing but NaN (a diverged step) costs no walks.
 struct RowScratch {
   float a[kHD], b[kHD];   // the wave's row (q or k) and its partner (dO or v)
   float p[64], ds[64];
@@ -194,6 +196,13 @@ __device__ __forceinline__ void span_row_fwd(const SpanArgs& a, int64_t m, int h
   wave_sync();
   row_to_lds(s.a, a.qkv + m * ROW + (int64_t)h * kHD);
   wave_sync();
+  f16* orow = out + m * (int64_t)a.nq * kHD + (int64_t)h * kHD + 2 * lane;
+  const float own = __fmul_rn(row_dot(s.a, kb + m * ROW), a.qk_scale);
+  if (own != own || own == INFINITY) {   // 2^(inf - inf)
+    *reinterpret_cast<f16x2*>(orow) = f16x2{(f16)NAN, (f16)NAN};
+    if (lane == 0) lse[(int64_t)h * a.n_tokens + m] = NAN;
+    return;
+  }
   const KeyRuns kr = key_runs(a, m);
   const int64_t n = kr.na + kr.nb;
   float mx = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
@@ -227,7 +236,7 @@ __device__ __forceinline__ void span_row_fwd(const SpanArgs& a, int64_t m, int h
   f16x2 r;
   r[0] = (f16)__fmul_rn(o0, inv);
   r[1] = (f16)__fmul_rn(o1, inv);
-  *reinterpret_cast<f16x2*>(out + m * (int64_t)a.nq * kHD + (int64_t)h * kHD + 2 * lane) = r;
+  *reinterpret_cast<f16x2*>(orow) = r;
   if (lane == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(mx, log2f(l));
 }
 
@@ -245,6 +254,13 @@ __device__ __forceinline__ void span_row_dq(const SpanArgs& a, int64_t m, int h,
   row_to_lds(s.b, dout + m * OROW + (int64_t)h * kHD);
   wave_sync();
   const float lm = lse[(int64_t)h * a.n_tokens + m], dm = delta[(int64_t)h * a.n_tokens + m];
+  f16* grow = dq + m * OROW + (int64_t)h * kHD + 2 * lane;
+  const float own = __fmul_rn(exp2f(__builtin_fmaf(row_dot(s.a, kb + m * ROW), a.qk_scale, -lm)),
+                              __fsub_rn(row_dot(s.b, vb + m * ROW), dm));
+  if (own != own) {
+    *reinterpret_cast<f16x2*>(grow) = f16x2{(f16)NAN, (f16)NAN};
+    return;
+  }
   const KeyRuns kr = key_runs(a, m);
   const int64_t n = kr.na + kr.nb;
   float g0 = 0.0f, g1 = 0.0f;
@@ -268,7 +284,7 @@ __device__ __forceinline__ void span_row_dq(const SpanArgs& a, int64_t m, int h,
   f16x2 r;
   r[0] = (f16)__fmul_rn(g0, a.sm_scale);
   r[1] = (f16)__fmul_rn(g1, a.sm_scale);
-  *reinterpret_cast<f16x2*>(dq + m * OROW + (int64_t)h * kHD + 2 * lane) = r;
+  *reinterpret_cast<f16x2*>(grow) = r;
 }
 
 // dk and dv of key n, KV head g, summed over the queries that see it and the heads of its group
@@ -283,6 +299,25 @@ __device__ __forceinline__ void span_key_dkdv(const SpanArgs& a, int64_t n, int 
   row_to_lds(s.a, krow);
   row_to_lds(s.b, krow + (int64_t)a.nkv * kHD);
   wave_sync();
+  const int64_t off = n * (int64_t)a.nkv * kHD + (int64_t)g * kHD + 2 * lane;
+  // dk is NaN where the token's own dS is, dv where its own P is or, by columns, its own dO
+  bool p_nan = false, ds_nan = false, col0 = false, col1 = false;
+  for (int hh = g * gin; hh < (g + 1) * gin; ++hh) {
+    const f16* orow = dout + n * OROW + (int64_t)hh * kHD;
+    const float p = exp2f(__builtin_fmaf(row_dot(s.a, a.qkv + n * ROW + (int64_t)hh * kHD), a.qk_scale,
+                                         -lse[(int64_t)hh * a.n_tokens + n]));
+    const float ds = __fmul_rn(p, __fsub_rn(row_dot(s.b, orow), delta[(int64_t)hh * a.n_tokens + n]));
+    const f16x2 o = *reinterpret_cast<const f16x2*>(orow + 2 * lane);
+    p_nan |= p != p;
+    ds_nan |= ds != ds;
+    col0 |= o[0] != o[0];
+    col1 |= o[1] != o[1];
+  }
+  if (ds_nan && (p_nan || __builtin_amdgcn_ballot_w64(!(col0 && col1)) == 0)) {
+    *reinterpret_cast<f16x2*>(dk + off) = f16x2{(f16)NAN, (f16)NAN};
+    *reinterpret_cast<f16x2*>(dv + off) = f16x2{(f16)NAN, (f16)NAN};
+    return;
+  }
   const int64_t end = key_end(a, n);
   float dk0 = 0.0f, dk1 = 0.0f, dv0 = 0.0f, dv1 = 0.0f;
   for (int hh = g * gin; hh < (g + 1) * gin; ++hh)
@@ -310,7 +345,6 @@ __device__ __forceinline__ void span_key_dkdv(const SpanArgs& a, int64_t n, int 
         dv1 = __builtin_fmaf(s.p[j], (float)o[1], dv1);
       }
     }
-  const int64_t off = n * (int64_t)a.nkv * kHD + (int64_t)g * kHD + 2 * lane;
   f16x2 r;
   r[0] = (f16)__fmul_rn(dk0, a.sm_scale);
   r[1] = (f16)__fmul_rn(dk1, a.sm_scale);

@@ -337,6 +337,44 @@ def test_unseen_rows_have_no_influence(torch, monkeypatch, spec, bad, clean, val
         assert bool(torch.isnan(got[0][~same]).all())
 
 
+@pytest.mark.parametrize("what", ["all", "q", "k", "v", "dout"])
+def test_batches_of_nothing_but_nan(torch, what):
+    """What the definition makes of a batch whose queries, keys, values or gradients are all NaN."""
+    nq, nkv = 4, 2
+    meta = _meta(("window", [700, 41], 100, 4), nq, nkv)
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=12)
+    cols = {"q": slice(0, nq * HD), "k": slice(nq * HD, (nq + nkv) * HD), "v": slice((nq + nkv) * HD, None)}
+    for name, c in cols.items():
+        if what in (name, "all"):
+            qkv[:, c] = float("nan")
+    if what in ("dout", "all"):
+        dout[:] = float("nan")
+    out, lse, dq, dk, dv = _run(qkv, dout, meta, nq, nkv)
+    nan = lambda t: bool(torch.isnan(t).all())     # noqa: E731
+    finite = lambda t: bool(torch.isfinite(t).all())   # noqa: E731
+    assert finite(out) if what == "dout" else nan(out)
+    assert nan(lse) if what in ("q", "k", "all") else finite(lse)
+    assert nan(dq) and nan(dk)
+    assert finite(dv) if what == "v" else nan(dv)
+
+
+def test_one_column_of_nan_stays_one(torch):
+    """A NaN in one column of every value row and of every gradient row: that column of out and of dv."""
+    nq, nkv = 4, 2
+    meta = _meta(("prefix", [(70, [30, 45])]), nq, nkv)
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=13)
+    want = _run(qkv, dout, meta, nq, nkv)
+    qkv.view(-1, nq + 2 * nkv, HD)[:, nq + nkv:, 5] = float("nan")
+    dout.view(-1, nq, HD)[:, :, 7] = float("nan")
+    got = _run(qkv, dout, meta, nq, nkv)
+    for t, w, heads, col in ((got[0], want[0], nq, 5), (got[4], want[4], nkv, 7)):
+        t, w = t.view(-1, heads, HD), w.view(-1, heads, HD)
+        assert bool(torch.isnan(t[..., col]).all())
+        rest = [c for c in range(HD) if c != col]
+        # the same sums, in another order at the most
+        assert bool(((t - w)[..., rest].double().abs() <= 2.0 ** -9 * w[..., rest].double().abs() + 2.0 ** -9).all())
+
+
 def test_repeats_and_streams(torch):
     """The same bits on every call, on a stream of its own, and on two streams at once."""
     nq, nkv = 12, 2
