@@ -123,45 +123,60 @@ __device__ __forceinline__ f32x4 quad(const f32x16& x, int q) {
 }
 
 // One query row or one key row at a time, a wave each, over exactly the keys (or queries) that it
-// sees: nothing else is read, so whatever a masked row holds cannot reach the result.  Where a token's
-// term with itself, which it always sees, is NaN already, so is the whole row, and the walk is spared: a
-// batch of nothing but NaN (a diverged step) costs no walks.
-struct RowScratch {
-  float a[kHD], b[kHD];   // the wave's row (q or k) and its partner (dO or v)
-  float p[64], ds[64];
+// sees: nothing else is read, so whatever a masked row holds cannot reach the result.  16 lanes hold a
+// row, 8 columns each, so a wave takes four rows of a walk at a time, each quarter sums every fourth,
+// and the loads of kWalk such steps are in flight.  A walk ends where nothing but NaN can come of
+// it; a query's first look is at its term with itself, where a key's walk begins, so a batch of nothing
+// but NaN (a diverged step) costs no walks.
+constexpr int kWalk = 4;
+
+struct Row8 {
+  float x[8];
 };
-
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+__device__ __forceinline__ f16x8 row_load(const f16* row) {
+  return *reinterpret_cast<const f16x8*>(row + 8 * (threadIdx.x & 15));
 }
-
-__device__ __forceinline__ float wave_sum(float v) {
+__device__ __forceinline__ Row8 row8(const f16* row) {
+  const f16x8 v = row_load(row);
+  Row8 r;
 #pragma unroll
-  for (int x = 32; x > 0; x >>= 1) v = __fadd_rn(v, __shfl_xor(v, x));
-  return v;
+  for (int i = 0; i < 8; ++i) r.x[i] = (float)v[i];
+  return r;
 }
-
-__device__ __forceinline__ void row_to_lds(float* dst, const f16* src) {
-  const int lane = threadIdx.x & 63;
-  const f16x2 v = *reinterpret_cast<const f16x2*>(src + 2 * lane);
-  dst[2 * lane] = (float)v[0];
-  dst[2 * lane + 1] = (float)v[1];
+__device__ __forceinline__ void store8(f16* row, const Row8& r) {   // by the first quarter
+  f16x8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (f16)r.x[i];
+  if ((threadIdx.x & 63) < 16) *reinterpret_cast<f16x8*>(row + 8 * (threadIdx.x & 15)) = v;
 }
+__device__ __forceinline__ Row8 fill8(float x) { return Row8{{x, x, x, x, x, x, x, x}}; }
 
-// dot product of a row in LDS with this lane's row in memory
-__device__ __forceinline__ float row_dot(const float* a, const f16* row) {
+// x and its value in another lane of the 16, by a DPP control
+template <int kCtrl>
+__device__ __forceinline__ float add_dpp(float x) {
+  return __fadd_rn(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), kCtrl, 0xf, 0xf, true)));
+}
+// the dot product of the quarter's row with one held the same way: lanes 1 and 2 further in a quad,
+// then the other quad of the half (half mirror) and the other half (mirror), the same sum in every lane
+__device__ __forceinline__ float row_dot(const Row8& a, const f16x8& b) {
   float s = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < kHD / 8; ++i) {
-    const f16x8 x = *reinterpret_cast<const f16x8*>(row + 8 * i);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = __builtin_fmaf(a[8 * i + e], (float)x[e], s);
-  }
-  return s;
+  for (int i = 0; i < 8; ++i) s = __builtin_fmaf(a.x[i], (float)b[i], s);
+  return add_dpp<0x140>(add_dpp<0x141>(add_dpp<0x4e>(add_dpp<0xb1>(s))));
 }
-
+__device__ __forceinline__ void row_add(Row8& r, float w, const f16x8& b) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.x[i] = __builtin_fmaf(w, (float)b[i], r.x[i]);
+}
+// the quarters' sums together, times scale
+__device__ __forceinline__ Row8 row_sum(Row8 r, float scale) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    r.x[i] = __fadd_rn(r.x[i], __shfl_xor(r.x[i], 16));
+    r.x[i] = __fmul_rn(__fadd_rn(r.x[i], __shfl_xor(r.x[i], 32)), scale);
+  }
+  return r;
+}
 // The keys that query m sees, as na keys from a0 and nb from b0 (kept within [0, m] whatever spans
 // holds, so every row read exists).
 struct KeyRuns {
@@ -186,172 +201,161 @@ __device__ __forceinline__ int64_t key_end(const SpanArgs& a, int64_t n) {
 }
 
 // out and lse of query m, head h
-__device__ __forceinline__ void span_row_fwd(const SpanArgs& a, int64_t m, int h, f16* out, float* lse,
-                                          RowScratch& s) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void span_row_fwd(const SpanArgs& a, int64_t m, int h, f16* out, float* lse) {
   const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD;
-  const int kvh = h / (a.nq / a.nkv);
+  const int kvh = h / (a.nq / a.nkv), quarter = (threadIdx.x >> 4) & 3;
   const f16* kb = a.qkv + (int64_t)(a.nq + kvh) * kHD;
   const f16* vb = kb + (int64_t)a.nkv * kHD;
-  wave_sync();
-  row_to_lds(s.a, a.qkv + m * ROW + (int64_t)h * kHD);
-  wave_sync();
-  f16* orow = out + m * (int64_t)a.nq * kHD + (int64_t)h * kHD + 2 * lane;
-  const float own = __fmul_rn(row_dot(s.a, kb + m * ROW), a.qk_scale);
-  if (own != own || own == INFINITY) {   // 2^(inf - inf)
-    *reinterpret_cast<f16x2*>(orow) = f16x2{(f16)NAN, (f16)NAN};
-    if (lane == 0) lse[(int64_t)h * a.n_tokens + m] = NAN;
-    return;
-  }
+  const Row8 q = row8(a.qkv + m * ROW + (int64_t)h * kHD);
+  f16* orow = out + m * (int64_t)a.nq * kHD + (int64_t)h * kHD;
+  const float own = __fmul_rn(row_dot(q, row_load(kb + m * ROW)), a.qk_scale);
+  bool nan = own != own || own == INFINITY;   // 2^(inf - inf)
   const KeyRuns kr = key_runs(a, m);
   const int64_t n = kr.na + kr.nb;
-  float mx = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int64_t i0 = 0; i0 < n; i0 += 64) {
-    const bool on = i0 + lane < n;
-    float x = -INFINITY;
-    if (on) x = __fmul_rn(row_dot(s.a, kb + kr.row(i0 + lane) * ROW), a.qk_scale);
-    // a NaN score has to reach the sum: the maximum leaves it out, 2^(x - max) below does not
-    float t = x;
+  float mx = -INFINITY, l = 0.0f;
+  Row8 o = fill8(0.0f);
+  for (int64_t i0 = 0; i0 < n && !nan; i0 += 4 * kWalk) {
+    f16x8 k[kWalk], v[kWalk];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) t = fmaxf(t, __shfl_xor(t, d));
-    const float m_new = fmaxf(mx, t);
-    const float ref = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = mx == -INFINITY ? 0.0f : exp2f(__fsub_rn(mx, ref));
-    const float p = on ? exp2f(__fsub_rn(x, ref)) : 0.0f;
-    mx = m_new;
-    l = __fadd_rn(__fmul_rn(l, alpha), wave_sum(p));
-    o0 = __fmul_rn(o0, alpha);
-    o1 = __fmul_rn(o1, alpha);
-    wave_sync();
-    s.p[lane] = p;
-    wave_sync();
-    const int cnt = n - i0 < 64 ? (int)(n - i0) : 64;
-    for (int j = 0; j < cnt; ++j) {
-      const f16x2 v = *reinterpret_cast<const f16x2*>(vb + kr.row(i0 + j) * ROW + 2 * lane);
-      o0 = __builtin_fmaf(s.p[j], (float)v[0], o0);
-      o1 = __builtin_fmaf(s.p[j], (float)v[1], o1);
+    for (int u = 0; u < kWalk; ++u) {
+      const int64_t i = i0 + 4 * u + quarter, off = kr.row(i < n ? i : n - 1) * ROW;
+      k[u] = row_load(kb + off);
+      v[u] = row_load(vb + off);
     }
+    float sc[kWalk];
+#pragma unroll
+    for (int u = 0; u < kWalk; ++u) sc[u] = __fmul_rn(row_dot(q, k[u]), a.qk_scale);
+#pragma unroll
+    for (int u = 0; u < kWalk; ++u) {
+      const float x = sc[u];
+      if (i0 + 4 * u + quarter < n) {
+        // a NaN score has to reach the sum: the maximum leaves it out, 2^(x - max) below does not
+        const float m_new = fmaxf(mx, x), ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = mx == -INFINITY ? 0.0f : exp2f(__fsub_rn(mx, ref));
+        const float p = exp2f(__fsub_rn(x, ref));
+        mx = m_new;
+        l = __builtin_fmaf(l, alpha, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o.x[e] = __fmul_rn(o.x[e], alpha);
+        row_add(o, p, v[u]);
+      }
+    }
+    nan = __builtin_amdgcn_ballot_w64(l != l) != 0;
   }
-  const float inv = __fdiv_rn(1.0f, l);
-  f16x2 r;
-  r[0] = (f16)__fmul_rn(o0, inv);
-  r[1] = (f16)__fmul_rn(o1, inv);
-  *reinterpret_cast<f16x2*>(orow) = r;
-  if (lane == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(mx, log2f(l));
+  if (nan) {
+    store8(orow, fill8(NAN));
+    if ((threadIdx.x & 63) == 0) lse[(int64_t)h * a.n_tokens + m] = NAN;
+    return;
+  }
+  // a quarter without keys has added nothing: its sums stay out
+  float all = fmaxf(mx, __shfl_xor(mx, 16));
+  all = fmaxf(all, __shfl_xor(all, 32));
+  const float w = mx == -INFINITY ? 0.0f : exp2f(__fsub_rn(mx, all));
+  l = __fmul_rn(l, w);
+  l = __fadd_rn(l, __shfl_xor(l, 16));
+  l = __fadd_rn(l, __shfl_xor(l, 32));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o.x[e] = __fmul_rn(o.x[e], w);
+  store8(orow, row_sum(o, __fdiv_rn(1.0f, l)));
+  if ((threadIdx.x & 63) == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(all, log2f(l));
 }
 
 // dq of query m, head h
 __device__ __forceinline__ void span_row_dq(const SpanArgs& a, int64_t m, int h, const f16* dout,
-                                         const float* lse, const float* delta, f16* dq,
-                                         RowScratch& s) {
-  const int lane = threadIdx.x & 63;
+                                            const float* lse, const float* delta, f16* dq) {
   const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
-  const int kvh = h / (a.nq / a.nkv);
+  const int kvh = h / (a.nq / a.nkv), quarter = (threadIdx.x >> 4) & 3;
   const f16* kb = a.qkv + (int64_t)(a.nq + kvh) * kHD;
   const f16* vb = kb + (int64_t)a.nkv * kHD;
-  wave_sync();
-  row_to_lds(s.a, a.qkv + m * ROW + (int64_t)h * kHD);
-  row_to_lds(s.b, dout + m * OROW + (int64_t)h * kHD);
-  wave_sync();
+  const Row8 q = row8(a.qkv + m * ROW + (int64_t)h * kHD), d = row8(dout + m * OROW + (int64_t)h * kHD);
   const float lm = lse[(int64_t)h * a.n_tokens + m], dm = delta[(int64_t)h * a.n_tokens + m];
-  f16* grow = dq + m * OROW + (int64_t)h * kHD + 2 * lane;
-  const float own = __fmul_rn(exp2f(__builtin_fmaf(row_dot(s.a, kb + m * ROW), a.qk_scale, -lm)),
-                              __fsub_rn(row_dot(s.b, vb + m * ROW), dm));
-  if (own != own) {
-    *reinterpret_cast<f16x2*>(grow) = f16x2{(f16)NAN, (f16)NAN};
-    return;
-  }
+  auto grad = [&](const f16x8& k, const f16x8& v) {
+    const float p = exp2f(__builtin_fmaf(row_dot(q, k), a.qk_scale, -lm));
+    return __fmul_rn(p, __fsub_rn(row_dot(d, v), dm));
+  };
+  const float own = grad(row_load(kb + m * ROW), row_load(vb + m * ROW));
+  bool nan = own != own;   // in every column
   const KeyRuns kr = key_runs(a, m);
   const int64_t n = kr.na + kr.nb;
-  float g0 = 0.0f, g1 = 0.0f;
-  for (int64_t i0 = 0; i0 < n; i0 += 64) {
-    float ds = 0.0f;
-    if (i0 + lane < n) {
-      const int64_t off = kr.row(i0 + lane) * ROW;
-      const float p = exp2f(__builtin_fmaf(row_dot(s.a, kb + off), a.qk_scale, -lm));
-      ds = __fmul_rn(p, __fsub_rn(row_dot(s.b, vb + off), dm));
+  Row8 g = fill8(0.0f);
+  for (int64_t i0 = 0; i0 < n && !nan; i0 += 4 * kWalk) {
+    f16x8 k[kWalk], v[kWalk];
+#pragma unroll
+    for (int u = 0; u < kWalk; ++u) {
+      const int64_t i = i0 + 4 * u + quarter, off = kr.row(i < n ? i : n - 1) * ROW;
+      k[u] = row_load(kb + off);
+      v[u] = row_load(vb + off);
     }
-    wave_sync();
-    s.ds[lane] = ds;
-    wave_sync();
-    const int cnt = n - i0 < 64 ? (int)(n - i0) : 64;
-    for (int j = 0; j < cnt; ++j) {
-      const f16x2 k = *reinterpret_cast<const f16x2*>(kb + kr.row(i0 + j) * ROW + 2 * lane);
-      g0 = __builtin_fmaf(s.ds[j], (float)k[0], g0);
-      g1 = __builtin_fmaf(s.ds[j], (float)k[1], g1);
-    }
+    float ds[kWalk];
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < kWalk; ++u) ds[u] = grad(k[u], v[u]);
+#pragma unroll
+    for (int u = 0; u < kWalk; ++u)
+      if (i0 + 4 * u + quarter < n) {
+        any |= ds[u] != ds[u];
+        row_add(g, ds[u], k[u]);
+      }
+    nan = __builtin_amdgcn_ballot_w64(any) != 0;
   }
-  f16x2 r;
-  r[0] = (f16)__fmul_rn(g0, a.sm_scale);
-  r[1] = (f16)__fmul_rn(g1, a.sm_scale);
-  *reinterpret_cast<f16x2*>(grow) = r;
+  store8(dq + m * OROW + (int64_t)h * kHD, nan ? fill8(NAN) : row_sum(g, a.sm_scale));
 }
 
 // dk and dv of key n, KV head g, summed over the queries that see it and the heads of its group
 __device__ __forceinline__ void span_key_dkdv(const SpanArgs& a, int64_t n, int g, const f16* dout,
-                                           const float* lse, const float* delta, f16* dk, f16* dv,
-                                           RowScratch& s) {
-  const int lane = threadIdx.x & 63;
+                                              const float* lse, const float* delta, f16* dk, f16* dv) {
   const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
-  const int gin = a.nq / a.nkv;
+  const int gin = a.nq / a.nkv, quarter = (threadIdx.x >> 4) & 3;
   const f16* krow = a.qkv + n * ROW + (int64_t)(a.nq + g) * kHD;
-  wave_sync();
-  row_to_lds(s.a, krow);
-  row_to_lds(s.b, krow + (int64_t)a.nkv * kHD);
-  wave_sync();
-  const int64_t off = n * (int64_t)a.nkv * kHD + (int64_t)g * kHD + 2 * lane;
-  // dk is NaN where the token's own dS is, dv where its own P is or, by columns, its own dO
-  bool p_nan = false, ds_nan = false, col0 = false, col1 = false;
-  for (int hh = g * gin; hh < (g + 1) * gin; ++hh) {
-    const f16* orow = dout + n * OROW + (int64_t)hh * kHD;
-    const float p = exp2f(__builtin_fmaf(row_dot(s.a, a.qkv + n * ROW + (int64_t)hh * kHD), a.qk_scale,
-                                         -lse[(int64_t)hh * a.n_tokens + n]));
-    const float ds = __fmul_rn(p, __fsub_rn(row_dot(s.b, orow), delta[(int64_t)hh * a.n_tokens + n]));
-    const f16x2 o = *reinterpret_cast<const f16x2*>(orow + 2 * lane);
-    p_nan |= p != p;
-    ds_nan |= ds != ds;
-    col0 |= o[0] != o[0];
-    col1 |= o[1] != o[1];
-  }
-  if (ds_nan && (p_nan || __builtin_amdgcn_ballot_w64(!(col0 && col1)) == 0)) {
-    *reinterpret_cast<f16x2*>(dk + off) = f16x2{(f16)NAN, (f16)NAN};
-    *reinterpret_cast<f16x2*>(dv + off) = f16x2{(f16)NAN, (f16)NAN};
-    return;
-  }
+  const Row8 k = row8(krow), v = row8(krow + (int64_t)a.nkv * kHD);
+  Row8 gk = fill8(0.0f), gv = fill8(0.0f);
+  bool dk_nan = false, dv_nan = false;   // in every column
   const int64_t end = key_end(a, n);
-  float dk0 = 0.0f, dk1 = 0.0f, dv0 = 0.0f, dv1 = 0.0f;
-  for (int hh = g * gin; hh < (g + 1) * gin; ++hh)
-    for (int64_t m0 = n; m0 < end; m0 += 64) {
-      const int64_t m = m0 + lane;
-      const f16* qb = a.qkv + (int64_t)hh * kHD;
-      const f16* ob = dout + (int64_t)hh * kHD;
-      float p = 0.0f, ds = 0.0f;
-      if (m < end) {
-        p = exp2f(__builtin_fmaf(row_dot(s.a, qb + m * ROW), a.qk_scale,
-                                 -lse[(int64_t)hh * a.n_tokens + m]));
-        ds = __fmul_rn(p, __fsub_rn(row_dot(s.b, ob + m * OROW), delta[(int64_t)hh * a.n_tokens + m]));
+  for (int hh = g * gin; hh < (g + 1) * gin; ++hh) {
+    const f16* qb = a.qkv + (int64_t)hh * kHD;
+    const f16* ob = dout + (int64_t)hh * kHD;
+    const float* lb = lse + (int64_t)hh * a.n_tokens;
+    const float* db = delta + (int64_t)hh * a.n_tokens;
+    for (int64_t m0 = n; m0 < end && !(dk_nan && dv_nan); m0 += 4 * kWalk) {
+      f16x8 q[kWalk], o[kWalk];
+      float lm[kWalk], dm[kWalk];
+#pragma unroll
+      for (int u = 0; u < kWalk; ++u) {
+        const int64_t i = m0 + 4 * u + quarter, m = i < end ? i : end - 1;
+        q[u] = row_load(qb + m * ROW);
+        o[u] = row_load(ob + m * OROW);
+        lm[u] = lb[m];
+        dm[u] = db[m];
       }
-      wave_sync();
-      s.p[lane] = p;
-      s.ds[lane] = ds;
-      wave_sync();
-      const int cnt = end - m0 < 64 ? (int)(end - m0) : 64;
-      for (int j = 0; j < cnt; ++j) {
-        const f16x2 q = *reinterpret_cast<const f16x2*>(qb + (m0 + j) * ROW + 2 * lane);
-        const f16x2 o = *reinterpret_cast<const f16x2*>(ob + (m0 + j) * OROW + 2 * lane);
-        dk0 = __builtin_fmaf(s.ds[j], (float)q[0], dk0);
-        dk1 = __builtin_fmaf(s.ds[j], (float)q[1], dk1);
-        dv0 = __builtin_fmaf(s.p[j], (float)o[0], dv0);
-        dv1 = __builtin_fmaf(s.p[j], (float)o[1], dv1);
+      float p[kWalk], ds[kWalk];
+      bool p_nan = false, ds_nan = false;
+#pragma unroll
+      for (int u = 0; u < kWalk; ++u) {
+        p[u] = exp2f(__builtin_fmaf(row_dot(k, q[u]), a.qk_scale, -lm[u]));
+        ds[u] = __fmul_rn(p[u], __fsub_rn(row_dot(v, o[u]), dm[u]));
       }
+#pragma unroll
+      for (int u = 0; u < kWalk; ++u)
+        if (m0 + 4 * u + quarter < end) {
+          p_nan |= p[u] != p[u];
+          ds_nan |= ds[u] != ds[u];
+          row_add(gk, ds[u], q[u]);
+          row_add(gv, p[u], o[u]);
+        }
+      // every column of dv is NaN where each is in a quarter's sum
+      bool all = true;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) all &= gv.x[e] != gv.x[e];
+      uint64_t cols = __builtin_amdgcn_ballot_w64(all);
+      cols |= cols >> 32;
+      cols |= cols >> 16;
+      dk_nan |= __builtin_amdgcn_ballot_w64(ds_nan) != 0;
+      dv_nan |= __builtin_amdgcn_ballot_w64(p_nan) != 0 || (cols & 0xffff) == 0xffff;
     }
-  f16x2 r;
-  r[0] = (f16)__fmul_rn(dk0, a.sm_scale);
-  r[1] = (f16)__fmul_rn(dk1, a.sm_scale);
-  *reinterpret_cast<f16x2*>(dk + off) = r;
-  r[0] = (f16)dv0;
-  r[1] = (f16)dv1;
-  *reinterpret_cast<f16x2*>(dv + off) = r;
+  }
+  const int64_t off = n * (int64_t)a.nkv * kHD + (int64_t)g * kHD;
+  store8(dk + off, dk_nan ? fill8(NAN) : row_sum(gk, a.sm_scale));
+  store8(dv + off, dv_nan ? fill8(NAN) : row_sum(gv, 1.0f));
 }
 
 // the launch arguments, with the checks both entry points share

@@ -76,22 +76,22 @@ constexpr int kAhead1 = 6, kAhead2 = 4;
 // or infinity of a masked row is not 0.  bad: row flags in LDS, written before a barrier.
 template <int W>
 __device__ __forceinline__ void redo_dq(const SpanArgs& a, int t0, int phase, int rows, int g,
-                                        const int* bad, RowScratch* s, const f16* dout, const float* lse,
+                                        const int* bad, const f16* dout, const float* lse,
                                         const float* delta, f16* dq) {
   const int gin = a.nq / a.nkv, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   for (int i = wave; i < rows; i += W) {
     if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
-    span_row_dq(a, t0 + (phase + i) / gin, g * gin + (phase + i) % gin, dout, lse, delta, dq, s[wave]);
+    span_row_dq(a, t0 + (phase + i) / gin, g * gin + (phase + i) % gin, dout, lse, delta, dq);
   }
 }
 template <int W>
 __device__ __forceinline__ void redo_dkdv(const SpanArgs& a, int k0, int nk, int g, const int* bad,
-                                          RowScratch* s, const f16* dout, const float* lse,
-                                          const float* delta, f16* dk, f16* dv) {
+                                          const f16* dout, const float* lse, const float* delta,
+                                          f16* dk, f16* dv) {
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   for (int i = wave; i < nk; i += W) {
     if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
-    span_key_dkdv(a, (int64_t)k0 + i, g, dout, lse, delta, dk, dv, s[wave]);
+    span_key_dkdv(a, (int64_t)k0 + i, g, dout, lse, delta, dk, dv);
   }
 }
 
@@ -375,7 +375,7 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
       *reinterpret_cast<f16x8*>(dq + (int64_t)(it.t0 + sr / gin) * OROW +
                                 (int64_t)(it.g * gin + sr % gin) * kHD + 8 * cc) = v;
   }
-  redo_dq<4>(a, it.t0, it.phase, it.rows, it.g, bad, reinterpret_cast<RowScratch*>(Vs), dout, lse, delta, dq);
+  redo_dq<4>(a, it.t0, it.phase, it.rows, it.g, bad, dout, lse, delta, dq);
 }
 
 // dK and dV of a block of up to kBM keys, summed over the heads of the KV head's group: K and V stay in
@@ -603,8 +603,7 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
     return;
   }
   store_dkdv(a, k0, nk, g, dkacc, dvacc, Qs, Ds, bad, dk, dv);
-  __syncthreads();   // the staged rows have been read
-  redo_dkdv<4>(a, k0, nk, g, bad, reinterpret_cast<RowScratch*>(Qs), dout, lse, delta, dk, dv);
+  redo_dkdv<4>(a, k0, nk, g, bad, dout, lse, delta, dk, dv);
 }
 
 // The same for a block of at most 32 keys (sinks, whose walk is the whole sequence): a step takes two
@@ -768,8 +767,7 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
   }
   __syncthreads();   // the sums have been read
   store_group(a, true, k0, 0, nk, g, w, x, y, Qs, Ds, bad, nullptr, dk, dv);
-  __syncthreads();   // and the staged rows
-  redo_dkdv<4>(a, k0, nk, g, bad, reinterpret_cast<RowScratch*>(Qs), dout, lse, delta, dk, dv);
+  redo_dkdv<4>(a, k0, nk, g, bad, dout, lse, delta, dk, dv);
 }
 
 // Every item of the backward in one launch, longest walks first (the plan's order): dK/dV walks and
@@ -820,7 +818,6 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_join_kernel(
     phase = (phase + 32 * w) % gin;
   }
   __shared__ __attribute__((aligned(16))) f16 S0[32 * kStride16], S1[32 * kStride16];
-  __shared__ RowScratch scratch[kAThreads / 64];
   __shared__ int bad[32];
   if (threadIdx.x < 32) bad[threadIdx.x] = 0;
   __syncthreads();
@@ -856,8 +853,8 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_join_kernel(
   sum(x, p);
   if (keys) sum(y, p + kUnitFloats);
   store_group(a, keys, t0, phase, rows, g, hb, x, y, S0, S1, bad, dq, dk, dv);
-  if (keys) redo_dkdv<4>(a, t0, rows, g, bad, scratch, dout, lse, delta, dk, dv);
-  else redo_dq<4>(a, t0, phase, rows, g, bad, scratch, dout, lse, delta, dq);
+  if (keys) redo_dkdv<4>(a, t0, rows, g, bad, dout, lse, delta, dk, dv);
+  else redo_dq<4>(a, t0, phase, rows, g, bad, dout, lse, delta, dq);
 }
 
 }  // namespace

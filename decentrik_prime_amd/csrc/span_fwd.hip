@@ -19,14 +19,14 @@ __device__ __forceinline__ float half_max(float x) {
 
 // The rows whose result is not finite, recomputed over exactly the keys that they see: a masked key's
 // probability is 0, but 0 times a NaN or infinity in its value row is not.  bad [kBM]: row flags in
-// LDS, written before a barrier; s: a scratch per wave.
+// LDS, written before a barrier.
 template <int W>
 __device__ __forceinline__ void redo_rows(const SpanArgs& a, int t0, int phase, int rows, int g,
-                                          const int* bad, RowScratch* s, f16* out, float* lse) {
+                                          const int* bad, f16* out, float* lse) {
   const int gin = a.nq / a.nkv, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   for (int i = wave; i < rows; i += W) {
     if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
-    span_row_fwd(a, t0 + (phase + i) / gin, g * gin + (phase + i) % gin, out, lse, s[wave]);
+    span_row_fwd(a, t0 + (phase + i) / gin, g * gin + (phase + i) % gin, out, lse);
   }
 }
 
@@ -271,8 +271,7 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
       *reinterpret_cast<f16x8*>(out + (int64_t)(it.t0 + sr / gin) * a.nq * kHD +
                                 (int64_t)(it.g * gin + sr % gin) * kHD + 8 * cc) = v;
   }
-  __syncthreads();   // the staged rows have been read
-  redo_rows<4>(a, it.t0, it.phase, it.rows, it.g, bad, reinterpret_cast<RowScratch*>(ring), out, lse);
+  redo_rows<4>(a, it.t0, it.phase, it.rows, it.g, bad, out, lse);
 }
 
 // The partials of a block put together: O = sum_s O_s 2^(m_s - m) / l, m = max m_s, l likewise, in slot
@@ -295,7 +294,6 @@ __global__ __launch_bounds__(kAThreads) void span_join_kernel(SpanArgs a, const 
   t0 += (phase + 32 * qw) / gin;
   phase = (phase + 32 * qw) % gin;
   __shared__ __attribute__((aligned(16))) f16 stage[32 * kStride16];
-  __shared__ RowScratch scratch[kAThreads / 64];
   __shared__ int bad[32];
   if (threadIdx.x < 32) bad[threadIdx.x] = 0;
   __syncthreads();
@@ -356,7 +354,7 @@ __global__ __launch_bounds__(kAThreads) void span_join_kernel(SpanArgs a, const 
       *reinterpret_cast<f16x8*>(out + ((int64_t)t0 + rr / gin) * a.nq * kHD +
                                 (int64_t)(g * gin + rr % gin) * kHD + 8 * cc) = v;
   }
-  redo_rows<4>(a, t0, phase, rows, g, bad, scratch, out, lse);
+  redo_rows<4>(a, t0, phase, rows, g, bad, out, lse);
 }
 
 }  // namespace

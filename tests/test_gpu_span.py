@@ -358,6 +358,38 @@ def test_batches_of_nothing_but_nan(torch, what):
     assert finite(dv) if what == "v" else nan(dv)
 
 
+@pytest.mark.parametrize("spec,up,down", [(("window", [30, 400], 90, 3), 130, 141),
+                                          (("prefix", [(150, [40, 5, 77])]), 20, 155)])
+@pytest.mark.parametrize("cut", [False, True])
+def test_infinities_reach_who_sees_them(torch, monkeypatch, spec, up, down, cut):
+    """+inf in one value row and one gradient row and -inf in another of each: +inf, -inf, or NaN where
+    both come together, in out and dv; lse as without them."""
+    nq, nkv = 4, 2
+    if cut:
+        from decentrik_prime_amd import k_attn
+        monkeypatch.setattr(k_attn, "_fwd_tiles", lambda blocks: 1)
+        monkeypatch.setattr(k_attn, "_bwd_cost", lambda cost: 4)
+    log(f"span attention with infinities in rows {up} and {down}, {spec}")
+    meta = _meta(spec, nq, nkv)
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=14)
+    want = _run(qkv, dout, meta, nq, nkv)
+    vis = torch.from_numpy(_visible(spec)).cuda()
+    bad = qkv.clone()
+    for row, x in ((up, float("inf")), (down, -float("inf"))):
+        bad[row, (nq + nkv) * HD:] = x
+        dout[row] = x
+    out, lse, _, _, dv = _run(bad, dout, meta, nq, nkv)
+    # the same sums, in another order at the most
+    assert bool(((lse - want[1]).abs() <= 2.0 ** -12).all())
+    for t, sees_up, sees_down, what in ((out, vis[:, up], vis[:, down], "out"),
+                                        (dv, vis[up], vis[down], "dv")):
+        t = t.float()
+        for rows, f in ((sees_up & ~sees_down, torch.isposinf), (sees_down & ~sees_up, torch.isneginf),
+                        (sees_up & sees_down, torch.isnan), (~sees_up & ~sees_down, torch.isfinite)):
+            assert bool(f(t[rows]).all()), what
+        assert bool((sees_up ^ sees_down).any()) and bool((sees_up & sees_down).any())
+
+
 def test_one_column_of_nan_stays_one(torch):
     """A NaN in one column of every value row and of every gradient row: that column of out and of dv."""
     nq, nkv = 4, 2
