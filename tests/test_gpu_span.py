@@ -99,6 +99,8 @@ CASES = [
     (("prefix", [(200, [1] * 70)]), 12, 2), (("prefix", [(64, [64, 128, 0, 63])]), 2, 2),
     (("prefix", [(500, [40, 3, 77, 0, 190]), (0, [33]), (17, [1, 300]), (300, [0])]), 28, 4),
     (("prefix", [(1100, [150, 90, 301])]), 6, 1), (("prefix", [(77, [9] * 33)]), 8, 8),
+    # a group of more heads than a block has rows
+    (("window", [70, 3], 5, 2), 130, 1), (("prefix", [(40, [1, 7, 30])]), 400, 2),
 ]
 
 
