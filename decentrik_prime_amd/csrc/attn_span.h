@@ -55,6 +55,36 @@ __device__ __forceinline__ bool full_tile(const SpanItem& it, int t) {
   return t < it.f0 || (t >= it.f1 && t < it.f2);
 }
 
+constexpr int kStride16 = kHD + 8;   // halves per staged row of a result
+
+// The wave's 32 staged rows of a result [n_tokens, nq, hd], those that are in the block and not bad, 16
+// bytes a lane, four whole rows per store.  One division, and the flags read before the first store: on
+// their own in every step they took 0.13 us a step.
+__device__ __forceinline__ void store_rows(const SpanArgs& a, const SpanItem& it, int wave, int lane,
+                                           const f16* stage, const int* bad, f16* dst) {
+  const int gin = a.nq / a.nkv, srow = 32 * wave + (lane >> 4), sr = it.phase + srow;
+  int t = sr / gin, h = sr - t * gin;
+  const int dt = 4 / gin, dh = 4 - dt * gin;
+  int keep[8];
+  f16x8 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    keep[i] = (srow + 4 * i < it.rows) & !bad[srow + 4 * i];
+    v[i] = *reinterpret_cast<const f16x8*>(stage + (4 * i + (lane >> 4)) * kStride16 + 8 * (lane & 15));
+  }
+  f16* const base = dst + ((int64_t)it.t0 * a.nq + it.g * gin) * kHD + 8 * (lane & 15);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (keep[i]) *reinterpret_cast<f16x8*>(base + ((int64_t)t * a.nq + h) * kHD) = v[i];
+    t += dt;
+    h += dh;
+    if (h >= gin) {
+      h -= gin;
+      ++t;
+    }
+  }
+}
+
 // A tile of the item's keys, one operand, by LDS DMA: instruction i fills rows 4 (W i + wave) .. + 3 of
 // the tile (W waves), 16 lanes a row, from a scalar base per tile and a 32-bit offset per lane.  In the
 // tile that holds keys of both runs the second run's lie a gap further on (span_item: it fits).  Keys
@@ -112,7 +142,6 @@ __device__ __forceinline__ void key_ends_load(const SpanArgs& a, const SpanItem&
   dma4(a.spans + 4 * row + 3, __builtin_amdgcn_readfirstlane(lds_addr(dst)));
 }
 
-constexpr int kStride16 = kHD + 8;   // halves per staged row of a result
 
 // Where quad q of result block hb of wave w's rows stands in a partial: 16 bytes per lane, lane-major.
 __device__ __forceinline__ int part_off(int w, int hb, int q, int lane) {
@@ -129,6 +158,18 @@ __device__ __forceinline__ f32x4 quad(const f32x16& x, int q) {
 // it; a query's first look is at its term with itself, where a key's walk begins, so a batch of nothing
 // but NaN (a diverged step) costs no walks.
 constexpr int kWalk = 4;
+
+// redo(i) for the flagged rows of a block, every fourth to a wave.  All flags are read at once: one
+// after the other, for a block without any, took 1.6 us.
+template <class F>
+__device__ __forceinline__ void bad_rows(const int* bad, int rows, F redo) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const uint64_t lo = __builtin_amdgcn_ballot_w64(lane < rows && bad[lane]);
+  const uint64_t hi = __builtin_amdgcn_ballot_w64(64 + lane < rows && bad[64 + lane]);
+  if ((lo | hi) == 0) return;
+  for (int i = wave; i < rows; i += 4)
+    if ((i < 64 ? lo : hi) >> (i & 63) & 1) redo(i);
+}
 
 struct Row8 {
   float x[8];

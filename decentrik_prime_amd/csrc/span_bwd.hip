@@ -74,25 +74,18 @@ constexpr int kAhead1 = 6, kAhead2 = 4;
 
 // The rows (or keys) whose result is not finite, recomputed over exactly what they see: 0 times a NaN
 // or infinity of a masked row is not 0.  bad: row flags in LDS, written before a barrier.
-template <int W>
 __device__ __forceinline__ void redo_dq(const SpanArgs& a, int t0, int phase, int rows, int g,
                                         const int* bad, const f16* dout, const float* lse,
                                         const float* delta, f16* dq) {
-  const int gin = a.nq / a.nkv, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  for (int i = wave; i < rows; i += W) {
-    if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
+  const int gin = a.nq / a.nkv;
+  bad_rows(bad, rows, [&](int i) {
     span_row_dq(a, t0 + (phase + i) / gin, g * gin + (phase + i) % gin, dout, lse, delta, dq);
-  }
+  });
 }
-template <int W>
 __device__ __forceinline__ void redo_dkdv(const SpanArgs& a, int k0, int nk, int g, const int* bad,
                                           const f16* dout, const float* lse, const float* delta,
                                           f16* dk, f16* dv) {
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  for (int i = wave; i < nk; i += W) {
-    if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
-    span_key_dkdv(a, (int64_t)k0 + i, g, dout, lse, delta, dk, dv);
-  }
+  bad_rows(bad, nk, [&](int i) { span_key_dkdv(a, (int64_t)k0 + i, g, dout, lse, delta, dk, dv); });
 }
 
 // The wave's 32 keys of dK and dV, rounded, staged in its quarter of two LDS buffers and written back
@@ -117,15 +110,19 @@ __device__ __forceinline__ void store_dkdv(const SpanArgs& a, int k0, int nk, in
     if (chk != 0.0f) bad[32 * w + r] = 1;
   }
   __syncthreads();
+  const int key = 32 * w + (lane >> 4), cc = lane & 15;
+  int keep[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) keep[i] = (key + 4 * i < nk) & !bad[key + 4 * i];
+  const int64_t o = (((int64_t)k0 + key) * a.nkv + g) * kHD + 8 * cc;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = 4 * i + (lane >> 4), cc = lane & 15, key = 32 * w + r;
+    const int r = 4 * i + (lane >> 4);
     const f16x8 kv = *reinterpret_cast<const f16x8*>(kst + r * kStride16 + 8 * cc);
     const f16x8 vv = *reinterpret_cast<const f16x8*>(vst + r * kStride16 + 8 * cc);
-    if (key < nk && !bad[key]) {
-      const int64_t o = ((int64_t)k0 + key) * a.nkv * kHD + (int64_t)g * kHD + 8 * cc;
-      *reinterpret_cast<f16x8*>(dk + o) = kv;
-      *reinterpret_cast<f16x8*>(dv + o) = vv;
+    if (keep[i]) {
+      *reinterpret_cast<f16x8*>(dk + o + (int64_t)(4 * i) * a.nkv * kHD) = kv;
+      *reinterpret_cast<f16x8*>(dv + o + (int64_t)(4 * i) * a.nkv * kHD) = vv;
     }
   }
 }
@@ -366,16 +363,8 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
     }
   if (chk != 0.0f) bad[row] = 1;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 4 * i + (lane >> 4), cc = lane & 15;
-    const int srow = 32 * w + r, sr = it.phase + srow;
-    const f16x8 v = *reinterpret_cast<const f16x8*>(stage + r * kStride16 + 8 * cc);
-    if (srow < it.rows && !bad[srow])
-      *reinterpret_cast<f16x8*>(dq + (int64_t)(it.t0 + sr / gin) * OROW +
-                                (int64_t)(it.g * gin + sr % gin) * kHD + 8 * cc) = v;
-  }
-  redo_dq<4>(a, it.t0, it.phase, it.rows, it.g, bad, dout, lse, delta, dq);
+  store_rows(a, it, w, lane, stage, bad, dq);
+  redo_dq(a, it.t0, it.phase, it.rows, it.g, bad, dout, lse, delta, dq);
 }
 
 // dK and dV of a block of up to kBM keys, summed over the heads of the KV head's group: K and V stay in
@@ -603,7 +592,7 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
     return;
   }
   store_dkdv(a, k0, nk, g, dkacc, dvacc, Qs, Ds, bad, dk, dv);
-  redo_dkdv<4>(a, k0, nk, g, bad, dout, lse, delta, dk, dv);
+  redo_dkdv(a, k0, nk, g, bad, dout, lse, delta, dk, dv);
 }
 
 // The same for a block of at most 32 keys (sinks, whose walk is the whole sequence): a step takes two
@@ -767,7 +756,7 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
   }
   __syncthreads();   // the sums have been read
   store_group(a, true, k0, 0, nk, g, w, x, y, Qs, Ds, bad, nullptr, dk, dv);
-  redo_dkdv<4>(a, k0, nk, g, bad, dout, lse, delta, dk, dv);
+  redo_dkdv(a, k0, nk, g, bad, dout, lse, delta, dk, dv);
 }
 
 // Every item of the backward in one launch, longest walks first (the plan's order): dK/dV walks and
@@ -853,8 +842,8 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_join_kernel(
   sum(x, p);
   if (keys) sum(y, p + kUnitFloats);
   store_group(a, keys, t0, phase, rows, g, hb, x, y, S0, S1, bad, dq, dk, dv);
-  if (keys) redo_dkdv<4>(a, t0, rows, g, bad, dout, lse, delta, dk, dv);
-  else redo_dq<4>(a, t0, phase, rows, g, bad, dout, lse, delta, dq);
+  if (keys) redo_dkdv(a, t0, rows, g, bad, dout, lse, delta, dk, dv);
+  else redo_dq(a, t0, phase, rows, g, bad, dout, lse, delta, dq);
 }
 
 }  // namespace

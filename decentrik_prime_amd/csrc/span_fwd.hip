@@ -20,14 +20,12 @@ __device__ __forceinline__ float half_max(float x) {
 // The rows whose result is not finite, recomputed over exactly the keys that they see: a masked key's
 // probability is 0, but 0 times a NaN or infinity in its value row is not.  bad [kBM]: row flags in
 // LDS, written before a barrier.
-template <int W>
 __device__ __forceinline__ void redo_rows(const SpanArgs& a, int t0, int phase, int rows, int g,
                                           const int* bad, f16* out, float* lse) {
-  const int gin = a.nq / a.nkv, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  for (int i = wave; i < rows; i += W) {
-    if (!__builtin_amdgcn_readfirstlane(bad[i])) continue;
+  const int gin = a.nq / a.nkv;
+  bad_rows(bad, rows, [&](int i) {
     span_row_fwd(a, t0 + (phase + i) / gin, g * gin + (phase + i) % gin, out, lse);
-  }
+  });
 }
 
 // A workgroup per item: 4 waves of 32 stacked rows, lane l % 32 a row, over 64-key tiles.
@@ -262,16 +260,8 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
   if (chk != 0.0f) bad[row] = 1;
   else if (mval && hl == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(m_i, log2f(l_i));
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 4 * i + (lane >> 4), cc = lane & 15;
-    const int srow = 32 * wave + r, sr = it.phase + srow;
-    const f16x8 v = *reinterpret_cast<const f16x8*>(ostage + r * kStride16 + 8 * cc);
-    if (srow < it.rows && !bad[srow])
-      *reinterpret_cast<f16x8*>(out + (int64_t)(it.t0 + sr / gin) * a.nq * kHD +
-                                (int64_t)(it.g * gin + sr % gin) * kHD + 8 * cc) = v;
-  }
-  redo_rows<4>(a, it.t0, it.phase, it.rows, it.g, bad, out, lse);
+  store_rows(a, it, wave, lane, ostage, bad, out);
+  redo_rows(a, it.t0, it.phase, it.rows, it.g, bad, out, lse);
 }
 
 // The partials of a block put together: O = sum_s O_s 2^(m_s - m) / l, m = max m_s, l likewise, in slot
@@ -354,7 +344,7 @@ __global__ __launch_bounds__(kAThreads) void span_join_kernel(SpanArgs a, const 
       *reinterpret_cast<f16x8*>(out + ((int64_t)t0 + rr / gin) * a.nq * kHD +
                                 (int64_t)(g * gin + rr % gin) * kHD + 8 * cc) = v;
   }
-  redo_rows<4>(a, t0, phase, rows, g, bad, out, lse);
+  redo_rows(a, t0, phase, rows, g, bad, out, lse);
 }
 
 }  // namespace
