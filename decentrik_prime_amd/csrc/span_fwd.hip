@@ -63,6 +63,7 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
   f32x16 oacc[kHD / 32];
 #pragma unroll
   for (int hb = 0; hb < kHD / 32; ++hb) oacc[hb] = zero16();
+  constexpr float kMasked = -3.0e38f;
   float m_i = -1.0e30f, l_i = 0.0f;   // l_i: this lane's half of the keys (joined at the end)
   const int n_tiles = it.te - it.tb;
   const uint64_t kbase = uniform64((uint64_t)(a.qkv + (int64_t)(a.nq + it.g) * kHD));
@@ -111,22 +112,20 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
   __syncthreads();   // every wave is done with K of tile 0
   // tile t, whose scores are in sc: its softmax and O^T += V^T P^T, beside the scores of tile t + 1
   // into sn (after the last tile: of a stale stage, never used).  MASK: key j of the tile counts iff
-  // j <= jlim and the key's end lies past this lane's token; the others' probabilities are set to 0
-  // (a lane may see none of a tile's keys before its first).
+  // j <= jlim and the key's end lies past this lane's token; the others' probabilities come out as 0, also
+  // where a lane has seen no key yet: kMasked lies as far below m_i's start as any score above it.
   auto tile = [&](int t, f32x16 (&sc)[2], f32x16 (&sn)[2], auto mask_c) {
     constexpr bool MASK = decltype(mask_c)::value;
     const unsigned va = fresh(vcol + (unsigned)((t % kStages) * kTileHalves * 2));
     const int lim = jlim - (it.tb + t) * kBN - 4 * hl;
-    unsigned on = 0;
     if constexpr (MASK) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const i32x4 e4 = *reinterpret_cast<const i32x4*>(&ends[t % kStages][8 * q + 4 * hl]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool k = (8 * q + e <= lim) & (m < e4[e]);
-          on |= k ? 1u << (4 * q + e) : 0u;
-          sc[q >> 2][4 * (q & 3) + e] = k ? sc[q >> 2][4 * (q & 3) + e] : -1.0e30f;
+          const bool seen = (8 * q + e <= lim) & (m < e4[e]);
+          sc[q >> 2][4 * (q & 3) + e] = seen ? sc[q >> 2][4 * (q & 3) + e] : kMasked;
         }
       }
     }
@@ -157,8 +156,7 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        float p = ex2(__builtin_fmaf(sc[kb][v], a.qk_scale, -m_i));
-        if constexpr (MASK) p = (on >> (16 * kb + v)) & 1 ? p : 0.0f;
+        const float p = ex2(__builtin_fmaf(sc[kb][v], a.qk_scale, -m_i));
         rs[v & 3] = __fadd_rn(rs[v & 3], p);
         pf[2 * kb + (v >> 3)][v & 7] = (f16)p;
       }
