@@ -390,12 +390,6 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
   const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
   const bool nval = 32 * w + c < nk;
   const int n = k0 + (nval ? 32 * w + c : 0);   // this lane's key
-  const int end = (int)key_end(a, n);
-  // the first end among the wave's keys
-  int end_min = nval ? end : INT32_MAX;
-#pragma unroll
-  for (int x = 32; x > 0; x >>= 1) end_min = min(end_min, __shfl_xor(end_min, x));
-  end_min = __builtin_amdgcn_readfirstlane(end_min);
 
   const int n_tiles = te - tb;
   if (tid < kBN) lse_s[kBwdStages][tid] = 0.0f;
@@ -427,6 +421,7 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
 
   // this lane's key and value rows as B operands, loaded unconditionally and selected at once
   // (the compiler's wait for them stands here, not in the loop)
+  const int end = (int)key_end(a, n);
   f16x8 kf[kHD / 16], vf[kHD / 16];
   {
     const f16* krow = a.qkv + (int64_t)n * ROW + (int64_t)(a.nq + g) * kHD + 8 * hl;
@@ -444,6 +439,11 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
       vf[s] = nval ? vf[s] : zero8();
     }
   }
+  // the first end among the wave's keys
+  int end_min = nval ? end : INT32_MAX;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) end_min = min(end_min, __shfl_xor(end_min, x));
+  end_min = __builtin_amdgcn_readfirstlane(end_min);
   f32x16 dkacc[kHD / 32], dvacc[kHD / 32];
 #pragma unroll
   for (int hb = 0; hb < kHD / 32; ++hb) dkacc[hb] = dvacc[hb] = zero16();
@@ -618,11 +618,6 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
   const int64_t ROW = (int64_t)(a.nq + 2 * a.nkv) * kHD, OROW = (int64_t)a.nq * kHD;
   const bool nval = c < nk;
   const int n = k0 + (nval ? c : 0);   // this lane's key
-  const int end = (int)key_end(a, n);
-  int end_min = nval ? end : INT32_MAX;
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) end_min = min(end_min, __shfl_xor(end_min, x));
-  end_min = __builtin_amdgcn_readfirstlane(end_min);
   if (tid < kBM) bad[tid] = 0;
 
   const int n_tiles = te - tb, n_steps = (n_tiles + 1) / 2;
@@ -646,6 +641,7 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
   };
   issue(0);
   issue(1);
+  const int end = (int)key_end(a, n);
   f16x8 kf[kHD / 16], vf[kHD / 16];
   {
     const f16* krow = a.qkv + (int64_t)n * ROW + (int64_t)(a.nq + g) * kHD + 8 * hl;
@@ -663,6 +659,10 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
       vf[s] = nval ? vf[s] : zero8();
     }
   }
+  int end_min = nval ? end : INT32_MAX;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) end_min = min(end_min, __shfl_xor(end_min, x));
+  end_min = __builtin_amdgcn_readfirstlane(end_min);
   f32x16 dkacc[kHD / 32], dvacc[kHD / 32];
 #pragma unroll
   for (int hb = 0; hb < kHD / 32; ++hb) dkacc[hb] = dvacc[hb] = zero16();
