@@ -204,8 +204,6 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
     if (wave == 0) key_ends_load(a, it, it.tb + t, ends[st], lane);
   };
   issue(0);
-  issue(1);
-  issue(2);
   // this lane's query and dO rows and statistics, loaded unconditionally and selected at once (the
   // compiler's wait for them stands here, not in the loop)
   f16x8 qf[kHD / 16], dof[kHD / 16];
@@ -248,8 +246,8 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
     else sacc[kb] = mfma(f, qf[s], s == 0 ? zero16() : sacc[kb]);
   };
   f16x8 fr[kAhead1];
-  // the wait for all three tiles costs no more than the query rows' own
   tile_barrier();
+  issue(1);   // behind the rows and tile 0, which the first products wait for
   f32x16 s_a[2], d_a[2], s_b[2], d_b[2];
   {
     const unsigned ka = fresh(krow), va = fresh(vrow);
@@ -261,6 +259,8 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
       if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(ka, va, i + kAhead1);
       __builtin_amdgcn_sched_barrier(0);
     }
+    tile_barrier();
+    issue(2);
     const unsigned ka1 = fresh(krow + kStageBytes), va1 = fresh(vrow + kStageBytes);
 #pragma unroll
     for (int i = 0; i < kAhead1; ++i) fr[i] = rd1(ka1, va1, i);
@@ -416,8 +416,6 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
     }
   };
   issue(0);
-  issue(1);
-  issue(2);
 
   // this lane's key and value rows as B operands, loaded unconditionally and selected at once
   // (the compiler's wait for them stands here, not in the loop)
@@ -467,6 +465,7 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
   f32x4 ls[2], dl[2];
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the row of zeros is written
   tile_barrier();
+  issue(1);   // behind the rows and tile 0, which the first products wait for
   f32x16 s_a[2], d_a[2], s_b[2], d_b[2];
   {
     const unsigned qa = fresh(qrow), da = fresh(drow);
@@ -478,6 +477,8 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
       if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(qa, da, i + kAhead1);
       __builtin_amdgcn_sched_barrier(0);
     }
+    tile_barrier();
+    issue(2);
     const unsigned qa1 = fresh(qrow + kStageBytes), da1 = fresh(drow + kStageBytes);
 #pragma unroll
     for (int i = 0; i < kAhead1; ++i) fr[i] = rd1(qa1, da1, i);
