@@ -11,11 +11,13 @@
 // Bound: a tile's step (64 queries x 128 keys, or 128 rows x 64 keys) keeps attn.hip's order at one
 // wave per SIMD, the next tile's products beside this tile's P and dS; it takes 2.1 us (dQ 1.7) at the
 // clock that power allows, 40 % of the matrix rate, S and dP computed for dK/dV and again for dQ.  An
-// item begins with 4 to 6 us for its rows and first tiles and ends with 2 to 3 us of stores.  Measured on
-// MI355X, 12 query / 2 KV heads (graph replays of the three launches): 8192 tokens, window 1024, 4 sinks
-// 258 us; 2048 tokens, window 256, 47; a prompt of 4096 with 16 answers of 512 1088 (623 TFLOP/s).
-// dQ in a launch of its own (two workgroups to a CU) took 267, 53 and 1014: here its blocks fill the
-// ends of the dK/dV walks.
+// item begins with 3 to 5 us for its rows and first tile and ends with 2 to 3 us of stores.  Neither the
+// operand reads (left out, a tile is 0 to 4 % faster) nor the exponentials beside S and dP (half of them
+// beside dK and dV: unchanged) bound a tile on their own.  Measured on MI355X, 12 query / 2 KV heads
+// (graph replays of the three launches): 8192 tokens, window 1024, 4 sinks 252 us; 2048 tokens, window
+// 256, 43; a prompt of 4096 with 16 answers of 512 1088 (623 TFLOP/s).  dQ in a launch of its own (two
+// workgroups to a CU) took 267, 53 and 1014 when these took 258, 47 and 1088: its blocks fill the ends of
+// the dK/dV walks.
 #include "attn_delta.h"
 #include "attn_span.h"
 

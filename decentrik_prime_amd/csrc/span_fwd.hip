@@ -33,12 +33,15 @@ __device__ __forceinline__ void redo_rows(const SpanArgs& a, int t0, int phase, 
 // Bound: per tile a wave has 32 MFMAs (1024 clocks), about as many clocks of exponentials and
 // conversions, and 48 LDS operand reads, one after the other for a wave on its own.  So the scores of
 // the next tile stand beside the exponentials of the current one (K runs a tile ahead of V), and a CU
-// holds two workgroups (two stages of K and V, 66 KB; 254 registers), whose first loads, barriers and
+// holds two workgroups (two stages of K and V, 66 KB; 227 registers), whose first loads, barriers and
 // stores stand beside the other's products.  Stacking a group's heads on the rows makes a block span
 // 128 / gin tokens: fewer masked keys at a window's edges, and answers of a token fill blocks.
 // Measured on MI355X, 12 query / 2 KV heads (graph replays): 16384 tokens, window 4096, 4 sinks 427 us
-// (846 TFLOP/s); 8192 tokens, window 1024, 87; a prompt of 8192 with 64 answers of a token 257; one
+// (846 TFLOP/s); 8192 tokens, window 1024, 84; a prompt of 8192 with 64 answers of a token 252; one
 // workgroup of 8 waves to a CU, the waves of a SIMD on alternate tiles, took 500, 100 and 302.
+// 20 tokens, one tile, take 7.4: launch 2.2, the item 0.5, first loads 1.9, the tile's code, run for the
+// first time, 2.5 (a further tile 1.1), the rows' stores.  A last tile without the next one's scores, or a
+// whole tile on its own unmasked, spilled registers.
 // Walks are cut where one would outlast the rest (k_attn._fwd_tiles): that prompt uncut 360 us.
 __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
     SpanArgs a, const int32_t* __restrict__ items, int n_slots, f16* __restrict__ out,

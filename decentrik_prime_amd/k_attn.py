@@ -253,15 +253,17 @@ def _key_blocks(key_runs, spans, gin, nkv):
 
 def _fwd_tiles(blocks):
     """Tiles per item of the forward at most: a little over the share of one of the 512 workgroups that run
-    at a time, two to a CU, and no fewer than make up for a partial."""
-    return max(6, int(0.6 * blocks[:, _TE].sum() / 256) + 1)
+    at a time, two to a CU, and no fewer than make up for a partial (over 15 batches 23.4 us; 24.1 with at
+    least 4, 24.3 with 8)."""
+    return max(5, int(0.6 * blocks[:, _TE].sum() / 256) + 1)
 
 
 def _bwd_cost(cost):
     """Cost per item of the backward at most: a CU's share of the whole (256 CUs, an item each at a time)
     and a little, so that no walk (a prompt's or a sink's keys over every later query) outlasts the rest,
-    and few partials are written."""
-    return int(1.25 * cost.sum() / 256) + 12
+    and few partials are written (over 13 batches 49.4 us; 50.4 with + 4 or + 12, 51.8 with + 18, 51.3 with a
+    factor of 1, 52.6 with 1.6)."""
+    return int(1.25 * cost.sum() / 256) + 8
 
 
 def _split_items(blocks, cost, most):
