@@ -377,8 +377,8 @@ def span_attention_forward(qkv, meta, nq, nkv, hd):
     attention_forward."""
     _check_span(qkv, meta, nq, nkv, hd)
     n, dev = meta.n_tokens, qkv.device
-    out = torch.empty((n, nq * hd), dtype=torch.float16, device=dev)
-    lse = torch.empty((nq, n), dtype=torch.float32, device=dev)
+    out = torch.empty(n, nq * hd, dtype=torch.float16, device=dev)
+    lse = torch.empty(nq, n, dtype=torch.float32, device=dev)
     ws = torch.empty(meta.fwd_bytes, dtype=torch.uint8, device=dev) if meta.fwd_bytes else None
     _launch(dev, _lib.lib().dk_attn_span_fwd, "dk_attn_span_fwd", qkv.data_ptr(), meta.spans.data_ptr(),
             meta.items.data_ptr(), meta.items.shape[0], meta.joins.data_ptr(), meta.joins.shape[0],
@@ -397,10 +397,10 @@ def span_attention_backward(qkv, out, lse, dout, meta, nq, nkv, hd):
         _t(t, (dt,), what, shape)
         if t.device != dev:
             raise ValueError(f"{what} is on {t.device}, qkv on {dev}")
-    delta = torch.empty((nq, n), dtype=torch.float32, device=dev)
-    dq = torch.empty((n, nq * hd), dtype=torch.float16, device=dev)
-    dk = torch.empty((n, nkv * hd), dtype=torch.float16, device=dev)
-    dv = torch.empty((n, nkv * hd), dtype=torch.float16, device=dev)
+    delta = torch.empty(nq, n, dtype=torch.float32, device=dev)
+    dq = torch.empty(n, nq * hd, dtype=torch.float16, device=dev)
+    dk = torch.empty(n, nkv * hd, dtype=torch.float16, device=dev)
+    dv = torch.empty(n, nkv * hd, dtype=torch.float16, device=dev)
     ws = torch.empty(meta.bwd_bytes, dtype=torch.uint8, device=dev) if meta.bwd_bytes else None
     _launch(dev, _lib.lib().dk_attn_span_bwd, "dk_attn_span_bwd", qkv.data_ptr(), out.data_ptr(),
             lse.data_ptr(), dout.data_ptr(), meta.spans.data_ptr(), meta.items_bwd.data_ptr(),
