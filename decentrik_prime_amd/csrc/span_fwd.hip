@@ -116,7 +116,7 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
   // tile t, whose scores are in sc: its softmax and O^T += V^T P^T, beside the scores of tile t + 1
   // into sn (after the last tile: of a stale stage, never used).  MASK: key j of the tile counts iff
   // j <= jlim and the key's end lies past this lane's token; the others' probabilities come out as 0, also
-  // where a lane has seen no key yet: kMasked lies as far below m_i's start as any score above it.
+  // where a lane has seen no key yet: kMasked, scaled, lies far below m_i's start, and that below any score.
   auto tile = [&](int t, f32x16 (&sc)[2], f32x16 (&sn)[2], auto mask_c) {
     constexpr bool MASK = decltype(mask_c)::value;
     const unsigned va = fresh(vcol + (unsigned)((t % kStages) * kTileHalves * 2));
