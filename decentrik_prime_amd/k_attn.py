@@ -224,13 +224,15 @@ def _query_blocks(runs, spans, nq, nkv):
     if (a0 + na > b0)[far].any():
         raise ValueError(f"rows of {row_bytes} bytes are too long for keys that far apart")
     nk = na + last + 1 - b0
-    # every row sees the first run, and of the second the keys from the last row's kbeg to t0
+    # every row sees the first run up to t0, also where both are one, and the keys from the last row's kbeg
+    # to t0
+    first = np.where(one, np.minimum(a1, t0 + 1) - a0, seen)
     lo = np.maximum(spans[last, 2], b0) - b0 + na
     hi = t0 - b0 + na + 1
     x = np.zeros((j0.size, 16), np.int64)
     x[:, _T0], x[:, _PHASE], x[:, _N_ROWS] = t0, j0 % gin, rows
     x[:, _A0], x[:, _NA], x[:, _B0], x[:, _NK] = a0, na, b0, nk
-    x[:, _F0] = np.where((lo == na) & (na == seen), hi, seen) // _KEYS
+    x[:, _F0] = np.where(lo <= first, hi, first) // _KEYS
     x[:, _F1] = -(-lo // _KEYS)
     x[:, _F2] = np.maximum(hi // _KEYS, x[:, _F1])
     x[:, _TE], x[:, _SLOT] = -(-nk // _KEYS), -1

@@ -217,3 +217,31 @@ def test_c_entry_refusals_before_any_launch():
         assert need == slots * 128 * 128 * 4
         assert bwd(n_units=slots) == bwd(n_units=slots, ws=p, nbytes=need - 1) == _lib.DK_ERR_WORKSPACE
     assert lib.dk_attn_span_workspace(0) == lib.dk_attn_span_bwd_workspace(0) == 0
+
+
+@pytest.mark.parametrize("nq,nkv", [(12, 2), (2, 2), (300, 2)])
+@pytest.mark.parametrize("near", [False, True])
+def test_tiles_that_every_row_sees_are_named_full(monkeypatch, nq, nkv, near):
+    """A tile of 64 keys that all rows of a block see whole runs without a mask: none is missed, whether
+    the block's keys are two runs or have grown together (a prompt with its first or only answer, a window
+    that meets the sinks)."""
+    if near:
+        monkeypatch.setattr(k_attn, "_REACH", 127 * 2 * HD * (nq + 2 * nkv))
+    gin = nq // nkv
+    metas = [k_attn.prefix_meta(g, nq, nkv, "cpu") for g in (
+        [(500, [200])], [(64, [64])], [(63, [1])], [(300, [1, 200, 70])], [(0, [150]), (200, [130])])]
+    metas += [k_attn.window_meta(*w, nq, nkv, "cpu") for w in (
+        ([700], 200, 130), ([700], 100, 600), ([300, 90], 64, 64), ([400], 1000, 0), ([400], 130, 4))]
+    for meta in metas:
+        s = np.asarray(meta.spans, np.int64)
+        named = 0
+        for it in np.asarray(meta.items, np.int64):
+            t0, phase, rows, g, a0, na, b0, nk, f0, f1, f2 = it[:11]
+            m = t0 + (phase + np.arange(rows))[:, None] // gin
+            j = np.arange(nk // 64 * 64)
+            key = np.where(j < na, a0 + j, b0 + j - na)
+            seen = ((j <= m - b0 + na) & (m < s[key, 3])).all(0).reshape(-1, 64).all(1)
+            t = np.arange(nk // 64)
+            np.testing.assert_array_equal((t < f0) | ((t >= f1) & (t < f2)), seen)
+            named += int(seen.sum())
+        assert named or meta.n_tokens < 128
