@@ -34,6 +34,7 @@ class PackedBatch:
     n_lab      tokens with a target
     B, T       batch rows and padded length
     groups     None, or the batch's (prompt length, [answer lengths]) (pack_answers)
+    copies_sorted None (one each), or [n] int64: the batch rows that hold each token, sorted order
     """
     lens: list
     ids: torch.Tensor
@@ -47,6 +48,7 @@ class PackedBatch:
     B: int
     T: int
     groups: list = None
+    copies_sorted: torch.Tensor = None
 
 
 def _row_length(mask_row):
@@ -105,20 +107,21 @@ def pack_answers(groups, vocab):
     answer, each as if it stood alone behind its prompt: the prompt's last token, whose target differs
     from answer to answer, begins each answer.  Returns None when the batch is not packable: no answers,
     an empty prompt or answer, or an id outside the vocabulary."""
-    shape, lens, ids, tgt, rows, longest = [], [], [], [], [], 0
+    shape, lens, ids, tgt, rows, copies, longest = [], [], [], [], [], [], 0
 
-    def piece(tokens, targets, row):
+    def piece(tokens, targets, row, held_by=1):
         lens.append(tokens.numel())
         ids.append(tokens)
         tgt.append(targets)
         rows.append(torch.full((tokens.numel(),), row, dtype=torch.int64))
+        copies.append(torch.full((tokens.numel(),), held_by, dtype=torch.int64))
     B = 0
     for prompt, answers in groups:
         prompt = torch.as_tensor(prompt, dtype=torch.int64, device="cpu")
         answers = [torch.as_tensor(a, dtype=torch.int64, device="cpu") for a in answers]
         if any(t.dim() != 1 or t.numel() == 0 for t in (prompt, *answers)) or not answers:
             return None
-        piece(prompt[:-1], torch.full((prompt.numel() - 1,), -1, dtype=torch.int64), B)
+        piece(prompt[:-1], torch.full((prompt.numel() - 1,), -1, dtype=torch.int64), B, len(answers))
         for a in answers:
             piece(torch.cat([prompt[-1:], a]), torch.cat([a, a.new_full((1,), -1)]), B)
             longest = max(longest, prompt.numel() + a.numel())
@@ -126,21 +129,23 @@ def pack_answers(groups, vocab):
         shape.append((prompt.numel() - 1, [1 + a.numel() for a in answers]))
     if B == 0:
         return None
-    ids, tgt, rows = torch.cat(ids), torch.cat(tgt), torch.cat(rows)
+    ids, tgt, rows, copies = torch.cat(ids), torch.cat(tgt), torch.cat(rows), torch.cat(copies)
     if int(ids.min()) < 0 or int(ids.max()) >= vocab:
         return None
     has = tgt >= 0
     perm = torch.sort((~has).to(torch.int8), stable=True).indices
     return PackedBatch(lens=lens, ids=ids, tgt=tgt, perm=perm, tgt_sorted=tgt[perm],
                        row_sorted=rows[perm], valid_sorted=has[perm], n_real=int(ids.numel()),
-                       n_lab=int(has.sum()), B=B, T=longest, groups=shape)
+                       n_lab=int(has.sum()), B=B, T=longest, groups=shape,
+                       copies_sorted=copies[perm])
 
 
 def batch_metrics(batch, stats):
     """The trainer's metrics of one packed batch from the head's per-token stats [n, 4] = (loss,
     entropy, hit, lse) in sorted order, on the host (solution/fast_qwen.py:1551-1565):
-    entropy = mean over all real tokens, accuracy = hits over tokens with a target, and per batch
-    row the mean loss over its tokens with a target and their count.  Sums in float64."""
+    entropy = mean over all real tokens (a shared prompt's once for every row that holds it),
+    accuracy = hits over tokens with a target, and per batch row the mean loss over its tokens with a
+    target and their count.  Sums in float64."""
     st = torch.as_tensor(stats).to("cpu", torch.float64)
     if st.dim() != 2 or st.shape[0] != batch.n_real or st.shape[1] < 3:
         raise ValueError(f"stats must be [{batch.n_real}, 4] in the batch's sorted order")
@@ -148,7 +153,10 @@ def batch_metrics(batch, stats):
     rows = torch.as_tensor(batch.row_sorted, dtype=torch.int64)
     loss_sum = torch.zeros(batch.B, dtype=torch.float64).index_add_(0, rows[valid], st[valid, 0])
     count = torch.bincount(rows[valid], minlength=batch.B)
-    return {"entropy": float(st[:, 1].sum()) / batch.n_real,
+    held_by = torch.ones(batch.n_real, dtype=torch.float64)
+    if batch.copies_sorted is not None:
+        held_by = torch.as_tensor(batch.copies_sorted).double()
+    return {"entropy": float((st[:, 1] * held_by).sum()) / float(held_by.sum()),
             "accuracy": float(st[valid, 2].sum()) / batch.n_lab if batch.n_lab else 0.0,
             "n_lab": batch.n_lab,
             "row_loss": [float(s) / max(int(c), 1) for s, c in zip(loss_sum, count)],

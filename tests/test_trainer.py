@@ -198,3 +198,46 @@ def test_pack_answers_refuses():
     for groups in ([], [([1, 2], [])], [([], [[1]])], [([1], [[]])], [([1], [[40]])], [([-1], [[3]])],
                    [([[1, 2]], [[3]])]):
         assert trainer.pack_answers(groups, vocab=40) is None
+
+
+def test_metrics_of_shared_prompts_are_those_of_rows_of_their_own():
+    """batch_metrics of a batch packed by pack_answers equal those of the same answers as rows with a
+    prompt each: a prompt's token counts once for every answer behind it."""
+    rng = np.random.default_rng(8)
+    groups = [(rng.integers(0, 40, p), [rng.integers(0, 40, a) for a in ans])
+              for p, ans in ((6, (3, 1, 4)), (1, (5,)), (9, (2, 2)))]
+    shared = trainer.pack_answers(groups, vocab=40)
+    whole = [(np.concatenate([p, a]), len(p)) for p, ans in groups for a in ans]
+    T = max(len(w) for w, _ in whole)
+    ids, mask, labels = (torch.zeros(len(whole), T, dtype=torch.int64) for _ in range(3))
+    labels -= 100
+    for b, (w, n) in enumerate(whole):
+        ids[b, :len(w)], mask[b, :len(w)] = torch.from_numpy(w), 1
+        labels[b, n:len(w)] = torch.from_numpy(w[n:])
+    rows = trainer.pack(ids, mask, labels, 40)
+    # (loss, entropy, hit, lse) of a token, by what stands before it and what comes next
+    known = {}
+
+    def stats(batch, before):
+        out = torch.zeros(batch.n_real, 4, dtype=torch.float64)
+        for i, t in enumerate(batch.perm.tolist()):
+            seen = tuple(before(t))
+            ent = known.setdefault(seen, rng.random())
+            tgt = int(batch.tgt[t])
+            loss, hit = known.setdefault((seen, tgt), (rng.random(), float(rng.integers(0, 2))))
+            out[i] = torch.tensor([loss if tgt >= 0 else 0.0, ent, hit if tgt >= 0 else 0.0, 0.0])
+        return out
+    from oracle import attn
+    vis = attn.prefix_visible(shared.groups)
+    ends = np.cumsum(rows.lens)
+    starts = ends - np.asarray(rows.lens)
+
+    def in_row(t):
+        return rows.ids[starts[np.searchsorted(ends, t, side="right")]:t + 1].tolist()
+    a = trainer.batch_metrics(shared, stats(shared, lambda t: shared.ids[np.nonzero(vis[t])[0]].tolist()))
+    b = trainer.batch_metrics(rows, stats(rows, in_row))
+    # sums of at most 60 values in [0, 1) in 64 bits, in another order
+    assert abs(a["entropy"] - b["entropy"]) < 60 * 2.0 ** -52
+    assert abs(a["accuracy"] - b["accuracy"]) < 2.0 ** -52
+    np.testing.assert_allclose(a["row_loss"], b["row_loss"], rtol=1e-14)
+    assert a["row_tokens"] == b["row_tokens"] and a["n_lab"] == b["n_lab"]
