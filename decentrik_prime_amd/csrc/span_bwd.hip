@@ -24,6 +24,7 @@
 namespace {
 
 constexpr int kUnitFloats = kBM * kHD;   // a partial of dQ; dK and dV take two
+constexpr int64_t kDeltaWgs = 1 << 16;   // of the delta launch at most: 2^20 rows a round
 
 // The tile ring of both backward kernels: a tile of two operands (kBN rows each) in one of four
 // LDS stages, filled by LDS DMA.  Wave w's instruction i fills chunks (4 i + w) 64 + lane of an
@@ -873,9 +874,8 @@ extern "C" int dk_attn_span_bwd(const void* qkv, const void* out, const float* l
     return DK_ERR_ALIGN;
   if (n_units > 0 && (!workspace || workspace_bytes < dk_attn_span_bwd_workspace(n_units)))
     return DK_ERR_WORKSPACE;
-  const int64_t pairs = n_tokens * nq, wgs = (pairs + 15) / 16;
-  if (n_items > INT32_MAX / kAThreads || n_joins > INT32_MAX / (4 * kAThreads) || wgs > INT32_MAX / kAThreads)
-    return DK_ERR_INVALID;
+  const int64_t pairs = n_tokens * nq, wgs = (pairs + 15) / 16 < kDeltaWgs ? (pairs + 15) / 16 : kDeltaWgs;
+  if (n_items > INT32_MAX / kAThreads || n_joins > INT32_MAX / (4 * kAThreads)) return DK_ERR_INVALID;
   hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)wgs), dim3(kAThreads), 0, stream,
                      (const f16*)out, (const f16*)dout, delta, n_tokens, nq);
   DK_CHECK_LAUNCH();

@@ -163,6 +163,9 @@ class SpanMeta:
         blocks = np.concatenate([_key_blocks(key_runs, spans, nq // nkv, nkv), blocks])
         cost = blocks[:, _TE] * _TILE_COST[blocks[:, _KIND]]
         items_b, joins_b, self.n_units = _split_items(blocks, cost, _bwd_cost(cost))
+        if max(len(items), len(items_b)) > MAX_SPAN_ITEMS or max(len(joins), len(joins_b)) > MAX_SPAN_JOINS:
+            raise ValueError(f"a batch of {max(len(items), len(items_b))} items and {max(len(joins), len(joins_b))} "
+                             f"split walks (at most {MAX_SPAN_ITEMS} and {MAX_SPAN_JOINS})")
         lib = _lib.lib()
         self.fwd_bytes = lib.dk_attn_span_workspace(self.n_slots)
         self.bwd_bytes = lib.dk_attn_span_bwd_workspace(self.n_units)
@@ -179,6 +182,10 @@ class SpanMeta:
 
 
 MAX_SPAN_TOKENS = (1 << 30) - 1
+# what a launch takes (include/dk.h): blocks of 128 rows of every run and KV head, their cuts, and twice that
+# in the backward; runs are sequences, sinks, prompts and groups' answers
+MAX_SPAN_ITEMS = ((1 << 31) - 1) // 256
+MAX_SPAN_JOINS = ((1 << 31) - 1) // 1024
 _KEYS = 64            # keys of a tile
 _ROWS = 128           # stacked query rows of a block
 _REACH = 0xfff00000   # DK_ATTN_SPAN_REACH_BYTES

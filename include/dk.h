@@ -178,7 +178,8 @@ int dk_attn_bwd(const void* qkv, const void* out, const float* lse, const void* 
  * [f1, f2).  slot -1: the block's rows of out and lse; slot s >= 0: partial s of the workspace
  * (dk_attn_span_workspace(n_slots) bytes, 256-byte aligned, n_slots the count of partials), which
  * joins [n_joins][8] int32 put together: t0, phase, rows, g, first slot, slots, 0, 0.  An entry that
- * names rows outside the batch or slots outside the workspace is skipped. */
+ * names rows outside the batch or slots outside the workspace is skipped.  Either direction takes up to
+ * 2^30 - 1 tokens, 2^23 - 1 items and 2^21 - 1 joins (DK_ERR_INVALID beyond). */
 #define DK_ATTN_SPAN_ITEM_INTS 16
 /* A tile with keys of both runs has them within this many bytes of qkv rows (an item that does not is
  * skipped, too; one whose na is a multiple of 64 has no such tile). */

@@ -504,3 +504,26 @@ def test_a_layer_around_it(torch):
         _near(have, want, 2.0 ** -11 * want.abs() + 2.0 ** -22 * (heads.abs().amax(2, keepdim=True)) + 2.0 ** -24,
               "rotated gradient")
     assert torch.equal(dqkv[:, (nq + nkv) * HD:], dv)
+
+
+def test_more_rows_than_the_delta_launch_has_lanes(torch):
+    """2^20 and some (token, query head) rows of a backward: delta's workgroups go round more than once.
+    One-token sequences, whose dv is the sum of the group's gradients and whose dq and dk are 0, behind
+    some longer ones that repeat at the end."""
+    nq, nkv = 48, 2
+    ones = (1 << 20) // nq
+    lens = [70, 3] + [1] * ones + [70, 3]
+    log(f"span attention, {sum(lens) * nq} rows")
+    meta = _meta(("window", lens, 40, 2), nq, nkv)
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=21)
+    qkv[-73:], dout[-73:] = qkv[:73], dout[:73]
+    got = _run(qkv, dout, meta, nq, nkv)
+    for t in (got[0], got[2], got[3], got[4]):
+        assert torch.equal(t[:73], t[-73:])
+    v, do = qkv[73:-73, (nq + nkv) * HD:].double().view(-1, nkv, HD), dout[73:-73].double().view(-1, nkv, nq // nkv, HD)
+    # dS = P (dO V - out dO): 0 but for the two sums' rounding, HD 2^-24 of their magnitudes, twice
+    mag = float((do.abs() * v[:, :, None].abs()).sum(3).amax())
+    lim = 2 * HD * 2.0 ** -24 * mag * 8 * HD ** -0.5 * (nq // nkv)
+    assert float(got[2][73:-73].abs().max()) <= lim and float(got[3][73:-73].abs().max()) <= lim
+    _near(got[4][73:-73].view(-1, nkv, HD), do.sum(2),
+          2.0 ** -10 * do.abs().sum(2) + 2.0 ** -11 * do.sum(2).abs() + 2.0 ** -24, "dv")

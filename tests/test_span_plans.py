@@ -245,3 +245,23 @@ def test_tiles_that_every_row_sees_are_named_full(monkeypatch, nq, nkv, near):
             np.testing.assert_array_equal((t < f0) | ((t >= f1) & (t < f2)), seen)
             named += int(seen.sum())
         assert named or meta.n_tokens < 128
+
+
+def test_plan_refuses_more_items_than_a_launch_takes(monkeypatch):
+    """A plan that is built can be run in both directions: what the launches do not take is refused here."""
+    meta = k_attn.window_meta([700, 1, 1], 90, 3, NQ, NKV, "cpu")
+    most = max(len(meta.items), len(meta.items_bwd))
+    assert len(meta.items_bwd) > len(meta.items)
+    assert k_attn.MAX_SPAN_ITEMS <= (1 << 31) // 256 and k_attn.MAX_SPAN_JOINS <= (1 << 31) // 1024
+    for limit in (most - 1, len(meta.items) - 1):
+        monkeypatch.setattr(k_attn, "MAX_SPAN_ITEMS", limit)
+        with pytest.raises(ValueError):
+            k_attn.window_meta([700, 1, 1], 90, 3, NQ, NKV, "cpu")
+    monkeypatch.setattr(k_attn, "MAX_SPAN_ITEMS", most)
+    k_attn.window_meta([700, 1, 1], 90, 3, NQ, NKV, "cpu")
+    monkeypatch.setattr(k_attn, "_fwd_tiles", lambda blocks: 1)
+    monkeypatch.setattr(k_attn, "MAX_SPAN_ITEMS", 1 << 20)
+    joins = len(k_attn.window_meta([700], 400, 3, NQ, NKV, "cpu").joins)
+    monkeypatch.setattr(k_attn, "MAX_SPAN_JOINS", joins - 1)
+    with pytest.raises(ValueError):
+        k_attn.window_meta([700], 400, 3, NQ, NKV, "cpu")
