@@ -243,7 +243,9 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
   static_assert(4 * 32 * kStride16 <= 2 * kStages * kTileHalves, "O staging in the ring");
   f16* ostage = ring + wave * 32 * kStride16;
   const float inv_l = __fdiv_rn(1.0f, l_i);   // rows past the block: not stored
-  float chk = __fmul_rn(l_i, 0.0f);           // NaN if anything below is not finite
+  // NaN if anything is not finite, also where P's rounding took a mean of values at the type's maximum
+  // past it (the redone row holds P in fp32)
+  float chk = __fmul_rn(l_i, 0.0f);
 #pragma unroll
   for (int hb = 0; hb < kHD / 32; ++hb)
 #pragma unroll
@@ -251,9 +253,8 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
       f16x4 o;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float ov = oacc[hb][4 * q + e];
-        chk = __builtin_fmaf(ov, 0.0f, chk);
-        o[e] = (f16)__fmul_rn(ov, inv_l);
+        o[e] = (f16)__fmul_rn(oacc[hb][4 * q + e], inv_l);
+        chk = __builtin_fmaf((float)o[e], 0.0f, chk);
       }
       *reinterpret_cast<f16x4*>(ostage + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = o;
     }
@@ -320,14 +321,14 @@ __global__ __launch_bounds__(kAThreads) void span_join_kernel(SpanArgs a, const 
     }
   }
   const float inv_l = __fdiv_rn(1.0f, l);
-  float chk = __fmul_rn(l, 0.0f);   // NaN if a value is not finite
+  float chk = __fmul_rn(l, 0.0f);   // NaN if a value is not finite, rounded
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     f16x4 x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      chk = __builtin_fmaf(o[q][e], 0.0f, chk);
       x[e] = (f16)__fmul_rn(o[q][e], inv_l);
+      chk = __builtin_fmaf((float)x[e], 0.0f, chk);
     }
     *reinterpret_cast<f16x4*>(stage + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = x;
   }

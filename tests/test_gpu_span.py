@@ -527,3 +527,27 @@ def test_more_rows_than_the_delta_launch_has_lanes(torch):
     assert float(got[2][73:-73].abs().max()) <= lim and float(got[3][73:-73].abs().max()) <= lim
     _near(got[4][73:-73].view(-1, nkv, HD), do.sum(2),
           2.0 ** -10 * do.abs().sum(2) + 2.0 ** -11 * do.sum(2).abs() + 2.0 ** -24, "dv")
+
+
+@pytest.mark.parametrize("cut", [False, True])
+def test_values_at_the_types_maximum(torch, monkeypatch, cut):
+    """Values of +-65504 throughout, most of a row's weight on one key of a later tile: their mean is
+    +-65504 whatever the weights, and no rounding of the weights (2^-11 of each, where 2^-12 more would
+    round to infinity) takes it past the type's range."""
+    from decentrik_prime_amd import k_attn
+    nq, nkv, n = 4, 1, 300
+    if cut:
+        monkeypatch.setattr(k_attn, "_fwd_tiles", lambda blocks: 2)
+    meta = _meta(("window", [n], n, 0), nq, nkv)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(15)
+    qkv = torch.zeros(n, (nq + 2 * nkv) * HD, device="cuda", dtype=torch.float16)
+    x = qkv.view(n, nq + 2 * nkv, HD)
+    x[:, :nq, 0] = 4 + 4 * torch.rand(n, nq, device="cuda", generator=g).half()
+    x[:, nq, 0] = -200.0
+    x[0, nq, 0], x[100, nq, 0] = 0.0, 6.0      # 3 to 6 in log2 units above key 0's score
+    x[:, nq + 1] = 65504.0
+    x[:, nq + 1, ::3] = -65504.0
+    out, lse = k_attn.span_attention_forward(qkv, meta, nq, nkv, HD)
+    assert bool(torch.isfinite(lse).all()) and bool(torch.isfinite(out).all())
+    _near(out.view(n, nq, HD), x[:, nq + 1:].double().expand(n, nq, HD), (2.0 ** -10 + 2.0 ** -11) * 65504, "out")
