@@ -1,13 +1,19 @@
 // Forward of the attention over part of the keys (attn_span.h): with s = scale q . k over the keys that a
-// row sees (log2 units), m = max s, l = sum 2^(s - m): out = sum 2^(s - m) v / l, lse = m + log2 l, m and
-// l running over the tiles.  P is rounded to fp16 for its product (half a step, 2^-11 of each value; the
-// sum l takes it unrounded), everything else is fp32 up to the one rounding of out.  Built with the MFMA
-// accumulators in VGPRs like attn_fwd.hip.
+// row sees (log2 units), m a reference near max s, l = sum 2^(s - m): out = sum 2^(s - m) v / l,
+// lse = m + log2 l, m and l running over the tiles.  P = 2^(s - m) is rounded to fp16 for its product (the
+// sum l takes it unrounded), everything else is fp32 up to the one rounding of out.  That rounding is half a
+// step, 2^-11 of each value, down to 2^-21 of the row's largest P, and 2^-32 of the largest below: m lies
+// kUp under the largest score, so the largest P is 2^7 to 2^15 and the type's subnormals begin that much
+// further down (behind a sink that takes a row's weight and has no value, small P are all there is).
+// Built with the MFMA accumulators in VGPRs like attn_fwd.hip.
 #include "attn_span.h"
 
 namespace {
 
 constexpr int kStages = 2;   // of each operand's ring
+// A row's reference m is set kUp (log2 units) under its largest score, and again once a score exceeds m by
+// more than kTop: P stays below 2^15, half of fp16's range.
+constexpr float kUp = 7.0f, kTop = 15.0f;
 // a partial: O (part_off) and the rows' m and l
 constexpr int kPartFloats = kBM * kHD + 2 * kBM;
 
@@ -139,11 +145,10 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
 #pragma unroll
       for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[kb][v]);
     mx = half_max(mx);
-    // m_i moves (and O and l are rescaled) only when some lane's maximum exceeds it by more than
-    // 2^8, so p stays below 256
+    // m_i moves (and O and l are rescaled) only when some lane's maximum exceeds it by more than kTop
     const float mt = __fmul_rn(mx, a.qk_scale);
-    if (__builtin_amdgcn_ballot_w64(mt > m_i + 8.0f) != 0) {
-      const float m_new = fmaxf(m_i, mt);
+    if (__builtin_amdgcn_ballot_w64(mt > m_i + kTop) != 0) {
+      const float m_new = fmaxf(m_i, __fsub_rn(mt, kUp));
       const float alpha = ex2(__fsub_rn(m_i, m_new));
       l_i = __fmul_rn(l_i, alpha);
       m_i = m_new;

@@ -551,3 +551,35 @@ def test_values_at_the_types_maximum(torch, monkeypatch, cut):
     out, lse = k_attn.span_attention_forward(qkv, meta, nq, nkv, HD)
     assert bool(torch.isfinite(lse).all()) and bool(torch.isfinite(out).all())
     _near(out.view(n, nq, HD), x[:, nq + 1:].double().expand(n, nq, HD), (2.0 ** -10 + 2.0 ** -11) * 65504, "out")
+
+
+@pytest.mark.parametrize("spec,cut", [(("window", [5000], 4500, 1), False), (("window", [5000], 4500, 1), True),
+                                      (("prefix", [(4500, [300, 1])]), False)])
+def test_small_weights_behind_a_sink(torch, monkeypatch, spec, cut):
+    """A first key that takes nearly all of every row's weight and has no value of its own, as sinks do:
+    the output is what the thousands of others, 2^-18 to 2^-26 each, add up to.  P's rounding to fp16 is
+    2^-11 of the value, or 2^-32 of the row's largest below its normal range (the tiles hold P times 2^7)."""
+    from decentrik_prime_amd import k_attn
+    nq, nkv = 4, 2
+    if cut:
+        monkeypatch.setattr(k_attn, "_fwd_tiles", lambda blocks: 9)
+    log(f"span attention, small weights behind a sink, {spec}")
+    meta = _meta(spec, nq, nkv)
+    n = meta.n_tokens
+    qkv, _ = _inputs(torch, n, nq, nkv, seed=16, scale=0.1)
+    x = qkv.view(n, nq + 2 * nkv, HD)
+    x[:, :nq, 0] = torch.tensor([6.5, 7.3, 8.1, 9.4], device="cuda").half()
+    x[:, nq:nq + nkv, 0] = 0.0
+    x[0, nq:nq + nkv, 0] = 21.6
+    x[:, nq + nkv:] = 1.0 + x[:, nq + nkv:].abs()
+    x[0, nq + nkv:] = 0.0
+    out, lse = k_attn.span_attention_forward(qkv, meta, nq, nkv, HD)
+    vis = torch.from_numpy(_visible(spec)).cuda()
+    for h in range(nq):
+        q, k, v = (x[:, i].double() for i in (h, nq + h // 2, nq + nkv + h // 2))
+        sc = torch.where(vis, HD ** -0.5 * (q @ k.t()), -float("inf"))
+        p = torch.softmax(sc, 1)
+        floor = 2.0 ** -32 * p.amax(1, keepdim=True) * (vis.double() @ v.abs())
+        # the scores' fp32 sums: up to 26 in log2 units, P off by 2^-24 HD 2^5 at the most, below 2^-11
+        _near(out.view(n, nq, HD)[:, h], p @ v, 1.5 * 2.0 ** -10 * (p @ v) + floor + 2.0 ** -25, f"head {h}: out")
+        _near(lse[h], torch.logsumexp(sc, 1) / math.log(2.0), 2.0 ** -12, f"head {h}: lse")
