@@ -250,7 +250,7 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
   const float inv_l = __fdiv_rn(1.0f, l_i);   // rows past the block: not stored
   // NaN if anything is not finite, also where P's rounding took a mean of values at the type's maximum
   // past it (the redone row holds P in fp32)
-  float chk = __fmul_rn(l_i, 0.0f);
+  f16x4 chk = {0, 0, 0, 0};
 #pragma unroll
   for (int hb = 0; hb < kHD / 32; ++hb)
 #pragma unroll
@@ -259,12 +259,13 @@ __global__ __launch_bounds__(kAThreads, 2) void span_fwd_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         o[e] = (f16)__fmul_rn(oacc[hb][4 * q + e], inv_l);
-        chk = __builtin_fmaf((float)o[e], 0.0f, chk);
       }
+      chk = __builtin_elementwise_fma(o, f16x4{0, 0, 0, 0}, chk);
       *reinterpret_cast<f16x4*>(ostage + c * kStride16 + hb * 32 + 8 * q + 4 * hl) = o;
     }
-  chk = __fadd_rn(chk, __shfl_xor(chk, 32));
-  if (chk != 0.0f) bad[row] = 1;
+  float sum = __fadd_rn((float)(chk[0] + chk[1]), (float)(chk[2] + chk[3]));
+  sum = __fadd_rn(__builtin_fmaf(l_i, 0.0f, sum), __shfl_xor(sum, 32));
+  if (sum != 0.0f) bad[row] = 1;
   else if (mval && hl == 0) lse[(int64_t)h * a.n_tokens + m] = __fadd_rn(m_i, log2f(l_i));
   __syncthreads();
   store_rows(a, it, wave, lane, ostage, bad, out);
