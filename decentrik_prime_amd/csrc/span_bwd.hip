@@ -3,10 +3,17 @@
 // summed over the queries that see a key and the heads of its group.  Three launches: delta; dK/dV
 // and dQ on MFMA tiles; the partials of walks that were split, if any.
 //
-// P and dS are rounded to fp16 for their products (half a step, 2^-11 of each value), and out, which
-// delta is taken from, is the returned fp16 one; sums, statistics and results are fp32 up to one
-// rounding of dq, dk and dv.  Against 64 bits (2-norms) dq and dk come out 3.3e-4 off, of which dS 2.2e-4,
-// their own rounding 2.1e-4 and delta 1.2e-4; dv 2.9e-4.  fp32 gradients would hold no more than that.
+// P and dS are rounded to fp16 for their products, half a step, 2^-11 of each value.  dS is P, about 1 over
+// the keys that a row sees, times dout's size, so as it stands it would lie below 2^-14, where fp16's steps
+// no longer shrink, for ordinary windows and gradients: both are held 2^up up (P by a larger exponent,
+// which costs nothing for a row on a lane and one subtraction a value in dK/dV; the sums are scaled back
+// in fp32), which puts the end of the shrinking steps at 2^-30 of its dO row's norm for dQ, and for dK and
+// dV at 2^-39 of the largest |dP - delta| that the walk's norms allow (up 15 at most: at 2^-40).  up is
+// taken from dout and from what a block's keys are seen by, and moves nothing but where those steps end.
+// out, which delta is taken from, is the returned fp16 one; sums, statistics and results are fp32 up to one
+// rounding of dq, dk and dv.  Against 64 bits (2-norms) dq and dk come out 3.2e-4 off, of which dS 2.2e-4,
+// their own rounding 2.1e-4 and delta 1.2e-4, dv 2.9e-4, for any size of dout whose gradients fp16 holds
+// (at dout ~ 1e-4 their own rounding is 3e-3 of them).
 //
 // Bound: a tile's step (64 queries x 128 keys, or 128 rows x 64 keys) keeps attn.hip's order at one
 // wave per SIMD, the next tile's products beside this tile's P and dS; it takes 2.1 us (dQ 1.7) at the
@@ -74,6 +81,117 @@ __device__ __forceinline__ void tile_barrier() {
 }
 
 constexpr int kAhead1 = 6, kAhead2 = 4;
+
+// The up of the top.  dQ, per query row with |dO| = r: 2^up r lies in [2^5, 2^6) (up from 0 to 24).  |dS| is
+// at most max |dP| / 2 (P (1 - P) of a difference of two), so it fits where the values' norms stay below
+// 2^11; a row that does not is redone, as for any overflow.
+constexpr int kUpRows = 24;
+__device__ __forceinline__ int clamp_up(int up, int most) { return up < 0 ? 0 : up > most ? most : up; }
+__device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }   // x >= 0
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(127 + e) << 23); }
+__device__ __forceinline__ int up_of_row(float r2) { return clamp_up(5 - (exponent(r2) >> 1), kUpRows); }
+__device__ __forceinline__ float norm2(const f16x8 (&x)[kHD / 16]) {   // of a row whose halves two lanes hold
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kHD / 16; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+      s = __builtin_amdgcn_fdot2(f16x2{x[i][e], x[i][e + 1]}, f16x2{x[i][e], x[i][e + 1]}, s, false);
+  return __fadd_rn(s, __shfl_xor(s, 32));
+}
+
+// dK and dV, per walk: |dP - delta| is at most (largest norm of the walk's dO rows) (largest norm of the
+// block's value rows) + (largest |delta|), and 2^up times that at most 2^15, which with P at most 1 fits
+// (up from 0 to 15, for P itself).  What is not finite is left out: its rows and keys are redone whatever
+// up is.  The norms' exponents come with the deltas (attn_delta.h), which a walk reads once before its first
+// tile's P: 0.5 to 1 us an item, behind the first products.  Setting up tile by tile instead (looking at the
+// next tile beside dK's products and rescaling the sums where it was too much) took 9 to 13 % of the whole.
+constexpr int kUpKeys = 15;
+struct WalkPeak {   // not negative, so the bits order them
+  unsigned code, delta, v2;   // norm_code of the largest norm, bits of the largest |delta| and |v|^2
+};
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned finite_bits(float x) {   // of |x|, 0 where it is not finite
+  const unsigned b = __float_as_uint(x) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+// The deltas of the walk over query tiles [tb, te) (per_head to a head) of the heads from h0 on, kFlight to a
+// thread at a time: 8 heads by 256 rows, 4 by 512, 2 by 1024 or 1 by 2048.  Where the walk has more than one
+// head each is taken whole; what lies past the last row or head is that row or head again.
+struct WalkScan {
+  static constexpr int kFlight = 8;
+  const float* row;
+  int64_t n_tokens;
+  int rows, heads, shift, r0, hb;
+  __device__ __forceinline__ WalkScan(const float* delta, int64_t n, int h0, int k0, int qend, int per_head,
+                                      int tb, int te)
+      : n_tokens(n), r0(0), hb(0) {
+    const int first = tb / per_head;
+    heads = (te - 1) / per_head - first + 1;
+    const int lo = heads > 1 ? 0 : (tb - first * per_head) * kBN;
+    const int hi = heads > 1 ? qend - k0 : (te - first * per_head) * kBN;
+    rows = (hi < qend - k0 ? hi : qend - k0) - lo;
+    shift = heads > 4 ? 3 : heads > 2 ? 2 : heads - 1;
+    row = delta + (int64_t)(h0 + first) * n + k0 + lo;
+  }
+  __device__ __forceinline__ void load(float (&d)[kFlight]) const {
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const int h = hb + (u & ((1 << shift) - 1));
+      const unsigned r = (unsigned)r0 + (unsigned)(u >> shift) * kAThreads + threadIdx.x, last = (unsigned)rows - 1;
+      d[u] = *reinterpret_cast<const float*>(
+          reinterpret_cast<const char*>(row + (h < heads ? h : heads - 1) * n_tokens) + (r < last ? r : last) * 4u);
+    }
+  }
+  __device__ __forceinline__ bool next() {
+    r0 += (kFlight >> shift) * kAThreads;
+    if (r0 < rows) return true;
+    r0 = 0;
+    hb += kFlight;
+    return hb < heads;
+  }
+};
+// This thread's peak, from its first loads and the rest of the walk's.
+__device__ __forceinline__ WalkPeak walk_peak(WalkScan scan, float (&d)[WalkScan::kFlight]) {
+  WalkPeak p{0, 0, 0};
+  for (;;) {
+#pragma unroll
+    for (int u = 0; u < WalkScan::kFlight; ++u) {
+      const unsigned b = finite_bits(d[u]);
+      p.code = larger(p.code, b & (kNormCodes - 1));
+      p.delta = larger(p.delta, b);
+    }
+    if (!scan.next()) return p;
+    scan.load(d);
+  }
+}
+// the largest of the wave's lanes, in every lane: within the rows of 16, then on to the next rows
+template <int kCtrl>
+__device__ __forceinline__ unsigned larger_dpp(unsigned x) {
+  return larger(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, 0xf, 0xf, false));
+}
+__device__ __forceinline__ unsigned wave_largest(unsigned x) {
+  x = larger_dpp<0x118>(larger_dpp<0x114>(larger_dpp<0x112>(larger_dpp<0x111>(x))));
+  return (unsigned)__builtin_amdgcn_readlane((int)larger_dpp<0x143>(larger_dpp<0x142>(x)), 63);
+}
+// the wave's part into peaks, read behind a barrier
+__device__ __forceinline__ void peak_out(const WalkPeak& p, float v2, int wave, WalkPeak* peaks) {
+  const WalkPeak w{wave_largest(p.code), wave_largest(p.delta), wave_largest(finite_bits(v2))};
+  if ((threadIdx.x & 63) == 0) peaks[wave] = w;
+}
+__device__ __forceinline__ int up_of_walk(const WalkPeak* peaks) {
+  WalkPeak p = peaks[0];
+#pragma unroll
+  for (int w = 1; w < kAThreads / 64; ++w) {
+    p.code = larger(p.code, peaks[w].code);
+    p.delta = larger(p.delta, peaks[w].delta);
+    p.v2 = larger(p.v2, peaks[w].v2);
+  }
+  // |v| < 2^(exponent(|v|^2) / 2 + 1)
+  const float bound = __fadd_rn(pow2(norm_exponent((int)p.code) + (exponent(__uint_as_float(p.v2)) >> 1) + 1),
+                                __uint_as_float(p.delta));
+  return __builtin_amdgcn_readfirstlane(clamp_up(14 - exponent(bound), kUpKeys));
+}
 
 // The rows (or keys) whose result is not finite, recomputed over exactly what they see: 0 times a NaN
 // or infinity of a masked row is not 0.  bad: row flags in LDS, written before a barrier.
@@ -232,6 +350,8 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
     lse_m = mval ? lse_m : 0.0f;
     dl_m = mval ? dl_m : 0.0f;
   }
+  const int up = up_of_row(norm2(dof));
+  const float up_lse = __fsub_rn((float)up, lse_m);
   if (threadIdx.x < kBM) bad[threadIdx.x] = 0;
   f32x16 dqacc[kHD / 32];
 #pragma unroll
@@ -243,9 +363,12 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
   auto rd1 = [&](unsigned ka, unsigned va, int i) {
     return lds_read8((((i >> 1) & 1) ? va : ka) ^ (unsigned)(32 * (i >> 2)), (i & 1) * 32 * kHD * 2);
   };
+  f32x16 delta0;   // what dP^T begins with, for dP - delta
+#pragma unroll
+  for (int v = 0; v < 16; ++v) delta0[v] = -dl_m;
   auto product = [&](f32x16 (&sacc)[2], f32x16 (&dpacc)[2], const f16x8& f, int i) {
     const int s = i >> 2, kb = i & 1;
-    if ((i >> 1) & 1) dpacc[kb] = mfma(f, dof[s], s == 0 ? zero16() : dpacc[kb]);
+    if ((i >> 1) & 1) dpacc[kb] = mfma(f, dof[s], s == 0 ? delta0 : dpacc[kb]);
     else sacc[kb] = mfma(f, qf[s], s == 0 ? zero16() : sacc[kb]);
   };
   f16x8 fr[kAhead1];
@@ -282,7 +405,7 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           sc[q >> 2][4 * (q & 3) + e] =
-              (8 * q + e <= lim) & (m < e4[e]) ? sc[q >> 2][4 * (q & 3) + e] : -1.0e30f;
+              ((8 * q + e <= lim) & (m < e4[e])) ? sc[q >> 2][4 * (q & 3) + e] : -1.0e30f;
       }
     }
     const unsigned nst = (unsigned)((t + 1) % kBwdStages) * kStageBytes;
@@ -299,8 +422,8 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
         if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(ka, va, i + kAhead1);
       }
       const int kb = i >> 4, v = i & 15;
-      const float p = ex2(__builtin_fmaf(sc[kb][v], a.qk_scale, -lse_m));
-      dc[kb][v] = __fmul_rn(p, __fsub_rn(dc[kb][v], dl_m));
+      const float p = ex2(__builtin_fmaf(sc[kb][v], a.qk_scale, up_lse));
+      dc[kb][v] = __fmul_rn(p, dc[kb][v]);
       if (i & 1) dsf[i >> 3].h[(i >> 1) & 3] = pinned(dc[kb][v - 1], dc[kb][v]);
       if (i >= 32 - kAhead2) gr[i - (32 - kAhead2)] = rd2(i - (32 - kAhead2));
       if constexpr (MORE) __builtin_amdgcn_sched_barrier(0);
@@ -338,6 +461,11 @@ __device__ __forceinline__ void dq_item(const SpanArgs& a, const int32_t* items,
     }
   }
   step(t, s_a, d_a, s_b, d_b, Last{});
+  const float back = pow2(-up);
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) dqacc[hb][v] = __fmul_rn(dqacc[hb][v], back);
   __syncthreads();
   if (it.slot >= 0) {
     float* part = parts + (int64_t)it.slot * kUnitFloats;
@@ -378,7 +506,8 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
                                           const f16* __restrict__ dout, const float* __restrict__ lse,
                                           const float* __restrict__ delta, f16* __restrict__ dk,
                                           f16* __restrict__ dv, float* __restrict__ parts, f16* Qs,
-                                          f16* Ds, float (*lse_s)[kBN], float (*dl_s)[kBN], int* bad) {
+                                          f16* Ds, float (*lse_s)[kBN], float (*dl_s)[kBN], int* bad,
+                                          WalkPeak* peaks) {
   const int32_t* p = items + (int64_t)idx * kItemInts;
   auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(p[k]); };
   const int k0 = u(0), nk = u(2), g = u(3), qend = u(4), tb = u(11), te = u(12), slot = u(13);
@@ -420,10 +549,12 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
   };
   issue(0);
 
-  // this lane's key and value rows as B operands, loaded unconditionally and selected at once
-  // (the compiler's wait for them stands here, not in the loop)
+  // this lane's key row and its value row negated as B operands, loaded unconditionally and selected at
+  // once (the compiler's wait for them, and for the walk's first deltas, stands here, not in the loop)
   const int end = (int)key_end(a, n);
   f16x8 kf[kHD / 16], vf[kHD / 16];
+  const WalkScan scan(delta, a.n_tokens, g * gin, k0, qend, per_head, tb, te);
+  float first[WalkScan::kFlight];
   {
     const f16* krow = a.qkv + (int64_t)n * ROW + (int64_t)(a.nq + g) * kHD + 8 * hl;
     const f16* vrow = krow + (int64_t)a.nkv * kHD;
@@ -432,12 +563,13 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
       kf[s] = *reinterpret_cast<const f16x8*>(krow + 16 * s);
       vf[s] = *reinterpret_cast<const f16x8*>(vrow + 16 * s);
     }
+    scan.load(first);
 #pragma unroll
     for (int s = 0; s < kHD / 16; ++s) asm volatile("" : "+v"(kf[s]), "+v"(vf[s]));
 #pragma unroll
     for (int s = 0; s < kHD / 16; ++s) {
       kf[s] = nval ? kf[s] : zero8();
-      vf[s] = nval ? vf[s] : zero8();
+      vf[s] = nval ? -vf[s] : zero8();
     }
   }
   // the first end among the wave's keys
@@ -450,14 +582,15 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
   for (int hb = 0; hb < kHD / 32; ++hb) dkacc[hb] = dvacc[hb] = zero16();
   const unsigned qrow = lds_addr(Qs) + row_base(lane), drow = lds_addr(Ds) + row_base(lane);
   const unsigned qcol = lds_addr(Qs) + col_base(lane), dcol = lds_addr(Ds) + col_base(lane);
-  // operand i of a tile's products S = Q K^T and dP = dO V^T (queries qb * 32 + (row of the
-  // result), keys on the lanes): sub-step i / 4, dP for i / 2 odd, query half i % 2
+  // operand i of a tile's products S = Q K^T and then delta - dP = delta + dO (-V)^T (queries qb * 32 +
+  // (row of the result), keys on the lanes): sub-step i % 16 / 2, query half i % 2.  The second begin with
+  // delta in their accumulators, read beside the first.
   auto rd1 = [&](unsigned qa, unsigned da, int i) {
-    return lds_read8((((i >> 1) & 1) ? da : qa) ^ (unsigned)(32 * (i >> 2)), (i & 1) * 32 * kHD * 2);
+    return lds_read8((i < 16 ? qa : da) ^ (unsigned)(32 * ((i & 15) >> 1)), (i & 1) * 32 * kHD * 2);
   };
   auto product = [&](f32x16 (&sacc)[2], f32x16 (&dpacc)[2], const f16x8& f, int i) {
-    const int s = i >> 2, qb = i & 1;
-    if ((i >> 1) & 1) dpacc[qb] = mfma(f, vf[s], s == 0 ? zero16() : dpacc[qb]);
+    const int s = (i & 15) >> 1, qb = i & 1;
+    if (i >= 16) dpacc[qb] = mfma(f, vf[s], dpacc[qb]);
     else sacc[qb] = mfma(f, kf[s], s == 0 ? zero16() : sacc[qb]);
   };
   // the statistics of rows 8 g + 4 (l / 32) + 0..3 of the tile in stage st (g = 0..7)
@@ -465,13 +598,19 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
     return *reinterpret_cast<const f32x4*>(&tab[st][8 * g + 4 * hl]);
   };
   f16x8 fr[kAhead1];
-  f32x4 ls[2], dl[2];
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the row of zeros is written
+  f32x4 ls[2];
+  auto delta_in = [&](f32x16 (&d)[2], int st, int g) {
+    const f32x4 x = stat(dl_s, st, g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[g >> 2][4 * (g & 3) + e] = x[e];
+  };
   tile_barrier();
   issue(1);   // behind the rows and tile 0, which the first products wait for
   f32x16 s_a[2], d_a[2], s_b[2], d_b[2];
   {
     const unsigned qa = fresh(qrow), da = fresh(drow);
+#pragma unroll
+    for (int g = 0; g < 8; ++g) delta_in(d_a, 0, g);
 #pragma unroll
     for (int i = 0; i < kAhead1; ++i) fr[i] = rd1(qa, da, i);
 #pragma unroll
@@ -480,14 +619,17 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
       if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(qa, da, i + kAhead1);
       __builtin_amdgcn_sched_barrier(0);
     }
+    peak_out(walk_peak(scan, first), norm2(vf), wave, peaks);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the row of zeros and the peaks are written
     tile_barrier();
     issue(2);
     const unsigned qa1 = fresh(qrow + kStageBytes), da1 = fresh(drow + kStageBytes);
 #pragma unroll
     for (int i = 0; i < kAhead1; ++i) fr[i] = rd1(qa1, da1, i);
     ls[0] = stat(lse_s, 0, 0);
-    dl[0] = stat(dl_s, 0, 0);
   }
+  const int up = up_of_walk(peaks);
+  const float upf = (float)up;
   auto step = [&](int t, f32x16 (&sc)[2], f32x16 (&dc)[2], f32x16 (&sn)[2], f32x16 (&dn)[2],
                   auto more_c) {
     constexpr bool MORE = decltype(more_c)::value;   // tile t + 1 exists
@@ -528,14 +670,12 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
       if constexpr (MORE) {
         product(sn, dn, fr[i % kAhead1], i);
         if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(qa, da, i + kAhead1);
+        if (i < 8) delta_in(dn, (t + 1) % kBwdStages, i);
       }
       const int qb = i >> 4, v = i & 15, g = i >> 2;
-      if ((i & 3) == 0 && g + 1 < 8) {
-        ls[(g + 1) & 1] = stat(lse_s, lrow, g + 1);
-        dl[(g + 1) & 1] = stat(dl_s, st, g + 1);
-      }
-      sc[qb][v] = ex2(__builtin_fmaf(sc[qb][v], scale, -ls[g & 1][i & 3]));
-      dc[qb][v] = __fmul_rn(sc[qb][v], __fsub_rn(dc[qb][v], dl[g & 1][i & 3]));
+      if ((i & 3) == 0 && g + 1 < 8) ls[(g + 1) & 1] = stat(lse_s, lrow, g + 1);
+      sc[qb][v] = ex2(__builtin_fmaf(sc[qb][v], scale, __fsub_rn(upf, ls[g & 1][i & 3])));
+      dc[qb][v] = __fmul_rn(sc[qb][v], dc[qb][v]);
       if (i & 1) {
         pf[i >> 3].h[(i >> 1) & 3] = pinned(sc[qb][v - 1], sc[qb][v]);
         dsf[i >> 3].h[(i >> 1) & 3] = pinned(dc[qb][v - 1], dc[qb][v]);
@@ -549,7 +689,7 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
     }
     const unsigned nst2 = (unsigned)((t + 2) % kBwdStages) * kStageBytes;
     const unsigned qa2 = fresh(qrow + nst2), da2 = fresh(drow + nst2);
-    // dV += P^T dO, dK += dS^T Q over the tile's 64 queries, 16 per step
+    // dV += P^T dO, -dK += -dS^T Q over the tile's 64 queries, 16 per step
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const int hb = (i >> 1) & 3;
@@ -560,7 +700,6 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
         // (past the last tile: a stale stage, never used)
         if (i >= 32 - kAhead1) fr[i - (32 - kAhead1)] = rd1(qa2, da2, i - (32 - kAhead1));
         if (i == 28) ls[0] = stat(lse_s, (t + 1) % kBwdStages, 0);
-        if (i == 29) dl[0] = stat(dl_s, (t + 1) % kBwdStages, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -582,6 +721,14 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
     }
   }
   step(t, s_a, d_a, s_b, d_b, Last{});
+  const float back = pow2(-up);
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      dkacc[hb][v] = __fmul_rn(dkacc[hb][v], -back);
+      dvacc[hb][v] = __fmul_rn(dvacc[hb][v], back);
+    }
   __syncthreads();
   if (slot >= 0) {
     float* part = parts + (int64_t)slot * kUnitFloats;
@@ -607,7 +754,8 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
                                             const f16* __restrict__ dout, const float* __restrict__ lse,
                                             const float* __restrict__ delta, f16* __restrict__ dk,
                                             f16* __restrict__ dv, float* __restrict__ parts, f16* Qs,
-                                            f16* Ds, float (*lse_s)[kBN], float (*dl_s)[kBN], int* bad) {
+                                            f16* Ds, float (*lse_s)[kBN], float (*dl_s)[kBN], int* bad,
+                                            WalkPeak* peaks) {
   const int32_t* p = items + (int64_t)idx * kItemInts;
   auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(p[k]); };
   const int k0 = u(0), nk = u(2), g = u(3), qend = u(4), tb = u(11), te = u(12), slot = u(13);
@@ -647,6 +795,8 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
   issue(1);
   const int end = (int)key_end(a, n);
   f16x8 kf[kHD / 16], vf[kHD / 16];
+  const WalkScan scan(delta, a.n_tokens, g * gin, k0, qend, per_head, tb, te);
+  float first[WalkScan::kFlight];
   {
     const f16* krow = a.qkv + (int64_t)n * ROW + (int64_t)(a.nq + g) * kHD + 8 * hl;
     const f16* vrow = krow + (int64_t)a.nkv * kHD;
@@ -655,6 +805,7 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
       kf[s] = *reinterpret_cast<const f16x8*>(krow + 16 * s);
       vf[s] = *reinterpret_cast<const f16x8*>(vrow + 16 * s);
     }
+    scan.load(first);
 #pragma unroll
     for (int s = 0; s < kHD / 16; ++s) asm volatile("" : "+v"(kf[s]), "+v"(vf[s]));
 #pragma unroll
@@ -675,6 +826,10 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
   const unsigned qrow = lds_addr(Qs) + row_base(lane) + hoff, drow = lds_addr(Ds) + row_base(lane) + hoff;
   const unsigned qcol = lds_addr(Qs) + col_base(lane) + hoff, dcol = lds_addr(Ds) + col_base(lane) + hoff;
   int walk = tb % per_head;   // the step's first tile within its head
+  peak_out(walk_peak(scan, first), norm2(vf), wave, peaks);
+  __syncthreads();            // the peaks are written
+  const int up = up_of_walk(peaks);
+  const float upf = (float)up;
   for (int s = 0; s < n_steps; ++s) {
     tile_barrier();   // the step's tiles are there, and every wave is done with those before
     issue(2 * s + 2);
@@ -705,7 +860,7 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int v = 4 * q + e, off = 8 * q + e;
-        float x = __builtin_fmaf(sc[v], a.qk_scale, -l[e]);
+        float x = __builtin_fmaf(sc[v], a.qk_scale, __fsub_rn(upf, l[e]));
         if (masked) x = ((off >= lo) & (off < hi)) ? x : -1.0e30f;
         const float pv = ex2(x);
         pf[v >> 3][v & 7] = (f16)pv;
@@ -724,6 +879,14 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
   }
   __syncthreads();
   // the waves' sums, in wave order: 16 KB a wave of each, then wave w takes columns 32 w .. + 31
+  const float back = pow2(-up);
+#pragma unroll
+  for (int hb = 0; hb < kHD / 32; ++hb)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      dkacc[hb][v] = __fmul_rn(dkacc[hb][v], back);
+      dvacc[hb][v] = __fmul_rn(dvacc[hb][v], back);
+    }
   float* kx = reinterpret_cast<float*>(Qs);
   float* vx = reinterpret_cast<float*>(Ds);
 #pragma unroll
@@ -774,12 +937,15 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_kernel(
   __shared__ __attribute__((aligned(1024))) f16 T1[kBwdStages * kTileHalves];
   __shared__ __attribute__((aligned(16))) float lse_s[kBwdStages + 1][kBN], dl_s[kBwdStages][kBN];
   __shared__ int bad[kBM];
+  __shared__ WalkPeak peaks[kAThreads / 64];
   const int idx = (int)blockIdx.x;
   const int kind = __builtin_amdgcn_readfirstlane(items[(int64_t)idx * kItemInts + 14]);
   if (kind == 2)
-    dkdv_narrow(a, items, idx, n_units, dout, lse, delta, dk, dv, parts, T0, T1, lse_s, dl_s, bad);
+    dkdv_narrow(a, items, idx, n_units, dout, lse, delta, dk, dv, parts, T0, T1, lse_s, dl_s, bad,
+                peaks);
   else if (kind == 1)
-    dkdv_item(a, items, idx, n_units, dout, lse, delta, dk, dv, parts, T0, T1, lse_s, dl_s, bad);
+    dkdv_item(a, items, idx, n_units, dout, lse, delta, dk, dv, parts, T0, T1, lse_s, dl_s, bad,
+              peaks);
   else
     dq_item(a, items, idx, n_units, dout, lse, delta, dq, parts, T0, T1,
             reinterpret_cast<int (*)[kBN]>(lse_s), bad);
@@ -876,7 +1042,7 @@ extern "C" int dk_attn_span_bwd(const void* qkv, const void* out, const float* l
     return DK_ERR_WORKSPACE;
   const int64_t pairs = n_tokens * nq, wgs = (pairs + 15) / 16 < kDeltaWgs ? (pairs + 15) / 16 : kDeltaWgs;
   if (n_items > INT32_MAX / kAThreads || n_joins > INT32_MAX / (4 * kAThreads)) return DK_ERR_INVALID;
-  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)wgs), dim3(kAThreads), 0, stream,
+  hipLaunchKernelGGL(attn_delta_kernel<true>, dim3((unsigned)wgs), dim3(kAThreads), 0, stream,
                      (const f16*)out, (const f16*)dout, delta, n_tokens, nq);
   DK_CHECK_LAUNCH();
   hipLaunchKernelGGL(span_bwd_kernel, dim3((unsigned)n_items), dim3(kAThreads), 0, stream, a, items,

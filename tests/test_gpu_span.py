@@ -583,3 +583,126 @@ def test_small_weights_behind_a_sink(torch, monkeypatch, spec, cut):
         # the scores' fp32 sums: up to 26 in log2 units, P off by 2^-24 HD 2^5 at the most, below 2^-11
         _near(out.view(n, nq, HD)[:, h], p @ v, 1.5 * 2.0 ** -10 * (p @ v) + floor + 2.0 ** -25, f"head {h}: out")
         _near(lse[h], torch.logsumexp(sc, 1) / math.log(2.0), 2.0 ** -12, f"head {h}: lse")
+
+
+def _spread(x, y=1.0):
+    """The square of a 2-norm's expected error when every value of x is rounded to fp16 on its own (at most
+    half a step, 2^-11, evenly spread: a third of the square) and weighted by y."""
+    return 2.0 ** -22 / 3 * (x.square() * y).sum()
+
+
+def _check_norms(torch, spec, nq, nkv, qkv, dout, got, rows=None, what=""):
+    """dq, dk and dv of the tokens `rows` (all) against the formulas in 2-norms: P and dS rounded to fp16 on
+    their own, delta from the returned out (rounded, and P before it), and the results' own rounding, which
+    is taken as it is.  Half as much again is allowed for what the sums' errors, 2^-24 a term, and the
+    chance of the rest may add."""
+    vis = torch.from_numpy(_visible(spec)).cuda()
+    n, gin, sm = qkv.shape[0], nq // nkv, HD ** -0.5
+    rows = slice(0, n) if rows is None else rows
+    x = qkv.double().view(n, nq + 2 * nkv, HD)
+    dq, dk, dv = (t.double().view(n, -1, HD)[rows] for t in got[2:])
+    wk, wv = (torch.zeros(n, nkv, HD, dtype=torch.float64, device="cuda") for _ in range(2))
+    ek, ev = [0.0] * nkv, [0.0] * nkv
+    part = torch.zeros(n, 1, dtype=torch.float64, device="cuda")
+    part[rows] = 1.0
+
+    def near(got, want, spread, name):
+        own = (want.half().double() - want).square().sum()
+        err, lim = float((got - want).norm()), 1.5 * float((own + spread).sqrt())
+        log(f"{what}{name}: 2-norm error {err / float(want.norm()):.3g}, at most {lim / float(want.norm()):.3g}")
+        assert err <= lim, f"{what}{name}: {err:.3g} > {lim:.3g}"
+    for h in range(nq):
+        g = h // gin
+        q, k, v = x[:, h], x[:, nq + g], x[:, nq + nkv + g]
+        do = dout.view(n, nq, HD)[:, h].double()
+        p = torch.softmax(torch.where(vis, sm * (q @ k.t()), -float("inf")), 1)
+        o = p @ v
+        ds = p * (do @ v.t() - (o * do).sum(1, keepdim=True))
+        # delta's error per row: out's rounding and, before it, P's
+        off = 2.0 ** -22 / 3 * ((o.square() + p.square() @ v.square()) * do.square()).sum(1, keepdim=True)
+        near(dq[:, h], (sm * (ds @ k))[rows], sm * sm * (_spread(ds * part, k.square().sum(1)) +
+                                                         (off * part * (p @ k).square()).sum()), f"head {h} dq")
+        wk[:, g] += sm * (ds.t() @ q)
+        wv[:, g] += p.t() @ do
+        ek[g] += sm * sm * (_spread(ds * part.t(), q.square().sum(1, keepdim=True)) +
+                            ((p * part.t()).square() * off * q.square().sum(1, keepdim=True)).sum())
+        ev[g] += _spread(p * part.t(), do.square().sum(1, keepdim=True))
+    for g in range(nkv):
+        near(dk[:, g], wk[rows, g], ek[g], f"KV head {g} dk")
+        near(dv[:, g], wv[rows, g], ev[g], f"KV head {g} dv")
+
+
+@pytest.mark.parametrize("size", [300.0, 1.0, 1e-3, 1e-4])
+@pytest.mark.parametrize("spec,cut", [(("window", [2500], 1500, 4), False), (("window", [2500, 40], 2500, 0), True),
+                                      (("prefix", [(1400, [300, 1, 200]), (0, [90])]), False)])
+def test_gradients_of_any_size(torch, monkeypatch, spec, cut, size):
+    """Walks of some thousand keys with dout large and small: dS is P times dout's size, and the roundings
+    stay those of each value whatever that is."""
+    from decentrik_prime_amd import k_attn
+    nq, nkv = 4, 2
+    if cut:
+        monkeypatch.setattr(k_attn, "_fwd_tiles", lambda blocks: 7)
+        monkeypatch.setattr(k_attn, "_bwd_cost", lambda cost: 60)
+    log(f"span attention, dout ~ {size}, {spec}")
+    meta = _meta(spec, nq, nkv)
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=17)
+    dout = (dout.float() * size).half()
+    _check_norms(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv))
+
+
+@pytest.mark.parametrize("cut", [False, True])
+def test_gradients_of_several_sizes_in_a_batch(torch, monkeypatch, cut):
+    """Small gradients beside large ones of another sequence or group, and behind a prompt whose own are 0
+    (a loss over the answers alone)."""
+    from decentrik_prime_amd import k_attn
+    nq, nkv = 4, 2
+    if cut:
+        monkeypatch.setattr(k_attn, "_bwd_cost", lambda cost: 40)
+    for spec, small in ((("window", [70, 1100, 300], 900, 4), slice(70, 1170)),
+                        (("prefix", [(300, [20, 7]), (900, [200, 150])]), slice(327, 1577))):
+        log(f"span attention, gradients of several sizes, {spec}")
+        meta = _meta(spec, nq, nkv)
+        qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=18)
+        sizes = torch.full((meta.n_tokens, 1), 200.0, device="cuda")
+        sizes[small] = 1e-4
+        if spec[0] == "prefix":
+            sizes[327:327 + 900] = 0.0
+        dout = (dout.float() * sizes).half()
+        _check_norms(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv), small, "the small ones, ")
+
+
+def test_even_weights_over_many_keys(torch):
+    """Queries of 0 give every key that they see the same weight, 2^-16 at the end: out and dv are plain
+    sums."""
+    nq, nkv, n = 1, 1, 70000
+    log(f"span attention, even weights over {n} keys")
+    meta = _meta(("window", [n], n, 0), nq, nkv)
+    qkv, dout = _inputs(torch, n, nq, nkv, seed=19)
+    qkv[:, :HD] = 0.0
+    qkv[:, 2 * HD:] += 1.0
+    out, lse, _, dk, dv = _run(qkv, dout, meta, nq, nkv)
+    m = torch.arange(1, n + 1, device="cuda", dtype=torch.float64)[:, None]
+    v, do = qkv[:, 2 * HD:].double(), dout.double()
+    want = v.cumsum(0) / m
+    # P is 2^7 exactly: the sums' errors of fp32 (n 2^-24 of the magnitudes at the most) and out's rounding
+    _near(out, want, n * 2.0 ** -24 * v.abs().cumsum(0) / m + 2.0 ** -11 * want.abs() + 2.0 ** -25, "out")
+    _near(lse[0], m[:, 0].log2(), 2.0 ** -12, "lse")
+    assert float(dk.abs().max()) == 0.0
+    sums = (do / m).flip(0).cumsum(0).flip(0)
+    spread = 2.0 ** -22 / 3 * ((do / m).square().flip(0).cumsum(0)).sum()
+    own = (sums.half().double() - sums).square().sum()
+    err, lim = float((dv.double() - sums).norm()), 1.5 * float((own + spread).sqrt())
+    assert err <= lim, f"dv: {err:.3g} > {lim:.3g}"
+
+
+@pytest.mark.parametrize("scale", [1e-2, 1e3])
+def test_gradients_with_values_of_any_size(torch, scale):
+    """Small and very large values: dS in fp16 overflows for the largest, and those rows are redone."""
+    nq, nkv = 4, 2
+    spec = ("window", [1200], 1000, 4)
+    log(f"span attention, values ~ {scale}")
+    meta = _meta(spec, nq, nkv)
+    qkv, dout = _inputs(torch, meta.n_tokens, nq, nkv, seed=20)
+    qkv[:, (nq + nkv) * HD:] *= scale
+    dout = (dout.float() * (1.0 if scale < 1 else 1e-2)).half()
+    _check_norms(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv))
