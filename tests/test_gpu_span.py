@@ -706,3 +706,94 @@ def test_gradients_with_values_of_any_size(torch, scale):
     qkv[:, (nq + nkv) * HD:] *= scale
     dout = (dout.float() * (1.0 if scale < 1 else 1e-2)).half()
     _check_norms(torch, spec, nq, nkv, qkv, dout, _run(qkv, dout, meta, nq, nkv))
+
+
+def test_sinks_of_rows_past_four_gigabytes(torch):
+    """dk and dv of the sinks of a sequence of 4.6 GB of qkv rows: the walks whose query tiles lie furthest
+    from their first, cut and joined, each value a sum over six million rows.  P from the returned lse and
+    delta from the returned out; the other rows' results are at least finite."""
+    nq, nkv, window, sinks = 12, 2, 70, 5
+    gin, sm = nq // nkv, HD ** -0.5
+    n = (1 << 32) // (2 * HD * (nq + 2 * nkv)) + 70000
+    log(f"span attention, sinks of one sequence of {n} tokens")
+    meta = _meta(("window", [n], window, sinks), nq, nkv)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(23)
+    qkv = torch.randn(n, (nq + 2 * nkv) * HD, device="cuda", generator=g, dtype=torch.float16)
+    dout = torch.randn(n, nq * HD, device="cuda", generator=g, dtype=torch.float16)
+    out, lse, dq, dk, dv = _run(qkv, dout, meta, nq, nkv)
+    for t in (out, lse, dq, dk, dv):
+        assert bool(torch.isfinite(t).all())
+    wk, wv = (torch.zeros(nkv, sinks, HD, dtype=torch.float64, device="cuda") for _ in range(2))
+    ek, ev = [0.0] * nkv, [0.0] * nkv
+    keys = qkv[:sinks].double().view(sinks, nq + 2 * nkv, HD)
+    for m0 in range(0, n, 1 << 15):
+        m = torch.arange(m0, min(m0 + (1 << 15), n), device="cuda")
+        seen = m[:, None] >= torch.arange(sinks, device="cuda")
+        for h in range(nq):
+            kv, cols = h // gin, slice(h * HD, (h + 1) * HD)
+            q, o, do = (t[m0:m0 + m.numel(), cols].double() for t in (qkv, out, dout))
+            p = torch.where(seen, torch.exp2(q @ keys[:, nq + kv].t() * (sm / math.log(2.0)) -
+                                             lse[h, m, None].double()), 0.0)
+            ds = p * (do @ keys[:, nq + nkv + kv].t() - (o * do).sum(1, keepdim=True))
+            wk[kv] += sm * (ds.t() @ q)
+            wv[kv] += p.t() @ do
+            ek[kv] += sm * sm * _spread(ds, q.square().sum(1, keepdim=True))
+            ev[kv] += _spread(p, do.square().sum(1, keepdim=True))
+    for t, want, spread, what in ((dk, wk, ek, "dk"), (dv, wv, ev, "dv")):
+        for kv in range(nkv):
+            got = t[:sinks].view(sinks, nkv, HD)[:, kv].double()
+            # the fp32 sums' errors, 2^-24 a step of walks of some thousand steps, are far below the roundings
+            own = (want[kv].half().double() - want[kv]).square().sum()
+            err, lim = float((got - want[kv]).norm()), 1.5 * float((own + spread[kv]).sqrt())
+            log(f"KV head {kv} {what}: {err / float(want[kv].norm()):.3g}, at most {lim / float(want[kv].norm()):.3g}")
+            assert err <= lim, what
+
+
+@pytest.mark.parametrize("cut", [False, True])
+def test_growing_scores_forward_and_backward(torch, monkeypatch, cut):
+    """test_growing_scores for both heads, lse and the gradients, and with walks cut so that the partials'
+    maxima lie far apart: the backward forms P again from lse, at scores up to 190 in log2 units."""
+    from decentrik_prime_amd import k_attn
+    nq, nkv, sm = 2, 1, HD ** -0.5
+    if cut:
+        monkeypatch.setattr(k_attn, "_fwd_tiles", lambda blocks: 2)
+        monkeypatch.setattr(k_attn, "_bwd_cost", lambda cost: 8)
+    for spec in (("window", [700], 150, 3), ("prefix", [(300, [100, 200])])):
+        log(f"span attention, growing scores forward and backward, {spec}, cut {cut}")
+        meta = _meta(spec, nq, nkv)
+        n = meta.n_tokens
+        qkv, dout = _inputs(torch, n, nq, nkv, seed=5, scale=0.3)
+        qkv[:, 2 * HD] = (0.25 * meta.positions).half()
+        qkv[:, 0] = qkv[:, HD] = 8.0
+        out, lse, dq, dk, dv = _run(qkv, dout, meta, nq, nkv)
+        vis = torch.from_numpy(_visible(spec)).cuda()
+        x = qkv.double().view(n, nq + 2, HD)
+        k, v = x[:, 2], x[:, 3]
+        wk, wv, lk, lv = (torch.zeros(n, HD, dtype=torch.float64, device="cuda") for _ in range(4))
+        # s is off by HD 2^-24 of its 190 at most, lse by 2^-23 of its size and the sum's log2: P, relative,
+        # by HD 2^-24 190 ln 2 < 2^-9.9; with its rounding, 2^-11, and the sums', below 2^-9
+        rel = 2.0 ** -9
+        for h in range(nq):
+            q, do = x[:, h], dout.view(n, nq, HD)[:, h].double()
+            sc = torch.where(vis, sm * (q @ k.t()), -float("inf"))
+            assert float(sc[vis].max()) / math.log(2.0) < 190
+            p = torch.softmax(sc, 1)
+            o = p @ v
+            lo = rel * (p @ v.abs()) + 2.0 ** -11 * o.abs() + 2.0 ** -24
+            _near(out.view(n, nq, HD)[:, h], o, lo, f"head {h}: out")
+            _near(lse[h], torch.logsumexp(sc, 1) / math.log(2.0), HD * 2.0 ** -24 * 190 + 2.0 ** -12, f"head {h}: lse")
+            dl = (o * do).sum(1, keepdim=True)
+            ds = p * (do @ v.t() - dl)
+            eds = torch.where(vis, 1.5 * rel * ds.abs() + 2.0 ** -30 + HD * 2.0 ** -23 * p * (
+                do.abs() @ v.abs().t() + (o * do).abs().sum(1, keepdim=True)) +
+                (lo * do.abs()).sum(1, keepdim=True) * p + 2.0 ** -19 * dl.abs() * p, 0.0)
+            want = sm * (ds @ k)
+            _near(dq.view(n, nq, HD)[:, h], want, sm * (eds @ k.abs()) + 2.0 ** -11 * want.abs() + 2.0 ** -24,
+                  f"head {h}: dq")
+            wk += sm * (ds.t() @ q)
+            lk += sm * (eds.t() @ q.abs())
+            wv += p.t() @ do
+            lv += torch.where(vis, rel * p + 2.0 ** -30, 0.0).t() @ do.abs()
+        _near(dk, wk, lk + 2.0 ** -11 * wk.abs() + 2.0 ** -24, "dk")
+        _near(dv, wv, lv + 2.0 ** -11 * wv.abs() + 2.0 ** -24, "dv")
