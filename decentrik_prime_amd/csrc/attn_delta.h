@@ -37,8 +37,7 @@ __global__ __launch_bounds__(kAThreads) void attn_delta_kernel(const f16* __rest
       float r = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) r = __builtin_fmaf((float)gv[j], (float)gv[j], r);
-#pragma unroll
-      for (int x = 1; x < 16; x <<= 1) r = __fadd_rn(r, __shfl_xor(r, x));
+      r = sum16(r);
       const unsigned bits = ((__float_as_uint(s) + kNormCodes / 2) & ~(unsigned)(kNormCodes - 1)) | norm_code(r);
       s = __builtin_fabsf(s) < INFINITY ? __uint_as_float(bits) : s;
     }
