@@ -15,13 +15,13 @@
 // of which dS 2.2e-4, their own rounding 2.1e-4 and delta 1.2e-4, dv 2.9e-4, for any size of dout whose
 // gradients fp16 holds (at dout ~ 1e-4 their own rounding is 2 to 4e-3 of them, and nearly all of it).
 //
-// Bound: a tile's step (64 queries x 128 keys, or 128 rows x 64 keys) keeps attn.hip's order at one
-// wave per SIMD, the next tile's products (in dK/dV all of S before dP) beside this tile's P and dS; it
-// takes 2.1 us (dQ 1.7) at the
-// clock that power allows, 40 % of the matrix rate, S and dP computed for dK/dV and again for dQ.  An
-// item begins with 3 to 5 us for its rows and first tile and ends with 2 to 3 us of stores.  Neither the
-// operand reads (left out, a tile is 0 to 4 % faster) nor the exponentials beside S and dP (half of them
-// beside dK and dV: unchanged) bound a tile on their own; what the rest of a tile waits for is not known.
+// Bound: a tile's step (64 queries x 128 keys, or 128 rows x 64 keys) keeps attn.hip's order at one wave
+// per SIMD, the next tile's products (in dK/dV all of S before dP) beside this tile's P and dS; it takes
+// 2.1 us (dQ 1.7) at the clock that power allows, 40 % of the matrix rate, S and dP computed for dK/dV and
+// again for dQ.  An item begins with 3 to 5 us for its rows and first tile and ends with 2 to 3 us of
+// stores.  Neither the operand reads (left out, a tile is 0 to 4 % faster) nor the exponentials beside S
+// and dP (half of them beside dK and dV: unchanged) bound a tile on their own; what the rest of a tile
+// waits for is not known.
 // Measured on MI355X, 12 query / 2 KV heads (the three launches, back to back): 8192 tokens, window 1024,
 // 4 sinks 236 us; 2048 tokens, window 256, 41; a prompt of 4096 with 16 answers of 512 1090 (621 TFLOP/s).
 // A subtraction a value more in dK/dV's P is 1 % of a tile; begun with delta in its accumulators, dP needs
