@@ -500,7 +500,7 @@ extern "C" int dk_attn_bwd(const void* qkv, const void* out, const float* lse, c
       !dk_aligned(delta, 4) || !dk_aligned(dq, 16) || !dk_aligned(dkp, 4) || !dk_aligned(dvp, 4))
     return DK_ERR_ALIGN;
   const int64_t pairs = n_tokens * nq;
-  hipLaunchKernelGGL(attn_delta_kernel<false>, dim3((unsigned)((pairs + 15) / 16)), dim3(kAThreads), 0,
+  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)((pairs + 15) / 16)), dim3(kAThreads), 0,
                      stream, (const f16*)out, (const f16*)dout, delta, n_tokens, nq);
   DK_CHECK_LAUNCH();
   hipLaunchKernelGGL(attn_bwd_kernel, dim3((unsigned)(2 * n_blocks * nq)), dim3(kAThreads), 0,

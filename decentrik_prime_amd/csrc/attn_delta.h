@@ -4,19 +4,8 @@
 
 namespace {
 
-// The exponent of a row's norm in kNormCodes steps, norm < 2^norm_exponent(code): 2^-11, below which the
-// span backward makes no difference, to 2^20, above the norm of 128 fp16 values.
-constexpr int kNormCodes = 32;
-__device__ __forceinline__ int norm_code(float norm2) {   // finite
-  const int c = (((int)(__float_as_uint(norm2) >> 23) - 127 + 2) >> 1) + 11;
-  return c < 0 ? 0 : c > kNormCodes - 1 ? kNormCodes - 1 : c;
-}
-__device__ __forceinline__ int norm_exponent(int code) { return code - 11; }
-
 // delta[h][t] = sum_d O[t][h][d] dO[t][h][d] (solution/k_attn.py:84-94): 16 lanes per (token, head), in
-// rounds where the launch has fewer.  With kNorms a finite delta is rounded to 19 bits (2^-19 of its value,
-// where O's rounding has made it off by more) and its last 5 hold norm_code of dO's row.
-template <bool kNorms>
+// rounds where the launch has fewer
 __global__ __launch_bounds__(kAThreads) void attn_delta_kernel(const f16* __restrict__ o,
                                                                const f16* __restrict__ dout,
                                                                float* __restrict__ delta,
@@ -33,14 +22,6 @@ __global__ __launch_bounds__(kAThreads) void attn_delta_kernel(const f16* __rest
     for (int j = 0; j < 8; ++j) s = __fadd_rn(s, __fmul_rn((float)ov[j], (float)gv[j]));
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) s = __fadd_rn(s, __shfl_xor(s, x));
-    if constexpr (kNorms) {
-      float r = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) r = __builtin_fmaf((float)gv[j], (float)gv[j], r);
-      r = sum16(r);
-      const unsigned bits = ((__float_as_uint(s) + kNormCodes / 2) & ~(unsigned)(kNormCodes - 1)) | norm_code(r);
-      s = __builtin_fabsf(s) < INFINITY ? __uint_as_float(bits) : s;
-    }
     if ((threadIdx.x & 15) == 0) delta[(int64_t)hh * n_tokens + t] = s;
   }
 }

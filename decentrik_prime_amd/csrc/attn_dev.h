@@ -132,17 +132,6 @@ struct Frag8 {
   }
 };
 
-// x and its value in another lane of the 16, by a DPP control
-template <int kCtrl>
-__device__ __forceinline__ float add_dpp(float x) {
-  return __fadd_rn(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), kCtrl, 0xf, 0xf, true)));
-}
-// the sum over 16 lanes: those 1 and 2 further in a quad, then the other quad of the half (half mirror) and
-// the other half (mirror), the same sum in every lane
-__device__ __forceinline__ float sum16(float x) {
-  return add_dpp<0x140>(add_dpp<0x141>(add_dpp<0x4e>(add_dpp<0xb1>(x))));
-}
-
 // 2^x on the hardware exponential (v_exp_f32); arguments here are <= 0 (scores minus their row
 // maximum or log-sum-exp), results below the normal range flush to zero.
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -192,12 +192,18 @@ __device__ __forceinline__ void store8(f16* row, const Row8& r) {   // by the fi
 }
 __device__ __forceinline__ Row8 fill8(float x) { return Row8{{x, x, x, x, x, x, x, x}}; }
 
-// the dot product of the quarter's row with one held the same way
+// x and its value in another lane of the 16, by a DPP control
+template <int kCtrl>
+__device__ __forceinline__ float add_dpp(float x) {
+  return __fadd_rn(x, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), kCtrl, 0xf, 0xf, true)));
+}
+// the dot product of the quarter's row with one held the same way: lanes 1 and 2 further in a quad,
+// then the other quad of the half (half mirror) and the other half (mirror), the same sum in every lane
 __device__ __forceinline__ float row_dot(const Row8& a, const f16x8& b) {
   float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) s = __builtin_fmaf(a.x[i], (float)b[i], s);
-  return sum16(s);
+  return add_dpp<0x140>(add_dpp<0x141>(add_dpp<0x4e>(add_dpp<0xb1>(s))));
 }
 __device__ __forceinline__ void row_add(Row8& r, float w, const f16x8& b) {
 #pragma unroll

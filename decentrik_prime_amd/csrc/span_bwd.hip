@@ -8,8 +8,8 @@
 // no longer shrink, for ordinary windows and gradients: both are held 2^up up (P by a larger exponent,
 // which costs nothing for a row on a lane and one subtraction a value in dK/dV; the sums are scaled back
 // in fp32), which puts the end of the shrinking steps at 2^-30 of its dO row's norm for dQ, and for dK and
-// dV at 2^-39 of the largest |dP - delta| that the walk's norms allow (up 15 at most: at 2^-40).  up is
-// taken from dout and from what a block's keys are seen by, and moves nothing but where those steps end.
+// dV at 2^-34 of the walk's largest |delta| (up 15 at most: at 2^-40).  up is taken from dout and, for a
+// block of keys, from the rows that see any of them, and moves nothing but where those steps end.
 // out, which delta is taken from, is the returned fp16 one; sums, statistics and results are fp32 up to one
 // rounding of dq, dk and dv.  Against 64 bits (2-norms) dq comes out 3.0 to 3.6e-4 off and dk 3.1 to 3.4e-4,
 // of which dS 2.2e-4, their own rounding 2.1e-4 and delta 1.2e-4, dv 2.9e-4, for any size of dout whose
@@ -102,18 +102,18 @@ __device__ __forceinline__ float norm2(const f16x8 (&x)[kHD / 16]) {   // of a r
   return __fadd_rn(s, __shfl_xor(s, 32));
 }
 
-// dK and dV, per walk: |dP - delta| is at most (largest norm of the walk's dO rows) (largest norm of the
-// block's value rows) + (largest |delta|), and 2^up times that at most 2^15, which with P at most 1 fits
-// (up from 0 to 15, for P itself).  What is not finite is left out: its rows and keys are redone whatever
-// up is.  The norms' exponents come with the deltas (attn_delta.h), which a walk reads once before its first
-// tile's P: 0.5 to 1 us an item, behind the first products.  Setting up tile by tile instead (looking at the
-// next tile beside dK's products and rescaling the sums where it was too much) took 9 to 13 % of the whole.
+// dK and dV, per walk: 2^up times the walk's largest |delta| lies in [2^9, 2^10) (up from 0 to 15, for P
+// itself), so that dS fits up to 2^6 times that.  delta is the mean of a row's dP under P, about |dP| times the
+// root of the sum of P^2, which is no less than P, so over a walk's rows no dS comes out larger by much: over
+// 5686 blocks of drawn batches by 1.4 at most, 11 in a walk of a few rows.  Where one is 2^6 times larger,
+// in a walk of a row or two whose delta happens to vanish, its key is redone as for any overflow.  A walk
+// reads its deltas once before its first tile's P, behind the first products.  Setting up tile by tile
+// instead (looking at the next tile beside dK's products and rescaling the sums where it was too much)
+// took 9 to 13 % of the whole; norms' exponents in the deltas' last bits, for a bound, left noise in dS
+// where it cancels to 0 (a row that sees one key).
 constexpr int kUpKeys = 15;
-struct WalkPeak {   // not negative, so the bits order them
-  unsigned code, delta, v2;   // norm_code of the largest norm, bits of the largest |delta| and |v|^2
-};
 __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
-__device__ __forceinline__ unsigned finite_bits(float x) {   // of |x|, 0 where it is not finite
+__device__ __forceinline__ unsigned finite_bits(float x) {   // of |x|, which they order; 0 where it is not finite
   const unsigned b = __float_as_uint(x) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
 }
@@ -153,16 +153,12 @@ struct WalkScan {
     return hb < heads;
   }
 };
-// This thread's peak, from its first loads and the rest of the walk's.
-__device__ __forceinline__ WalkPeak walk_peak(WalkScan scan, float (&d)[WalkScan::kFlight]) {
-  WalkPeak p{0, 0, 0};
+// The bits of this thread's largest, from its first loads and the rest of the walk's.
+__device__ __forceinline__ unsigned walk_peak(WalkScan scan, float (&d)[WalkScan::kFlight]) {
+  unsigned p = 0;
   for (;;) {
 #pragma unroll
-    for (int u = 0; u < WalkScan::kFlight; ++u) {
-      const unsigned b = finite_bits(d[u]);
-      p.code = larger(p.code, b & (kNormCodes - 1));
-      p.delta = larger(p.delta, b);
-    }
+    for (int u = 0; u < WalkScan::kFlight; ++u) p = larger(p, finite_bits(d[u]));
     if (!scan.next()) return p;
     scan.load(d);
   }
@@ -177,22 +173,13 @@ __device__ __forceinline__ unsigned wave_largest(unsigned x) {
   return (unsigned)__builtin_amdgcn_readlane((int)larger_dpp<0x143>(larger_dpp<0x142>(x)), 63);
 }
 // the wave's part into peaks, read behind a barrier
-__device__ __forceinline__ void peak_out(const WalkPeak& p, float v2, int wave, WalkPeak* peaks) {
-  const WalkPeak w{wave_largest(p.code), wave_largest(p.delta), wave_largest(finite_bits(v2))};
-  if ((threadIdx.x & 63) == 0) peaks[wave] = w;
+__device__ __forceinline__ void peak_out(unsigned p, int wave, unsigned* peaks) {
+  p = wave_largest(p);
+  if ((threadIdx.x & 63) == 0) peaks[wave] = p;
 }
-__device__ __forceinline__ int up_of_walk(const WalkPeak* peaks) {
-  WalkPeak p = peaks[0];
-#pragma unroll
-  for (int w = 1; w < kAThreads / 64; ++w) {
-    p.code = larger(p.code, peaks[w].code);
-    p.delta = larger(p.delta, peaks[w].delta);
-    p.v2 = larger(p.v2, peaks[w].v2);
-  }
-  // |v| < 2^(exponent(|v|^2) / 2 + 1)
-  const float bound = __fadd_rn(pow2(norm_exponent((int)p.code) + (exponent(__uint_as_float(p.v2)) >> 1) + 1),
-                                __uint_as_float(p.delta));
-  return __builtin_amdgcn_readfirstlane(clamp_up(14 - exponent(bound), kUpKeys));
+__device__ __forceinline__ int up_of_walk(const unsigned* peaks) {
+  const unsigned p = larger(larger(peaks[0], peaks[1]), larger(peaks[2], peaks[3]));
+  return __builtin_amdgcn_readfirstlane(clamp_up(9 - exponent(__uint_as_float(p)), kUpKeys));
 }
 
 // The rows (or keys) whose result is not finite, recomputed over exactly what they see: 0 times a NaN
@@ -509,7 +496,7 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
                                           const float* __restrict__ delta, f16* __restrict__ dk,
                                           f16* __restrict__ dv, float* __restrict__ parts, f16* Qs,
                                           f16* Ds, float (*lse_s)[kBN], float (*dl_s)[kBN], int* bad,
-                                          WalkPeak* peaks) {
+                                          unsigned* peaks) {
   const int32_t* p = items + (int64_t)idx * kItemInts;
   auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(p[k]); };
   const int k0 = u(0), nk = u(2), g = u(3), qend = u(4), tb = u(11), te = u(12), slot = u(13);
@@ -621,7 +608,7 @@ __device__ __forceinline__ void dkdv_item(const SpanArgs& a, const int32_t* item
       if (i + kAhead1 < 32) fr[i % kAhead1] = rd1(qa, da, i + kAhead1);
       __builtin_amdgcn_sched_barrier(0);
     }
-    peak_out(walk_peak(scan, first), norm2(vf), wave, peaks);
+    peak_out(walk_peak(scan, first), wave, peaks);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the row of zeros and the peaks are written
     tile_barrier();
     issue(2);
@@ -757,7 +744,7 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
                                             const float* __restrict__ delta, f16* __restrict__ dk,
                                             f16* __restrict__ dv, float* __restrict__ parts, f16* Qs,
                                             f16* Ds, float (*lse_s)[kBN], float (*dl_s)[kBN], int* bad,
-                                            WalkPeak* peaks) {
+                                            unsigned* peaks) {
   const int32_t* p = items + (int64_t)idx * kItemInts;
   auto u = [&](int k) { return __builtin_amdgcn_readfirstlane(p[k]); };
   const int k0 = u(0), nk = u(2), g = u(3), qend = u(4), tb = u(11), te = u(12), slot = u(13);
@@ -828,7 +815,7 @@ __device__ __forceinline__ void dkdv_narrow(const SpanArgs& a, const int32_t* it
   const unsigned qrow = lds_addr(Qs) + row_base(lane) + hoff, drow = lds_addr(Ds) + row_base(lane) + hoff;
   const unsigned qcol = lds_addr(Qs) + col_base(lane) + hoff, dcol = lds_addr(Ds) + col_base(lane) + hoff;
   int walk = tb % per_head;   // the step's first tile within its head
-  peak_out(walk_peak(scan, first), norm2(vf), wave, peaks);
+  peak_out(walk_peak(scan, first), wave, peaks);
   __syncthreads();            // the peaks are written
   const int up = up_of_walk(peaks);
   const float upf = (float)up;
@@ -939,7 +926,7 @@ __global__ __launch_bounds__(kAThreads) void span_bwd_kernel(
   __shared__ __attribute__((aligned(1024))) f16 T1[kBwdStages * kTileHalves];
   __shared__ __attribute__((aligned(16))) float lse_s[kBwdStages + 1][kBN], dl_s[kBwdStages][kBN];
   __shared__ int bad[kBM];
-  __shared__ WalkPeak peaks[kAThreads / 64];
+  __shared__ unsigned peaks[kAThreads / 64];
   const int idx = (int)blockIdx.x;
   const int kind = __builtin_amdgcn_readfirstlane(items[(int64_t)idx * kItemInts + 14]);
   if (kind == 2)
@@ -1044,7 +1031,7 @@ extern "C" int dk_attn_span_bwd(const void* qkv, const void* out, const float* l
     return DK_ERR_WORKSPACE;
   const int64_t pairs = n_tokens * nq, wgs = (pairs + 15) / 16 < kDeltaWgs ? (pairs + 15) / 16 : kDeltaWgs;
   if (n_items > INT32_MAX / kAThreads || n_joins > INT32_MAX / (4 * kAThreads)) return DK_ERR_INVALID;
-  hipLaunchKernelGGL(attn_delta_kernel<true>, dim3((unsigned)wgs), dim3(kAThreads), 0, stream,
+  hipLaunchKernelGGL(attn_delta_kernel, dim3((unsigned)wgs), dim3(kAThreads), 0, stream,
                      (const f16*)out, (const f16*)dout, delta, n_tokens, nq);
   DK_CHECK_LAUNCH();
   hipLaunchKernelGGL(span_bwd_kernel, dim3((unsigned)n_items), dim3(kAThreads), 0, stream, a, items,

@@ -797,3 +797,24 @@ def test_growing_scores_forward_and_backward(torch, monkeypatch, cut):
             lv += torch.where(vis, rel * p + 2.0 ** -30, 0.0).t() @ do.abs()
         _near(dk, wk, lk + 2.0 ** -11 * wk.abs() + 2.0 ** -24, "dk")
         _near(dv, wv, lv + 2.0 ** -11 * wv.abs() + 2.0 ** -24, "dv")
+
+
+@pytest.mark.parametrize("spec", [("window", [700, 1, 90], 1, 0), ("window", [1] * 300, 5, 2), ("prefix", [(0, [1] * 200)])])
+@pytest.mark.parametrize("size", [1.0, 0.1])
+def test_rows_that_see_one_key_have_no_gradient(torch, spec, size):
+    """P = 1 and out = v, so dS = dout . v - delta is 0 but for the rounding of two fp32 sums of HD products:
+    sqrt(HD) half steps of partial sums at random in each, together 2^-21 of the products' norm."""
+    nq, nkv = 8, 2
+    log(f"span attention, one key to a row, dout ~ {size}, {spec[0]}")
+    meta = _meta(spec, nq, nkv)
+    n, gin = meta.n_tokens, nq // nkv
+    qkv, dout = _inputs(torch, n, nq, nkv, seed=25)
+    dout = (dout.float() * size).half()
+    out, _, dq, dk, _ = _run(qkv, dout, meta, nq, nkv)
+    x, do = qkv.view(n, nq + 2 * nkv, HD).double(), dout.view(n, nq, HD).double()
+    k, v = (x[:, i:i + nkv].repeat_interleave(gin, 1) for i in (nq, nq + nkv))
+    assert torch.equal(out.view(n, nq, HD).double(), v)
+    ds = 2.0 ** -21 * (do * v).norm(dim=2)
+    for got, by, what in ((dq, k, "dq"), (dk, x[:, :nq], "dk")):
+        err, lim = float(got.double().norm()), float((ds * by.norm(dim=2)).norm()) * HD ** -0.5
+        assert err <= lim, f"{what}: {err:.3g} > {lim:.3g}"
