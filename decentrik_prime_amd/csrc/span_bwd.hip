@@ -12,8 +12,9 @@
 // block of keys, from the rows that see any of them, and moves nothing but where those steps end.
 // out, which delta is taken from, is the returned fp16 one; sums, statistics and results are fp32 up to one
 // rounding of dq, dk and dv.  Against 64 bits (2-norms) dq comes out 3.0 to 3.6e-4 off and dk 3.1 to 3.4e-4,
-// of which dS 2.2e-4, their own rounding 2.1e-4 and delta 1.2e-4, dv 2.9e-4, for any size of dout whose
-// gradients fp16 holds (at dout ~ 1e-4 their own rounding is 2 to 4e-3 of them, and nearly all of it).
+// of which dS 2.2e-4, their own rounding 2.1e-4 and delta 1.2e-4 (more where rows see few keys: 5e-4 in all),
+// dv 2.9e-4, for any size of dout whose gradients fp16 holds (at dout ~ 1e-4 their own rounding is 2 to 4e-3
+// of them, and nearly all of it).
 //
 // Bound: a tile's step (64 queries x 128 keys, or 128 rows x 64 keys) keeps attn.hip's order at one wave
 // per SIMD, the next tile's products (in dK/dV all of S before dP) beside this tile's P and dS; it takes
@@ -23,7 +24,7 @@
 // and dP (half of them beside dK and dV: unchanged) bound a tile on their own; what the rest of a tile
 // waits for is not known.
 // Measured on MI355X, 12 query / 2 KV heads (the three launches, back to back): 8192 tokens, window 1024,
-// 4 sinks 236 us; 2048 tokens, window 256, 41; a prompt of 4096 with 16 answers of 512 1090 (621 TFLOP/s).
+// 4 sinks 235 us; 2048 tokens, window 256, 41; a prompt of 4096 with 16 answers of 512 1098 (617 TFLOP/s).
 // A subtraction a value more in dK/dV's P is 1 % of a tile; begun with delta in its accumulators, dP needs
 // none.  dQ in a launch of its own (two workgroups to a CU) took 267, 53 and 1014 when these took 258, 47
 // and 1088: its blocks fill the ends of the dK/dV walks.

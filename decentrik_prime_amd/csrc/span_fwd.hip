@@ -43,7 +43,7 @@ __device__ __forceinline__ void redo_rows(const SpanArgs& a, int t0, int phase, 
 // stores stand beside the other's products.  Stacking a group's heads on the rows makes a block span
 // 128 / gin tokens: fewer masked keys at a window's edges, and answers of a token fill blocks.
 // Measured on MI355X, 12 query / 2 KV heads (passes back to back): 16384 tokens, window 4096, 4 sinks
-// 425 us (849 TFLOP/s); 8192 tokens, window 1024, 78; a prompt of 8192 with 64 answers of a token 243; one
+// 424 us (851 TFLOP/s); 8192 tokens, window 1024, 78; a prompt of 8192 with 64 answers of a token 248; one
 // workgroup of 8 waves to a CU, the waves of a SIMD on alternate tiles, took 1.17 to 1.2 times as long.
 // 20 tokens, one tile, take 7.4: launch 2.2, the item 0.5, first loads 1.9, the tile's code, run for the
 // first time, 2.5, the rows' stores 0.3; the second tile 2.1, later ones 1.1 and 2.0 in turn.  A last tile without the next one's scores, or a
