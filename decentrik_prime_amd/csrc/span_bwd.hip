@@ -12,7 +12,7 @@
 // block of keys, from the rows that see any of them, and moves nothing but where those steps end.
 // out, which delta is taken from, is the returned fp16 one; sums, statistics and results are fp32 up to one
 // rounding of dq, dk and dv.  Against 64 bits (2-norms) dq comes out 3.0 to 3.6e-4 off and dk 3.1 to 3.4e-4,
-// of which dS 2.2e-4, their own rounding 2.1e-4 and delta 1.2e-4 (more where rows see few keys: 5e-4 in all),
+// of which dS 2.2e-4, their own rounding 2.1e-4 and delta 1.2e-4 (more where rows see few keys: 9e-4 in all at two),
 // dv 2.9e-4, for any size of dout whose gradients fp16 holds (at dout ~ 1e-4 their own rounding is 2 to 4e-3
 // of them, and nearly all of it).
 //
