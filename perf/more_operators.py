@@ -313,7 +313,7 @@ def run(state):
     if case["op"] == "policy":
         return k_loss.policy_loss(state["logp"], state["old"], state["adv"], state["meta"], ref=state["ref"],
                                   kl_coef=case["kl"], clip_low=case["low"], clip_high=case["high"],
-                                  reduction=case["reduction"])
+                                  reduction=case["reduction"], per_token=case["per_token"])
     if case["op"] == "preference":
         return k_loss.preference_loss(state["logp"], state["ref"], state["meta"], beta=case["beta"],
                                       kind=case["kind"], label_smoothing=case["smoothing"],
