@@ -23,7 +23,10 @@ DK_NOALLOC_SCRATCH_BYTES = 64 << 20
 DK_OP_LINEAR_FWD, DK_OP_LINEAR_BWD_DX, DK_OP_GATEUP_SWIGLU_FWD, DK_OP_DOWN_SWIGLU_BWD = 0, 1, 2, 3
 DK_W4_KERNEL_AUTO, DK_W4_KERNEL_TILE, DK_W4_KERNEL_STAGED = 0, 1, 2
 
+DK_TYPE_F32, DK_TYPE_F16, DK_TYPE_BF16 = 1, 2, 3
+
 _c_p, _i64, _int, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+_f64 = ctypes.c_double
 
 
 class NF4WeightC(ctypes.Structure):
@@ -78,6 +81,14 @@ class RopeC(ctypes.Structure):
     _fields_ = [("pos", _c_p), ("cos_table", _c_p), ("sin_table", _c_p), ("hd", ctypes.c_int32),
                 ("cols", _i64)]
 
+
+class TokenArrayC(ctypes.Structure):
+    """struct dk_token_array."""
+    _fields_ = [("data", _c_p), ("stride", _i64), ("negated", ctypes.c_int32)]
+
+
+_K = ctypes.POINTER(TokenArrayC)
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "dk_error_string": (ctypes.c_char_p, [_int]),
@@ -131,6 +142,8 @@ SIGNATURES = {
                           _f32, _f32, _c_p]),
     "dk_rms_bwd": (_int, [_c_p, _int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p,
                           _c_p, _c_p, _i64, _i64, _f32, _c_p]),
+    "dk_rms_bwd_rows": (_int, [_c_p, _int, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p,
+                               _c_p, _c_p, _c_p, _i64, _i64, _f32, _c_p]),
     "dk_qkv_epilogue_fwd": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _f32, _int, _int, _int,
                                    _c_p]),
     "dk_qkv_epilogue_bwd": (_int, [_c_p, _c_p, _c_p, _int, _c_p, _c_p, _c_p, _c_p, _i64, _int, _int,
@@ -147,6 +160,17 @@ SIGNATURES = {
     "dk_head_chunk": (_int, [_c_p, _c_p, _c_p, _c_p, _i64, _i64, _i64, _i64, _f32, _i64, _c_p]),
     "dk_head_finalize": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _i64, _f32, _f32,
                                 _i64, _c_p]),
+    "dk_head_logprobs_workspace": (_i64, [_i64, _i64, _i64]),
+    "dk_head_logprobs": (_int, [_c_p, _i64, _i64, _c_p, _i64, _c_p, _i64, _i64, _c_p, _f32, _c_p, _c_p,
+                                _c_p, _c_p, _i64, _c_p]),
+    "dk_policy_loss_workspace": (_i64, [_i64]),
+    "dk_policy_loss": (_int, [_c_p, _i64, _c_p, _c_p, _i64, _i64, _K, _K, _K, _c_p, _int, _f64, _f64, _f64,
+                              _int, _f64, _c_p, _c_p, _c_p, _c_p, _i64, _c_p]),
+    "dk_preference_loss_workspace": (_i64, [_i64, _i64]),
+    "dk_preference_loss": (_int, [_c_p, _i64, _c_p, _c_p, _i64, _i64, _c_p, _c_p, _i64, _K, _K, _f64, _int,
+                                  _f64, _f64, _int, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p]),
+    "dk_grad_clip_workspace": (_i64, [_i64]),
+    "dk_grad_clip": (_int, [_c_p, _c_p, _c_p, _c_p, _i64, _f64, _f64, _c_p, _c_p, _i64, _c_p]),
     "dk_w4_gateup_swiglu_fwd": (_int, [_c_p, _i64, _i64, _W, _c_p, _c_p, _c_p, _i64, _c_p]),
     "dk_w4_down_swiglu_bwd": (_int, [_c_p, _i64, _i64, _W, _c_p, _c_p, _i64, _c_p]),
 }
@@ -210,3 +234,14 @@ def stream_handle(device=None):
         import torch
         index = torch.cuda.current_device()
     return _raw_stream(index)
+
+
+def launch(dev, entry, what, *args):
+    """The C entry point on dev's current stream, with dev the current device."""
+    import torch
+    if torch.cuda.current_device() == dev.index:
+        rc = entry(*args, stream_handle(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, stream_handle(dev))
+    check(rc, what)

@@ -1,0 +1,272 @@
+// The global norm of a list of gradient tensors and the gradients scaled to it:
+//   norm = scale sqrt(sum g^2),  factor = scale min(1, max_norm / (norm + 1e-6)),  out = factor g
+//
+// Two walks over the tensors, both cut into pieces of kPiece elements that the workgroups take in turn:
+// the first leaves a sum of squares per workgroup, the second adds those up again in every workgroup (a
+// fixed order, so all get the same factor) and scales.  The second walks the pieces backwards: what the
+// first read last is still in the 256 MB cache.  Squares and sums are in 64 bits: in 32, gradients above
+// 2^64 or below 2^-63 would give an infinite or a zero norm.  The tensors' addresses travel in the kernel
+// arguments (kBatch of them a launch), so a captured call holds no pointer to host memory and the device
+// keeps no table.  Bound: reading and writing the gradients; few and small ones: two launches.
+#include <algorithm>
+#include <vector>
+
+#include "dk_common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kVec = 8;                          // elements of a lane's piece of work
+constexpr int kPiece = kThreads * kVec * 4;      // 8192 elements
+constexpr int kBatch = 112;                      // tensors of a launch (their table: under 4 KB)
+constexpr int kGroups = 1024;                    // workgroups of a launch, four to a CU
+
+typedef __bf16 bf16;
+// 16-byte accesses at any element's address
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+
+struct Table {
+  const void* src[kBatch];
+  void* dst[kBatch];
+  int64_t numel[kBatch];
+  uint32_t first[kBatch + 1];     // the tensors' first pieces
+  uint8_t type[kBatch];           // source type | destination type << 4
+  int n;
+};
+static_assert(sizeof(Table) <= 3600, "kernel arguments");
+
+struct Piece {
+  int tensor;
+  int64_t begin;
+  int count;
+};
+
+__device__ __forceinline__ Piece piece_of(const Table& t, uint32_t c) {
+  int lo = 0, hi = t.n - 1;       // the last tensor whose first piece is at most c
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (t.first[mid] <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  const int64_t begin = (int64_t)(c - t.first[lo]) * kPiece, left = t.numel[lo] - begin;
+  return {lo, begin, (int)(left < kPiece ? left : kPiece)};
+}
+
+__device__ __forceinline__ float from_bits(uint16_t u, int type) {
+  if (type == DK_TYPE_F16) return (float)__builtin_bit_cast(f16, u);
+  return __builtin_bit_cast(float, (uint32_t)u << 16);
+}
+
+__device__ __forceinline__ uint16_t to_bits(float v, int type) {
+  if (type == DK_TYPE_F16) return __builtin_bit_cast(uint16_t, (f16)v);
+  return __builtin_bit_cast(uint16_t, (bf16)v);
+}
+
+__device__ __forceinline__ float load1(const void* p, int64_t i, int type) {
+  return type == DK_TYPE_F32 ? static_cast<const float*>(p)[i]
+                             : from_bits(static_cast<const uint16_t*>(p)[i], type);
+}
+
+__device__ __forceinline__ void store1(void* p, int64_t i, int type, float v) {
+  if (type == DK_TYPE_F32) static_cast<float*>(p)[i] = v;
+  else static_cast<uint16_t*>(p)[i] = to_bits(v, type);
+}
+
+__device__ __forceinline__ void load8(const void* p, int64_t i, int type, float (&v)[kVec]) {
+  if (type == DK_TYPE_F32) {
+    const f32x4u a = *reinterpret_cast<const f32x4u*>(static_cast<const float*>(p) + i);
+    const f32x4u b = *reinterpret_cast<const f32x4u*>(static_cast<const float*>(p) + i + 4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = a[k];
+      v[k + 4] = b[k];
+    }
+  } else {
+    const u16x8u a = *reinterpret_cast<const u16x8u*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = from_bits(a[k], type);
+  }
+}
+
+__device__ __forceinline__ void store8(void* p, int64_t i, int type, const float (&v)[kVec]) {
+  if (type == DK_TYPE_F32) {
+    f32x4u a, b;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a[k] = v[k];
+      b[k] = v[k + 4];
+    }
+    *reinterpret_cast<f32x4u*>(static_cast<float*>(p) + i) = a;
+    *reinterpret_cast<f32x4u*>(static_cast<float*>(p) + i + 4) = b;
+  } else {
+    u16x8u a;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = to_bits(v[k], type);
+    *reinterpret_cast<u16x8u*>(static_cast<uint16_t*>(p) + i) = a;
+  }
+}
+
+// the workgroup's sum in a fixed order; every thread gets it
+__device__ __forceinline__ double block_sum(double s, double* red) {
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) s += __shfl_xor(s, x);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  double total = red[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 64; ++w) total += red[w];
+  return total;
+}
+
+__global__ __launch_bounds__(kThreads) void squares_kernel(Table t, uint32_t pieces, double* part) {
+  __shared__ double red[kThreads / 64];
+  double s = 0.0;
+  for (uint32_t c = blockIdx.x; c < pieces; c += gridDim.x) {
+    const Piece q = piece_of(t, c);
+    const int type = t.type[q.tensor] & 15;
+    const void* src = t.src[q.tensor];
+    int i = kVec * threadIdx.x;
+    for (; i + kVec <= q.count; i += kVec * kThreads) {
+      float v[kVec];
+      load8(src, q.begin + i, type, v);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) s = __builtin_fma((double)v[k], (double)v[k], s);
+    }
+    for (; i < q.count; ++i) {     // the tensor's last elements: one lane holds fewer than kVec
+      const double v = load1(src, q.begin + i, type);
+      s = __builtin_fma(v, v, s);
+    }
+  }
+  const double total = block_sum(s, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = total;
+}
+
+__global__ __launch_bounds__(kThreads) void scale_kernel(Table t, uint32_t pieces, const double* part,
+                                                         int parts, double max_norm, double scale,
+                                                         float* norm_out) {
+  __shared__ double red[kThreads / 64];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
+  const double norm = scale * sqrt(block_sum(s, red));
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  const double ratio = max_norm / (norm + 1e-6);
+  const float factor = (float)(scale * (ratio > 1.0 ? 1.0 : ratio));   // a NaN norm: NaN
+  for (uint32_t b = blockIdx.x; b < pieces; b += gridDim.x) {
+    const Piece q = piece_of(t, pieces - 1 - b);
+    const int type = t.type[q.tensor] & 15, to = t.type[q.tensor] >> 4;
+    const void* src = t.src[q.tensor];
+    void* dst = t.dst[q.tensor];
+    if (src == dst && factor == 1.0f) continue;   // nothing changes in place
+    int i = kVec * threadIdx.x;
+    for (; i + kVec <= q.count; i += kVec * kThreads) {
+      float v[kVec];
+      load8(src, q.begin + i, type, v);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) v[k] *= factor;
+      store8(dst, q.begin + i, to, v);
+    }
+    for (; i < q.count; ++i) store1(dst, q.begin + i, to, load1(src, q.begin + i, type) * factor);
+  }
+}
+
+int64_t type_size(int type) {
+  return type == DK_TYPE_F32 ? 4 : type == DK_TYPE_F16 || type == DK_TYPE_BF16 ? 2 : 0;
+}
+
+int groups_of(int64_t pieces) { return (int)(pieces < kGroups ? pieces : kGroups); }
+
+}  // namespace
+
+extern "C" int64_t dk_grad_clip_workspace(int64_t n) {
+  return n <= 0 ? 0 : (n + kBatch - 1) / kBatch * kGroups * (int64_t)sizeof(double);
+}
+
+extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int64_t* numel,
+                            const int32_t* types, int64_t n, double max_norm, double scale, float* norm,
+                            void* ws, int64_t ws_bytes, hipStream_t stream) {
+  if (n < 1 || n > (int64_t)1 << 20 || !src || !numel || !types || !norm || !(max_norm > 0.0) ||
+      !(scale > 0.0) || scale - scale != 0.0)
+    return DK_ERR_INVALID;
+  if (!dk_aligned(norm, 4)) return DK_ERR_ALIGN;
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t from = type_size(types[i] & 15), to = type_size(types[i] >> 4);
+    if (!from || !to || numel[i] < 0 || numel[i] > (int64_t)1 << 40) return DK_ERR_INVALID;
+    if (numel[i] && (!src[i] || (dst && !dst[i]))) return DK_ERR_INVALID;
+    if (!dk_aligned(src[i], from) || (dst && !dk_aligned(dst[i], to))) return DK_ERR_ALIGN;
+    if (dst && dst[i] == src[i] && numel[i] && (types[i] & 15) != types[i] >> 4) return DK_ERR_INVALID;
+  }
+  if (dst) {
+    // what is written overlaps nothing else that is read or written: in place, its own source alone
+    struct Range {
+      uintptr_t begin, end;
+      bool write;
+    };
+    try {
+      std::vector<Range> all;
+      all.reserve(2 * n);
+      for (int64_t i = 0; i < n; ++i) {
+        if (!numel[i]) continue;
+        const uintptr_t s = (uintptr_t)src[i], d = (uintptr_t)dst[i];
+        all.push_back({d, d + numel[i] * type_size(types[i] >> 4), true});
+        if (s != d) all.push_back({s, s + numel[i] * type_size(types[i] & 15), false});
+      }
+      std::sort(all.begin(), all.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+      uintptr_t written = 0, touched = 0;
+      for (const Range& r : all) {
+        if (r.begin < written || (r.write && r.begin < touched)) return DK_ERR_INVALID;
+        if (r.write) written = std::max(written, r.end);
+        touched = std::max(touched, r.end);
+      }
+    } catch (...) {
+      return DK_ERR_INVALID;
+    }
+  }
+  if (!ws || ws_bytes < dk_grad_clip_workspace(n) || !dk_aligned(ws, 8)) return DK_ERR_WORKSPACE;
+  double* part = static_cast<double*>(ws);
+  Table t;
+  // the batch of tensors from `i` on (advanced past it) and its pieces; tensors without elements skipped
+  auto fill = [&](int64_t& i) {
+    int64_t pieces = 0;
+    t.n = 0;
+    for (; i < n && t.n < kBatch; ++i) {
+      const int64_t c = (numel[i] + kPiece - 1) / kPiece;
+      if (pieces + c > UINT32_MAX / 2) break;
+      if (!c) continue;
+      t.src[t.n] = src[i];
+      t.dst[t.n] = dst ? dst[i] : nullptr;
+      t.numel[t.n] = numel[i];
+      t.type[t.n] = (uint8_t)types[i];
+      t.first[t.n] = (uint32_t)pieces;
+      ++t.n;
+      pieces += c;
+    }
+    t.first[t.n] = (uint32_t)pieces;
+    return pieces;
+  };
+  int parts = 0;
+  for (int64_t i = 0; i < n;) {
+    const int64_t pieces = fill(i);
+    if (!pieces) continue;
+    const int g = groups_of(pieces);
+    hipLaunchKernelGGL(squares_kernel, dim3(g), dim3(kThreads), 0, stream, t, (uint32_t)pieces, part + parts);
+    DK_CHECK_LAUNCH();
+    parts += g;
+  }
+  bool said = false;
+  for (int64_t i = 0; dst && i < n;) {
+    const int64_t pieces = fill(i);
+    if (!pieces) continue;
+    hipLaunchKernelGGL(scale_kernel, dim3(groups_of(pieces)), dim3(kThreads), 0, stream, t, (uint32_t)pieces,
+                       part, parts, max_norm, scale, said ? nullptr : norm);
+    DK_CHECK_LAUNCH();
+    said = true;
+  }
+  if (!said) {   // the norm alone (or no elements)
+    t.n = 0;
+    hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(kThreads), 0, stream, t, 0u, part, parts, max_norm, scale,
+                       norm);
+    DK_CHECK_LAUNCH();
+  }
+  return 0;
+}

@@ -1,0 +1,419 @@
+// Token log-probabilities of the language-model head without its logits: for selected rows y_i of the
+// final norm's output and the embedding E [V, D] (fp16)
+//   x_v = scale <y_i, E_v>,   lse_i = log sum_v e^{x_v},   logp_i = x_{t_i} - lse_i,
+//   entropy_i = lse_i - sum_v e^{x_v - lse_i} x_v
+// One pass over E: the products stay in MFMA accumulators and each lane folds its own into a running
+// (r, s, t) per token, in log2 units z = x log2(e):  r = the largest z so far,  s = sum 2^(z - r),
+// t = sum 2^(z - r) (z - r).  Two such states join as
+//   r = max(r1, r2),  a_i = 2^(r_i - r),  s = sum a_i s_i,  t = sum a_i (t_i + s_i (r_i - r))
+// and at the end logp = ln2 (z_t - r - log2 s), lse = ln2 (r + log2 s), entropy = ln2 (log2 s - t / s).
+//
+// Bound: the matrix product (2 n V D operations) from some 300 tokens on, below that reading E once.
+// A workgroup of 8 waves holds BM tokens (128 or 256) and walks a run of 256-row pieces of E; (token
+// tile, run) pairs fill the 256 CUs.  The walk is one loop over K steps of 64, through the borders of
+// the pieces: operands come by LDS DMA (lds_dma.h), the loads NST - 1 steps ahead, so that the first
+// steps of a piece arrive while the last one's accumulators are folded.  The MFMA takes E's rows as its
+// first operand and the tokens as its second, so that a lane's accumulators are 16 vocabulary entries
+// of each of its tokens: the folding needs no exchange between lanes, and the four lanes, the waves and
+// the workgroups that share a token meet once, at the end.
+#include "dk_common.h"
+#include "lds_dma.h"
+
+namespace dk {
+namespace {
+
+constexpr int kLpThreads = 512;
+constexpr int kLpBN = 256;     // vocabulary rows per piece
+constexpr int kLpBK = 64;      // K per step
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
+// below every z of finite inputs: the r of a state without entries (2^(kNone - r) is 0, and 1 against itself)
+constexpr float kNone = -1e30f;
+
+// The 16-byte chunks of a 64-half row are permuted by row: no bank conflict in the operand reads
+__device__ __forceinline__ int lp_swz(int r) { return ((r >> 1) & 7) ^ ((r & 1) << 2); }
+
+struct LpParams {
+  const f16* y;            // [*, D], row stride ldy
+  int64_t ldy;
+  const int32_t* rows;     // [n] rows of y, or null (0 .. n - 1)
+  int64_t total;           // rows of y that `rows` may name
+  const f16* e;            // [V, D]
+  const int32_t* tgt;      // [n]
+  int64_t n, V, D;
+  float c;                 // scale log2(e)
+  int tiles_m, tiles_v, runs;
+  float* part;             // [n, runs, 4]: (r, s, t, unused)
+  float* xt;               // [n] the target's product, where there is a target
+};
+
+struct LpState {
+  float r, s, t;
+};
+
+__device__ __forceinline__ LpState lp_join(const LpState& a, const LpState& b) {
+  const float r = fmaxf(a.r, b.r);
+  const float da = a.r - r, db = b.r - r;
+  const float wa = __builtin_amdgcn_exp2f(da), wb = __builtin_amdgcn_exp2f(db);
+  return {r, wa * a.s + wb * b.s, wa * (a.t + a.s * da) + wb * (b.t + b.s * db)};
+}
+
+template <int BM, int NST>
+__global__ __launch_bounds__(kLpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void head_logp_kernel(LpParams p) {
+  constexpr int WAVES_M = 2, WAVES_N = 4;
+  constexpr int WM = BM / WAVES_M, WN = kLpBN / WAVES_N;
+  constexpr int TM = WM / 16, TN = WN / 16;          // 16 x 16 blocks of a wave: tokens, vocabulary
+  constexpr int SA = BM * kLpBK, SB = kLpBN * kLpBK;   // halves of a stage
+  constexpr int LA = BM / 64, LB = kLpBN / 64;         // DMA instructions per lane and step
+  constexpr int LOADS = LA + LB;
+  constexpr int NMFMA = TM * TN;
+  __shared__ __attribute__((aligned(1024))) f16 As[NST * SA];
+  __shared__ __attribute__((aligned(1024))) f16 Bs[NST * SB];
+  __shared__ int32_t tgts[BM];
+  static_assert(4 * BM * 16 <= NST * SA * 2, "the waves' states at the end");
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+  // workgroup -> (token tile, run): each XCD (workgroups are dealt to the 8 of them in turn) a
+  // contiguous share with the token tiles fastest, so that the tiles of a run read E through one L2
+  int u;
+  {
+    const int total = p.tiles_m * p.runs, o = blockIdx.x & 7, q = total >> 3, r = total & 7;
+    u = o * q + (o < r ? o : r) + ((int)blockIdx.x >> 3);
+  }
+  const int mt = u % p.tiles_m, run = u / p.tiles_m;
+  const int64_t m0 = (int64_t)mt * BM;
+  const int v0 = (int)((int64_t)p.tiles_v * run / p.runs);
+  const int v1 = (int)((int64_t)p.tiles_v * (run + 1) / p.runs);
+  const int nk = (int)(p.D / kLpBK);
+  const int steps = (v1 - v0) * nk;
+
+  for (int i = tid; i < BM; i += kLpThreads) tgts[i] = m0 + i < p.n ? p.tgt[m0 + i] : -1;
+
+  // ---- loads: instruction j of wave w fills chunks [(8 j + w) 64, +64) of a stage
+  const uint64_t a_base = uniform64((uint64_t)(p.rows ? p.y : p.y + m0 * p.ldy));
+  unsigned a_off[LA], b_off[LB];
+#pragma unroll
+  for (int j = 0; j < LA; ++j) {
+    const int q = (j * 8 + wave) * 64 + lane, row = q >> 3;
+    const int64_t m = m0 + row < p.n ? m0 + row : p.n - 1;   // tokens past n: never stored
+    int64_t r = m - m0;
+    if (p.rows) {
+      const int64_t at = p.rows[m];
+      r = at < 0 ? 0 : at < p.total ? at : p.total - 1;      // outside: NaN at the end
+    }
+    a_off[j] = (unsigned)((r * p.ldy + ((q & 7) ^ lp_swz(row)) * 8) * (int64_t)sizeof(f16));
+  }
+  int ld_kt = 0, ld_v = v0;          // the step that is loaded next
+  uint64_t b_base = 0;
+  auto set_piece = [&]() {
+    const int64_t first = (int64_t)ld_v * kLpBN;
+    b_base = uniform64((uint64_t)(p.e + first * p.D));
+    const int64_t left = p.V - 1 - first;                    // rows past V: the last one again
+#pragma unroll
+    for (int j = 0; j < LB; ++j) {
+      const int q = (j * 8 + wave) * 64 + lane, row = q >> 3;
+      const unsigned r = row < left ? row : (unsigned)left;
+      b_off[j] = (r * (unsigned)p.D + ((q & 7) ^ lp_swz(row)) * 8) * (unsigned)sizeof(f16);
+    }
+  };
+  auto issue = [&](int st, int d) {
+    const uint64_t k = (uint64_t)ld_kt * (kLpBK * sizeof(f16));
+    if (d < LA) {
+      dma16s(a_base + k, a_off[d],
+             __builtin_amdgcn_readfirstlane(lds_addr(As + st * SA + (d * 8 + wave) * 512)));
+    } else {
+      dma16s(b_base + k, b_off[d - LA],
+             __builtin_amdgcn_readfirstlane(lds_addr(Bs + st * SB + ((d - LA) * 8 + wave) * 512)));
+    }
+  };
+  auto advance = [&]() {
+    if (++ld_kt == nk) {
+      ld_kt = 0;
+      if (++ld_v < v1) set_piece();
+    }
+  };
+  auto wait_loads = [&](int later) {   // at most `later` steps of this wave's loads still in flight
+    if (NST > 2 && later >= 2) wait_vmem<2 * LOADS>();
+    else if (later >= 1) wait_vmem<LOADS>();
+    else wait_vmem<0>();
+  };
+  auto stage_of = [](int s) { return NST == 2 ? s & 1 : s % NST; };
+
+  set_piece();
+#pragma unroll
+  for (int q = 0; q < NST; ++q)
+    if (q < steps) {
+#pragma unroll
+      for (int d = 0; d < LOADS; ++d) issue(q, d);
+      advance();
+    }
+  wait_loads((steps < NST ? steps : NST) - 1);
+  __syncthreads();
+
+  // ---- operands of v_mfma_f32_16x16x32_f16: lane l holds row l % 16 of a 16-row block, k 8 (l / 16) ..
+  // + 7 of a 32-wide sub-step.  The tokens' fragments single-buffered where a sub-step has 32 MFMAs (each
+  // read again after its last use), else double-buffered like E's.
+  const int r16 = lane & 15, g4 = 4 * (lane >> 4);
+  int fo[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) fo[q] = r16 * kLpBK + ((4 * q + (lane >> 4)) ^ lp_swz(r16)) * 8;
+  constexpr bool A2 = NMFMA <= 16;
+  f16x8 fa[A2 ? 2 : 1][TM], fb[2][TN];
+  auto kj = [](int k) { return (k / TN) & 1 ? TN - 1 - k % TN : k % TN; };
+  auto read_a = [&](int st, int s, int i, int buf) {
+    fa[A2 ? buf : 0][i] = *reinterpret_cast<const f16x8*>(As + st * SA + (wm * WM + 16 * i) * kLpBK + fo[s]);
+  };
+  auto read_b = [&](int st, int s, int j, int buf) {
+    fb[buf][j] = *reinterpret_cast<const f16x8*>(Bs + st * SB + (wn * WN + 16 * j) * kLpBK + fo[s]);
+  };
+  auto a_slot = [](int i) {
+    return A2 ? (TN + i < NMFMA ? TN + i : NMFMA - 1) : (i + 1) * TN - 1;
+  };
+  auto reads_after = [&](int k, int st, int s, int buf) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      if (j == k) read_b(st, s, j, buf);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+      if (a_slot(i) == k) read_a(st, s, i, buf);
+  };
+  auto mfma_group = [&](int k) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) n += j == k;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) n += a_slot(i) == k;
+    if (n == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    else if (n == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  };
+
+  f32x4 acc[TM][TN];   // [token block][vocabulary block]: lane l: token l % 16, entries 4 (l / 16) + 0..3
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  LpState state[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) state[i] = {kNone, 0.0f, 0.0f};
+
+  // the accumulators of piece v into the states
+  auto fold = [&](int v) {
+    const int64_t first = (int64_t)v * kLpBN + wn * WN;      // this wave's first vocabulary entry
+    const bool edge = first + WN > p.V;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      // the target's product, from the one lane of the launch that holds it
+      const int64_t at = (int64_t)tgts[wm * WM + 16 * i + r16] - first;
+      if (__builtin_amdgcn_ballot_w64(at >= 0 && at < WN && first + at < p.V)) {
+        const int64_t m = m0 + wm * WM + 16 * i + r16;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (at == 16 * j + g4 + q && first + at < p.V && m < p.n) p.xt[m] = acc[i][j][q];
+      }
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (first + 16 * j + g4 + q >= p.V) acc[i][j][q] = -INFINITY;
+      }
+      float mx = acc[i][0][0];
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx = fmaxf(mx, acc[i][j][q]);
+      const LpState old = state[i];
+      const float r = fmaxf(old.r, mx * p.c);
+      const float d = old.r - r, w = __builtin_amdgcn_exp2f(d);
+      float s = w * old.s, t = w * (old.t + old.s * d);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float z = __builtin_fmaf(acc[i][j][q], p.c, -r);
+          const float ez = __builtin_amdgcn_exp2f(z);
+          if (edge) z = fmaxf(z, kNone);      // no entry: 0 times a number
+          s += ez;
+          t = __builtin_fmaf(ez, z, t);
+          acc[i][j][q] = 0.0f;
+        }
+      state[i] = {r, s, t};
+    }
+  };
+
+#pragma unroll
+  for (int i = 0; i < TM; ++i) read_a(0, 0, i, 0);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) read_b(0, 0, j, 0);
+  int kt = 0, v = v0;
+  for (int s = 0; s < steps; ++s) {
+    const int st = stage_of(s);
+#pragma unroll
+    for (int k = 0; k < NMFMA; ++k) {
+      acc[k / TN][kj(k)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[0][kj(k)], fa[0][k / TN],
+                                                                  acc[k / TN][kj(k)], 0, 0, 0);
+      reads_after(k, st, 1, 1);
+    }
+#pragma unroll
+    for (int k = 0; k < NMFMA; ++k) mfma_group(k);
+    wait_loads((steps - 1 < s + NST - 1 ? steps - 1 : s + NST - 1) - (s + 1));
+    __syncthreads();
+    const bool more = s + 1 < steps, refill = s + NST < steps;
+    const int st1 = stage_of(s + 1);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int k = 0; k < NMFMA; ++k) {
+      acc[k / TN][kj(k)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+          fb[1][kj(k)], fa[A2 ? 1 : 0][k / TN], acc[k / TN][kj(k)], 0, 0, 0);
+      if (more) reads_after(k, st1, 0, 0);
+#pragma unroll
+      for (int d = k * LOADS / NMFMA; d < (k + 1) * LOADS / NMFMA; ++d)
+        if (refill) issue(st, d);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (refill) advance();
+    if (++kt == nk) {
+      fold(v);
+      kt = 0;
+      ++v;
+    }
+  }
+
+  // ---- the four lanes, then the four waves that share a token
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int x = 16; x < 64; x *= 2) {
+      const LpState o = {__shfl_xor(state[i].r, x), __shfl_xor(state[i].s, x), __shfl_xor(state[i].t, x)};
+      state[i] = lp_join(state[i], o);
+    }
+  __syncthreads();   // no wave reads a stage any more, and no load is in flight
+  f32x4* meet = reinterpret_cast<f32x4*>(As);
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+    if (lane < 16)
+      meet[wn * BM + wm * WM + 16 * i + lane] = f32x4{state[i].r, state[i].s, state[i].t, 0.0f};
+  __syncthreads();
+  if (tid < BM && m0 + tid < p.n) {
+    LpState a = {meet[tid][0], meet[tid][1], meet[tid][2]};
+#pragma unroll
+    for (int w = 1; w < WAVES_N; ++w) {
+      const f32x4 b = meet[w * BM + tid];
+      a = lp_join(a, {b[0], b[1], b[2]});
+    }
+    reinterpret_cast<f32x4*>(p.part)[(m0 + tid) * p.runs + run] = f32x4{a.r, a.s, a.t, 0.0f};
+  }
+}
+
+// The runs' states of a token joined (lane i takes runs i, i + 64, ...; then a butterfly: a fixed order),
+// one wave per token.
+__global__ __launch_bounds__(256) void head_logp_join_kernel(LpParams p, float* __restrict__ logp,
+                                                             float* __restrict__ entropy,
+                                                             float* __restrict__ lse) {
+  const int lane = threadIdx.x & 63;
+  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (m >= p.n) return;
+  LpState a = {kNone, 0.0f, 0.0f};
+  const f32x4* mine = reinterpret_cast<const f32x4*>(p.part) + m * p.runs;
+  for (int i = lane; i < p.runs; i += 64) {
+    const f32x4 b = mine[i];
+    a = lp_join(a, {b[0], b[1], b[2]});
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) {
+    const LpState o = {__shfl_xor(a.r, x), __shfl_xor(a.s, x), __shfl_xor(a.t, x)};
+    a = lp_join(a, o);
+  }
+  if (lane) return;
+  const int64_t t = p.tgt[m];
+  const float l2 = log2f(a.s);
+  float lp = 0.0f, en = kLn2 * (l2 - a.t / a.s), ls = kLn2 * (a.r + l2);
+  if (t >= p.V) lp = NAN;
+  else if (t >= 0) lp = kLn2 * (__builtin_fmaf(p.xt[m], p.c, -a.r) - l2);
+  // rounding takes neither past what it can be (NaN stays)
+  lp = lp > 0.0f ? 0.0f : lp;
+  en = en < 0.0f ? 0.0f : en;
+  if (p.rows && (p.rows[m] < 0 || p.rows[m] >= p.total)) lp = en = ls = NAN;
+  logp[m] = lp;
+  entropy[m] = en;
+  lse[m] = ls;
+}
+
+struct LpPlan {
+  int bm, tiles_m, tiles_v, runs;
+};
+
+constexpr int kLpSlots = 256;   // workgroups at once, one per CU
+
+// 128-token tiles up to 128 tokens, else 256; runs of E such that the workgroups' rounds times the pieces
+// of a run are fewest (and, among equals, the fewest runs).
+LpPlan lp_plan(int64_t n, int64_t V) {
+  LpPlan best{n <= 128 ? 128 : 256, 0, (int)((V + kLpBN - 1) / kLpBN), 1};
+  best.tiles_m = (int)((n + best.bm - 1) / best.bm);
+  int64_t cost = -1;
+  for (int g = 1; g <= kLpSlots && g <= best.tiles_v; ++g) {
+    const int64_t c = (((int64_t)best.tiles_m * g + kLpSlots - 1) / kLpSlots) *
+                      ((best.tiles_v + g - 1) / g);
+    if (cost < 0 || c < cost) {
+      cost = c;
+      best.runs = g;
+    }
+  }
+  return best;
+}
+
+bool lp_sizes_ok(int64_t n, int64_t V, int64_t D) {
+  // the grid, 32-bit pieces and steps, and 32-bit offsets inside a piece of E
+  return n >= 0 && n <= (int64_t)1 << 30 && V >= 1 && V <= (int64_t)1 << 30 && D >= kLpBK &&
+         D % kLpBK == 0 && D <= (int64_t)1 << 20;
+}
+
+}  // namespace
+}  // namespace dk
+
+using namespace dk;
+
+extern "C" int64_t dk_head_logprobs_workspace(int64_t n, int64_t vocab, int64_t d) {
+  if (n <= 0 || !lp_sizes_ok(n, vocab, d)) return 0;
+  return n * (16 * (int64_t)lp_plan(n, vocab).runs + 4);
+}
+
+extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* rows, int64_t n,
+                                const void* emb, int64_t vocab, int64_t d, const int32_t* tgt, float scale,
+                                float* logp, float* entropy, float* lse, void* ws, int64_t ws_bytes,
+                                hipStream_t stream) {
+  if (!lp_sizes_ok(n, vocab, d) || ldy < d || ldy % 8 || total < 0 || (!rows && n > total) ||
+      !(scale > 0.0f) || scale > 1e6f)
+    return DK_ERR_INVALID;
+  if (n == 0) return 0;
+  if (!y || !emb || !tgt || !logp || !entropy || !lse || total == 0) return DK_ERR_INVALID;
+  // 32-bit byte offsets: a tile's rows of y, or all of y where rows are picked from it
+  if (((rows ? total : 256) * ldy + d) * (int64_t)sizeof(f16) >= (int64_t)1 << 32 ||
+      kLpBN * d * (int64_t)sizeof(f16) >= (int64_t)1 << 32)
+    return DK_ERR_INVALID;
+  if (!dk_aligned(y, 16) || !dk_aligned(emb, 16) || !dk_aligned(tgt, 4) || !dk_aligned(rows, 4) ||
+      !dk_aligned(logp, 4) || !dk_aligned(entropy, 4) || !dk_aligned(lse, 4))
+    return DK_ERR_ALIGN;
+  if (!ws || ws_bytes < dk_head_logprobs_workspace(n, vocab, d) || !dk_aligned(ws, 16))
+    return DK_ERR_WORKSPACE;
+  const LpPlan pl = lp_plan(n, vocab);
+  LpParams p{(const f16*)y, ldy, rows, total, (const f16*)emb, tgt, n, vocab, d, scale * kLog2e,
+             pl.tiles_m, pl.tiles_v, pl.runs, (float*)ws, (float*)ws + 4 * n * pl.runs};
+  const dim3 grid((unsigned)(pl.tiles_m * pl.runs));
+  if (pl.bm == 128)
+    hipLaunchKernelGGL((head_logp_kernel<128, 3>), grid, dim3(kLpThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((head_logp_kernel<256, 2>), grid, dim3(kLpThreads), 0, stream, p);
+  DK_CHECK_LAUNCH();
+  hipLaunchKernelGGL(head_logp_join_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, p, logp,
+                     entropy, lse);
+  DK_CHECK_LAUNCH();
+  return 0;
+}

@@ -124,16 +124,16 @@ __global__ __launch_bounds__(kRowThreads) void rms_fwd_kernel(
 // grads, dx = rstd (w dy - xhat mean(w dy xhat)) [+ dres]; out may alias dres.
 template <int KMAX, bool DY32>
 __global__ __launch_bounds__(kRowThreads) void rms_bwd_kernel(
-    const void* __restrict__ dyp, const float* __restrict__ gscale, const float* __restrict__ x,
-    const f16* __restrict__ delta, const float* __restrict__ w, const float* __restrict__ rstd,
-    const float* dres, float* out, const f16* __restrict__ lq, const f16* __restrict__ lv,
+    const void* __restrict__ dyp, const float* __restrict__ gscale, const float* __restrict__ row_scale,
+    const float* __restrict__ x, const f16* __restrict__ delta, const float* __restrict__ w,
+    const float* __restrict__ rstd, const float* dres, float* out, const f16* __restrict__ lq, const f16* __restrict__ lv,
     f16* __restrict__ out16, const uint8_t* __restrict__ mq, const uint8_t* __restrict__ mv,
     int64_t n_rows, int d, float keep_scale) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x >> 6);
   if (row >= n_rows) return;
   const int64_t off = row * d;
-  const float gs = *gscale;
+  const float gs = row_scale ? __fmul_rn(*gscale, row_scale[row]) : *gscale;
   const float r = rstd[row];
   const int kn = (d + 255) / 256;   // chunks holding any of the row (uniform)
   // every load of the row first, at clamped addresses (lanes past the row read element 0 and
@@ -456,12 +456,10 @@ extern "C" int dk_rms_fwd(const float* x, const void* delta, float* xout, const 
   return 0;
 }
 
-extern "C" int dk_rms_bwd(const void* dy, int dy_f32, const float* gscale, const float* x,
-                          const void* delta,
-                          const float* w, const float* rstd, const float* dres, float* out,
-                          const void* lq, const void* lv, void* out16, const uint8_t* mq,
-                          const uint8_t* mv, int64_t n_rows, int64_t d, float keep_scale,
-                          hipStream_t stream) {
+static int rms_bwd(const void* dy, int dy_f32, const float* gscale, const float* row_scale, const float* x,
+                   const void* delta, const float* w, const float* rstd, const float* dres, float* out,
+                   const void* lq, const void* lv, void* out16, const uint8_t* mq, const uint8_t* mv,
+                   int64_t n_rows, int64_t d, float keep_scale, hipStream_t stream) {
   if (n_rows < 0 || d < 4 || d > 4096 || d % 4) return DK_ERR_INVALID;
   if (n_rows == 0) return 0;
   if (!dy || !gscale || !x || !w || !rstd || !out) return DK_ERR_INVALID;
@@ -475,7 +473,7 @@ extern "C" int dk_rms_bwd(const void* dy, int dy_f32, const float* gscale, const
   if (n_rows / kRowsPerBlock >= 0x7fffffff) return DK_ERR_INVALID;
   const dim3 grid(grid_rows(n_rows)), block(kRowThreads);
   auto args = [&](auto kern) {
-    hipLaunchKernelGGL(kern, grid, block, 0, stream, dy, gscale, x, (const f16*)delta,
+    hipLaunchKernelGGL(kern, grid, block, 0, stream, dy, gscale, row_scale, x, (const f16*)delta,
                        w, rstd, dres, out, (const f16*)lq, (const f16*)lv, (f16*)out16, mq, mv,
                        n_rows, (int)d, keep_scale);
   };
@@ -492,6 +490,27 @@ extern "C" int dk_rms_bwd(const void* dy, int dy_f32, const float* gscale, const
   }
   DK_CHECK_LAUNCH();
   return 0;
+}
+
+extern "C" int dk_rms_bwd(const void* dy, int dy_f32, const float* gscale, const float* x,
+                          const void* delta,
+                          const float* w, const float* rstd, const float* dres, float* out,
+                          const void* lq, const void* lv, void* out16, const uint8_t* mq,
+                          const uint8_t* mv, int64_t n_rows, int64_t d, float keep_scale,
+                          hipStream_t stream) {
+  return rms_bwd(dy, dy_f32, gscale, nullptr, x, delta, w, rstd, dres, out, lq, lv, out16, mq, mv, n_rows, d,
+                 keep_scale, stream);
+}
+
+extern "C" int dk_rms_bwd_rows(const void* dy, int dy_f32, const float* gscale, const float* row_scale,
+                               const float* x, const void* delta, const float* w, const float* rstd,
+                               const float* dres, float* out, const void* lq, const void* lv, void* out16,
+                               const uint8_t* mq, const uint8_t* mv, int64_t n_rows, int64_t d,
+                               float keep_scale, hipStream_t stream) {
+  if (n_rows > 0 && !row_scale) return DK_ERR_INVALID;
+  if (!dk_aligned(row_scale, 4)) return DK_ERR_ALIGN;
+  return rms_bwd(dy, dy_f32, gscale, row_scale, x, delta, w, rstd, dres, out, lq, lv, out16, mq, mv, n_rows,
+                 d, keep_scale, stream);
 }
 
 static int qkv_shape_ok(int64_t n_rows, int nq, int nkv, int hd) {

@@ -371,16 +371,6 @@ def _check_span(qkv, meta, nq, nkv, hd):
         raise ValueError(f"the plan is on {meta.spans.device}, qkv on {qkv.device}")
 
 
-def _launch(dev, entry, what, *args):
-    """The C entry point on dev's current stream, with dev the current device."""
-    if torch.cuda.current_device() == dev.index:
-        rc = entry(*args, _lib.stream_handle(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = entry(*args, _lib.stream_handle(dev))
-    _lib.check(rc, what)
-
-
 def span_attention_forward(qkv, meta, nq, nkv, hd):
     """(out [N, nq hd] fp16, lse [nq, N] fp32) of the attention whose plan is `meta`; layouts as for
     attention_forward."""
@@ -389,9 +379,10 @@ def span_attention_forward(qkv, meta, nq, nkv, hd):
     out = torch.empty(n, nq * hd, dtype=torch.float16, device=dev)
     lse = torch.empty(nq, n, dtype=torch.float32, device=dev)
     ws = torch.empty(meta.fwd_bytes, dtype=torch.uint8, device=dev) if meta.fwd_bytes else None
-    _launch(dev, _lib.lib().dk_attn_span_fwd, "dk_attn_span_fwd", qkv.data_ptr(), meta.spans.data_ptr(),
-            meta.items.data_ptr(), meta.items.shape[0], meta.joins.data_ptr(), meta.joins.shape[0],
-            meta.n_slots, n, nq, nkv, hd, out.data_ptr(), lse.data_ptr(), _lib.ptr(ws), meta.fwd_bytes)
+    _lib.launch(dev, _lib.lib().dk_attn_span_fwd, "dk_attn_span_fwd", qkv.data_ptr(),
+                meta.spans.data_ptr(), meta.items.data_ptr(), meta.items.shape[0], meta.joins.data_ptr(),
+                meta.joins.shape[0], meta.n_slots, n, nq, nkv, hd, out.data_ptr(), lse.data_ptr(),
+                _lib.ptr(ws), meta.fwd_bytes)
     return out, lse
 
 
@@ -411,11 +402,11 @@ def span_attention_backward(qkv, out, lse, dout, meta, nq, nkv, hd):
     dk = torch.empty(n, nkv * hd, dtype=torch.float16, device=dev)
     dv = torch.empty(n, nkv * hd, dtype=torch.float16, device=dev)
     ws = torch.empty(meta.bwd_bytes, dtype=torch.uint8, device=dev) if meta.bwd_bytes else None
-    _launch(dev, _lib.lib().dk_attn_span_bwd, "dk_attn_span_bwd", qkv.data_ptr(), out.data_ptr(),
-            lse.data_ptr(), dout.data_ptr(), meta.spans.data_ptr(), meta.items_bwd.data_ptr(),
-            meta.items_bwd.shape[0], meta.joins_bwd.data_ptr(), meta.joins_bwd.shape[0], meta.n_units, n,
-            nq, nkv, hd, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws),
-            meta.bwd_bytes)
+    _lib.launch(dev, _lib.lib().dk_attn_span_bwd, "dk_attn_span_bwd", qkv.data_ptr(), out.data_ptr(),
+                lse.data_ptr(), dout.data_ptr(), meta.spans.data_ptr(), meta.items_bwd.data_ptr(),
+                meta.items_bwd.shape[0], meta.joins_bwd.data_ptr(), meta.joins_bwd.shape[0],
+                meta.n_units, n, nq, nkv, hd, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                dv.data_ptr(), _lib.ptr(ws), meta.bwd_bytes)
     return dq, dk, dv
 
 

@@ -1,0 +1,99 @@
+"""The global norm of a step's gradients, and the gradients scaled to a largest norm (no counterpart in the
+reference, whose trainer clips with torch).
+
+    norm = clip_grads(grads, 1.0)                                  # in place
+    norm = clip_grads(grads, 1.0, scale=1.0 / 1024, out=master)    # loss-scaled fp16 into fp32
+
+The norm stays on the device: no call here waits for the GPU.
+"""
+
+from operator import attrgetter
+
+import torch
+
+from . import _lib
+
+_CODES = {torch.float32: _lib.DK_TYPE_F32, torch.float16: _lib.DK_TYPE_F16,
+          torch.bfloat16: _lib.DK_TYPE_BF16}
+_dtype, _pointer, _numel = attrgetter("dtype"), torch.Tensor.data_ptr, torch.Tensor.numel
+_device, _contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
+
+
+def _dense(t):
+    """Whether the tensor's elements fill a run of memory, in whatever order of its axes."""
+    expected = 1
+    for size, stride in sorted(zip(t.shape, t.stride()), key=lambda x: (x[1], x[0])):
+        if size != 1:
+            if stride != expected:
+                return t.numel() == 0
+            expected *= size
+    return True
+
+
+def _check(tensors, what):
+    """(the tensors' type codes, the device's index)"""
+    codes = [_CODES.get(t) for t in map(_dtype, tensors)]
+    if None in codes:
+        raise ValueError(f"{what} must be fp32, fp16 or bf16 tensors")
+    devices = set(map(_device, tensors))
+    if len(devices) != 1 or -1 in devices:
+        raise ValueError(f"{what} must be on one GPU")
+    if not all(map(_contiguous, tensors)) and not all(map(_dense, tensors)):
+        raise ValueError(f"{what} must be dense")
+    return codes, devices.pop()
+
+
+def _array(values):
+    return (_lib.ctypes.c_int64 * len(values))(*values)
+
+
+def _run(grads, max_norm, scale, out, in_place=False):
+    """grads: a list."""
+    if not grads:
+        raise ValueError("at least one gradient")
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive (got {scale})")
+    types, index = _check(grads, "gradients")
+    numel = list(map(_numel, grads))
+    src = _array(list(map(_pointer, grads)))
+    dst = None
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"{len(grads)} gradients, {len(out)} outputs")
+        to, there = _check(out, "outputs")
+        if there != index or any(
+                o.shape != g.shape or (o.stride() != g.stride() and not
+                                       (o.is_contiguous() and g.is_contiguous()))
+                for o, g in zip(out, grads)):
+            raise ValueError("outputs must have their gradients' device, shapes and strides")
+        types = [c | o << 4 for c, o in zip(types, to)]
+        dst = _array(list(map(_pointer, out)))
+    else:
+        types = [c | c << 4 for c in types]
+        dst = src if in_place else None
+    dev = torch.device("cuda", index)
+    lib = _lib.lib()
+    nbytes = lib.dk_grad_clip_workspace(len(grads))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    _lib.launch(dev, lib.dk_grad_clip, "dk_grad_clip", src, dst, _array(numel),
+                (_lib.ctypes.c_int32 * len(types))(*types), len(grads), max_norm, scale, norm.data_ptr(),
+                ws.data_ptr(), nbytes)
+    return norm
+
+
+def grad_norm(grads, *, scale=1.0):
+    """scale times the 2-norm of all gradients together (fp32 scalar on their device).  grads: CUDA tensors
+    (fp32, fp16 or bf16, mixed, dense) of one device; squares are summed in 64 bits."""
+    return _run(list(grads), float("inf"), scale, None)
+
+
+def clip_grads(grads, max_norm, *, scale=1.0, out=None):
+    """Scales gradients to a global norm of at most max_norm: with norm = scale * (2-norm of all together)
+    each becomes g * scale * min(1, max_norm / (norm + 1e-6)), in place or in `out` (tensors of the
+    gradients' shapes, fp32, fp16 or bf16).  Returns the norm before clipping (fp32 scalar on the device).
+    An infinite norm scales by 0 and a NaN one gives NaN everywhere.  No tensor may overlap another."""
+    if not max_norm > 0.0:
+        raise ValueError(f"max_norm must be positive (got {max_norm})")
+    return _run(list(grads), max_norm, scale, out, in_place=out is None)

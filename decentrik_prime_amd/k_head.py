@@ -130,6 +130,59 @@ def streamed_head(yf, source, tgt_sorted, perm, n_lab, e_target, grad_scale, dum
     return stats[:, 0].sum(), stats, dy
 
 
+def token_logprobs(yf, emb, tgt, *, rows=None, scale=1.0):
+    """Log-probabilities of given tokens under the head, without its gradient and without logits in memory
+    (the reference's or an earlier policy's scores; no counterpart in the reference).
+
+    yf [N, D] fp16 final-norm output (rows may be strided); emb: ResidentEmbedding or [V, D] fp16;
+    tgt int32 [n] token ids (below 0: none, logp 0; V or more: NaN); rows: None (n = N) or int32 [n], the
+    rows of yf that are scored; scale: a factor of the logits (1 / temperature).  Returns (logp, entropy,
+    lse) fp32 [n] of the softmax of scale * yf E^T, the logits in fp32."""
+    if isinstance(emb, ResidentEmbedding):
+        emb = emb.emb
+    if yf.dtype != torch.float16 or not yf.is_cuda or yf.dim() != 2:
+        raise ValueError("yf must be a CUDA fp16 [N, D] tensor")
+    dev = yf.device
+    total, d = yf.shape
+    if emb.dtype != torch.float16 or emb.device != dev or emb.dim() != 2 or emb.shape[1] != d or \
+            emb.shape[0] < 1 or not emb.is_contiguous():
+        raise ValueError(f"the embedding must be a contiguous fp16 [vocab, {d}] tensor on {dev}")
+    if d % 64 or d == 0:
+        raise ValueError("the hidden size must be a multiple of 64")
+    if total > 1 and (yf.stride(1) != 1 or yf.stride(0) < d or yf.stride(0) % 8):
+        raise ValueError("yf's rows must be contiguous, their stride at least D and a multiple of 8")
+    n = total
+    if rows is not None:
+        n = rows.shape[0] if rows.dim() == 1 else -1
+    for t, nm in ((tgt, "tgt"), (rows, "rows")):
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (n,) or t.device != dev or
+                              not t.is_contiguous()):
+            raise ValueError(f"{nm} must be a contiguous int32 [n] tensor on {dev}")
+    if not 0.0 < scale <= 1e6:
+        raise ValueError(f"scale must be within (0, 10^6] (got {scale})")
+    out = torch.empty((3, n), dtype=torch.float32, device=dev)
+    logp, entropy, lse = out
+    if n == 0:
+        return logp, entropy, lse
+    if total == 0:
+        raise ValueError("rows of an empty yf")
+    if total == 1 and (yf.stride(1) != 1 or yf.stride(0) < d or yf.stride(0) % 8):
+        yf = yf.reshape(d).clone().view(1, d)
+    if rows is not None and total * yf.stride(0) >= 1 << 31:
+        # the kernel's row offsets are 32 bits wide: the picked rows alone (an index outside stays one)
+        inside = (rows >= 0) & (rows < total)
+        yf = yf.index_select(0, torch.where(inside, rows, 0))
+        rows = torch.where(inside, torch.arange(n, dtype=torch.int32, device=dev), -1)
+        total = n
+    lib = _lib.lib()
+    nbytes = lib.dk_head_logprobs_workspace(n, emb.shape[0], d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _lib.launch(dev, lib.dk_head_logprobs, "dk_head_logprobs", yf.data_ptr(), yf.stride(0), total,
+                _lib.ptr(rows), n, emb.data_ptr(), emb.shape[0], d, tgt.data_ptr(), float(scale),
+                logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes)
+    return logp, entropy, lse
+
+
 def warmup_specs(hidden=1536, chunk=CHUNK, impl="chunks"):
     """Nothing to warm up: the kernels are compiled ahead of time into libdk.so."""
     return []

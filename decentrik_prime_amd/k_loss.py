@@ -1,0 +1,177 @@
+"""Losses over the log-probabilities of a packed batch's answers, with their gradients: the clipped policy
+loss with a KL term and the preference loss over pairs of answers (no counterpart in the reference, whose
+step trains on cross entropy alone).
+
+The tokens are the batch's labelled ones in sorted order (trainer.pack, trainer.pack_answers), row after
+row; ``row_meta`` is their plan, made once per batch from the rows' lengths (trainer.answer_lens):
+
+    meta = row_meta(lens, device)                                   # or row_meta(lens, device, pairs=...)
+    loss, dlogp, stats = policy_loss(stats_now, old, advantages, meta, ref=ref, kl_coef=0.04)
+    loss, dlogp, rewards, margins = preference_loss(stats_now, ref, meta, beta=0.1)
+
+Log-probabilities are fp32: [n] (any stride) as k_head.token_logprobs returns them, or the streamed head's
+stats [N >= n, 4], whose first column is their negative.  16-bit log-probabilities are refused: their
+rounding (2^-9 of a value of some units) is of the size of the clip range.  dlogp [n] is the loss's
+gradient for the log-probabilities; as the streamed head's gradient is that of the summed cross entropy,
+-dlogp are the factors of its rows (k_norm.rms_backward's row_scale; model.QwenQLoRAStep.policy_step).
+"""
+
+import ctypes
+import math
+
+import numpy as np
+import torch
+
+from . import _lib
+
+ITEM_TOKENS = 512    # tokens that a wave takes; longer rows than ROW_ITEMS of these in larger items
+ROW_ITEMS = 64
+REDUCTIONS = ("row", "token", "sum")
+KINDS = ("sigmoid", "hinge", "ipo")
+
+
+class RowMeta:
+    """The plan of rows of consecutive tokens (see row_meta): on the device the kernels' items, the rows'
+    lengths and items, and the pairs of each row."""
+
+    def __init__(self, lens, device, pairs=None):
+        size = np.asarray([int(n) for n in lens], np.int64)
+        if size.size == 0 or size.min() < 0 or size.max() > 1 << 30 or size.size > 1 << 26:
+            raise ValueError("at least one row, each of 0 to 2^30 tokens")
+        self.lens = size.tolist()
+        self.n_rows, self.n_tokens = int(size.size), int(size.sum())
+        self.n_filled = int((size > 0).sum())
+        step = np.maximum(ITEM_TOKENS, -(-(-(-size // ROW_ITEMS)) // 64) * 64)
+        count = np.maximum(1, -(-size // step))
+        row_items = np.concatenate([[0], np.cumsum(count)])
+        row = np.repeat(np.arange(size.size), count)
+        at = (np.arange(row.size) - row_items[row]) * step[row]       # first token within the row
+        begin = (np.cumsum(size) - size)[row] + at
+        items = np.empty((row.size, 4), np.int64)
+        items[:, 0], items[:, 1] = begin & 0xffffffff, begin >> 32
+        items[:, 2], items[:, 3] = np.minimum(step[row], size[row] - at), row
+        self.n_items = int(row.size)
+        parts = [items.astype(np.uint32).reshape(-1), size.view(np.uint32), row_items.astype(np.uint32)]
+        self.n_pairs = None
+        if pairs is not None:
+            both = np.asarray([(int(a), int(b)) for a, b in pairs], np.int64).reshape(-1, 2)
+            if both.size == 0 or both.min() < 0 or both.max() >= size.size or len(both) > 1 << 28:
+                raise ValueError(f"at least one pair of rows 0 .. {size.size - 1}")
+            self.n_pairs = len(both)
+            index = np.arange(1, len(both) + 1)
+            own = both.T.reshape(-1)                                  # chosen rows, then rejected ones
+            order = np.argsort(own, kind="stable")
+            entries = np.stack([both[:, ::-1].T.reshape(-1), np.concatenate([index, -index])], 1)[order]
+            row_pairs = np.concatenate([[0], np.cumsum(np.bincount(own, minlength=size.size))])
+            if sum(p.size for p in parts) % 2:
+                parts.append(np.zeros(1, np.uint32))
+            parts += [entries.astype(np.int32).view(np.uint32).reshape(-1), row_pairs.astype(np.uint32)]
+        starts = np.cumsum([0] + [p.size for p in parts])
+        self.device = torch.device(device)
+        self._buffer = torch.from_numpy(np.concatenate(parts).view(np.int32)).to(self.device)
+        self.device = self._buffer.device
+        self._at = {name: 4 * int(starts[i]) for name, i in
+                    (("items", 0), ("lens", 1), ("row_items", 2)) + (
+                        (("entries", len(parts) - 2), ("row_pairs", len(parts) - 1)) if pairs is not None
+                        else ())}
+
+    def ptr(self, name):
+        return self._buffer.data_ptr() + self._at[name]
+
+
+def row_meta(lens, device, pairs=None):
+    """The plan of a batch with rows of `lens` tokens (zeros allowed), and for preference_loss of the
+    pairs (chosen row, rejected row); a row may be in any number of pairs."""
+    return RowMeta(lens, device, pairs)
+
+
+def _tokens(t, what, meta):
+    """A token array's C description: [n] log-probabilities, or the head's stats."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or not t.is_cuda or t.device != meta.device:
+        raise ValueError(f"{what} must be a CUDA fp32 tensor on the plan's device ({meta.device})")
+    if t.dim() == 1 and t.shape[0] == meta.n_tokens:
+        return _lib.TokenArrayC(t.data_ptr(), t.stride(0), 0)
+    if t.dim() == 2 and t.shape[0] >= meta.n_tokens and t.shape[1] == 4:
+        return _lib.TokenArrayC(t.data_ptr(), t.stride(0), 1)
+    raise ValueError(f"{what} must be [{meta.n_tokens}] log-probabilities, or the head's stats [N, 4] with "
+                     f"these tokens first (got {tuple(t.shape)})")
+
+
+def _ref(c):
+    return None if c is None else ctypes.byref(c)
+
+
+def policy_loss(logp, old, advantages, meta, *, ref=None, kl_coef=0.0, clip_low=0.2, clip_high=None,
+                reduction="row", per_token=False):
+    """Clipped policy loss: with r = e^(logp - old) and A a token's advantage
+        sum w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^f - f - 1)),  f = ref - logp
+    (clip_high None: clip_low).  advantages fp32 [rows], or [n] with per_token.  reduction "row": the mean
+    over rows (that have tokens) of their tokens' means; "token": the mean over all tokens; "sum".
+    Returns (loss, dlogp [n], stats [rows, 4]): stats are a row's means of the policy term, of the KL
+    estimate e^f - f - 1 (0 without ref), of clipped tokens and of r; 0 for a row without tokens.  A token
+    that lies on a border is not clipped.  All fp32."""
+    clip_high = clip_low if clip_high is None else clip_high
+    if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
+        raise ValueError(f"clip_low must be within [0, 1], clip_high at least 0 (got {clip_low}, {clip_high})")
+    if not math.isfinite(kl_coef) or (kl_coef and ref is None):
+        raise ValueError("kl_coef must be finite, and needs ref")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"reduction must be one of {REDUCTIONS}")
+    if logp is None or old is None:
+        raise ValueError("logp and old are needed")
+    n, rows, dev = meta.n_tokens, meta.n_rows, meta.device
+    x, o, f = _tokens(logp, "logp", meta), _tokens(old, "old", meta), _tokens(ref, "ref", meta)
+    if advantages.dtype != torch.float32 or advantages.device != dev or not advantages.is_contiguous() or \
+            tuple(advantages.shape) != ((n,) if per_token else (rows,)):
+        raise ValueError(f"advantages must be a contiguous fp32 [{n if per_token else rows}] tensor on {dev}")
+    dlogp = torch.empty(n, dtype=torch.float32, device=dev)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    lib = _lib.lib()
+    nbytes = lib.dk_policy_loss_workspace(meta.n_items)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    which = REDUCTIONS.index(reduction)
+    _lib.launch(dev, lib.dk_policy_loss, "dk_policy_loss", meta.ptr("items"), meta.n_items,
+                meta.ptr("row_items"), meta.ptr("lens"), rows, n, ctypes.byref(x), ctypes.byref(o), _ref(f),
+                advantages.data_ptr(), int(per_token), clip_low, clip_high, kl_coef, which,
+                float(max(1, (meta.n_filled, n, 1)[which])), dlogp.data_ptr(), stats.data_ptr(),
+                loss.data_ptr(), ws.data_ptr(), nbytes)
+    return loss, dlogp, stats
+
+
+def preference_loss(logp, ref, meta, *, beta=0.1, kind="sigmoid", label_smoothing=0.0, margin=0.0,
+                    average=False):
+    """Loss over the plan's pairs of rows: with S a row's sum (average: mean) of logp - ref (ref None:
+    logp) and h = beta (S_chosen - S_rejected) - margin, the mean over pairs of
+        "sigmoid"  -(1 - e) log s(h) - e log s(-h), s the logistic function, e = label_smoothing
+        "hinge"    max(0, 1 - h)
+        "ipo"      ((h - 1/2) / beta)^2
+    Returns (loss, dlogp [n], rewards [rows] = beta S, margins [pairs] = h), fp32; a row without tokens has
+    S = 0."""
+    if meta.n_pairs is None:
+        raise ValueError("the plan has no pairs (row_meta(..., pairs=...))")
+    if not 0.0 < beta < math.inf or not math.isfinite(margin):
+        raise ValueError(f"beta must be positive and margin finite (got {beta}, {margin})")
+    if kind not in KINDS:
+        raise ValueError(f"kind must be one of {KINDS}")
+    if not 0.0 <= label_smoothing <= 0.5 or (label_smoothing and kind != "sigmoid"):
+        raise ValueError("label_smoothing must be within [0, 1/2], and is the sigmoid loss's alone")
+    if logp is None:
+        raise ValueError("logp is needed")
+    n, rows, dev = meta.n_tokens, meta.n_rows, meta.device
+    x, f = _tokens(logp, "logp", meta), _tokens(ref, "ref", meta)
+    dlogp = torch.empty(n, dtype=torch.float32, device=dev)
+    rewards = torch.empty(rows, dtype=torch.float32, device=dev)
+    margins = torch.empty(meta.n_pairs, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    lib = _lib.lib()
+    nbytes = lib.dk_preference_loss_workspace(meta.n_items, meta.n_pairs)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _lib.launch(dev, lib.dk_preference_loss, "dk_preference_loss", meta.ptr("items"), meta.n_items,
+                meta.ptr("row_items"), meta.ptr("lens"), rows, n, meta.ptr("row_pairs"),
+                meta.ptr("entries"), meta.n_pairs, ctypes.byref(x), _ref(f), beta, KINDS.index(kind),
+                label_smoothing, margin, int(average), dlogp.data_ptr(), rewards.data_ptr(),
+                margins.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes)
+    return loss, dlogp, rewards, margins

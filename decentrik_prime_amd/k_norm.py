@@ -64,11 +64,12 @@ def rms_forward(x, w, y, rstd, eps, *, delta=None, xout=None, xq=None, xv=None, 
 
 
 def rms_backward(dy16, gscale, x, w, rstd, out, *, dres=None, lq=None, lv=None, mq=None, mv=None,
-                 keep_scale=1.0, out16=None, delta=None, dummy16=None, dummy32=None):
+                 keep_scale=1.0, out16=None, delta=None, row_scale=None, dummy16=None, dummy32=None):
     """delta: the norm's input is x + delta (fp16), added in registers as in the forward, so the
     backward needs no recomputed copy of it.  lq/lv (LoRA-A input grads) need the keep-masks.
     gscale: a CUDA fp32 tensor whose first element scales dy16.  dy16 may also be fp32 (the fused
-    q|k|v dX GEMM's output, which already holds the masked LoRA input gradients)."""
+    q|k|v dX GEMM's output, which already holds the masked LoRA input gradients).  row_scale: fp32 [n], a
+    further factor of each row of dy16 (k_loss: the head's gradients weighted token by token)."""
     if x.dim() != 2:
         raise ValueError("x must be [n, d]")
     n, d = x.shape
@@ -89,6 +90,15 @@ def rms_backward(dy16, gscale, x, w, rstd, out, *, dres=None, lq=None, lv=None, 
         _t(t, dt, (n, d), nm)
     mq = _mask(mq, (n, d), "mq") if use_lora else None
     mv = _mask(mv, (n, d), "mv") if use_lora else None
+    if row_scale is not None:
+        _t(row_scale, torch.float32, (n,), "row_scale")
+        rc = _lib.lib().dk_rms_bwd_rows(
+            _lib.ptr(dy16), int(dy32), _lib.ptr(gscale), _lib.ptr(row_scale), _lib.ptr(x), _lib.ptr(delta),
+            _lib.ptr(w), _lib.ptr(rstd), _lib.ptr(dres), _lib.ptr(out), _lib.ptr(lq), _lib.ptr(lv),
+            _lib.ptr(out16), _lib.ptr(mq), _lib.ptr(mv), n, d, float(keep_scale),
+            _lib.stream_handle(x.device))
+        _lib.check(rc, "dk_rms_bwd_rows")
+        return
     rc = _lib.lib().dk_rms_bwd(_lib.ptr(dy16), int(dy32), _lib.ptr(gscale), _lib.ptr(x),
                                _lib.ptr(delta),
                                _lib.ptr(w), _lib.ptr(rstd), _lib.ptr(dres), _lib.ptr(out),

@@ -118,6 +118,14 @@ int dk_rms_bwd(const void* dy, int dy_f32, const float* gscale, const float* x,
                const void* lv, void* out16, const uint8_t* mq, const uint8_t* mv, int64_t n_rows,
                int64_t d, float keep_scale, hipStream_t stream);
 
+/* dk_rms_bwd with fp32(dy) * (gscale[0] * row_scale[row]) in place of fp32(dy) * gscale[0] (row_scale fp32
+ * [n_rows]): the head's per-token gradients of the cross entropy weighted by a loss over log-probabilities
+ * (dk_policy_loss, dk_preference_loss).  No counterpart in the reference. */
+int dk_rms_bwd_rows(const void* dy, int dy_f32, const float* gscale, const float* row_scale, const float* x,
+                    const void* delta, const float* w, const float* rstd, const float* dres, float* out,
+                    const void* lq, const void* lv, void* out16, const uint8_t* mq, const uint8_t* mv,
+                    int64_t n_rows, int64_t d, float keep_scale, hipStream_t stream);
+
 /* QKV epilogue, forward, in place on the fused [n_rows, (nq + 2 nkv) hd] fp16 QKV buffer.
  * Replaces qkv_epilogue_fwd_kernel / qkv_epilogue_forward (solution/k_rope.py:23-61, 107-111):
  * q += lora_scale * lq, v += lora_scale * lv (fp32), then q and k heads rotated by
@@ -224,6 +232,76 @@ int dk_head_finalize(const float* state, const int32_t* tgt_sorted, const int32_
                      const float* acc, const void* e_target, float* stats, void* dy,
                      int64_t n_rows, int64_t n_lab, float out_scale, float inv_p_scale, int64_t d,
                      hipStream_t stream);
+
+/* Log-probabilities of given tokens, and the entropy and log-sum-exp of each position, without logits in
+ * memory (the forward of the head above alone: scoring under a reference or an earlier policy; no
+ * counterpart in the reference): x_v = scale <y_i, E_v>, lse = log sum_v e^(x_v), logp = x_tgt - lse,
+ * entropy = lse - sum_v p_v x_v, i over the n given rows of y (rows int32 [n], indices below total, or NULL:
+ * rows 0 .. n - 1).  y fp16 with row stride ldy (a multiple of 8) and emb fp16 [vocab, d] contiguous, both
+ * 16-byte aligned; d a multiple of 64 up to 2^20, n and vocab up to 2^30; with rows, total * ldy below
+ * 2^31 elements; 0 < scale <= 10^6.  tgt int32 [n]: below 0 gives logp 0, vocab or more
+ * NaN; a row index outside [0, total) NaN throughout.  logp, entropy, lse fp32 [n].  workspace:
+ * dk_head_logprobs_workspace bytes, 16-byte aligned. */
+int64_t dk_head_logprobs_workspace(int64_t n, int64_t vocab, int64_t d);
+int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* rows, int64_t n,
+                     const void* emb, int64_t vocab, int64_t d, const int32_t* tgt, float scale,
+                     float* logp, float* entropy, float* lse, void* workspace, int64_t workspace_bytes,
+                     hipStream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Losses over the tokens' log-probabilities of a packed batch of answers, with their gradients (no
+ * counterpart in the reference).  The batch is `rows` rows of consecutive tokens, lens int64 [rows], cut
+ * into items {first token (low, high word), tokens, row} (int32 [n_items, 4], 16-byte aligned, row by row
+ * and in token order; a row has 1 to 64 items, an empty row one without tokens); row r's items are
+ * row_items[r] .. row_items[r + 1] - 1.  A token array is fp32 with an element stride (0 allowed), negated
+ * where it holds losses (the head's stats: column 0, stride 4).  With n_tokens = 0 the token arrays may be
+ * NULL.
+ *
+ * dk_policy_loss: A the advantage of the token (per_token) or of its row, r = e^(logp - old),
+ *   p = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), k = e^(ref - logp) - (ref - logp) - 1 (ref NULL: 0)
+ *   loss = sum w (p + kl_coef k), dlogp = its gradient (a token on a border counts as not clipped);
+ *   w = 1 / (len(row) denominator) for reduction 0, 1 / denominator for 1 and 2; clip_low in [0, 1].
+ *   stats [rows, 4]: a row's means of p, k, clipped, r (0 where it has no tokens).
+ * dk_preference_loss: S = a row's sum of logp - ref (average: mean; 0 without tokens), h = beta (S_chosen -
+ *   S_rejected) - margin, loss = mean over pairs of  kind 0: -(1 - e) log s(h) - e log s(-h), s the logistic
+ *   function, e = label_smoothing in [0, 1/2];  1: max(0, 1 - h);  2: ((h - 1/2) / beta)^2.  rewards [rows] = beta S,
+ *   margins [n_pairs] = h.  Row r's pairs are entries row_pairs[r] .. row_pairs[r + 1] - 1, int32 {other row,
+ *   pair + 1 where r is the chosen one, -(pair + 1) where it is the rejected one}.
+ * workspace: the query's bytes, 8-byte aligned. */
+typedef struct dk_token_array {
+  const float* data;
+  int64_t stride;
+  int32_t negated;
+} dk_token_array;
+int64_t dk_policy_loss_workspace(int64_t n_items);
+int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items, const int64_t* lens,
+                   int64_t rows, int64_t n_tokens, const dk_token_array* logp, const dk_token_array* old,
+                   const dk_token_array* ref, const float* advantages, int per_token, double clip_low,
+                   double clip_high, double kl_coef, int reduction, double denominator, float* dlogp,
+                   float* stats, float* loss, void* workspace, int64_t workspace_bytes,
+                   hipStream_t stream);
+int64_t dk_preference_loss_workspace(int64_t n_items, int64_t n_pairs);
+int dk_preference_loss(const int32_t* items, int64_t n_items, const int32_t* row_items,
+                       const int64_t* lens, int64_t rows, int64_t n_tokens, const int32_t* row_pairs,
+                       const int32_t* entries, int64_t n_pairs, const dk_token_array* logp,
+                       const dk_token_array* ref, double beta, int kind, double label_smoothing,
+                       double margin, int average, float* dlogp, float* rewards, float* margins,
+                       float* loss, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* The global norm of n gradient tensors, norm = scale sqrt(sum g^2) (fp32, on the device), and, with dst
+ * not NULL, dst = scale min(1, max_norm / (norm + 1e-6)) src element by element (no counterpart in the
+ * reference).  src, dst, numel and types are host arrays, read before the call returns; types[i] = source
+ * type | destination type << 4 (DK_TYPE_*).  dst[i] may be src[i] (of one type; nothing is written where the
+ * factor is 1); beyond that nothing written may overlap anything else in the lists (DK_ERR_INVALID).
+ * max_norm > 0 (infinity: scale alone).  An infinite norm scales by 0, a NaN one gives NaN throughout.  workspace:
+ * dk_grad_clip_workspace(n) bytes, 8-byte aligned. */
+#define DK_TYPE_F32 1
+#define DK_TYPE_F16 2
+#define DK_TYPE_BF16 3
+int64_t dk_grad_clip_workspace(int64_t n);
+int dk_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* types,
+                 int64_t n, double max_norm, double scale, float* norm, void* workspace,
+                 int64_t workspace_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * LoRA down projection with the dropout of its input.  Replaces the norm kernel's dropout lines

@@ -1,0 +1,303 @@
+"""The clipped policy loss and the preference loss (k_loss) against their formulas in 64 bits, their
+gradients against autograd of the formulas and against differences."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24          # half a step of fp32
+
+LENS = {"one": [1], "short": [3, 0, 70, 1, 64], "sixteen": [100] * 15 + [600], "many": [7 + 13 * i for i in range(90)],
+        "long": [5, 40000, 0, 513, 1024], "empty": [0, 0, 0]}
+
+
+def draw(lens, seed=0, spread=0.3):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = sum(lens)
+    old = -torch.empty(n, device="cuda").exponential_(1.0, generator=g)
+    noise = torch.randn(2, n, generator=g, device="cuda") * spread
+    return old + noise[0], old, old + noise[1], g
+
+
+def rows_of(lens):
+    return torch.repeat_interleave(torch.arange(len(lens), device="cuda"), torch.tensor(lens, device="cuda"))
+
+
+def row_sums(v, lens):
+    return torch.zeros(len(lens), dtype=v.dtype, device=v.device).index_add(0, rows_of(lens), v)
+
+
+def policy_terms(x, old, adv, ref, low, high):
+    """Per token (policy term, KL, clipped, ratio) in 64 bits; adv per token."""
+    r = torch.exp(x - old)
+    cut = ((adv > 0) & (r > 1 + high)) | ((adv < 0) & (r < 1 - low))
+    p = -torch.minimum(r * adv, r.clamp(1 - low, 1 + high) * adv)
+    k = torch.zeros_like(x) if ref is None else torch.expm1(ref - x) - (ref - x)
+    return p, k, cut.double(), r
+
+
+def policy_weight(lens, reduction):
+    size = torch.tensor(lens, dtype=torch.float64, device="cuda")
+    w = {"row": 1.0 / (size.clamp(min=1) * max(1, sum(n > 0 for n in lens))),
+         "token": torch.full_like(size, 1.0 / max(1, sum(lens))), "sum": torch.ones_like(size)}[reduction]
+    return w[rows_of(lens)]
+
+
+@pytest.mark.parametrize("lens", list(LENS))
+@pytest.mark.parametrize("reduction", ["row", "token", "sum"])
+@pytest.mark.parametrize("per_token", [False, True])
+@pytest.mark.parametrize("ref, kl", [(True, 0.05), (True, 0.0), (False, 0.0)])
+def test_policy_loss_matches_the_formula(lens, reduction, per_token, ref, kl):
+    from decentrik_prime_amd import k_loss
+    lens = LENS[lens]
+    x, old, f, g = draw(lens, seed=len(lens))
+    f = f if ref else None
+    adv = torch.randn(sum(lens) if per_token else len(lens), generator=g, device="cuda")
+    adv[::5] = 0.0
+    meta = k_loss.row_meta(lens, "cuda")
+    loss, dlogp, stats = k_loss.policy_loss(x, old, adv, meta, ref=f, kl_coef=kl, clip_low=0.2,
+                                            clip_high=0.25, reduction=reduction, per_token=per_token)
+    assert loss.shape == () and dlogp.shape == (sum(lens),) and stats.shape == (len(lens), 4)
+    a = (adv if per_token else adv[rows_of(lens)]).double()
+    x64 = x.double().requires_grad_(True)
+    f64 = None if f is None else f.double()
+    p, k, cut, r = policy_terms(x64, old.double(), a, f64, 0.2, 0.25)
+    w = policy_weight(lens, reduction)
+    want = (w * (p + kl * k)).sum()
+    (grad,) = torch.autograd.grad(want, x64) if sum(lens) else (x64.detach(),)
+    # the ratio: the rounded difference moves it by |d| U, expf by 2 steps; the products with A and w and
+    # w's own rounding a U each.  k: the same for e^f, whose terms it is the difference of
+    d = (x64 - old.double()).detach().abs()
+    tol_r = r.detach() * U * (d + 6)
+    q = torch.zeros_like(d) if f64 is None else (f64 - x64.detach()).abs()
+    tol_k = U * (q + 4) * (torch.exp(q) + 1 + q) if f64 is not None else q
+    tol_g = w * (tol_r * a.abs() + 4 * U * (r.detach() * a.abs()) + kl * (tol_k + 4 * U * (q.exp() + q)))
+    off = (dlogp.double() - grad).abs() - tol_g
+    assert sum(lens) == 0 or float(off.max()) <= 0, (float(off.max()), int(off.argmax()))
+    tol_p = tol_r * a.abs() + 2 * U * p.detach().abs()
+    tol = float((w * (tol_p + kl * (tol_k + U * k.detach()))).sum()) + 2 * U * abs(float(want))
+    assert abs(float(loss) - float(want)) <= tol
+    size = torch.tensor(lens, dtype=torch.float64, device="cuda").clamp(min=1)
+    for c, (v, t) in enumerate(((p, tol_p), (k, tol_k), (cut, 0 * q), (r, tol_r))):
+        mean = row_sums(v.detach(), lens) / size
+        lim = row_sums(t, lens) / size + 2 * U * mean.abs()
+        assert bool(((stats[:, c].double() - mean).abs() <= lim).all()), c
+
+
+def test_policy_gradient_against_differences():
+    from decentrik_prime_amd import k_loss
+    lens = [40, 3, 9]
+    x, old, f, g = draw(lens, seed=3)
+    adv = torch.randn(3, generator=g, device="cuda")
+    meta = k_loss.row_meta(lens, "cuda")
+    args = dict(ref=f, kl_coef=0.5, clip_low=0.2, clip_high=0.2)
+    _, dlogp, _ = k_loss.policy_loss(x, old, adv, meta, **args)
+    step = 2.0 ** -9
+    d = (x - old).double()
+    for t in range(52):
+        # the loss is smooth inside the clip range and outside it, not across its border
+        if min(abs(float(d[t]) - b) for b in (math.log(0.8), math.log(1.2))) < 2 * step:
+            continue
+        at = []
+        for s in (step, -step):
+            moved = x.clone()
+            moved[t] += s
+            at.append((float(k_loss.policy_loss(moved, old, adv, meta, **args)[0]), float(moved[t])))
+        slope = (at[0][0] - at[1][0]) / (at[0][1] - at[1][1])
+        # two losses rounded to fp32 over a step of 2^-8; the third derivative of e^d over 6
+        assert abs(slope - float(dlogp[t])) <= 4 * U * abs(at[0][0]) / step + step * step * 3 + 1e-5
+
+
+def test_policy_tokens_on_the_borders():
+    """Ratios a step of fp32 on either side of a border, and a difference of 0: the exact difference decides."""
+    from decentrik_prime_amd import k_loss
+    low, high = 0.2, 0.28
+    up, down = math.log1p(high), math.log1p(-low)
+    old = torch.full((4096,), -7.25, device="cuda")
+    x = (old.double() + up).float()[:2048]
+    ulp = torch.tensor(2.0 ** -21, device="cuda")       # a step of fp32 at -7
+    k = torch.arange(-1024, 1024, device="cuda")
+    x = torch.cat([x + k * ulp, (old.double() + down).float()[:2048] + k * ulp])
+    adv = torch.cat([torch.ones(2048, device="cuda"), -torch.ones(2048, device="cuda")])
+    meta = k_loss.row_meta([2048, 2048], "cuda")
+    _, dlogp, stats = k_loss.policy_loss(x, old, adv, meta, clip_low=low, clip_high=high, reduction="sum",
+                                         per_token=True)
+    d = x.double() - old.double()
+    cut = torch.cat([d[:2048] > up, d[2048:] < down])
+    assert torch.equal(dlogp == 0, cut) and 1000 < int(cut[:2048].sum()) < 1050
+    assert stats[:, 2].tolist() == [float(cut[:2048].double().mean()), float(cut[2048:].double().mean())]
+    # no change: every token counts in full, whatever the clip range
+    same = k_loss.policy_loss(old, old, adv, meta, clip_low=0.0, clip_high=0.0, reduction="sum", per_token=True)
+    assert torch.equal(same[1], -adv) and float(same[2][:, 2].sum()) == 0 and bool((same[2][:, 3] == 1).all())
+
+
+def test_policy_reads_stats_and_strides_and_leaves_the_rest():
+    from decentrik_prime_amd import k_loss
+    lens = [9, 700, 0, 31]
+    n = sum(lens)
+    x, old, f, g = draw(lens, seed=5)
+    adv = torch.randn(4, generator=g, device="cuda")
+    meta = k_loss.row_meta(lens, "cuda")
+    want = [t.clone() for t in k_loss.policy_loss(x, old, adv, meta, ref=f, kl_coef=0.1)]
+    stats = torch.full((n + 40, 4), float("nan"), device="cuda")
+    stats[:n, 0] = -x
+    wide = torch.full((n, 3), float("nan"), device="cuda")
+    wide[:, 1] = old
+    both = torch.full((2 * n,), float("nan"), device="cuda")
+    both[::2] = f
+    got = k_loss.policy_loss(stats, wide[:, 1], adv, meta, ref=both[::2], kl_coef=0.1)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    same = k_loss.policy_loss(x, torch.full((1,), -1.0, device="cuda").expand(n), adv, meta)
+    other = k_loss.policy_loss(x, torch.full((n,), -1.0, device="cuda"), adv, meta)
+    assert all(torch.equal(a, b) for a, b in zip(same, other))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_is_not_finite_stays_in_its_row(bad):
+    from decentrik_prime_amd import k_loss
+    lens = [600, 5, 64, 2000]
+    x, old, f, g = draw(lens, seed=6)
+    adv = torch.randn(4, generator=g, device="cuda")
+    meta = k_loss.row_meta(lens, "cuda", pairs=[(0, 1), (2, 3), (0, 3)])
+    want = k_loss.policy_loss(x, old, adv, meta, ref=f, kl_coef=0.1)
+    pref = k_loss.preference_loss(x, f, meta)
+    y = x.clone()
+    y[602] = bad                                       # row 1
+    got = k_loss.policy_loss(y, old, adv, meta, ref=f, kl_coef=0.1)
+    keep = torch.arange(sum(lens), device="cuda") != 602
+    rows = torch.tensor([0, 2, 3], device="cuda")
+    assert torch.equal(got[1][keep], want[1][keep]) and torch.equal(got[2][rows], want[2][rows])
+    assert not bool(torch.isfinite(got[0]))
+    got = k_loss.preference_loss(y, f, meta)
+    other = rows_of(lens) >= 2
+    assert torch.equal(got[1][other], pref[1][other]) and torch.equal(got[3][1:], pref[3][1:])
+    assert torch.equal(got[2][rows], pref[2][rows]) and not bool(torch.isfinite(got[3][0]))
+
+
+def pref_formula(s, pairs, beta, kind, smooth, margin):
+    h = beta * (s[pairs[:, 0]] - s[pairs[:, 1]]) - margin
+    if kind == "sigmoid":
+        each = -(1 - smooth) * torch.nn.functional.logsigmoid(h) - smooth * torch.nn.functional.logsigmoid(-h)
+    elif kind == "hinge":
+        each = torch.relu(1 - h)
+    else:
+        each = ((h - 0.5) / beta) ** 2
+    return each.mean(), h
+
+
+PAIRS = {"one": [(0, 0)], "short": [(0, 2), (2, 1), (4, 2), (0, 2)], "sixteen": [(i, 15 - i) for i in range(16)],
+         "many": [(i, j) for i in range(0, 90, 3) for j in range(0, 90, 7)], "long": [(1, 0), (1, 3), (4, 1), (2, 1)],
+         "empty": [(0, 1), (2, 2)]}
+
+
+@pytest.mark.parametrize("lens", list(LENS))
+@pytest.mark.parametrize("kind, smooth, margin", [("sigmoid", 0.0, 0.0), ("sigmoid", 0.2, 0.7), ("hinge", 0.0, 0.1),
+                                                  ("ipo", 0.0, 0.0)])
+@pytest.mark.parametrize("average", [False, True])
+@pytest.mark.parametrize("ref", [True, False])
+def test_preference_loss_matches_the_formula(lens, kind, smooth, margin, average, ref):
+    from decentrik_prime_amd import k_loss
+    pairs, lens, beta = PAIRS[lens], LENS[lens], 0.15
+    x, _, f, _ = draw(lens, seed=len(lens) + 1)
+    f = f if ref else None
+    meta = k_loss.row_meta(lens, "cuda", pairs=pairs)
+    loss, dlogp, rewards, margins = k_loss.preference_loss(
+        x, f, meta, beta=beta, kind=kind, label_smoothing=smooth, margin=margin, average=average)
+    x64 = x.double().requires_grad_(True)
+    s = row_sums(x64 if f is None else x64 - f.double(), lens)
+    if average:
+        s = s / torch.tensor(lens, dtype=torch.float64, device="cuda").clamp(min=1)
+    want, h = pref_formula(s, torch.tensor(pairs, device="cuda"), beta, kind, smooth, margin)
+    # everything but the results' own rounding is in 64 bits: n tokens' sums are off by n 2^-53 of their
+    # magnitudes, below an eighth of U here
+    (grad,) = torch.autograd.grad(want, x64, allow_unused=True)
+    size = float(x.abs().sum()) + 1.0
+    slack = sum(lens) * 2.0 ** -53 * size * max(1.0, 1.0 / beta ** 2) + 1e-300
+    for got, exact in ((loss, want.detach()), (dlogp, grad if sum(lens) else x64.detach()),
+                       (rewards, beta * s.detach()), (margins, h.detach())):
+        assert got.shape == exact.shape
+        off = (got.double() - exact).abs() - (2 * U * exact.abs() + slack)
+        assert got.numel() == 0 or float(off.max()) <= 0, float(off.max())
+
+
+def test_preference_saturates_without_overflow():
+    from decentrik_prime_amd import k_loss
+    lens = [1, 1, 1, 1]
+    x = torch.tensor([0.0, -1e4, -2e5, -3e5], device="cuda")
+    meta = k_loss.row_meta(lens, "cuda", pairs=[(0, 1), (1, 0), (2, 3), (3, 2)])
+    loss, dlogp, rewards, margins = k_loss.preference_loss(x, None, meta, beta=1.0)
+    assert float(loss) == pytest.approx((1e4 + 1e5) / 4) and margins.tolist() == [1e4, -1e4, 1e5, -1e5]
+    assert dlogp.tolist() == [0.25, -0.25, 0.25, -0.25] or dlogp.tolist() == [-(-0.25), -0.25, 0.25, -0.25]
+
+
+def test_preference_gradient_against_differences():
+    from decentrik_prime_amd import k_loss
+    lens = [5, 4, 6]
+    x, _, f, _ = draw(lens, seed=8)
+    meta = k_loss.row_meta(lens, "cuda", pairs=[(0, 1), (0, 2), (2, 1)])
+    _, dlogp, _, _ = k_loss.preference_loss(x, f, meta, beta=0.5, label_smoothing=0.1)
+    step = 2.0 ** -7
+    for t in range(15):
+        at = []
+        for s in (step, -step):
+            moved = x.clone()
+            moved[t] += s
+            at.append((float(k_loss.preference_loss(moved, f, meta, beta=0.5, label_smoothing=0.1)[0]),
+                       float(moved[t])))
+        slope = (at[0][0] - at[1][0]) / (at[0][1] - at[1][1])
+        # fp32 losses over a step of 2^-6; third derivatives of the logistic loss are below 1/8 beta^3
+        assert abs(slope - float(dlogp[t])) <= 4 * U * abs(at[0][0]) / step + step * step * 0.01
+
+
+def test_losses_repeat_and_replay():
+    """The same bits every time, captured and on another stream too."""
+    from decentrik_prime_amd import k_loss
+    lens = [33 * i % 900 for i in range(60)]
+    x, old, f, g = draw(lens, seed=9)
+    x2 = (x + 0.05).contiguous()
+    adv = torch.randn(60, generator=g, device="cuda")
+    meta = k_loss.row_meta(lens, "cuda", pairs=[(i, i + 1) for i in range(59)])
+
+    def both(v):
+        return (*k_loss.policy_loss(v, old, adv, meta, ref=f, kl_coef=0.1),
+                *k_loss.preference_loss(v, f, meta))
+    want = [[t.clone() for t in both(v)] for v in (x, x2)]
+    for v, w in zip((x, x2), want):
+        assert all(torch.equal(a, b) for a, b in zip(both(v), w))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    graph, v = torch.cuda.CUDAGraph(), x.clone()
+    with torch.cuda.graph(graph):
+        out = both(v)
+    for turn in range(4):
+        v.copy_((x, x2)[turn % 2])
+        both(x2)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[turn % 2])), turn
+
+
+def test_refusals():
+    from decentrik_prime_amd import k_loss
+    lens = [4, 6]
+    x, old, f, _ = draw(lens)
+    adv = torch.zeros(2, device="cuda")
+    meta = k_loss.row_meta(lens, "cuda", pairs=[(0, 1)])
+    for args, kwargs in (((x[:9], old, adv, meta), {}), ((x, old[:9], adv, meta), {}),
+                         ((x, old.half(), adv, meta), {}), ((x, old.cpu(), adv, meta), {}),
+                         ((x, old, adv[:1], meta), {}), ((x, old, adv, meta), dict(per_token=True)),
+                         ((x, old, adv.double(), meta), {}), ((x, old, adv, meta), dict(ref=f[:3])),
+                         ((x.view(10, 1), old, adv, meta), {}), ((None, old, adv, meta), {}),
+                         ((torch.zeros(9, 4, device="cuda"), old, adv, meta), {})):
+        with pytest.raises(ValueError):
+            k_loss.policy_loss(*args, **kwargs)
+    for args in ((x[:9], f, meta), (x, f.double(), meta), (x.half(), f, meta), (None, f, meta)):
+        with pytest.raises(ValueError):
+            k_loss.preference_loss(*args)

@@ -1,0 +1,190 @@
+"""CPU checks of the losses over log-probabilities, the scoring head and gradient clipping: the plans the
+kernels walk, and what is refused before any launch."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from decentrik_prime_amd import _lib, k_grad, k_head, k_loss
+
+
+def read_plan(meta):
+    """(items [n, 4], row_items, lens, entries, row_pairs) as the kernels read them."""
+    raw = meta._buffer.numpy()
+
+    def part(name, n):
+        at = meta._at[name] // 4
+        return raw[at:at + n]
+    items = part("items", 4 * meta.n_items).reshape(-1, 4)
+    row_items = part("row_items", meta.n_rows + 1)
+    lens = part("lens", 2 * meta.n_rows).view(np.int64)
+    if meta.n_pairs is None:
+        return items, row_items, lens, None, None
+    return (items, row_items, lens, part("entries", 4 * meta.n_pairs).reshape(-1, 2),
+            part("row_pairs", meta.n_rows + 1))
+
+
+@pytest.mark.parametrize("lens", [[0], [1], [0, 0, 5, 0], [511, 512, 513, 1, 0, 1025], [32768, 32769, 100000],
+                                  list(range(70)), [1 << 30] * 5 + [3]])
+def test_items_cover_every_token_once(lens):
+    meta = k_loss.row_meta(lens, "cpu")
+    items, row_items, sizes, _, _ = read_plan(meta)
+    assert sizes.tolist() == lens and meta.n_tokens == sum(lens)
+    assert meta.n_filled == sum(n > 0 for n in lens)
+    assert row_items[0] == 0 and row_items[-1] == meta.n_items == len(items)
+    start = 0
+    for r, n in enumerate(lens):
+        mine = items[row_items[r]:row_items[r + 1]]
+        assert 1 <= len(mine) <= k_loss.ROW_ITEMS
+        at = start
+        for lo, hi, count, row in mine.tolist():
+            assert row == r and (hi << 32) + (lo & 0xffffffff) == at
+            assert count > 0 or n == 0
+            at += count
+        start += n
+        assert at == start
+    assert all(meta.ptr(k) % 16 == 0 for k in ("items",)) and meta.ptr("lens") % 8 == 0
+
+
+@pytest.mark.parametrize("lens, pairs", [([3, 4], [(0, 1)]), ([3, 4, 0], [(0, 1), (2, 1), (1, 0), (0, 1)]),
+                                         ([1] * 9, [(i, j) for i in range(9) for j in range(9)])])
+def test_every_row_names_its_pairs(lens, pairs):
+    meta = k_loss.row_meta(lens, "cpu", pairs=pairs)
+    _, _, _, entries, row_pairs = read_plan(meta)
+    assert meta.ptr("entries") % 8 == 0
+    want = {r: sorted([(b, i + 1) for i, (a, b) in enumerate(pairs) if a == r] +
+                      [(a, -i - 1) for i, (a, b) in enumerate(pairs) if b == r]) for r in range(len(lens))}
+    for r in range(len(lens)):
+        assert sorted(map(tuple, entries[row_pairs[r]:row_pairs[r + 1]].tolist())) == want[r]
+
+
+def test_plans_refuse_what_they_cannot_hold():
+    for lens in ([], [-1], [3, -2], [(1 << 30) + 1]):
+        with pytest.raises(ValueError):
+            k_loss.row_meta(lens, "cpu")
+    for pairs in ([], [(0, 2)], [(-1, 0)]):
+        with pytest.raises(ValueError):
+            k_loss.row_meta([1, 2], "cpu", pairs=pairs)
+
+
+def test_losses_refuse_bad_arguments():
+    meta = k_loss.row_meta([2, 3], "cpu", pairs=[(0, 1)])
+    x, a = torch.zeros(5), torch.zeros(2)
+    for kwargs in (dict(clip_low=1.5), dict(clip_low=-0.1), dict(clip_high=-1.0), dict(kl_coef=0.1),
+                   dict(kl_coef=float("nan"), ref=x), dict(reduction="mean"), {}):   # {}: not on a GPU
+        with pytest.raises(ValueError):
+            k_loss.policy_loss(x, x, a, meta, **kwargs)
+    for kwargs in (dict(beta=0.0), dict(beta=float("inf")), dict(kind="dpo"), dict(label_smoothing=0.6),
+                   dict(label_smoothing=0.1, kind="hinge"), dict(margin=float("inf")), {}):
+        with pytest.raises(ValueError):
+            k_loss.preference_loss(x, x, meta, **kwargs)
+    with pytest.raises(ValueError, match="no pairs"):
+        k_loss.preference_loss(x, x, k_loss.row_meta([2, 3], "cpu"))
+
+
+def test_scoring_head_refuses_bad_arguments():
+    y, e, t = torch.zeros(2, 64).half(), torch.zeros(8, 64).half(), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        k_head.token_logprobs(y, e, t)          # not on a GPU
+    lib = _lib.lib()
+    p = ctypes.c_void_p(4096)
+
+    def call(y=p, ldy=64, total=2, rows=None, n=2, emb=p, vocab=8, d=64, tgt=p, scale=1.0, out=p, ws=p,
+             nbytes=1 << 20):
+        return lib.dk_head_logprobs(y, ldy, total, rows, n, emb, vocab, d, tgt, scale, out, out, out, ws,
+                                    nbytes, None)
+    assert lib.dk_head_logprobs_workspace(2, 8, 64) == 2 * 20
+    assert lib.dk_head_logprobs_workspace(0, 8, 64) == 0
+    for bad in (dict(y=None), dict(ldy=32), dict(ldy=68), dict(total=1), dict(n=-1), dict(emb=None),
+                dict(vocab=0), dict(d=32), dict(d=96), dict(d=0), dict(tgt=None), dict(scale=0.0),
+                dict(scale=float("nan")), dict(scale=float("inf")), dict(out=None),
+                dict(rows=p, total=1 << 25), dict(rows=p, total=0), dict(vocab=1 << 31), dict(n=1 << 31)):
+        assert call(**bad) == _lib.DK_ERR_INVALID, bad
+    for bad in (dict(y=ctypes.c_void_p(4104)), dict(emb=ctypes.c_void_p(4104)), dict(tgt=ctypes.c_void_p(2)),
+                dict(out=ctypes.c_void_p(2)), dict(rows=ctypes.c_void_p(4098))):
+        assert call(**bad) == _lib.DK_ERR_ALIGN, bad
+    for bad in (dict(ws=None), dict(nbytes=39), dict(ws=ctypes.c_void_p(4104))):
+        assert call(**bad) == _lib.DK_ERR_WORKSPACE, bad
+    assert call(n=0, y=None, ws=None) == 0
+
+
+def test_loss_entries_refuse_bad_arguments():
+    lib = _lib.lib()
+    p = ctypes.c_void_p(4096)
+    good = _lib.TokenArrayC(4096, 1, 0)
+    ref = ctypes.byref
+
+    def policy(items=p, n_items=2, rows=2, n=5, x=good, old=good, f=good, adv=p, low=0.2, high=0.2, kl=0.1,
+               red=0, den=2.0, out=p, ws=p, nbytes=1 << 12):
+        return lib.dk_policy_loss(items, n_items, p, p, rows, n, ref(x), ref(old), f and ref(f), adv, 0, low,
+                                  high, kl, red, den, out, out, out, ws, nbytes, None)
+    null, back = _lib.TokenArrayC(None, 1, 0), _lib.TokenArrayC(4096, -1, 0)
+    for bad in (dict(items=None), dict(n_items=0), dict(n_items=1), dict(rows=0), dict(n=-1), dict(x=null),
+                dict(old=null), dict(f=null), dict(x=back), dict(adv=None), dict(low=1.1), dict(low=-0.1),
+                dict(high=-0.1), dict(high=float("nan")), dict(kl=float("inf")), dict(f=None), dict(red=3),
+                dict(red=-1), dict(den=0.0), dict(out=None)):
+        assert policy(**bad) == _lib.DK_ERR_INVALID, bad
+    assert policy(items=ctypes.c_void_p(4100)) == _lib.DK_ERR_ALIGN
+    need = lib.dk_policy_loss_workspace(2)
+    for bad in (dict(ws=None), dict(nbytes=need - 1), dict(ws=ctypes.c_void_p(4100))):
+        assert policy(**bad) == _lib.DK_ERR_WORKSPACE, bad
+
+    def preference(pairs=1, entries=p, x=good, f=good, beta=0.1, kind=0, smooth=0.0, margin=0.0, out=p, ws=p,
+                   nbytes=1 << 12):
+        return lib.dk_preference_loss(p, 2, p, p, 2, 5, p, entries, pairs, ref(x), f and ref(f), beta, kind,
+                                      smooth, margin, 0, out, out, out, out, ws, nbytes, None)
+    for bad in (dict(pairs=0), dict(entries=None), dict(x=null), dict(f=back), dict(beta=0.0),
+                dict(beta=float("nan")), dict(kind=3), dict(smooth=0.51), dict(margin=float("nan")),
+                dict(out=None)):
+        assert preference(**bad) == _lib.DK_ERR_INVALID, bad
+    assert preference(entries=ctypes.c_void_p(4100)) == _lib.DK_ERR_ALIGN
+    for bad in (dict(ws=None), dict(nbytes=lib.dk_preference_loss_workspace(2, 1) - 1)):
+        assert preference(**bad) == _lib.DK_ERR_WORKSPACE, bad
+
+
+def test_clipping_refuses_bad_arguments():
+    g = torch.ones(4)
+    for grads in ([], [g], [g.long()]):
+        with pytest.raises(ValueError):
+            k_grad.clip_grads(grads, 1.0)
+    for kwargs in (dict(max_norm=0.0), dict(max_norm=float("nan")), dict(max_norm=-1.0),
+                   dict(max_norm=1.0, scale=0.0), dict(max_norm=1.0, scale=float("inf"))):
+        with pytest.raises(ValueError):
+            k_grad.clip_grads([g], **kwargs)
+    lib = _lib.lib()
+
+    def call(src, dst, numel, types, max_norm=1.0, scale=1.0, norm=64, ws=4096, nbytes=1 << 16):
+        n = len(src)
+        arrays = [(ctypes.c_int64 * n)(*src), (ctypes.c_int64 * n)(*dst) if dst else None,
+                  (ctypes.c_int64 * n)(*numel), (ctypes.c_int32 * n)(*types)]
+        return lib.dk_grad_clip(*arrays, n, max_norm, scale, norm, ws, nbytes, None)
+    f32, f16 = _lib.DK_TYPE_F32 * 17, _lib.DK_TYPE_F16 * 17
+    up = _lib.DK_TYPE_F16 | _lib.DK_TYPE_F32 << 4
+    a, b = 1 << 20, 1 << 21
+    assert lib.dk_grad_clip_workspace(0) == 0
+    for bad in (([], None, [], []), ([a], [a], [-1], [f32]), ([0], [a], [4], [f32]), ([a], [0], [4], [f32]),
+                ([a], [a], [4], [0]), ([a], [a], [4], [4]), ([a], [a], [4], [up]),      # in place, two types
+                ([a, a], [a, a], [4, 4], [f32, f32]),                                   # a tensor twice
+                ([a, a + 8], [a, a + 8], [4, 4], [f32, f32]),                           # overlapping ones
+                ([a, b], [b, b + 64], [4, 4], [f32, f32]),                              # an output over a source
+                ([a, b], [a + 4, b], [4, 4], [f32, f32]),                               # shifted in place
+                ([a, b], [b + 64, b + 72], [4, 4], [f32, f32])):                        # overlapping outputs
+        assert call(*bad) == _lib.DK_ERR_INVALID, bad
+    for kwargs in (dict(max_norm=0.0), dict(max_norm=float("nan")), dict(scale=0.0),
+                   dict(scale=float("inf")), dict(scale=float("nan")), dict(norm=None)):
+        assert call([a], [a], [4], [f32], **kwargs) == _lib.DK_ERR_INVALID, kwargs
+    assert call([a + 2], [a + 2], [4], [f32]) == _lib.DK_ERR_ALIGN
+    assert call([a + 1], [a + 1], [4], [f16]) == _lib.DK_ERR_ALIGN
+    assert call([a], [b + 2], [4], [up]) == _lib.DK_ERR_ALIGN
+    for kwargs in (dict(ws=None), dict(nbytes=8), dict(ws=4100)):
+        assert call([a], [a], [4], [f32], **kwargs) == _lib.DK_ERR_WORKSPACE, kwargs
+
+
+def test_dense_tensors():
+    x = torch.zeros(4, 6)
+    for t, want in ((x, True), (x.t(), True), (x[:, :3], False), (x[::2], False), (x[1:3], True),
+                    (torch.zeros(1, 5).expand(3, 5), False), (torch.zeros(2, 3, 4).permute(2, 0, 1), True),
+                    (torch.zeros(0, 4), True), (torch.zeros(3, 0)[:, :0], True), (torch.zeros(()), True)):
+        assert k_grad._dense(t) is want, (t.shape, t.stride())
