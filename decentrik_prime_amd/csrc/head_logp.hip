@@ -94,7 +94,7 @@ void head_logp_kernel(LpParams p) {
 
   // ---- loads: instruction j of wave w fills chunks [(8 j + w) 64, +64) of a stage
   const uint64_t a_base = uniform64((uint64_t)(p.rows ? p.y : p.y + m0 * p.ldy));
-  unsigned a_off[LA], b_off[LB];
+  unsigned a_off[LA];
 #pragma unroll
   for (int j = 0; j < LA; ++j) {
     const int q = (j * 8 + wave) * 64 + lane, row = q >> 3;
@@ -108,25 +108,25 @@ void head_logp_kernel(LpParams p) {
   }
   int ld_kt = 0, ld_v = v0;          // the step that is loaded next
   uint64_t b_base = 0;
+  int b_last = 0;                    // the piece's last row in E: rows past V are this one again
   auto set_piece = [&]() {
     const int64_t first = (int64_t)ld_v * kLpBN;
     b_base = uniform64((uint64_t)(p.e + first * p.D));
-    const int64_t left = p.V - 1 - first;                    // rows past V: the last one again
-#pragma unroll
-    for (int j = 0; j < LB; ++j) {
-      const int q = (j * 8 + wave) * 64 + lane, row = q >> 3;
-      const unsigned r = row < left ? row : (unsigned)left;
-      b_off[j] = (r * (unsigned)p.D + ((q & 7) ^ lp_swz(row)) * 8) * (unsigned)sizeof(f16);
-    }
+    b_last = (int)(p.V - 1 - first < kLpBN ? p.V - 1 - first : kLpBN);
   };
+  // E's offsets are formed load by load (three instructions beside 16 or more MFMAs): held in registers
+  // they would push the accumulators' kernel into scratch memory
+  const int b_row = wave * 8 + (lane >> 3), b_chunk = ((lane & 7) ^ lp_swz(b_row)) * 16;
+  const unsigned d2 = (unsigned)p.D * (unsigned)sizeof(f16);   // below 2^24, as is a row's number
   auto issue = [&](int st, int d) {
     const uint64_t k = (uint64_t)ld_kt * (kLpBK * sizeof(f16));
     if (d < LA) {
       dma16s(a_base + k, a_off[d],
              __builtin_amdgcn_readfirstlane(lds_addr(As + st * SA + (d * 8 + wave) * 512)));
     } else {
-      dma16s(b_base + k, b_off[d - LA],
-             __builtin_amdgcn_readfirstlane(lds_addr(Bs + st * SB + ((d - LA) * 8 + wave) * 512)));
+      const int j = d - LA, row = b_row + 64 * j < b_last ? b_row + 64 * j : b_last;
+      dma16s(b_base + k, __umul24(row, d2) + b_chunk,
+             __builtin_amdgcn_readfirstlane(lds_addr(Bs + st * SB + (j * 8 + wave) * 512)));
     }
   };
   auto advance = [&]() {
@@ -202,26 +202,34 @@ void head_logp_kernel(LpParams p) {
 
   // the accumulators of piece v into the states
   auto fold = [&](int v) {
-    const int64_t first = (int64_t)v * kLpBN + wn * WN;      // this wave's first vocabulary entry
-    const bool edge = first + WN > p.V;
+    const int first = v * kLpBN + wn * WN + g4;              // this lane's first vocabulary entry
+    const bool edge = (v + 1) * (int64_t)kLpBN > p.V;
+    // a target's product, from the one lane of the launch that holds it
+    bool mine = false;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      // the target's product, from the one lane of the launch that holds it
-      const int64_t at = (int64_t)tgts[wm * WM + 16 * i + r16] - first;
-      if (__builtin_amdgcn_ballot_w64(at >= 0 && at < WN && first + at < p.V)) {
-        const int64_t m = m0 + wm * WM + 16 * i + r16;
+    for (int i = 0; i < TM; ++i)
+      mine |= (unsigned)(tgts[wm * WM + 16 * i + r16] - first) < (unsigned)WN;
+    if (__builtin_amdgcn_ballot_w64(mine)) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int at = tgts[wm * WM + 16 * i + r16] - first;
+        float x = acc[i][0][0];
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (at == 16 * j + g4 + q && first + at < p.V && m < p.n) p.xt[m] = acc[i][j][q];
+          for (int q = 0; q < 4; ++q) x = at == 16 * j + q ? acc[i][j][q] : x;
+        if (at >= 0 && at < WN && (at & 15) < 4 && at + first < p.V)
+          p.xt[m0 + wm * WM + 16 * i + r16] = x;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
       if (edge) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if (first + 16 * j + g4 + q >= p.V) acc[i][j][q] = -INFINITY;
+            if (first + 16 * j + q >= p.V) acc[i][j][q] = -INFINITY;
       }
       float mx = acc[i][0][0];
 #pragma unroll
@@ -244,6 +252,7 @@ void head_logp_kernel(LpParams p) {
           acc[i][j][q] = 0.0f;
         }
       state[i] = {r, s, t};
+      __builtin_amdgcn_sched_barrier(0);      // one token block's temporaries at a time
     }
   };
 
