@@ -16,6 +16,8 @@
 // first operand and the tokens as its second, so that a lane's accumulators are 16 vocabulary entries
 // of each of its tokens: the folding needs no exchange between lanes, and the four lanes, the waves and
 // the workgroups that share a token meet once, at the end.
+#include <utility>
+
 #include "dk_common.h"
 #include "lds_dma.h"
 
@@ -23,7 +25,6 @@ namespace dk {
 namespace {
 
 constexpr int kLpThreads = 512;
-constexpr int kLpBN = 256;     // vocabulary rows per piece
 constexpr int kLpBK = 64;      // K per step
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -32,6 +33,12 @@ constexpr float kNone = -1e30f;
 
 // The 16-byte chunks of a 64-half row are permuted by row: no bank conflict in the operand reads
 __device__ __forceinline__ int lp_swz(int r) { return ((r >> 1) & 7) ^ ((r & 1) << 2); }
+
+// How the launch is cut: `tiles` tiles of `bm` tokens, each over `runs` runs of E, and (tail > 0) the tokens
+// behind them as one tile of 128 over `tail` runs.  A run is a whole number of pieces of bn rows of E.
+struct LpPlan {
+  int bm, bn, tiles, runs, tail, pieces;
+};
 
 struct LpParams {
   const f16* y;            // [*, D], row stride ldy
@@ -42,10 +49,17 @@ struct LpParams {
   const int32_t* tgt;      // [n]
   int64_t n, V, D;
   float c;                 // scale log2(e)
-  int tiles_m, tiles_v, runs;
-  float* part;             // [n, runs, 4]: (r, s, t, unused)
+  LpPlan plan;
+  float* part;             // per token and run: (r, s, t, unused)
   float* xt;               // [n] the target's product, where there is a target
 };
+
+// f(0), ..., f(N - 1) with constant arguments (a loop of this size is past the compiler's limit for unrolling,
+// and an array indexed by a loop that stays one is kept in memory)
+template <class F, int... I>
+__device__ __forceinline__ void each(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
 
 struct LpState {
   float r, s, t;
@@ -58,37 +72,39 @@ __device__ __forceinline__ LpState lp_join(const LpState& a, const LpState& b) {
   return {r, wa * a.s + wb * b.s, wa * (a.t + a.s * da) + wb * (b.t + b.s * db)};
 }
 
-template <int BM, int NST>
-__global__ __launch_bounds__(kLpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void head_logp_kernel(LpParams p) {
-  constexpr int WAVES_M = 2, WAVES_N = 4;
-  constexpr int WM = BM / WAVES_M, WN = kLpBN / WAVES_N;
+__device__ __forceinline__ int lp_runs(const LpPlan& pl, int64_t m) {
+  return m < (int64_t)pl.tiles * pl.bm ? pl.runs : pl.tail;
+}
+
+// token m's first state in LpParams::part
+__device__ __forceinline__ int64_t lp_part(const LpPlan& pl, int64_t m) {
+  const int64_t whole = (int64_t)pl.tiles * pl.bm;
+  return m < whole ? m * pl.runs : whole * pl.runs + (m - whole) * pl.tail;
+}
+
+// The walk of tokens m0 .. m0 + BM - 1 over run `run` of `runs`, in pieces of BN rows of E; WAVES_M x
+// 8 / WAVES_M waves; NST stages of operands in LDS
+template <int BM, int BN, int WAVES_M, int NST>
+__device__ __forceinline__ void lp_walk(const LpParams& p, f16* As, int32_t* tgts, int64_t m0, int run, int runs) {
+  constexpr int WAVES_N = 8 / WAVES_M;
+  constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
   constexpr int TM = WM / 16, TN = WN / 16;          // 16 x 16 blocks of a wave: tokens, vocabulary
-  constexpr int SA = BM * kLpBK, SB = kLpBN * kLpBK;   // halves of a stage
-  constexpr int LA = BM / 64, LB = kLpBN / 64;         // DMA instructions per lane and step
+  constexpr int SA = BM * kLpBK, SB = BN * kLpBK;   // halves of a stage
+  constexpr int LA = BM / 64, LB = BN / 64;         // DMA instructions per lane and step
   constexpr int LOADS = LA + LB;
   constexpr int NMFMA = TM * TN;
-  __shared__ __attribute__((aligned(1024))) f16 As[NST * SA];
-  __shared__ __attribute__((aligned(1024))) f16 Bs[NST * SB];
-  __shared__ int32_t tgts[BM];
-  static_assert(4 * BM * 16 <= NST * SA * 2, "the waves' states at the end");
+  f16* Bs = As + NST * SA;
+  static_assert(WAVES_N * BM * 16 <= NST * SA * 2, "the waves' states at the end");
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-  // workgroup -> (token tile, run): each XCD (workgroups are dealt to the 8 of them in turn) a
-  // contiguous share with the token tiles fastest, so that the tiles of a run read E through one L2
-  int u;
-  {
-    const int total = p.tiles_m * p.runs, o = blockIdx.x & 7, q = total >> 3, r = total & 7;
-    u = o * q + (o < r ? o : r) + ((int)blockIdx.x >> 3);
-  }
-  const int mt = u % p.tiles_m, run = u / p.tiles_m;
-  const int64_t m0 = (int64_t)mt * BM;
-  const int v0 = (int)((int64_t)p.tiles_v * run / p.runs);
-  const int v1 = (int)((int64_t)p.tiles_v * (run + 1) / p.runs);
+  // the run's rows of E: [v0, v1)
+  const int v0 = __builtin_amdgcn_readfirstlane((int)((int64_t)p.plan.pieces * run / runs) * BN);
+  int v1 = __builtin_amdgcn_readfirstlane((int)((int64_t)p.plan.pieces * (run + 1) / runs) * BN);
+  v1 = v1 < p.V ? v1 : (int)p.V;
   const int nk = (int)(p.D / kLpBK);
-  const int steps = (v1 - v0) * nk;
+  const int steps = (v1 - v0 + BN - 1) / BN * nk;
 
   for (int i = tid; i < BM; i += kLpThreads) tgts[i] = m0 + i < p.n ? p.tgt[m0 + i] : -1;
 
@@ -106,13 +122,13 @@ void head_logp_kernel(LpParams p) {
     }
     a_off[j] = (unsigned)((r * p.ldy + ((q & 7) ^ lp_swz(row)) * 8) * (int64_t)sizeof(f16));
   }
-  int ld_kt = 0, ld_v = v0;          // the step that is loaded next
+  int ld_kt = 0;                     // the step that is loaded next
+  int ld_v = v0;
   uint64_t b_base = 0;
-  int b_last = 0;                    // the piece's last row in E: rows past V are this one again
+  int b_last = 0;                    // the piece's last row in E: rows past the run are this one again
   auto set_piece = [&]() {
-    const int64_t first = (int64_t)ld_v * kLpBN;
-    b_base = uniform64((uint64_t)(p.e + first * p.D));
-    b_last = (int)(p.V - 1 - first < kLpBN ? p.V - 1 - first : kLpBN);
+    b_base = uniform64((uint64_t)(p.e + (int64_t)ld_v * p.D));
+    b_last = v1 - 1 - ld_v < BN ? v1 - 1 - ld_v : BN;
   };
   // E's offsets are formed load by load (three instructions beside 16 or more MFMAs): held in registers
   // they would push the accumulators' kernel into scratch memory
@@ -132,11 +148,14 @@ void head_logp_kernel(LpParams p) {
   auto advance = [&]() {
     if (++ld_kt == nk) {
       ld_kt = 0;
-      if (++ld_v < v1) set_piece();
+      if ((ld_v += BN) < v1) set_piece();
     }
   };
   auto wait_loads = [&](int later) {   // at most `later` steps of this wave's loads still in flight
-    if (NST > 2 && later >= 2) wait_vmem<2 * LOADS>();
+    if (NST > 5 && later >= 5) wait_vmem<5 * LOADS>();
+    else if (NST > 4 && later >= 4) wait_vmem<4 * LOADS>();
+    else if (NST > 3 && later >= 3) wait_vmem<3 * LOADS>();
+    else if (NST > 2 && later >= 2) wait_vmem<2 * LOADS>();
     else if (later >= 1) wait_vmem<LOADS>();
     else wait_vmem<0>();
   };
@@ -200,10 +219,10 @@ void head_logp_kernel(LpParams p) {
 #pragma unroll
   for (int i = 0; i < TM; ++i) state[i] = {kNone, 0.0f, 0.0f};
 
-  // the accumulators of piece v into the states
+  // the accumulators of the piece that begins at entry v into the states.  Entries past v1 are entry v1 - 1
+  // again: they leave the largest as it is, and their 2^(z - r) is dropped.
   auto fold = [&](int v) {
-    const int first = v * kLpBN + wn * WN + g4;              // this lane's first vocabulary entry
-    const bool edge = (v + 1) * (int64_t)kLpBN > p.V;
+    const int first = v + wn * WN + g4;                      // this lane's first vocabulary entry
     // a target's product, from the one lane of the launch that holds it
     bool mine = false;
 #pragma unroll
@@ -218,19 +237,12 @@ void head_logp_kernel(LpParams p) {
         for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q) x = at == 16 * j + q ? acc[i][j][q] : x;
-        if (at >= 0 && at < WN && (at & 15) < 4 && at + first < p.V)
+        if (at >= 0 && at < WN && (at & 15) < 4 && at + first < v1)
           p.xt[m0 + wm * WM + 16 * i + r16] = x;
       }
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      if (edge) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (first + 16 * j + q >= p.V) acc[i][j][q] = -INFINITY;
-      }
       float mx = acc[i][0][0];
 #pragma unroll
       for (int j = 0; j < TN; ++j)
@@ -241,16 +253,13 @@ void head_logp_kernel(LpParams p) {
       const float d = old.r - r, w = __builtin_amdgcn_exp2f(d);
       float s = w * old.s, t = w * (old.t + old.s * d);
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float z = __builtin_fmaf(acc[i][j][q], p.c, -r);
-          const float ez = __builtin_amdgcn_exp2f(z);
-          if (edge) z = fmaxf(z, kNone);      // no entry: 0 times a number
-          s += ez;
-          t = __builtin_fmaf(ez, z, t);
-          acc[i][j][q] = 0.0f;
-        }
+      for (int k = 0; k < 4 * TN; ++k) {
+        const float z = __builtin_fmaf(acc[i][k >> 2][k & 3], p.c, -r);
+        float ez = __builtin_amdgcn_exp2f(z);
+        ez = first + 16 * (k >> 2) + (k & 3) < v1 ? ez : 0.0f;
+        s += ez;
+        t = __builtin_fmaf(ez, z, t);
+      }
       state[i] = {r, s, t};
       __builtin_amdgcn_sched_barrier(0);      // one token block's temporaries at a time
     }
@@ -276,8 +285,8 @@ void head_logp_kernel(LpParams p) {
     const bool more = s + 1 < steps, refill = s + NST < steps;
     const int st1 = stage_of(s + 1);
     __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int k = 0; k < NMFMA; ++k) {
+    each([&](auto kc) __attribute__((always_inline)) {
+      constexpr int k = decltype(kc)::value;
       acc[k / TN][kj(k)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
           fb[1][kj(k)], fa[A2 ? 1 : 0][k / TN], acc[k / TN][kj(k)], 0, 0, 0);
       if (more) reads_after(k, st1, 0, 0);
@@ -285,13 +294,17 @@ void head_logp_kernel(LpParams p) {
       for (int d = k * LOADS / NMFMA; d < (k + 1) * LOADS / NMFMA; ++d)
         if (refill) issue(st, d);
       __builtin_amdgcn_sched_barrier(0);
-    }
+    }, std::make_integer_sequence<int, NMFMA>{});
     __builtin_amdgcn_s_setprio(0);
     if (refill) advance();
     if (++kt == nk) {
       fold(v);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       kt = 0;
-      ++v;
+      v += BN;
     }
   }
 
@@ -317,7 +330,28 @@ void head_logp_kernel(LpParams p) {
       const f32x4 b = meet[w * BM + tid];
       a = lp_join(a, {b[0], b[1], b[2]});
     }
-    reinterpret_cast<f32x4*>(p.part)[(m0 + tid) * p.runs + run] = f32x4{a.r, a.s, a.t, 0.0f};
+    reinterpret_cast<f32x4*>(p.part)[lp_part(p.plan, m0 + tid) + run] = f32x4{a.r, a.s, a.t, 0.0f};
+  }
+}
+
+constexpr int lp_halves(int bm, int bn, int nst) { return nst * (bm + bn) * kLpBK; }
+
+template <int BM, int BN, int WAVES_M, int NST, bool TAIL>
+__global__ __launch_bounds__(kLpThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void head_logp_kernel(LpParams p) {
+  constexpr int mine = lp_halves(BM, BN, NST), tail = TAIL ? lp_halves(128, BN, 3) : 0;
+  __shared__ __attribute__((aligned(1024))) f16 S[mine > tail ? mine : tail];
+  __shared__ int32_t tgts[BM];
+  // each XCD (workgroups are dealt to the 8 of them in turn) a contiguous share of (tile, run) with the
+  // tiles fastest, so that the tiles of a run read E through one L2
+  const int total = gridDim.x, o = blockIdx.x & 7, q = total >> 3, r = total & 7;
+  const int u = o * q + (o < r ? o : r) + ((int)blockIdx.x >> 3);
+  const int whole = p.plan.tiles * p.plan.runs;
+  if (!TAIL || u < whole) {
+    lp_walk<BM, BN, WAVES_M, NST>(p, S, tgts, (int64_t)(u % p.plan.tiles) * BM, u / p.plan.tiles,
+                                  p.plan.runs);
+  } else if constexpr (TAIL) {
+    lp_walk<128, BN, 2, 3>(p, S, tgts, (int64_t)p.plan.tiles * BM, u - whole, p.plan.tail);
   }
 }
 
@@ -330,8 +364,9 @@ __global__ __launch_bounds__(256) void head_logp_join_kernel(LpParams p, float* 
   const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= p.n) return;
   LpState a = {kNone, 0.0f, 0.0f};
-  const f32x4* mine = reinterpret_cast<const f32x4*>(p.part) + m * p.runs;
-  for (int i = lane; i < p.runs; i += 64) {
+  const f32x4* mine = reinterpret_cast<const f32x4*>(p.part) + lp_part(p.plan, m);
+  const int runs = lp_runs(p.plan, m);
+  for (int i = lane; i < runs; i += 64) {
     const f32x4 b = mine[i];
     a = lp_join(a, {b[0], b[1], b[2]});
   }
@@ -355,27 +390,47 @@ __global__ __launch_bounds__(256) void head_logp_join_kernel(LpParams p, float* 
   lse[m] = ls;
 }
 
-struct LpPlan {
-  int bm, tiles_m, tiles_v, runs;
-};
-
 constexpr int kLpSlots = 256;   // workgroups at once, one per CU
 
-// 128-token tiles up to 128 tokens, else 256; runs of E such that the workgroups' rounds times the pieces
-// of a run are fewest (and, among equals, the fewest runs).
+// Up to 128 tokens reading E bounds the call: one tile, small pieces of E in deep stages, a run for every CU.
+// More tokens: tiles of 256 by pieces of 256, as many runs as make the rounds of workgroups times the pieces
+// of a run fewest (among equals, the fewest).  Up to 128 tokens behind at most 16 whole tiles are a tile of
+// 128 in the same launch, whose pieces take kTailCost of a whole tile's.
+constexpr float kTailCost = 0.62f;
+
 LpPlan lp_plan(int64_t n, int64_t V) {
-  LpPlan best{n <= 128 ? 128 : 256, 0, (int)((V + kLpBN - 1) / kLpBN), 1};
-  best.tiles_m = (int)((n + best.bm - 1) / best.bm);
-  int64_t cost = -1;
-  for (int g = 1; g <= kLpSlots && g <= best.tiles_v; ++g) {
-    const int64_t c = (((int64_t)best.tiles_m * g + kLpSlots - 1) / kLpSlots) *
-                      ((best.tiles_v + g - 1) / g);
-    if (cost < 0 || c < cost) {
+  if (n <= 128) {
+    const int64_t pieces = (V + 127) / 128;
+    return {n <= 64 ? 64 : 128, 128, 1, (int)(pieces < kLpSlots ? pieces : kLpSlots), 0, (int)pieces};
+  }
+  const int64_t pieces = (V + 255) / 256, rest = n % 256;
+  LpPlan best{256, 256, (int)((n + 255) / 256), 1, 0, (int)pieces};
+  float cost = -1.0f;
+  for (int g = 1; g <= kLpSlots && g <= pieces; ++g) {
+    const float c = (float)((((int64_t)best.tiles * g + kLpSlots - 1) / kLpSlots) * ((pieces + g - 1) / g));
+    if (cost < 0.0f || c < cost) {
       cost = c;
       best.runs = g;
     }
   }
+  const int whole = (int)(n / 256);
+  if (rest == 0 || rest > 128 || whole < 1 || whole > 16) return best;
+  for (int g = 1; g <= pieces && whole * g < kLpSlots; ++g) {
+    const int64_t left = kLpSlots - whole * g, tail = left < pieces ? left : pieces;
+    const float a = (float)((pieces + g - 1) / g), b = kTailCost * (float)((pieces + tail - 1) / tail);
+    const float c = a > b ? a : b;
+    if (c < cost) {
+      cost = c;
+      best = {256, 256, whole, g, (int)tail, (int)pieces};
+    }
+  }
   return best;
+}
+
+// (token, run) states of a plan
+int64_t lp_states(const LpPlan& pl, int64_t n) {
+  const int64_t whole = (int64_t)pl.tiles * pl.bm;
+  return pl.tail ? whole * pl.runs + (n - whole) * pl.tail : n * pl.runs;
 }
 
 bool lp_sizes_ok(int64_t n, int64_t V, int64_t D) {
@@ -391,7 +446,7 @@ using namespace dk;
 
 extern "C" int64_t dk_head_logprobs_workspace(int64_t n, int64_t vocab, int64_t d) {
   if (n <= 0 || !lp_sizes_ok(n, vocab, d)) return 0;
-  return n * (16 * (int64_t)lp_plan(n, vocab).runs + 4);
+  return 16 * lp_states(lp_plan(n, vocab), n) + 4 * n;
 }
 
 extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* rows, int64_t n,
@@ -405,7 +460,7 @@ extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const
   if (!y || !emb || !tgt || !logp || !entropy || !lse || total == 0) return DK_ERR_INVALID;
   // 32-bit byte offsets: a tile's rows of y, or all of y where rows are picked from it
   if (((rows ? total : 256) * ldy + d) * (int64_t)sizeof(f16) >= (int64_t)1 << 32 ||
-      kLpBN * d * (int64_t)sizeof(f16) >= (int64_t)1 << 32)
+      256 * d * (int64_t)sizeof(f16) >= (int64_t)1 << 32)
     return DK_ERR_INVALID;
   if (!dk_aligned(y, 16) || !dk_aligned(emb, 16) || !dk_aligned(tgt, 4) || !dk_aligned(rows, 4) ||
       !dk_aligned(logp, 4) || !dk_aligned(entropy, 4) || !dk_aligned(lse, 4))
@@ -413,13 +468,17 @@ extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const
   if (!ws || ws_bytes < dk_head_logprobs_workspace(n, vocab, d) || !dk_aligned(ws, 16))
     return DK_ERR_WORKSPACE;
   const LpPlan pl = lp_plan(n, vocab);
-  LpParams p{(const f16*)y, ldy, rows, total, (const f16*)emb, tgt, n, vocab, d, scale * kLog2e,
-             pl.tiles_m, pl.tiles_v, pl.runs, (float*)ws, (float*)ws + 4 * n * pl.runs};
-  const dim3 grid((unsigned)(pl.tiles_m * pl.runs));
-  if (pl.bm == 128)
-    hipLaunchKernelGGL((head_logp_kernel<128, 3>), grid, dim3(kLpThreads), 0, stream, p);
+  LpParams p{(const f16*)y, ldy, rows, total, (const f16*)emb, tgt, n, vocab, d, scale * kLog2e, pl,
+             (float*)ws, (float*)ws + 4 * lp_states(pl, n)};
+  const dim3 grid((unsigned)(pl.tiles * pl.runs + pl.tail)), block(kLpThreads);
+  if (pl.bm == 64)
+    hipLaunchKernelGGL((head_logp_kernel<64, 128, 2, 6, false>), grid, block, 0, stream, p);
+  else if (pl.bm == 128)
+    hipLaunchKernelGGL((head_logp_kernel<128, 128, 4, 4, false>), grid, block, 0, stream, p);
+  else if (pl.tail == 0)
+    hipLaunchKernelGGL((head_logp_kernel<256, 256, 2, 2, false>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((head_logp_kernel<256, 2>), grid, dim3(kLpThreads), 0, stream, p);
+    hipLaunchKernelGGL((head_logp_kernel<256, 256, 2, 2, true>), grid, block, 0, stream, p);
   DK_CHECK_LAUNCH();
   hipLaunchKernelGGL(head_logp_join_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, p, logp,
                      entropy, lse);
