@@ -220,28 +220,37 @@ def ptr(t):
 
 
 _raw_stream = None
+_current_device = None
+
+
+def _bind_torch():
+    global _raw_stream, _current_device
+    import torch
+    torch.cuda.init()
+    _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def stream_handle(device=None):
     """The current stream of `device` as the integer handle the C ABI takes (0: the default
     stream), without building a torch.cuda.Stream object per call."""
-    global _raw_stream
     if _raw_stream is None:
-        import torch
-        _raw_stream = torch._C._cuda_getCurrentRawStream
+        _bind_torch()
     index = device.index if device is not None else None
     if index is None:
-        import torch
-        index = torch.cuda.current_device()
+        index = _current_device()
     return _raw_stream(index)
 
 
 def launch(dev, entry, what, *args):
     """The C entry point on dev's current stream, with dev the current device."""
-    import torch
-    if torch.cuda.current_device() == dev.index:
-        rc = entry(*args, stream_handle(dev))
+    if _raw_stream is None:
+        _bind_torch()
+    index = dev.index
+    if _current_device() == index:
+        rc = entry(*args, _raw_stream(index))
     else:
+        import torch
         with torch.cuda.device(dev):
-            rc = entry(*args, stream_handle(dev))
-    check(rc, what)
+            rc = entry(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)

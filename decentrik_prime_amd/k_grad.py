@@ -7,6 +7,7 @@ reference, whose trainer clips with torch).
 The norm stays on the device: no call here waits for the GPU.
 """
 
+from array import array
 from operator import attrgetter
 
 import torch
@@ -15,6 +16,7 @@ from . import _lib
 
 _CODES = {torch.float32: _lib.DK_TYPE_F32, torch.float16: _lib.DK_TYPE_F16,
           torch.bfloat16: _lib.DK_TYPE_BF16}
+# a list's properties are read by maps over C functions: a step has hundreds of small gradients
 _dtype, _pointer, _numel = attrgetter("dtype"), torch.Tensor.data_ptr, torch.Tensor.numel
 _device, _contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
 
@@ -32,19 +34,17 @@ def _dense(t):
 
 def _check(tensors, what):
     """(the tensors' type codes, the device's index)"""
-    codes = [_CODES.get(t) for t in map(_dtype, tensors)]
-    if None in codes:
+    types = list(map(_dtype, tensors))
+    kinds = set(types)
+    if not kinds <= _CODES.keys():
         raise ValueError(f"{what} must be fp32, fp16 or bf16 tensors")
     devices = set(map(_device, tensors))
     if len(devices) != 1 or -1 in devices:
         raise ValueError(f"{what} must be on one GPU")
     if not all(map(_contiguous, tensors)) and not all(map(_dense, tensors)):
         raise ValueError(f"{what} must be dense")
+    codes = [_CODES[types[0]]] * len(types) if len(kinds) == 1 else [_CODES[t] for t in types]
     return codes, devices.pop()
-
-
-def _array(values):
-    return (_lib.ctypes.c_int64 * len(values))(*values)
 
 
 def _run(grads, max_norm, scale, out, in_place=False):
@@ -54,9 +54,9 @@ def _run(grads, max_norm, scale, out, in_place=False):
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive (got {scale})")
     types, index = _check(grads, "gradients")
-    numel = list(map(_numel, grads))
-    src = _array(list(map(_pointer, grads)))
-    dst = None
+    to = types
+    # the host arrays live until the call returns
+    src, numel, dst = array("q", map(_pointer, grads)), array("q", map(_numel, grads)), None
     if out is not None:
         out = list(out)
         if len(out) != len(grads):
@@ -67,19 +67,18 @@ def _run(grads, max_norm, scale, out, in_place=False):
                                        (o.is_contiguous() and g.is_contiguous()))
                 for o, g in zip(out, grads)):
             raise ValueError("outputs must have their gradients' device, shapes and strides")
-        types = [c | o << 4 for c, o in zip(types, to)]
-        dst = _array(list(map(_pointer, out)))
-    else:
-        types = [c | c << 4 for c in types]
-        dst = src if in_place else None
+        dst = array("q", map(_pointer, out))
+    elif in_place:
+        dst = src
+    codes = array("i", [a | b << 4 for a, b in zip(types, to)])
     dev = torch.device("cuda", index)
     lib = _lib.lib()
     nbytes = lib.dk_grad_clip_workspace(len(grads))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    _lib.launch(dev, lib.dk_grad_clip, "dk_grad_clip", src, dst, _array(numel),
-                (_lib.ctypes.c_int32 * len(types))(*types), len(grads), max_norm, scale, norm.data_ptr(),
-                ws.data_ptr(), nbytes)
+    _lib.launch(dev, lib.dk_grad_clip, "dk_grad_clip", src.buffer_info()[0],
+                None if dst is None else dst.buffer_info()[0], numel.buffer_info()[0],
+                codes.buffer_info()[0], len(grads), max_norm, scale, norm.data_ptr(), ws.data_ptr(), nbytes)
     return norm
 
 
