@@ -9,6 +9,7 @@
 // arguments (kBatch of them a launch), so a captured call holds no pointer to host memory and the device
 // keeps no table.  Bound: reading and writing the gradients; few and small ones: two launches.
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "dk_common.h"
@@ -17,7 +18,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kVec = 8;                          // elements of a lane's piece of work
-constexpr int kPiece = kThreads * kVec * 4;      // 8192 elements
+constexpr int kRuns = 4;
+constexpr int kPiece = kThreads * kVec * kRuns;  // 8192 elements
 constexpr int kBatch = 112;                      // tensors of a launch (their table: under 4 KB)
 constexpr int kGroups = 1024;                    // workgroups of a launch, four to a CU
 
@@ -53,44 +55,63 @@ __device__ __forceinline__ Piece piece_of(const Table& t, uint32_t c) {
   return {lo, begin, (int)(left < kPiece ? left : kPiece)};
 }
 
-__device__ __forceinline__ float from_bits(uint16_t u, int type) {
-  if (type == DK_TYPE_F16) return (float)__builtin_bit_cast(f16, u);
+template <int TYPE>
+__device__ __forceinline__ float from_bits(uint16_t u) {
+  if (TYPE == DK_TYPE_F16) return (float)__builtin_bit_cast(f16, u);
   return __builtin_bit_cast(float, (uint32_t)u << 16);
 }
 
-__device__ __forceinline__ uint16_t to_bits(float v, int type) {
-  if (type == DK_TYPE_F16) return __builtin_bit_cast(uint16_t, (f16)v);
+template <int TYPE>
+__device__ __forceinline__ uint16_t to_bits(float v) {
+  if (TYPE == DK_TYPE_F16) return __builtin_bit_cast(uint16_t, (f16)v);
   return __builtin_bit_cast(uint16_t, (bf16)v);
 }
 
-__device__ __forceinline__ float load1(const void* p, int64_t i, int type) {
-  return type == DK_TYPE_F32 ? static_cast<const float*>(p)[i]
-                             : from_bits(static_cast<const uint16_t*>(p)[i], type);
+template <int TYPE>
+__device__ __forceinline__ float load1(const void* p, int64_t i) {
+  if constexpr (TYPE == DK_TYPE_F32) return static_cast<const float*>(p)[i];
+  else return from_bits<TYPE>(static_cast<const uint16_t*>(p)[i]);
 }
 
-__device__ __forceinline__ void store1(void* p, int64_t i, int type, float v) {
-  if (type == DK_TYPE_F32) static_cast<float*>(p)[i] = v;
-  else static_cast<uint16_t*>(p)[i] = to_bits(v, type);
+template <int TYPE>
+__device__ __forceinline__ void store1(void* p, int64_t i, float v) {
+  if constexpr (TYPE == DK_TYPE_F32) static_cast<float*>(p)[i] = v;
+  else static_cast<uint16_t*>(p)[i] = to_bits<TYPE>(v);
 }
 
-__device__ __forceinline__ void load8(const void* p, int64_t i, int type, float (&v)[kVec]) {
-  if (type == DK_TYPE_F32) {
-    const f32x4u a = *reinterpret_cast<const f32x4u*>(static_cast<const float*>(p) + i);
-    const f32x4u b = *reinterpret_cast<const f32x4u*>(static_cast<const float*>(p) + i + 4);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = a[k];
-      v[k + 4] = b[k];
-    }
+// kVec elements as loaded, and as numbers
+template <int TYPE>
+struct Raw {
+  f32x4u a, b;
+};
+template <>
+struct Raw<DK_TYPE_F16> {
+  u16x8u a;
+};
+template <>
+struct Raw<DK_TYPE_BF16> {
+  u16x8u a;
+};
+
+template <int TYPE>
+__device__ __forceinline__ Raw<TYPE> load8(const void* p, int64_t i) {
+  if constexpr (TYPE == DK_TYPE_F32) {
+    const float* q = static_cast<const float*>(p) + i;
+    return {*reinterpret_cast<const f32x4u*>(q), *reinterpret_cast<const f32x4u*>(q + 4)};
   } else {
-    const u16x8u a = *reinterpret_cast<const u16x8u*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = from_bits(a[k], type);
+    return {*reinterpret_cast<const u16x8u*>(static_cast<const uint16_t*>(p) + i)};
   }
 }
 
-__device__ __forceinline__ void store8(void* p, int64_t i, int type, const float (&v)[kVec]) {
-  if (type == DK_TYPE_F32) {
+template <int TYPE>
+__device__ __forceinline__ float number(const Raw<TYPE>& r, int k) {
+  if constexpr (TYPE == DK_TYPE_F32) return k < 4 ? r.a[k] : r.b[k - 4];
+  else return from_bits<TYPE>(r.a[k]);
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[kVec]) {
+  if constexpr (TYPE == DK_TYPE_F32) {
     f32x4u a, b;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -102,9 +123,35 @@ __device__ __forceinline__ void store8(void* p, int64_t i, int type, const float
   } else {
     u16x8u a;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = to_bits(v[k], type);
+    for (int k = 0; k < 8; ++k) a[k] = to_bits<TYPE>(v[k]);
     *reinterpret_cast<u16x8u*>(static_cast<uint16_t*>(p) + i) = a;
   }
+}
+
+// f with the type as a constant
+template <class F>
+__device__ __forceinline__ void with_type(int type, F&& f) {
+  if (type == DK_TYPE_F32) f(std::integral_constant<int, DK_TYPE_F32>{});
+  else if (type == DK_TYPE_F16) f(std::integral_constant<int, DK_TYPE_F16>{});
+  else f(std::integral_constant<int, DK_TYPE_BF16>{});
+}
+
+// A piece: vec(raw elements, place) for each run of kVec, all loads of a whole piece before the first use;
+// one(element's place) for the last elements of a tensor.
+template <int TYPE, class V, class O>
+__device__ __forceinline__ void walk(const void* src, const Piece& q, V&& vec, O&& one) {
+  const int i0 = kVec * threadIdx.x;
+  if (q.count == kPiece) {
+    Raw<TYPE> r[kRuns];
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) r[u] = load8<TYPE>(src, q.begin + i0 + u * kVec * kThreads);
+#pragma unroll
+    for (int u = 0; u < kRuns; ++u) vec(r[u], q.begin + i0 + u * kVec * kThreads);
+    return;
+  }
+  int i = i0;
+  for (; i + kVec <= q.count; i += kVec * kThreads) vec(load8<TYPE>(src, q.begin + i), q.begin + i);
+  for (; i < q.count; ++i) one(q.begin + i);   // one lane, fewer than kVec
 }
 
 // the workgroup's sum in a fixed order; every thread gets it
@@ -124,19 +171,18 @@ __global__ __launch_bounds__(kThreads) void squares_kernel(Table t, uint32_t pie
   double s = 0.0;
   for (uint32_t c = blockIdx.x; c < pieces; c += gridDim.x) {
     const Piece q = piece_of(t, c);
-    const int type = t.type[q.tensor] & 15;
     const void* src = t.src[q.tensor];
-    int i = kVec * threadIdx.x;
-    for (; i + kVec <= q.count; i += kVec * kThreads) {
-      float v[kVec];
-      load8(src, q.begin + i, type, v);
+    with_type(t.type[q.tensor] & 15, [&](auto type) {
+      constexpr int T = decltype(type)::value;
+      auto add = [&](double v) { s = __builtin_fma(v, v, s); };
+      walk<T>(
+          src, q,
+          [&](const Raw<T>& r, int64_t) {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) s = __builtin_fma((double)v[k], (double)v[k], s);
-    }
-    for (; i < q.count; ++i) {     // the tensor's last elements: one lane holds fewer than kVec
-      const double v = load1(src, q.begin + i, type);
-      s = __builtin_fma(v, v, s);
-    }
+            for (int k = 0; k < kVec; ++k) add((double)number<T>(r, k));
+          },
+          [&](int64_t i) { add((double)load1<T>(src, i)); });
+    });
   }
   const double total = block_sum(s, red);
   if (threadIdx.x == 0) part[blockIdx.x] = total;
@@ -154,19 +200,23 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, uint32_t piece
   const float factor = (float)(scale * (ratio > 1.0 ? 1.0 : ratio));   // a NaN norm: NaN
   for (uint32_t b = blockIdx.x; b < pieces; b += gridDim.x) {
     const Piece q = piece_of(t, pieces - 1 - b);
-    const int type = t.type[q.tensor] & 15, to = t.type[q.tensor] >> 4;
     const void* src = t.src[q.tensor];
     void* dst = t.dst[q.tensor];
     if (src == dst && factor == 1.0f) continue;   // nothing changes in place
-    int i = kVec * threadIdx.x;
-    for (; i + kVec <= q.count; i += kVec * kThreads) {
-      float v[kVec];
-      load8(src, q.begin + i, type, v);
+    with_type(t.type[q.tensor] & 15, [&](auto type) {
+      with_type(t.type[q.tensor] >> 4, [&](auto to) {
+        constexpr int T = decltype(type)::value, U = decltype(to)::value;
+        walk<T>(
+            src, q,
+            [&](const Raw<T>& r, int64_t i) {
+              float v[kVec];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) v[k] *= factor;
-      store8(dst, q.begin + i, to, v);
-    }
-    for (; i < q.count; ++i) store1(dst, q.begin + i, to, load1(src, q.begin + i, type) * factor);
+              for (int k = 0; k < kVec; ++k) v[k] = number<T>(r, k) * factor;
+              store8<U>(dst, i, v);
+            },
+            [&](int64_t i) { store1<U>(dst, i, load1<T>(src, i) * factor); });
+      });
+    });
   }
 }
 
@@ -183,18 +233,18 @@ extern "C" int64_t dk_grad_clip_workspace(int64_t n) {
 }
 
 extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int64_t* numel,
-                            const int32_t* types, int64_t n, double max_norm, double scale, float* norm,
+                            const int32_t* types, const int32_t* dst_types, int64_t n, double max_norm, double scale, float* norm,
                             void* ws, int64_t ws_bytes, hipStream_t stream) {
-  if (n < 1 || n > (int64_t)1 << 20 || !src || !numel || !types || !norm || !(max_norm > 0.0) ||
+  if (n < 1 || n > (int64_t)1 << 20 || !src || !numel || !types || (dst && !dst_types) || !norm || !(max_norm > 0.0) ||
       !(scale > 0.0) || scale - scale != 0.0)
     return DK_ERR_INVALID;
   if (!dk_aligned(norm, 4)) return DK_ERR_ALIGN;
   for (int64_t i = 0; i < n; ++i) {
-    const int64_t from = type_size(types[i] & 15), to = type_size(types[i] >> 4);
+    const int64_t from = type_size(types[i]), to = dst ? type_size(dst_types[i]) : from;
     if (!from || !to || numel[i] < 0 || numel[i] > (int64_t)1 << 40) return DK_ERR_INVALID;
     if (numel[i] && (!src[i] || (dst && !dst[i]))) return DK_ERR_INVALID;
     if (!dk_aligned(src[i], from) || (dst && !dk_aligned(dst[i], to))) return DK_ERR_ALIGN;
-    if (dst && dst[i] == src[i] && numel[i] && (types[i] & 15) != types[i] >> 4) return DK_ERR_INVALID;
+    if (dst && dst[i] == src[i] && numel[i] && types[i] != dst_types[i]) return DK_ERR_INVALID;
   }
   if (dst) {
     // what is written overlaps nothing else that is read or written: in place, its own source alone
@@ -208,8 +258,8 @@ extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int6
       for (int64_t i = 0; i < n; ++i) {
         if (!numel[i]) continue;
         const uintptr_t s = (uintptr_t)src[i], d = (uintptr_t)dst[i];
-        all.push_back({d, d + numel[i] * type_size(types[i] >> 4), true});
-        if (s != d) all.push_back({s, s + numel[i] * type_size(types[i] & 15), false});
+        all.push_back({d, d + numel[i] * type_size(dst_types[i]), true});
+        if (s != d) all.push_back({s, s + numel[i] * type_size(types[i]), false});
       }
       std::sort(all.begin(), all.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
       uintptr_t written = 0, touched = 0;
@@ -236,7 +286,7 @@ extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int6
       t.src[t.n] = src[i];
       t.dst[t.n] = dst ? dst[i] : nullptr;
       t.numel[t.n] = numel[i];
-      t.type[t.n] = (uint8_t)types[i];
+      t.type[t.n] = (uint8_t)(types[i] | (dst ? dst_types[i] : 0) << 4);
       t.first[t.n] = (uint32_t)pieces;
       ++t.n;
       pieces += c;

@@ -1,9 +1,9 @@
 // Losses over the log-probabilities of a packed batch's answers, forward and gradient in one call: the
 // clipped policy loss with a KL term, and the preference loss over pairs of answers.
 //
-// A batch is rows (answers) of consecutive tokens; the host cuts them into items of at most a few
-// thousand tokens of one row (k_loss.RowMeta), a wave each.  An item is {first token (two words), tokens,
-// row}; an empty row has one item without tokens.
+// A batch is rows (answers) of consecutive tokens; the host cuts them into items (k_loss.RowMeta), a wave
+// each: {first token (two words), tokens, row, the row's tokens, its items, the item's place among them, 0}.
+// One 32-byte load tells a wave all that it needs before its tokens.  An empty row has one item without tokens.
 //
 // Policy, per token with advantage A:  r = e^(logp - old),  clipped where A > 0 and r > 1 + high or A < 0
 // and r < 1 - low,  p = -A r (clipped: -A times the bound),  f = ref - logp,  k = e^f - f - 1
@@ -20,8 +20,10 @@
 namespace {
 
 constexpr int kWaves = 4;        // items of a workgroup
-constexpr int kOneWaves = 16;    // items that a single workgroup takes in one launch
+constexpr int kOneWaves = 16;    // the single workgroup of a call with few items
+constexpr int kOneItems = 64;
 constexpr int kAhead = 8;        // tokens of a lane in flight
+constexpr int kPairs = 1024;     // pairs of a workgroup
 
 struct Tokens {          // a token array: element i at p[i * stride], negated where it holds losses
   const float* p;
@@ -33,11 +35,12 @@ struct Tokens {          // a token array: element i at p[i * stride], negated w
 struct Item {
   int64_t begin;
   int count, row;
+  int len, of, at;       // its row's tokens and items, and which of them it is
 };
 
 __device__ __forceinline__ Item item_of(const int4* items, int i) {
-  const int4 v = items[i];
-  return {(int64_t)(((uint64_t)(uint32_t)v.y << 32) | (uint32_t)v.x), v.z, v.w};
+  const int4 v = items[2 * (int64_t)i], w = items[2 * (int64_t)i + 1];
+  return {(int64_t)(((uint64_t)(uint32_t)v.y << 32) | (uint32_t)v.x), v.z, v.w, w.x, w.y, w.z};
 }
 
 // the sum over the wave's lanes (a butterfly: every lane gets it, in one order)
@@ -65,7 +68,6 @@ __device__ __forceinline__ float expm1_minus(float f) {
 struct PolicyParams {
   const int4* items;
   const int32_t* row_items;   // [rows + 1] a row's items
-  const int64_t* lens;        // [rows]
   int n_items, rows;
   Tokens logp, old, ref;      // ref.p null: none
   const float* adv;
@@ -85,41 +87,38 @@ struct Sums {
   double v[4];
 };
 
-// a token's share of the loss
-__device__ __forceinline__ double policy_weight(const PolicyParams& p, int row) {
-  const int64_t len = p.lens[row];
-  return p.reduction == 0 && len > 0 ? p.inv / (double)len : p.inv;
-}
-
-// one item: dlogp, and the sums of p, k, clipped and r
-__device__ __forceinline__ Sums policy_item(const PolicyParams& p, const Item& it, double weight) {
+// One item: dlogp, and the sums of p, k, clipped and r.  Returns its share of the loss.
+__device__ __forceinline__ double policy_item(const PolicyParams& p, const Item& it, Sums& s) {
   const int lane = threadIdx.x & 63;
+  s = Sums{};
+  if (it.count == 0) return 0.0;
+  const double weight = p.reduction == 0 ? p.inv / (double)it.len : p.inv;   // a token's share of the loss
   const float w = (float)weight;
-  const float row_adv = p.adv_per_token ? 0.0f : p.adv[it.row];
-  Sums s{};
+  const float* adv = p.adv_per_token ? p.adv + it.begin : p.adv + it.row;
   for (int t0 = 0; t0 < it.count; t0 += 64 * kAhead) {
     float x[kAhead], o[kAhead], rf[kAhead], a[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {   // every load before the first use, at tokens inside the item
-      const int t = t0 + 64 * u + lane;
-      const int64_t i = it.begin + (t < it.count ? t : it.count - 1);
-      x[u] = p.logp.at(i);
-      o[u] = p.old.at(i);
-      rf[u] = p.ref.p ? p.ref.at(i) : 0.0f;
-      a[u] = p.adv_per_token ? p.adv[i] : row_adv;
+      const int t = t0 + 64 * u + lane, in = t < it.count ? t : it.count - 1;
+      const int64_t i = it.begin + in;
+      x[u] = p.logp.p[i * p.logp.stride];
+      o[u] = p.old.p[i * p.old.stride];
+      rf[u] = p.ref.p ? p.ref.p[i * p.ref.stride] : 0.0f;
+      a[u] = adv[p.adv_per_token ? in : 0];
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int t = t0 + 64 * u + lane;
       if (t >= it.count) continue;
-      const double d = (double)x[u] - (double)o[u];
-      const bool up = a[u] > 0.0f && d > p.log_high, down = a[u] < 0.0f && d < p.log_low;
+      const float xs = p.logp.sign * x[u], av = a[u];
+      const double d = (double)xs - (double)(p.old.sign * o[u]);
+      const bool up = av > 0.0f && d > p.log_high, down = av < 0.0f && d < p.log_low;
       const float r = expf((float)d);
-      const float kept = up || down ? 0.0f : r * a[u];
-      const float pol = up ? p.high * a[u] : down ? p.low * a[u] : kept;
+      const float kept = up || down ? 0.0f : r * av;
+      const float pol = up ? p.high * av : down ? p.low * av : kept;
       float g = -kept, k = 0.0f;
       if (p.ref.p) {
-        const float f = (float)((double)rf[u] - (double)x[u]);
+        const float f = (float)((double)(p.ref.sign * rf[u]) - (double)xs);
         k = expm1_minus(f);
         g -= p.beta * (f + k);
       }
@@ -132,38 +131,60 @@ __device__ __forceinline__ Sums policy_item(const PolicyParams& p, const Item& i
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) s.v[q] = wave_sum(s.v[q]);
-  return s;
+  return weight * (s.v[0] + (double)p.beta * s.v[1]);
 }
 
-__device__ __forceinline__ void store_stats(const PolicyParams& p, int row, const Sums& s) {
-  const int64_t len = p.lens[row];
+__device__ __forceinline__ void store_stats(const PolicyParams& p, int64_t row, int len, const Sums& s) {
   const double inv = len > 0 ? 1.0 / (double)len : 0.0;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) p.stats[4 * (int64_t)row + q] = (float)(s.v[q] * inv);
+  for (int q = 0; q < 4; ++q) p.stats[4 * row + q] = (float)(s.v[q] * inv);
 }
 
-// WAVES items per workgroup.  One workgroup (WAVES = kOneWaves) writes everything; otherwise rows of one
-// item write their stats, and the second launch sums the workgroups' losses and the other rows' items.
-template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void policy_kernel(PolicyParams p) {
+// Up to kOneItems items: everything in one workgroup and launch.
+__global__ __launch_bounds__(64 * kOneWaves) void policy_one_kernel(PolicyParams p) {
+  __shared__ Sums sums[kOneItems];
+  __shared__ double loss[kOneItems];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int i = blockIdx.x * WAVES + wave;
-  __shared__ double loss[WAVES];
-  __shared__ Sums sums[WAVES];
-  __shared__ int row_of[WAVES];
+  for (int i = wave; i < p.n_items; i += kOneWaves) {
+    Sums s;
+    const double l = policy_item(p, item_of(p.items, i), s);
+    if (lane == 0) {
+      sums[i] = s;
+      loss[i] = l;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < p.n_items) {     // a row's first item
+    const Item it = item_of(p.items, threadIdx.x);
+    if (it.at == 0) {
+      Sums s{};
+      for (int i = threadIdx.x; i < (int)threadIdx.x + it.of; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s.v[q] += sums[i].v[q];
+      store_stats(p, it.row, it.len, s);
+    }
+  }
+  if (wave == kOneWaves - 1) {
+    const double total = wave_sum(lane < p.n_items ? loss[lane] : 0.0);
+    if (lane == 0) *p.loss = (float)total;
+  }
+}
+
+// kWaves items per workgroup.  Rows of one item write their stats; the second launch sums the workgroups'
+// losses and the other rows' items.
+__global__ __launch_bounds__(64 * kWaves) void policy_kernel(PolicyParams p) {
+  __shared__ double loss[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = blockIdx.x * kWaves + wave;
   double mine = 0.0;
   if (i < p.n_items) {
     const Item it = item_of(p.items, i);
-    const double w = policy_weight(p, it.row);
-    const Sums s = policy_item(p, it, w);
-    mine = it.count > 0 ? w * (s.v[0] + (double)p.beta * s.v[1]) : 0.0;
-    const bool whole = p.row_items[it.row + 1] - p.row_items[it.row] == 1;
+    Sums s;
+    mine = policy_item(p, it, s);
     if (lane == 0) {
-      if (whole) store_stats(p, it.row, s);
-      if (WAVES == kOneWaves) {
-        sums[wave] = s;
-        row_of[wave] = whole ? -1 : it.row;
-      } else if (!whole) {
+      if (it.of == 1) {
+        store_stats(p, it.row, it.len, s);
+      } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q) p.part[4 * (int64_t)i + q] = s.v[q];
       }
@@ -174,24 +195,27 @@ __global__ __launch_bounds__(64 * WAVES) void policy_kernel(PolicyParams p) {
   if (threadIdx.x == 0) {
     double total = 0.0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) total += loss[w];
-    if (WAVES == kOneWaves) *p.loss = (float)total;
-    else p.part[4 * (int64_t)p.n_items + blockIdx.x] = total;
-  }
-  if (WAVES == kOneWaves && lane == 0 && i < p.n_items && row_of[wave] >= 0 &&
-      p.row_items[row_of[wave]] == i) {
-    Sums s{};
-    for (int w = wave; w < WAVES && w < p.n_items && row_of[w] == row_of[wave]; ++w)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) s.v[q] += sums[w].v[q];
-    store_stats(p, row_of[wave], s);
+    for (int w = 0; w < kWaves; ++w) total += loss[w];
+    p.part[4 * (int64_t)p.n_items + blockIdx.x] = total;
   }
 }
 
 constexpr int kSumThreads = 1024;
 
-// n numbers' sum over a workgroup of kSumThreads, in a fixed order; thread 0 has it
-__device__ __forceinline__ double block_sum(const double* v, int64_t n, double* red) {
+// the sum of THREADS threads' values, in a fixed order; thread 0 has it
+template <int THREADS>
+__device__ __forceinline__ double block_sum(double s, double* red) {
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  double total = 0.0;
+  if (threadIdx.x == 0)
+    for (int w = 0; w < THREADS / 64; ++w) total += red[w];
+  return total;
+}
+
+// n numbers' sum over a workgroup of kSumThreads; thread 0 has it
+__device__ __forceinline__ double array_sum(const double* v, int64_t n, double* red) {
   double s = 0.0;
   int64_t i = threadIdx.x;
   for (; i + 3 * kSumThreads < n; i += 4 * kSumThreads) {
@@ -202,13 +226,7 @@ __device__ __forceinline__ double block_sum(const double* v, int64_t n, double* 
     for (int u = 0; u < 4; ++u) s += a[u];
   }
   for (; i < n; i += kSumThreads) s += v[i];
-  s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  double total = 0.0;
-  if (threadIdx.x == 0)
-    for (int w = 0; w < kSumThreads / 64; ++w) total += red[w];
-  return total;
+  return block_sum<kSumThreads>(s, red);
 }
 
 // Workgroup 0: the loss.  The others: a wave per row of several items (its items by lane; a row has at
@@ -216,7 +234,7 @@ __device__ __forceinline__ double block_sum(const double* v, int64_t n, double* 
 __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(PolicyParams p, int workgroups) {
   __shared__ double red[kSumThreads / 64];
   if (blockIdx.x == 0) {
-    const double total = block_sum(p.part + 4 * (int64_t)p.n_items, workgroups, red);
+    const double total = array_sum(p.part + 4 * (int64_t)p.n_items, workgroups, red);
     if (threadIdx.x == 0) *p.loss = (float)total;
     return;
   }
@@ -231,16 +249,16 @@ __global__ __launch_bounds__(kSumThreads) void policy_sum_kernel(PolicyParams p,
     for (int q = 0; q < 4; ++q) s.v[q] += p.part[4 * (int64_t)i + q];
 #pragma unroll
   for (int q = 0; q < 4; ++q) s.v[q] = wave_sum(s.v[q]);
-  if (lane == 0) store_stats(p, (int)row, s);
+  if (lane == 0) store_stats(p, row, item_of(p.items, b).len, s);
 }
 
 // ---------------------------------------------------------------------------------------------
 struct PrefParams {
   const int4* items;
   const int32_t* row_items;    // [rows + 1]
-  const int64_t* lens;         // [rows]
   const int32_t* row_pairs;    // [rows + 1] a row's entries in `entries`
-  const int2* entries;         // (other row, pair + 1: this row is chosen, -(pair + 1): rejected)
+  const int2* entries;         // (other row, 1: this row is chosen, 0: rejected)
+  const int2* pairs;           // (chosen, rejected)
   int n_items, rows, n_pairs;
   Tokens logp, ref;            // ref.p null: none
   double beta, margin, smoothing;
@@ -250,7 +268,7 @@ struct PrefParams {
   float* rewards;              // [rows]
   float* margins;              // [pairs]
   float* loss;
-  double* part;                // [n_items] items' sums of logp - ref; then a loss per pair
+  double* part;                // [n_items] items' sums of logp - ref; then a loss per workgroup of pairs
 };
 
 __device__ __forceinline__ double pref_item(const PrefParams& p, const Item& it) {
@@ -262,12 +280,13 @@ __device__ __forceinline__ double pref_item(const PrefParams& p, const Item& it)
     for (int u = 0; u < kAhead; ++u) {
       const int t = t0 + 64 * u + lane;
       const int64_t i = it.begin + (t < it.count ? t : it.count - 1);
-      x[u] = p.logp.at(i);
-      r[u] = p.ref.p ? p.ref.at(i) : 0.0f;
+      x[u] = p.logp.p[i * p.logp.stride];
+      r[u] = p.ref.p ? p.ref.p[i * p.ref.stride] : 0.0f;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (t0 + 64 * u + lane < it.count) s += (double)x[u] - (double)r[u];
+      if (t0 + 64 * u + lane < it.count)
+        s += (double)(p.logp.sign * x[u]) - (double)(p.ref.sign * r[u]);
   }
   return wave_sum(s);
 }
@@ -275,16 +294,27 @@ __device__ __forceinline__ double pref_item(const PrefParams& p, const Item& it)
 // S of a row from its items' sums, one lane (items in order)
 __device__ __forceinline__ double row_score(const PrefParams& p, const double* part, int row) {
   const int b = p.row_items[row], e = p.row_items[row + 1];
+  const int len = p.items[2 * (int64_t)b + 1].x;
   double s = 0.0;
   for (int i = b; i < e; ++i) s += part[i];
-  const int64_t len = p.lens[row];
   return p.average && len > 0 ? s / (double)len : s;
 }
+
+// where the rows' S come from: the items' sums in memory, or the one workgroup's own table
+struct FromItems {
+  const PrefParams& p;
+  __device__ __forceinline__ double operator()(int row) const { return row_score(p, p.part, row); }
+};
+
+struct FromTable {
+  const double* s;
+  __device__ __forceinline__ double operator()(int row) const { return s[row]; }
+};
 
 // L(h) and L'(h)
 __device__ __forceinline__ double pref_loss(const PrefParams& p, double h, double* slope) {
   if (p.kind == 0) {
-    // -(1 - e) log s(h) - e log s(-h): log(1 + e^-|h|) is one of the two softplus terms' part
+    // -(1 - e) log s(h) - e log s(-h) = (1 - e) max(-h, 0) + e max(h, 0) + log(1 + e^-|h|)
     const double tail = log1p(exp(-fabs(h)));
     *slope = p.smoothing / (1.0 + exp(-h)) - (1.0 - p.smoothing) / (1.0 + exp(h));
     return (1.0 - p.smoothing) * (fmax(-h, 0.0) + tail) + p.smoothing * (fmax(h, 0.0) + tail);
@@ -303,51 +333,56 @@ __device__ __forceinline__ double pref_h(const PrefParams& p, double chosen, dou
 }
 
 // The item's gradient from the items' sums: the row's coefficient (its pairs by lane), then the tokens.
-// The row's first item also writes its reward, and the margins and losses of the pairs that it is the
-// chosen row of.
-__device__ __forceinline__ void pref_apply(const PrefParams& p, const double* part, int i, const Item& it,
-                                           double* pair_loss) {
+// The row's first item also writes its reward.
+template <class Score>
+__device__ __forceinline__ void pref_apply(const PrefParams& p, const Score& score, const Item& it) {
   const int lane = threadIdx.x & 63;
-  const double own = row_score(p, part, it.row);
-  const bool first = p.row_items[it.row] == i;
-  if (first && lane == 0) p.rewards[it.row] = (float)(p.beta * own);
+  const double own = score(it.row);
+  if (it.at == 0 && lane == 0) p.rewards[it.row] = (float)(p.beta * own);
+  if (it.count == 0) return;
   double g = 0.0;
   for (int e = p.row_pairs[it.row] + lane; e < p.row_pairs[it.row + 1]; e += 64) {
     const int2 en = p.entries[e];
-    const double other = row_score(p, part, en.x);
-    const bool chosen = en.y > 0;
+    const double other = score(en.x);
     double slope;
-    const double h = chosen ? pref_h(p, own, other) : pref_h(p, other, own);
-    const double l = pref_loss(p, h, &slope);
-    g += chosen ? slope : -slope;
-    if (chosen && first) {
-      p.margins[en.y - 1] = (float)h;
-      pair_loss[en.y - 1] = l;
-    }
+    pref_loss(p, en.y ? pref_h(p, own, other) : pref_h(p, other, own), &slope);
+    g += en.y ? slope : -slope;
   }
   g = wave_sum(g) * p.beta / (double)p.n_pairs;
-  const int64_t len = p.lens[it.row];
-  const float gf = (float)(p.average && len > 0 ? g / (double)len : g);
+  const float gf = (float)(p.average ? g / (double)it.len : g);
   for (int t = lane; t < it.count; t += 64) p.dlogp[it.begin + t] = gf;
 }
 
-// every item and pair in one workgroup
+// margins of pairs i, i + step, ... below end; the sum of their losses
+template <class Score>
+__device__ __forceinline__ double pref_pairs(const PrefParams& p, const Score& score, int i, int end, int step) {
+  double s = 0.0;
+  for (; i < end; i += step) {
+    const int2 pr = p.pairs[i];
+    const double h = pref_h(p, score(pr.x), score(pr.y));
+    double slope;
+    s += pref_loss(p, h, &slope);
+    p.margins[i] = (float)h;
+  }
+  return s;
+}
+
+// Up to kOneItems items and kPairs pairs: everything in one workgroup and launch.
 __global__ __launch_bounds__(64 * kOneWaves) void pref_one_kernel(PrefParams p) {
+  __shared__ double sums[kOneItems], scores[kOneItems];
+  __shared__ double red[kOneWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  __shared__ double sums[kOneWaves];
-  __shared__ double red[kSumThreads / 64];
-  static_assert(64 * kOneWaves == kSumThreads, "block_sum's threads");
-  Item it{0, 0, 0};
-  if (wave < p.n_items) {
-    it = item_of(p.items, wave);
-    const double s = pref_item(p, it);
-    if (lane == 0) sums[wave] = s;
+  for (int i = wave; i < p.n_items; i += kOneWaves) {
+    const double s = pref_item(p, item_of(p.items, i));
+    if (lane == 0) sums[i] = s;
   }
   __syncthreads();
-  double* pair_loss = p.part + p.n_items;
-  if (wave < p.n_items) pref_apply(p, sums, wave, it, pair_loss);
+  if (threadIdx.x < p.rows) scores[threadIdx.x] = row_score(p, sums, threadIdx.x);   // rows <= items
   __syncthreads();
-  const double total = block_sum(pair_loss, p.n_pairs, red);
+  const FromTable score{scores};
+  for (int i = wave; i < p.n_items; i += kOneWaves) pref_apply(p, score, item_of(p.items, i));
+  const double l = pref_pairs(p, score, threadIdx.x, p.n_pairs, 64 * kOneWaves);
+  const double total = block_sum<64 * kOneWaves>(l, red);
   if (threadIdx.x == 0) *p.loss = (float)(total / (double)p.n_pairs);
 }
 
@@ -358,15 +393,27 @@ __global__ __launch_bounds__(64 * kWaves) void pref_sum_kernel(PrefParams p) {
   if ((threadIdx.x & 63) == 0) p.part[i] = s;
 }
 
-__global__ __launch_bounds__(64 * kWaves) void pref_apply_kernel(PrefParams p) {
-  const int i = blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (i >= p.n_items) return;
-  pref_apply(p, p.part, i, item_of(p.items, i), p.part + p.n_items);
+// The first pair_wgs workgroups: kPairs pairs each (one alone: the loss too); the others: kWaves items.
+__global__ __launch_bounds__(64 * kWaves) void pref_apply_kernel(PrefParams p, int pair_wgs) {
+  __shared__ double red[kWaves];
+  const int b = blockIdx.x;
+  if (b < pair_wgs) {
+    const int first = b * kPairs, end = first + kPairs < p.n_pairs ? first + kPairs : p.n_pairs;
+    const double l = pref_pairs(p, FromItems{p}, first + threadIdx.x, end, 64 * kWaves);
+    const double total = block_sum<64 * kWaves>(l, red);
+    if (threadIdx.x == 0) {
+      if (pair_wgs == 1) *p.loss = (float)(total / (double)p.n_pairs);
+      else p.part[p.n_items + b] = total;
+    }
+    return;
+  }
+  const int i = (b - pair_wgs) * kWaves + (threadIdx.x >> 6);
+  if (i < p.n_items) pref_apply(p, FromItems{p}, item_of(p.items, i));
 }
 
-__global__ __launch_bounds__(kSumThreads) void pref_loss_kernel(PrefParams p) {
+__global__ __launch_bounds__(kSumThreads) void pref_loss_kernel(PrefParams p, int pair_wgs) {
   __shared__ double red[kSumThreads / 64];
-  const double total = block_sum(p.part + p.n_items, p.n_pairs, red);
+  const double total = array_sum(p.part + p.n_items, pair_wgs, red);
   if (threadIdx.x == 0) *p.loss = (float)(total / (double)p.n_pairs);
 }
 
@@ -385,35 +432,35 @@ bool rows_ok(int64_t n_items, int64_t rows) {
 }  // namespace
 
 extern "C" int64_t dk_policy_loss_workspace(int64_t n_items) {
-  return n_items <= 0 ? 0 : (4 * n_items + (n_items + kWaves - 1) / kWaves) * (int64_t)sizeof(double);
+  return n_items <= kOneItems ? 0 : (4 * n_items + (n_items + kWaves - 1) / kWaves) * (int64_t)sizeof(double);
 }
 
-extern "C" int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items,
-                              const int64_t* lens, int64_t rows, int64_t n_tokens,
-                              const dk_token_array* logp, const dk_token_array* old, const dk_token_array* ref, const float* advantages,
-                              int per_token, double clip_low, double clip_high, double kl_coef,
-                              int reduction, double denominator, float* dlogp, float* stats, float* loss,
-                              void* ws, int64_t ws_bytes, hipStream_t stream) {
-  if (!rows_ok(n_items, rows) || !items || !row_items || !lens || !tokens_ok(logp, n_tokens) ||
+extern "C" int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items, int64_t rows,
+                              int64_t n_tokens, const dk_token_array* logp, const dk_token_array* old,
+                              const dk_token_array* ref, const float* advantages, int per_token,
+                              double clip_low, double clip_high, double kl_coef, int reduction,
+                              double denominator, float* dlogp, float* stats, float* loss, void* ws,
+                              int64_t ws_bytes, hipStream_t stream) {
+  if (!rows_ok(n_items, rows) || !items || !row_items || !tokens_ok(logp, n_tokens) ||
       !tokens_ok(old, n_tokens) || (ref && !tokens_ok(ref, n_tokens)) || (n_tokens > 0 && !dlogp) || !stats ||
       !loss || (!advantages && (n_tokens > 0 || !per_token)) ||
-      !(clip_low >= 0.0 && clip_low <= 1.0) ||
-      !(clip_high >= 0.0) || !(kl_coef - kl_coef == 0.0) || (kl_coef != 0.0 && !ref) || reduction < 0 ||
-      reduction > 2 || !(denominator > 0.0))
+      !(clip_low >= 0.0 && clip_low <= 1.0) || !(clip_high >= 0.0) || !(kl_coef - kl_coef == 0.0) ||
+      (kl_coef != 0.0 && !ref) || reduction < 0 || reduction > 2 || !(denominator > 0.0))
     return DK_ERR_INVALID;
-  if (!dk_aligned(items, 16) || !dk_aligned(lens, 8)) return DK_ERR_ALIGN;
-  if (!ws || ws_bytes < dk_policy_loss_workspace(n_items) || !dk_aligned(ws, 8)) return DK_ERR_WORKSPACE;
-  PolicyParams p{reinterpret_cast<const int4*>(items), row_items, lens, (int)n_items, (int)rows,
+  if (!dk_aligned(items, 16) || !dk_aligned(row_items, 4)) return DK_ERR_ALIGN;
+  const int64_t need = dk_policy_loss_workspace(n_items);
+  if (need && (!ws || ws_bytes < need || !dk_aligned(ws, 8))) return DK_ERR_WORKSPACE;
+  PolicyParams p{reinterpret_cast<const int4*>(items), row_items, (int)n_items, (int)rows,
                  tokens_of(logp), tokens_of(old), tokens_of(ref), advantages, per_token,
                  log1p(-clip_low), log1p(clip_high), (float)(1.0 - clip_low), (float)(1.0 + clip_high),
                  (float)kl_coef, reduction, 1.0 / denominator, dlogp, stats, loss, (double*)ws};
-  if (n_items <= kOneWaves) {
-    hipLaunchKernelGGL((policy_kernel<kOneWaves>), dim3(1), dim3(64 * kOneWaves), 0, stream, p);
+  if (n_items <= kOneItems) {
+    hipLaunchKernelGGL(policy_one_kernel, dim3(1), dim3(64 * kOneWaves), 0, stream, p);
     DK_CHECK_LAUNCH();
     return 0;
   }
   const int wgs = (int)((n_items + kWaves - 1) / kWaves);
-  hipLaunchKernelGGL((policy_kernel<kWaves>), dim3(wgs), dim3(64 * kWaves), 0, stream, p);
+  hipLaunchKernelGGL(policy_kernel, dim3(wgs), dim3(64 * kWaves), 0, stream, p);
   DK_CHECK_LAUNCH();
   const int64_t more = n_items > rows ? (rows + kSumThreads / 64 - 1) / (kSumThreads / 64) : 0;
   hipLaunchKernelGGL(policy_sum_kernel, dim3((unsigned)(1 + more)), dim3(kSumThreads), 0, stream, p, wgs);
@@ -421,41 +468,47 @@ extern "C" int dk_policy_loss(const int32_t* items, int64_t n_items, const int32
   return 0;
 }
 
+static int64_t pair_groups(int64_t pairs) { return (pairs + kPairs - 1) / kPairs; }
+
 extern "C" int64_t dk_preference_loss_workspace(int64_t n_items, int64_t pairs) {
-  return n_items <= 0 || pairs <= 0 ? 0 : (n_items + pairs) * (int64_t)sizeof(double);
+  if (n_items <= kOneItems && pairs <= kPairs) return 0;
+  return (n_items + pair_groups(pairs)) * (int64_t)sizeof(double);
 }
 
 extern "C" int dk_preference_loss(const int32_t* items, int64_t n_items, const int32_t* row_items,
-                                  const int64_t* lens, int64_t rows, int64_t n_tokens,
-                                  const int32_t* row_pairs, const int32_t* entries, int64_t n_pairs,
-                                  const dk_token_array* logp,
-                                  const dk_token_array* ref, double beta, int kind, double label_smoothing,
-                                  double margin, int average, float* dlogp, float* rewards,
-                                  float* margins, float* loss, void* ws, int64_t ws_bytes,
-                                  hipStream_t stream) {
+                                  int64_t rows, int64_t n_tokens, const int32_t* row_pairs,
+                                  const int32_t* entries, const int32_t* pairs, int64_t n_pairs,
+                                  const dk_token_array* logp, const dk_token_array* ref, double beta,
+                                  int kind, double label_smoothing, double margin, int average,
+                                  float* dlogp, float* rewards, float* margins, float* loss, void* ws,
+                                  int64_t ws_bytes, hipStream_t stream) {
   if (!rows_ok(n_items, rows) || n_pairs < 1 || n_pairs > (int64_t)1 << 28 || !items || !row_items ||
-      !lens || !row_pairs || !entries || !tokens_ok(logp, n_tokens) ||
-      (ref && !tokens_ok(ref, n_tokens)) || (n_tokens > 0 && !dlogp) || !rewards || !margins || !loss || !(beta > 0.0) || kind < 0 ||
-      kind > 2 || !(label_smoothing >= 0.0 && label_smoothing <= 0.5) || !(margin - margin == 0.0))
+      !row_pairs || !entries || !pairs || !tokens_ok(logp, n_tokens) || (ref && !tokens_ok(ref, n_tokens)) ||
+      (n_tokens > 0 && !dlogp) || !rewards || !margins || !loss || !(beta > 0.0) || !(1.0 / beta > 0.0) ||
+      kind < 0 || kind > 2 || !(label_smoothing >= 0.0 && label_smoothing <= 0.5) || !(margin - margin == 0.0))
     return DK_ERR_INVALID;
-  if (!dk_aligned(items, 16) || !dk_aligned(lens, 8) || !dk_aligned(entries, 8)) return DK_ERR_ALIGN;
-  if (!ws || ws_bytes < dk_preference_loss_workspace(n_items, n_pairs) || !dk_aligned(ws, 8))
-    return DK_ERR_WORKSPACE;
-  PrefParams p{reinterpret_cast<const int4*>(items), row_items, lens, row_pairs,
-               reinterpret_cast<const int2*>(entries), (int)n_items, (int)rows, (int)n_pairs,
-               tokens_of(logp), tokens_of(ref), beta, margin, label_smoothing, kind, average, dlogp, rewards,
-               margins, loss, (double*)ws};
-  if (n_items <= kOneWaves) {
+  if (!dk_aligned(items, 16) || !dk_aligned(row_items, 4) || !dk_aligned(row_pairs, 4) ||
+      !dk_aligned(entries, 8) || !dk_aligned(pairs, 8))
+    return DK_ERR_ALIGN;
+  const int64_t need = dk_preference_loss_workspace(n_items, n_pairs);
+  if (need && (!ws || ws_bytes < need || !dk_aligned(ws, 8))) return DK_ERR_WORKSPACE;
+  PrefParams p{reinterpret_cast<const int4*>(items), row_items, row_pairs,
+               reinterpret_cast<const int2*>(entries), reinterpret_cast<const int2*>(pairs), (int)n_items,
+               (int)rows, (int)n_pairs, tokens_of(logp), tokens_of(ref), beta, margin, label_smoothing, kind,
+               average, dlogp, rewards, margins, loss, (double*)ws};
+  if (need == 0) {
     hipLaunchKernelGGL(pref_one_kernel, dim3(1), dim3(64 * kOneWaves), 0, stream, p);
     DK_CHECK_LAUNCH();
     return 0;
   }
-  const int wgs = (int)((n_items + kWaves - 1) / kWaves);
+  const int wgs = (int)((n_items + kWaves - 1) / kWaves), pair_wgs = (int)pair_groups(n_pairs);
   hipLaunchKernelGGL(pref_sum_kernel, dim3(wgs), dim3(64 * kWaves), 0, stream, p);
   DK_CHECK_LAUNCH();
-  hipLaunchKernelGGL(pref_apply_kernel, dim3(wgs), dim3(64 * kWaves), 0, stream, p);
+  hipLaunchKernelGGL(pref_apply_kernel, dim3(pair_wgs + wgs), dim3(64 * kWaves), 0, stream, p, pair_wgs);
   DK_CHECK_LAUNCH();
-  hipLaunchKernelGGL(pref_loss_kernel, dim3(1), dim3(kSumThreads), 0, stream, p);
-  DK_CHECK_LAUNCH();
+  if (pair_wgs > 1) {
+    hipLaunchKernelGGL(pref_loss_kernel, dim3(1), dim3(kSumThreads), 0, stream, p, pair_wgs);
+    DK_CHECK_LAUNCH();
+  }
   return 0;
 }

@@ -16,9 +16,8 @@ from . import _lib
 
 _CODES = {torch.float32: _lib.DK_TYPE_F32, torch.float16: _lib.DK_TYPE_F16,
           torch.bfloat16: _lib.DK_TYPE_BF16}
-# a list's properties are read by maps over C functions: a step has hundreds of small gradients
-_dtype, _pointer, _numel = attrgetter("dtype"), torch.Tensor.data_ptr, torch.Tensor.numel
-_device, _contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
+# a step has hundreds of small gradients: each property is read in the way that takes the least host time
+_dtype, _device, _contiguous = attrgetter("dtype"), torch.Tensor.get_device, torch.Tensor.is_contiguous
 
 
 def _dense(t):
@@ -34,8 +33,7 @@ def _dense(t):
 
 def _check(tensors, what):
     """(the tensors' type codes, the device's index)"""
-    types = list(map(_dtype, tensors))
-    kinds = set(types)
+    kinds = set(map(_dtype, tensors))
     if not kinds <= _CODES.keys():
         raise ValueError(f"{what} must be fp32, fp16 or bf16 tensors")
     devices = set(map(_device, tensors))
@@ -43,7 +41,10 @@ def _check(tensors, what):
         raise ValueError(f"{what} must be on one GPU")
     if not all(map(_contiguous, tensors)) and not all(map(_dense, tensors)):
         raise ValueError(f"{what} must be dense")
-    codes = [_CODES[types[0]]] * len(types) if len(kinds) == 1 else [_CODES[t] for t in types]
+    if len(kinds) == 1:
+        codes = array("i", [_CODES[kinds.pop()]]) * len(tensors)
+    else:
+        codes = array("i", [_CODES[t.dtype] for t in tensors])
     return codes, devices.pop()
 
 
@@ -56,7 +57,8 @@ def _run(grads, max_norm, scale, out, in_place=False):
     types, index = _check(grads, "gradients")
     to = types
     # the host arrays live until the call returns
-    src, numel, dst = array("q", map(_pointer, grads)), array("q", map(_numel, grads)), None
+    src, dst = array("q", [g.data_ptr() for g in grads]), None
+    numel = array("q", [g.nelement() for g in grads])
     if out is not None:
         out = list(out)
         if len(out) != len(grads):
@@ -67,10 +69,9 @@ def _run(grads, max_norm, scale, out, in_place=False):
                                        (o.is_contiguous() and g.is_contiguous()))
                 for o, g in zip(out, grads)):
             raise ValueError("outputs must have their gradients' device, shapes and strides")
-        dst = array("q", map(_pointer, out))
+        dst = array("q", [o.data_ptr() for o in out])
     elif in_place:
         dst = src
-    codes = array("i", [a | b << 4 for a, b in zip(types, to)])
     dev = torch.device("cuda", index)
     lib = _lib.lib()
     nbytes = lib.dk_grad_clip_workspace(len(grads))
@@ -78,7 +79,7 @@ def _run(grads, max_norm, scale, out, in_place=False):
     norm = torch.empty((), dtype=torch.float32, device=dev)
     _lib.launch(dev, lib.dk_grad_clip, "dk_grad_clip", src.buffer_info()[0],
                 None if dst is None else dst.buffer_info()[0], numel.buffer_info()[0],
-                codes.buffer_info()[0], len(grads), max_norm, scale, norm.data_ptr(), ws.data_ptr(), nbytes)
+                types.buffer_info()[0], to.buffer_info()[0], len(grads), max_norm, scale, norm.data_ptr(), ws.data_ptr(), nbytes)
     return norm
 
 

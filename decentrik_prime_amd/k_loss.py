@@ -16,7 +16,6 @@ gradient for the log-probabilities; as the streamed head's gradient is that of t
 -dlogp are the factors of its rows (k_norm.rms_backward's row_scale; model.QwenQLoRAStep.policy_step).
 """
 
-import ctypes
 import math
 
 import numpy as np
@@ -31,8 +30,8 @@ KINDS = ("sigmoid", "hinge", "ipo")
 
 
 class RowMeta:
-    """The plan of rows of consecutive tokens (see row_meta): on the device the kernels' items, the rows'
-    lengths and items, and the pairs of each row."""
+    """The plan of rows of consecutive tokens (see row_meta): on the device the kernels' items, each row's
+    items, and the pairs with each row's share of them."""
 
     def __init__(self, lens, device, pairs=None):
         size = np.asarray([int(n) for n in lens], np.int64)
@@ -45,38 +44,37 @@ class RowMeta:
         count = np.maximum(1, -(-size // step))
         row_items = np.concatenate([[0], np.cumsum(count)])
         row = np.repeat(np.arange(size.size), count)
-        at = (np.arange(row.size) - row_items[row]) * step[row]       # first token within the row
+        place = np.arange(row.size) - row_items[row]
+        at = place * step[row]                                        # first token within the row
         begin = (np.cumsum(size) - size)[row] + at
-        items = np.empty((row.size, 4), np.int64)
+        items = np.zeros((row.size, 8), np.int64)
         items[:, 0], items[:, 1] = begin & 0xffffffff, begin >> 32
         items[:, 2], items[:, 3] = np.minimum(step[row], size[row] - at), row
+        items[:, 4], items[:, 5], items[:, 6] = size[row], count[row], place
         self.n_items = int(row.size)
-        parts = [items.astype(np.uint32).reshape(-1), size.view(np.uint32), row_items.astype(np.uint32)]
+        parts = {"items": items}
         self.n_pairs = None
         if pairs is not None:
             both = np.asarray([(int(a), int(b)) for a, b in pairs], np.int64).reshape(-1, 2)
             if both.size == 0 or both.min() < 0 or both.max() >= size.size or len(both) > 1 << 28:
                 raise ValueError(f"at least one pair of rows 0 .. {size.size - 1}")
             self.n_pairs = len(both)
-            index = np.arange(1, len(both) + 1)
             own = both.T.reshape(-1)                                  # chosen rows, then rejected ones
-            order = np.argsort(own, kind="stable")
-            entries = np.stack([both[:, ::-1].T.reshape(-1), np.concatenate([index, -index])], 1)[order]
-            row_pairs = np.concatenate([[0], np.cumsum(np.bincount(own, minlength=size.size))])
-            if sum(p.size for p in parts) % 2:
-                parts.append(np.zeros(1, np.uint32))
-            parts += [entries.astype(np.int32).view(np.uint32).reshape(-1), row_pairs.astype(np.uint32)]
-        starts = np.cumsum([0] + [p.size for p in parts])
-        self.device = torch.device(device)
-        self._buffer = torch.from_numpy(np.concatenate(parts).view(np.int32)).to(self.device)
+            other, chosen = both[:, ::-1].T.reshape(-1), np.repeat([1, 0], len(both))
+            parts["entries"] = np.stack([other, chosen], 1)[np.argsort(own, kind="stable")]
+            parts["pairs"] = both
+            parts["row_pairs"] = np.concatenate([[0], np.cumsum(np.bincount(own, minlength=size.size))])
+        parts["row_items"] = row_items
+        flat = [p.reshape(-1).astype(np.uint32) for p in parts.values()]
+        starts = np.cumsum([0] + [p.size for p in flat])
+        self._buffer = torch.from_numpy(np.concatenate(flat).view(np.int32)).to(torch.device(device))
         self.device = self._buffer.device
-        self._at = {name: 4 * int(starts[i]) for name, i in
-                    (("items", 0), ("lens", 1), ("row_items", 2)) + (
-                        (("entries", len(parts) - 2), ("row_pairs", len(parts) - 1)) if pairs is not None
-                        else ())}
-
-    def ptr(self, name):
-        return self._buffer.data_ptr() + self._at[name]
+        first = self._buffer.data_ptr()
+        self.at = {name: first + 4 * int(s) for name, s in zip(parts, starts)}   # addresses in the buffer
+        lib = _lib.lib()
+        self.policy_bytes = lib.dk_policy_loss_workspace(self.n_items)
+        self.preference_bytes = 0 if pairs is None else lib.dk_preference_loss_workspace(self.n_items,
+                                                                                         self.n_pairs)
 
 
 def row_meta(lens, device, pairs=None):
@@ -89,7 +87,7 @@ def _tokens(t, what, meta):
     """A token array's C description: [n] log-probabilities, or the head's stats."""
     if t is None:
         return None
-    if t.dtype != torch.float32 or not t.is_cuda or t.device != meta.device:
+    if t.dtype != torch.float32 or t.get_device() != meta.device.index:   # (a CPU tensor's is -1)
         raise ValueError(f"{what} must be a CUDA fp32 tensor on the plan's device ({meta.device})")
     if t.dim() == 1 and t.shape[0] == meta.n_tokens:
         return _lib.TokenArrayC(t.data_ptr(), t.stride(0), 0)
@@ -97,10 +95,6 @@ def _tokens(t, what, meta):
         return _lib.TokenArrayC(t.data_ptr(), t.stride(0), 1)
     raise ValueError(f"{what} must be [{meta.n_tokens}] log-probabilities, or the head's stats [N, 4] with "
                      f"these tokens first (got {tuple(t.shape)})")
-
-
-def _ref(c):
-    return None if c is None else ctypes.byref(c)
 
 
 def policy_loss(logp, old, advantages, meta, *, ref=None, kl_coef=0.0, clip_low=0.2, clip_high=None,
@@ -129,15 +123,13 @@ def policy_loss(logp, old, advantages, meta, *, ref=None, kl_coef=0.0, clip_low=
     dlogp = torch.empty(n, dtype=torch.float32, device=dev)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    lib = _lib.lib()
-    nbytes = lib.dk_policy_loss_workspace(meta.n_items)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    which = REDUCTIONS.index(reduction)
-    _lib.launch(dev, lib.dk_policy_loss, "dk_policy_loss", meta.ptr("items"), meta.n_items,
-                meta.ptr("row_items"), meta.ptr("lens"), rows, n, ctypes.byref(x), ctypes.byref(o), _ref(f),
-                advantages.data_ptr(), int(per_token), clip_low, clip_high, kl_coef, which,
-                float(max(1, (meta.n_filled, n, 1)[which])), dlogp.data_ptr(), stats.data_ptr(),
-                loss.data_ptr(), ws.data_ptr(), nbytes)
+    nbytes = meta.policy_bytes
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    which, at = REDUCTIONS.index(reduction), meta.at
+    _lib.launch(dev, _lib.lib().dk_policy_loss, "dk_policy_loss", at["items"], meta.n_items,
+                at["row_items"], rows, n, x, o, f, advantages.data_ptr(), per_token, clip_low, clip_high,
+                kl_coef, which, (meta.n_filled, n, 1)[which] or 1, dlogp.data_ptr(), stats.data_ptr(),
+                loss.data_ptr(), _lib.ptr(ws), nbytes)
     return loss, dlogp, stats
 
 
@@ -166,12 +158,10 @@ def preference_loss(logp, ref, meta, *, beta=0.1, kind="sigmoid", label_smoothin
     rewards = torch.empty(rows, dtype=torch.float32, device=dev)
     margins = torch.empty(meta.n_pairs, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    lib = _lib.lib()
-    nbytes = lib.dk_preference_loss_workspace(meta.n_items, meta.n_pairs)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _lib.launch(dev, lib.dk_preference_loss, "dk_preference_loss", meta.ptr("items"), meta.n_items,
-                meta.ptr("row_items"), meta.ptr("lens"), rows, n, meta.ptr("row_pairs"),
-                meta.ptr("entries"), meta.n_pairs, ctypes.byref(x), _ref(f), beta, KINDS.index(kind),
-                label_smoothing, margin, int(average), dlogp.data_ptr(), rewards.data_ptr(),
-                margins.data_ptr(), loss.data_ptr(), ws.data_ptr(), nbytes)
+    nbytes, at = meta.preference_bytes, meta.at
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _lib.launch(dev, _lib.lib().dk_preference_loss, "dk_preference_loss", at["items"], meta.n_items,
+                at["row_items"], rows, n, at["row_pairs"], at["entries"], at["pairs"], meta.n_pairs, x, f,
+                beta, KINDS.index(kind), label_smoothing, margin, average, dlogp.data_ptr(),
+                rewards.data_ptr(), margins.data_ptr(), loss.data_ptr(), _lib.ptr(ws), nbytes)
     return loss, dlogp, rewards, margins

@@ -250,12 +250,12 @@ int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* r
 
 /* ------------------------------------------------------------------------------------------
  * Losses over the tokens' log-probabilities of a packed batch of answers, with their gradients (no
- * counterpart in the reference).  The batch is `rows` rows of consecutive tokens, lens int64 [rows], cut
- * into items {first token (low, high word), tokens, row} (int32 [n_items, 4], 16-byte aligned, row by row
- * and in token order; a row has 1 to 64 items, an empty row one without tokens); row r's items are
- * row_items[r] .. row_items[r + 1] - 1.  A token array is fp32 with an element stride (0 allowed), negated
- * where it holds losses (the head's stats: column 0, stride 4).  With n_tokens = 0 the token arrays may be
- * NULL.
+ * counterpart in the reference).  The batch is `rows` rows of consecutive tokens cut into items {first token
+ * (low, high word), tokens, row, the row's tokens, the row's items, the item's place among them, 0} (int32
+ * [n_items, 8], 16-byte aligned, row by row and in token order; a row has 1 to 64 items and at most 2^30
+ * tokens, an empty row one item without tokens); row r's items are row_items[r] .. row_items[r + 1] - 1.  A
+ * token array is fp32 with an element stride (0 allowed), negated where it holds losses (the head's stats:
+ * column 0, stride 4).  With n_tokens = 0 the token arrays may be NULL.
  *
  * dk_policy_loss: A the advantage of the token (per_token) or of its row, r = e^(logp - old),
  *   p = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), k = e^(ref - logp) - (ref - logp) - 1 (ref NULL: 0)
@@ -265,33 +265,33 @@ int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* r
  * dk_preference_loss: S = a row's sum of logp - ref (average: mean; 0 without tokens), h = beta (S_chosen -
  *   S_rejected) - margin, loss = mean over pairs of  kind 0: -(1 - e) log s(h) - e log s(-h), s the logistic
  *   function, e = label_smoothing in [0, 1/2];  1: max(0, 1 - h);  2: ((h - 1/2) / beta)^2.  rewards [rows] = beta S,
- *   margins [n_pairs] = h.  Row r's pairs are entries row_pairs[r] .. row_pairs[r + 1] - 1, int32 {other row,
- *   pair + 1 where r is the chosen one, -(pair + 1) where it is the rejected one}.
- * workspace: the query's bytes, 8-byte aligned. */
+ *   margins [n_pairs] = h.  pairs int32 {chosen, rejected}; row r's are entries row_pairs[r] ..
+ *   row_pairs[r + 1] - 1, int32 {other row, 1 where r is the chosen one, else 0}.
+ * workspace: the query's bytes, 8-byte aligned (NULL where that is 0). */
 typedef struct dk_token_array {
   const float* data;
   int64_t stride;
   int32_t negated;
 } dk_token_array;
 int64_t dk_policy_loss_workspace(int64_t n_items);
-int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items, const int64_t* lens,
-                   int64_t rows, int64_t n_tokens, const dk_token_array* logp, const dk_token_array* old,
+int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items, int64_t rows,
+                   int64_t n_tokens, const dk_token_array* logp, const dk_token_array* old,
                    const dk_token_array* ref, const float* advantages, int per_token, double clip_low,
                    double clip_high, double kl_coef, int reduction, double denominator, float* dlogp,
                    float* stats, float* loss, void* workspace, int64_t workspace_bytes,
                    hipStream_t stream);
 int64_t dk_preference_loss_workspace(int64_t n_items, int64_t n_pairs);
 int dk_preference_loss(const int32_t* items, int64_t n_items, const int32_t* row_items,
-                       const int64_t* lens, int64_t rows, int64_t n_tokens, const int32_t* row_pairs,
-                       const int32_t* entries, int64_t n_pairs, const dk_token_array* logp,
+                       int64_t rows, int64_t n_tokens, const int32_t* row_pairs,
+                       const int32_t* entries, const int32_t* pairs, int64_t n_pairs, const dk_token_array* logp,
                        const dk_token_array* ref, double beta, int kind, double label_smoothing,
                        double margin, int average, float* dlogp, float* rewards, float* margins,
                        float* loss, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /* The global norm of n gradient tensors, norm = scale sqrt(sum g^2) (fp32, on the device), and, with dst
  * not NULL, dst = scale min(1, max_norm / (norm + 1e-6)) src element by element (no counterpart in the
- * reference).  src, dst, numel and types are host arrays, read before the call returns; types[i] = source
- * type | destination type << 4 (DK_TYPE_*).  dst[i] may be src[i] (of one type; nothing is written where the
+ * reference).  src, dst, numel, types and dst_types (DK_TYPE_*) are host arrays, read before the call
+ * returns.  dst[i] may be src[i] (of one type; nothing is written where the
  * factor is 1); beyond that nothing written may overlap anything else in the lists (DK_ERR_INVALID).
  * max_norm > 0 (infinity: scale alone).  An infinite norm scales by 0, a NaN one gives NaN throughout.  workspace:
  * dk_grad_clip_workspace(n) bytes, 8-byte aligned. */
@@ -300,8 +300,8 @@ int dk_preference_loss(const int32_t* items, int64_t n_items, const int32_t* row
 #define DK_TYPE_BF16 3
 int64_t dk_grad_clip_workspace(int64_t n);
 int dk_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* types,
-                 int64_t n, double max_norm, double scale, float* norm, void* workspace,
-                 int64_t workspace_bytes, hipStream_t stream);
+                 const int32_t* dst_types, int64_t n, double max_norm, double scale, float* norm,
+                 void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * LoRA down projection with the dropout of its input.  Replaces the norm kernel's dropout lines

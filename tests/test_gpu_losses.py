@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 U = 2.0 ** -24          # half a step of fp32
 
 LENS = {"one": [1], "short": [3, 0, 70, 1, 64], "sixteen": [100] * 15 + [600], "many": [7 + 13 * i for i in range(90)],
-        "long": [5, 40000, 0, 513, 1024], "empty": [0, 0, 0]}
+        "long": [5, 40000, 0, 513, 1024], "empty": [0, 0, 0], "crowd": [1 + i % 7 for i in range(200)],
+        "sixty-four": [9] * 63 + [500], "sixty-five": [9] * 65}
 
 
 def draw(lens, seed=0, spread=0.3):
@@ -190,7 +191,8 @@ def pref_formula(s, pairs, beta, kind, smooth, margin):
 
 PAIRS = {"one": [(0, 0)], "short": [(0, 2), (2, 1), (4, 2), (0, 2)], "sixteen": [(i, 15 - i) for i in range(16)],
          "many": [(i, j) for i in range(0, 90, 3) for j in range(0, 90, 7)], "long": [(1, 0), (1, 3), (4, 1), (2, 1)],
-         "empty": [(0, 1), (2, 2)]}
+         "empty": [(0, 1), (2, 2)], "crowd": [(i, (i + 1 + 7 * k) % 200) for i in range(200) for k in range(13)],
+         "sixty-four": [(i, j) for i in range(33) for j in range(31)], "sixty-five": [(64, 0), (0, 64), (63, 1)]}
 
 
 @pytest.mark.parametrize("lens", list(LENS))

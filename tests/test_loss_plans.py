@@ -11,27 +11,26 @@ from decentrik_prime_amd import _lib, k_grad, k_head, k_loss
 
 
 def read_plan(meta):
-    """(items [n, 4], row_items, lens, entries, row_pairs) as the kernels read them."""
-    raw = meta._buffer.numpy()
+    """(items [n, 8], row_items, entries, pairs, row_pairs) as the kernels read them."""
+    raw, first = meta._buffer.numpy(), meta._buffer.data_ptr()
 
     def part(name, n):
-        at = meta._at[name] // 4
+        at = (meta.at[name] - first) // 4
         return raw[at:at + n]
-    items = part("items", 4 * meta.n_items).reshape(-1, 4)
+    items = part("items", 8 * meta.n_items).reshape(-1, 8)
     row_items = part("row_items", meta.n_rows + 1)
-    lens = part("lens", 2 * meta.n_rows).view(np.int64)
     if meta.n_pairs is None:
-        return items, row_items, lens, None, None
-    return (items, row_items, lens, part("entries", 4 * meta.n_pairs).reshape(-1, 2),
-            part("row_pairs", meta.n_rows + 1))
+        return items, row_items, None, None, None
+    return (items, row_items, part("entries", 4 * meta.n_pairs).reshape(-1, 2),
+            part("pairs", 2 * meta.n_pairs).reshape(-1, 2), part("row_pairs", meta.n_rows + 1))
 
 
 @pytest.mark.parametrize("lens", [[0], [1], [0, 0, 5, 0], [511, 512, 513, 1, 0, 1025], [32768, 32769, 100000],
                                   list(range(70)), [1 << 30] * 5 + [3]])
 def test_items_cover_every_token_once(lens):
     meta = k_loss.row_meta(lens, "cpu")
-    items, row_items, sizes, _, _ = read_plan(meta)
-    assert sizes.tolist() == lens and meta.n_tokens == sum(lens)
+    items, row_items = read_plan(meta)[:2]
+    assert meta.lens == lens and meta.n_tokens == sum(lens)
     assert meta.n_filled == sum(n > 0 for n in lens)
     assert row_items[0] == 0 and row_items[-1] == meta.n_items == len(items)
     start = 0
@@ -39,23 +38,25 @@ def test_items_cover_every_token_once(lens):
         mine = items[row_items[r]:row_items[r + 1]]
         assert 1 <= len(mine) <= k_loss.ROW_ITEMS
         at = start
-        for lo, hi, count, row in mine.tolist():
-            assert row == r and (hi << 32) + (lo & 0xffffffff) == at
+        for place, (lo, hi, count, row, size, of, which, _) in enumerate(mine.tolist()):
+            assert (row, size, of, which) == (r, n, len(mine), place)
+            assert (hi << 32) + (lo & 0xffffffff) == at
             assert count > 0 or n == 0
             at += count
         start += n
         assert at == start
-    assert all(meta.ptr(k) % 16 == 0 for k in ("items",)) and meta.ptr("lens") % 8 == 0
+    assert meta.at["items"] % 16 == 0
 
 
 @pytest.mark.parametrize("lens, pairs", [([3, 4], [(0, 1)]), ([3, 4, 0], [(0, 1), (2, 1), (1, 0), (0, 1)]),
                                          ([1] * 9, [(i, j) for i in range(9) for j in range(9)])])
 def test_every_row_names_its_pairs(lens, pairs):
     meta = k_loss.row_meta(lens, "cpu", pairs=pairs)
-    _, _, _, entries, row_pairs = read_plan(meta)
-    assert meta.ptr("entries") % 8 == 0
-    want = {r: sorted([(b, i + 1) for i, (a, b) in enumerate(pairs) if a == r] +
-                      [(a, -i - 1) for i, (a, b) in enumerate(pairs) if b == r]) for r in range(len(lens))}
+    _, _, entries, kept, row_pairs = read_plan(meta)
+    assert meta.at["entries"] % 8 == 0 and meta.at["pairs"] % 8 == 0
+    assert list(map(tuple, kept.tolist())) == pairs
+    want = {r: sorted([(b, 1) for a, b in pairs if a == r] + [(a, 0) for a, b in pairs if b == r])
+            for r in range(len(lens))}
     for r in range(len(lens)):
         assert sorted(map(tuple, entries[row_pairs[r]:row_pairs[r + 1]].tolist())) == want[r]
 
@@ -116,9 +117,9 @@ def test_loss_entries_refuse_bad_arguments():
     good = _lib.TokenArrayC(4096, 1, 0)
     ref = ctypes.byref
 
-    def policy(items=p, n_items=2, rows=2, n=5, x=good, old=good, f=good, adv=p, low=0.2, high=0.2, kl=0.1,
+    def policy(items=p, n_items=100, rows=2, n=5, x=good, old=good, f=good, adv=p, low=0.2, high=0.2, kl=0.1,
                red=0, den=2.0, out=p, ws=p, nbytes=1 << 12):
-        return lib.dk_policy_loss(items, n_items, p, p, rows, n, ref(x), ref(old), f and ref(f), adv, 0, low,
+        return lib.dk_policy_loss(items, n_items, p, rows, n, ref(x), ref(old), f and ref(f), adv, 0, low,
                                   high, kl, red, den, out, out, out, ws, nbytes, None)
     null, back = _lib.TokenArrayC(None, 1, 0), _lib.TokenArrayC(4096, -1, 0)
     for bad in (dict(items=None), dict(n_items=0), dict(n_items=1), dict(rows=0), dict(n=-1), dict(x=null),
@@ -127,20 +128,22 @@ def test_loss_entries_refuse_bad_arguments():
                 dict(red=-1), dict(den=0.0), dict(out=None)):
         assert policy(**bad) == _lib.DK_ERR_INVALID, bad
     assert policy(items=ctypes.c_void_p(4100)) == _lib.DK_ERR_ALIGN
-    need = lib.dk_policy_loss_workspace(2)
+    assert lib.dk_policy_loss_workspace(64) == 0        # one workgroup
+    need = lib.dk_policy_loss_workspace(100)
     for bad in (dict(ws=None), dict(nbytes=need - 1), dict(ws=ctypes.c_void_p(4100))):
         assert policy(**bad) == _lib.DK_ERR_WORKSPACE, bad
 
-    def preference(pairs=1, entries=p, x=good, f=good, beta=0.1, kind=0, smooth=0.0, margin=0.0, out=p, ws=p,
+    def preference(pairs=5000, entries=p, x=good, f=good, beta=0.1, kind=0, smooth=0.0, margin=0.0, out=p, ws=p,
                    nbytes=1 << 12):
-        return lib.dk_preference_loss(p, 2, p, p, 2, 5, p, entries, pairs, ref(x), f and ref(f), beta, kind,
+        return lib.dk_preference_loss(p, 2, p, 2, 5, p, entries, p, pairs, ref(x), f and ref(f), beta, kind,
                                       smooth, margin, 0, out, out, out, out, ws, nbytes, None)
     for bad in (dict(pairs=0), dict(entries=None), dict(x=null), dict(f=back), dict(beta=0.0),
                 dict(beta=float("nan")), dict(kind=3), dict(smooth=0.51), dict(margin=float("nan")),
                 dict(out=None)):
         assert preference(**bad) == _lib.DK_ERR_INVALID, bad
     assert preference(entries=ctypes.c_void_p(4100)) == _lib.DK_ERR_ALIGN
-    for bad in (dict(ws=None), dict(nbytes=lib.dk_preference_loss_workspace(2, 1) - 1)):
+    assert lib.dk_preference_loss_workspace(64, 1024) == 0
+    for bad in (dict(ws=None), dict(nbytes=lib.dk_preference_loss_workspace(2, 5000) - 1)):
         assert preference(**bad) == _lib.DK_ERR_WORKSPACE, bad
 
 
@@ -158,14 +161,15 @@ def test_clipping_refuses_bad_arguments():
     def call(src, dst, numel, types, max_norm=1.0, scale=1.0, norm=64, ws=4096, nbytes=1 << 16):
         n = len(src)
         arrays = [(ctypes.c_int64 * n)(*src), (ctypes.c_int64 * n)(*dst) if dst else None,
-                  (ctypes.c_int64 * n)(*numel), (ctypes.c_int32 * n)(*types)]
+                  (ctypes.c_int64 * n)(*numel), (ctypes.c_int32 * n)(*[t & 15 for t in types]),
+                  (ctypes.c_int32 * n)(*[t >> 4 for t in types])]
         return lib.dk_grad_clip(*arrays, n, max_norm, scale, norm, ws, nbytes, None)
     f32, f16 = _lib.DK_TYPE_F32 * 17, _lib.DK_TYPE_F16 * 17
     up = _lib.DK_TYPE_F16 | _lib.DK_TYPE_F32 << 4
     a, b = 1 << 20, 1 << 21
     assert lib.dk_grad_clip_workspace(0) == 0
     for bad in (([], None, [], []), ([a], [a], [-1], [f32]), ([0], [a], [4], [f32]), ([a], [0], [4], [f32]),
-                ([a], [a], [4], [0]), ([a], [a], [4], [4]), ([a], [a], [4], [up]),      # in place, two types
+                ([a], [a], [4], [0]), ([a], [a], [4], [4 * 17]), ([a], [a], [4], [up]),      # in place, two types
                 ([a, a], [a, a], [4, 4], [f32, f32]),                                   # a tensor twice
                 ([a, a + 8], [a, a + 8], [4, 4], [f32, f32]),                           # overlapping ones
                 ([a, b], [b, b + 64], [4, 4], [f32, f32]),                              # an output over a source
