@@ -163,10 +163,10 @@ SIGNATURES = {
     "dk_head_logprobs_workspace": (_i64, [_i64, _i64, _i64]),
     "dk_head_logprobs": (_int, [_c_p, _i64, _i64, _c_p, _i64, _c_p, _i64, _i64, _c_p, _f32, _c_p, _c_p,
                                 _c_p, _c_p, _i64, _c_p]),
-    "dk_policy_loss_workspace": (_i64, [_i64]),
+    "dk_policy_loss_workspace": (_i64, [_i64, _i64]),
     "dk_policy_loss": (_int, [_c_p, _i64, _c_p, _i64, _i64, _K, _K, _K, _c_p, _int, _f64, _f64, _f64, _int,
                               _f64, _c_p, _c_p, _c_p, _c_p, _i64, _c_p]),
-    "dk_preference_loss_workspace": (_i64, [_i64, _i64]),
+    "dk_preference_loss_workspace": (_i64, [_i64, _i64, _i64]),
     "dk_preference_loss": (_int, [_c_p, _i64, _c_p, _i64, _i64, _c_p, _c_p, _c_p, _i64, _K, _K, _f64, _int,
                                   _f64, _f64, _int, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p]),
     "dk_grad_clip_workspace": (_i64, [_i64]),

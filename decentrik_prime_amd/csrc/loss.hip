@@ -22,6 +22,7 @@ namespace {
 constexpr int kWaves = 4;        // items of a workgroup
 constexpr int kOneWaves = 16;    // the single workgroup of a call with few items
 constexpr int kOneItems = 64;
+constexpr int64_t kOneTokens = 1 << 15;
 constexpr int kAhead = 8;        // tokens of a lane in flight
 constexpr int kPairs = 1024;     // pairs of a workgroup
 
@@ -95,6 +96,7 @@ __device__ __forceinline__ double policy_item(const PolicyParams& p, const Item&
   const double weight = p.reduction == 0 ? p.inv / (double)it.len : p.inv;   // a token's share of the loss
   const float w = (float)weight;
   const float* adv = p.adv_per_token ? p.adv + it.begin : p.adv + it.row;
+  int clipped = 0;
   for (int t0 = 0; t0 < it.count; t0 += 64 * kAhead) {
     float x[kAhead], o[kAhead], rf[kAhead], a[kAhead];
 #pragma unroll
@@ -125,10 +127,11 @@ __device__ __forceinline__ double policy_item(const PolicyParams& p, const Item&
       p.dlogp[it.begin + t] = g * w;
       s.v[0] -= (double)pol;
       s.v[1] += (double)k;
-      s.v[2] += up || down ? 1.0 : 0.0;
+      clipped += up || down;
       s.v[3] += (double)r;
     }
   }
+  s.v[2] = (double)clipped;
 #pragma unroll
   for (int q = 0; q < 4; ++q) s.v[q] = wave_sum(s.v[q]);
   return weight * (s.v[0] + (double)p.beta * s.v[1]);
@@ -257,7 +260,7 @@ struct PrefParams {
   const int4* items;
   const int32_t* row_items;    // [rows + 1]
   const int32_t* row_pairs;    // [rows + 1] a row's entries in `entries`
-  const int2* entries;         // (other row, 1: this row is chosen, 0: rejected)
+  const int2* entries;         // (other row, pair + 1: this row is chosen, -(pair + 1): rejected)
   const int2* pairs;           // (chosen, rejected)
   int n_items, rows, n_pairs;
   Tokens logp, ref;            // ref.p null: none
@@ -300,23 +303,14 @@ __device__ __forceinline__ double row_score(const PrefParams& p, const double* p
   return p.average && len > 0 ? s / (double)len : s;
 }
 
-// where the rows' S come from: the items' sums in memory, or the one workgroup's own table
-struct FromItems {
-  const PrefParams& p;
-  __device__ __forceinline__ double operator()(int row) const { return row_score(p, p.part, row); }
-};
-
-struct FromTable {
-  const double* s;
-  __device__ __forceinline__ double operator()(int row) const { return s[row]; }
-};
-
 // L(h) and L'(h)
 __device__ __forceinline__ double pref_loss(const PrefParams& p, double h, double* slope) {
   if (p.kind == 0) {
-    // -(1 - e) log s(h) - e log s(-h) = (1 - e) max(-h, 0) + e max(h, 0) + log(1 + e^-|h|)
-    const double tail = log1p(exp(-fabs(h)));
-    *slope = p.smoothing / (1.0 + exp(-h)) - (1.0 - p.smoothing) / (1.0 + exp(h));
+    // -(1 - e) log s(h) - e log s(-h) = (1 - e) max(-h, 0) + e max(h, 0) + log(1 + e^-|h|); its slope is
+    // e s(h) - (1 - e) s(-h), both from e^-|h|
+    const double u = exp(-fabs(h)), tail = log1p(u), near = 1.0 / (1.0 + u), far = u * near;
+    *slope = h < 0.0 ? p.smoothing * far - (1.0 - p.smoothing) * near
+                     : p.smoothing * near - (1.0 - p.smoothing) * far;
     return (1.0 - p.smoothing) * (fmax(-h, 0.0) + tail) + p.smoothing * (fmax(h, 0.0) + tail);
   }
   if (p.kind == 1) {
@@ -332,44 +326,20 @@ __device__ __forceinline__ double pref_h(const PrefParams& p, double chosen, dou
   return p.beta * (chosen - rejected) - p.margin;
 }
 
-// The item's gradient from the items' sums: the row's coefficient (its pairs by lane), then the tokens.
-// The row's first item also writes its reward.
-template <class Score>
-__device__ __forceinline__ void pref_apply(const PrefParams& p, const Score& score, const Item& it) {
+// a row's score in the rewards, and the coefficient of its tokens from the sum of its pairs' slopes
+__device__ __forceinline__ void pref_tokens(const PrefParams& p, const Item& it, double own, double slopes) {
   const int lane = threadIdx.x & 63;
-  const double own = score(it.row);
   if (it.at == 0 && lane == 0) p.rewards[it.row] = (float)(p.beta * own);
   if (it.count == 0) return;
-  double g = 0.0;
-  for (int e = p.row_pairs[it.row] + lane; e < p.row_pairs[it.row + 1]; e += 64) {
-    const int2 en = p.entries[e];
-    const double other = score(en.x);
-    double slope;
-    pref_loss(p, en.y ? pref_h(p, own, other) : pref_h(p, other, own), &slope);
-    g += en.y ? slope : -slope;
-  }
-  g = wave_sum(g) * p.beta / (double)p.n_pairs;
+  const double g = slopes * p.beta / (double)p.n_pairs;
   const float gf = (float)(p.average ? g / (double)it.len : g);
   for (int t = lane; t < it.count; t += 64) p.dlogp[it.begin + t] = gf;
 }
 
-// margins of pairs i, i + step, ... below end; the sum of their losses
-template <class Score>
-__device__ __forceinline__ double pref_pairs(const PrefParams& p, const Score& score, int i, int end, int step) {
-  double s = 0.0;
-  for (; i < end; i += step) {
-    const int2 pr = p.pairs[i];
-    const double h = pref_h(p, score(pr.x), score(pr.y));
-    double slope;
-    s += pref_loss(p, h, &slope);
-    p.margins[i] = (float)h;
-  }
-  return s;
-}
-
-// Up to kOneItems items and kPairs pairs: everything in one workgroup and launch.
+// Up to kOneItems items and kPairs pairs: everything in one workgroup and launch, the rows' scores and the
+// pairs' slopes in LDS.
 __global__ __launch_bounds__(64 * kOneWaves) void pref_one_kernel(PrefParams p) {
-  __shared__ double sums[kOneItems], scores[kOneItems];
+  __shared__ double sums[kOneItems], scores[kOneItems], slopes[kPairs];
   __shared__ double red[kOneWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int i = wave; i < p.n_items; i += kOneWaves) {
@@ -379,11 +349,25 @@ __global__ __launch_bounds__(64 * kOneWaves) void pref_one_kernel(PrefParams p) 
   __syncthreads();
   if (threadIdx.x < p.rows) scores[threadIdx.x] = row_score(p, sums, threadIdx.x);   // rows <= items
   __syncthreads();
-  const FromTable score{scores};
-  for (int i = wave; i < p.n_items; i += kOneWaves) pref_apply(p, score, item_of(p.items, i));
-  const double l = pref_pairs(p, score, threadIdx.x, p.n_pairs, 64 * kOneWaves);
-  const double total = block_sum<64 * kOneWaves>(l, red);
+  double l = 0.0;
+  static_assert(64 * kOneWaves == kPairs, "a thread per pair");
+  if (threadIdx.x < p.n_pairs) {
+    const int2 pr = p.pairs[threadIdx.x];
+    const double h = pref_h(p, scores[pr.x], scores[pr.y]);
+    l = pref_loss(p, h, &slopes[threadIdx.x]);
+    p.margins[threadIdx.x] = (float)h;
+  }
+  const double total = block_sum<64 * kOneWaves>(l, red);   // (its barrier publishes the slopes)
   if (threadIdx.x == 0) *p.loss = (float)(total / (double)p.n_pairs);
+  for (int i = wave; i < p.n_items; i += kOneWaves) {
+    const Item it = item_of(p.items, i);
+    double g = 0.0;
+    for (int e = p.row_pairs[it.row] + lane; e < p.row_pairs[it.row + 1]; e += 64) {
+      const int k = p.entries[e].y;
+      g += k > 0 ? slopes[k - 1] : -slopes[-k - 1];
+    }
+    pref_tokens(p, it, scores[it.row], wave_sum(g));
+  }
 }
 
 __global__ __launch_bounds__(64 * kWaves) void pref_sum_kernel(PrefParams p) {
@@ -393,13 +377,21 @@ __global__ __launch_bounds__(64 * kWaves) void pref_sum_kernel(PrefParams p) {
   if ((threadIdx.x & 63) == 0) p.part[i] = s;
 }
 
-// The first pair_wgs workgroups: kPairs pairs each (one alone: the loss too); the others: kWaves items.
+// The first pair_wgs workgroups: kPairs pairs each (one alone: the loss too); the others: kWaves items, the
+// slopes of a row's pairs by lane.
 __global__ __launch_bounds__(64 * kWaves) void pref_apply_kernel(PrefParams p, int pair_wgs) {
   __shared__ double red[kWaves];
   const int b = blockIdx.x;
   if (b < pair_wgs) {
-    const int first = b * kPairs, end = first + kPairs < p.n_pairs ? first + kPairs : p.n_pairs;
-    const double l = pref_pairs(p, FromItems{p}, first + threadIdx.x, end, 64 * kWaves);
+    const int end = (b + 1) * kPairs < p.n_pairs ? (b + 1) * kPairs : p.n_pairs;
+    double l = 0.0;
+    for (int i = b * kPairs + threadIdx.x; i < end; i += 64 * kWaves) {
+      const int2 pr = p.pairs[i];
+      const double h = pref_h(p, row_score(p, p.part, pr.x), row_score(p, p.part, pr.y));
+      double slope;
+      l += pref_loss(p, h, &slope);
+      p.margins[i] = (float)h;
+    }
     const double total = block_sum<64 * kWaves>(l, red);
     if (threadIdx.x == 0) {
       if (pair_wgs == 1) *p.loss = (float)(total / (double)p.n_pairs);
@@ -408,7 +400,18 @@ __global__ __launch_bounds__(64 * kWaves) void pref_apply_kernel(PrefParams p, i
     return;
   }
   const int i = (b - pair_wgs) * kWaves + (threadIdx.x >> 6);
-  if (i < p.n_items) pref_apply(p, FromItems{p}, item_of(p.items, i));
+  if (i >= p.n_items) return;
+  const Item it = item_of(p.items, i);
+  const double own = row_score(p, p.part, it.row);
+  double g = 0.0;
+  for (int e = p.row_pairs[it.row] + (threadIdx.x & 63); e < p.row_pairs[it.row + 1]; e += 64) {
+    const int2 en = p.entries[e];
+    const double other = row_score(p, p.part, en.x);
+    double slope;
+    pref_loss(p, en.y > 0 ? pref_h(p, own, other) : pref_h(p, other, own), &slope);
+    g += en.y > 0 ? slope : -slope;
+  }
+  pref_tokens(p, it, own, wave_sum(g));
 }
 
 __global__ __launch_bounds__(kSumThreads) void pref_loss_kernel(PrefParams p, int pair_wgs) {
@@ -431,8 +434,14 @@ bool rows_ok(int64_t n_items, int64_t rows) {
 
 }  // namespace
 
-extern "C" int64_t dk_policy_loss_workspace(int64_t n_items) {
-  return n_items <= kOneItems ? 0 : (4 * n_items + (n_items + kWaves - 1) / kWaves) * (int64_t)sizeof(double);
+// Few items and tokens take one workgroup and launch: 32 answers of 16,000 tokens in all 9 us where two
+// launches take 5 each and their gap; 64 items of long rows would keep its CU busy for far longer than those.
+static bool one_group(int64_t n_items, int64_t n_tokens) {
+  return n_items <= kOneItems && n_tokens <= kOneTokens;
+}
+
+extern "C" int64_t dk_policy_loss_workspace(int64_t n_items, int64_t n_tokens) {
+  return n_items <= 0 || one_group(n_items, n_tokens) ? 0 : (4 * n_items + (n_items + kWaves - 1) / kWaves) * (int64_t)sizeof(double);
 }
 
 extern "C" int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items, int64_t rows,
@@ -448,13 +457,13 @@ extern "C" int dk_policy_loss(const int32_t* items, int64_t n_items, const int32
       (kl_coef != 0.0 && !ref) || reduction < 0 || reduction > 2 || !(denominator > 0.0))
     return DK_ERR_INVALID;
   if (!dk_aligned(items, 16) || !dk_aligned(row_items, 4)) return DK_ERR_ALIGN;
-  const int64_t need = dk_policy_loss_workspace(n_items);
+  const int64_t need = dk_policy_loss_workspace(n_items, n_tokens);
   if (need && (!ws || ws_bytes < need || !dk_aligned(ws, 8))) return DK_ERR_WORKSPACE;
   PolicyParams p{reinterpret_cast<const int4*>(items), row_items, (int)n_items, (int)rows,
                  tokens_of(logp), tokens_of(old), tokens_of(ref), advantages, per_token,
                  log1p(-clip_low), log1p(clip_high), (float)(1.0 - clip_low), (float)(1.0 + clip_high),
                  (float)kl_coef, reduction, 1.0 / denominator, dlogp, stats, loss, (double*)ws};
-  if (n_items <= kOneItems) {
+  if (need == 0) {
     hipLaunchKernelGGL(policy_one_kernel, dim3(1), dim3(64 * kOneWaves), 0, stream, p);
     DK_CHECK_LAUNCH();
     return 0;
@@ -470,8 +479,8 @@ extern "C" int dk_policy_loss(const int32_t* items, int64_t n_items, const int32
 
 static int64_t pair_groups(int64_t pairs) { return (pairs + kPairs - 1) / kPairs; }
 
-extern "C" int64_t dk_preference_loss_workspace(int64_t n_items, int64_t pairs) {
-  if (n_items <= kOneItems && pairs <= kPairs) return 0;
+extern "C" int64_t dk_preference_loss_workspace(int64_t n_items, int64_t n_tokens, int64_t pairs) {
+  if (n_items <= 0 || (one_group(n_items, n_tokens) && pairs <= kPairs)) return 0;
   return (n_items + pair_groups(pairs)) * (int64_t)sizeof(double);
 }
 
@@ -490,7 +499,7 @@ extern "C" int dk_preference_loss(const int32_t* items, int64_t n_items, const i
   if (!dk_aligned(items, 16) || !dk_aligned(row_items, 4) || !dk_aligned(row_pairs, 4) ||
       !dk_aligned(entries, 8) || !dk_aligned(pairs, 8))
     return DK_ERR_ALIGN;
-  const int64_t need = dk_preference_loss_workspace(n_items, n_pairs);
+  const int64_t need = dk_preference_loss_workspace(n_items, n_tokens, n_pairs);
   if (need && (!ws || ws_bytes < need || !dk_aligned(ws, 8))) return DK_ERR_WORKSPACE;
   PrefParams p{reinterpret_cast<const int4*>(items), row_items, row_pairs,
                reinterpret_cast<const int2*>(entries), reinterpret_cast<const int2*>(pairs), (int)n_items,

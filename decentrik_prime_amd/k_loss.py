@@ -60,8 +60,9 @@ class RowMeta:
                 raise ValueError(f"at least one pair of rows 0 .. {size.size - 1}")
             self.n_pairs = len(both)
             own = both.T.reshape(-1)                                  # chosen rows, then rejected ones
-            other, chosen = both[:, ::-1].T.reshape(-1), np.repeat([1, 0], len(both))
-            parts["entries"] = np.stack([other, chosen], 1)[np.argsort(own, kind="stable")]
+            other, index = both[:, ::-1].T.reshape(-1), np.arange(1, len(both) + 1)
+            entries = np.stack([other, np.concatenate([index, -index])], 1)
+            parts["entries"] = entries[np.argsort(own, kind="stable")]
             parts["pairs"] = both
             parts["row_pairs"] = np.concatenate([[0], np.cumsum(np.bincount(own, minlength=size.size))])
         parts["row_items"] = row_items
@@ -72,9 +73,9 @@ class RowMeta:
         first = self._buffer.data_ptr()
         self.at = {name: first + 4 * int(s) for name, s in zip(parts, starts)}   # addresses in the buffer
         lib = _lib.lib()
-        self.policy_bytes = lib.dk_policy_loss_workspace(self.n_items)
-        self.preference_bytes = 0 if pairs is None else lib.dk_preference_loss_workspace(self.n_items,
-                                                                                         self.n_pairs)
+        self.policy_bytes = lib.dk_policy_loss_workspace(self.n_items, self.n_tokens)
+        self.preference_bytes = lib.dk_preference_loss_workspace(self.n_items, self.n_tokens,
+                                                                 self.n_pairs or 0)
 
 
 def row_meta(lens, device, pairs=None):

@@ -266,21 +266,21 @@ int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* r
  *   S_rejected) - margin, loss = mean over pairs of  kind 0: -(1 - e) log s(h) - e log s(-h), s the logistic
  *   function, e = label_smoothing in [0, 1/2];  1: max(0, 1 - h);  2: ((h - 1/2) / beta)^2.  rewards [rows] = beta S,
  *   margins [n_pairs] = h.  pairs int32 {chosen, rejected}; row r's are entries row_pairs[r] ..
- *   row_pairs[r + 1] - 1, int32 {other row, 1 where r is the chosen one, else 0}.
+ *   row_pairs[r + 1] - 1, int32 {other row, pair + 1 where r is the chosen one, else -(pair + 1)}.
  * workspace: the query's bytes, 8-byte aligned (NULL where that is 0). */
 typedef struct dk_token_array {
   const float* data;
   int64_t stride;
   int32_t negated;
 } dk_token_array;
-int64_t dk_policy_loss_workspace(int64_t n_items);
+int64_t dk_policy_loss_workspace(int64_t n_items, int64_t n_tokens);
 int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items, int64_t rows,
                    int64_t n_tokens, const dk_token_array* logp, const dk_token_array* old,
                    const dk_token_array* ref, const float* advantages, int per_token, double clip_low,
                    double clip_high, double kl_coef, int reduction, double denominator, float* dlogp,
                    float* stats, float* loss, void* workspace, int64_t workspace_bytes,
                    hipStream_t stream);
-int64_t dk_preference_loss_workspace(int64_t n_items, int64_t n_pairs);
+int64_t dk_preference_loss_workspace(int64_t n_items, int64_t n_tokens, int64_t n_pairs);
 int dk_preference_loss(const int32_t* items, int64_t n_items, const int32_t* row_items,
                        int64_t rows, int64_t n_tokens, const int32_t* row_pairs,
                        const int32_t* entries, const int32_t* pairs, int64_t n_pairs, const dk_token_array* logp,

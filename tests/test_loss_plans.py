@@ -55,8 +55,8 @@ def test_every_row_names_its_pairs(lens, pairs):
     _, _, entries, kept, row_pairs = read_plan(meta)
     assert meta.at["entries"] % 8 == 0 and meta.at["pairs"] % 8 == 0
     assert list(map(tuple, kept.tolist())) == pairs
-    want = {r: sorted([(b, 1) for a, b in pairs if a == r] + [(a, 0) for a, b in pairs if b == r])
-            for r in range(len(lens))}
+    want = {r: sorted([(b, i + 1) for i, (a, b) in enumerate(pairs) if a == r] +
+                      [(a, -i - 1) for i, (a, b) in enumerate(pairs) if b == r]) for r in range(len(lens))}
     for r in range(len(lens)):
         assert sorted(map(tuple, entries[row_pairs[r]:row_pairs[r + 1]].tolist())) == want[r]
 
@@ -128,8 +128,9 @@ def test_loss_entries_refuse_bad_arguments():
                 dict(red=-1), dict(den=0.0), dict(out=None)):
         assert policy(**bad) == _lib.DK_ERR_INVALID, bad
     assert policy(items=ctypes.c_void_p(4100)) == _lib.DK_ERR_ALIGN
-    assert lib.dk_policy_loss_workspace(64) == 0        # one workgroup
-    need = lib.dk_policy_loss_workspace(100)
+    assert lib.dk_policy_loss_workspace(64, 1 << 15) == 0        # one workgroup
+    need = lib.dk_policy_loss_workspace(100, 5)
+    assert need == lib.dk_policy_loss_workspace(100, 1 << 20) > 0
     for bad in (dict(ws=None), dict(nbytes=need - 1), dict(ws=ctypes.c_void_p(4100))):
         assert policy(**bad) == _lib.DK_ERR_WORKSPACE, bad
 
@@ -142,8 +143,8 @@ def test_loss_entries_refuse_bad_arguments():
                 dict(out=None)):
         assert preference(**bad) == _lib.DK_ERR_INVALID, bad
     assert preference(entries=ctypes.c_void_p(4100)) == _lib.DK_ERR_ALIGN
-    assert lib.dk_preference_loss_workspace(64, 1024) == 0
-    for bad in (dict(ws=None), dict(nbytes=lib.dk_preference_loss_workspace(2, 5000) - 1)):
+    assert lib.dk_preference_loss_workspace(64, 1 << 15, 1024) == 0
+    for bad in (dict(ws=None), dict(nbytes=lib.dk_preference_loss_workspace(2, 5, 5000) - 1)):
         assert preference(**bad) == _lib.DK_ERR_WORKSPACE, bad
 
 
