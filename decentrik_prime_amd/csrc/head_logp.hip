@@ -392,36 +392,67 @@ __global__ __launch_bounds__(256) void head_logp_join_kernel(LpParams p, float* 
 
 constexpr int kLpSlots = 256;   // workgroups at once, one per CU
 
-// Up to 128 tokens reading E bounds the call: one tile, small pieces of E in deep stages, a run for every CU.
-// More tokens: tiles of 256 by pieces of 256, as many runs as make the rounds of workgroups times the pieces
-// of a run fewest (among equals, the fewest).  Up to 128 tokens behind at most 16 whole tiles are a tile of
-// 128 in the same launch, whose pieces take kTailCost of a whole tile's.
-constexpr float kTailCost = 0.62f;
+// Estimated microseconds of a plan: fixed, and for every round of workgroups its pieces of E, each of D / 64
+// steps (step + load * busy; busy: the share of the CUs that the round fills) and a fold; never below reading
+// E once.  The constants are fits to 40 to 1600 tokens over vocabularies of 1000 to 64000 and D of 256 and
+// 1536 on MI355X (graph replays).  The small tiles take the small calls (100 tokens, 4000 x 1536: 20 us
+// against 41 on 256 x 256), the large ones from a few hundred tokens and some 10^4 entries on (1600 tokens of
+// 64000 x 1536: 310 against 377 on 128 x 256, 408 on 128 x 128).
+struct LpCost {
+  int bm, bn;
+  float fixed, step, load, fold;
+};
+constexpr LpCost kLpCost[] = {{64, 128, 7.4f, 0.475f, 0.035f, 0.3f},
+                              {128, 128, 7.5f, 0.52f, 0.115f, 0.5f},
+                              {128, 256, 8.3f, 0.85f, 0.25f, 0.9f},
+                              {256, 256, 10.5f, 1.2f, 0.57f, 1.8f}};
+constexpr float kReadUs = 5.4e6f;   // bytes of E a microsecond
 
-LpPlan lp_plan(int64_t n, int64_t V) {
-  if (n <= 128) {
-    const int64_t pieces = (V + 127) / 128;
-    return {n <= 64 ? 64 : 128, 128, 1, (int)(pieces < kLpSlots ? pieces : kLpSlots), 0, (int)pieces};
-  }
-  const int64_t pieces = (V + 255) / 256, rest = n % 256;
-  LpPlan best{256, 256, (int)((n + 255) / 256), 1, 0, (int)pieces};
-  float cost = -1.0f;
-  for (int g = 1; g <= kLpSlots && g <= pieces; ++g) {
-    const float c = (float)((((int64_t)best.tiles * g + kLpSlots - 1) / kLpSlots) * ((pieces + g - 1) / g));
-    if (cost < 0.0f || c < cost) {
-      cost = c;
-      best.runs = g;
+float lp_pieces_us(const LpCost& c, int64_t pieces, int64_t workgroups, float steps) {
+  const float busy = workgroups < kLpSlots ? (float)workgroups / kLpSlots : 1.0f;
+  return (float)pieces * (steps * (c.step + c.load * busy) + c.fold);
+}
+
+// The plan of least estimated time: tiles of one shape over as many runs of E as give one to four rounds of
+// workgroups; for 256 x 256 also whole tiles with up to 128 tokens behind them as a tile of 128 x 256 in the
+// same launch (853 tokens of 151936 x 1536 423 -> 409 us, 300 246 -> 218).
+LpPlan lp_plan(int64_t n, int64_t V, int64_t D) {
+  const float steps = (float)(D / kLpBK), read = (float)(2 * V * D) / kReadUs;
+  LpPlan best{};
+  float best_us = -1.0f, best_work = 0.0f;
+  auto consider = [&](float work, const LpPlan& pl, float fixed) {
+    const float us = fixed + (work > read ? work : read);
+    if (best_us < 0.0f || us < best_us || (us == best_us && work < best_work)) {
+      best_us = us;
+      best_work = work;
+      best = pl;
+    }
+  };
+  for (const LpCost& c : kLpCost) {
+    const int64_t tiles = (n + c.bm - 1) / c.bm, pieces = (V + c.bn - 1) / c.bn;
+    for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+      int64_t g = rounds * kLpSlots / tiles;
+      g = g < 1 ? 1 : g < pieces ? g : pieces;
+      const int64_t each = (pieces + g - 1) / g;
+      g = (pieces + each - 1) / each;            // the fewest runs of that many pieces
+      const int64_t all = (tiles * g + kLpSlots - 1) / kLpSlots;
+      consider(lp_pieces_us(c, all * each, tiles * g, steps),
+               LpPlan{c.bm, c.bn, (int)tiles, (int)g, 0, (int)pieces}, c.fixed);
     }
   }
-  const int whole = (int)(n / 256);
-  if (rest == 0 || rest > 128 || whole < 1 || whole > 16) return best;
-  for (int g = 1; g <= pieces && whole * g < kLpSlots; ++g) {
-    const int64_t left = kLpSlots - whole * g, tail = left < pieces ? left : pieces;
-    const float a = (float)((pieces + g - 1) / g), b = kTailCost * (float)((pieces + tail - 1) / tail);
-    const float c = a > b ? a : b;
-    if (c < cost) {
-      cost = c;
-      best = {256, 256, whole, g, (int)tail, (int)pieces};
+  const LpCost &big = kLpCost[3], &small = kLpCost[2];
+  const int64_t whole = n / 256, rest = n % 256, pieces = (V + 255) / 256;
+  if (rest >= 1 && rest <= 128 && whole >= 1 && whole < kLpSlots) {
+    const int64_t most = (kLpSlots - 1) / whole, least = (pieces + most - 1) / most;
+    for (int64_t each = least; each < least + 4; ++each) {
+      const int64_t g = (pieces + each - 1) / each;
+      int64_t left = kLpSlots - whole * g;
+      if (left > pieces) left = pieces;
+      const int64_t behind = (pieces + left - 1) / left;
+      const float a = lp_pieces_us(big, each, kLpSlots, steps), b = lp_pieces_us(small, behind, kLpSlots, steps);
+      consider(a > b ? a : b,
+               LpPlan{256, 256, (int)whole, (int)g, (int)((pieces + behind - 1) / behind), (int)pieces},
+               big.fixed);
     }
   }
   return best;
@@ -446,7 +477,7 @@ using namespace dk;
 
 extern "C" int64_t dk_head_logprobs_workspace(int64_t n, int64_t vocab, int64_t d) {
   if (n <= 0 || !lp_sizes_ok(n, vocab, d)) return 0;
-  return 16 * lp_states(lp_plan(n, vocab), n) + 4 * n;
+  return 16 * lp_states(lp_plan(n, vocab, d), n) + 4 * n;
 }
 
 extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* rows, int64_t n,
@@ -467,14 +498,16 @@ extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const
     return DK_ERR_ALIGN;
   if (!ws || ws_bytes < dk_head_logprobs_workspace(n, vocab, d) || !dk_aligned(ws, 16))
     return DK_ERR_WORKSPACE;
-  const LpPlan pl = lp_plan(n, vocab);
+  const LpPlan pl = lp_plan(n, vocab, d);
   LpParams p{(const f16*)y, ldy, rows, total, (const f16*)emb, tgt, n, vocab, d, scale * kLog2e, pl,
              (float*)ws, (float*)ws + 4 * lp_states(pl, n)};
   const dim3 grid((unsigned)(pl.tiles * pl.runs + pl.tail)), block(kLpThreads);
   if (pl.bm == 64)
     hipLaunchKernelGGL((head_logp_kernel<64, 128, 2, 6, false>), grid, block, 0, stream, p);
-  else if (pl.bm == 128)
+  else if (pl.bm == 128 && pl.bn == 128)
     hipLaunchKernelGGL((head_logp_kernel<128, 128, 4, 4, false>), grid, block, 0, stream, p);
+  else if (pl.bm == 128)
+    hipLaunchKernelGGL((head_logp_kernel<128, 256, 2, 3, false>), grid, block, 0, stream, p);
   else if (pl.tail == 0)
     hipLaunchKernelGGL((head_logp_kernel<256, 256, 2, 2, false>), grid, block, 0, stream, p);
   else
