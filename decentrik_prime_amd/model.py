@@ -20,11 +20,15 @@ the tokens and targets are random ids, each sequence's targets its next token (-
 
 ``window`` (and ``sinks``) or ``groups`` select k_attn's attention over part of the keys in place of
 causal attention: a sliding window in every layer, or answers behind shared prompts.
+
+``policy_step`` and ``preference_step`` train on k_loss's losses over the tokens' log-probabilities in
+place of cross entropy, ``score`` gives the log-probabilities that they compare with, and ``clip_grads``
+bounds the gradients' global norm.
 """
 
 import torch
 
-from . import k_attn, k_head, k_norm, k_rope
+from . import k_attn, k_grad, k_head, k_loss, k_norm, k_rope
 from .stack import D, KV, NF4LinearStack, layer_flops
 from .w4linear import (down_swiglu_backward, gateup_swiglu_forward, linear_backward_dx,
                        linear_backward_dx_lora, linear_forward, linear_forward_rope,
@@ -145,6 +149,7 @@ class QwenQLoRAStep(NF4LinearStack):
         self.perm = torch.cat([torch.nonzero(has)[:, 0], torch.nonzero(~has)[:, 0]]).to(torch.int32)
         self.tgt_sorted = tgt.index_select(0, self.perm.long()).contiguous()
         self.n_lab = int(has.sum())
+        self.labelled = self.perm[:self.n_lab].long()
         self.e_target = self.emb.index_select(0, self.tgt_sorted[:self.n_lab].long()).contiguous()
         self.tgt = tgt
 
@@ -195,15 +200,24 @@ class QwenQLoRAStep(NF4LinearStack):
         return k_head.streamed_head(self.yf, self.source, self.tgt_sorted, self.perm, self.n_lab,
                                     self.e_target, self.head_grad_scale)
 
-    def backward(self, dy_head, g_loss=1.0):
-        """LoRA gradients of g_loss * loss_sum: self.grads[i] = (dA_q, dB_q, dA_v, dB_v) fp32."""
+    def backward(self, dy_head, g_loss=1.0, dlogp=None):
+        """LoRA gradients of g_loss * loss_sum: self.grads[i] = (dA_q, dB_q, dA_v, dB_v) fp32.  dlogp [n_lab]
+        (fp32, sorted order): of g_loss * a loss with this gradient for the tokens' log-probabilities
+        instead (loss_sum's is -1 each)."""
         self._pass = getattr(self, "_pass", 0) + 1
         self._forward = False
         w16, side, done = self._w16, self._side, self._done
         gscale = torch.full((1,), float(g_loss) / self.head_grad_scale, dtype=torch.float32,
                             device=self.device)
         dh, dh16 = self.dh, self.dh16
-        k_norm.rms_backward(dy_head, gscale, self.hf, self.w_final, self.rstd_f, dh, out16=dh16)
+        row_scale = None
+        if dlogp is not None:
+            if dlogp.dtype != torch.float32 or tuple(dlogp.shape) != (self.n_lab,):
+                raise ValueError(f"dlogp must be fp32 [{self.n_lab}] (the tokens with a target)")
+            row_scale = torch.zeros(self.m, dtype=torch.float32, device=self.device)
+            row_scale.index_copy_(0, self.labelled, -dlogp)
+        k_norm.rms_backward(dy_head, gscale, self.hf, self.w_final, self.rstd_f, dh, out16=dh16,
+                            row_scale=row_scale)
         ks = self.keep_scale
         for i in reversed(range(self.n_layers)):
             Lw, lo, z = self.layers[i], self.lora[i], self.z[i]
@@ -251,3 +265,79 @@ class QwenQLoRAStep(NF4LinearStack):
         loss, stats, dy_head = self.forward()
         self.backward(dy_head)
         return loss
+
+    def score(self, adapters=True, scale=1.0):
+        """(logp, entropy) fp32 [n_lab] of the batch's targets in sorted order, without dropout: under the
+        adapters (a policy's scores of its own samples) or, with adapters False, under the frozen weights
+        alone (the reference).  scale: a factor of the logits (1 / temperature).  The logits are summed in
+        fp32, where forward()'s stats round them to fp16.  What a pending backward() reads stays as it is."""
+        self._pass = getattr(self, "_pass", 0) + 1
+        self._forward = True
+        dev, f16, f32 = self.device, torch.float16, torch.float32
+        w16, side, done, m = self._w16, self._side, self._done, self.m
+        attend = k_attn.span_attention_forward if self.span else k_attn.attention_forward
+        x, xsum, h = self.x0, torch.empty(m, D, dtype=f32, device=dev), torch.empty(m, D, dtype=f32, device=dev)
+        y, op, d16 = (torch.empty(m, D, dtype=f16, device=dev) for _ in range(3))
+        qkv = torch.empty(m, (NQ + 2 * NKV) * HD, dtype=f16, device=dev)
+        act = torch.empty_like(self.act)
+        rstd = torch.empty(m, dtype=f32, device=dev)
+        z = [torch.empty_like(self.z[0][t]) for t in ("q", "v")]
+        d_prev = None
+        for i in range(self.n_layers):
+            Lw, lo = self.layers[i], self.lora[i]
+            k_norm.rms_forward(x, self.w_in[i], y, rstd, self.eps, delta=d_prev,
+                               xout=xsum if d_prev is not None else None)
+            x = x if d_prev is None else xsum
+            terms = []
+            if adapters:
+                self._lora_downs(i, lambda dq: lora_down_multi(
+                    y, [(lo["Aq"], None, 1.0), (lo["Av"], None, 1.0)], outs=z, dequant=dq))
+                terms = [(z[0], lo["Bq"], 0, D, self.s), (z[1], lo["Bv"], D + KV, D + 2 * KV, self.s)]
+            else:
+                self._deferred = None     # (a dequant that waits for the downs: w16 below runs it)
+            linear_forward_rope(y, Lw["qkv"], lo["bias"], terms, self.pos, self.cos, self.sin,
+                                (NQ + NKV) * HD, out=qkv, w16=w16("qkv", i), side=side("qkv", i + 1))
+            done("qkv", i + 1)
+            att, _ = attend(qkv, self.meta, NQ, NKV, HD)
+            linear_forward(att, Lw["o"], out=op, w16=w16("o", i), side=side("o", i + 1))
+            done("o", i + 1)
+            k_norm.rms_forward(x, self.w_post[i], y, rstd, self.eps, delta=op, xout=h)
+            gateup_swiglu_forward(y, Lw["gu"], act=act, save_gu=False, w16=w16("gu", i),
+                                  side=side("gu", i + 1))
+            done("gu", i + 1)
+            linear_forward(act, Lw["d"], out=d16, w16=w16("d", i), side=side("d", i + 1))
+            done("d", i + 1)
+            x, d_prev = h, d16
+        k_norm.rms_forward(x, self.w_final, y, rstd, self.eps, delta=d_prev)
+        logp, entropy, _ = k_head.token_logprobs(y, self.source, self.tgt_sorted[:self.n_lab],
+                                                 rows=self.perm[:self.n_lab], scale=scale)
+        return logp, entropy
+
+    def _check_rows(self, meta):
+        if meta.n_tokens != self.n_lab:
+            raise ValueError(f"the plan has {meta.n_tokens} tokens, the batch {self.n_lab} with a target")
+
+    def policy_step(self, meta, old, advantages, *, ref=None, g_loss=1.0, **options):
+        """A training step on the clipped policy loss: meta the plan of the batch's answers
+        (k_loss.row_meta(trainer.answer_lens(batch), ...)), old (and ref) log-probabilities in sorted order
+        (score(), or the head's stats of an earlier forward()), options as k_loss.policy_loss.  Returns
+        (loss, its stats per answer, the head's stats); the gradients of g_loss * loss are in self.grads."""
+        self._check_rows(meta)
+        _, stats, dy = self.forward()
+        loss, dlogp, rows = k_loss.policy_loss(stats, old, advantages, meta, ref=ref, **options)
+        self.backward(dy, g_loss, dlogp=dlogp)
+        return loss, rows, stats
+
+    def preference_step(self, meta, ref, *, g_loss=1.0, **options):
+        """A training step on the preference loss over meta's pairs of answers (options as
+        k_loss.preference_loss; ref None: without a reference).  Returns (loss, rewards, margins, the head's
+        stats); the gradients of g_loss * loss are in self.grads."""
+        self._check_rows(meta)
+        _, stats, dy = self.forward()
+        loss, dlogp, rewards, margins = k_loss.preference_loss(stats, ref, meta, **options)
+        self.backward(dy, g_loss, dlogp=dlogp)
+        return loss, rewards, margins, stats
+
+    def clip_grads(self, max_norm):
+        """Scales self.grads in place to a global norm of at most max_norm; returns the norm before."""
+        return k_grad.clip_grads([g for layer in self.grads for g in layer], max_norm)

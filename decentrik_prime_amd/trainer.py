@@ -12,6 +12,13 @@ none of it is on the NF4 linear path.
     loss_sum, stats, dy = step.forward()
     loss = compute_loss(loss_sum, batch, num_items_in_batch)
     metrics = batch_metrics(batch, stats.cpu())
+
+Training from rewards or preferences (no counterpart in the reference) takes the same batches:
+
+    meta = k_loss.row_meta(answer_lens(batch), device)          # or (..., pairs=[(chosen, rejected)])
+    old, _ = step.score()                                       # ref, _ = step.score(adapters=False)
+    loss, rows, stats = step.policy_step(meta, old, advantages, ref=ref, kl_coef=0.04)
+    norm = step.clip_grads(1.0)
 """
 
 from dataclasses import dataclass
@@ -138,6 +145,13 @@ def pack_answers(groups, vocab):
                        row_sorted=rows[perm], valid_sorted=has[perm], n_real=int(ids.numel()),
                        n_lab=int(has.sum()), B=B, T=longest, groups=shape,
                        copies_sorted=copies[perm])
+
+
+def answer_lens(batch):
+    """Tokens with a target of each batch row: in the sorted order they stand row after row before the
+    tokens without one, as k_loss.row_meta's rows do."""
+    rows = torch.as_tensor(batch.row_sorted, dtype=torch.int64)[:batch.n_lab]
+    return torch.bincount(rows, minlength=batch.B).tolist()
 
 
 def batch_metrics(batch, stats):

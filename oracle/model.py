@@ -19,13 +19,14 @@ import math
 import torch
 
 
-def qwen_step(p, lens, nq=12, nkv=2, hd=128, visible=None):
+def qwen_step(p, lens, nq=12, nkv=2, hd=128, visible=None, weights=None):
     """p: CPU tensors x0 [n, D] fp32, emb [V, D], tgt [n] (-1 = none), pos [n], cos / sin
     [positions, hd], w_final [D], eps, ks (dropout keep scale), s (LoRA scale), and layers: dicts
     of wqkv [(nq + 2 nkv) hd, D], bias, wo [D, nq hd], wgu [2 I, D] (gate rows, then up rows),
     wd [D, I], w_in, w_post [D], Aq [r, D], Bq [nq hd, r], Av [r, D], Bv [nkv hd, r], mq / mv
     [n, D] (nonzero = keep).  visible [n, n] bool: the keys that each query sees, in place of causal
-    attention inside sequences of lengths lens.  Returns (loss_sum, [(dA_q, dB_q, dA_v, dB_v) per layer])."""
+    attention inside sequences of lengths lens.  weights [n]: factors of the tokens' cross entropies (1).
+    Returns (loss_sum, [(dA_q, dB_q, dA_v, dB_v) per layer])."""
     dt = torch.float64
     eps, ks, s = float(p["eps"]), float(p["ks"]), float(p["s"])
     n = p["x0"].shape[0]
@@ -79,6 +80,7 @@ def qwen_step(p, lens, nq=12, nkv=2, hd=128, visible=None):
     logits = yf @ p["emb"].to(dt).T
     tgt = p["tgt"].long()
     valid = tgt >= 0
-    loss = torch.nn.functional.cross_entropy(logits[valid], tgt[valid], reduction="sum")
+    each = torch.nn.functional.cross_entropy(logits[valid], tgt[valid], reduction="none")
+    loss = each.sum() if weights is None else (each * weights.to(dt)[valid]).sum()
     loss.backward()
     return float(loss.detach()), [tuple(A[k].grad for k in ("Aq", "Bq", "Av", "Bv")) for A in params]

@@ -1,0 +1,185 @@
+"""Training steps from rewards and preferences (model.QwenQLoRAStep.score, policy_step, preference_step,
+clip_grads) on packed answers, against float64 autograd of the decoder with the same token weights."""
+
+import numpy as np
+import pytest
+import torch
+
+from tests.helpers import host, log
+from tests.test_gpu_model import _reference_inputs
+
+pytestmark = pytest.mark.gpu
+
+VOCAB = 4096
+
+
+def _groups(seed=3):
+    rng = np.random.default_rng(seed)
+    return [(rng.integers(0, VOCAB, p), [rng.integers(0, VOCAB, a) for a in ans])
+            for p, ans in ((70, (30, 1, 45)), (9, (40, 12)))]
+
+
+def _step(shared=True, **kw):
+    """(batch, step) of the groups' answers, behind shared prompts or in rows of their own."""
+    from decentrik_prime_amd import model, trainer
+    if shared:
+        batch = trainer.pack_answers(_groups(), VOCAB)
+    else:
+        whole = [(np.concatenate([p, a]), len(p)) for p, ans in _groups() for a in ans]
+        ids, mask, labels = (torch.zeros(len(whole), 130, dtype=torch.int64) for _ in range(3))
+        labels -= 100
+        for b, (w, n) in enumerate(whole):
+            ids[b, :len(w)], mask[b, :len(w)] = torch.from_numpy(w), 1
+            labels[b, n:len(w)] = torch.from_numpy(w[n:])
+        batch = trainer.pack(ids, mask, labels, VOCAB)
+    return batch, model.QwenQLoRAStep.for_batch(batch, n_layers=2, vocab=VOCAB, seed=5, head_chunk=1024, **kw)
+
+
+def _visible(batch):
+    from oracle import attn
+    return None if batch.groups is None else torch.from_numpy(attn.prefix_visible(batch.groups))
+
+
+def _check_grads(st, want):
+    """LoRA gradients as the causal step's test holds them: within 1e-2 of their largest."""
+    for i in range(2):
+        for nm, got, ref in zip(("dA_q", "dB_q", "dA_v", "dB_v"), st.grads[i], want[i]):
+            g, r = host(got).astype(np.float64), ref.numpy()
+            err = float(np.abs(g - r).max()) / float(np.abs(r).max())
+            assert err <= 1e-2, f"layer {i} {nm}: {err:.3g}"
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_policy_step_matches_float64(shared):
+    from decentrik_prime_amd import k_loss, k_nf4, trainer
+    from oracle import model as ref
+    batch, st = _step(shared)
+    log(f"policy step, shared prompts {shared}")
+    lens = trainer.answer_lens(batch)
+    assert lens == [30, 1, 45, 40, 12]
+    meta = k_loss.row_meta(lens, "cuda")
+    old, _ = st.score()
+    base, _ = st.score(adapters=False)
+    adv = torch.tensor([1.0, -0.5, 0.25, -2.0, 0.0], device="cuda")
+    old = old + 0.1 * torch.randn(old.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    loss, rows, stats = st.policy_step(meta, old, adv, ref=base, kl_coef=0.1)
+    again, dlogp, rows2 = k_loss.policy_loss(stats, old, adv, meta, ref=base, kl_coef=0.1)
+    assert torch.equal(loss, again) and torch.equal(rows, rows2)
+    weights = torch.zeros(st.m)
+    weights[st.labelled.cpu()] = -dlogp.cpu()
+    _, want = ref.qwen_step(_reference_inputs(torch, st, k_nf4), st.lens, visible=_visible(batch),
+                            weights=weights)
+    _check_grads(st, want)
+    # the norm, and the gradients scaled to a quarter of it
+    before = [g.clone() for layer in st.grads for g in layer]
+    norm = float(torch.cat([g.reshape(-1) for g in before]).double().norm())
+    assert float(st.clip_grads(norm / 4)) == pytest.approx(norm, rel=1e-6)
+    for a, b in zip((g for layer in st.grads for g in layer), before):
+        assert torch.allclose(a, b * 0.25, rtol=1e-4, atol=0)     # (1e-6 beside the norm)
+
+
+def test_preference_step_matches_float64():
+    from decentrik_prime_amd import k_loss, k_nf4, trainer
+    from oracle import model as ref
+    batch, st = _step()
+    log("preference step")
+    meta = k_loss.row_meta(trainer.answer_lens(batch), "cuda", pairs=[(0, 1), (2, 0), (3, 4)])
+    base, _ = st.score(adapters=False)
+    loss, rewards, margins, stats = st.preference_step(meta, base, beta=0.3, label_smoothing=0.1)
+    again, dlogp, r2, m2 = k_loss.preference_loss(stats, base, meta, beta=0.3, label_smoothing=0.1)
+    assert torch.equal(loss, again) and torch.equal(rewards, r2) and torch.equal(margins, m2)
+    weights = torch.zeros(st.m)
+    weights[st.labelled.cpu()] = -dlogp.cpu()
+    _, want = ref.qwen_step(_reference_inputs(torch, st, k_nf4), st.lens, visible=_visible(batch),
+                            weights=weights)
+    _check_grads(st, want)
+
+
+def test_unit_weights_are_the_cross_entropy_step():
+    """dlogp of -1 throughout: the gradients of backward() without it, bit for bit, and halved with it."""
+    _, st = _step()
+    _, _, dy = st.forward()
+    plain = [g.clone() for layer in st.backward(dy) for g in layer]
+    _, _, dy = st.forward()
+    ones = torch.full((st.n_lab,), -1.0, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip((g for la in st.backward(dy, dlogp=ones) for g in la), plain))
+    with pytest.raises(ValueError):
+        st.backward(dy, dlogp=ones[1:])
+
+
+@pytest.mark.parametrize("ahead", ["layer", "carried", ("gu", "d", "qkv", "o")])
+def test_score_between_forward_and_backward(ahead):
+    """Scoring, with adapters and without, before a step and inside it: the step's loss and gradients stay
+    the same bits, and so do the scores; without dropout they are the step's own log-probabilities."""
+    _, st = _step(ahead=ahead)
+    for i in range(2):
+        for k in ("mq", "mv"):
+            st.lora[i][k] = torch.ones_like(st.lora[i][k])
+    st.keep_scale = 1.0
+    loss = st.step()
+    want = [g.clone() for layer in st.grads for g in layer]
+    first = [t.clone() for a in (True, False) for t in st.score(adapters=a)]
+    again, stats, dy = st.forward()
+    middle = [t.clone() for a in (True, False) for t in st.score(adapters=a)]
+    grads = [g for layer in st.backward(dy) for g in layer]
+    assert torch.equal(loss, again) and all(torch.equal(a, b) for a, b in zip(grads, want))
+    assert all(torch.equal(a, b) for a, b in zip(first, middle))
+    # the training head's logits are rounded to fp16; hidden states alike but for the adapters' input,
+    # rounded once there
+    n = st.n_lab
+    tol = 2.0 ** -11 * 2 * float(stats[:, 3].abs().max() + stats[:n, 0].max()) + 5e-3
+    assert float((first[0] + stats[:n, 0]).abs().max()) <= tol
+    assert float((first[1] - stats[:n, 1]).abs().max()) <= tol
+    assert float((first[2] - first[0]).abs().max()) > 1e-3          # the adapters matter
+
+
+def test_score_without_adapters_is_the_base_model():
+    _, st = _step()
+    base = [t.clone() for t in st.score(adapters=False)]
+    for i in range(2):
+        st.lora[i]["Bq"].zero_()
+        st.lora[i]["Bv"].zero_()
+    for a, b in zip(st.score(), base):
+        assert torch.equal(a, b)
+    warm = st.score(scale=0.5)
+    assert float((warm[1] - base[1]).min()) > 0                     # a higher temperature: more entropy
+
+
+def test_plans_of_another_batch_are_refused():
+    from decentrik_prime_amd import k_loss
+    _, st = _step()
+    meta = k_loss.row_meta([3, 4], "cuda", pairs=[(0, 1)])
+    x = torch.zeros(7, device="cuda")
+    with pytest.raises(ValueError):
+        st.policy_step(meta, x, torch.zeros(2, device="cuda"))
+    with pytest.raises(ValueError):
+        st.preference_step(meta, x)
+
+
+@pytest.mark.parametrize("d", [64, 1536, 4096])
+@pytest.mark.parametrize("fp32", [False, True])
+def test_norm_backward_with_a_factor_per_row(d, fp32):
+    from decentrik_prime_amd import k_norm
+    from oracle import norm
+    g = torch.Generator(device="cuda").manual_seed(d)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g, device="cuda")
+    n = 37
+    x, w, dres = randn(n, d), 1 + 0.1 * randn(d), randn(n, d)
+    dy = randn(n, d) if fp32 else randn(n, d).half()
+    rstd = torch.rsqrt(x.square().mean(1) + 1e-6)
+    gscale, scale = torch.full((1,), 0.5, device="cuda"), randn(n)
+    scale[3] = 0.0
+    out, plain, one = dres.clone(), dres.clone(), dres.clone()
+    k_norm.rms_backward(dy, gscale, x, w, rstd, out, dres=out, row_scale=scale)
+    up = host(dy).astype(np.float64) * 0.5 * host(scale).astype(np.float64)[:, None]
+    want = norm.rms_bwd_float64(up, host(x).astype(np.float64), host(w), 1e-6) + host(dres)
+    assert np.allclose(host(out), want, rtol=1e-4, atol=1e-4)      # as without factors
+    assert torch.equal(out[3], dres[3])
+    k_norm.rms_backward(dy, gscale, x, w, rstd, plain, dres=plain)
+    k_norm.rms_backward(dy, gscale, x, w, rstd, one, dres=one, row_scale=torch.ones_like(scale))
+    assert torch.equal(one, plain)
+    for bad in (scale[1:], scale.double(), scale.cpu(), scale.view(n, 1)):
+        with pytest.raises(ValueError):
+            k_norm.rms_backward(dy, gscale, x, w, rstd, out, row_scale=bad)

@@ -241,3 +241,17 @@ def test_metrics_of_shared_prompts_are_those_of_rows_of_their_own():
     assert abs(a["accuracy"] - b["accuracy"]) < 2.0 ** -52
     np.testing.assert_allclose(a["row_loss"], b["row_loss"], rtol=1e-14)
     assert a["row_tokens"] == b["row_tokens"] and a["n_lab"] == b["n_lab"]
+
+
+def test_answer_lens_are_the_rows_tokens_with_a_target():
+    from decentrik_prime_amd import k_loss
+    ids, mask, labels = _batch()
+    labels[1] = -100                                   # a row without targets
+    b = trainer.pack(ids, mask, labels, vocab=50)
+    lens = trainer.answer_lens(b)
+    assert lens == [int((b.tgt[sum(b.lens[:r]):sum(b.lens[:r + 1])] >= 0).sum()) for r in range(3)]
+    assert lens[1] == 0 and sum(lens) == b.n_lab
+    assert b.row_sorted[:b.n_lab].tolist() == [r for r, n in enumerate(lens) for _ in range(n)]
+    assert k_loss.row_meta(lens, "cpu").n_tokens == b.n_lab
+    groups = [([1, 2, 3], [[4, 5], [6]]), ([7], [[8, 9, 10], [11], [12, 13]])]
+    assert trainer.answer_lens(trainer.pack_answers(groups, 50)) == [2, 1, 3, 1, 2]
