@@ -227,17 +227,17 @@ __device__ __forceinline__ void lp_walk(const LpParams& p, f16* As, int32_t* tgt
     bool mine = false;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
-      mine |= (unsigned)(tgts[wm * WM + 16 * i + r16] - first) < (unsigned)WN;
+      mine |= (unsigned)tgts[wm * WM + 16 * i + r16] - (unsigned)first < (unsigned)WN;
     if (__builtin_amdgcn_ballot_w64(mine)) {
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const int at = tgts[wm * WM + 16 * i + r16] - first;
+        const unsigned at = (unsigned)tgts[wm * WM + 16 * i + r16] - (unsigned)first;
         float x = acc[i][0][0];
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x = at == 16 * j + q ? acc[i][j][q] : x;
-        if (at >= 0 && at < WN && (at & 15) < 4 && at + first < v1)
+          for (int q = 0; q < 4; ++q) x = at == 16u * j + q ? acc[i][j][q] : x;
+        if (at < (unsigned)WN && (at & 15) < 4 && (int)at + first < v1)
           p.xt[m0 + wm * WM + 16 * i + r16] = x;
       }
     }
@@ -429,15 +429,16 @@ LpPlan lp_plan(int64_t n, int64_t V, int64_t D) {
     }
   };
   for (const LpCost& c : kLpCost) {
-    const int64_t tiles = (n + c.bm - 1) / c.bm, pieces = (V + c.bn - 1) / c.bn;
-    for (int64_t rounds = 1; rounds <= 4; ++rounds) {
-      int64_t g = rounds * kLpSlots / tiles;
+    const uint32_t tiles = ((uint32_t)n + c.bm - 1) / c.bm, pieces = ((uint32_t)V + c.bn - 1) / c.bn;
+    for (uint32_t rounds = 1; rounds <= 4; ++rounds) {
+      uint32_t g = rounds * kLpSlots / tiles;
       g = g < 1 ? 1 : g < pieces ? g : pieces;
-      const int64_t each = (pieces + g - 1) / g;
-      g = (pieces + each - 1) / each;            // the fewest runs of that many pieces
-      const int64_t all = (tiles * g + kLpSlots - 1) / kLpSlots;
-      consider(lp_pieces_us(c, all * each, tiles * g, steps),
-               LpPlan{c.bm, c.bn, (int)tiles, (int)g, 0, (int)pieces}, c.fixed);
+      const uint32_t each = (pieces + g - 1) / g;
+      const uint32_t runs = (pieces + each - 1) / each;   // the fewest runs of that many pieces
+      const int64_t all = ((int64_t)tiles * runs + kLpSlots - 1) / kLpSlots;
+      consider(lp_pieces_us(c, all * each, (int64_t)tiles * runs, steps),
+               LpPlan{c.bm, c.bn, (int)tiles, (int)runs, 0, (int)pieces}, c.fixed);
+      if (g == pieces) break;
     }
   }
   const LpCost &big = kLpCost[3], &small = kLpCost[2];

@@ -15,7 +15,7 @@ many times over): the reference's host-memory EmbeddingStream is not needed on t
 import torch
 
 from . import _lib
-from .w4linear import _h16_workspace
+from .w4linear import _h16_workspace, _needed
 
 STATE_W = 8          # per-row running state: m, s, t, argmax, x_target, (pad)
 CHUNK = 32768        # vocabulary rows per chunk (a multiple of 64): at 2048 tokens a 134 MB
@@ -160,8 +160,7 @@ def token_logprobs(yf, emb, tgt, *, rows=None, scale=1.0):
             raise ValueError(f"{nm} must be a contiguous int32 [n] tensor on {dev}")
     if not 0.0 < scale <= 1e6:
         raise ValueError(f"scale must be within (0, 10^6] (got {scale})")
-    out = torch.empty((3, n), dtype=torch.float32, device=dev)
-    logp, entropy, lse = out
+    logp, entropy, lse = torch.empty((3, n), dtype=torch.float32, device=dev).unbind(0)
     if n == 0:
         return logp, entropy, lse
     if total == 0:
@@ -175,10 +174,11 @@ def token_logprobs(yf, emb, tgt, *, rows=None, scale=1.0):
         rows = torch.where(inside, torch.arange(n, dtype=torch.int32, device=dev), -1)
         total = n
     lib = _lib.lib()
-    nbytes = lib.dk_head_logprobs_workspace(n, emb.shape[0], d)
+    vocab = emb.shape[0]
+    nbytes = _needed(("logprobs", n, vocab, d), lambda: lib.dk_head_logprobs_workspace(n, vocab, d))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.launch(dev, lib.dk_head_logprobs, "dk_head_logprobs", yf.data_ptr(), yf.stride(0), total,
-                _lib.ptr(rows), n, emb.data_ptr(), emb.shape[0], d, tgt.data_ptr(), float(scale),
+                _lib.ptr(rows), n, emb.data_ptr(), vocab, d, tgt.data_ptr(), scale,
                 logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes)
     return logp, entropy, lse
 

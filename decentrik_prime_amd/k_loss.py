@@ -72,10 +72,18 @@ class RowMeta:
         self.device = self._buffer.device
         first = self._buffer.data_ptr()
         self.at = {name: first + 4 * int(s) for name, s in zip(parts, starts)}   # addresses in the buffer
+        self._stream = _lib.stream_handle(self.device) if self.device.type == "cuda" else None
         lib = _lib.lib()
         self.policy_bytes = lib.dk_policy_loss_workspace(self.n_items, self.n_tokens)
         self.preference_bytes = lib.dk_preference_loss_workspace(self.n_items, self.n_tokens,
                                                                  self.n_pairs or 0)
+
+    def kept(self):
+        """The kernels' addresses; a plan used on another stream than the one it was made on keeps its memory
+        until that stream is done with it, also when it is dropped before."""
+        if _lib.stream_handle(self.device) != self._stream:
+            self._buffer.record_stream(torch.cuda.current_stream(self.device))
+        return self.at
 
 
 def row_meta(lens, device, pairs=None):
@@ -126,7 +134,7 @@ def policy_loss(logp, old, advantages, meta, *, ref=None, kl_coef=0.0, clip_low=
     loss = torch.empty((), dtype=torch.float32, device=dev)
     nbytes = meta.policy_bytes
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    which, at = REDUCTIONS.index(reduction), meta.at
+    which, at = REDUCTIONS.index(reduction), meta.kept()
     _lib.launch(dev, _lib.lib().dk_policy_loss, "dk_policy_loss", at["items"], meta.n_items,
                 at["row_items"], rows, n, x, o, f, advantages.data_ptr(), per_token, clip_low, clip_high,
                 kl_coef, which, (meta.n_filled, n, 1)[which] or 1, dlogp.data_ptr(), stats.data_ptr(),
@@ -159,7 +167,7 @@ def preference_loss(logp, ref, meta, *, beta=0.1, kind="sigmoid", label_smoothin
     rewards = torch.empty(rows, dtype=torch.float32, device=dev)
     margins = torch.empty(meta.n_pairs, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes, at = meta.preference_bytes, meta.at
+    nbytes, at = meta.preference_bytes, meta.kept()
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.launch(dev, _lib.lib().dk_preference_loss, "dk_preference_loss", at["items"], meta.n_items,
                 at["row_items"], rows, n, at["row_pairs"], at["entries"], at["pairs"], meta.n_pairs, x, f,

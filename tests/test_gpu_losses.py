@@ -286,6 +286,28 @@ def test_losses_repeat_and_replay():
         assert all(torch.equal(a, b) for a, b in zip(out, want[turn % 2])), turn
 
 
+def test_a_plan_dropped_while_another_stream_uses_it():
+    """The plan's memory is not handed out again before the side stream's kernels have read it."""
+    from decentrik_prime_amd import k_loss
+    lens = [33 * i % 900 for i in range(60)]
+    x, old, f, g = draw(lens, seed=10)
+    adv = torch.randn(60, generator=g, device="cuda")
+    want = [t.clone() for t in k_loss.policy_loss(x, old, adv, k_loss.row_meta(lens, "cuda"))]
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        meta = k_loss.row_meta(lens, "cuda")
+        size = meta._buffer.numel()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            got = k_loss.policy_loss(x, old, adv, meta)
+        del meta
+        others = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del others
+
+
 def test_refusals():
     from decentrik_prime_amd import k_loss
     lens = [4, 6]
