@@ -28,10 +28,16 @@ constexpr int kPairs = 1024;     // pairs of a workgroup
 
 struct Tokens {          // a token array: element i at p[i * stride], negated where it holds losses
   const float* p;
-  int64_t stride;
+  uint32_t stride;
   float sign;
-  __device__ __forceinline__ float at(int64_t i) const { return sign * p[i * stride]; }
+  // an item's first element (in scalar registers), and element i behind it (one multiply-add)
+  __device__ __forceinline__ const float* from(int64_t begin) const { return p + begin * stride; }
+  __device__ __forceinline__ float at(const float* first, int i) const {
+    return first[(uint64_t)(uint32_t)i * stride];
+  }
 };
+
+__device__ __forceinline__ int wave_of() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 struct Item {
   int64_t begin;
@@ -96,16 +102,17 @@ __device__ __forceinline__ double policy_item(const PolicyParams& p, const Item&
   const double weight = p.reduction == 0 ? p.inv / (double)it.len : p.inv;   // a token's share of the loss
   const float w = (float)weight;
   const float* adv = p.adv_per_token ? p.adv + it.begin : p.adv + it.row;
+  const float *xp = p.logp.from(it.begin), *op = p.old.from(it.begin);
+  const float* rp = p.ref.p ? p.ref.from(it.begin) : xp;
   int clipped = 0;
   for (int t0 = 0; t0 < it.count; t0 += 64 * kAhead) {
     float x[kAhead], o[kAhead], rf[kAhead], a[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {   // every load before the first use, at tokens inside the item
       const int t = t0 + 64 * u + lane, in = t < it.count ? t : it.count - 1;
-      const int64_t i = it.begin + in;
-      x[u] = p.logp.p[i * p.logp.stride];
-      o[u] = p.old.p[i * p.old.stride];
-      rf[u] = p.ref.p ? p.ref.p[i * p.ref.stride] : 0.0f;
+      x[u] = p.logp.at(xp, in);
+      o[u] = p.old.at(op, in);
+      rf[u] = p.ref.p ? p.ref.at(rp, in) : 0.0f;
       a[u] = adv[p.adv_per_token ? in : 0];
     }
 #pragma unroll
@@ -147,7 +154,7 @@ __device__ __forceinline__ void store_stats(const PolicyParams& p, int64_t row, 
 __global__ __launch_bounds__(64 * kOneWaves) void policy_one_kernel(PolicyParams p) {
   __shared__ Sums sums[kOneItems];
   __shared__ double loss[kOneItems];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_of();
   for (int i = wave; i < p.n_items; i += kOneWaves) {
     Sums s;
     const double l = policy_item(p, item_of(p.items, i), s);
@@ -177,7 +184,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void policy_one_kernel(PolicyParams
 // losses and the other rows' items.
 __global__ __launch_bounds__(64 * kWaves) void policy_kernel(PolicyParams p) {
   __shared__ double loss[kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_of();
   const int i = blockIdx.x * kWaves + wave;
   double mine = 0.0;
   if (i < p.n_items) {
@@ -276,15 +283,16 @@ struct PrefParams {
 
 __device__ __forceinline__ double pref_item(const PrefParams& p, const Item& it) {
   const int lane = threadIdx.x & 63;
+  const float* xp = p.logp.from(it.begin);
+  const float* rp = p.ref.p ? p.ref.from(it.begin) : xp;
   double s = 0.0;
   for (int t0 = 0; t0 < it.count; t0 += 64 * kAhead) {
     float x[kAhead], r[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int t = t0 + 64 * u + lane;
-      const int64_t i = it.begin + (t < it.count ? t : it.count - 1);
-      x[u] = p.logp.p[i * p.logp.stride];
-      r[u] = p.ref.p ? p.ref.p[i * p.ref.stride] : 0.0f;
+      const int t = t0 + 64 * u + lane, in = t < it.count ? t : it.count - 1;
+      x[u] = p.logp.at(xp, in);
+      r[u] = p.ref.p ? p.ref.at(rp, in) : 0.0f;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
@@ -341,7 +349,7 @@ __device__ __forceinline__ void pref_tokens(const PrefParams& p, const Item& it,
 __global__ __launch_bounds__(64 * kOneWaves) void pref_one_kernel(PrefParams p) {
   __shared__ double sums[kOneItems], scores[kOneItems], slopes[kPairs];
   __shared__ double red[kOneWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = wave_of();
   for (int i = wave; i < p.n_items; i += kOneWaves) {
     const double s = pref_item(p, item_of(p.items, i));
     if (lane == 0) sums[i] = s;
@@ -371,7 +379,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void pref_one_kernel(PrefParams p) 
 }
 
 __global__ __launch_bounds__(64 * kWaves) void pref_sum_kernel(PrefParams p) {
-  const int i = blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int i = blockIdx.x * kWaves + wave_of();
   if (i >= p.n_items) return;
   const double s = pref_item(p, item_of(p.items, i));
   if ((threadIdx.x & 63) == 0) p.part[i] = s;
@@ -399,7 +407,7 @@ __global__ __launch_bounds__(64 * kWaves) void pref_apply_kernel(PrefParams p, i
     }
     return;
   }
-  const int i = (b - pair_wgs) * kWaves + (threadIdx.x >> 6);
+  const int i = (b - pair_wgs) * kWaves + wave_of();
   if (i >= p.n_items) return;
   const Item it = item_of(p.items, i);
   const double own = row_score(p, p.part, it.row);
@@ -421,11 +429,11 @@ __global__ __launch_bounds__(kSumThreads) void pref_loss_kernel(PrefParams p, in
 }
 
 bool tokens_ok(const dk_token_array* t, int64_t n) {
-  return t && n >= 0 && (n == 0 || t->data) && t->stride >= 0;
+  return t && n >= 0 && (n == 0 || t->data) && t->stride >= 0 && t->stride <= INT32_MAX;
 }
 
 Tokens tokens_of(const dk_token_array* t) {
-  return t ? Tokens{t->data, t->stride, t->negated ? -1.0f : 1.0f} : Tokens{nullptr, 1, 1.0f};
+  return t ? Tokens{t->data, (uint32_t)t->stride, t->negated ? -1.0f : 1.0f} : Tokens{nullptr, 1, 1.0f};
 }
 
 bool rows_ok(int64_t n_items, int64_t rows) {

@@ -254,7 +254,7 @@ int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* r
  * (low, high word), tokens, row, the row's tokens, the row's items, the item's place among them, 0} (int32
  * [n_items, 8], 16-byte aligned, row by row and in token order; a row has 1 to 64 items and at most 2^30
  * tokens, an empty row one item without tokens); row r's items are row_items[r] .. row_items[r + 1] - 1.  A
- * token array is fp32 with an element stride (0 allowed), negated where it holds losses (the head's stats:
+ * token array is fp32 with an element stride (0 to 2^31 - 1), negated where it holds losses (the head's stats:
  * column 0, stride 4).  With n_tokens = 0 the token arrays may be NULL.
  *
  * dk_policy_loss: A the advantage of the token (per_token) or of its row, r = e^(logp - old),

@@ -122,8 +122,9 @@ def test_loss_entries_refuse_bad_arguments():
         return lib.dk_policy_loss(items, n_items, p, rows, n, ref(x), ref(old), f and ref(f), adv, 0, low,
                                   high, kl, red, den, out, out, out, ws, nbytes, None)
     null, back = _lib.TokenArrayC(None, 1, 0), _lib.TokenArrayC(4096, -1, 0)
+    far = _lib.TokenArrayC(4096, 1 << 31, 0)
     for bad in (dict(items=None), dict(n_items=0), dict(n_items=1), dict(rows=0), dict(n=-1), dict(x=null),
-                dict(old=null), dict(f=null), dict(x=back), dict(adv=None), dict(low=1.1), dict(low=-0.1),
+                dict(old=null), dict(f=null), dict(x=back), dict(x=far), dict(adv=None), dict(low=1.1), dict(low=-0.1),
                 dict(high=-0.1), dict(high=float("nan")), dict(kl=float("inf")), dict(f=None), dict(red=3),
                 dict(red=-1), dict(den=0.0), dict(out=None)):
         assert policy(**bad) == _lib.DK_ERR_INVALID, bad
