@@ -363,12 +363,22 @@ __global__ __launch_bounds__(256) void head_logp_join_kernel(LpParams p, float* 
   const int lane = threadIdx.x & 63;
   const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= p.n) return;
-  LpState a = {kNone, 0.0f, 0.0f};
+  // what the result needs beside the states, loaded with them
+  const int64_t t = p.tgt[m];
+  const int64_t at = p.rows ? p.rows[m] : 0;
+  const float xt = p.xt[m];                    // (unwritten where there is no target: not used)
   const f32x4* mine = reinterpret_cast<const f32x4*>(p.part) + lp_part(p.plan, m);
   const int runs = lp_runs(p.plan, m);
-  for (int i = lane; i < runs; i += 64) {
-    const f32x4 b = mine[i];
-    a = lp_join(a, {b[0], b[1], b[2]});
+  LpState a = {kNone, 0.0f, 0.0f};
+  for (int i = lane; i < runs; i += 256) {     // four loads in flight; a run past the last joins as nothing
+    f32x4 b[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) b[u] = mine[i + 64 * u < runs ? i + 64 * u : lane < runs ? lane : 0];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool in = i + 64 * u < runs;
+      a = lp_join(a, {in ? b[u][0] : kNone, in ? b[u][1] : 0.0f, in ? b[u][2] : 0.0f});
+    }
   }
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) {
@@ -376,15 +386,14 @@ __global__ __launch_bounds__(256) void head_logp_join_kernel(LpParams p, float* 
     a = lp_join(a, o);
   }
   if (lane) return;
-  const int64_t t = p.tgt[m];
   const float l2 = log2f(a.s);
   float lp = 0.0f, en = kLn2 * (l2 - a.t / a.s), ls = kLn2 * (a.r + l2);
   if (t >= p.V) lp = NAN;
-  else if (t >= 0) lp = kLn2 * (__builtin_fmaf(p.xt[m], p.c, -a.r) - l2);
+  else if (t >= 0) lp = kLn2 * (__builtin_fmaf(xt, p.c, -a.r) - l2);
   // rounding takes neither past what it can be (NaN stays)
   lp = lp > 0.0f ? 0.0f : lp;
   en = en < 0.0f ? 0.0f : en;
-  if (p.rows && (p.rows[m] < 0 || p.rows[m] >= p.total)) lp = en = ls = NAN;
+  if (p.rows && (at < 0 || at >= p.total)) lp = en = ls = NAN;
   logp[m] = lp;
   entropy[m] = en;
   lse[m] = ls;

@@ -160,7 +160,7 @@ def token_logprobs(yf, emb, tgt, *, rows=None, scale=1.0):
             raise ValueError(f"{nm} must be a contiguous int32 [n] tensor on {dev}")
     if not 0.0 < scale <= 1e6:
         raise ValueError(f"scale must be within (0, 10^6] (got {scale})")
-    logp, entropy, lse = torch.empty((3, n), dtype=torch.float32, device=dev).unbind(0)
+    logp, entropy, lse = torch.empty(3, n, dtype=torch.float32, device=dev).unbind(0)
     if n == 0:
         return logp, entropy, lse
     if total == 0:

@@ -29,54 +29,70 @@ REDUCTIONS = ("row", "token", "sum")
 KINDS = ("sigmoid", "hinge", "ipo")
 
 
+def _whole(values, what):
+    """A list of whole numbers as int64."""
+    values = np.asarray(values)
+    if values.size and values.dtype.kind not in "iu":
+        raise ValueError(f"{what} must be whole numbers")
+    return values.astype(np.int64)
+
+
 class RowMeta:
     """The plan of rows of consecutive tokens (see row_meta): on the device the kernels' items, each row's
     items, and the pairs with each row's share of them."""
 
     def __init__(self, lens, device, pairs=None):
-        size = np.asarray([int(n) for n in lens], np.int64)
-        if size.size == 0 or size.min() < 0 or size.max() > 1 << 30 or size.size > 1 << 26:
+        size = _whole(lens, "lens").reshape(-1)
+        rows = size.size
+        if rows == 0 or rows > 1 << 26 or size.min() < 0 or size.max() > 1 << 30:
             raise ValueError("at least one row, each of 0 to 2^30 tokens")
-        self.lens = size.tolist()
-        self.n_rows, self.n_tokens = int(size.size), int(size.sum())
-        self.n_filled = int((size > 0).sum())
+        self.n_rows, self.n_tokens = int(rows), int(size.sum())
+        self.n_filled = int(np.count_nonzero(size))
         step = np.maximum(ITEM_TOKENS, -(-(-(-size // ROW_ITEMS)) // 64) * 64)
         count = np.maximum(1, -(-size // step))
-        row_items = np.concatenate([[0], np.cumsum(count)])
-        row = np.repeat(np.arange(size.size), count)
-        place = np.arange(row.size) - row_items[row]
+        last = np.cumsum(count)
+        n = self.n_items = int(last[-1])
+        self.n_pairs = None
+        both = None
+        if pairs is not None:
+            both = _whole(pairs, "pairs").reshape(-1, 2)
+            if both.size == 0 or both.min() < 0 or both.max() >= rows or len(both) > 1 << 28:
+                raise ValueError(f"at least one pair of rows 0 .. {rows - 1}")
+            self.n_pairs = len(both)
+        # one buffer: items, the pairs' entries and the pairs, row_pairs, row_items
+        k = self.n_pairs or 0
+        first = np.cumsum([0, 8 * n, 4 * k, 2 * k, (rows + 1) if k else 0]).tolist()
+        flat = np.empty(first[-1] + rows + 1, np.int32)
+        items = flat[:8 * n].reshape(n, 8)
+        row = np.repeat(np.arange(rows), count)
+        of = count[row]
+        place = np.arange(n) - (last - count)[row]
         at = place * step[row]                                        # first token within the row
         begin = (np.cumsum(size) - size)[row] + at
-        items = np.zeros((row.size, 8), np.int64)
-        items[:, 0], items[:, 1] = begin & 0xffffffff, begin >> 32
+        items[:, 0], items[:, 1] = begin.astype(np.uint32).view(np.int32), begin >> 32
         items[:, 2], items[:, 3] = np.minimum(step[row], size[row] - at), row
-        items[:, 4], items[:, 5], items[:, 6] = size[row], count[row], place
-        self.n_items = int(row.size)
-        parts = {"items": items}
-        self.n_pairs = None
-        if pairs is not None:
-            both = np.asarray([(int(a), int(b)) for a, b in pairs], np.int64).reshape(-1, 2)
-            if both.size == 0 or both.min() < 0 or both.max() >= size.size or len(both) > 1 << 28:
-                raise ValueError(f"at least one pair of rows 0 .. {size.size - 1}")
-            self.n_pairs = len(both)
+        items[:, 4], items[:, 5], items[:, 6], items[:, 7] = size[row], of, place, 0
+        flat[first[4]] = 0
+        flat[first[4] + 1:] = last
+        if k:
             own = both.T.reshape(-1)                                  # chosen rows, then rejected ones
-            other, index = both[:, ::-1].T.reshape(-1), np.arange(1, len(both) + 1)
-            entries = np.stack([other, np.concatenate([index, -index])], 1)
-            parts["entries"] = entries[np.argsort(own, kind="stable")]
-            parts["pairs"] = both
-            parts["row_pairs"] = np.concatenate([[0], np.cumsum(np.bincount(own, minlength=size.size))])
-        parts["row_items"] = row_items
-        flat = [p.reshape(-1).astype(np.uint32) for p in parts.values()]
-        starts = np.cumsum([0] + [p.size for p in flat])
-        self._buffer = torch.from_numpy(np.concatenate(flat).view(np.int32)).to(torch.device(device))
+            index = np.arange(1, k + 1)
+            order = np.argsort(own, kind="stable")
+            entries = flat[first[1]:first[2]].reshape(2 * k, 2)
+            entries[:, 0] = both[:, ::-1].T.reshape(-1)[order]
+            entries[:, 1] = np.concatenate([index, -index])[order]
+            flat[first[2]:first[3]] = both.reshape(-1)
+            flat[first[3]] = 0
+            flat[first[3] + 1:first[4]] = np.cumsum(np.bincount(own, minlength=rows))
+        self._buffer = torch.from_numpy(flat).to(torch.device(device))
         self.device = self._buffer.device
-        first = self._buffer.data_ptr()
-        self.at = {name: first + 4 * int(s) for name, s in zip(parts, starts)}   # addresses in the buffer
+        base = self._buffer.data_ptr()
+        self.at = {name: base + 4 * i for name, i in
+                   zip(("items", "entries", "pairs", "row_pairs", "row_items"), first)}
         self._stream = _lib.stream_handle(self.device) if self.device.type == "cuda" else None
         lib = _lib.lib()
-        self.policy_bytes = lib.dk_policy_loss_workspace(self.n_items, self.n_tokens)
-        self.preference_bytes = lib.dk_preference_loss_workspace(self.n_items, self.n_tokens,
-                                                                 self.n_pairs or 0)
+        self.policy_bytes = lib.dk_policy_loss_workspace(n, self.n_tokens)
+        self.preference_bytes = lib.dk_preference_loss_workspace(n, self.n_tokens, k)
 
     def kept(self):
         """The kernels' addresses; a plan used on another stream than the one it was made on keeps its memory
@@ -131,7 +147,7 @@ def policy_loss(logp, old, advantages, meta, *, ref=None, kl_coef=0.0, clip_low=
         raise ValueError(f"advantages must be a contiguous fp32 [{n if per_token else rows}] tensor on {dev}")
     dlogp = torch.empty(n, dtype=torch.float32, device=dev)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
+    loss = torch.empty_strided((), (), dtype=torch.float32, device=dev)
     nbytes = meta.policy_bytes
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     which, at = REDUCTIONS.index(reduction), meta.kept()
@@ -166,7 +182,7 @@ def preference_loss(logp, ref, meta, *, beta=0.1, kind="sigmoid", label_smoothin
     dlogp = torch.empty(n, dtype=torch.float32, device=dev)
     rewards = torch.empty(rows, dtype=torch.float32, device=dev)
     margins = torch.empty(meta.n_pairs, dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
+    loss = torch.empty_strided((), (), dtype=torch.float32, device=dev)
     nbytes, at = meta.preference_bytes, meta.kept()
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.launch(dev, _lib.lib().dk_preference_loss, "dk_preference_loss", at["items"], meta.n_items,

@@ -19,6 +19,7 @@ def read_plan(meta):
         return raw[at:at + n]
     items = part("items", 8 * meta.n_items).reshape(-1, 8)
     row_items = part("row_items", meta.n_rows + 1)
+    assert row_items.size == meta.n_rows + 1
     if meta.n_pairs is None:
         return items, row_items, None, None, None
     return (items, row_items, part("entries", 4 * meta.n_pairs).reshape(-1, 2),
@@ -30,7 +31,7 @@ def read_plan(meta):
 def test_items_cover_every_token_once(lens):
     meta = k_loss.row_meta(lens, "cpu")
     items, row_items = read_plan(meta)[:2]
-    assert meta.lens == lens and meta.n_tokens == sum(lens)
+    assert meta.n_rows == len(lens) and meta.n_tokens == sum(lens)
     assert meta.n_filled == sum(n > 0 for n in lens)
     assert row_items[0] == 0 and row_items[-1] == meta.n_items == len(items)
     start = 0
@@ -62,10 +63,10 @@ def test_every_row_names_its_pairs(lens, pairs):
 
 
 def test_plans_refuse_what_they_cannot_hold():
-    for lens in ([], [-1], [3, -2], [(1 << 30) + 1]):
+    for lens in ([], [-1], [3, -2], [(1 << 30) + 1], [1.5], ["a"]):
         with pytest.raises(ValueError):
             k_loss.row_meta(lens, "cpu")
-    for pairs in ([], [(0, 2)], [(-1, 0)]):
+    for pairs in ([], [(0, 2)], [(-1, 0)], [(0.0, 1.0)]):
         with pytest.raises(ValueError):
             k_loss.row_meta([1, 2], "cpu", pairs=pairs)
 
