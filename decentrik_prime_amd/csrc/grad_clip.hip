@@ -7,7 +7,13 @@
 // first read last is still in the 256 MB cache.  Squares and sums are in 64 bits: in 32, gradients above
 // 2^64 or below 2^-63 would give an infinite or a zero norm.  The tensors' addresses travel in the kernel
 // arguments (kBatch of them a launch), so a captured call holds no pointer to host memory and the device
-// keeps no table.  Bound: reading and writing the gradients; few and small ones: two launches.
+// keeps no table.
+//
+// Bound: reading and writing the gradients.  233 million fp16 elements into fp32 117 + 275 us (4.0 TB/s beside
+// the write-back of the previous call's output, 5.9 without one; 5.1 TB/s, a copy's rate); 112 tensors of
+// 2.2 million elements in place 4.9 + 4.2 us, and 39 us of host time for their addresses and checks.  512
+// workgroups or pieces of half the size read slower (117 and 96 us alone against 79), 2048 the same with
+// twice the sums to add up again; stores past the caches 387 -> 422 us.
 #include <algorithm>
 #include <type_traits>
 #include <vector>

@@ -13,8 +13,14 @@
 //
 // Differences of log-probabilities and the clip's borders are formed in 64 bits (a token within rounding
 // of a border would gain or lose its whole gradient), exponentials in 32, sums over tokens in 64 and in an
-// order that the sizes alone give.  Bound: latency up to some 10^5 tokens (one or two launches), beyond
-// that reading the token arrays once.
+// order that the sizes alone give.
+//
+// Bound: latency.  Up to 64 items and 32768 tokens one workgroup does everything in one launch: 1024 tokens'
+// policy loss 4.1 us, 237 tokens' preference loss 4.0, 32 answers in 112 pairs 10.0 (in three launches 14 with
+// their gaps).  Beyond, a wave per item and a second launch for what crosses items: one million tokens'
+// policy loss 9.8 + 4.0 us (29 MB, half of them the stats' other columns; some 80 vector instructions a
+// token are a third of it), the preference loss of 1024 answers 3.6 + 6.2.  A call's host time, about 12 us,
+// is longer than any of these but the first.
 #include "dk_common.h"
 
 namespace {
@@ -442,8 +448,8 @@ bool rows_ok(int64_t n_items, int64_t rows) {
 
 }  // namespace
 
-// Few items and tokens take one workgroup and launch: 32 answers of 16,000 tokens in all 9 us where two
-// launches take 5 each and their gap; 64 items of long rows would keep its CU busy for far longer than those.
+// Few items and tokens take one workgroup and launch (see the top); 64 items of long rows would keep its CU
+// busy for far longer than two launches take.
 static bool one_group(int64_t n_items, int64_t n_tokens) {
   return n_items <= kOneItems && n_tokens <= kOneTokens;
 }
