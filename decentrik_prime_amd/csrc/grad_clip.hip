@@ -203,7 +203,8 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, uint32_t piece
   const double norm = scale * sqrt(block_sum(s, red));
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const double ratio = max_norm / (norm + 1e-6);
-  const float factor = (float)(scale * (ratio > 1.0 ? 1.0 : ratio));   // a NaN norm: NaN
+  // a NaN norm gives NaN; no largest norm: `scale` alone, whatever the norm
+  const float factor = (float)(scale * (ratio > 1.0 || max_norm == INFINITY ? 1.0 : ratio));
   for (uint32_t b = blockIdx.x; b < pieces; b += gridDim.x) {
     const Piece q = piece_of(t, pieces - 1 - b);
     const void* src = t.src[q.tensor];

@@ -93,7 +93,8 @@ def clip_grads(grads, max_norm, *, scale=1.0, out=None):
     """Scales gradients to a global norm of at most max_norm: with norm = scale * (2-norm of all together)
     each becomes g * scale * min(1, max_norm / (norm + 1e-6)), in place or in `out` (tensors of the
     gradients' shapes, fp32, fp16 or bf16).  Returns the norm before clipping (fp32 scalar on the device).
-    An infinite norm scales by 0 and a NaN one gives NaN everywhere.  No tensor may overlap another."""
+    An infinite norm scales by 0 and a NaN one gives NaN everywhere (with max_norm infinite only scale counts).
+    No tensor may overlap another."""
     if not max_norm > 0.0:
         raise ValueError(f"max_norm must be positive (got {max_norm})")
     return _run(list(grads), max_norm, scale, out, in_place=out is None)

@@ -29,12 +29,12 @@ REDUCTIONS = ("row", "token", "sum")
 KINDS = ("sigmoid", "hinge", "ipo")
 
 
-def _whole(values, what):
-    """A list of whole numbers as int64."""
+def _whole(values, what, shape):
+    """A list of whole numbers, or of pairs of them, as int64."""
     values = np.asarray(values)
-    if values.size and values.dtype.kind not in "iu":
-        raise ValueError(f"{what} must be whole numbers")
-    return values.astype(np.int64)
+    if values.size and (values.dtype.kind not in "iu" or values.shape[1:] != shape or values.ndim == 0):
+        raise ValueError(f"{what} must be whole numbers" if not shape else f"{what} must be pairs of whole numbers")
+    return values.astype(np.int64).reshape(-1, *shape)
 
 
 class RowMeta:
@@ -42,7 +42,7 @@ class RowMeta:
     items, and the pairs with each row's share of them."""
 
     def __init__(self, lens, device, pairs=None):
-        size = _whole(lens, "lens").reshape(-1)
+        size = _whole(lens, "lens", ())
         rows = size.size
         if rows == 0 or rows > 1 << 26 or size.min() < 0 or size.max() > 1 << 30:
             raise ValueError("at least one row, each of 0 to 2^30 tokens")
@@ -55,7 +55,7 @@ class RowMeta:
         self.n_pairs = None
         both = None
         if pairs is not None:
-            both = _whole(pairs, "pairs").reshape(-1, 2)
+            both = _whole(pairs, "pairs", (2,))
             if both.size == 0 or both.min() < 0 or both.max() >= rows or len(both) > 1 << 28:
                 raise ValueError(f"at least one pair of rows 0 .. {rows - 1}")
             self.n_pairs = len(both)

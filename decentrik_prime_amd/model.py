@@ -340,4 +340,6 @@ class QwenQLoRAStep(NF4LinearStack):
 
     def clip_grads(self, max_norm):
         """Scales self.grads in place to a global norm of at most max_norm; returns the norm before."""
+        if any(layer is None for layer in self.grads):
+            raise ValueError("no gradients yet (backward)")
         return k_grad.clip_grads([g for layer in self.grads for g in layer], max_norm)

@@ -293,7 +293,8 @@ int dk_preference_loss(const int32_t* items, int64_t n_items, const int32_t* row
  * reference).  src, dst, numel, types and dst_types (DK_TYPE_*) are host arrays, read before the call
  * returns.  dst[i] may be src[i] (of one type; nothing is written where the
  * factor is 1); beyond that nothing written may overlap anything else in the lists (DK_ERR_INVALID).
- * max_norm > 0 (infinity: scale alone).  An infinite norm scales by 0, a NaN one gives NaN throughout.  workspace:
+ * max_norm > 0 (infinity: scale alone, whatever the norm); else an infinite norm scales by 0 and a NaN one gives
+ * NaN throughout.  workspace:
  * dk_grad_clip_workspace(n) bytes, 8-byte aligned. */
 #define DK_TYPE_F32 1
 #define DK_TYPE_F16 2

@@ -103,6 +103,18 @@ def test_norms_beyond_the_squares_of_fp32(size):
         check(k_grad.clip_grads(grads, 1.0), grads, norm, want)
 
 
+def test_a_gradient_of_more_than_2_to_the_31_elements():
+    from decentrik_prime_amd import k_grad
+    n = (1 << 31) + 5
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    for at in (0, 1 << 20, (1 << 31) - 1, 1 << 31, n - 1):
+        g[at] = 3.0
+    assert float(k_grad.clip_grads([g], 1.0)) == pytest.approx(math.sqrt(45), rel=1e-6)
+    assert int((g != 0).sum()) == 5
+    for at in (0, 1 << 20, (1 << 31) - 1, 1 << 31, n - 1):
+        assert float(g[at]) == pytest.approx(3 / math.sqrt(45), rel=2.0 ** -8)
+
+
 def test_what_is_not_finite():
     from decentrik_prime_amd import k_grad
     for bad, rest in ((float("inf"), 0.0), (float("nan"), float("nan"))):
@@ -112,6 +124,17 @@ def test_what_is_not_finite():
         assert not math.isfinite(float(norm)) and bool(torch.isnan(grads[0][2999]))
         for t in (grads[0][:2999], grads[1]):
             assert bool(torch.isnan(t).all()) if math.isnan(rest) else bool((t == 0).all())
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_no_largest_norm_scales_alone(bad):
+    from decentrik_prime_amd import k_grad
+    grads = [torch.ones(3000, device="cuda"), torch.ones(10, device="cuda").half()]
+    grads[0][7] = bad
+    assert not math.isfinite(float(k_grad.clip_grads(grads, math.inf, scale=0.5)))
+    assert not math.isfinite(float(grads[0][7]))
+    grads[0][7] = 0.5
+    assert all(bool((g == 0.5).all()) for g in grads)
 
 
 def test_captured_and_on_another_stream():

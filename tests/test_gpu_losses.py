@@ -286,6 +286,47 @@ def test_losses_repeat_and_replay():
         assert all(torch.equal(a, b) for a, b in zip(out, want[turn % 2])), turn
 
 
+def test_two_streams_share_a_plan():
+    """Calls that overlap on two streams, on one plan: each has its own scratch memory."""
+    from decentrik_prime_amd import k_loss
+    lens = [33 * i % 900 for i in range(200)]
+    x, old, f, g = draw(lens, seed=11)
+    y = (x - 0.1).contiguous()
+    adv = torch.randn(200, generator=g, device="cuda")
+    meta = k_loss.row_meta(lens, "cuda", pairs=[(i, 199 - i) for i in range(100)])
+
+    def both(v):
+        return (*k_loss.policy_loss(v, old, adv, meta, ref=f, kl_coef=0.1), *k_loss.preference_loss(v, f, meta))
+    want = [[t.clone() for t in both(v)] for v in (x, y)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for k, v in enumerate((x, y)):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(both(v))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
+
+
+def test_tokens_past_32_bits_of_offsets():
+    """A token array whose elements lie 2 * 10^6 apart: 9.6 GB."""
+    from decentrik_prime_amd import k_loss
+    lens = [700, 0, 500]
+    x, old, f, g = draw(lens, seed=12)
+    adv = torch.randn(3, generator=g, device="cuda")
+    meta = k_loss.row_meta(lens, "cuda", pairs=[(0, 2), (1, 0)])
+    wide = torch.empty(1200 * 2_000_003, device="cuda").as_strided((1200,), (2_000_003,))
+    wide.copy_(x)
+    for a, b in zip(k_loss.policy_loss(wide, old, adv, meta), k_loss.policy_loss(x, old, adv, meta)):
+        assert torch.equal(a, b)
+    for a, b in zip(k_loss.preference_loss(wide, f, meta), k_loss.preference_loss(x, f, meta)):
+        assert torch.equal(a, b)
+
+
 def test_a_plan_dropped_while_another_stream_uses_it():
     """The plan's memory is not handed out again before the side stream's kernels have read it."""
     from decentrik_prime_amd import k_loss

@@ -154,6 +154,8 @@ def test_plans_of_another_batch_are_refused():
         st.policy_step(meta, x, torch.zeros(2, device="cuda"))
     with pytest.raises(ValueError):
         st.preference_step(meta, x)
+    with pytest.raises(ValueError, match="no gradients"):
+        st.clip_grads(1.0)
 
 
 @pytest.mark.parametrize("d", [64, 1536, 4096])

@@ -63,10 +63,10 @@ def test_every_row_names_its_pairs(lens, pairs):
 
 
 def test_plans_refuse_what_they_cannot_hold():
-    for lens in ([], [-1], [3, -2], [(1 << 30) + 1], [1.5], ["a"]):
+    for lens in ([], [-1], [3, -2], [(1 << 30) + 1], [1.5], ["a"], [[1, 2]], 3, [True]):
         with pytest.raises(ValueError):
             k_loss.row_meta(lens, "cpu")
-    for pairs in ([], [(0, 2)], [(-1, 0)], [(0.0, 1.0)]):
+    for pairs in ([], [(0, 2)], [(-1, 0)], [(0.0, 1.0)], [0, 1], [(0, 1, 1, 0)], [(0, 1), (1,)]):
         with pytest.raises(ValueError):
             k_loss.row_meta([1, 2], "cpu", pairs=pairs)
 

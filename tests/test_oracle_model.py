@@ -61,3 +61,19 @@ def test_structural_zeros():
     for dAq, dBq, dAv, dBv in grads:
         assert torch.count_nonzero(dAq) == 0 and torch.count_nonzero(dAv) == 0   # B = 0 blocks A
         assert torch.count_nonzero(dBq) > 0 and torch.count_nonzero(dBv) > 0
+
+
+def test_token_weights_are_linear():
+    """Weights of 1 give the plain loss; losses and gradients of two sets of weights add up."""
+    p, lens = _params(2)
+    n = sum(lens)
+    plain, grads = model.qwen_step(p, lens, NQ, NKV, HD)
+    ones, same = model.qwen_step(p, lens, NQ, NKV, HD, weights=torch.ones(n))
+    assert abs(ones - plain) <= 1e-12 * plain
+    a = torch.linspace(-1.0, 2.0, n, dtype=torch.float64)
+    la, ga = model.qwen_step(p, lens, NQ, NKV, HD, weights=a)
+    lb, gb = model.qwen_step(p, lens, NQ, NKV, HD, weights=1.0 - a)
+    assert abs(la + lb - plain) <= 1e-10 * plain
+    for x, s, y, z in zip(grads, same, ga, gb):
+        for t in range(4):
+            assert torch.allclose(s[t], x[t]) and torch.allclose(y[t] + z[t], x[t], atol=1e-9)
