@@ -19,8 +19,8 @@
 // policy loss 4.1 us, 237 tokens' preference loss 4.0, 32 answers in 112 pairs 10.0 (in three launches 14 with
 // their gaps).  Beyond, a wave per item and a second launch for what crosses items: one million tokens'
 // policy loss 9.8 + 4.0 us (29 MB, half of them the stats' other columns; some 80 vector instructions a
-// token are a third of it), the preference loss of 1024 answers 3.6 + 6.2.  A call's host time, about 12 us,
-// is longer than any of these but the first.
+// token are a third of it), the preference loss of 1024 answers 3.6 + 6.2.  A call's host time, 10 to 13
+// us, is longer than most of these.
 #include "dk_common.h"
 
 namespace {
@@ -434,12 +434,13 @@ __global__ __launch_bounds__(kSumThreads) void pref_loss_kernel(PrefParams p, in
   if (threadIdx.x == 0) *p.loss = (float)(total / (double)p.n_pairs);
 }
 
-bool tokens_ok(const dk_token_array* t, int64_t n) {
-  return t && n >= 0 && (n == 0 || t->data) && t->stride >= 0 && t->stride <= INT32_MAX;
+// a token array that is there, or (ref alone) may be absent
+bool tokens_ok(const dk_token_array& t, int64_t n, bool absent) {
+  return (t.data || n == 0 || absent) && t.stride >= 0 && t.stride <= INT32_MAX;
 }
 
-Tokens tokens_of(const dk_token_array* t) {
-  return t ? Tokens{t->data, (uint32_t)t->stride, t->negated ? -1.0f : 1.0f} : Tokens{nullptr, 1, 1.0f};
+Tokens tokens_of(const dk_token_array& t) {
+  return {t.data, (uint32_t)t.stride, t.negated ? -1.0f : 1.0f};
 }
 
 bool rows_ok(int64_t n_items, int64_t rows) {
@@ -458,25 +459,27 @@ extern "C" int64_t dk_policy_loss_workspace(int64_t n_items, int64_t n_tokens) {
   return n_items <= 0 || one_group(n_items, n_tokens) ? 0 : (4 * n_items + (n_items + kWaves - 1) / kWaves) * (int64_t)sizeof(double);
 }
 
-extern "C" int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items, int64_t rows,
-                              int64_t n_tokens, const dk_token_array* logp, const dk_token_array* old,
-                              const dk_token_array* ref, const float* advantages, int per_token,
-                              double clip_low, double clip_high, double kl_coef, int reduction,
-                              double denominator, float* dlogp, float* stats, float* loss, void* ws,
-                              int64_t ws_bytes, hipStream_t stream) {
-  if (!rows_ok(n_items, rows) || !items || !row_items || !tokens_ok(logp, n_tokens) ||
-      !tokens_ok(old, n_tokens) || (ref && !tokens_ok(ref, n_tokens)) || (n_tokens > 0 && !dlogp) || !stats ||
-      !loss || (!advantages && (n_tokens > 0 || !per_token)) ||
-      !(clip_low >= 0.0 && clip_low <= 1.0) || !(clip_high >= 0.0) || !(kl_coef - kl_coef == 0.0) ||
-      (kl_coef != 0.0 && !ref) || reduction < 0 || reduction > 2 || !(denominator > 0.0))
+extern "C" int dk_policy_loss(const dk_policy_args* args, hipStream_t stream) {
+  if (!args) return DK_ERR_INVALID;
+  const dk_policy_args& a = *args;
+  const int64_t n_items = a.n_items, rows = a.rows, n_tokens = a.n_tokens;
+  if (!rows_ok(n_items, rows) || n_tokens < 0 || !a.items || !a.row_items ||
+      !tokens_ok(a.logp, n_tokens, false) || !tokens_ok(a.old, n_tokens, false) ||
+      !tokens_ok(a.ref, n_tokens, true) || (n_tokens > 0 && !a.dlogp) || !a.stats || !a.loss ||
+      (!a.advantages && (n_tokens > 0 || !a.per_token)) || !(a.clip_low >= 0.0 && a.clip_low <= 1.0) ||
+      !(a.clip_high >= 0.0) || !(a.kl_coef - a.kl_coef == 0.0) ||
+      (a.kl_coef != 0.0 && !a.ref.data && n_tokens > 0) || a.reduction < 0 || a.reduction > 2 ||
+      !(a.denominator > 0.0))
     return DK_ERR_INVALID;
-  if (!dk_aligned(items, 16) || !dk_aligned(row_items, 4)) return DK_ERR_ALIGN;
+  if (!dk_aligned(a.items, 16) || !dk_aligned(a.row_items, 4)) return DK_ERR_ALIGN;
   const int64_t need = dk_policy_loss_workspace(n_items, n_tokens);
-  if (need && (!ws || ws_bytes < need || !dk_aligned(ws, 8))) return DK_ERR_WORKSPACE;
-  PolicyParams p{reinterpret_cast<const int4*>(items), row_items, (int)n_items, (int)rows,
-                 tokens_of(logp), tokens_of(old), tokens_of(ref), advantages, per_token,
-                 log1p(-clip_low), log1p(clip_high), (float)(1.0 - clip_low), (float)(1.0 + clip_high),
-                 (float)kl_coef, reduction, 1.0 / denominator, dlogp, stats, loss, (double*)ws};
+  if (need && (!a.workspace || a.workspace_bytes < need || !dk_aligned(a.workspace, 8)))
+    return DK_ERR_WORKSPACE;
+  PolicyParams p{reinterpret_cast<const int4*>(a.items), a.row_items, (int)n_items, (int)rows,
+                 tokens_of(a.logp), tokens_of(a.old), tokens_of(a.ref), a.advantages, a.per_token != 0,
+                 log1p(-a.clip_low), log1p(a.clip_high), (float)(1.0 - a.clip_low),
+                 (float)(1.0 + a.clip_high), (float)a.kl_coef, (int)a.reduction, 1.0 / a.denominator, a.dlogp,
+                 a.stats, a.loss, (double*)a.workspace};
   if (need == 0) {
     hipLaunchKernelGGL(policy_one_kernel, dim3(1), dim3(64 * kOneWaves), 0, stream, p);
     DK_CHECK_LAUNCH();
@@ -498,27 +501,27 @@ extern "C" int64_t dk_preference_loss_workspace(int64_t n_items, int64_t n_token
   return (n_items + pair_groups(pairs)) * (int64_t)sizeof(double);
 }
 
-extern "C" int dk_preference_loss(const int32_t* items, int64_t n_items, const int32_t* row_items,
-                                  int64_t rows, int64_t n_tokens, const int32_t* row_pairs,
-                                  const int32_t* entries, const int32_t* pairs, int64_t n_pairs,
-                                  const dk_token_array* logp, const dk_token_array* ref, double beta,
-                                  int kind, double label_smoothing, double margin, int average,
-                                  float* dlogp, float* rewards, float* margins, float* loss, void* ws,
-                                  int64_t ws_bytes, hipStream_t stream) {
-  if (!rows_ok(n_items, rows) || n_pairs < 1 || n_pairs > (int64_t)1 << 28 || !items || !row_items ||
-      !row_pairs || !entries || !pairs || !tokens_ok(logp, n_tokens) || (ref && !tokens_ok(ref, n_tokens)) ||
-      (n_tokens > 0 && !dlogp) || !rewards || !margins || !loss || !(beta > 0.0) || !(1.0 / beta > 0.0) ||
-      kind < 0 || kind > 2 || !(label_smoothing >= 0.0 && label_smoothing <= 0.5) || !(margin - margin == 0.0))
+extern "C" int dk_preference_loss(const dk_preference_args* args, hipStream_t stream) {
+  if (!args) return DK_ERR_INVALID;
+  const dk_preference_args& a = *args;
+  const int64_t n_items = a.n_items, n_tokens = a.n_tokens, n_pairs = a.n_pairs;
+  if (!rows_ok(n_items, a.rows) || n_tokens < 0 || n_pairs < 1 || n_pairs > (int64_t)1 << 28 || !a.items ||
+      !a.row_items || !a.row_pairs || !a.entries || !a.pairs || !tokens_ok(a.logp, n_tokens, false) ||
+      !tokens_ok(a.ref, n_tokens, true) || (n_tokens > 0 && !a.dlogp) || !a.rewards || !a.margins || !a.loss ||
+      !(a.beta > 0.0) || !(1.0 / a.beta > 0.0) || a.kind < 0 || a.kind > 2 ||
+      !(a.label_smoothing >= 0.0 && a.label_smoothing <= 0.5) || !(a.margin - a.margin == 0.0))
     return DK_ERR_INVALID;
-  if (!dk_aligned(items, 16) || !dk_aligned(row_items, 4) || !dk_aligned(row_pairs, 4) ||
-      !dk_aligned(entries, 8) || !dk_aligned(pairs, 8))
+  if (!dk_aligned(a.items, 16) || !dk_aligned(a.row_items, 4) || !dk_aligned(a.row_pairs, 4) ||
+      !dk_aligned(a.entries, 8) || !dk_aligned(a.pairs, 8))
     return DK_ERR_ALIGN;
   const int64_t need = dk_preference_loss_workspace(n_items, n_tokens, n_pairs);
-  if (need && (!ws || ws_bytes < need || !dk_aligned(ws, 8))) return DK_ERR_WORKSPACE;
-  PrefParams p{reinterpret_cast<const int4*>(items), row_items, row_pairs,
-               reinterpret_cast<const int2*>(entries), reinterpret_cast<const int2*>(pairs), (int)n_items,
-               (int)rows, (int)n_pairs, tokens_of(logp), tokens_of(ref), beta, margin, label_smoothing, kind,
-               average, dlogp, rewards, margins, loss, (double*)ws};
+  if (need && (!a.workspace || a.workspace_bytes < need || !dk_aligned(a.workspace, 8)))
+    return DK_ERR_WORKSPACE;
+  PrefParams p{reinterpret_cast<const int4*>(a.items), a.row_items, a.row_pairs,
+               reinterpret_cast<const int2*>(a.entries), reinterpret_cast<const int2*>(a.pairs), (int)n_items,
+               (int)a.rows, (int)n_pairs, tokens_of(a.logp), tokens_of(a.ref), a.beta, a.margin,
+               a.label_smoothing, (int)a.kind, a.average != 0, a.dlogp, a.rewards, a.margins, a.loss,
+               (double*)a.workspace};
   if (need == 0) {
     hipLaunchKernelGGL(pref_one_kernel, dim3(1), dim3(64 * kOneWaves), 0, stream, p);
     DK_CHECK_LAUNCH();

@@ -109,15 +109,15 @@ def row_meta(lens, device, pairs=None):
 
 
 def _tokens(t, what, meta):
-    """A token array's C description: [n] log-probabilities, or the head's stats."""
+    """A token array's (address, stride, negated): [n] log-probabilities, or the head's stats."""
     if t is None:
-        return None
+        return 0, 0, 0
     if t.dtype != torch.float32 or t.get_device() != meta.device.index:   # (a CPU tensor's is -1)
         raise ValueError(f"{what} must be a CUDA fp32 tensor on the plan's device ({meta.device})")
     if t.dim() == 1 and t.shape[0] == meta.n_tokens:
-        return _lib.TokenArrayC(t.data_ptr(), t.stride(0), 0)
+        return t.data_ptr(), t.stride(0), 0
     if t.dim() == 2 and t.shape[0] >= meta.n_tokens and t.shape[1] == 4:
-        return _lib.TokenArrayC(t.data_ptr(), t.stride(0), 1)
+        return t.data_ptr(), t.stride(0), 1
     raise ValueError(f"{what} must be [{meta.n_tokens}] log-probabilities, or the head's stats [N, 4] with "
                      f"these tokens first (got {tuple(t.shape)})")
 
@@ -141,7 +141,7 @@ def policy_loss(logp, old, advantages, meta, *, ref=None, kl_coef=0.0, clip_low=
     if logp is None or old is None:
         raise ValueError("logp and old are needed")
     n, rows, dev = meta.n_tokens, meta.n_rows, meta.device
-    x, o, f = _tokens(logp, "logp", meta), _tokens(old, "old", meta), _tokens(ref, "ref", meta)
+    tokens = _tokens(logp, "logp", meta) + _tokens(old, "old", meta) + _tokens(ref, "ref", meta)
     if advantages.dtype != torch.float32 or advantages.device != dev or not advantages.is_contiguous() or \
             tuple(advantages.shape) != ((n,) if per_token else (rows,)):
         raise ValueError(f"advantages must be a contiguous fp32 [{n if per_token else rows}] tensor on {dev}")
@@ -151,10 +151,11 @@ def policy_loss(logp, old, advantages, meta, *, ref=None, kl_coef=0.0, clip_low=
     nbytes = meta.policy_bytes
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     which, at = REDUCTIONS.index(reduction), meta.kept()
-    _lib.launch(dev, _lib.lib().dk_policy_loss, "dk_policy_loss", at["items"], meta.n_items,
-                at["row_items"], rows, n, x, o, f, advantages.data_ptr(), per_token, clip_low, clip_high,
-                kl_coef, which, (meta.n_filled, n, 1)[which] or 1, dlogp.data_ptr(), stats.data_ptr(),
-                loss.data_ptr(), _lib.ptr(ws), nbytes)
+    args = _lib.POLICY_ARGS.pack(
+        at["items"], meta.n_items, at["row_items"], rows, n, *tokens, advantages.data_ptr(),
+        1 if per_token else 0, clip_low, clip_high, kl_coef, which, (meta.n_filled, n, 1)[which] or 1,
+        dlogp.data_ptr(), stats.data_ptr(), loss.data_ptr(), ws.data_ptr() if nbytes else 0, nbytes)
+    _lib.launch(dev, _lib.lib().dk_policy_loss, "dk_policy_loss", args)
     return loss, dlogp, stats
 
 
@@ -178,15 +179,17 @@ def preference_loss(logp, ref, meta, *, beta=0.1, kind="sigmoid", label_smoothin
     if logp is None:
         raise ValueError("logp is needed")
     n, rows, dev = meta.n_tokens, meta.n_rows, meta.device
-    x, f = _tokens(logp, "logp", meta), _tokens(ref, "ref", meta)
+    tokens = _tokens(logp, "logp", meta) + _tokens(ref, "ref", meta)
     dlogp = torch.empty(n, dtype=torch.float32, device=dev)
     rewards = torch.empty(rows, dtype=torch.float32, device=dev)
     margins = torch.empty(meta.n_pairs, dtype=torch.float32, device=dev)
     loss = torch.empty_strided((), (), dtype=torch.float32, device=dev)
     nbytes, at = meta.preference_bytes, meta.kept()
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _lib.launch(dev, _lib.lib().dk_preference_loss, "dk_preference_loss", at["items"], meta.n_items,
-                at["row_items"], rows, n, at["row_pairs"], at["entries"], at["pairs"], meta.n_pairs, x, f,
-                beta, KINDS.index(kind), label_smoothing, margin, average, dlogp.data_ptr(),
-                rewards.data_ptr(), margins.data_ptr(), loss.data_ptr(), _lib.ptr(ws), nbytes)
+    args = _lib.PREFERENCE_ARGS.pack(
+        at["items"], meta.n_items, at["row_items"], rows, n, at["row_pairs"], at["entries"], at["pairs"],
+        meta.n_pairs, *tokens, beta, KINDS.index(kind), label_smoothing, margin, 1 if average else 0,
+        dlogp.data_ptr(), rewards.data_ptr(), margins.data_ptr(), loss.data_ptr(),
+        ws.data_ptr() if nbytes else 0, nbytes)
+    _lib.launch(dev, _lib.lib().dk_preference_loss, "dk_preference_loss", args)
     return loss, dlogp, rewards, margins

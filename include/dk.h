@@ -267,26 +267,57 @@ int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* r
  *   function, e = label_smoothing in [0, 1/2];  1: max(0, 1 - h);  2: ((h - 1/2) / beta)^2.  rewards [rows] = beta S,
  *   margins [n_pairs] = h.  pairs int32 {chosen, rejected}; row r's are entries row_pairs[r] ..
  *   row_pairs[r + 1] - 1, int32 {other row, pair + 1 where r is the chosen one, else -(pair + 1)}.
- * workspace: the query's bytes, 8-byte aligned (NULL where that is 0). */
+ * workspace: the query's bytes, 8-byte aligned (NULL where that is 0).  The arguments travel in one struct of
+ * 8-byte fields. */
 typedef struct dk_token_array {
-  const float* data;
+  const float* data;   /* NULL: none (ref) */
   int64_t stride;
-  int32_t negated;
+  int64_t negated;
 } dk_token_array;
+typedef struct dk_policy_args {
+  const int32_t* items;
+  int64_t n_items;
+  const int32_t* row_items;
+  int64_t rows;
+  int64_t n_tokens;
+  dk_token_array logp, old, ref;
+  const float* advantages;
+  int64_t per_token;
+  double clip_low, clip_high, kl_coef;
+  int64_t reduction;
+  double denominator;
+  float* dlogp;
+  float* stats;
+  float* loss;
+  void* workspace;
+  int64_t workspace_bytes;
+} dk_policy_args;
 int64_t dk_policy_loss_workspace(int64_t n_items, int64_t n_tokens);
-int dk_policy_loss(const int32_t* items, int64_t n_items, const int32_t* row_items, int64_t rows,
-                   int64_t n_tokens, const dk_token_array* logp, const dk_token_array* old,
-                   const dk_token_array* ref, const float* advantages, int per_token, double clip_low,
-                   double clip_high, double kl_coef, int reduction, double denominator, float* dlogp,
-                   float* stats, float* loss, void* workspace, int64_t workspace_bytes,
-                   hipStream_t stream);
+int dk_policy_loss(const dk_policy_args* args, hipStream_t stream);
+typedef struct dk_preference_args {
+  const int32_t* items;
+  int64_t n_items;
+  const int32_t* row_items;
+  int64_t rows;
+  int64_t n_tokens;
+  const int32_t* row_pairs;
+  const int32_t* entries;
+  const int32_t* pairs;
+  int64_t n_pairs;
+  dk_token_array logp, ref;
+  double beta;
+  int64_t kind;
+  double label_smoothing, margin;
+  int64_t average;
+  float* dlogp;
+  float* rewards;
+  float* margins;
+  float* loss;
+  void* workspace;
+  int64_t workspace_bytes;
+} dk_preference_args;
 int64_t dk_preference_loss_workspace(int64_t n_items, int64_t n_tokens, int64_t n_pairs);
-int dk_preference_loss(const int32_t* items, int64_t n_items, const int32_t* row_items,
-                       int64_t rows, int64_t n_tokens, const int32_t* row_pairs,
-                       const int32_t* entries, const int32_t* pairs, int64_t n_pairs, const dk_token_array* logp,
-                       const dk_token_array* ref, double beta, int kind, double label_smoothing,
-                       double margin, int average, float* dlogp, float* rewards, float* margins,
-                       float* loss, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+int dk_preference_loss(const dk_preference_args* args, hipStream_t stream);
 
 /* The global norm of n gradient tensors, norm = scale sqrt(sum g^2) (fp32, on the device), and, with dst
  * not NULL, dst = scale min(1, max_norm / (norm + 1e-6)) src element by element (no counterpart in the

@@ -2,8 +2,8 @@
 kernels walk, and what is refused before any launch."""
 
 import ctypes
+import re
 
-import numpy as np
 import pytest
 import torch
 
@@ -112,41 +112,72 @@ def test_scoring_head_refuses_bad_arguments():
     assert call(n=0, y=None, ws=None) == 0
 
 
+def _fields(struct_name):
+    """The fields of a struct of dk.h, token arrays as three, and the format of each."""
+    text = re.sub(r"/\*.*?\*/", "", open(_lib.HEADER).read(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (struct_name, struct_name), text, re.S).group(1)
+    out = []
+    for line in filter(None, (x.strip() for x in body.split(";"))):
+        kind, names = re.match(r"((?:const )?\w+\*?) (.*)", line, re.S).groups()
+        for name in names.split(","):
+            if kind == "dk_token_array":
+                out += [(name.strip() + s, f) for s, f in (("", "Q"), ("_stride", "q"), ("_negated", "q"))]
+            else:
+                out.append((name.strip(), "Q" if kind.endswith("*") else {"int64_t": "q", "double": "d"}[kind]))
+    return out
+
+
+@pytest.mark.parametrize("name, packed", [("dk_policy_args", _lib.POLICY_ARGS),
+                                          ("dk_preference_args", _lib.PREFERENCE_ARGS)])
+def test_packed_arguments_are_the_headers_structs(name, packed):
+    fields = _fields(name)
+    assert packed.format == "".join(f for _, f in fields) and packed.size == 8 * len(fields)
+
+
 def test_loss_entries_refuse_bad_arguments():
     lib = _lib.lib()
-    p = ctypes.c_void_p(4096)
-    good = _lib.TokenArrayC(4096, 1, 0)
-    ref = ctypes.byref
+    p = 4096
 
-    def policy(items=p, n_items=100, rows=2, n=5, x=good, old=good, f=good, adv=p, low=0.2, high=0.2, kl=0.1,
-               red=0, den=2.0, out=p, ws=p, nbytes=1 << 12):
-        return lib.dk_policy_loss(items, n_items, p, rows, n, ref(x), ref(old), f and ref(f), adv, 0, low,
-                                  high, kl, red, den, out, out, out, ws, nbytes, None)
-    null, back = _lib.TokenArrayC(None, 1, 0), _lib.TokenArrayC(4096, -1, 0)
-    far = _lib.TokenArrayC(4096, 1 << 31, 0)
-    for bad in (dict(items=None), dict(n_items=0), dict(n_items=1), dict(rows=0), dict(n=-1), dict(x=null),
-                dict(old=null), dict(f=null), dict(x=back), dict(x=far), dict(adv=None), dict(low=1.1), dict(low=-0.1),
-                dict(high=-0.1), dict(high=float("nan")), dict(kl=float("inf")), dict(f=None), dict(red=3),
-                dict(red=-1), dict(den=0.0), dict(out=None)):
+    def call(entry, struct_name, packed, good, bad):
+        names = [n for n, _ in _fields(struct_name)]
+        assert set(good) <= set(names) and set(bad) <= set(names)
+        values = {**{n: p for n in names}, **good, **bad}
+        return entry(packed.pack(*(values[n] for n in names)), None)
+
+    def policy(**bad):
+        good = dict(n_items=100, rows=2, n_tokens=5, per_token=0, clip_low=0.2, clip_high=0.2, kl_coef=0.1,
+                    reduction=0, denominator=2.0, workspace_bytes=1 << 12,
+                    **{f"{t}_{k}": v for t in ("logp", "old", "ref") for k, v in (("stride", 1), ("negated", 0))})
+        return call(lib.dk_policy_loss, "dk_policy_args", _lib.POLICY_ARGS, good, bad)
+    for bad in (dict(items=0), dict(row_items=0), dict(n_items=0), dict(n_items=1), dict(rows=0),
+                dict(n_tokens=-1), dict(logp=0), dict(old=0), dict(ref=0), dict(logp_stride=-1),
+                dict(ref_stride=1 << 31), dict(advantages=0), dict(clip_low=1.1), dict(clip_low=-0.1),
+                dict(clip_high=-0.1), dict(clip_high=float("nan")), dict(kl_coef=float("inf")),
+                dict(reduction=3), dict(reduction=-1), dict(denominator=0.0), dict(dlogp=0), dict(stats=0),
+                dict(loss=0)):
         assert policy(**bad) == _lib.DK_ERR_INVALID, bad
-    assert policy(items=ctypes.c_void_p(4100)) == _lib.DK_ERR_ALIGN
+    assert lib.dk_policy_loss(None, None) == _lib.DK_ERR_INVALID
+    assert policy(items=4100) == policy(row_items=4097) == _lib.DK_ERR_ALIGN
     assert lib.dk_policy_loss_workspace(64, 1 << 15) == 0        # one workgroup
     need = lib.dk_policy_loss_workspace(100, 5)
     assert need == lib.dk_policy_loss_workspace(100, 1 << 20) > 0
-    for bad in (dict(ws=None), dict(nbytes=need - 1), dict(ws=ctypes.c_void_p(4100))):
+    for bad in (dict(workspace=0), dict(workspace_bytes=need - 1), dict(workspace=4100)):
         assert policy(**bad) == _lib.DK_ERR_WORKSPACE, bad
 
-    def preference(pairs=5000, entries=p, x=good, f=good, beta=0.1, kind=0, smooth=0.0, margin=0.0, out=p, ws=p,
-                   nbytes=1 << 12):
-        return lib.dk_preference_loss(p, 2, p, 2, 5, p, entries, p, pairs, ref(x), f and ref(f), beta, kind,
-                                      smooth, margin, 0, out, out, out, out, ws, nbytes, None)
-    for bad in (dict(pairs=0), dict(entries=None), dict(x=null), dict(f=back), dict(beta=0.0),
-                dict(beta=float("nan")), dict(kind=3), dict(smooth=0.51), dict(margin=float("nan")),
-                dict(out=None)):
+    def preference(**bad):
+        good = dict(n_items=2, rows=2, n_tokens=5, n_pairs=5000, beta=0.1, kind=0, label_smoothing=0.0,
+                    margin=0.0, average=0, workspace_bytes=1 << 16, logp_stride=1, logp_negated=0,
+                    ref_stride=1, ref_negated=0)
+        return call(lib.dk_preference_loss, "dk_preference_args", _lib.PREFERENCE_ARGS, good, bad)
+    for bad in (dict(n_pairs=0), dict(entries=0), dict(pairs=0), dict(row_pairs=0), dict(logp=0),
+                dict(ref_stride=-1), dict(beta=0.0), dict(beta=float("nan")), dict(beta=float("inf")),
+                dict(kind=3), dict(label_smoothing=0.51), dict(margin=float("nan")), dict(dlogp=0),
+                dict(rewards=0), dict(margins=0), dict(loss=0)):
         assert preference(**bad) == _lib.DK_ERR_INVALID, bad
-    assert preference(entries=ctypes.c_void_p(4100)) == _lib.DK_ERR_ALIGN
+    assert lib.dk_preference_loss(None, None) == _lib.DK_ERR_INVALID
+    assert preference(entries=4100) == preference(pairs=4100) == _lib.DK_ERR_ALIGN
     assert lib.dk_preference_loss_workspace(64, 1 << 15, 1024) == 0
-    for bad in (dict(ws=None), dict(nbytes=lib.dk_preference_loss_workspace(2, 5, 5000) - 1)):
+    for bad in (dict(workspace=0), dict(workspace_bytes=lib.dk_preference_loss_workspace(2, 5, 5000) - 1)):
         assert preference(**bad) == _lib.DK_ERR_WORKSPACE, bad
 
 
