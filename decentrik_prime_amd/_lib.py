@@ -224,7 +224,8 @@ def _bind_torch():
     global _raw_stream, _current_device
     import torch
     torch.cuda.init()
-    _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+    _current_device = torch._C._cuda_getDevice
+    _raw_stream = torch._C._cuda_getCurrentRawStream      # last: what another thread looks at first
 
 
 def stream_handle(device=None):
