@@ -7,7 +7,7 @@
 //
 // Policy, per token with advantage A:  r = e^(logp - old),  clipped where A > 0 and r > 1 + high or A < 0
 // and r < 1 - low,  p = -A r (clipped: -A times the bound),  f = ref - logp,  k = e^f - f - 1
-//   loss = sum w (p + beta k),   dlogp = w (-[not clipped] A r - beta (f + k))        (e^f - 1 = f + k)
+//   loss = sum w (p + beta k),   dlogp = w (-[not clipped] A r - beta (e^f - 1))
 // Preference, S = a row's sum (or mean) of logp - ref, h = beta (S_chosen - S_rejected) - margin:
 //   loss = mean over pairs of L(h),   dlogp of a row's tokens = sum over its pairs of +-beta L'(h) / pairs
 //
@@ -63,10 +63,18 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// e^f - f - 1.  Near 0 by its series (the terms up to f^9: the next is below 2^-34 of the sum at 1/2),
-// where the difference would leave few digits.
-__device__ __forceinline__ float expm1_minus(float f) {
-  if (fabsf(f) >= 0.5f) return (expf(f) - 1.0f) - f;
+// k = e^f - f - 1 and its slope e^f - 1.  Near 0 k by its series (the terms up to f^9: the next is below 2^-34
+// of the sum at 1/2), where the difference would leave few digits, and the slope as f + k; elsewhere k from
+// the slope, which f + k would lose behind a large k (e^f of a token that the reference all but rules out).
+struct Kl {
+  float k, slope;
+};
+
+__device__ __forceinline__ Kl kl_of(float f) {
+  if (fabsf(f) >= 0.5f) {
+    const float slope = expf(f) - 1.0f;
+    return {slope - f, slope};
+  }
   float q = 1.0f / 362880;
   q = q * f + 1.0f / 40320;
   q = q * f + 1.0f / 5040;
@@ -75,7 +83,8 @@ __device__ __forceinline__ float expm1_minus(float f) {
   q = q * f + 1.0f / 24;
   q = q * f + 1.0f / 6;
   q = q * f + 0.5f;
-  return q * f * f;
+  const float k = q * f * f;
+  return {k, f + k};
 }
 
 struct PolicyParams {
@@ -133,9 +142,9 @@ __device__ __forceinline__ double policy_item(const PolicyParams& p, const Item&
       const float pol = up ? p.high * av : down ? p.low * av : kept;
       float g = -kept, k = 0.0f;
       if (p.ref.p) {
-        const float f = (float)((double)(p.ref.sign * rf[u]) - (double)xs);
-        k = expm1_minus(f);
-        g -= p.beta * (f + k);
+        const Kl kl = kl_of((float)((double)(p.ref.sign * rf[u]) - (double)xs));
+        k = kl.k;
+        g -= p.beta * kl.slope;
       }
       p.dlogp[it.begin + t] = g * w;
       s.v[0] -= (double)pol;
@@ -325,7 +334,8 @@ __device__ __forceinline__ double pref_loss(const PrefParams& p, double h, doubl
     const double u = exp(-fabs(h)), tail = log1p(u), near = 1.0 / (1.0 + u), far = u * near;
     *slope = h < 0.0 ? p.smoothing * far - (1.0 - p.smoothing) * near
                      : p.smoothing * near - (1.0 - p.smoothing) * far;
-    return (1.0 - p.smoothing) * (fmax(-h, 0.0) + tail) + p.smoothing * (fmax(h, 0.0) + tail);
+    const double with = (1.0 - p.smoothing) * (fmax(-h, 0.0) + tail);
+    return p.smoothing == 0.0 ? with : with + p.smoothing * (fmax(h, 0.0) + tail);   // (0 times infinity is 0)
   }
   if (p.kind == 1) {
     *slope = h < 1.0 ? -1.0 : h >= 1.0 ? 0.0 : h;   // NaN stays

@@ -135,6 +135,24 @@ def test_policy_tokens_on_the_borders():
     assert torch.equal(same[1], -adv) and float(same[2][:, 2].sum()) == 0 and bool((same[2][:, 3] == 1).all())
 
 
+@pytest.mark.parametrize("rows", [1, 100])
+def test_policy_kl_far_from_the_reference(rows):
+    """The KL term's gradient e^f - 1 keeps its digits where e^f - f - 1 is large, and at infinity."""
+    from decentrik_prime_amd import k_loss
+    f = [-math.inf, -1e8, -1e5, -1000.0, -90.0, -20.0, -3.0, -0.75, -0.5, -0.4375, -2.0 ** -12, 0.0, 2.0 ** -12,
+         0.4375, 0.5, 0.75, 3.0, 20.0, 80.0]
+    n = len(f) * rows
+    ref = torch.tensor(f * rows, device="cuda")
+    x, beta = torch.zeros(n, device="cuda"), 0.125
+    meta = k_loss.row_meta([len(f)] * rows, "cuda")
+    _, dlogp, _ = k_loss.policy_loss(x, x, torch.zeros(rows, device="cuda"), meta, ref=ref, kl_coef=beta,
+                                     reduction="sum")
+    want = -beta * torch.expm1(ref.double())
+    # expf is off by up to 2 steps, the difference, f + k and the product round once each
+    assert bool(((dlogp.double() - want).abs() <= beta * U * (6 * ref.double().exp() + 4 * torch.expm1(
+        ref.double()).abs())).all())
+
+
 def test_policy_reads_stats_and_strides_and_leaves_the_rest():
     from decentrik_prime_amd import k_loss
     lens = [9, 700, 0, 31]
@@ -233,6 +251,20 @@ def test_preference_saturates_without_overflow():
     loss, dlogp, rewards, margins = k_loss.preference_loss(x, None, meta, beta=1.0)
     assert float(loss) == pytest.approx((1e4 + 1e5) / 4) and margins.tolist() == [1e4, -1e4, 1e5, -1e5]
     assert dlogp.tolist() == [0.25, -0.25, 0.25, -0.25] or dlogp.tolist() == [-(-0.25), -0.25, 0.25, -0.25]
+
+
+@pytest.mark.parametrize("rows", [2, 100])
+def test_preference_of_an_answer_ruled_out(rows):
+    """A rejected answer of probability 0: its pair's loss and slope are 0, the others' as without it."""
+    from decentrik_prime_amd import k_loss
+    x = -torch.ones(rows, device="cuda")
+    x[1] = -math.inf
+    pairs = [(0, 1)] + [(i, i + 1) for i in range(2, rows - 1)]
+    meta = k_loss.row_meta([1] * rows, "cuda", pairs=pairs)
+    loss, dlogp, rewards, margins = k_loss.preference_loss(x, None, meta, beta=0.5)
+    rest = (len(pairs) - 1) / len(pairs) * math.log(2.0)
+    assert abs(float(loss) - rest) <= 2 * U * rest and float(margins[0]) == math.inf
+    assert float(rewards[1]) == -math.inf and dlogp[:2].tolist() == [0.0, 0.0] and bool(dlogp.isfinite().all())
 
 
 def test_preference_gradient_against_differences():
