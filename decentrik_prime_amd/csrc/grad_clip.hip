@@ -9,8 +9,8 @@
 // arguments (kBatch of them a launch), so a captured call holds no pointer to host memory and the device
 // keeps no table.
 //
-// Bound: reading and writing the gradients.  233 million fp16 elements into fp32 117 + 275 us (4.0 TB/s beside
-// the write-back of the previous call's output, 5.9 without one; 5.1 TB/s, a copy's rate); 112 tensors of
+// Bound: reading and writing the gradients.  233 million fp16 elements into fp32 105 to 117 + 272 us (4.0 to
+// 4.4 TB/s beside the write-back of the previous call's output, 5.9 without one; 5.1 TB/s, a copy's rate); 112 tensors of
 // 2.2 million elements in place 4.9 + 4.2 us, and 39 us of host time for their addresses and checks.  512
 // workgroups or pieces of half the size read slower (117 and 96 us alone against 79), 2048 the same with
 // twice the sums to add up again; stores past the caches 387 -> 422 us.
@@ -240,10 +240,10 @@ extern "C" int64_t dk_grad_clip_workspace(int64_t n) {
 }
 
 extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int64_t* numel,
-                            const int32_t* types, const int32_t* dst_types, int64_t n, double max_norm, double scale, float* norm,
-                            void* ws, int64_t ws_bytes, hipStream_t stream) {
-  if (n < 1 || n > (int64_t)1 << 20 || !src || !numel || !types || (dst && !dst_types) || !norm || !(max_norm > 0.0) ||
-      !(scale > 0.0) || scale - scale != 0.0)
+                            const int32_t* types, const int32_t* dst_types, int64_t n, double max_norm,
+                            double scale, float* norm, void* ws, int64_t ws_bytes, hipStream_t stream) {
+  if (n < 1 || n > (int64_t)1 << 20 || !src || !numel || !types || (dst && !dst_types) || !norm ||
+      !(max_norm > 0.0) || !(scale > 0.0) || scale - scale != 0.0)
     return DK_ERR_INVALID;
   if (!dk_aligned(norm, 4)) return DK_ERR_ALIGN;
   for (int64_t i = 0; i < n; ++i) {

@@ -20,7 +20,7 @@
 //
 // Measured on MI355X, 151936 x 1536 (a call's two launches): one token 84 us (5.5 TB/s of E; a copy reaches
 // 5.1), 853 tokens 406, 2048 tokens 806 (1.19 PFLOP/s, at the clock that power allows; the library's product
-// alone, which writes the logits, 958 to 979); 37 tokens of 32003 x 1024 19.1 us (15.8 the walk).  Folding
+// alone, which writes the logits, 958 to 979); 37 tokens of 32003 x 1024 18.1 us (15.5 the walk).  Folding
 // takes about 4 % of a large piece, the two steps behind a tile's border nothing that shows.
 #include <utility>
 

@@ -18,8 +18,8 @@
 // Bound: latency.  Up to 64 items and 32768 tokens one workgroup does everything in one launch: 1024 tokens'
 // policy loss 4.1 us, 237 tokens' preference loss 4.0, 32 answers in 112 pairs 10.0 (in three launches 14 with
 // their gaps).  Beyond, a wave per item and a second launch for what crosses items: one million tokens'
-// policy loss 9.8 + 4.0 us (29 MB, half of them the stats' other columns; some 80 vector instructions a
-// token are a third of it), the preference loss of 1024 answers 3.6 + 6.2.  A call's host time, 10 to 13
+// policy loss 8.4 to 9.3 + 3.9 us (29 MB, half of them the stats' other columns; some 80 vector instructions
+// a token are a third of it), the preference loss of 1024 answers 3.7 + 6.2.  A call's host time, some 10
 // us, is longer than most of these.
 #include "dk_common.h"
 
@@ -466,7 +466,8 @@ static bool one_group(int64_t n_items, int64_t n_tokens) {
 }
 
 extern "C" int64_t dk_policy_loss_workspace(int64_t n_items, int64_t n_tokens) {
-  return n_items <= 0 || one_group(n_items, n_tokens) ? 0 : (4 * n_items + (n_items + kWaves - 1) / kWaves) * (int64_t)sizeof(double);
+  if (n_items <= 0 || one_group(n_items, n_tokens)) return 0;
+  return (4 * n_items + (n_items + kWaves - 1) / kWaves) * (int64_t)sizeof(double);
 }
 
 extern "C" int dk_policy_loss(const dk_policy_args* args, hipStream_t stream) {

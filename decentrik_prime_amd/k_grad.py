@@ -79,7 +79,8 @@ def _run(grads, max_norm, scale, out, in_place=False):
     norm = torch.empty_strided((), (), dtype=torch.float32, device=dev)
     _lib.launch(dev, lib.dk_grad_clip, "dk_grad_clip", src.buffer_info()[0],
                 None if dst is None else dst.buffer_info()[0], numel.buffer_info()[0],
-                types.buffer_info()[0], to.buffer_info()[0], len(grads), max_norm, scale, norm.data_ptr(), ws.data_ptr(), nbytes)
+                types.buffer_info()[0], to.buffer_info()[0], len(grads), max_norm, scale, norm.data_ptr(),
+                ws.data_ptr(), nbytes)
     return norm
 
 
