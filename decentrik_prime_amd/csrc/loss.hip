@@ -138,13 +138,14 @@ __device__ __forceinline__ double policy_item(const PolicyParams& p, const Item&
       const double d = (double)xs - (double)(p.old.sign * o[u]);
       const bool up = av > 0.0f && d > p.log_high, down = av < 0.0f && d < p.log_low;
       const float r = expf((float)d);
-      const float kept = up || down ? 0.0f : r * av;
+      // (an advantage of 0 leaves nothing of any ratio, an infinite one included; of NaN it leaves NaN)
+      const float kept = up || down || (av == 0.0f && d == d) ? 0.0f : r * av;
       const float pol = up ? p.high * av : down ? p.low * av : kept;
       float g = -kept, k = 0.0f;
       if (p.ref.p) {
         const Kl kl = kl_of((float)((double)(p.ref.sign * rf[u]) - (double)xs));
         k = kl.k;
-        g -= p.beta * kl.slope;
+        if (p.beta != 0.0f) g -= p.beta * kl.slope;   // (a reference that is watched alone: at any distance)
       }
       p.dlogp[it.begin + t] = g * w;
       s.v[0] -= (double)pol;
@@ -156,7 +157,7 @@ __device__ __forceinline__ double policy_item(const PolicyParams& p, const Item&
   s.v[2] = (double)clipped;
 #pragma unroll
   for (int q = 0; q < 4; ++q) s.v[q] = wave_sum(s.v[q]);
-  return weight * (s.v[0] + (double)p.beta * s.v[1]);
+  return weight * (p.beta != 0.0f ? s.v[0] + (double)p.beta * s.v[1] : s.v[0]);
 }
 
 __device__ __forceinline__ void store_stats(const PolicyParams& p, int64_t row, int len, const Sums& s) {

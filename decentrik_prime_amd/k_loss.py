@@ -130,7 +130,8 @@ def policy_loss(logp, old, advantages, meta, *, ref=None, kl_coef=0.0, clip_low=
     over rows (that have tokens) of their tokens' means; "token": the mean over all tokens; "sum".
     Returns (loss, dlogp [n], stats [rows, 4]): stats are a row's means of the policy term, of the KL
     estimate e^f - f - 1 (0 without ref), of clipped tokens and of r; 0 for a row without tokens.  A token
-    that lies on a border is not clipped.  All fp32."""
+    that lies on a border is not clipped.  An advantage of 0, and a kl_coef of 0, leave nothing of their
+    terms, infinite ones included.  All fp32."""
     clip_high = clip_low if clip_high is None else clip_high
     if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
         raise ValueError(f"clip_low must be within [0, 1], clip_high at least 0 (got {clip_low}, {clip_high})")

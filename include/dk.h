@@ -260,7 +260,8 @@ int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* r
  * dk_policy_loss: A the advantage of the token (per_token) or of its row, r = e^(logp - old),
  *   p = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), k = e^(ref - logp) - (ref - logp) - 1 (ref NULL: 0)
  *   loss = sum w (p + kl_coef k), dlogp = its gradient (a token on a border counts as not clipped);
- *   w = 1 / (len(row) denominator) for reduction 0, 1 / denominator for 1 and 2; clip_low in [0, 1].
+ *   w = 1 / (len(row) denominator) for reduction 0, 1 / denominator for 1 and 2; clip_low in [0, 1].  Terms with
+ *   A = 0, and with kl_coef = 0 those of k, are 0 also where r or k is infinite.
  *   stats [rows, 4]: a row's means of p, k, clipped, r (0 where it has no tokens).
  * dk_preference_loss: S = a row's sum of logp - ref (average: mean; 0 without tokens), h = beta (S_chosen -
  *   S_rejected) - margin, loss = mean over pairs of  kind 0: -(1 - e) log s(h) - e log s(-h), s the logistic

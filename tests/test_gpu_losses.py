@@ -153,6 +153,47 @@ def test_policy_kl_far_from_the_reference(rows):
         ref.double()).abs())).all())
 
 
+@pytest.mark.parametrize("rows", [1, 100])
+@pytest.mark.parametrize("reduction", ["row", "sum"])
+def test_policy_terms_without_weight_are_nothing(rows, reduction):
+    """Advantages of 0 at any ratio, and a reference that is watched alone (kl_coef 0) at any distance: both
+    terms are 0 where their exponentials pass fp32, or pass every number.  100 rows take two launches."""
+    from decentrik_prime_amd import k_loss
+    far = [100.0, 800.0, 88.75, math.inf, 1.0, 0.0]
+    n = len(far)
+    x = torch.zeros(2 * n * rows, device="cuda")
+    away = torch.tensor(far * rows, device="cuda").view(rows, n)
+    zero = torch.zeros_like(away)
+    # of each two rows the first has no advantage and far ratios, the second a far reference
+    old = torch.stack([-away, zero], 1).reshape(-1)
+    ref = torch.stack([zero, torch.where(away.isinf(), -away, away)], 1).reshape(-1)
+    adv = torch.tensor([0.0, -1.5] * rows, device="cuda")
+    meta = k_loss.row_meta([n] * (2 * rows), "cuda")
+    w = 1.0 / (2 * rows * n) if reduction == "row" else 1.0
+    loss, dlogp, stats = k_loss.policy_loss(x, old, adv, meta, ref=ref, kl_coef=0.0, reduction=reduction)
+    want = torch.stack([zero, torch.full_like(zero, 1.5 * w)], 1).reshape(-1)
+    assert bool(((dlogp - want).abs() <= 2 * U * want).all())
+    total = 1.5 * w * n * rows
+    assert abs(float(loss) - total) <= 2 * U * total
+    assert bool((stats[::2, 0] == 0).all()) and bool((stats[1::2, 0] == 1.5).all())
+    # the KL term alone: of rows without advantage at far ratios
+    loss, dlogp, _ = k_loss.policy_loss(x, old, torch.zeros_like(adv), meta, ref=torch.full_like(x, 0.25),
+                                        kl_coef=0.5, reduction=reduction)
+    slope = 0.5 * math.expm1(0.25) * w
+    assert bool(((dlogp + slope).abs() <= 8 * U * slope).all())      # (f + k and two products)
+    total = 0.5 * (math.expm1(0.25) - 0.25) * w * x.numel()
+    assert abs(float(loss) - total) <= 16 * U * total                # (a series of ten terms)
+
+
+def test_policy_of_a_token_that_is_not_a_number_stays_so():
+    """A NaN log-probability (a target outside the vocabulary) is not hidden by an advantage of 0."""
+    from decentrik_prime_amd import k_loss
+    x = torch.tensor([-1.0, math.nan, -2.0], device="cuda")
+    meta = k_loss.row_meta([3], "cuda")
+    loss, dlogp, _ = k_loss.policy_loss(x, torch.full_like(x, -1.0), torch.zeros(1, device="cuda"), meta)
+    assert math.isnan(float(loss)) and dlogp.isnan().tolist() == [False, True, False]
+
+
 def test_policy_reads_stats_and_strides_and_leaves_the_rest():
     from decentrik_prime_amd import k_loss
     lens = [9, 700, 0, 31]
