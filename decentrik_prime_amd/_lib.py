@@ -167,6 +167,8 @@ SIGNATURES = {
     "dk_preference_loss_workspace": (_i64, [_i64, _i64, _i64]),
     "dk_preference_loss": (_int, [ctypes.c_char_p, _c_p]),
     "dk_grad_clip_workspace": (_i64, [_i64]),
+    "dk_row_factors": (_int, [_c_p, _c_p, _i64, _c_p, _i64, _c_p, _c_p]),
+    "dk_grad_scale": (_int, [_c_p, _c_p, _c_p, _i64, _c_p, _f64, _c_p]),
     "dk_grad_clip": (_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _i64, _f64, _f64, _c_p, _c_p, _i64, _c_p]),
     "dk_w4_gateup_swiglu_fwd": (_int, [_c_p, _i64, _i64, _W, _c_p, _c_p, _c_p, _i64, _c_p]),
     "dk_w4_down_swiglu_bwd": (_int, [_c_p, _i64, _i64, _W, _c_p, _c_p, _i64, _c_p]),

@@ -194,17 +194,8 @@ __global__ __launch_bounds__(kThreads) void squares_kernel(Table t, uint32_t pie
   if (threadIdx.x == 0) part[blockIdx.x] = total;
 }
 
-__global__ __launch_bounds__(kThreads) void scale_kernel(Table t, uint32_t pieces, const double* part,
-                                                         int parts, double max_norm, double scale,
-                                                         float* norm_out) {
-  __shared__ double red[kThreads / 64];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
-  const double norm = scale * sqrt(block_sum(s, red));
-  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
-  const double ratio = max_norm / (norm + 1e-6);
-  // a NaN norm gives NaN; no largest norm: `scale` alone, whatever the norm
-  const float factor = (float)(scale * (ratio > 1.0 || max_norm == INFINITY ? 1.0 : ratio));
+// dst = factor src over all pieces, the last one first
+__device__ __forceinline__ void scale_pieces(const Table& t, uint32_t pieces, float factor) {
   for (uint32_t b = blockIdx.x; b < pieces; b += gridDim.x) {
     const Piece q = piece_of(t, pieces - 1 - b);
     const void* src = t.src[q.tensor];
@@ -227,6 +218,25 @@ __global__ __launch_bounds__(kThreads) void scale_kernel(Table t, uint32_t piece
   }
 }
 
+__global__ __launch_bounds__(kThreads) void scale_kernel(Table t, uint32_t pieces, const double* part,
+                                                         int parts, double max_norm, double scale,
+                                                         float* norm_out) {
+  __shared__ double red[kThreads / 64];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
+  const double norm = scale * sqrt(block_sum(s, red));
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  const double ratio = max_norm / (norm + 1e-6);
+  // a NaN norm gives NaN; no largest norm: `scale` alone, whatever the norm
+  const float factor = (float)(scale * (ratio > 1.0 || max_norm == INFINITY ? 1.0 : ratio));
+  scale_pieces(t, pieces, factor);
+}
+
+// every element times scale by[0]
+__global__ __launch_bounds__(kThreads) void times_kernel(Table t, uint32_t pieces, const float* by, double scale) {
+  scale_pieces(t, pieces, (float)(scale * (double)*by));
+}
+
 int64_t type_size(int type) {
   return type == DK_TYPE_F32 ? 4 : type == DK_TYPE_F16 || type == DK_TYPE_BF16 ? 2 : 0;
 }
@@ -239,6 +249,74 @@ extern "C" int64_t dk_grad_clip_workspace(int64_t n) {
   return n <= 0 ? 0 : (n + kBatch - 1) / kBatch * kGroups * (int64_t)sizeof(double);
 }
 
+namespace {
+
+struct Lists {
+  const void* const* src;
+  void* const* dst;            // null: nothing is written
+  const int64_t* numel;
+  const int32_t *types, *dst_types;
+  int64_t n;
+};
+
+int check_lists(const Lists& l) {
+  for (int64_t i = 0; i < l.n; ++i) {
+    const int64_t from = type_size(l.types[i]), to = l.dst ? type_size(l.dst_types[i]) : from;
+    if (!from || !to || l.numel[i] < 0 || l.numel[i] > (int64_t)1 << 40) return DK_ERR_INVALID;
+    if (l.numel[i] && (!l.src[i] || (l.dst && !l.dst[i]))) return DK_ERR_INVALID;
+    if (!dk_aligned(l.src[i], from) || (l.dst && !dk_aligned(l.dst[i], to))) return DK_ERR_ALIGN;
+    if (l.dst && l.dst[i] == l.src[i] && l.numel[i] && l.types[i] != l.dst_types[i]) return DK_ERR_INVALID;
+  }
+  if (!l.dst) return 0;
+  // what is written overlaps nothing else that is read or written: in place, its own source alone
+  struct Range {
+    uintptr_t begin, end;
+    bool write;
+  };
+  try {
+    std::vector<Range> all;
+    all.reserve(2 * l.n);
+    for (int64_t i = 0; i < l.n; ++i) {
+      if (!l.numel[i]) continue;
+      const uintptr_t s = (uintptr_t)l.src[i], d = (uintptr_t)l.dst[i];
+      all.push_back({d, d + l.numel[i] * type_size(l.dst_types[i]), true});
+      if (s != d) all.push_back({s, s + l.numel[i] * type_size(l.types[i]), false});
+    }
+    std::sort(all.begin(), all.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    uintptr_t written = 0, touched = 0;
+    for (const Range& r : all) {
+      if (r.begin < written || (r.write && r.begin < touched)) return DK_ERR_INVALID;
+      if (r.write) written = std::max(written, r.end);
+      touched = std::max(touched, r.end);
+    }
+  } catch (...) {
+    return DK_ERR_INVALID;
+  }
+  return 0;
+}
+
+// the batch of tensors from `i` on (advanced past it) and its pieces; tensors without elements skipped
+int64_t fill(const Lists& l, Table& t, int64_t& i) {
+  int64_t pieces = 0;
+  t.n = 0;
+  for (; i < l.n && t.n < kBatch; ++i) {
+    const int64_t c = (l.numel[i] + kPiece - 1) / kPiece;
+    if (pieces + c > UINT32_MAX / 2) break;
+    if (!c) continue;
+    t.src[t.n] = l.src[i];
+    t.dst[t.n] = l.dst ? l.dst[i] : nullptr;
+    t.numel[t.n] = l.numel[i];
+    t.type[t.n] = (uint8_t)(l.types[i] | (l.dst ? l.dst_types[i] : 0) << 4);
+    t.first[t.n] = (uint32_t)pieces;
+    ++t.n;
+    pieces += c;
+  }
+  t.first[t.n] = (uint32_t)pieces;
+  return pieces;
+}
+
+}  // namespace
+
 extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int64_t* numel,
                             const int32_t* types, const int32_t* dst_types, int64_t n, double max_norm,
                             double scale, float* norm, void* ws, int64_t ws_bytes, hipStream_t stream) {
@@ -246,64 +324,14 @@ extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int6
       !(max_norm > 0.0) || !(scale > 0.0) || scale - scale != 0.0)
     return DK_ERR_INVALID;
   if (!dk_aligned(norm, 4)) return DK_ERR_ALIGN;
-  for (int64_t i = 0; i < n; ++i) {
-    const int64_t from = type_size(types[i]), to = dst ? type_size(dst_types[i]) : from;
-    if (!from || !to || numel[i] < 0 || numel[i] > (int64_t)1 << 40) return DK_ERR_INVALID;
-    if (numel[i] && (!src[i] || (dst && !dst[i]))) return DK_ERR_INVALID;
-    if (!dk_aligned(src[i], from) || (dst && !dk_aligned(dst[i], to))) return DK_ERR_ALIGN;
-    if (dst && dst[i] == src[i] && numel[i] && types[i] != dst_types[i]) return DK_ERR_INVALID;
-  }
-  if (dst) {
-    // what is written overlaps nothing else that is read or written: in place, its own source alone
-    struct Range {
-      uintptr_t begin, end;
-      bool write;
-    };
-    try {
-      std::vector<Range> all;
-      all.reserve(2 * n);
-      for (int64_t i = 0; i < n; ++i) {
-        if (!numel[i]) continue;
-        const uintptr_t s = (uintptr_t)src[i], d = (uintptr_t)dst[i];
-        all.push_back({d, d + numel[i] * type_size(dst_types[i]), true});
-        if (s != d) all.push_back({s, s + numel[i] * type_size(types[i]), false});
-      }
-      std::sort(all.begin(), all.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
-      uintptr_t written = 0, touched = 0;
-      for (const Range& r : all) {
-        if (r.begin < written || (r.write && r.begin < touched)) return DK_ERR_INVALID;
-        if (r.write) written = std::max(written, r.end);
-        touched = std::max(touched, r.end);
-      }
-    } catch (...) {
-      return DK_ERR_INVALID;
-    }
-  }
+  const Lists l{src, dst, numel, types, dst_types, n};
+  if (const int rc = check_lists(l)) return rc;
   if (!ws || ws_bytes < dk_grad_clip_workspace(n) || !dk_aligned(ws, 8)) return DK_ERR_WORKSPACE;
   double* part = static_cast<double*>(ws);
   Table t;
-  // the batch of tensors from `i` on (advanced past it) and its pieces; tensors without elements skipped
-  auto fill = [&](int64_t& i) {
-    int64_t pieces = 0;
-    t.n = 0;
-    for (; i < n && t.n < kBatch; ++i) {
-      const int64_t c = (numel[i] + kPiece - 1) / kPiece;
-      if (pieces + c > UINT32_MAX / 2) break;
-      if (!c) continue;
-      t.src[t.n] = src[i];
-      t.dst[t.n] = dst ? dst[i] : nullptr;
-      t.numel[t.n] = numel[i];
-      t.type[t.n] = (uint8_t)(types[i] | (dst ? dst_types[i] : 0) << 4);
-      t.first[t.n] = (uint32_t)pieces;
-      ++t.n;
-      pieces += c;
-    }
-    t.first[t.n] = (uint32_t)pieces;
-    return pieces;
-  };
   int parts = 0;
   for (int64_t i = 0; i < n;) {
-    const int64_t pieces = fill(i);
+    const int64_t pieces = fill(l, t, i);
     if (!pieces) continue;
     const int g = groups_of(pieces);
     hipLaunchKernelGGL(squares_kernel, dim3(g), dim3(kThreads), 0, stream, t, (uint32_t)pieces, part + parts);
@@ -312,7 +340,7 @@ extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int6
   }
   bool said = false;
   for (int64_t i = 0; dst && i < n;) {
-    const int64_t pieces = fill(i);
+    const int64_t pieces = fill(l, t, i);
     if (!pieces) continue;
     hipLaunchKernelGGL(scale_kernel, dim3(groups_of(pieces)), dim3(kThreads), 0, stream, t, (uint32_t)pieces,
                        part, parts, max_norm, scale, said ? nullptr : norm);
@@ -323,6 +351,23 @@ extern "C" int dk_grad_clip(const void* const* src, void* const* dst, const int6
     t.n = 0;
     hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(kThreads), 0, stream, t, 0u, part, parts, max_norm, scale,
                        norm);
+    DK_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+extern "C" int dk_grad_scale(void* const* tensors, const int64_t* numel, const int32_t* types, int64_t n,
+                             const float* factor, double scale, hipStream_t stream) {
+  if (n < 1 || n > (int64_t)1 << 20 || !tensors || !numel || !types || !factor) return DK_ERR_INVALID;
+  if (!dk_aligned(factor, 4)) return DK_ERR_ALIGN;
+  const Lists l{(const void* const*)tensors, tensors, numel, types, types, n};
+  if (const int rc = check_lists(l)) return rc;
+  Table t;
+  for (int64_t i = 0; i < n;) {
+    const int64_t pieces = fill(l, t, i);
+    if (!pieces) continue;
+    hipLaunchKernelGGL(times_kernel, dim3(groups_of(pieces)), dim3(kThreads), 0, stream, t, (uint32_t)pieces,
+                       factor, scale);
     DK_CHECK_LAUNCH();
   }
   return 0;

@@ -445,6 +445,37 @@ __global__ __launch_bounds__(kSumThreads) void pref_loss_kernel(PrefParams p, in
   if (threadIdx.x == 0) *p.loss = (float)(total / (double)p.n_pairs);
 }
 
+// factors[rows] = 0, but -dlogp[i] / unit at row at[i]; unit is the largest power of two up to the largest
+// |dlogp| (1 where that is 0 or not finite), so the division is exact.  One workgroup: 2 us for a batch of
+// 2048 tokens.
+__global__ __launch_bounds__(kSumThreads) void row_factors_kernel(const float* __restrict__ dlogp,
+                                                                  const int32_t* __restrict__ at, int64_t n,
+                                                                  float* factors, int64_t rows, float* unit) {
+  __shared__ uint32_t red[kSumThreads / 64];
+  uint32_t top = 0;                       // |x|'s bits are in order, infinity and NaN above all numbers
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < n; i += kSumThreads) {
+    const uint32_t bits = __float_as_uint(dlogp[i]) & 0x7fffffffu;
+    top = bits > top ? bits : top;
+  }
+  for (int64_t i = threadIdx.x; i < rows; i += kSumThreads) factors[i] = 0.0f;
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) {
+    const uint32_t o = __shfl_xor(top, x);
+    top = o > top ? o : top;
+  }
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();                        // (the zeros are written, too)
+#pragma unroll
+  for (int w = 0; w < kSumThreads / 64; ++w) top = red[w] > top ? red[w] : top;
+  constexpr uint32_t inf = 0x7f800000u, least = 0x00800000u;
+  const float u = top == 0 || top >= inf ? 1.0f : __uint_as_float(top < least ? least : top & inf);
+  if (threadIdx.x == 0) *unit = u;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < n; i += kSumThreads)
+    if ((uint64_t)(int64_t)at[i] < (uint64_t)rows) factors[at[i]] = -dlogp[i] / u;
+}
+
 // a token array that is there, or (ref alone) may be absent
 bool tokens_ok(const dk_token_array& t, int64_t n, bool absent) {
   return (t.data || n == 0 || absent) && t.stride >= 0 && t.stride <= INT32_MAX;
@@ -548,5 +579,16 @@ extern "C" int dk_preference_loss(const dk_preference_args* args, hipStream_t st
     hipLaunchKernelGGL(pref_loss_kernel, dim3(1), dim3(kSumThreads), 0, stream, p, pair_wgs);
     DK_CHECK_LAUNCH();
   }
+  return 0;
+}
+
+extern "C" int dk_row_factors(const float* dlogp, const int32_t* at, int64_t n, float* factors, int64_t rows,
+                              float* unit, hipStream_t stream) {
+  if (n < 0 || rows < 0 || !unit || (n > 0 && (!dlogp || !at)) || (rows > 0 && !factors)) return DK_ERR_INVALID;
+  if (!dk_aligned(dlogp, 4) || !dk_aligned(at, 4) || !dk_aligned(factors, 4) || !dk_aligned(unit, 4))
+    return DK_ERR_ALIGN;
+  hipLaunchKernelGGL(row_factors_kernel, dim3(1), dim3(kSumThreads), 0, stream, dlogp, at, n, factors, rows,
+                     unit);
+  DK_CHECK_LAUNCH();
   return 0;
 }

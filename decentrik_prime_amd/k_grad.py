@@ -99,3 +99,18 @@ def clip_grads(grads, max_norm, *, scale=1.0, out=None):
     if not max_norm > 0.0:
         raise ValueError(f"max_norm must be positive (got {max_norm})")
     return _run(list(grads), max_norm, scale, out, in_place=out is None)
+
+
+def scale_grads(grads, factor, *, scale=1.0):
+    """Each gradient times scale * factor in place; factor: an fp32 scalar tensor on their device, which the
+    host does not wait for (the unit of k_loss.row_factors).  No tensor may overlap another."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("at least one gradient")
+    types, index = _check(grads, "gradients")
+    if factor.dtype != torch.float32 or factor.get_device() != index or factor.numel() != 1:
+        raise ValueError("factor must be an fp32 scalar on the gradients' device")
+    at = array("q", [g.data_ptr() for g in grads])        # (the host arrays live until the call returns)
+    numel = array("q", [g.nelement() for g in grads])
+    _lib.launch(torch.device("cuda", index), _lib.lib().dk_grad_scale, "dk_grad_scale", at.buffer_info()[0],
+                numel.buffer_info()[0], types.buffer_info()[0], len(grads), factor.data_ptr(), float(scale))

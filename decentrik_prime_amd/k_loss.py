@@ -13,7 +13,8 @@ Log-probabilities are fp32: [n] (any stride) as k_head.token_logprobs returns th
 stats [N >= n, 4], whose first column is their negative.  16-bit log-probabilities are refused: their
 rounding (2^-9 of a value of some units) is of the size of the clip range.  dlogp [n] is the loss's
 gradient for the log-probabilities; as the streamed head's gradient is that of the summed cross entropy,
--dlogp are the factors of its rows (k_norm.rms_backward's row_scale; model.QwenQLoRAStep.policy_step).
+-dlogp are the factors of its rows (row_factors, k_norm.rms_backward's row_scale;
+model.QwenQLoRAStep.policy_step).
 """
 
 import math
@@ -194,3 +195,24 @@ def preference_loss(logp, ref, meta, *, beta=0.1, kind="sigmoid", label_smoothin
         ws.data_ptr() if nbytes else 0, nbytes)
     _lib.launch(dev, _lib.lib().dk_preference_loss, "dk_preference_loss", args)
     return loss, dlogp, rewards, margins
+
+
+def row_factors(dlogp, rows, n):
+    """A loss's gradient dlogp [k] as factors of the head's rows (k_norm.rms_backward's row_scale): fp32 [n], 0
+    but for -dlogp / unit at rows (int32 [k], none twice; those outside are left out), and unit, the largest
+    power of two up to the largest |dlogp| (an fp32 scalar; 1 if that is 0 or not finite).  Losses that are
+    means over many tokens have gradients of 1e-4 and less, which a backward in fp16 would lose: divided by
+    unit it has the range of the cross entropy's, and k_grad.scale_grads(gradients, unit) undoes it in fp32."""
+    dev = dlogp.device
+    if dlogp.dtype != torch.float32 or dlogp.dim() != 1 or not dlogp.is_cuda:
+        raise ValueError("dlogp must be a CUDA fp32 [k] tensor")
+    if rows.dtype != torch.int32 or rows.shape != dlogp.shape or rows.device != dev or not rows.is_contiguous():
+        raise ValueError(f"rows must be a contiguous int32 [{dlogp.shape[0]}] tensor on {dev}")
+    if n < 0:
+        raise ValueError("n must be at least 0")
+    dlogp = dlogp.contiguous()
+    factors = torch.empty(n, dtype=torch.float32, device=dev)
+    unit = torch.empty_strided((), (), dtype=torch.float32, device=dev)
+    _lib.launch(dev, _lib.lib().dk_row_factors, "dk_row_factors", dlogp.data_ptr(), rows.data_ptr(),
+                dlogp.shape[0], factors.data_ptr(), n, unit.data_ptr())
+    return factors, unit

@@ -203,19 +203,20 @@ class QwenQLoRAStep(NF4LinearStack):
     def backward(self, dy_head, g_loss=1.0, dlogp=None):
         """LoRA gradients of g_loss * loss_sum: self.grads[i] = (dA_q, dB_q, dA_v, dB_v) fp32.  dlogp [n_lab]
         (fp32, sorted order): of g_loss * a loss with this gradient for the tokens' log-probabilities
-        instead (loss_sum's is -1 each)."""
+        instead (loss_sum's is -1 each); dlogp may be of any size, and g_loss is a factor in fp32 there."""
+        dh, dh16 = self.dh, self.dh16
+        row_scale, up = None, float(g_loss)
+        if dlogp is not None:
+            if dlogp.dtype != torch.float32 or tuple(dlogp.shape) != (self.n_lab,) or dlogp.device != dh.device:
+                raise ValueError(f"dlogp must be fp32 [{self.n_lab}] (the tokens with a target) on {dh.device}")
+            # the gradients between here and the adapters' are fp16: the largest factor is 1 to 2, and the
+            # adapters' fp32 gradients get the rest
+            row_scale, unit = k_loss.row_factors(dlogp, self.perm[:self.n_lab], self.m)
+            up = 1.0
         self._pass = getattr(self, "_pass", 0) + 1
         self._forward = False
         w16, side, done = self._w16, self._side, self._done
-        gscale = torch.full((1,), float(g_loss) / self.head_grad_scale, dtype=torch.float32,
-                            device=self.device)
-        dh, dh16 = self.dh, self.dh16
-        row_scale = None
-        if dlogp is not None:
-            if dlogp.dtype != torch.float32 or tuple(dlogp.shape) != (self.n_lab,):
-                raise ValueError(f"dlogp must be fp32 [{self.n_lab}] (the tokens with a target)")
-            row_scale = torch.zeros(self.m, dtype=torch.float32, device=self.device)
-            row_scale.index_copy_(0, self.labelled, -dlogp)
+        gscale = torch.full((1,), up / self.head_grad_scale, dtype=torch.float32, device=self.device)
         k_norm.rms_backward(dy_head, gscale, self.hf, self.w_final, self.rstd_f, dh, out16=dh16,
                             row_scale=row_scale)
         ks = self.keep_scale
@@ -259,6 +260,8 @@ class QwenQLoRAStep(NF4LinearStack):
                 k_norm.rms_backward(self.dx32, self.one, self.xin[i], self.w_in[i], self.rstd1[i],
                                     dh, dres=dh, out16=dh16)
             self.grads[i] = (daq, dbq, dav, dbv)
+        if dlogp is not None:
+            k_grad.scale_grads([g for layer in self.grads for g in layer], unit, scale=float(g_loss))
         return self.grads
 
     def step(self):

@@ -320,6 +320,14 @@ typedef struct dk_preference_args {
 int64_t dk_preference_loss_workspace(int64_t n_items, int64_t n_tokens, int64_t n_pairs);
 int dk_preference_loss(const dk_preference_args* args, hipStream_t stream);
 
+/* A loss's gradient for the log-probabilities of n tokens as factors of the head's rows (dk_rms_bwd_rows):
+ * factors[rows] = 0, but -dlogp[i] / unit[0] at row at[i] (int32 [n], no row twice; indices outside are left
+ * out).  unit[0] is the largest power of two up to the largest |dlogp| (1 where that is 0 or not finite): a
+ * backward in fp16 has the range that it has for the cross entropy's gradient, whatever the loss's size, and
+ * dk_grad_scale gives its results the factor back. */
+int dk_row_factors(const float* dlogp, const int32_t* at, int64_t n, float* factors, int64_t rows,
+                   float* unit, hipStream_t stream);
+
 /* The global norm of n gradient tensors, norm = scale sqrt(sum g^2) (fp32, on the device), and, with dst
  * not NULL, dst = scale min(1, max_norm / (norm + 1e-6)) src element by element (no counterpart in the
  * reference).  src, dst, numel, types and dst_types (DK_TYPE_*) are host arrays, read before the call
@@ -335,6 +343,10 @@ int64_t dk_grad_clip_workspace(int64_t n);
 int dk_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* types,
                  const int32_t* dst_types, int64_t n, double max_norm, double scale, float* norm,
                  void* workspace, int64_t workspace_bytes, hipStream_t stream);
+/* n gradient tensors (as for dk_grad_clip, none overlapping another) times scale * factor[0] in place, factor
+ * fp32 on the device. */
+int dk_grad_scale(void* const* tensors, const int64_t* numel, const int32_t* types, int64_t n,
+                  const float* factor, double scale, hipStream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * LoRA down projection with the dropout of its input.  Replaces the norm kernel's dropout lines

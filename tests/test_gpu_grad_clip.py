@@ -166,6 +166,26 @@ def test_captured_and_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(out, want[turn % 2])), turn
 
 
+@pytest.mark.parametrize("sizes", list(SIZES))
+@pytest.mark.parametrize("types", list(TYPES))
+def test_scaling_by_a_number_on_the_device(sizes, types):
+    from decentrik_prime_amd import k_grad
+    for by, scale in ((0.3, 1.0), (2.0 ** -20, -3.0), (1.0, 1.0), (0.0, 2.0), (4.0, 0.0)):
+        grads = make(SIZES[sizes], TYPES[types], seed=2)
+        want = [g.double() * float(torch.tensor(by)) * scale for g in grads]
+        k_grad.scale_grads(grads, torch.tensor(by, device="cuda"), scale=scale)
+        for g, w in zip(grads, want):
+            info = torch.finfo(g.dtype)      # the factor's and the product's rounding, and the result's own
+            tol = w.abs() * (3 * U + info.eps / 2) + info.tiny * info.eps / 2
+            assert bool(((g.double() - w).abs() <= tol).all()), (by, scale)
+    one = [torch.ones(4, device="cuda")]
+    for bad in (torch.ones(2, device="cuda"), torch.ones((), device="cuda").half(), torch.ones(())):
+        with pytest.raises(ValueError):
+            k_grad.scale_grads(one, bad)
+    with pytest.raises(ValueError):
+        k_grad.scale_grads(one + one, torch.ones((), device="cuda"))
+
+
 def test_refusals():
     from decentrik_prime_amd import k_grad
     g = torch.ones(8, 8, device="cuda")

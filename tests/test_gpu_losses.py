@@ -327,6 +327,65 @@ def test_preference_gradient_against_differences():
         assert abs(slope - float(dlogp[t])) <= 4 * U * abs(at[0][0]) / step + step * step * 0.01
 
 
+@pytest.mark.parametrize("n, rows", [(0, 0), (0, 5), (1, 1), (700, 900), (5000, 5000), (100_003, 200_000)])
+@pytest.mark.parametrize("size", [1.0, 3e-7, 2.0 ** -140, 2.0 ** 127])
+def test_row_factors(n, rows, size):
+    """Rows of a batch, in any order, get -dlogp over a power of two that leaves the largest at 1 to 2."""
+    from decentrik_prime_amd import k_loss
+    g = torch.Generator(device="cuda").manual_seed(n)
+    dlogp = (torch.rand(n, generator=g, device="cuda") * 2 - 1) * size
+    at = torch.randperm(rows, generator=g, device="cuda")[:n].int()
+    factors, unit = k_loss.row_factors(dlogp, at, rows)
+    assert factors.shape == (rows,) and unit.shape == ()
+    top, u = float(dlogp.abs().max()) if n else 0.0, float(unit)
+    assert math.frexp(u)[0] == 0.5
+    assert u == 1.0 if top == 0 else u <= top < 2 * u if top >= 2.0 ** -126 else u == 2.0 ** -126
+    want = torch.zeros(rows, device="cuda", dtype=torch.float64)
+    want[at.long()] = -dlogp.double() / u
+    # exact, but where the quotient is below fp32's smallest number
+    assert bool(((factors.double() - want).abs() <= 2.0 ** -149).all())
+    strided = torch.stack([dlogp, dlogp], 1)[:, 0]
+    assert torch.equal(k_loss.row_factors(strided, at, rows)[0], factors)
+
+
+def test_row_factors_of_what_is_not_finite_and_outside():
+    from decentrik_prime_amd import k_loss
+    at = torch.tensor([2, -1, 4, 0], dtype=torch.int32, device="cuda")
+    for bad in (math.inf, -math.inf, math.nan):
+        factors, unit = k_loss.row_factors(torch.tensor([bad, 1.0, 2.0, 0.25], device="cuda"), at, 4)
+        assert float(unit) == 1.0 and factors[[0, 1, 3]].tolist() == [-0.25, 0.0, 0.0]
+        assert torch.equal(factors[2].nan_to_num(5.0), torch.tensor(-bad, device="cuda").nan_to_num(5.0))
+    x = torch.zeros(4, device="cuda")
+    for args in ((x.double(), at, 4), (x[:3], at, 4), (x, at.long(), 4), (x, at.cpu(), 4), (x, at, -1),
+                 (x.view(2, 2), at.view(2, 2), 4)):
+        with pytest.raises(ValueError):
+            k_loss.row_factors(*args)
+
+
+def test_a_weighted_gradient_captured():
+    """The factors and the scaling replay with new gradients."""
+    from decentrik_prime_amd import k_grad, k_loss
+    at = torch.randperm(3000, device="cuda")[:2000].int()
+    first, second = torch.randn(2, 2000, device="cuda").unbind(0)
+    second = second * 1e-6
+
+    def run(v):
+        factors, unit = k_loss.row_factors(v, at, 3000)
+        out = [factors.clone(), factors[:77].clone()]
+        k_grad.scale_grads(out, unit, scale=0.5)
+        return (factors, unit, *out)
+    want = [[t.clone() for t in run(v)] for v in (first, second)]
+    graph, v = torch.cuda.CUDAGraph(), first.clone()
+    with torch.cuda.graph(graph):
+        out = run(v)
+    for turn in range(4):
+        v.copy_((first, second)[turn % 2])
+        run(second)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[turn % 2])), turn
+
+
 def test_losses_repeat_and_replay():
     """The same bits every time, captured and on another stream too."""
     from decentrik_prime_amd import k_loss

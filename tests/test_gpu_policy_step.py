@@ -107,6 +107,72 @@ def test_unit_weights_are_the_cross_entropy_step():
         st.backward(dy, dlogp=ones[1:])
 
 
+@pytest.mark.parametrize("shift", [-40, -20, -3, 30])
+def test_gradients_keep_their_digits_at_any_size_of_the_loss(shift):
+    """A loss's gradient times a power of two: the LoRA gradients times it, bit for bit."""
+    _, st = _step()
+    g = torch.Generator("cuda").manual_seed(2)
+    dlogp = torch.randn(st.n_lab, generator=g, device="cuda")
+    _, _, dy = st.forward()
+    want = [t.double() * 2.0 ** shift for layer in st.backward(dy, dlogp=dlogp) for t in layer]
+    _, _, dy = st.forward()
+    got = [t.double() for layer in st.backward(dy, dlogp=dlogp * 2.0 ** shift) for t in layer]
+    for a, b in zip(got, want):
+        assert float(b.abs().max()) > 0 and torch.equal(a, b)
+    _, _, dy = st.forward()
+    got = [t.double() for layer in st.backward(dy, 2.0 ** shift, dlogp=dlogp) for t in layer]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_small_weights_match_float64():
+    """2048 tokens in 16 answers, advantages near 1e-2 and means over rows and tokens (a token's weight is
+    near 5e-6), and a preference loss over 40 pairs with beta 0.1."""
+    from decentrik_prime_amd import k_loss, k_nf4, model, trainer
+    from oracle import model as ref
+    rng = np.random.default_rng(8)
+    groups = [(rng.integers(0, VOCAB, 65), [rng.integers(0, VOCAB, 112) for _ in range(4)]) for _ in range(4)]
+    batch = trainer.pack_answers(groups, VOCAB)
+    st = model.QwenQLoRAStep.for_batch(batch, n_layers=2, vocab=VOCAB, seed=5, head_chunk=1024)
+    assert st.m == 2064
+    lens = trainer.answer_lens(batch)
+    pairs = [(int(a), int(b)) for a, b in rng.integers(0, 16, (40, 2)) if a != b]
+    meta = k_loss.row_meta(lens, "cuda", pairs=pairs)
+    old, _ = st.score()
+    base, _ = st.score(adapters=False)
+    adv = 1e-2 * torch.randn(16, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    p = _reference_inputs(torch, st, k_nf4)
+    for which in ("policy", "preference"):
+        if which == "policy":
+            _, _, stats = st.policy_step(meta, old, adv, ref=base, kl_coef=1e-3)
+            _, dlogp, _ = k_loss.policy_loss(stats, old, adv, meta, ref=base, kl_coef=1e-3)
+        else:
+            _, _, _, stats = st.preference_step(meta, base, beta=0.1, average=True)
+            _, dlogp, _, _ = k_loss.preference_loss(stats, base, meta, beta=0.1, average=True)
+        log(f"{which}: largest weight {float(dlogp.abs().max()):.3g}")
+        assert 0 < float(dlogp.abs().max()) < 1e-3
+        weights = torch.zeros(st.m)
+        weights[st.labelled.cpu()] = -dlogp.cpu()
+        _, want = ref.qwen_step(p, st.lens, visible=_visible(batch), weights=weights)
+        _check_grads(st, want)
+
+
+def test_losses_that_are_nothing_or_not_finite():
+    """No gradient at all gives zeros, as does a batch without targets; an infinite one is not hidden."""
+    from decentrik_prime_amd import k_loss, trainer
+    batch, st = _step()
+    for dlogp in (torch.zeros(st.n_lab, device="cuda"), torch.full((st.n_lab,), np.inf, device="cuda")):
+        _, _, dy = st.forward()
+        grads = [g for layer in st.backward(dy, dlogp=dlogp) for g in layer]
+        for g in grads:
+            assert bool((g == 0).all()) if not bool(dlogp.isinf().any()) else not bool(g.isfinite().all())
+    st.use_tokens(batch.ids, torch.full_like(batch.tgt, -1))
+    meta = k_loss.row_meta([0] * batch.B, "cuda")
+    none = torch.zeros(0, device="cuda")
+    loss, rows, _ = st.policy_step(meta, none, torch.ones(batch.B, device="cuda"))
+    assert float(loss) == 0 and bool((rows == 0).all())
+    assert all(bool((g == 0).all()) for layer in st.grads for g in layer)
+
+
 @pytest.mark.parametrize("ahead", ["layer", "carried", ("gu", "d", "qkv", "o")])
 def test_score_between_forward_and_backward(ahead):
     """Scoring, with adapters and without, before a step and inside it: the step's loss and gradients stay

@@ -226,3 +226,31 @@ def test_dense_tensors():
                     (torch.zeros(1, 5).expand(3, 5), False), (torch.zeros(2, 3, 4).permute(2, 0, 1), True),
                     (torch.zeros(0, 4), True), (torch.zeros(3, 0)[:, :0], True), (torch.zeros(()), True)):
         assert k_grad._dense(t) is want, (t.shape, t.stride())
+
+
+def test_row_factors_and_scaling_refuse_bad_arguments():
+    g, t = torch.ones(4), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        k_loss.row_factors(g, t, 4)             # not on a GPU
+    with pytest.raises(ValueError):
+        k_grad.scale_grads([g], torch.ones(()))
+    with pytest.raises(ValueError):
+        k_grad.scale_grads([], torch.ones(()))
+    lib, p = _lib.lib(), 4096
+
+    def factors(dlogp=p, at=p, n=4, out=p, rows=9, unit=p):
+        return lib.dk_row_factors(dlogp, at, n, out, rows, unit, None)
+    for bad in (dict(dlogp=None), dict(at=None), dict(n=-1), dict(out=None), dict(rows=-1), dict(unit=None)):
+        assert factors(**bad) == _lib.DK_ERR_INVALID, bad
+    for bad in (dict(dlogp=4098), dict(at=4097), dict(out=4098), dict(unit=4099)):
+        assert factors(**bad) == _lib.DK_ERR_ALIGN, bad
+
+    def scale(at, numel, types, factor=p):
+        n = len(at)
+        return lib.dk_grad_scale((ctypes.c_int64 * n)(*at), (ctypes.c_int64 * n)(*numel),
+                                 (ctypes.c_int32 * n)(*types), n, factor, 1.0, None)
+    a, f32 = 1 << 20, _lib.DK_TYPE_F32
+    for bad in (([], [], []), ([0], [4], [f32]), ([a], [-1], [f32]), ([a], [4], [0]), ([a, a], [4, 4], [f32, f32]),
+                ([a, a + 8], [4, 4], [f32, f32]), ([a], [4], [f32], None)):
+        assert scale(*bad) == _lib.DK_ERR_INVALID, bad
+    assert scale([a + 2], [4], [f32]) == scale([a], [4], [f32], p + 2) == _lib.DK_ERR_ALIGN
