@@ -505,10 +505,9 @@ extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const
     return DK_ERR_INVALID;
   if (n == 0) return 0;
   if (!y || !emb || !tgt || !logp || !entropy || !lse || total == 0) return DK_ERR_INVALID;
-  // 32-bit byte offsets: a tile's rows of y, or all of y where rows are picked from it
-  if (((rows ? total : 256) * ldy + d) * (int64_t)sizeof(f16) >= (int64_t)1 << 32 ||
-      256 * d * (int64_t)sizeof(f16) >= (int64_t)1 << 32)
-    return DK_ERR_INVALID;
+  // 32-bit byte offsets: of a tile's rows of y, or of all of y where rows are picked from it
+  const int64_t reach = rows ? total : n < 256 ? n : 256;
+  if (reach > 1 && ldy > (((int64_t)1 << 31) - 1 - d) / (reach - 1)) return DK_ERR_INVALID;
   if (!dk_aligned(y, 16) || !dk_aligned(emb, 16) || !dk_aligned(tgt, 4) || !dk_aligned(rows, 4) ||
       !dk_aligned(logp, 4) || !dk_aligned(entropy, 4) || !dk_aligned(lse, 4))
     return DK_ERR_ALIGN;

@@ -21,6 +21,7 @@ STATE_W = 8          # per-row running state: m, s, t, argmax, x_target, (pad)
 CHUNK = 32768        # vocabulary rows per chunk (a multiple of 64): at 2048 tokens a 134 MB
                      # logits buffer; measured 2.81 / 2.49 / 2.45 ms per full-vocabulary call at
                      # 8192 / 16384 / 32768 (fewer split-K reduces and launches per call)
+OFFSETS = 1 << 31    # elements of yf that the scoring head's offsets reach
 
 
 class ResidentEmbedding:
@@ -167,12 +168,22 @@ def token_logprobs(yf, emb, tgt, *, rows=None, scale=1.0):
         raise ValueError("rows of an empty yf")
     if total == 1 and (yf.stride(1) != 1 or yf.stride(0) < d or yf.stride(0) % 8):
         yf = yf.reshape(d).clone().view(1, d)
-    if rows is not None and total * yf.stride(0) >= 1 << 31:
-        # the kernel's row offsets are 32 bits wide: the picked rows alone (an index outside stays one)
-        inside = (rows >= 0) & (rows < total)
-        yf = yf.index_select(0, torch.where(inside, rows, 0))
-        rows = torch.where(inside, torch.arange(n, dtype=torch.int32, device=dev), -1)
-        total = n
+    # the kernel's row offsets are 32 bits wide, over all of yf or (without rows) over 256 rows
+    if ((total if rows is not None else min(total, 256)) - 1) * yf.stride(0) + d >= OFFSETS:
+        if rows is None:
+            yf = yf.contiguous()
+        elif n > (OFFSETS - 1) // d:
+            for i in range(0, n, (OFFSETS - 1) // d):
+                part = slice(i, i + (OFFSETS - 1) // d)
+                for whole, piece in zip((logp, entropy, lse),
+                                        token_logprobs(yf, emb, tgt[part], rows=rows[part], scale=scale)):
+                    whole[part] = piece
+            return logp, entropy, lse
+        else:                  # the picked rows alone (an index outside stays one)
+            inside = (rows >= 0) & (rows < total)
+            yf = yf.index_select(0, torch.where(inside, rows, 0))
+            rows = torch.where(inside, torch.arange(n, dtype=torch.int32, device=dev), -1)
+            total = n
     lib = _lib.lib()
     vocab = emb.shape[0]
     nbytes = _needed(("logprobs", n, vocab, d), lambda: lib.dk_head_logprobs_workspace(n, vocab, d))

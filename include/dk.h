@@ -238,9 +238,9 @@ int dk_head_finalize(const float* state, const int32_t* tgt_sorted, const int32_
  * counterpart in the reference): x_v = scale <y_i, E_v>, lse = log sum_v e^(x_v), logp = x_tgt - lse,
  * entropy = lse - sum_v p_v x_v, i over the n given rows of y (rows int32 [n], indices below total, or NULL:
  * rows 0 .. n - 1).  y fp16 with row stride ldy (a multiple of 8) and emb fp16 [vocab, d] contiguous, both
- * 16-byte aligned; d a multiple of 64 up to 2^20, n and vocab up to 2^30; with rows, total * ldy below
- * 2^31 elements; 0 < scale <= 10^6.  tgt int32 [n]: below 0 gives logp 0, vocab or more
- * NaN; a row index outside [0, total) NaN throughout.  logp, entropy, lse fp32 [n].  workspace:
+ * 16-byte aligned; d a multiple of 64 up to 2^20, n and vocab up to 2^30; the last row's end, (total - 1) ldy + d,
+ * below 2^31 elements with rows, (min(n, 256) - 1) ldy + d without; 0 < scale <= 10^6.  tgt int32 [n]: below 0
+ * gives logp 0, vocab or more NaN; a row index outside [0, total) NaN throughout.  logp, entropy, lse fp32 [n].  workspace:
  * dk_head_logprobs_workspace bytes, 16-byte aligned. */
 int64_t dk_head_logprobs_workspace(int64_t n, int64_t vocab, int64_t d);
 int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* rows, int64_t n,

@@ -162,6 +162,46 @@ def test_embedding_and_rows_past_4_gib():
     assert all(bool(torch.isnan(g[2])) for g in got)
 
 
+@pytest.mark.parametrize("n, stride", [(200, 1 << 24), (2, 1 << 31), (300, 1 << 23)])
+def test_rows_far_apart(n, stride):
+    """Rows whose offsets within 256 of them pass 32 bits, and rows at the last stride that does not."""
+    from decentrik_prime_amd import k_head
+    y, e, tgt = inputs(n, 500, 64, seed=n)
+    wide = torch.empty((n - 1) * stride + 64, dtype=torch.float16, device="cuda").as_strided((n, 64), (stride, 1))
+    wide.copy_(y)
+    for a, b in zip(k_head.token_logprobs(wide, e, tgt), k_head.token_logprobs(y, e, tgt)):
+        assert torch.equal(a, b)
+    rows = torch.randint(0, n, (77,), dtype=torch.int32, device="cuda")
+    rows[5] = n
+    tgt = torch.randint(0, 500, (77,), dtype=torch.int32, device="cuda")
+    for a, b in zip(k_head.token_logprobs(wide, e, tgt, rows=rows), k_head.token_logprobs(y, e, tgt, rows=rows)):
+        assert torch.equal(a.nan_to_num(nan=5.0), b.nan_to_num(nan=5.0)) and bool(a[5].isnan())
+
+
+def some_rows(n, around):
+    """The first and last tokens, those around given ones, and 500 more."""
+    near = torch.cat([torch.arange(max(0, a - 3), min(n, a + 3)) for a in (0, n - 1, *around)])
+    return torch.cat([near, torch.randint(0, n, (500,), generator=torch.Generator().manual_seed(1))]).cuda()
+
+
+def test_picked_rows_of_more_than_2_to_the_31_elements():
+    """Rows picked from 4 GiB of hidden states, more of them than 32-bit offsets reach."""
+    from decentrik_prime_amd import k_head
+    total, n = (1 << 25) + 8, (1 << 25) + 1000
+    _, e, _ = inputs(1, 7, 64, seed=1)
+    y = torch.randn(1 << 12, 64, device="cuda").half().repeat((total >> 12) + 1, 1)[:total]
+    rows = (torch.arange(n, device="cuda", dtype=torch.int64) * 7 % total).int()
+    rows[1 << 20], rows[n - 2] = total, -1
+    tgt = (torch.arange(n, device="cuda") % 7).int()
+    got = k_head.token_logprobs(y, e, tgt, rows=rows)
+    some = some_rows(n, [(1 << 25) - 1])
+    some = some[(rows[some] >= 0) & (rows[some] < total)]
+    check([g[some] for g in got], *definition(y[rows[some].long()], e, tgt[some], 1.0))
+    for g in got:
+        bad = torch.nonzero(~g.isfinite())[:, 0]
+        assert bad.tolist() == [1 << 20, n - 2]
+
+
 def test_captured_and_on_another_stream():
     from decentrik_prime_amd import k_head
     y, e, tgt = inputs(300, 20000, 128)

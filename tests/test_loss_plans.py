@@ -112,6 +112,25 @@ def test_scoring_head_refuses_bad_arguments():
     assert call(n=0, y=None, ws=None) == 0
 
 
+@pytest.mark.parametrize("d, most", [(64, 1 << 25), (1536, (1 << 31) // 1536 + 1), (2048, 1 << 20)])
+def test_scoring_head_takes_rows_up_to_32_bits_of_offsets(d, most):
+    """The last row's end is what counts: below 2^31 elements with `rows`, within a tile of 256 without."""
+    lib, p = _lib.lib(), ctypes.c_void_p(4096)
+
+    def call(total, n=2, ldy=d, rows=p):           # (a workspace of 0 bytes: the next refusal, before any launch)
+        return lib.dk_head_logprobs(p, ldy, total, rows, n, p, 8, d, p, 1.0, p, p, p, p, 0, None)
+    assert call(most) == _lib.DK_ERR_INVALID
+    assert call(most - 1) == _lib.DK_ERR_WORKSPACE
+    assert call(2, ldy=(1 << 31) - d) == _lib.DK_ERR_INVALID
+    assert call(2, ldy=(1 << 31) - d - 8) == _lib.DK_ERR_WORKSPACE
+    assert call(1, ldy=1 << 40) == _lib.DK_ERR_WORKSPACE
+    assert call(1 << 62, ldy=1 << 40) == call(1 << 62, n=1 << 20, ldy=1 << 40, rows=None) == _lib.DK_ERR_INVALID
+    for n, ldy, fits in ((128, 1 << 24, True), (129, 1 << 24, False), (1000, 1 << 23, True),
+                         (1000, (1 << 23) + (1 << 16), False), (2, (1 << 31) - d, False), (1, 1 << 40, True)):
+        want = _lib.DK_ERR_WORKSPACE if fits else _lib.DK_ERR_INVALID
+        assert call(1 << 20, n, ldy, None) == want, (n, ldy)
+
+
 def _fields(struct_name):
     """The fields of a struct of dk.h, token arrays as three, and the format of each."""
     text = re.sub(r"/\*.*?\*/", "", open(_lib.HEADER).read(), flags=re.S)
