@@ -22,6 +22,7 @@
 // 5.1), 853 tokens 406, 2048 tokens 806 (1.19 PFLOP/s, at the clock that power allows; the library's product
 // alone, which writes the logits, 958 to 979); 37 tokens of 32003 x 1024 18.1 us (15.5 the walk).  Folding
 // takes about 4 % of a large piece, the two steps behind a tile's border nothing that shows.
+#include <algorithm>
 #include <utility>
 
 #include "dk_common.h"
@@ -480,6 +481,11 @@ int64_t lp_states(const LpPlan& pl, int64_t n) {
   return pl.tail ? whole * pl.runs + (n - whole) * pl.tail : n * pl.runs;
 }
 
+// Tokens of a launch: a wave per token in the join, and 2^32 work items are more than a launch takes
+constexpr int64_t kLpSlice = (int64_t)1 << 24;
+
+int64_t lp_bytes(int64_t n, int64_t V, int64_t D) { return 16 * lp_states(lp_plan(n, V, D), n) + 4 * n; }
+
 bool lp_sizes_ok(int64_t n, int64_t V, int64_t D) {
   // the grid, 32-bit pieces and steps, and 32-bit offsets inside a piece of E
   return n >= 0 && n <= (int64_t)1 << 30 && V >= 1 && V <= (int64_t)1 << 30 && D >= kLpBK &&
@@ -493,7 +499,9 @@ using namespace dk;
 
 extern "C" int64_t dk_head_logprobs_workspace(int64_t n, int64_t vocab, int64_t d) {
   if (n <= 0 || !lp_sizes_ok(n, vocab, d)) return 0;
-  return 16 * lp_states(lp_plan(n, vocab, d), n) + 4 * n;
+  if (n <= kLpSlice) return lp_bytes(n, vocab, d);
+  const int64_t whole = lp_bytes(kLpSlice, vocab, d), rest = n % kLpSlice;
+  return rest ? std::max(whole, lp_bytes(rest, vocab, d)) : whole;
 }
 
 extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* rows, int64_t n,
@@ -513,23 +521,26 @@ extern "C" int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const
     return DK_ERR_ALIGN;
   if (!ws || ws_bytes < dk_head_logprobs_workspace(n, vocab, d) || !dk_aligned(ws, 16))
     return DK_ERR_WORKSPACE;
-  const LpPlan pl = lp_plan(n, vocab, d);
-  LpParams p{(const f16*)y, ldy, rows, total, (const f16*)emb, tgt, n, vocab, d, scale * kLog2e, pl,
-             (float*)ws, (float*)ws + 4 * lp_states(pl, n)};
-  const dim3 grid((unsigned)(pl.tiles * pl.runs + pl.tail)), block(kLpThreads);
-  if (pl.bm == 64)
-    hipLaunchKernelGGL((head_logp_kernel<64, 128, 2, 6, false>), grid, block, 0, stream, p);
-  else if (pl.bm == 128 && pl.bn == 128)
-    hipLaunchKernelGGL((head_logp_kernel<128, 128, 4, 4, false>), grid, block, 0, stream, p);
-  else if (pl.bm == 128)
-    hipLaunchKernelGGL((head_logp_kernel<128, 256, 2, 3, false>), grid, block, 0, stream, p);
-  else if (pl.tail == 0)
-    hipLaunchKernelGGL((head_logp_kernel<256, 256, 2, 2, false>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((head_logp_kernel<256, 256, 2, 2, true>), grid, block, 0, stream, p);
-  DK_CHECK_LAUNCH();
-  hipLaunchKernelGGL(head_logp_join_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, p, logp,
-                     entropy, lse);
-  DK_CHECK_LAUNCH();
+  for (int64_t i = 0; i < n; i += kLpSlice) {
+    const int64_t m = n - i < kLpSlice ? n - i : kLpSlice;
+    const LpPlan pl = lp_plan(m, vocab, d);
+    LpParams p{(const f16*)y + (rows ? 0 : i * ldy), ldy, rows ? rows + i : nullptr, total, (const f16*)emb,
+               tgt + i, m, vocab, d, scale * kLog2e, pl, (float*)ws, (float*)ws + 4 * lp_states(pl, m)};
+    const dim3 grid((unsigned)(pl.tiles * pl.runs + pl.tail)), block(kLpThreads);
+    if (pl.bm == 64)
+      hipLaunchKernelGGL((head_logp_kernel<64, 128, 2, 6, false>), grid, block, 0, stream, p);
+    else if (pl.bm == 128 && pl.bn == 128)
+      hipLaunchKernelGGL((head_logp_kernel<128, 128, 4, 4, false>), grid, block, 0, stream, p);
+    else if (pl.bm == 128)
+      hipLaunchKernelGGL((head_logp_kernel<128, 256, 2, 3, false>), grid, block, 0, stream, p);
+    else if (pl.tail == 0)
+      hipLaunchKernelGGL((head_logp_kernel<256, 256, 2, 2, false>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((head_logp_kernel<256, 256, 2, 2, true>), grid, block, 0, stream, p);
+    DK_CHECK_LAUNCH();
+    hipLaunchKernelGGL(head_logp_join_kernel, dim3((unsigned)((m + 3) / 4)), dim3(256), 0, stream, p, logp + i,
+                       entropy + i, lse + i);
+    DK_CHECK_LAUNCH();
+  }
   return 0;
 }

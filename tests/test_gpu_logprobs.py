@@ -202,6 +202,19 @@ def test_picked_rows_of_more_than_2_to_the_31_elements():
         assert bad.tolist() == [1 << 20, n - 2]
 
 
+def test_more_tokens_than_a_launch_takes():
+    """2^26 tokens and some: a wave each would be 2^32 work items in one launch."""
+    from decentrik_prime_amd import k_head
+    n = (1 << 26) + 70
+    _, e, _ = inputs(1, 5, 64, seed=2)
+    y = torch.randn(1 << 12, 64, device="cuda").half().repeat((n >> 12) + 1, 1)[:n]
+    tgt = (torch.arange(n, device="cuda") % 5).int()
+    got = k_head.token_logprobs(y, e, tgt)
+    some = some_rows(n, [1 << 24, 1 << 25, 3 << 24, 1 << 26])
+    check([g[some] for g in got], *definition(y[some], e, tgt[some], 1.0))
+    assert all(bool(g.isfinite().all()) for g in got)
+
+
 def test_captured_and_on_another_stream():
     from decentrik_prime_amd import k_head
     y, e, tgt = inputs(300, 20000, 128)

@@ -131,6 +131,15 @@ def test_scoring_head_takes_rows_up_to_32_bits_of_offsets(d, most):
         assert call(1 << 20, n, ldy, None) == want, (n, ldy)
 
 
+def test_scoring_head_takes_many_tokens_in_launches_of_2_to_the_24():
+    """Their waves stay below 2^32 work items; the scratch memory is one launch's."""
+    need = _lib.lib().dk_head_logprobs_workspace
+    one = need(1 << 24, 8, 64)
+    assert one >= 20 << 24
+    for n in ((1 << 24) + 1, 1 << 26, (1 << 26) + 70, (1 << 30) - 5, 1 << 30):
+        assert need(n, 8, 64) == one
+
+
 def _fields(struct_name):
     """The fields of a struct of dk.h, token arrays as three, and the format of each."""
     text = re.sub(r"/\*.*?\*/", "", open(_lib.HEADER).read(), flags=re.S)
