@@ -485,8 +485,9 @@ Tokens tokens_of(const dk_token_array& t) {
   return {t.data, (uint32_t)t.stride, t.negated ? -1.0f : 1.0f};
 }
 
+// (a wave per item, and kSumThreads per 16 rows: 2^32 work items are more than a launch takes)
 bool rows_ok(int64_t n_items, int64_t rows) {
-  return rows >= 1 && rows <= n_items && n_items <= (int64_t)1 << 28;
+  return rows >= 1 && rows <= n_items && n_items <= (int64_t)1 << 25;
 }
 
 }  // namespace

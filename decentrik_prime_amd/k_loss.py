@@ -26,6 +26,7 @@ from . import _lib
 
 ITEM_TOKENS = 512    # tokens that a wave takes; longer rows than ROW_ITEMS of these in larger items
 ROW_ITEMS = 64
+MAX_ITEMS = 1 << 25  # a wave each: 2^32 work items are more than a launch takes
 REDUCTIONS = ("row", "token", "sum")
 KINDS = ("sigmoid", "hinge", "ipo")
 
@@ -45,7 +46,7 @@ class RowMeta:
     def __init__(self, lens, device, pairs=None):
         size = _whole(lens, "lens", ())
         rows = size.size
-        if rows == 0 or rows > 1 << 26 or size.min() < 0 or size.max() > 1 << 30:
+        if rows == 0 or size.min() < 0 or size.max() > 1 << 30:
             raise ValueError("at least one row, each of 0 to 2^30 tokens")
         self.n_rows, self.n_tokens = int(rows), int(size.sum())
         self.n_filled = int(np.count_nonzero(size))
@@ -53,6 +54,9 @@ class RowMeta:
         count = np.maximum(1, -(-size // step))
         last = np.cumsum(count)
         n = self.n_items = int(last[-1])
+        if n > MAX_ITEMS:
+            raise ValueError(f"a plan takes up to 2^25 items (here {n}: one for each {ITEM_TOKENS} tokens of a row, "
+                             f"up to {ROW_ITEMS} a row, and at least one a row)")
         self.n_pairs = None
         both = None
         if pairs is not None:
@@ -104,8 +108,8 @@ class RowMeta:
 
 
 def row_meta(lens, device, pairs=None):
-    """The plan of a batch with rows of `lens` tokens (zeros allowed), and for preference_loss of the
-    pairs (chosen row, rejected row); a row may be in any number of pairs."""
+    """The plan of a batch with rows of `lens` tokens (zeros allowed, 2^25 rows at most), and for
+    preference_loss of the pairs (chosen row, rejected row); a row may be in any number of pairs."""
     return RowMeta(lens, device, pairs)
 
 

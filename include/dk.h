@@ -252,8 +252,8 @@ int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* r
  * Losses over the tokens' log-probabilities of a packed batch of answers, with their gradients (no
  * counterpart in the reference).  The batch is `rows` rows of consecutive tokens cut into items {first token
  * (low, high word), tokens, row, the row's tokens, the row's items, the item's place among them, 0} (int32
- * [n_items, 8], 16-byte aligned, row by row and in token order; a row has 1 to 64 items and at most 2^30
- * tokens, an empty row one item without tokens); row r's items are row_items[r] .. row_items[r + 1] - 1.  A
+ * [n_items, 8], 16-byte aligned, row by row and in token order; n_items up to 2^25; a row has 1 to 64 items and
+ * at most 2^30 tokens, an empty row one item without tokens); row r's items are row_items[r] .. row_items[r + 1] - 1.  A
  * token array is fp32 with an element stride (0 to 2^31 - 1), negated where it holds losses (the head's stats:
  * column 0, stride 4).  With n_tokens = 0 the token arrays may be NULL.
  *

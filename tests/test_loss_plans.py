@@ -71,6 +71,22 @@ def test_plans_refuse_what_they_cannot_hold():
             k_loss.row_meta([1, 2], "cpu", pairs=pairs)
 
 
+def test_plans_hold_what_a_launch_takes():
+    """2^25 items: their waves stay below 2^32 work items."""
+    import numpy as np
+    for lens in (np.zeros((1 << 25) + 1, np.int8), np.full((1 << 19) + 1, 1 << 30)):
+        with pytest.raises(ValueError, match="items"):
+            k_loss.row_meta(lens, "cpu")
+    lib = _lib.lib()
+    for entry, struct_name, packed in ((lib.dk_policy_loss, "dk_policy_args", _lib.POLICY_ARGS),
+                                       (lib.dk_preference_loss, "dk_preference_args", _lib.PREFERENCE_ARGS)):
+        fields = _fields(struct_name)
+        for n, want in ((1 << 25, _lib.DK_ERR_WORKSPACE), ((1 << 25) + 1, _lib.DK_ERR_INVALID)):
+            values = {name: 4096 if f == "Q" else 0.25 if f == "d" else 1 for name, f in fields}
+            values.update(n_items=n, rows=1 << 20, n_tokens=5, workspace_bytes=0)
+            assert entry(packed.pack(*(values[name] for name, _ in fields)), None) == want
+
+
 def test_losses_refuse_bad_arguments():
     meta = k_loss.row_meta([2, 3], "cpu", pairs=[(0, 1)])
     x, a = torch.zeros(5), torch.zeros(2)
