@@ -12,8 +12,8 @@
 //   loss = mean over pairs of L(h),   dlogp of a row's tokens = sum over its pairs of +-beta L'(h) / pairs
 //
 // Differences of log-probabilities and the clip's borders are formed in 64 bits (a token within rounding
-// of a border would gain or lose its whole gradient), exponentials in 32, sums over tokens in 64 and in an
-// order that the sizes alone give.
+// of a border would gain or lose its whole gradient), exponentials in 32 (in 64 where they would pass that),
+// sums over tokens in 64 and in an order that the sizes alone give.
 //
 // Bound: latency.  Up to 64 items and 32768 tokens one workgroup does everything in one launch: 1024 tokens'
 // policy loss 4.1 us, 237 tokens' preference loss 4.0, 32 answers in 112 pairs 10.0 (in three launches 14 with
@@ -109,6 +109,72 @@ struct Sums {
   double v[4];
 };
 
+// One token in 32 bits: its slope for logp (before the weight), p, k, r and whether it is clipped
+struct PolicyTerms {
+  float g, pol, k, r;
+  bool cut;
+};
+
+__device__ __forceinline__ PolicyTerms policy_token(const PolicyParams& p, double d, double f, float av) {
+  const bool up = av > 0.0f && d > p.log_high, down = av < 0.0f && d < p.log_low;
+  const float r = expf((float)d);
+  // (an advantage of 0 leaves nothing of any ratio, an infinite one included; of NaN it leaves NaN)
+  const float kept = up || down || (av == 0.0f && d == d) ? 0.0f : r * av;
+  PolicyTerms o{-kept, up ? p.high * av : down ? p.low * av : kept, 0.0f, r, up || down};
+  if (p.ref.p) {
+    const Kl kl = kl_of((float)f);
+    o.k = kl.k;
+    if (p.beta != 0.0f) o.g -= p.beta * kl.slope;   // (a reference that is watched alone: at any distance)
+  }
+  return o;
+}
+
+// e^d or e^f past 10^26 is formed in 64 bits: its product with a small advantage, weight or kl_coef may be an
+// ordinary number where fp32 has only infinity.  A lane does its tokens of an item again when its sums say
+// that there is one; the others come out as before.
+constexpr double kFar = 60.0, kFarSum = 1e30;
+
+__device__ __forceinline__ void policy_again(const PolicyParams& p, const Item& it, double weight, Sums& s,
+                                             int& clipped) {
+  const float *xp = p.logp.from(it.begin), *op = p.old.from(it.begin);
+  const float* rp = p.ref.p ? p.ref.from(it.begin) : xp;
+  s = Sums{};
+  clipped = 0;
+#pragma unroll 1
+  for (int t = threadIdx.x & 63; t < it.count; t += 64) {
+    const double x = (double)(p.logp.sign * p.logp.at(xp, t));
+    const double d = x - (double)(p.old.sign * p.old.at(op, t));
+    const double f = p.ref.p ? (double)(p.ref.sign * p.ref.at(rp, t)) - x : 0.0;
+    const float av = p.adv_per_token ? p.adv[it.begin + t] : p.adv[it.row];
+    const PolicyTerms o = policy_token(p, d, f, av);
+    double pol = (double)o.pol, k = (double)o.k, r = (double)o.r;
+    if (d > kFar || f > kFar) {
+      double e[2] = {d, f};
+#pragma unroll 1
+      for (int q = 0; q < 2; ++q) {             // (one copy of the exponential: it holds many registers)
+        const double v = exp(e[0]);
+        e[0] = e[1];
+        e[1] = v;
+      }
+      r = e[0];
+      const double kept = o.cut || (av == 0.0f && d == d) ? 0.0 : r * (double)av;
+      pol = o.cut ? pol : kept;
+      double g = -kept;
+      if (p.ref.p) {
+        // (there e^f - f - 1 and e^f - 1 are e^f but for its last digits, and f may be infinite)
+        const double slope = f > kFar ? e[1] : (double)kl_of((float)f).slope;
+        k = f > kFar ? e[1] : k;
+        if (p.beta != 0.0f) g -= (double)p.beta * slope;
+      }
+      p.dlogp[it.begin + t] = (float)(g * weight);
+    }
+    s.v[0] -= pol;
+    s.v[1] += k;
+    clipped += o.cut;
+    s.v[3] += r;
+  }
+}
+
 // One item: dlogp, and the sums of p, k, clipped and r.  Returns its share of the loss.
 __device__ __forceinline__ double policy_item(const PolicyParams& p, const Item& it, Sums& s) {
   const int lane = threadIdx.x & 63;
@@ -134,26 +200,17 @@ __device__ __forceinline__ double policy_item(const PolicyParams& p, const Item&
     for (int u = 0; u < kAhead; ++u) {
       const int t = t0 + 64 * u + lane;
       if (t >= it.count) continue;
-      const float xs = p.logp.sign * x[u], av = a[u];
-      const double d = (double)xs - (double)(p.old.sign * o[u]);
-      const bool up = av > 0.0f && d > p.log_high, down = av < 0.0f && d < p.log_low;
-      const float r = expf((float)d);
-      // (an advantage of 0 leaves nothing of any ratio, an infinite one included; of NaN it leaves NaN)
-      const float kept = up || down || (av == 0.0f && d == d) ? 0.0f : r * av;
-      const float pol = up ? p.high * av : down ? p.low * av : kept;
-      float g = -kept, k = 0.0f;
-      if (p.ref.p) {
-        const Kl kl = kl_of((float)((double)(p.ref.sign * rf[u]) - (double)xs));
-        k = kl.k;
-        if (p.beta != 0.0f) g -= p.beta * kl.slope;   // (a reference that is watched alone: at any distance)
-      }
-      p.dlogp[it.begin + t] = g * w;
-      s.v[0] -= (double)pol;
-      s.v[1] += (double)k;
-      clipped += up || down;
-      s.v[3] += (double)r;
+      const double xs = (double)(p.logp.sign * x[u]);
+      const PolicyTerms v = policy_token(p, xs - (double)(p.old.sign * o[u]),
+                                         (double)(p.ref.sign * rf[u]) - xs, a[u]);
+      p.dlogp[it.begin + t] = v.g * w;
+      s.v[0] -= (double)v.pol;
+      s.v[1] += (double)v.k;
+      clipped += v.cut;
+      s.v[3] += (double)v.r;
     }
   }
+  if (!(s.v[1] + s.v[3] < kFarSum)) policy_again(p, it, weight, s, clipped);
   s.v[2] = (double)clipped;
 #pragma unroll
   for (int q = 0; q < 4; ++q) s.v[q] = wave_sum(s.v[q]);

@@ -185,6 +185,35 @@ def test_policy_terms_without_weight_are_nothing(rows, reduction):
     assert abs(float(loss) - total) <= 16 * U * total                # (a series of ten terms)
 
 
+@pytest.mark.parametrize("rows", [1, 100])
+def test_policy_terms_whose_exponentials_pass_fp32(rows):
+    """e^100 at an advantage, or a kl_coef, of 2^-100 is an ordinary number.  100 rows take two launches."""
+    from decentrik_prime_amd import k_loss
+    far = [0.5, 89.0, 20.0, 88.0, 88.71875, 88.75, 95.0, 100.0, 120.0, -3.0, 0.0]
+    d = torch.tensor(far * rows, device="cuda")
+    zero, tiny = torch.zeros_like(d), 2.0 ** -100
+    meta = k_loss.row_meta([len(far)] * rows, "cuda")
+    # expf is off by up to 2 steps; one product, a rounding of the result
+    none, weight = torch.zeros(rows, device="cuda"), torch.full((rows,), -tiny, device="cuda")
+    loss, dlogp, stats = k_loss.policy_loss(zero, -d, weight, meta, reduction="sum", clip_low=1.0)
+    want = tiny * d.double().exp()
+    assert bool(((dlogp.double() - want).abs() <= 6 * U * want).all())
+    assert abs(float(loss) - float(want.sum())) <= 6 * U * float(want.sum())
+    assert bool(((stats[:, 0].double() - want.sum() / d.numel()).abs() <= 6 * U * want.sum() / d.numel()).all())
+    loss, dlogp, stats = k_loss.policy_loss(zero, zero, none, meta, ref=d, kl_coef=tiny, reduction="sum")
+    slope, k = tiny * torch.expm1(d.double()), tiny * (torch.expm1(d.double()) - d.double())
+    assert bool(((dlogp.double() + slope).abs() <= tiny * U * (6 * d.double().exp() + 4)).all())
+    assert abs(float(loss) - float(k.sum())) <= 6 * U * float(k.sum())
+    # means that are numbers of fp32, of ratios and estimates that are not
+    lens = [16] * rows
+    meta, d = k_loss.row_meta(lens, "cuda"), torch.zeros(16 * rows, device="cuda")
+    d[::16] = 89.0
+    _, _, stats = k_loss.policy_loss(torch.zeros_like(d), -d, none, meta, ref=d)
+    want = math.exp(89.0) / 16
+    assert bool((stats[:, 2:] - torch.tensor([0.0, want], device="cuda")).abs().max() <= 2 * U * want)
+    assert bool((stats[:, 1] - want).abs().max() <= 2 * U * want)
+
+
 def test_policy_of_a_token_that_is_not_a_number_stays_so():
     """A NaN log-probability (a target outside the vocabulary) is not hidden by an advantage of 0."""
     from decentrik_prime_amd import k_loss
