@@ -26,7 +26,8 @@ constexpr int kThreads = 256;
 constexpr int kVec = 8;                          // elements of a lane's piece of work
 constexpr int kRuns = 4;
 constexpr int kPiece = kThreads * kVec * kRuns;  // 8192 elements
-constexpr int kBatch = 112;                      // tensors of a launch (their table: under 4 KB)
+constexpr int kBatch = 128;                      // tensors of a launch: the most, in powers of two, whose
+                                                 // table and the other arguments stay under 4 KB
 constexpr int kGroups = 1024;                    // workgroups of a launch, four to a CU
 
 typedef __bf16 bf16;
@@ -42,7 +43,7 @@ struct Table {
   uint8_t type[kBatch];           // source type | destination type << 4
   int n;
 };
-static_assert(sizeof(Table) <= 3600, "kernel arguments");
+static_assert(sizeof(Table) + 64 + 256 <= 4096, "kernel arguments, the launch's own 256 bytes among them");
 
 struct Piece {
   int tensor;

@@ -57,6 +57,19 @@ def test_clipping_matches_the_definition(sizes, types, max_norm, scale):
         assert all(torch.equal(a, b) for a, b in zip(grads, before))
 
 
+@pytest.mark.parametrize("n", [111, 127, 128, 129, 255, 256, 257, 1000])
+def test_any_number_of_tensors(n):
+    """Lists that fill launches exactly, and by one tensor more or fewer; every third without elements."""
+    from decentrik_prime_amd import k_grad
+    grads = make([0 if i % 3 == 2 else 1 + 37 * i for i in range(n)], TYPES["mixed"], seed=n)
+    norm, want = definition(grads, 0.5, 1.0)
+    outs = [torch.empty(g.shape, device="cuda") for g in grads]
+    check(k_grad.clip_grads(grads, 0.5, out=outs), outs, norm, want)
+    full = make([5] * n, TYPES["fp32"], seed=n + 1)
+    norm, want = definition(full, 0.5, 1.0)
+    check(k_grad.clip_grads(full, 0.5), full, norm, want)
+
+
 @pytest.mark.parametrize("types", list(TYPES))
 def test_pieces_of_buffers_at_any_element(types):
     """Gradients that begin anywhere in a buffer; what lies between them is left as it was."""
