@@ -363,6 +363,10 @@ extern "C" int dk_grad_scale(void* const* tensors, const int64_t* numel, const i
   if (!dk_aligned(factor, 4)) return DK_ERR_ALIGN;
   const Lists l{(const void* const*)tensors, tensors, numel, types, types, n};
   if (const int rc = check_lists(l)) return rc;
+  for (int64_t i = 0; i < n; ++i)   // (workgroups read the factor while others write)
+    if ((uintptr_t)factor + 4 > (uintptr_t)tensors[i] &&
+        (uintptr_t)factor < (uintptr_t)tensors[i] + numel[i] * type_size(types[i]))
+      return DK_ERR_INVALID;
   Table t;
   for (int64_t i = 0; i < n;) {
     const int64_t pieces = fill(l, t, i);

@@ -19,6 +19,8 @@ _CODES = {torch.float32: _lib.DK_TYPE_F32, torch.float16: _lib.DK_TYPE_F16,
 # a step has hundreds of small gradients: each property is read in the way that takes the least host time
 _dtype, _device, _contiguous = attrgetter("dtype"), torch.Tensor.get_device, torch.Tensor.is_contiguous
 
+_OVERLAP = "no gradient may overlap another or be listed twice, and a list holds up to 2^20"
+
 
 def _dense(t):
     """Whether the tensor's elements fill a run of memory, in whatever order of its axes."""
@@ -77,10 +79,13 @@ def _run(grads, max_norm, scale, out, in_place=False):
     nbytes = lib.dk_grad_clip_workspace(len(grads))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     norm = torch.empty_strided((), (), dtype=torch.float32, device=dev)
-    _lib.launch(dev, lib.dk_grad_clip, "dk_grad_clip", src.buffer_info()[0],
-                None if dst is None else dst.buffer_info()[0], numel.buffer_info()[0],
-                types.buffer_info()[0], to.buffer_info()[0], len(grads), max_norm, scale, norm.data_ptr(),
-                ws.data_ptr(), nbytes)
+    try:
+        _lib.launch(dev, lib.dk_grad_clip, "dk_grad_clip", src.buffer_info()[0],
+                    None if dst is None else dst.buffer_info()[0], numel.buffer_info()[0],
+                    types.buffer_info()[0], to.buffer_info()[0], len(grads), max_norm, scale, norm.data_ptr(),
+                    ws.data_ptr(), nbytes)
+    except ValueError as e:        # (all else that the entry refuses was checked above)
+        raise ValueError(f"{_OVERLAP}{'' if out is None else ', outputs included'} ({e})") from None
     return norm
 
 
@@ -103,7 +108,8 @@ def clip_grads(grads, max_norm, *, scale=1.0, out=None):
 
 def scale_grads(grads, factor, *, scale=1.0):
     """Each gradient times scale * factor in place; factor: an fp32 scalar tensor on their device, which the
-    host does not wait for (the unit of k_loss.row_factors).  No tensor may overlap another."""
+    host does not wait for (the unit of k_loss.row_factors).  No tensor may overlap another, nor hold the
+    factor."""
     grads = list(grads)
     if not grads:
         raise ValueError("at least one gradient")
@@ -112,5 +118,8 @@ def scale_grads(grads, factor, *, scale=1.0):
         raise ValueError("factor must be an fp32 scalar on the gradients' device")
     at = array("q", [g.data_ptr() for g in grads])        # (the host arrays live until the call returns)
     numel = array("q", [g.nelement() for g in grads])
-    _lib.launch(torch.device("cuda", index), _lib.lib().dk_grad_scale, "dk_grad_scale", at.buffer_info()[0],
-                numel.buffer_info()[0], types.buffer_info()[0], len(grads), factor.data_ptr(), float(scale))
+    try:
+        _lib.launch(torch.device("cuda", index), _lib.lib().dk_grad_scale, "dk_grad_scale", at.buffer_info()[0],
+                    numel.buffer_info()[0], types.buffer_info()[0], len(grads), factor.data_ptr(), float(scale))
+    except ValueError as e:
+        raise ValueError(f"{_OVERLAP}; the factor is in none of them ({e})") from None

@@ -344,7 +344,7 @@ int dk_grad_clip(const void* const* src, void* const* dst, const int64_t* numel,
                  const int32_t* dst_types, int64_t n, double max_norm, double scale, float* norm,
                  void* workspace, int64_t workspace_bytes, hipStream_t stream);
 /* n gradient tensors (as for dk_grad_clip, none overlapping another) times scale * factor[0] in place, factor
- * fp32 on the device. */
+ * fp32 on the device, in none of them (DK_ERR_INVALID). */
 int dk_grad_scale(void* const* tensors, const int64_t* numel, const int32_t* types, int64_t n,
                   const float* factor, double scale, hipStream_t stream);
 

@@ -210,3 +210,15 @@ def test_refusals():
         with pytest.raises(ValueError):
             k_grad.clip_grads(grads, 1.0, **kwargs)
     assert bool((g == 1).all())
+
+
+def test_overlaps_are_named():
+    from decentrik_prime_amd import k_grad
+    g = torch.ones(8, 8, device="cuda")
+    for call in (lambda: k_grad.clip_grads([g, g], 1.0), lambda: k_grad.clip_grads([g, g[2:]], 1.0),
+                 lambda: k_grad.clip_grads([g.view(-1)[:32]], 1.0, out=[g.view(-1)[1:33]]),
+                 lambda: k_grad.scale_grads([g, g[2:]], torch.ones((), device="cuda")),
+                 lambda: k_grad.scale_grads([g], g[7, 7])):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    assert bool((g == 1).all()) and float(k_grad.grad_norm([g, g])) == pytest.approx(math.sqrt(128))

@@ -297,4 +297,6 @@ def test_row_factors_and_scaling_refuse_bad_arguments():
     for bad in (([], [], []), ([0], [4], [f32]), ([a], [-1], [f32]), ([a], [4], [0]), ([a, a], [4, 4], [f32, f32]),
                 ([a, a + 8], [4, 4], [f32, f32]), ([a], [4], [f32], None)):
         assert scale(*bad) == _lib.DK_ERR_INVALID, bad
+    for inside in (a, a + 12, a + 1024):                                    # a factor that is scaled itself
+        assert scale([a, a + 1024], [4, 4], [f32, f32], inside) == _lib.DK_ERR_INVALID
     assert scale([a + 2], [4], [f32]) == scale([a], [4], [f32], p + 2) == _lib.DK_ERR_ALIGN
