@@ -272,8 +272,9 @@ class QwenQLoRAStep(NF4LinearStack):
     def score(self, adapters=True, scale=1.0):
         """(logp, entropy) fp32 [n_lab] of the batch's targets in sorted order, without dropout: under the
         adapters (a policy's scores of its own samples) or, with adapters False, under the frozen weights
-        alone (the reference).  scale: a factor of the logits (1 / temperature).  The logits are summed in
-        fp32, where forward()'s stats round them to fp16.  What a pending backward() reads stays as it is."""
+        alone (the reference).  scale: a factor of the logits (1 / temperature); the training steps have none,
+        their old and ref are scores at scale 1.  The logits are summed in fp32, where forward()'s stats
+        round them to fp16.  What a pending backward() reads stays as it is."""
         self._pass = getattr(self, "_pass", 0) + 1
         self._forward = True
         dev, f16, f32 = self.device, torch.float16, torch.float32
@@ -323,7 +324,8 @@ class QwenQLoRAStep(NF4LinearStack):
     def policy_step(self, meta, old, advantages, *, ref=None, g_loss=1.0, **options):
         """A training step on the clipped policy loss: meta the plan of the batch's answers
         (k_loss.row_meta(trainer.answer_lens(batch), ...)), old (and ref) log-probabilities in sorted order
-        (score(), or the head's stats of an earlier forward()), options as k_loss.policy_loss.  Returns
+        (score() at scale 1, or the head's stats of an earlier forward()), options as k_loss.policy_loss.  The
+        current log-probabilities are the head's, from logits rounded to fp16 (2^-11 of a logit).  Returns
         (loss, its stats per answer, the head's stats); the gradients of g_loss * loss are in self.grads."""
         self._check_rows(meta)
         _, stats, dy = self.forward()
@@ -333,8 +335,8 @@ class QwenQLoRAStep(NF4LinearStack):
 
     def preference_step(self, meta, ref, *, g_loss=1.0, **options):
         """A training step on the preference loss over meta's pairs of answers (options as
-        k_loss.preference_loss; ref None: without a reference).  Returns (loss, rewards, margins, the head's
-        stats); the gradients of g_loss * loss are in self.grads."""
+        k_loss.preference_loss; ref, as for policy_step, None: without a reference).  Returns (loss, rewards,
+        margins, the head's stats); the gradients of g_loss * loss are in self.grads."""
         self._check_rows(meta)
         _, stats, dy = self.forward()
         loss, dlogp, rewards, margins = k_loss.preference_loss(stats, ref, meta, **options)

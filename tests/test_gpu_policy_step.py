@@ -156,6 +156,32 @@ def test_small_weights_match_float64():
         _check_grads(st, want)
 
 
+def test_a_step_on_log_probabilities_of_fp32():
+    """The step in its parts, with the current log-probabilities from token_logprobs as score's are: without
+    dropout the ratio is 1 but for the adapters' input (no rounding of the logits to fp16 in between)."""
+    from decentrik_prime_amd import k_head, k_loss, k_nf4, trainer
+    from oracle import model as ref
+    batch, st = _step()
+    for i in range(2):
+        for k in ("mq", "mv"):
+            st.lora[i][k] = torch.ones_like(st.lora[i][k])
+    st.keep_scale = 1.0
+    meta = k_loss.row_meta(trainer.answer_lens(batch), "cuda")
+    old, _ = st.score()
+    base, _ = st.score(adapters=False)
+    adv = torch.tensor([1.0, -0.5, 0.25, -2.0, 0.0], device="cuda")
+    _, _, dy = st.forward()
+    logp, _, _ = k_head.token_logprobs(st.yf, st.source, st.tgt_sorted[:st.n_lab], rows=st.perm[:st.n_lab])
+    _, dlogp, rows = k_loss.policy_loss(logp, old, adv, meta, ref=base, kl_coef=0.1)
+    st.backward(dy, dlogp=dlogp)
+    assert float((logp - old).abs().max()) <= 5e-3 and float((rows[:, 3] - 1).abs().max()) <= 5e-3
+    weights = torch.zeros(st.m)
+    weights[st.labelled.cpu()] = -dlogp.cpu()
+    _, want = ref.qwen_step(_reference_inputs(torch, st, k_nf4), st.lens, visible=_visible(batch),
+                            weights=weights)
+    _check_grads(st, want)
+
+
 def test_losses_that_are_nothing_or_not_finite():
     """No gradient at all gives zeros, as does a batch without targets; an infinite one is not hidden."""
     from decentrik_prime_amd import k_loss, trainer
