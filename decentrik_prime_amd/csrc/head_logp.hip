@@ -315,7 +315,7 @@ __device__ __forceinline__ void lp_walk(const LpParams& p, f16* As, int32_t* tgt
     }
   }
 
-  // ---- the four lanes, then the four waves that share a token
+  // ---- the four lanes, then the WAVES_N waves that share a token
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll

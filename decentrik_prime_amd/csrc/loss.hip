@@ -503,8 +503,8 @@ __global__ __launch_bounds__(kSumThreads) void pref_loss_kernel(PrefParams p, in
 }
 
 // factors[rows] = 0, but -dlogp[i] / unit at row at[i]; unit is the largest power of two up to the largest
-// |dlogp| (1 where that is 0 or not finite), so the division is exact.  One workgroup: 2 us for a batch of
-// 2048 tokens.
+// |dlogp| (1 where that is 0 or not finite), so the division is exact.  One workgroup, bound by its loads'
+// latency: 4.7 us for 1520 answer tokens of 2048.
 __global__ __launch_bounds__(kSumThreads) void row_factors_kernel(const float* __restrict__ dlogp,
                                                                   const int32_t* __restrict__ at, int64_t n,
                                                                   float* factors, int64_t rows, float* unit) {

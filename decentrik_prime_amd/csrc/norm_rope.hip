@@ -126,7 +126,8 @@ template <int KMAX, bool DY32>
 __global__ __launch_bounds__(kRowThreads) void rms_bwd_kernel(
     const void* __restrict__ dyp, const float* __restrict__ gscale, const float* __restrict__ row_scale,
     const float* __restrict__ x, const f16* __restrict__ delta, const float* __restrict__ w,
-    const float* __restrict__ rstd, const float* dres, float* out, const f16* __restrict__ lq, const f16* __restrict__ lv,
+    const float* __restrict__ rstd, const float* dres, float* out,
+    const f16* __restrict__ lq, const f16* __restrict__ lv,
     f16* __restrict__ out16, const uint8_t* __restrict__ mq, const uint8_t* __restrict__ mv,
     int64_t n_rows, int d, float keep_scale) {
   const int lane = threadIdx.x & 63;

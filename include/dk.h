@@ -238,10 +238,11 @@ int dk_head_finalize(const float* state, const int32_t* tgt_sorted, const int32_
  * counterpart in the reference): x_v = scale <y_i, E_v>, lse = log sum_v e^(x_v), logp = x_tgt - lse,
  * entropy = lse - sum_v p_v x_v, i over the n given rows of y (rows int32 [n], indices below total, or NULL:
  * rows 0 .. n - 1).  y fp16 with row stride ldy (a multiple of 8) and emb fp16 [vocab, d] contiguous, both
- * 16-byte aligned; d a multiple of 64 up to 2^20, n and vocab up to 2^30; the last row's end, (total - 1) ldy + d,
- * below 2^31 elements with rows, (min(n, 256) - 1) ldy + d without; 0 < scale <= 10^6.  tgt int32 [n]: below 0
- * gives logp 0, vocab or more NaN; a row index outside [0, total) NaN throughout.  logp, entropy, lse fp32 [n].  workspace:
- * dk_head_logprobs_workspace bytes, 16-byte aligned. */
+ * 16-byte aligned; d a multiple of 64 up to 2^20, n and vocab up to 2^30 (tokens in launches of 2^24); the last
+ * row's end, (total - 1) ldy + d, below 2^31 elements with rows, (min(n, 256) - 1) ldy + d without;
+ * 0 < scale <= 10^6.  tgt int32 [n]: below 0 gives logp 0, vocab or more NaN; a row index outside [0, total)
+ * NaN throughout.  logp, entropy, lse fp32 [n].  workspace: dk_head_logprobs_workspace bytes, 16-byte
+ * aligned. */
 int64_t dk_head_logprobs_workspace(int64_t n, int64_t vocab, int64_t d);
 int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* rows, int64_t n,
                      const void* emb, int64_t vocab, int64_t d, const int32_t* tgt, float scale,
@@ -253,9 +254,9 @@ int dk_head_logprobs(const void* y, int64_t ldy, int64_t total, const int32_t* r
  * counterpart in the reference).  The batch is `rows` rows of consecutive tokens cut into items {first token
  * (low, high word), tokens, row, the row's tokens, the row's items, the item's place among them, 0} (int32
  * [n_items, 8], 16-byte aligned, row by row and in token order; n_items up to 2^25; a row has 1 to 64 items and
- * at most 2^30 tokens, an empty row one item without tokens); row r's items are row_items[r] .. row_items[r + 1] - 1.  A
- * token array is fp32 with an element stride (0 to 2^31 - 1), negated where it holds losses (the head's stats:
- * column 0, stride 4).  With n_tokens = 0 the token arrays may be NULL.
+ * at most 2^30 tokens, an empty row one item without tokens); row r's items are row_items[r] ..
+ * row_items[r + 1] - 1.  A token array is fp32 with an element stride (0 to 2^31 - 1), negated where it holds
+ * losses (the head's stats: column 0, stride 4).  With n_tokens = 0 the token arrays may be NULL.
  *
  * dk_policy_loss: A the advantage of the token (per_token) or of its row, r = e^(logp - old),
  *   p = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), k = e^(ref - logp) - (ref - logp) - 1 (ref NULL: 0)
