@@ -182,6 +182,30 @@ def test_a_step_on_log_probabilities_of_fp32():
     _check_grads(st, want)
 
 
+def test_a_captured_policy_step_replays():
+    """The whole step in a graph, on advantages of two sizes in turn, with eager steps between the replays."""
+    from decentrik_prime_amd import k_loss, trainer
+    batch, st = _step()
+    meta = k_loss.row_meta(trainer.answer_lens(batch), "cuda")
+    old, _ = st.score()
+    base, _ = st.score(adapters=False)
+    both = [torch.tensor(a, device="cuda") for a in ([1.0, -0.5, 0.25, -2.0, 0.0], [-1e-6, 2e-6, 0.0, 0.0, 5e-6])]
+
+    def run(a):
+        loss, rows, _ = st.policy_step(meta, old, a, ref=base, kl_coef=1e-7)
+        return [loss, rows, *(g for layer in st.grads for g in layer)]
+    want = [[t.clone() for t in run(a)] for a in both]
+    graph, adv = torch.cuda.CUDAGraph(), both[0].clone()
+    with torch.cuda.graph(graph):
+        out = run(adv)
+    for turn in range(4):
+        adv.copy_(both[turn % 2])
+        run(both[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[turn % 2])), turn
+
+
 def test_losses_that_are_nothing_or_not_finite():
     """No gradient at all gives zeros, as does a batch without targets; an infinite one is not hidden."""
     from decentrik_prime_amd import k_loss, trainer
